@@ -27,6 +27,7 @@ using namespace turbol;
 
 void register_kernel_ops(py::module_& ops);  // ops_bindings.cpp
 void register_llm_ops(py::module_& ops);      // llm_bindings.cpp
+void register_cache_ops(py::module_& ops);    // cache_bindings.cpp
 void register_comm_ops(py::module_& ops);     // comm_bindings.cpp
 void register_dist(py::module_& m);           // dist_bindings.cpp
 
@@ -792,6 +793,7 @@ PYBIND11_MODULE(turbol_core, m) {
   py::module_ ops = m.def_submodule("ops", "raw sm_100a kernel launchers on torch tensors");
   register_kernel_ops(ops);
   register_llm_ops(ops);
+  register_cache_ops(ops);
   register_comm_ops(ops);
   py::module_ dist = m.def_submodule("dist", "C++ distributed runtime: NcclCommunicator, DistributedTrainer, "
                                                "PipelineTrainer (turbol/distributed.hpp)");

@@ -1,0 +1,359 @@
+// torch-tensor entry points of the general rotary positions and the 8-bit
+// paged KV cache.  Each checks its arguments completely, whatever device they
+// are on, then launches on the current stream of their device and returns
+// true; for CPU tensors it returns false and the caller computes on the host.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <pybind11/pybind11.h>
+#include <torch/extension.h>
+
+#include <climits>
+
+#include "kernels.h"
+#include "turbol/common.hpp"
+
+namespace py = pybind11;
+
+namespace {
+
+void chk(bool c, const char* op, const char* m) {
+  if (!c) throw std::invalid_argument(std::string(op) + ": " + m);
+}
+void cuda_ok(int e, const char* what) {
+  if (e != 0) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(static_cast<cudaError_t>(e)));
+}
+
+int type_of(const at::Tensor& t, const char* op) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return TB_BF16;
+    case at::kHalf: return TB_F16;
+    case at::kFloat: return TB_F32;
+    default: throw std::invalid_argument(std::string(op) + ": bf16, fp16 or fp32 values");
+  }
+}
+
+// [T, H, D] rows with a contiguous last dimension.
+void rows3(const at::Tensor& t, const char* op, const char* m) {
+  chk(t.dim() == 3 && (t.size(2) <= 1 || t.stride(2) == 1) && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX, op, m);
+}
+
+// Bytes [lo, hi) that a view touches (empty: lo == hi).
+struct Range {
+  uintptr_t lo, hi;
+};
+Range range_of(const at::Tensor& t) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {p, p};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {p, p + static_cast<uintptr_t>(last + 1) * t.element_size()};
+}
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  const Range x = range_of(a), y = range_of(b);
+  return x.hi <= y.lo || y.hi <= x.lo || x.lo == x.hi || y.lo == y.hi;
+}
+// Whether two [T, H, D] views share no element: disjoint ranges, or column
+// slices of rows with the same stride.
+bool columns_apart(const at::Tensor& a, const at::Tensor& b) {
+  if (apart(a, b)) return true;
+  if (a.element_size() != b.element_size() || a.stride(0) != b.stride(0)) return false;
+  const int64_t e = a.element_size(), row = a.stride(0) * e;
+  const int64_t wa = ((a.size(1) - 1) * a.stride(1) + a.size(2)) * e, wb = ((b.size(1) - 1) * b.stride(1) + b.size(2)) * e;
+  if (row <= 0) return false;
+  int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr()));
+  d %= row;
+  if (d < 0) d += row;
+  return d >= wa && d + wb <= row;
+}
+// Whether a [T, H, D] view to be written names each element once.
+bool rows_distinct(const at::Tensor& t) {
+  if (t.numel() == 0) return true;
+  int64_t n0 = t.size(0), s0 = t.stride(0), n1 = t.size(1), s1 = t.stride(1);
+  if (n0 == 1) return n1 == 1 || s1 >= t.size(2);
+  if (n1 == 1) return s0 >= t.size(2);
+  if (s0 < s1) {
+    std::swap(n0, n1);
+    std::swap(s0, s1);
+  }
+  return s1 >= t.size(2) && s0 >= (n1 - 1) * s1 + t.size(2);
+}
+bool same_view(const at::Tensor& a, const at::Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.strides() == b.strides() && a.sizes() == b.sizes();
+}
+
+void index1(const at::Tensor& t, int64_t n, const char* op, const char* m) {
+  chk(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), op, m);
+}
+
+int* error_of(const py::object& e, const at::Device& dev, const char* op, at::Tensor& hold) {
+  if (e.is_none()) return nullptr;
+  hold = e.cast<at::Tensor>();
+  chk(hold.scalar_type() == at::kInt && hold.numel() >= 1 && hold.is_contiguous() && hold.device() == dev, op,
+      "error is an int32 tensor on the same device");
+  return hold.data_ptr<int>();
+}
+
+// The table's dimensions: R / 2 pairs for max_pos positions.
+void table_of(const at::Tensor& t, int64_t D, const char* op) {
+  chk(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(2) == 2 && t.is_contiguous() && t.size(0) >= 1 &&
+          t.size(0) <= INT_MAX && t.size(1) >= 1 && 2 * t.size(1) <= D,
+      op, "table is a contiguous fp32 [max_pos, R / 2, 2] with 1 <= R / 2 <= D / 2");
+  chk(reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0, op, "table is 8-byte aligned");
+}
+
+bool rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, const at::Tensor& out, bool interleaved,
+            bool transpose, const py::object& error) {
+  const char* op = "rotary";
+  rows3(x, op, "x is [T, H, D] with a contiguous last dimension");
+  const int dt = type_of(x, op);
+  rows3(out, op, "out is [T, H, D] with a contiguous last dimension");
+  chk(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type(), op, "out has x's shape and type");
+  chk(x.size(2) % 2 == 0 && x.size(2) <= INT_MAX, op, "an even head dimension");
+  index1(pos, x.size(0), op, "pos is a contiguous int32 [T]");
+  table_of(table, x.size(2), op);
+  const at::Device dev = x.device();
+  chk(out.device() == dev && pos.device() == dev && table.device() == dev, op, "all tensors on one device");
+  chk(rows_distinct(out), op, "out has overlapping rows");
+  chk(same_view(x, out) || columns_apart(x, out), op, "out is x itself or does not overlap it");
+  at::Tensor hold;
+  int* err = error_of(error, dev, op, hold);
+  if (!x.is_cuda()) return false;
+  if (x.numel() == 0) return true;
+  c10::cuda::CUDAGuard guard(dev);
+  TbRotaryArgs a{};
+  a.x = x.data_ptr();
+  a.y = out.data_ptr();
+  a.pos = pos.data_ptr<int>();
+  a.table = table.data_ptr<float>();
+  a.T = static_cast<int>(x.size(0));
+  a.H = static_cast<int>(x.size(1));
+  a.D = static_cast<int>(x.size(2));
+  a.R = static_cast<int>(2 * table.size(1));
+  a.max_pos = static_cast<int>(table.size(0));
+  a.xs_t = x.stride(0);
+  a.xs_h = x.stride(1);
+  a.ys_t = out.stride(0);
+  a.ys_h = out.stride(1);
+  a.dtype = dt;
+  a.interleaved = interleaved;
+  a.transpose = transpose;
+  a.err = err;
+  cuda_ok(tb_rotary(&a, turbol::StreamFor(x)), op);
+  return true;
+}
+
+TbQuantCache cache_of(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                      const at::Tensor& block_table, const char* op) {
+  chk(kc.scalar_type() == at::kFloat8_e4m3fn && vc.scalar_type() == at::kFloat8_e4m3fn && kc.dim() == 4 &&
+          kc.sizes() == vc.sizes() && kc.is_contiguous() && vc.is_contiguous(),
+      op, "kc and vc are contiguous float8_e4m3fn [num_blocks, Hk, block_size, D]");
+  chk(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.dim() == 3 && ks.sizes() == vs.sizes() &&
+          ks.is_contiguous() && vs.is_contiguous() && ks.sizes() == kc.sizes().slice(0, 3),
+      op, "ks and vs are contiguous fp32 [num_blocks, Hk, block_size]");
+  const int64_t D = kc.size(3);
+  chk(D == 64 || D == 128 || D == 256, op, "head dimension 64, 128 or 256");
+  chk(kc.size(1) >= 1 && kc.size(2) >= 1, op, "at least one KV head and one slot per block");
+  chk(kc.size(0) * kc.size(1) * kc.size(2) <= INT_MAX, op, "at most 2^31 - 1 rows (blocks x heads x slots)");
+  chk(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.is_contiguous() &&
+          block_table.size(0) <= INT_MAX && block_table.size(1) <= INT_MAX / kc.size(2),
+      op, "block_table is a contiguous int32 [num_seqs, max_blocks]");
+  for (const at::Tensor* t : {&vc, &ks, &vs, &block_table})
+    chk(t->device() == kc.device(), op, "all tensors on one device");
+  for (const at::Tensor* t : {&kc, &vc, &ks, &vs})
+    chk(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, op, "the cache tensors are 16-byte aligned");
+  TbQuantCache c{};
+  c.kc = kc.data_ptr();
+  c.vc = vc.data_ptr();
+  c.ks = ks.data_ptr<float>();
+  c.vs = vs.data_ptr<float>();
+  c.block_table = block_table.data_ptr<int>();
+  c.num_seqs = static_cast<int>(block_table.size(0));
+  c.max_blocks = static_cast<int>(block_table.size(1));
+  c.num_blocks = static_cast<int>(kc.size(0));
+  c.Hk = static_cast<int>(kc.size(1));
+  c.bs = static_cast<int>(kc.size(2));
+  c.D = static_cast<int>(D);
+  return c;
+}
+
+bool kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& seq, const at::Tensor& pos,
+                    const at::Tensor& block_table, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                    const py::object& q_, const py::object& q_out_, const py::object& table_, bool interleaved,
+                    const py::object& error) {
+  const char* op = "kv_quant_write";
+  TbKvQuantWriteArgs a{};
+  a.cache = cache_of(kc, vc, ks, vs, block_table, op);
+  const at::Device dev = kc.device();
+  rows3(k, op, "k is [T, Hk, D] with a contiguous last dimension");
+  rows3(v, op, "v is [T, Hk, D] with a contiguous last dimension");
+  a.rot.dtype = type_of(k, op);
+  chk(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), op, "k and v have the same shape and type");
+  chk(k.size(1) == a.cache.Hk && k.size(2) == a.cache.D, op, "k has the cache's heads and head dimension");
+  const int64_t T = k.size(0);
+  index1(seq, T, op, "seq_of_token is a contiguous int32 [T]");
+  index1(pos, T, op, "pos is a contiguous int32 [T]");
+  for (const at::Tensor* t : {&k, &v, &seq, &pos}) chk(t->device() == dev, op, "all tensors on one device");
+  const at::Tensor* caches[4] = {&kc, &vc, &ks, &vs};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = i + 1; j < 4; ++j) chk(apart(*caches[i], *caches[j]), op, "the cache tensors overlap");
+    for (const at::Tensor* t : {&k, &v, &seq, &pos, &block_table})
+      chk(apart(*caches[i], *t), op, "an input overlaps the cache");
+  }
+  at::Tensor q, q_out, table, hold;
+  a.rot.err = error_of(error, dev, op, hold);
+  if (!table_.is_none()) {
+    table = table_.cast<at::Tensor>();
+    table_of(table, a.cache.D, op);
+    chk(table.size(1) % 4 == 0, op, "a multiple of 8 rotated dimensions");
+    chk(table.device() == dev, op, "all tensors on one device");
+    a.rot.table = table.data_ptr<float>();
+    a.rot.R = static_cast<int>(2 * table.size(1));
+    a.rot.max_pos = static_cast<int>(table.size(0));
+    a.rot.interleaved = interleaved;
+  }
+  chk(q_.is_none() == q_out_.is_none(), op, "q and q_out come together");
+  if (!q_.is_none()) {
+    q = q_.cast<at::Tensor>();
+    q_out = q_out_.cast<at::Tensor>();
+    chk(!table_.is_none(), op, "q needs a table");
+    rows3(q, op, "q is [T, Hq, D] with a contiguous last dimension");
+    rows3(q_out, op, "q_out is [T, Hq, D] with a contiguous last dimension");
+    chk(q.size(0) == T && q.size(2) == a.cache.D && q.scalar_type() == k.scalar_type(), op,
+        "q has k's rows, head dimension and type");
+    chk(q_out.sizes() == q.sizes() && q_out.scalar_type() == q.scalar_type(), op, "q_out has q's shape and type");
+    chk(q.device() == dev && q_out.device() == dev, op, "all tensors on one device");
+    chk(rows_distinct(q_out), op, "q_out has overlapping rows");
+    chk(same_view(q, q_out) || columns_apart(q, q_out), op, "q_out is q itself or does not overlap it");
+    chk(columns_apart(q_out, k) && columns_apart(q_out, v), op, "q_out overlaps k or v");
+    for (int i = 0; i < 4; ++i) chk(apart(*caches[i], q) && apart(*caches[i], q_out), op, "q overlaps the cache");
+    a.rot.x = q.data_ptr();
+    a.rot.y = q_out.data_ptr();
+    a.rot.H = static_cast<int>(q.size(1));
+    a.rot.xs_t = q.stride(0);
+    a.rot.xs_h = q.stride(1);
+    a.rot.ys_t = q_out.stride(0);
+    a.rot.ys_h = q_out.stride(1);
+  }
+  if (!kc.is_cuda()) return false;
+  if (T == 0) return true;
+  c10::cuda::CUDAGuard guard(dev);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.ks_t = k.stride(0);
+  a.ks_h = k.stride(1);
+  a.vs_t = v.stride(0);
+  a.vs_h = v.stride(1);
+  a.seq = seq.data_ptr<int>();
+  a.pos = pos.data_ptr<int>();
+  a.T = static_cast<int>(T);
+  cuda_ok(tb_kv_quant_write(&a, turbol::StreamFor(kc)), op);
+  return true;
+}
+
+bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                   const at::Tensor& seq, const at::Tensor& pos, const at::Tensor& block_table, const at::Tensor& k_out,
+                   const at::Tensor& v_out, const py::object& error) {
+  const char* op = "kv_quant_read";
+  TbKvQuantReadArgs a{};
+  a.cache = cache_of(kc, vc, ks, vs, block_table, op);
+  const at::Device dev = kc.device();
+  rows3(k_out, op, "out is [T, Hk, D] with a contiguous last dimension");
+  rows3(v_out, op, "out is [T, Hk, D] with a contiguous last dimension");
+  a.dtype = type_of(k_out, op);
+  chk(k_out.sizes() == v_out.sizes() && k_out.scalar_type() == v_out.scalar_type(), op,
+      "the two outputs have the same shape and type");
+  chk(k_out.size(1) == a.cache.Hk && k_out.size(2) == a.cache.D, op, "out has the cache's heads and head dimension");
+  const int64_t T = k_out.size(0);
+  index1(seq, T, op, "seq_of_token is a contiguous int32 [T]");
+  index1(pos, T, op, "pos is a contiguous int32 [T]");
+  for (const at::Tensor* t : {&k_out, &v_out, &seq, &pos}) chk(t->device() == dev, op, "all tensors on one device");
+  chk(rows_distinct(k_out) && rows_distinct(v_out), op, "out has overlapping rows");
+  chk(columns_apart(k_out, v_out), op, "the two outputs overlap");
+  for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &seq, &pos, &block_table})
+    chk(apart(k_out, *t) && apart(v_out, *t), op, "out overlaps an input");
+  at::Tensor hold;
+  a.err = error_of(error, dev, op, hold);
+  if (!kc.is_cuda()) return false;
+  if (T == 0) return true;
+  c10::cuda::CUDAGuard guard(dev);
+  a.k = k_out.data_ptr();
+  a.v = v_out.data_ptr();
+  a.ks_t = k_out.stride(0);
+  a.ks_h = k_out.stride(1);
+  a.vs_t = v_out.stride(0);
+  a.vs_h = v_out.stride(1);
+  a.seq = seq.data_ptr<int>();
+  a.pos = pos.data_ptr<int>();
+  a.T = static_cast<int>(T);
+  cuda_ok(tb_kv_quant_read(&a, turbol::StreamFor(kc)), op);
+  return true;
+}
+
+bool decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                            const at::Tensor& vs, const at::Tensor& block_table, const at::Tensor& ctx_len,
+                            const at::Tensor& out, double scale, const py::object& error) {
+  const char* op = "decode_attention_quant";
+  TbDecodeAttnQuantArgs a{};
+  a.cache = cache_of(kc, vc, ks, vs, block_table, op);
+  const at::Device dev = kc.device();
+  rows3(q, op, "q is [B, Hq, D] with a contiguous last dimension");
+  rows3(out, op, "out is [B, Hq, D] with a contiguous last dimension");
+  a.dtype = type_of(q, op);
+  chk(a.dtype != TB_F32, op, "bf16 or fp16 q");
+  chk(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), op, "out has q's shape and type");
+  chk(q.size(2) == a.cache.D, op, "q has the cache's head dimension");
+  chk(q.size(1) >= 1 && q.size(1) % a.cache.Hk == 0, op, "the query heads are a multiple of the KV heads");
+  const int64_t B = q.size(0);
+  chk(block_table.size(0) == B, op, "one block_table row per sequence");
+  chk(B * q.size(1) <= INT_MAX, op, "at most 2^31 - 1 query rows");
+  index1(ctx_len, B, op, "ctx_len is a contiguous int32 [B]");
+  for (const at::Tensor* t : {&q, &out, &ctx_len}) chk(t->device() == dev, op, "all tensors on one device");
+  chk(rows_distinct(out), op, "out has overlapping rows");
+  chk(columns_apart(out, q), op, "out overlaps q");
+  for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &ctx_len, &block_table})
+    chk(apart(out, *t), op, "out overlaps an input");
+  chk(std::isfinite(scale), op, "a finite scale");
+  at::Tensor hold, ws;
+  a.err = error_of(error, dev, op, hold);
+  if (!kc.is_cuda()) return false;
+  if (B == 0) return true;
+  c10::cuda::CUDAGuard guard(dev);
+  a.q = q.data_ptr();
+  a.out = out.data_ptr();
+  a.qs_b = q.stride(0);
+  a.qs_h = q.stride(1);
+  a.os_b = out.stride(0);
+  a.os_h = out.stride(1);
+  a.ctx_len = ctx_len.data_ptr<int>();
+  a.B = static_cast<int>(B);
+  a.Hq = static_cast<int>(q.size(1));
+  a.scale = static_cast<float>(scale);
+  // from the caching allocator on the current stream (inside a capture: from
+  // the graph's own pool), so calls on other streams and graphs never share it
+  a.ws_bytes = tb_decode_attention_quant_ws_bytes(a.B, a.Hq, a.cache.Hk, a.cache.D, a.cache.max_blocks * a.cache.bs);
+  if (a.ws_bytes > 0) {
+    ws = at::empty({static_cast<int64_t>((a.ws_bytes + 3) / 4)}, ks.options());
+    a.ws = ws.data_ptr<float>();
+  }
+  cuda_ok(tb_decode_attention_quant(&a, turbol::StreamFor(kc)), op);
+  return true;
+}
+
+}  // namespace
+
+void register_cache_ops(py::module_& m) {
+  m.def("rotary", &rotary, py::arg("x"), py::arg("pos"), py::arg("table"), py::arg("out"),
+        py::arg("interleaved") = false, py::arg("transpose") = false, py::arg("error") = py::none(),
+        "out = rotary positions of x [T, H, D] (general form); false for CPU tensors, after the checks");
+  m.def("kv_quant_write", &kv_quant_write, py::arg("k"), py::arg("v"), py::arg("seq_of_token"), py::arg("pos"),
+        py::arg("block_table"), py::arg("kc"), py::arg("vc"), py::arg("ks"), py::arg("vs"), py::arg("q") = py::none(),
+        py::arg("q_out") = py::none(), py::arg("table") = py::none(), py::arg("interleaved") = false,
+        py::arg("error") = py::none(),
+        "quantises K and V rows into the 8-bit paged cache (with a table: rotates q and k first)");
+  m.def("kv_quant_read", &kv_quant_read, py::arg("kc"), py::arg("vc"), py::arg("ks"), py::arg("vs"),
+        py::arg("seq_of_token"), py::arg("pos"), py::arg("block_table"), py::arg("k_out"), py::arg("v_out"),
+        py::arg("error") = py::none(), "reads rows of the 8-bit paged cache back");
+  m.def("decode_attention_quant", &decode_attention_quant, py::arg("q"), py::arg("kc"), py::arg("vc"), py::arg("ks"),
+        py::arg("vs"), py::arg("block_table"), py::arg("ctx_len"), py::arg("out"), py::arg("scale"),
+        py::arg("error") = py::none(), "attention of one token per sequence over the 8-bit paged cache");
+}

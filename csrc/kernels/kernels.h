@@ -348,6 +348,82 @@ int tb_flash_attn_bwd_tc(const void* q, const void* k, const void* v, long long 
                          void* dv, long long lddqkv, int B, int T, int Hq, int Hk, float scale, float* ws,
                          size_t ws_bytes, int* err, cudaStream_t s);
 
+// ---------------- rotary positions, general form (rotary.cu) ----------------
+enum { TB_BF16 = 0, TB_F16 = 1, TB_F32 = 2 };
+// y = the rotation of x [T, H, D] by the table rows of pos (transpose: its
+// backward).  R (even) of D (even) dimensions rotate, the others are copied
+// (x == y: left alone).  A negative position marks padding, copied as it is; a
+// position >= max_pos makes the row NaN and sets *err (optional) to 1.
+// Strides in elements; x == y needs equal strides, else the two do not overlap.
+typedef struct {
+  const void* x;
+  void* y;
+  const int* pos;      // [T]
+  const float* table;  // [max_pos, R / 2, 2] (cos, sin)
+  int T, H, D, R, max_pos;
+  long long xs_t, xs_h, ys_t, ys_h;
+  int dtype;  // TB_BF16 / TB_F16 / TB_F32, of x and y
+  int interleaved, transpose;
+  int* err;
+} TbRotaryArgs;
+int tb_rotary(const TbRotaryArgs* args, cudaStream_t s);
+
+// ---------------- 8-bit paged KV cache (kv_quant.cu, decode_attn_quant.cu) ----------------
+// Codes: e4m3 [num_blocks, Hk, bs, D], D in {64, 128, 256}; scales: fp32
+// [num_blocks, Hk, bs]; a value is code * scale.  A token's slot is
+// (block_table[seq, pos / bs], pos % bs).
+typedef struct {
+  void *kc, *vc;
+  float *ks, *vs;
+  const int* block_table;  // [num_seqs, max_blocks]
+  int num_seqs, max_blocks, num_blocks, Hk, bs, D;
+} TbQuantCache;
+// Writes the K and V rows of T tokens: scale = max(amax, 2^-90) / 448, code =
+// e4m3(x * (448 / max(amax, 2^-90))).  With q, the q and k rows are first
+// rotated (rot.x / rot.y: q in and out, rot.H = Hq; R a multiple of 8, or 0);
+// k is quantised from the unrounded rotation and itself left alone.  A
+// negative position or sequence marks padding (nothing written, its q row
+// copied); a sequence, position or block out of range writes nothing and sets
+// *err to 1 (a position >= max_pos also makes the q row NaN).  No two tokens
+// may name the same slot.
+typedef struct {
+  TbQuantCache cache;
+  const void *k, *v;
+  long long ks_t, ks_h, vs_t, vs_h;
+  const int *seq, *pos;  // [T]
+  int T;
+  TbRotaryArgs rot;  // T, D, dtype, strides and layout of q; dtype is also that of k and v
+} TbKvQuantWriteArgs;
+int tb_kv_quant_write(const TbKvQuantWriteArgs* args, cudaStream_t s);
+// Reads the rows of T tokens back, code * scale rounded to dtype.  Rows of
+// padding tokens are left as they were; out of range: likewise, and *err = 1.
+typedef struct {
+  TbQuantCache cache;
+  void *k, *v;
+  long long ks_t, ks_h, vs_t, vs_h;
+  const int *seq, *pos;
+  int T, dtype;
+  int* err;
+} TbKvQuantReadArgs;
+int tb_kv_quant_read(const TbKvQuantReadArgs* args, cudaStream_t s);
+// out[b] = attention of the one token q[b] over the first ctx_len[b] tokens of
+// sequence b (zeros where ctx_len[b] <= 0).  Tokens in blocks out of range, or
+// behind the table, are left out and set *err to 1.
+typedef struct {
+  TbQuantCache cache;
+  const void* q;  // [B, Hq, D] bf16 / fp16
+  void* out;      // [B, Hq, D], the same type
+  long long qs_b, qs_h, os_b, os_h;
+  const int* ctx_len;  // [B], B == cache.num_seqs
+  int B, Hq, dtype;
+  float scale;
+  float* ws;  // tb_decode_attention_quant_ws_bytes()
+  size_t ws_bytes;
+  int* err;
+} TbDecodeAttnQuantArgs;
+size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens);
+int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s);
+
 // ---------------- NVLink peer-memory collectives ----------------
 #define TB_MAX_PEERS 8
 typedef struct {

@@ -193,3 +193,93 @@ def ppo_token_loss(lp, old_lp, adv, v, old_v, ret, clip=0.2, vclip=0.2, vf_coef=
                          ((ratio.detach() - 1).abs() > clip).float().sum(),
                          torch.tensor(float(lp.numel()), device=lp.device)])
     return loss.detach(), lp_t.grad, v_t.grad, stats
+
+
+def rotary(x, pos, table, interleaved=False, transpose=False, out=None, error=None):
+    """Rotary positions of x [T, H, D], general form (the math of the ``rotary``
+    kernel, computed in table's type)."""
+    R = 2 * table.shape[1]
+    p = pos.long()
+    bad, pad = p >= table.shape[0], p < 0
+    cs = table[p.clamp(0, table.shape[0] - 1)][:, None]
+    c, s = cs[..., 0], -cs[..., 1] if transpose else cs[..., 1]
+    xf = x.to(table.dtype)
+    a, b = (xf[..., 0:R:2], xf[..., 1:R:2]) if interleaved else (xf[..., : R // 2], xf[..., R // 2: R])
+    ya, yb = a * c - b * s, b * c + a * s
+    y = torch.stack([ya, yb], -1).flatten(-2) if interleaved else torch.cat([ya, yb], -1)
+    y = torch.cat([y, xf[..., R:]], -1)
+    y = torch.where(pad[:, None, None], xf, y).masked_fill(bad[:, None, None], float("nan")).to(x.dtype)
+    if error is not None and bool(bad.any()):
+        error[0] = 1
+    if out is None:
+        return y
+    out.copy_(y)
+    return out
+
+
+KV_AMAX_MIN = 2.0 ** -90  # keeps 448 / amax finite for rows of zeros
+
+
+def kv_quantise(x):
+    """(e4m3 codes, fp32 scales) of the rows x [..., D]."""
+    xf = x.float()
+    amax = xf.abs().amax(-1).clamp_min(KV_AMAX_MIN)
+    top = torch.full_like(amax, 448.0)  # tensor / tensor: IEEE division (a scalar operand becomes a reciprocal product)
+    return (xf * (top / amax)[..., None]).to(torch.float8_e4m3fn), amax / top
+
+
+def _slots(seq_of_token, pos, block_table, num_blocks, bs, error):
+    """(tokens that name a slot, their blocks, their places in the block)."""
+    live = (seq_of_token >= 0) & (pos >= 0)
+    ok = live & (seq_of_token < block_table.shape[0]) & (pos // bs < block_table.shape[1])
+    t = torch.nonzero(ok).squeeze(1)
+    blk = block_table[seq_of_token[t].long(), (pos[t] // bs).long()].long()
+    fine = (blk >= 0) & (blk < num_blocks)
+    if error is not None and (int(live.sum()) != int(ok.sum()) or not bool(fine.all())):
+        error[0] = 1
+    t, blk = t[fine], blk[fine]
+    return t, blk, (pos[t] % bs).long()
+
+
+def kv_quant_write(k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q=None, table=None, interleaved=False,
+                   q_out=None, error=None):
+    p = pos
+    if table is not None:
+        if q is not None:
+            rotary(q, pos, table, interleaved, out=q_out, error=error)
+        k = rotary(k.float(), pos, table, interleaved, error=error)
+        p = torch.where(pos < table.shape[0], pos, -1)
+    t, blk, slot = _slots(seq_of_token, p, block_table, kc.shape[0], kc.shape[2], error)
+    for x, c, s in ((k, kc, ks), (v, vc, vs)):
+        codes, scale = kv_quantise(x[t])
+        c.view(torch.uint8)[blk, :, slot] = codes.view(torch.uint8)
+        s[blk, :, slot] = scale
+
+
+def kv_quant_read(kc, vc, ks, vs, seq_of_token, pos, block_table, out, error=None):
+    t, blk, slot = _slots(seq_of_token, pos, block_table, kc.shape[0], kc.shape[2], error)
+    for c, s, o in ((kc, ks, out[0]), (vc, vs, out[1])):
+        codes = c.view(torch.uint8)[blk, :, slot].view(torch.float8_e4m3fn)
+        o[t] = (codes.float() * s[blk, :, slot][..., None]).to(o.dtype)
+    return out
+
+
+def decode_attention_quant(q, kc, vc, ks, vs, block_table, ctx_len, scale, out=None, error=None, dtype=torch.float32):
+    """One-token attention over the 8-bit paged cache, sequence by sequence, in
+    ``dtype``; out (if given) receives it rounded."""
+    B, Hq, D = q.shape
+    num_blocks, Hk, bs, _ = kc.shape
+    y = torch.zeros(B, Hq, D, dtype=dtype, device=q.device)
+    for b, n in enumerate(ctx_len.tolist()):
+        idx = torch.arange(max(n, 0), device=q.device)
+        t, blk, slot = _slots(torch.full_like(idx, b), idx, block_table, num_blocks, bs, error)
+        if t.numel() == 0:
+            continue
+        k, v = ((c.view(torch.uint8)[blk, :, slot].view(torch.float8_e4m3fn).to(dtype) *
+                 s[blk, :, slot].to(dtype)[..., None]).transpose(0, 1) for c, s in ((kc, ks), (vc, vs)))
+        w = torch.softmax(q[b].to(dtype).view(Hk, Hq // Hk, D) @ k.transpose(1, 2) * scale, -1)
+        y[b] = (w @ v).reshape(Hq, D)
+    if out is None:
+        return y
+    out.copy_(y)
+    return out
