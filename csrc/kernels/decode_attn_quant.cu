@@ -2,102 +2,686 @@
 //
 //   a_j = scale * ks_j * (q . k_j),   out = sum_j softmax(a)_j * vs_j * v_j
 //
-// with k_j, v_j the e4m3 codes and ks_j, vs_j the scales of token j.  One pass
-// over the context with the running maximum and sum of the softmax in fp32.
+// with k_j, v_j the e4m3 codes and ks_j, vs_j the scales of token j, for the
+// G = Hq / Hk query heads that share a KV head.
+//
+// The pages are the traffic (2 (D + 4) bytes per token and KV head), read once:
+//
+//  * Work is cut into tiles of 16 tokens and dealt out evenly over a grid of
+//    resident CTAs, whatever the contexts' lengths: CTA c takes the tiles
+//    [c n / N, (c + 1) n / N) of the list (sequence, KV head, tile), read off
+//    ctx_len on the device, so one captured call serves contexts that grow.
+//    A (sequence, KV head) that ends up in several CTAs leaves partial results
+//    (maximum, sum, unnormalised output) that a second kernel joins in a fixed
+//    order: no atomics, the same bits every time.
+//  * Each of a CTA's warps owns every fourth tile of a (sequence, KV head) and
+//    a ring of tiles in shared memory that it fills with cp.async, running
+//    ahead over the borders of contexts; nothing but the end of a (sequence,
+//    KV head) waits for another warp.
+//  * Products run on mma.sync m16n8k16 in fp16 (every e4m3 value is an fp16
+//    value) with the tokens, then the head's dimensions, as the 16 rows and the
+//    query heads as the 8 columns: with 5 to 8 query heads per KV head hardly a
+//    column is idle, and a tcgen05 tile (128 rows by 8 columns) would want the
+//    codes widened through shared memory first.  S^T = K q, whose accumulator,
+//    transposed in registers (movmatrix), is the operand of O^T = V^T w.
+//  * The running maximum m is of a_j + e_j, e_j the exponent of vs_j: then the
+//    weights w_j = exp2(a_j - m) vs_j lie in [0, 2) and fit fp16 however much
+//    the scales of tokens differ (round to 2^-11 relative, 2^-25 absolute at
+//    the small end), while the sum l of exp2(a_j - m) stays in fp32 range.
+//    q is brought into fp16 range by a power of two per head (exact).
 #include <math.h>
 
 #include "device_common.cuh"
 #include "kernels.h"
+#include "pdl.cuh"
 #include "vec_io.cuh"
 
 namespace {
 
-__device__ __forceinline__ float code_value(uint8_t c) {
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 16;       // tokens per tile
+constexpr int kMinTiles = 8;    // a CTA takes at least this many tiles, where contexts are that long
+constexpr int kWholeTokens = 256;  // contexts that cannot be longer are not split
+constexpr int kMinVsExp = -100;
+
+__device__ __forceinline__ uint32_t f16x2_of(uint32_t two_codes) {
   uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(c)));
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(r & 0xffff)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two_codes)));
+  return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Shared memory.  A ring stage holds 16 K rows and 16 V rows of codes (rows
+// padded by 16 bytes against bank conflicts), their scales and a mask of the
+// tokens that count.
+template <int D, int NT>
+struct Smem {
+  static constexpr int kStages = D == 256 ? 3 : D == 128 ? 3 : 4;
+  static constexpr int kRow = D + 16;
+  static constexpr int kStage = 2 * kTile * kRow + 2 * kTile * 4 + 16;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kQ = (D / 16) * NT * 32 * 8;
+  static constexpr int kOut = kWarps * kHeads * D * 4;
+  static constexpr int kScan = (2 * kWarps + 2) * 8;
+  static constexpr int kMisc = kWarps * kHeads * 8 + kHeads * 4 + kScan;
+  static constexpr int kBytes = kRing + kQ + kOut + kMisc;
+};
+
+// Partial results: per slot (two per CTA) heads x (D outputs, maximum, sum);
+// then one record per CTA: the (sequence, group) whose first part it holds, the
+// slot and the number of parts (0: none).
+template <int D, int NT>
+struct Partials {
+  static constexpr int kHeads = 8 * NT;
+  static constexpr size_t kSlot = static_cast<size_t>(kHeads) * (D + 2);
+  __device__ static float* out(float* ws, long long slot, int h) { return ws + slot * kSlot + h * D; }
+  __device__ static float* stat(float* ws, long long slot, int h) {
+    return ws + slot * kSlot + kHeads * D + h * 2;
+  }
+  __device__ static int* record(float* ws, int grid, int c) {
+    return reinterpret_cast<int*>(ws + 2ll * grid * kSlot) + 4ll * c;
+  }
+  static size_t bytes(int grid) { return (2 * grid * kSlot + 4 * static_cast<size_t>(grid)) * 4; }
+};
+
+struct Geometry {
+  int G, NG, HG;   // query heads per KV head, groups of 8 NT of them, groups per sequence
+  long long cap;   // tokens that a table row can name
+  int whole;       // one CTA per (sequence, group), nothing to join
+};
+
+__device__ __forceinline__ long long tokens_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
+  const long long n = a.ctx_len[b];
+  return n < 0 ? 0 : n < g.cap ? n : g.cap;
+}
+__device__ __forceinline__ long long tiles_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
+  return (tokens_of(a, g, b) + kTile - 1) / kTile;
 }
 
-// One CTA per (sequence, query head): each of its four warps takes every
-// fourth token, a lane D / 32 dimensions; the warps' partials are joined in
-// shared memory.
-template <typename T, int D>
-__global__ void decode_attn_quant_kernel(TbDecodeAttnQuantArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float sm[4], sl[4], so[4][D];
-  const int b = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, kh = h / (a.Hq / a.cache.Hk);
-  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const TbQuantCache& c = a.cache;
-  const T* q = static_cast<const T*>(a.q) + b * a.qs_b + h * a.qs_h;
-  float qf[E], acc[E] = {};
-#pragma unroll
-  for (int i = 0; i < E; ++i) qf[i] = tb::to_f32(q[lane + 32 * i]) * a.scale;
-  float m = -INFINITY, l = 0.f;
-  const long long cap = static_cast<long long>(c.max_blocks) * c.bs, want = a.ctx_len[b];
-  if (want > cap && a.err && threadIdx.x == 0) atomicCAS(a.err, 0, 1);
-  const long long ctx = want < cap ? want : cap;
-  for (long long j = w; j < ctx; j += 4) {
-    const int pb = static_cast<int>(j / c.bs);
-    const int blk = c.block_table[static_cast<long long>(b) * c.max_blocks + pb];
-    if (blk < 0 || blk >= c.num_blocks) {
-      if (a.err && lane == 0) atomicCAS(a.err, 0, 1);
-      continue;
-    }
-    const long long row = (static_cast<long long>(blk) * c.Hk + kh) * c.bs + (j - static_cast<long long>(pb) * c.bs);
-    const uint8_t* kr = static_cast<const uint8_t*>(c.kc) + row * D;
-    const uint8_t* vr = static_cast<const uint8_t*>(c.vc) + row * D;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) s += qf[i] * code_value(kr[lane + 32 * i]);
-    s = tb::warp_sum(s) * c.ks[row];
-    const float mn = fmaxf(m, s), mr = mn == -INFINITY ? 0.f : mn;
-    const float cor = __expf(m - mr), p = __expf(s - mr);
-    l = l * cor + p;
-    const float pv = p * c.vs[row];
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = acc[i] * cor + pv * code_value(vr[lane + 32 * i]);
-    m = mn;
+// Where a CTA (or a warp's prefetch) stands in the list of tiles: in sequence b,
+// group r, at tile t of the portion [.., end), with `rest` tiles behind it.
+struct Cursor {
+  int b, r;
+  long long t, end, rest, tokens;
+};
+
+// Moves on to the next portion; false at the end of the CTA's list.
+__device__ __forceinline__ bool next_portion(const TbDecodeAttnQuantArgs& a, const Geometry& g, Cursor& c) {
+  if (c.rest <= 0) return false;
+  long long n = (c.tokens + kTile - 1) / kTile;
+  if (++c.r == g.HG) {
+    c.r = 0;
+    do {
+      if (++c.b >= a.B) return false;
+      c.tokens = tokens_of(a, g, c.b);
+      n = (c.tokens + kTile - 1) / kTile;
+    } while (n == 0);
   }
-  if (lane == 0) {
-    sm[w] = m;
-    sl[w] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < E; ++i) so[w][lane + 32 * i] = acc[i];
-  __syncthreads();
-  float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  if (M == -INFINITY) M = 0.f;
-  float L = 0.f;
-  for (int i = 0; i < 4; ++i) L += sl[i] * __expf(sm[i] - M);
-  T* o = static_cast<T*>(a.out) + b * a.os_b + h * a.os_h;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float v = 0.f;
-    for (int i = 0; i < 4; ++i) v += so[i][d] * __expf(sm[i] - M);
-    o[d] = tb::from_f32<T>(L == 0.f ? 0.f : v / L);
-  }
+  c.t = 0;
+  c.end = n < c.rest ? n : c.rest;
+  c.rest -= c.end;
+  return true;
 }
 
 template <typename T>
-int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
-  const int grid = a.B * a.Hq;
-  switch (a.cache.D) {
-    case 64: decode_attn_quant_kernel<T, 64><<<grid, 128, 0, s>>>(a); break;
-    case 128: decode_attn_quant_kernel<T, 128><<<grid, 128, 0, s>>>(a); break;
-    case 256: decode_attn_quant_kernel<T, 256><<<grid, 128, 0, s>>>(a); break;
-    default: return static_cast<int>(cudaErrorInvalidValue);
+__device__ __forceinline__ void store_out4(T* p, bool aligned, float x, float y, float z, float w) {
+  if (aligned) {
+    const float f[4] = {x, y, z, w};
+    tb::store_vec<T, 4>(p, f);
+  } else {
+    p[0] = tb::from_f32<T>(x);
+    p[1] = tb::from_f32<T>(y);
+    p[2] = tb::from_f32<T>(z);
+    p[3] = tb::from_f32<T>(w);
   }
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool out4) {
+  using S = Smem<D, NT>;
+  using P = Partials<D, NT>;
+  constexpr int kStages = S::kStages, kHeads = S::kHeads, kRow = S::kRow;
+  constexpr int NCH = D / 64;  // 16-byte chunks of a K row per lane
+  constexpr int NW = D / 32;   // 4-byte words of a V row per lane
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* ring = smem;
+  uint2* qf = reinterpret_cast<uint2*>(smem + S::kRing);                 // [D / 16][NT][32] B fragments
+  float* so = reinterpret_cast<float*>(smem + S::kRing + S::kQ);         // [warps][heads][D]
+  float* sm = so + kWarps * kHeads * D;                                  // [warps][heads]
+  float* sl = sm + kWarps * kHeads;                                      // [warps][heads]
+  float* sc = sl + kWarps * kHeads;                                      // [heads] score factors
+  long long* sx = reinterpret_cast<long long*>(sc + kHeads);             // scan scratch
+  const TbQuantCache& c = a.cache;
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32, gq = lane / 4, tq = lane % 4;
+  const int Hq = a.Hq;
+
+  // ---- this CTA's list of tiles
+  Cursor cur;
+  long long first = 0, total = 0;
+  int N = gridDim.x;
+  if (g.whole) {
+    cur.b = blockIdx.x / g.HG;
+    cur.r = blockIdx.x % g.HG;
+    cur.tokens = tokens_of(a, g, cur.b);
+    cur.t = 0;
+    cur.end = (cur.tokens + kTile - 1) / kTile;
+    cur.rest = 0;
+    if (a.err && threadIdx.x == 0 && a.ctx_len[cur.b] > g.cap) atomicCAS(a.err, 0, 1);
+    if (cur.end == 0) {
+      T* o = static_cast<T*>(a.out) + static_cast<long long>(cur.b) * a.os_b;
+      const int kh = cur.r / g.NG, h0 = (cur.r % g.NG) * kHeads;
+      const int nh = g.G - h0 < kHeads ? g.G - h0 : kHeads;
+      for (int i = threadIdx.x; i < nh * D; i += kThreads)
+        o[static_cast<long long>(kh * g.G + h0 + i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
+      return;
+    }
+  } else {
+    // empty contexts, and contexts longer than their tables
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const int n = a.ctx_len[b];
+      if (a.err && threadIdx.x == 0 && n > g.cap) atomicCAS(a.err, 0, 1);
+      if (n <= 0 || g.cap == 0) {
+        T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
+        for (int i = threadIdx.x; i < Hq * D; i += kThreads)
+          o[static_cast<long long>(i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
+      }
+    }
+    // prefix sums of the sequences' tiles: each thread a run of sequences
+    const int per = (a.B + kThreads - 1) / kThreads, b0 = threadIdx.x * per;
+    const int b1 = b0 + per < a.B ? b0 + per : a.B;
+    long long mine = 0;
+    int some = 0;
+    for (int b = b0; b < b1; ++b) {
+      const long long n = tiles_of(a, g, b);
+      mine += n;
+      some += n > 0;
+    }
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const long long live = tb::warp_sum(some);
+    if (lane == 31) {
+      sx[w] = inc;
+      sx[kWarps + w] = live;
+    }
+    __syncthreads();
+    long long before = inc - mine, segs = 0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < w) before += sx[i];
+      total += sx[i];
+      segs += sx[kWarps + i];
+    }
+    total *= g.HG;
+    segs *= g.HG;
+    long long want = (total + kMinTiles - 1) / kMinTiles;
+    if (want < segs) want = segs;
+    if (want < N) N = static_cast<int>(want);
+    if (threadIdx.x == 0) P::record(a.ws, gridDim.x, blockIdx.x)[2] = 0;
+    if (static_cast<int>(blockIdx.x) >= N) return;
+    first = blockIdx.x * total / N;
+    const long long last = (blockIdx.x + 1) * total / N;
+    if (first >= before * g.HG && first < (before + mine) * g.HG) {
+      int b = b0;
+      long long at = before, n = tiles_of(a, g, b);
+      while (first >= (at + n) * g.HG) {
+        at += n;
+        n = tiles_of(a, g, ++b);
+      }
+      sx[2 * kWarps] = b;
+      sx[2 * kWarps + 1] = first - at * g.HG;
+    }
+    __syncthreads();
+    cur.b = static_cast<int>(sx[2 * kWarps]);
+    const long long off = sx[2 * kWarps + 1], n = tiles_of(a, g, cur.b);
+    cur.tokens = tokens_of(a, g, cur.b);
+    cur.r = static_cast<int>(off / n);
+    cur.t = off - cur.r * n;
+    cur.rest = last - first;
+    cur.end = n - cur.t < cur.rest ? n : cur.t + cur.rest;
+    cur.rest -= cur.end - cur.t;
+  }
+
+  // ---- this warp's prefetch: a cursor that runs ahead, and the cache rows of its next tile (lanes 0-15)
+  Cursor pre = cur;
+  pre.t += w;
+  bool more = true;
+  int row = -1;
+  auto look = [&]() {  // settles the cursor on a tile and looks its tokens' rows up
+    while (more && pre.t >= pre.end) {
+      more = next_portion(a, g, pre);
+      if (more) pre.t += w;
+    }
+    row = -1;
+    const long long tok = pre.t * kTile + lane;
+    if (more && lane < kTile && tok < pre.tokens) {
+      const int pb = static_cast<int>(tok) / c.bs;
+      const int blk = c.block_table[static_cast<long long>(pre.b) * c.max_blocks + pb];
+      if (blk >= 0 && blk < c.num_blocks) {
+        row = (blk * c.Hk + pre.r / g.NG) * c.bs + (static_cast<int>(tok) - pb * c.bs);
+      } else if (a.err) {
+        atomicCAS(a.err, 0, 1);
+      }
+    }
+  };
+  uint8_t* my_ring = ring + w * kStages * S::kStage;
+  const uint32_t my_ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
+  int put = 0;
+  auto issue = [&]() {  // copies the tile that the cursor stands on, then moves the cursor on
+    if (more) {
+      constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // chunks per row, rows per instruction
+      const uint32_t st = my_ring_s + put * S::kStage;
+#pragma unroll
+      for (int i = 0; i < kTile / kRows; ++i) {
+        const int tr = i * kRows + lane / kChunks, ch = lane % kChunks;
+        const int rr = __shfl_sync(0xffffffffu, row, tr);
+        const long long at = static_cast<long long>(rr < 0 ? 0 : rr) * D + ch * 16;
+        const int bytes = rr < 0 ? 0 : 16;
+        const uint32_t dst = st + tr * kRow + ch * 16;
+        cp_async16(dst, static_cast<const uint8_t*>(c.kc) + at, bytes);
+        cp_async16(dst + kTile * kRow, static_cast<const uint8_t*>(c.vc) + at, bytes);
+      }
+      const unsigned mask = __ballot_sync(0xffffffffu, row >= 0);
+      if (lane < kTile) {
+        const int rr = row < 0 ? 0 : row;
+        cp_async4(st + 2 * kTile * kRow + lane * 4, c.ks + rr, row < 0 ? 0 : 4);
+        cp_async4(st + 2 * kTile * kRow + kTile * 4 + lane * 4, c.vs + rr, row < 0 ? 0 : 4);
+      }
+      if (lane == 0)
+        *reinterpret_cast<unsigned*>(my_ring + put * S::kStage + 2 * kTile * kRow + 2 * kTile * 4) = mask;
+      put = put + 1 == kStages ? 0 : put + 1;
+      pre.t += kWarps;
+      look();
+    }
+    cp_commit();
+  };
+  look();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue();
+
+  // ---- portions of this CTA, one (sequence, group) each
+  int get = 0;
+  bool first_portion = true;
+  while (true) {
+    const int kh = cur.r / g.NG, h0 = (cur.r % g.NG) * kHeads;  // KV head, first of this group's query heads
+    const int nh = g.G - h0 < kHeads ? g.G - h0 : kHeads;
+    const long long ntiles = (cur.tokens + kTile - 1) / kTile;
+    // q as B fragments: lane (n = head, t) holds, for each k step, dimensions d0 .. d0 + 3 with
+    // d0 = (t * NCH + i) * 16 + 4 j, the same that it reads of a K row
+    for (int h = w; h < kHeads; h += kWarps) {
+      float v[D / 32][4 / (D < 128 ? 2 : 1)];
+      constexpr int E = D < 128 ? 2 : 4;  // dimensions per lane and round
+      uint32_t top = 0;
+      const T* q = static_cast<const T*>(a.q) + static_cast<long long>(cur.b) * a.qs_b +
+                   static_cast<long long>(kh * g.G + h0 + h) * a.qs_h;
+#pragma unroll
+      for (int i = 0; i < D / (32 * E); ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          v[i][e] = h < nh ? tb::to_f32(q[(i * 32 + lane) * E + e]) : 0.f;
+          top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+        }
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int e2 = max(static_cast<int>(top >> 23) - 127, -100);
+      const float f = pow2i(13 - e2);
+#pragma unroll
+      for (int i = 0; i < D / (32 * E); ++i) {
+        const int d = (i * 32 + lane) * E, ch = d / 16, j = d % 16 / 4;
+        uint32_t* to = reinterpret_cast<uint32_t*>(qf + (((ch % NCH) * 4 + j) * NT + h / 8) * 32 + (h % 8) * 4 + ch / NCH);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) to[(d % 4 + e) / 2] = pack_f16(v[i][e] * f, v[i][e + 1] * f);
+      }
+      // 2^(e2 - 13), times the scale in units of log 2
+      if (lane == 0) sc[h] = a.scale * 1.4426950408889634f * pow2i(e2 - 13);
+    }
+    __syncthreads();
+    float ch[NT][2], m[NT][2], l[NT][2], acc[2 * NW][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ch[n][e] = sc[n * 8 + 2 * tq + e];
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+      }
+#pragma unroll
+    for (int i = 0; i < 2 * NW; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
+
+    for (long long t = cur.t + w; t < cur.end; t += kWarps) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      const uint8_t* st = my_ring + get * S::kStage;
+      const float* scales = reinterpret_cast<const float*>(st + 2 * kTile * kRow);
+      const unsigned mask = *reinterpret_cast<const unsigned*>(st + 2 * kTile * kRow + 2 * kTile * 4);
+      // S^T [16 tokens, heads] = K q
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(st + gq * kRow + (tq * NCH + i) * 16);
+        const uint4 y = *reinterpret_cast<const uint4*>(st + (gq + 8) * kRow + (tq * NCH + i) * 16);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a0 = f16x2_of(xs[j]), a1 = f16x2_of(ys[j]), a2 = f16x2_of(xs[j] >> 16), a3 = f16x2_of(ys[j] >> 16);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 b = qf[((i * 4 + j) * NT + n) * 32 + lane];
+            mma16816(s[n], a0, a1, a2, a3, b.x, b.y);
+          }
+        }
+      }
+      // weights of tokens gq and gq + 8 for heads 2 tq and 2 tq + 1
+      const float k0 = scales[gq], k1 = scales[gq + 8], v0 = scales[kTile + gq], v1 = scales[kTile + gq + 8];
+      const bool in0 = mask >> gq & 1, in1 = mask >> (gq + 8) & 1;
+      const int x0 = static_cast<int>(__float_as_uint(v0) >> 23 & 255) - 127;
+      const int x1 = static_cast<int>(__float_as_uint(v1) >> 23 & 255) - 127;
+      const float e0 = static_cast<float>(max(x0, kMinVsExp)), e1 = static_cast<float>(max(x1, kMinVsExp));
+      uint32_t wb[NT][2];
+      bool grew = false;
+      float cor[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float lo = s[n][e] * ch[n][e] * k0, hi = s[n][2 + e] * ch[n][e] * k1;
+          float top = fmaxf(in0 ? lo + e0 : -INFINITY, in1 ? hi + e1 : -INFINITY);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float mn = fmaxf(m[n][e], top), mr = mn == -INFINITY ? 0.f : mn;
+          cor[n][e] = exp2_fast(m[n][e] - mr);
+          grew |= mn != m[n][e];
+          m[n][e] = mn;
+          p[e] = in0 ? exp2_fast(lo - mr) : 0.f;
+          p[2 + e] = in1 ? exp2_fast(hi - mr) : 0.f;
+        }
+        wb[n][0] = transpose8x8(pack_f16(in0 ? p[0] * v0 : 0.f, in0 ? p[1] * v0 : 0.f));
+        wb[n][1] = transpose8x8(pack_f16(in1 ? p[2] * v1 : 0.f, in1 ? p[3] * v1 : 0.f));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[n][e] = l[n][e] * cor[n][e] + (p[e] + p[2 + e]);
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int i = 0; i < 2 * NW; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][n][e] *= cor[n][e & 1];
+      }
+      // O^T [16 dimensions, heads] += V^T w: bytes of neighbouring tokens are paired before they are widened
+      const uint8_t* vr = st + kTile * kRow + 2 * tq * kRow;
+#pragma unroll
+      for (int kk = 0; kk < NW; kk += (NW < 4 ? NW : 4)) {
+        constexpr int U = NW < 4 ? NW : 4;  // words per load
+        using V = typename tb::RawOf<U * 4>::type;
+        const int at = NW < 4 ? gq * 8 : (kk / 4) * 128 + gq * 16;
+        V r[4];
+        r[0] = *reinterpret_cast<const V*>(vr + at);
+        r[1] = *reinterpret_cast<const V*>(vr + kRow + at);
+        r[2] = *reinterpret_cast<const V*>(vr + 8 * kRow + at);
+        r[3] = *reinterpret_cast<const V*>(vr + 9 * kRow + at);
+        const uint32_t* rw[4] = {reinterpret_cast<const uint32_t*>(&r[0]), reinterpret_cast<const uint32_t*>(&r[1]),
+                                 reinterpret_cast<const uint32_t*>(&r[2]), reinterpret_cast<const uint32_t*>(&r[3])};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t lo0 = __byte_perm(rw[0][u], rw[1][u], 0x5140), hi0 = __byte_perm(rw[0][u], rw[1][u], 0x7362);
+          const uint32_t lo1 = __byte_perm(rw[2][u], rw[3][u], 0x5140), hi1 = __byte_perm(rw[2][u], rw[3][u], 0x7362);
+          const uint32_t a0 = f16x2_of(lo0), a1 = f16x2_of(lo0 >> 16), a2 = f16x2_of(lo1), a3 = f16x2_of(lo1 >> 16);
+          const uint32_t c0 = f16x2_of(hi0), c1 = f16x2_of(hi0 >> 16), c2 = f16x2_of(hi1), c3 = f16x2_of(hi1 >> 16);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816(acc[2 * (kk + u)][n], a0, a1, a2, a3, wb[n][0], wb[n][1]);
+            mma16816(acc[2 * (kk + u) + 1][n], c0, c1, c2, c3, wb[n][0], wb[n][1]);
+          }
+        }
+      }
+      get = get + 1 == kStages ? 0 : get + 1;
+      __syncwarp();
+      issue();
+    }
+
+    // ---- join the warps
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = l[n][e];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        if (gq == 0) {
+          sm[w * kHeads + n * 8 + 2 * tq + e] = m[n][e];
+          sl[w * kHeads + n * 8 + 2 * tq + e] = v;
+        }
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+          const int d = NW < 4 ? gq * 8 + 4 * k : (k / 4) * 128 + gq * 16 + 4 * (k % 4);
+          *reinterpret_cast<float4*>(so + (w * kHeads + n * 8 + 2 * tq + e) * D + d) =
+              make_float4(acc[2 * k][n][e], acc[2 * k][n][2 + e], acc[2 * k + 1][n][e], acc[2 * k + 1][n][2 + e]);
+        }
+      }
+    __syncthreads();
+    const bool all = cur.t == 0 && cur.end == ntiles;  // the whole context was here
+    const long long slot = 2ll * blockIdx.x + (first_portion ? 0 : 1);
+    if (!all && cur.t == 0 && threadIdx.x == 0) {
+      // the first part: the others are in the CTAs up to the one that owns the last tile
+      int* rec = P::record(a.ws, gridDim.x, blockIdx.x);
+      const long long list_end = (blockIdx.x + 1) * total / N;             // list position behind this portion
+      const long long last_tile = list_end + (ntiles - cur.end) - 1;       // list position of the context's last tile
+      const long long owner = ((last_tile + 1) * N - 1) / total;
+      rec[0] = cur.b * g.HG + cur.r;
+      rec[1] = static_cast<int>(slot);
+      rec[2] = static_cast<int>(owner - blockIdx.x) + 1;
+    }
+    for (int i = threadIdx.x; i < nh * (D / 4); i += kThreads) {
+      const int h = i / (D / 4), d = i % (D / 4) * 4;
+      float M = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) M = fmaxf(M, sm[x * kHeads + h]);
+      const float mr = M == -INFINITY ? 0.f : M;
+      float L = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float f = exp2_fast(sm[x * kHeads + h] - mr);
+        const float4 v = *reinterpret_cast<const float4*>(so + (x * kHeads + h) * D + d);
+        L += f * sl[x * kHeads + h];
+        o0 += f * v.x;
+        o1 += f * v.y;
+        o2 += f * v.z;
+        o3 += f * v.w;
+      }
+      if (all) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        store_out4<T>(static_cast<T*>(a.out) + static_cast<long long>(cur.b) * a.os_b +
+                          static_cast<long long>(kh * g.G + h0 + h) * a.os_h + d,
+                      out4, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
+      } else {
+        *reinterpret_cast<float4*>(P::out(a.ws, slot, h) + d) = make_float4(o0, o1, o2, o3);
+        if (d == 0) {
+          P::stat(a.ws, slot, h)[0] = M;
+          P::stat(a.ws, slot, h)[1] = L;
+        }
+      }
+    }
+    first_portion = false;
+    if (!next_portion(a, g, cur)) break;
+  }
+  cp_wait<0>();
+}
+
+// Joins the parts of the contexts that were split: one CTA per first part and
+// query head, a warp every eighth part.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) decode_attn_quant_join_kernel(TbDecodeAttnQuantArgs a, Geometry g, int grid) {
+  using P = Partials<D, NT>;
+  constexpr int kW = 8, E = D / 32;
+  __shared__ float red[kW], sl[kW], so[kW][D];
+  tb::pdl_wait();
+  const int* rec = P::record(a.ws, grid, blockIdx.x);
+  const int n = rec[2];
+  if (n == 0) return;
+  const int h = blockIdx.y, seg = rec[0], r = seg % g.HG, b = seg / g.HG;
+  const int h0 = r % g.NG * P::kHeads;
+  if (h0 + h >= g.G) return;
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long long own = rec[1], next = 2ll * blockIdx.x;
+  auto slot = [&](int p) { return p == 0 ? own : next + 2ll * p; };
+  float M = -INFINITY;
+  for (int p = threadIdx.x; p < n; p += blockDim.x) M = fmaxf(M, P::stat(a.ws, slot(p), h)[0]);
+  M = tb::warp_max(M);
+  if (lane == 0) red[w] = M;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kW; ++i) M = fmaxf(M, red[i]);
+  if (M == -INFINITY) M = 0.f;
+  float L = 0.f, o[E] = {};
+#pragma unroll 4
+  for (int p = w; p < n; p += kW) {
+    const float* st = P::stat(a.ws, slot(p), h);
+    const float* v = P::out(a.ws, slot(p), h);
+    const float f = exp2_fast(st[0] - M);
+    L += f * st[1];
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] += f * v[i * 32 + lane];
+  }
+  if (lane == 0) sl[w] = L;
+#pragma unroll
+  for (int i = 0; i < E; ++i) so[w][i * 32 + lane] = o[i];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float l = 0.f, v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      l += sl[i];
+      v += so[i][threadIdx.x];
+    }
+    T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b +
+             static_cast<long long>(r / g.NG * g.G + h0 + h) * a.os_h;
+    out[threadIdx.x] = tb::from_f32<T>(l == 0.f ? 0.f : v / l);
+  }
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
+// CTAs per SM that shared memory (228 KB, 1 KB of it per CTA the system's) leaves room for.
+template <int D, int NT>
+constexpr int resident() {
+  return 233472 / (Smem<D, NT>::kBytes + 1024) < 8 ? 233472 / (Smem<D, NT>::kBytes + 1024) : 8;
+}
+
+template <int D, int NT>
+Geometry geometry(const TbDecodeAttnQuantArgs& a) {
+  Geometry g;
+  g.G = a.Hq / a.cache.Hk;
+  g.NG = (g.G + 8 * NT - 1) / (8 * NT);
+  g.HG = a.cache.Hk * g.NG;
+  g.cap = static_cast<long long>(a.cache.max_blocks) * a.cache.bs;
+  g.whole = g.cap <= kWholeTokens;
+  return g;
+}
+
+template <typename T, int D, int NT>
+int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
+  using S = Smem<D, NT>;
+  const Geometry g = geometry<D, NT>(a);
+  auto kernel = decode_attn_quant_kernel<T, D, NT>;
+  const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const bool out4 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.os_b % 4 == 0 && a.os_h % 4 == 0;
+  if (g.whole) {
+    kernel<<<a.B * g.HG, kThreads, S::kBytes, s>>>(a, g, out4);
+    return static_cast<int>(cudaGetLastError());
+  }
+  const int grid = sm_count() * resident<D, NT>();
+  if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
+  kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, out4);
+  const cudaError_t e1 = cudaGetLastError();
+  if (e1 != cudaSuccess) return static_cast<int>(e1);
+  decode_attn_quant_join_kernel<T, D, NT><<<dim3(grid, 8 * NT), 256, 0, s>>>(a, g, grid);
   return static_cast<int>(cudaGetLastError());
+}
+
+// 16 columns where more than 8 query heads share a KV head, else 8.
+template <typename T>
+int launch_type(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
+  const bool two = a.Hq / a.cache.Hk > 8;
+  switch (a.cache.D) {
+    case 64: return two ? launch<T, 64, 2>(a, s) : launch<T, 64, 1>(a, s);
+    case 128: return two ? launch<T, 128, 2>(a, s) : launch<T, 128, 1>(a, s);
+    case 256: return two ? launch<T, 256, 2>(a, s) : launch<T, 256, 1>(a, s);
+  }
+  return static_cast<int>(cudaErrorInvalidValue);
 }
 
 }  // namespace
 
-extern "C" size_t tb_decode_attention_quant_ws_bytes(int, int, int, int, int) { return 0; }
+extern "C" size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens) {
+  if (B <= 0 || Hk <= 0 || max_tokens <= kWholeTokens) return 0;
+  const bool two = Hq / Hk > 8;
+  const int n = sm_count();
+  switch (D) {
+    case 64: return two ? Partials<64, 2>::bytes(n * resident<64, 2>()) : Partials<64, 1>::bytes(n * resident<64, 1>());
+    case 128:
+      return two ? Partials<128, 2>::bytes(n * resident<128, 2>()) : Partials<128, 1>::bytes(n * resident<128, 1>());
+    case 256:
+      return two ? Partials<256, 2>::bytes(n * resident<256, 2>()) : Partials<256, 1>::bytes(n * resident<256, 1>());
+  }
+  return 0;
+}
 
 extern "C" int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s) {
   const TbDecodeAttnQuantArgs& a = *args;
   if (a.B <= 0 || a.Hq <= 0) return 0;
-  if (a.cache.Hk <= 0 || a.Hq % a.cache.Hk || a.cache.bs <= 0) return static_cast<int>(cudaErrorInvalidValue);
-  if (a.dtype == TB_BF16) return launch<__nv_bfloat16>(a, s);
-  if (a.dtype == TB_F16) return launch<__half>(a, s);
+  if (a.cache.Hk <= 0 || a.Hq % a.cache.Hk || a.cache.bs <= 0 || a.cache.num_seqs != a.B)
+    return static_cast<int>(cudaErrorInvalidValue);
+  if (a.dtype == TB_BF16) return launch_type<__nv_bfloat16>(a, s);
+  if (a.dtype == TB_F16) return launch_type<__half>(a, s);
   return static_cast<int>(cudaErrorInvalidValue);
 }
