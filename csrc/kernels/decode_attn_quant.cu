@@ -7,17 +7,16 @@
 //
 // The pages are the traffic (2 (D + 4) bytes per token and KV head), read once:
 //
-//  * Work is cut into tiles of 16 tokens and dealt out evenly over a grid of
-//    resident CTAs, whatever the contexts' lengths: CTA c takes the tiles
-//    [c n / N, (c + 1) n / N) of the list (sequence, KV head, tile), read off
-//    ctx_len on the device, so one captured call serves contexts that grow.
-//    A (sequence, KV head) that ends up in several CTAs leaves partial results
-//    (maximum, sum, unnormalised output) that a second kernel joins in a fixed
+//  * Work is cut into tiles of 16 tokens and dealt out evenly over the warps of
+//    a resident grid, whatever the contexts' lengths: worker i of n takes the
+//    tiles [i T / n, (i + 1) T / n) of the list (sequence, KV head, tile), read
+//    off ctx_len on the device, so one captured call serves contexts that grow.
+//  * A warp fills a ring of tiles in its shared memory with cp.async, running
+//    ahead over the borders of contexts, and waits for no other warp before
+//    the end of its list.  Contexts that end inside its list it writes out; the
+//    parts at the list's two ends (maximum, sum, unnormalised output) the CTA
+//    merges, and what is split over CTAs a second kernel joins, all in a fixed
 //    order: no atomics, the same bits every time.
-//  * Each of a CTA's warps owns every fourth tile of a (sequence, KV head) and
-//    a ring of tiles in shared memory that it fills with cp.async, running
-//    ahead over the borders of contexts; nothing but the end of a (sequence,
-//    KV head) waits for another warp.
 //  * Products run on mma.sync m16n8k16 in fp16 (every e4m3 value is an fp16
 //    value) with the tokens, then the head's dimensions, as the 16 rows and the
 //    query heads as the 8 columns: with 5 to 8 query heads per KV head hardly a
@@ -40,7 +39,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;       // tokens per tile
-constexpr int kMinTiles = 8;    // a CTA takes at least this many tiles, where contexts are that long
+constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that many
 constexpr int kWholeTokens = 256;  // contexts that cannot be longer are not split
 constexpr int kMinVsExp = -100;
 
@@ -85,24 +84,33 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 
 // Shared memory.  A ring stage holds 16 K rows and 16 V rows of codes (rows
 // padded by 16 bytes against bank conflicts), their scales and a mask of the
-// tokens that count.
+// tokens that count.  A part is heads x D outputs, then heads x (maximum, sum):
+// a warp's first one goes to its place behind the rings, its last one into its
+// own ring, drained by then.
 template <int D, int NT>
 struct Smem {
-  static constexpr int kStages = D == 256 ? 3 : D == 128 ? 3 : 4;
+  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 3 : 4;
   static constexpr int kRow = D + 16;
   static constexpr int kStage = 2 * kTile * kRow + 2 * kTile * 4 + 16;
-  static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kQ = (D / 16) * NT * 32 * 8;
-  static constexpr int kOut = kWarps * kHeads * D * 4;
-  static constexpr int kScan = (2 * kWarps + 2) * 8;
-  static constexpr int kMisc = kWarps * kHeads * 8 + kHeads * 4 + kScan;
-  static constexpr int kBytes = kRing + kQ + kOut + kMisc;
+  static constexpr int kPart = kHeads * (D + 2) * 4;
+  static constexpr bool kQRegs = D * NT <= 256;  // q fragments in registers, else per warp in shared memory
+  static constexpr int kQ = kQRegs ? 0 : (D / 16) * NT * 32 * 8;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kScan = (2 * kWarps + 2 * kWarps) * 8;
+  static constexpr int kBytes = kWarps * (kRing + kPart + kQ) + kScan + 2 * kWarps * 16;
+  static_assert(kRing >= kPart && kRing % 16 == 0 && kPart % 16 == 0, "a part fits a ring");
 };
 
-// Partial results: per slot (two per CTA) heads x (D outputs, maximum, sum);
-// then one record per CTA: the (sequence, group) whose first part it holds, the
-// slot and the number of parts (0: none).
+// CTAs per SM that shared memory (228 KB, 1 KB of it per CTA the system's) leaves room for.
+template <int D, int NT>
+constexpr int resident() {
+  return 233472 / (Smem<D, NT>::kBytes + 1024) < 8 ? 233472 / (Smem<D, NT>::kBytes + 1024) : 8;
+}
+
+// Workspace: two parts per CTA (what its list's ends leave), then one record per
+// CTA: the (sequence, group) whose first part it holds, which part, and the
+// number of CTAs that hold one (0: none).
 template <int D, int NT>
 struct Partials {
   static constexpr int kHeads = 8 * NT;
@@ -131,14 +139,14 @@ __device__ __forceinline__ long long tiles_of(const TbDecodeAttnQuantArgs& a, co
   return (tokens_of(a, g, b) + kTile - 1) / kTile;
 }
 
-// Where a CTA (or a warp's prefetch) stands in the list of tiles: in sequence b,
+// Where a warp (or its prefetch) stands in its list of tiles: in sequence b,
 // group r, at tile t of the portion [.., end), with `rest` tiles behind it.
 struct Cursor {
   int b, r;
   long long t, end, rest, tokens;
 };
 
-// Moves on to the next portion; false at the end of the CTA's list.
+// Moves on to the next portion; false at the end of the list.
 __device__ __forceinline__ bool next_portion(const TbDecodeAttnQuantArgs& a, const Geometry& g, Cursor& c) {
   if (c.rest <= 0) return false;
   long long n = (c.tokens + kTile - 1) / kTile;
@@ -170,52 +178,50 @@ __device__ __forceinline__ void store_out4(T* p, bool aligned, float x, float y,
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool out4) {
+__global__ void __launch_bounds__(kThreads, resident<D, NT>())
+    decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool q8, bool out4) {
   using S = Smem<D, NT>;
   using P = Partials<D, NT>;
   constexpr int kStages = S::kStages, kHeads = S::kHeads, kRow = S::kRow;
   constexpr int NCH = D / 64;  // 16-byte chunks of a K row per lane
   constexpr int NW = D / 32;   // 4-byte words of a V row per lane
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* ring = smem;
-  uint2* qf = reinterpret_cast<uint2*>(smem + S::kRing);                 // [D / 16][NT][32] B fragments
-  float* so = reinterpret_cast<float*>(smem + S::kRing + S::kQ);         // [warps][heads][D]
-  float* sm = so + kWarps * kHeads * D;                                  // [warps][heads]
-  float* sl = sm + kWarps * kHeads;                                      // [warps][heads]
-  float* sc = sl + kWarps * kHeads;                                      // [heads] score factors
-  long long* sx = reinterpret_cast<long long*>(sc + kHeads);             // scan scratch
   const TbQuantCache& c = a.cache;
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32, gq = lane / 4, tq = lane % 4;
-  const int Hq = a.Hq;
+  uint8_t* ring = smem + w * S::kRing;
+  float* first_part = reinterpret_cast<float*>(smem + kWarps * S::kRing + w * S::kPart);
+  uint2* q_smem = reinterpret_cast<uint2*>(smem + kWarps * (S::kRing + S::kPart) + w * S::kQ);
+  long long* scan = reinterpret_cast<long long*>(smem + kWarps * (S::kRing + S::kPart + S::kQ));
+  int4* meta = reinterpret_cast<int4*>(scan + 4 * kWarps);  // of the 2 kWarps parts: (sequence, group, opens | closes << 1, tiles behind it)
 
-  // ---- this CTA's list of tiles
+  // ---- this warp's list of tiles
   Cursor cur;
-  long long first = 0, total = 0;
+  long long total = 0;
   int N = gridDim.x;
   if (g.whole) {
     cur.b = blockIdx.x / g.HG;
     cur.r = blockIdx.x % g.HG;
     cur.tokens = tokens_of(a, g, cur.b);
-    cur.t = 0;
-    cur.end = (cur.tokens + kTile - 1) / kTile;
-    cur.rest = 0;
+    const int n = static_cast<int>((cur.tokens + kTile - 1) / kTile);
     if (a.err && threadIdx.x == 0 && a.ctx_len[cur.b] > g.cap) atomicCAS(a.err, 0, 1);
-    if (cur.end == 0) {
+    if (n == 0) {
       T* o = static_cast<T*>(a.out) + static_cast<long long>(cur.b) * a.os_b;
-      const int kh = cur.r / g.NG, h0 = (cur.r % g.NG) * kHeads;
-      const int nh = g.G - h0 < kHeads ? g.G - h0 : kHeads;
-      for (int i = threadIdx.x; i < nh * D; i += kThreads)
-        o[static_cast<long long>(kh * g.G + h0 + i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
+      const int h0 = cur.r / g.NG * g.G + cur.r % g.NG * kHeads, left = g.G - cur.r % g.NG * kHeads;
+      for (int i = threadIdx.x; i < (left < kHeads ? left : kHeads) * D; i += kThreads)
+        o[static_cast<long long>(h0 + i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
       return;
     }
+    cur.t = n * w / kWarps;
+    cur.end = n * (w + 1) / kWarps;
+    cur.rest = 0;
   } else {
     // empty contexts, and contexts longer than their tables
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
       const int n = a.ctx_len[b];
       if (a.err && threadIdx.x == 0 && n > g.cap) atomicCAS(a.err, 0, 1);
-      if (n <= 0 || g.cap == 0) {
+      if (n <= 0) {
         T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
-        for (int i = threadIdx.x; i < Hq * D; i += kThreads)
+        for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
           o[static_cast<long long>(i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
       }
     }
@@ -223,70 +229,63 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
     const int per = (a.B + kThreads - 1) / kThreads, b0 = threadIdx.x * per;
     const int b1 = b0 + per < a.B ? b0 + per : a.B;
     long long mine = 0;
-    int some = 0;
-    for (int b = b0; b < b1; ++b) {
-      const long long n = tiles_of(a, g, b);
-      mine += n;
-      some += n > 0;
-    }
+    for (int b = b0; b < b1; ++b) mine += tiles_of(a, g, b);
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    const long long live = tb::warp_sum(some);
-    if (lane == 31) {
-      sx[w] = inc;
-      sx[kWarps + w] = live;
-    }
+    if (lane == 31) scan[w] = inc;
     __syncthreads();
-    long long before = inc - mine, segs = 0;
+    long long before = inc - mine;
+#pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      if (i < w) before += sx[i];
-      total += sx[i];
-      segs += sx[kWarps + i];
+      if (i < w) before += scan[i];
+      total += scan[i];
     }
     total *= g.HG;
-    segs *= g.HG;
-    long long want = (total + kMinTiles - 1) / kMinTiles;
-    if (want < segs) want = segs;
+    before *= g.HG;
+    mine *= g.HG;
+    const long long want = (total + kMinTiles - 1) / kMinTiles;
     if (want < N) N = static_cast<int>(want);
     if (threadIdx.x == 0) P::record(a.ws, gridDim.x, blockIdx.x)[2] = 0;
     if (static_cast<int>(blockIdx.x) >= N) return;
-    first = blockIdx.x * total / N;
-    const long long last = (blockIdx.x + 1) * total / N;
-    if (first >= before * g.HG && first < (before + mine) * g.HG) {
-      int b = b0;
-      long long at = before, n = tiles_of(a, g, b);
-      while (first >= (at + n) * g.HG) {
-        at += n;
-        n = tiles_of(a, g, ++b);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const long long f = (static_cast<long long>(blockIdx.x) * kWarps + i) * total / (static_cast<long long>(N) * kWarps);
+      if (f >= before && f < before + mine) {
+        int b = b0;
+        long long at = before, n = tiles_of(a, g, b) * g.HG;
+        while (f >= at + n) {
+          at += n;
+          n = tiles_of(a, g, ++b) * g.HG;
+        }
+        scan[2 * kWarps + 2 * i] = b;
+        scan[2 * kWarps + 2 * i + 1] = f - at;
       }
-      sx[2 * kWarps] = b;
-      sx[2 * kWarps + 1] = first - at * g.HG;
     }
     __syncthreads();
-    cur.b = static_cast<int>(sx[2 * kWarps]);
-    const long long off = sx[2 * kWarps + 1], n = tiles_of(a, g, cur.b);
+    const long long me = static_cast<long long>(blockIdx.x) * kWarps + w, all = static_cast<long long>(N) * kWarps;
+    const long long first = me * total / all, last = (me + 1) * total / all;
+    cur.b = static_cast<int>(scan[2 * kWarps + 2 * w]);
+    const long long off = scan[2 * kWarps + 2 * w + 1];
     cur.tokens = tokens_of(a, g, cur.b);
+    const long long n = (cur.tokens + kTile - 1) / kTile;
     cur.r = static_cast<int>(off / n);
     cur.t = off - cur.r * n;
     cur.rest = last - first;
     cur.end = n - cur.t < cur.rest ? n : cur.t + cur.rest;
     cur.rest -= cur.end - cur.t;
   }
+  if (lane == 0) meta[2 * w] = meta[2 * w + 1] = make_int4(-1, 0, 0, 0);
 
-  // ---- this warp's prefetch: a cursor that runs ahead, and the cache rows of its next tile (lanes 0-15)
+  // ---- prefetch: a cursor that runs ahead, and the cache rows of its next tile (lanes 0-15)
   Cursor pre = cur;
-  pre.t += w;
   bool more = true;
   int row = -1;
   auto look = [&]() {  // settles the cursor on a tile and looks its tokens' rows up
-    while (more && pre.t >= pre.end) {
-      more = next_portion(a, g, pre);
-      if (more) pre.t += w;
-    }
+    if (more && pre.t >= pre.end) more = next_portion(a, g, pre);
     row = -1;
     const long long tok = pre.t * kTile + lane;
     if (more && lane < kTile && tok < pre.tokens) {
@@ -299,13 +298,12 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
       }
     }
   };
-  uint8_t* my_ring = ring + w * kStages * S::kStage;
-  const uint32_t my_ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
+  const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   int put = 0;
   auto issue = [&]() {  // copies the tile that the cursor stands on, then moves the cursor on
     if (more) {
       constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // chunks per row, rows per instruction
-      const uint32_t st = my_ring_s + put * S::kStage;
+      const uint32_t st = ring_s + put * S::kStage;
 #pragma unroll
       for (int i = 0; i < kTile / kRows; ++i) {
         const int tr = i * kRows + lane / kChunks, ch = lane % kChunks;
@@ -322,10 +320,9 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
         cp_async4(st + 2 * kTile * kRow + lane * 4, c.ks + rr, row < 0 ? 0 : 4);
         cp_async4(st + 2 * kTile * kRow + kTile * 4 + lane * 4, c.vs + rr, row < 0 ? 0 : 4);
       }
-      if (lane == 0)
-        *reinterpret_cast<unsigned*>(my_ring + put * S::kStage + 2 * kTile * kRow + 2 * kTile * 4) = mask;
+      if (lane == 0) *reinterpret_cast<unsigned*>(ring + put * S::kStage + 2 * kTile * kRow + 2 * kTile * 4) = mask;
       put = put + 1 == kStages ? 0 : put + 1;
-      pre.t += kWarps;
+      ++pre.t;
       look();
     }
     cp_commit();
@@ -334,51 +331,61 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
 
-  // ---- portions of this CTA, one (sequence, group) each
+  // ---- portions of this warp, one (sequence, group) each
   int get = 0;
-  bool first_portion = true;
-  while (true) {
-    const int kh = cur.r / g.NG, h0 = (cur.r % g.NG) * kHeads;  // KV head, first of this group's query heads
-    const int nh = g.G - h0 < kHeads ? g.G - h0 : kHeads;
-    const long long ntiles = (cur.tokens + kTile - 1) / kTile;
-    // q as B fragments: lane (n = head, t) holds, for each k step, dimensions d0 .. d0 + 3 with
-    // d0 = (t * NCH + i) * 16 + 4 j, the same that it reads of a K row
-    for (int h = w; h < kHeads; h += kWarps) {
-      float v[D / 32][4 / (D < 128 ? 2 : 1)];
-      constexpr int E = D < 128 ? 2 : 4;  // dimensions per lane and round
+  bool first_portion = true, going = cur.t < cur.end;
+  while (going) {
+    const int h0 = cur.r / g.NG * g.G + cur.r % g.NG * kHeads;  // first query head of the group
+    const int left = g.G - cur.r % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
+    // q as B fragments: lane (head gq, tq) holds, for k step (i, j), the dimensions (tq NCH + i) 16 + 4 j .. + 3, the
+    // same that it reads of a K row.  A power of two per head brings them into fp16's range.
+    uint2 qf[S::kQRegs ? NT * (D / 16) : 1];
+    float ch[NT][2], m[NT][2], l[NT][2], acc[2 * NW][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float v[D / 4];
       uint32_t top = 0;
+      const bool live = n * 8 + gq < nh;
       const T* q = static_cast<const T*>(a.q) + static_cast<long long>(cur.b) * a.qs_b +
-                   static_cast<long long>(kh * g.G + h0 + h) * a.qs_h;
+                   static_cast<long long>(h0 + (live ? n * 8 + gq : 0)) * a.qs_h + tq * (D / 4);
+      if (q8) {
 #pragma unroll
-      for (int i = 0; i < D / (32 * E); ++i)
+        for (int i = 0; i < D / 4; i += 8) {
+          float f[8];
+          tb::load_vec<T, 8>(q + i, f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          v[i][e] = h < nh ? tb::to_f32(q[(i * 32 + lane) * E + e]) : 0.f;
-          top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+          for (int e = 0; e < 8; ++e) v[i + e] = f[e];
         }
-      top = __reduce_max_sync(0xffffffffu, top);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) v[i] = tb::to_f32(q[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) {
+        if (!live) v[i] = 0.f;
+        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e2 = max(static_cast<int>(top >> 23) - 127, -100);
       const float f = pow2i(13 - e2);
 #pragma unroll
-      for (int i = 0; i < D / (32 * E); ++i) {
-        const int d = (i * 32 + lane) * E, ch = d / 16, j = d % 16 / 4;
-        uint32_t* to = reinterpret_cast<uint32_t*>(qf + (((ch % NCH) * 4 + j) * NT + h / 8) * 32 + (h % 8) * 4 + ch / NCH);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) to[(d % 4 + e) / 2] = pack_f16(v[i][e] * f, v[i][e + 1] * f);
+      for (int i = 0; i < D / 16; ++i) {
+        const uint2 x = make_uint2(pack_f16(v[4 * i] * f, v[4 * i + 1] * f), pack_f16(v[4 * i + 2] * f, v[4 * i + 3] * f));
+        if constexpr (S::kQRegs)
+          qf[i * NT + n] = x;
+        else
+          q_smem[(i * NT + n) * 32 + lane] = x;  // read by this lane only
       }
-      // 2^(e2 - 13), times the scale in units of log 2
-      if (lane == 0) sc[h] = a.scale * 1.4426950408889634f * pow2i(e2 - 13);
-    }
-    __syncthreads();
-    float ch[NT][2], m[NT][2], l[NT][2], acc[2 * NW][NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+      // 2^(e2 - 13), times the scale in units of log 2; a lane's columns are heads 2 tq and 2 tq + 1
+      const float mine = a.scale * 1.4426950408889634f * pow2i(e2 - 13);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        ch[n][e] = sc[n * 8 + 2 * tq + e];
+        ch[n][e] = __shfl_sync(0xffffffffu, mine, (2 * tq + e) * 4);
         m[n][e] = -INFINITY;
         l[n][e] = 0.f;
       }
+    }
 #pragma unroll
     for (int i = 0; i < 2 * NW; ++i)
 #pragma unroll
@@ -386,10 +393,10 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
 
-    for (long long t = cur.t + w; t < cur.end; t += kWarps) {
+    for (long long t = cur.t; t < cur.end; ++t) {
       cp_wait<kStages - 2>();
       __syncwarp();
-      const uint8_t* st = my_ring + get * S::kStage;
+      const uint8_t* st = ring + get * S::kStage;
       const float* scales = reinterpret_cast<const float*>(st + 2 * kTile * kRow);
       const unsigned mask = *reinterpret_cast<const unsigned*>(st + 2 * kTile * kRow + 2 * kTile * 4);
       // S^T [16 tokens, heads] = K q
@@ -406,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
           const uint32_t a0 = f16x2_of(xs[j]), a1 = f16x2_of(ys[j]), a2 = f16x2_of(xs[j] >> 16), a3 = f16x2_of(ys[j] >> 16);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint2 b = qf[((i * 4 + j) * NT + n) * 32 + lane];
+            const uint2 b = S::kQRegs ? qf[S::kQRegs ? (i * 4 + j) * NT + n : 0] : q_smem[((i * 4 + j) * NT + n) * 32 + lane];
             mma16816(s[n], a0, a1, a2, a3, b.x, b.y);
           }
         }
@@ -482,60 +489,108 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
       issue();
     }
 
-    // ---- join the warps
+    // ---- the end of the portion: a whole context is written out, a part kept for the CTA's merge
+    const bool opens = cur.t == 0;
+    const int behind = static_cast<int>((cur.tokens + kTile - 1) / kTile - cur.end);
+    const bool closes = behind == 0;
+    const int b = cur.b, r = cur.r;
+    going = next_portion(a, g, cur);
+    float* part = first_portion ? first_part : reinterpret_cast<float*>(ring);
+    if (!first_portion && !(opens && closes)) {  // the list's last portion: the ring is done with
+      cp_wait<0>();
+      __syncwarp();
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        const int h = n * 8 + 2 * tq + e;
         float v = l[n][e];
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (gq == 0) {
-          sm[w * kHeads + n * 8 + 2 * tq + e] = m[n][e];
-          sl[w * kHeads + n * 8 + 2 * tq + e] = v;
-        }
+        const float inv = v == 0.f ? 0.f : 1.f / v;
+        T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
           const int d = NW < 4 ? gq * 8 + 4 * k : (k / 4) * 128 + gq * 16 + 4 * (k % 4);
-          *reinterpret_cast<float4*>(so + (w * kHeads + n * 8 + 2 * tq + e) * D + d) =
-              make_float4(acc[2 * k][n][e], acc[2 * k][n][2 + e], acc[2 * k + 1][n][e], acc[2 * k + 1][n][2 + e]);
+          const float y0 = acc[2 * k][n][e], y1 = acc[2 * k][n][2 + e], y2 = acc[2 * k + 1][n][e],
+                      y3 = acc[2 * k + 1][n][2 + e];
+          if (opens && closes) {
+            if (h < nh) store_out4<T>(o + d, out4, y0 * inv, y1 * inv, y2 * inv, y3 * inv);
+          } else {
+            *reinterpret_cast<float4*>(part + h * D + d) = make_float4(y0, y1, y2, y3);
+          }
         }
+        if (!(opens && closes) && gq == 0)
+          *reinterpret_cast<float2*>(part + kHeads * D + 2 * h) = make_float2(m[n][e], v);
       }
-    __syncthreads();
-    const bool all = cur.t == 0 && cur.end == ntiles;  // the whole context was here
-    const long long slot = 2ll * blockIdx.x + (first_portion ? 0 : 1);
-    if (!all && cur.t == 0 && threadIdx.x == 0) {
-      // the first part: the others are in the CTAs up to the one that owns the last tile
+    if (!(opens && closes) && lane == 0)
+      meta[2 * w + (first_portion ? 0 : 1)] = make_int4(b, r, (opens ? 1 : 0) | (closes ? 2 : 0), behind);
+    first_portion = false;
+  }
+  cp_wait<0>();
+  __syncthreads();
+
+  // ---- merge the parts of this CTA: runs of the same (sequence, group)
+  bool first_run = true;
+  for (int x = 0; x < 2 * kWarps;) {
+    const int4 at = meta[x];
+    if (at.x < 0) {
+      ++x;
+      continue;
+    }
+    int y = x, bits = 0, behind = 0;  // behind: tiles of the context after the run
+    unsigned set = 0;
+    while (y < 2 * kWarps) {
+      const int4 o = meta[y];
+      if (o.x >= 0) {
+        if (o.x != at.x || o.y != at.y) break;
+        set |= 1u << y;
+        bits |= o.z;
+        behind = o.w;
+      }
+      ++y;
+    }
+    x = y;
+    const bool whole = bits == 3;
+    const int h0 = at.y / g.NG * g.G + at.y % g.NG * kHeads;
+    const int left = g.G - at.y % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
+    const long long slot = 2ll * blockIdx.x + (first_run ? 0 : 1);
+    if (bits == 1 && threadIdx.x == 0) {
+      // the first part of a context that goes on: the others are in the CTAs up to the one with its last tile
+      const long long all = static_cast<long long>(N) * kWarps;
+      const long long last_tile = (blockIdx.x + 1ll) * kWarps * total / all + behind - 1;
       int* rec = P::record(a.ws, gridDim.x, blockIdx.x);
-      const long long list_end = (blockIdx.x + 1) * total / N;             // list position behind this portion
-      const long long last_tile = list_end + (ntiles - cur.end) - 1;       // list position of the context's last tile
-      const long long owner = ((last_tile + 1) * N - 1) / total;
-      rec[0] = cur.b * g.HG + cur.r;
+      rec[0] = at.x * g.HG + at.y;
       rec[1] = static_cast<int>(slot);
-      rec[2] = static_cast<int>(owner - blockIdx.x) + 1;
+      rec[2] = static_cast<int>(((last_tile + 1) * all - 1) / total / kWarps - blockIdx.x) + 1;
     }
     for (int i = threadIdx.x; i < nh * (D / 4); i += kThreads) {
       const int h = i / (D / 4), d = i % (D / 4) * 4;
+      auto part_of = [&](int p) {
+        return p % 2 ? reinterpret_cast<const float*>(smem + p / 2 * S::kRing)
+                     : reinterpret_cast<const float*>(smem + kWarps * S::kRing + p / 2 * S::kPart);
+      };
       float M = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) M = fmaxf(M, sm[x * kHeads + h]);
+      for (unsigned r = set; r; r &= r - 1) M = fmaxf(M, part_of(__ffs(r) - 1)[kHeads * D + 2 * h]);
       const float mr = M == -INFINITY ? 0.f : M;
       float L = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float f = exp2_fast(sm[x * kHeads + h] - mr);
-        const float4 v = *reinterpret_cast<const float4*>(so + (x * kHeads + h) * D + d);
-        L += f * sl[x * kHeads + h];
+      for (unsigned r = set; r; r &= r - 1) {
+        const float* p = part_of(__ffs(r) - 1);
+        const float2 st = *reinterpret_cast<const float2*>(p + kHeads * D + 2 * h);
+        const float f = exp2_fast(st.x - mr);
+        const float4 v = *reinterpret_cast<const float4*>(p + h * D + d);
+        L += f * st.y;
         o0 += f * v.x;
         o1 += f * v.y;
         o2 += f * v.z;
         o3 += f * v.w;
       }
-      if (all) {
+      if (whole) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        store_out4<T>(static_cast<T*>(a.out) + static_cast<long long>(cur.b) * a.os_b +
-                          static_cast<long long>(kh * g.G + h0 + h) * a.os_h + d,
+        store_out4<T>(static_cast<T*>(a.out) + static_cast<long long>(at.x) * a.os_b +
+                          static_cast<long long>(h0 + h) * a.os_h + d,
                       out4, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
       } else {
         *reinterpret_cast<float4*>(P::out(a.ws, slot, h) + d) = make_float4(o0, o1, o2, o3);
@@ -545,10 +600,8 @@ __global__ void __launch_bounds__(kThreads) decode_attn_quant_kernel(TbDecodeAtt
         }
       }
     }
-    first_portion = false;
-    if (!next_portion(a, g, cur)) break;
+    first_run = false;
   }
-  cp_wait<0>();
 }
 
 // Joins the parts of the contexts that were split: one CTA per first part and
@@ -610,12 +663,6 @@ int sm_count() {
   return n;
 }
 
-// CTAs per SM that shared memory (228 KB, 1 KB of it per CTA the system's) leaves room for.
-template <int D, int NT>
-constexpr int resident() {
-  return 233472 / (Smem<D, NT>::kBytes + 1024) < 8 ? 233472 / (Smem<D, NT>::kBytes + 1024) : 8;
-}
-
 template <int D, int NT>
 Geometry geometry(const TbDecodeAttnQuantArgs& a) {
   Geometry g;
@@ -634,14 +681,15 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   auto kernel = decode_attn_quant_kernel<T, D, NT>;
   const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
   if (e != cudaSuccess) return static_cast<int>(e);
+  const bool q8 = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.qs_b % 8 == 0 && a.qs_h % 8 == 0;
   const bool out4 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.os_b % 4 == 0 && a.os_h % 4 == 0;
   if (g.whole) {
-    kernel<<<a.B * g.HG, kThreads, S::kBytes, s>>>(a, g, out4);
+    kernel<<<a.B * g.HG, kThreads, S::kBytes, s>>>(a, g, q8, out4);
     return static_cast<int>(cudaGetLastError());
   }
   const int grid = sm_count() * resident<D, NT>();
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
-  kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, out4);
+  kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, q8, out4);
   const cudaError_t e1 = cudaGetLastError();
   if (e1 != cudaSuccess) return static_cast<int>(e1);
   decode_attn_quant_join_kernel<T, D, NT><<<dim3(grid, 8 * NT), 256, 0, s>>>(a, g, grid);
