@@ -23,11 +23,13 @@
 //    column is idle, and a tcgen05 tile (128 rows by 8 columns) would want the
 //    codes widened through shared memory first.  S^T = K q, whose accumulator,
 //    transposed in registers (movmatrix), is the operand of O^T = V^T w.
-//  * The running maximum m is of a_j + e_j, e_j the exponent of vs_j: then the
-//    weights w_j = exp2(a_j - m) vs_j lie in [0, 2) and fit fp16 however much
-//    the scales of tokens differ (round to 2^-11 relative, 2^-25 absolute at
-//    the small end), while the sum l of exp2(a_j - m) stays in fp32 range.
-//    q is brought into fp16 range by a power of two per head (exact).
+//  * The weights' reference m follows the running maximum of a_j + log2 vs_j
+//    (a_j in units of log 2): then w_j = exp2(a_j - m) vs_j fits fp16 however
+//    much the scales of tokens differ (rounded to 2^-11 relative, 2^-25 absolute
+//    at the small end), while the sum l of exp2(a_j - m) stays in fp32 range.
+//    m moves only once the maximum is 2^8 above it, so weights stay below 2^8
+//    and most tiles need no reduction over the warp and no rescaling.  q is
+//    brought into fp16 range by a power of two per head (exact).
 #include <math.h>
 
 #include "device_common.cuh"
@@ -41,12 +43,14 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;       // tokens per tile
 constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that many
 constexpr int kWholeTokens = 256;  // contexts that cannot be longer are not split
-constexpr int kMinVsExp = -100;
+constexpr float kMinVsLog = -100.f;
+constexpr float kSlack = 8.f;   // the reference of the weights may lag behind their maximum by a factor of 2^8
 
-__device__ __forceinline__ uint32_t f16x2_of(uint32_t two_codes) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two_codes)));
-  return r;
+// The four codes of a word as two fp16 pairs.
+__device__ __forceinline__ void widen(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -67,6 +71,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // 2^e for e in [-126, 127]
@@ -109,8 +118,9 @@ constexpr int resident() {
 }
 
 // Workspace: two parts per CTA (what its list's ends leave), then one record per
-// CTA: the (sequence, group) whose first part it holds, which part, and the
-// number of CTAs that hold one (0: none).
+// CTA: of the context whose first part it holds (sequence x group, part, CTAs that
+// share it or 0), and the first CTA of the one that came over from the CTA before
+// (or -1).
 template <int D, int NT>
 struct Partials {
   static constexpr int kHeads = 8 * NT;
@@ -119,47 +129,46 @@ struct Partials {
   __device__ static float* stat(float* ws, long long slot, int h) {
     return ws + slot * kSlot + kHeads * D + h * 2;
   }
-  __device__ static int* record(float* ws, int grid, int c) {
-    return reinterpret_cast<int*>(ws + 2ll * grid * kSlot) + 4ll * c;
+  __device__ static int4* record(float* ws, int grid, int c) {
+    return reinterpret_cast<int4*>(ws + 2ll * grid * kSlot) + c;
   }
   static size_t bytes(int grid) { return (2 * grid * kSlot + 4 * static_cast<size_t>(grid)) * 4; }
 };
 
 struct Geometry {
   int G, NG, HG;   // query heads per KV head, groups of 8 NT of them, groups per sequence
-  long long cap;   // tokens that a table row can name
+  int cap;         // tokens that a table row can name
+  int shift;       // log2 of the page size, or -1
+  int tile_pages;  // pages hold whole tiles
   int whole;       // one CTA per (sequence, group), nothing to join
 };
 
-__device__ __forceinline__ long long tokens_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
-  const long long n = a.ctx_len[b];
+__device__ __forceinline__ int tokens_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
+  const int n = a.ctx_len[b];
   return n < 0 ? 0 : n < g.cap ? n : g.cap;
-}
-__device__ __forceinline__ long long tiles_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
-  return (tokens_of(a, g, b) + kTile - 1) / kTile;
 }
 
 // Where a warp (or its prefetch) stands in its list of tiles: in sequence b,
 // group r, at tile t of the portion [.., end), with `rest` tiles behind it.
 struct Cursor {
-  int b, r;
-  long long t, end, rest, tokens;
+  int b, r, tokens, t, end;
+  long long rest;
 };
+__device__ __forceinline__ int tiles(int tokens) { return tokens / kTile + (tokens % kTile != 0); }
 
 // Moves on to the next portion; false at the end of the list.
 __device__ __forceinline__ bool next_portion(const TbDecodeAttnQuantArgs& a, const Geometry& g, Cursor& c) {
   if (c.rest <= 0) return false;
-  long long n = (c.tokens + kTile - 1) / kTile;
   if (++c.r == g.HG) {
     c.r = 0;
     do {
       if (++c.b >= a.B) return false;
       c.tokens = tokens_of(a, g, c.b);
-      n = (c.tokens + kTile - 1) / kTile;
-    } while (n == 0);
+    } while (c.tokens == 0);
   }
+  const int n = tiles(c.tokens);
   c.t = 0;
-  c.end = n < c.rest ? n : c.rest;
+  c.end = n < c.rest ? n : static_cast<int>(c.rest);
   c.rest -= c.end;
   return true;
 }
@@ -192,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   float* first_part = reinterpret_cast<float*>(smem + kWarps * S::kRing + w * S::kPart);
   uint2* q_smem = reinterpret_cast<uint2*>(smem + kWarps * (S::kRing + S::kPart) + w * S::kQ);
   long long* scan = reinterpret_cast<long long*>(smem + kWarps * (S::kRing + S::kPart + S::kQ));
-  int4* meta = reinterpret_cast<int4*>(scan + 4 * kWarps);  // of the 2 kWarps parts: (sequence, group, opens | closes << 1, tiles behind it)
+  int4* meta = reinterpret_cast<int4*>(scan + 4 * kWarps);  // of the 2 kWarps parts: (sequence, group, opens | closes << 1 | first tile << 2, tiles behind it)
 
   // ---- this warp's list of tiles
   Cursor cur;
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     cur.b = blockIdx.x / g.HG;
     cur.r = blockIdx.x % g.HG;
     cur.tokens = tokens_of(a, g, cur.b);
-    const int n = static_cast<int>((cur.tokens + kTile - 1) / kTile);
+    const int n = tiles(cur.tokens);
     if (a.err && threadIdx.x == 0 && a.ctx_len[cur.b] > g.cap) atomicCAS(a.err, 0, 1);
     if (n == 0) {
       T* o = static_cast<T*>(a.out) + static_cast<long long>(cur.b) * a.os_b;
@@ -215,21 +224,12 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     cur.end = n * (w + 1) / kWarps;
     cur.rest = 0;
   } else {
-    // empty contexts, and contexts longer than their tables
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-      const int n = a.ctx_len[b];
-      if (a.err && threadIdx.x == 0 && n > g.cap) atomicCAS(a.err, 0, 1);
-      if (n <= 0) {
-        T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
-        for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
-          o[static_cast<long long>(i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
-      }
-    }
     // prefix sums of the sequences' tiles: each thread a run of sequences
     const int per = (a.B + kThreads - 1) / kThreads, b0 = threadIdx.x * per;
     const int b1 = b0 + per < a.B ? b0 + per : a.B;
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(a, g, b);
+#pragma unroll 4
+    for (int b = b0; b < b1; ++b) mine += tiles(tokens_of(a, g, b));
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -249,17 +249,17 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     mine *= g.HG;
     const long long want = (total + kMinTiles - 1) / kMinTiles;
     if (want < N) N = static_cast<int>(want);
-    if (threadIdx.x == 0) P::record(a.ws, gridDim.x, blockIdx.x)[2] = 0;
+    if (threadIdx.x == 0) *P::record(a.ws, gridDim.x, blockIdx.x) = make_int4(0, 0, 0, -1);
     if (static_cast<int>(blockIdx.x) >= N) return;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       const long long f = (static_cast<long long>(blockIdx.x) * kWarps + i) * total / (static_cast<long long>(N) * kWarps);
       if (f >= before && f < before + mine) {
         int b = b0;
-        long long at = before, n = tiles_of(a, g, b) * g.HG;
+        long long at = before, n = static_cast<long long>(tiles(tokens_of(a, g, b))) * g.HG;
         while (f >= at + n) {
           at += n;
-          n = tiles_of(a, g, ++b) * g.HG;
+          n = static_cast<long long>(tiles(tokens_of(a, g, ++b))) * g.HG;
         }
         scan[2 * kWarps + 2 * i] = b;
         scan[2 * kWarps + 2 * i + 1] = f - at;
@@ -271,54 +271,73 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     cur.b = static_cast<int>(scan[2 * kWarps + 2 * w]);
     const long long off = scan[2 * kWarps + 2 * w + 1];
     cur.tokens = tokens_of(a, g, cur.b);
-    const long long n = (cur.tokens + kTile - 1) / kTile;
+    const int n = tiles(cur.tokens);
     cur.r = static_cast<int>(off / n);
-    cur.t = off - cur.r * n;
+    cur.t = static_cast<int>(off - static_cast<long long>(cur.r) * n);
     cur.rest = last - first;
-    cur.end = n - cur.t < cur.rest ? n : cur.t + cur.rest;
+    cur.end = n - cur.t < cur.rest ? n : cur.t + static_cast<int>(cur.rest);
     cur.rest -= cur.end - cur.t;
   }
   if (lane == 0) meta[2 * w] = meta[2 * w + 1] = make_int4(-1, 0, 0, 0);
 
-  // ---- prefetch: a cursor that runs ahead, and the cache rows of its next tile (lanes 0-15)
+  // ---- prefetch: a cursor that runs ahead, and where its next tile lies: with pages of whole tiles the tile's first row
+  // and its number of tokens, else (lanes 0-15) each token's row
   Cursor pre = cur;
   bool more = true;
-  int row = -1;
-  auto look = [&]() {  // settles the cursor on a tile and looks its tokens' rows up
-    if (more && pre.t >= pre.end) more = next_portion(a, g, pre);
-    row = -1;
-    const long long tok = pre.t * kTile + lane;
-    if (more && lane < kTile && tok < pre.tokens) {
-      const int pb = static_cast<int>(tok) / c.bs;
-      const int blk = c.block_table[static_cast<long long>(pre.b) * c.max_blocks + pb];
-      if (blk >= 0 && blk < c.num_blocks) {
-        row = (blk * c.Hk + pre.r / g.NG) * c.bs + (static_cast<int>(tok) - pb * c.bs);
-      } else if (a.err) {
-        atomicCAS(a.err, 0, 1);
-      }
+  int row = -1, count = 0, pre_kh = cur.r / g.NG;
+  auto look = [&]() {
+    if (more && pre.t >= pre.end) {
+      more = next_portion(a, g, pre);
+      pre_kh = pre.r / g.NG;
     }
+    if (!more) return;
+    const int tok = pre.t * kTile + (g.tile_pages ? 0 : lane);
+    row = -1;
+    if (g.tile_pages || (lane < kTile && tok < pre.tokens)) {
+      const int pb = g.shift >= 0 ? tok >> g.shift : tok / c.bs;
+      const int blk = c.block_table[static_cast<long long>(pre.b) * c.max_blocks + pb];
+      if (blk >= 0 && blk < c.num_blocks)
+        row = (blk * c.Hk + pre_kh) * c.bs + (tok - pb * c.bs);
+      else if (a.err)
+        atomicCAS(a.err, 0, 1);
+    }
+    if (g.tile_pages) count = row < 0 ? 0 : min(pre.tokens - tok, kTile);
   };
   const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // chunks per row, rows per instruction
+  const uint32_t to_lane = ring_s + lane / kChunks * kRow + lane % kChunks * 16;
   int put = 0;
   auto issue = [&]() {  // copies the tile that the cursor stands on, then moves the cursor on
     if (more) {
-      constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // chunks per row, rows per instruction
-      const uint32_t st = ring_s + put * S::kStage;
+      const uint32_t st = ring_s + put * S::kStage, dst = to_lane + put * S::kStage;
+      unsigned mask;
+      if (g.tile_pages) {
+        // rows behind the context are copied as K (their scores are masked), but not as V: a NaN there times a weight of 0
+        const long long at = static_cast<long long>(count > 0 ? row : 0) * D + lane * 16;
+        const uint8_t *kp = static_cast<const uint8_t*>(c.kc) + at, *vp = static_cast<const uint8_t*>(c.vc) + at;
 #pragma unroll
-      for (int i = 0; i < kTile / kRows; ++i) {
-        const int tr = i * kRows + lane / kChunks, ch = lane % kChunks;
-        const int rr = __shfl_sync(0xffffffffu, row, tr);
-        const long long at = static_cast<long long>(rr < 0 ? 0 : rr) * D + ch * 16;
-        const int bytes = rr < 0 ? 0 : 16;
-        const uint32_t dst = st + tr * kRow + ch * 16;
-        cp_async16(dst, static_cast<const uint8_t*>(c.kc) + at, bytes);
-        cp_async16(dst + kTile * kRow, static_cast<const uint8_t*>(c.vc) + at, bytes);
-      }
-      const unsigned mask = __ballot_sync(0xffffffffu, row >= 0);
-      if (lane < kTile) {
-        const int rr = row < 0 ? 0 : row;
-        cp_async4(st + 2 * kTile * kRow + lane * 4, c.ks + rr, row < 0 ? 0 : 4);
-        cp_async4(st + 2 * kTile * kRow + kTile * 4 + lane * 4, c.vs + rr, row < 0 ? 0 : 4);
+        for (int i = 0; i < kTile / kRows; ++i) {
+          cp_async16(dst + i * kRows * kRow, kp + i * 512, count > 0 ? 16 : 0);
+          cp_async16(dst + (kTile + i * kRows) * kRow, vp + i * 512, i * kRows + lane / kChunks < count ? 16 : 0);
+        }
+        if (lane < 8)  // 16 scales of K, 16 of V
+          cp_async16(st + 2 * kTile * kRow + lane * 16,
+                     (lane < 4 ? c.ks : c.vs) + (count > 0 ? row : 0) + lane % 4 * 4, count > 0 ? 16 : 0);
+        mask = (1u << count) - 1;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTile / kRows; ++i) {
+          const int rr = __shfl_sync(0xffffffffu, row, i * kRows + lane / kChunks);
+          const long long at = static_cast<long long>(rr < 0 ? 0 : rr) * D + lane % kChunks * 16;
+          cp_async16(dst + i * kRows * kRow, static_cast<const uint8_t*>(c.kc) + at, rr < 0 ? 0 : 16);
+          cp_async16(dst + (kTile + i * kRows) * kRow, static_cast<const uint8_t*>(c.vc) + at, rr < 0 ? 0 : 16);
+        }
+        mask = __ballot_sync(0xffffffffu, row >= 0);
+        if (lane < kTile) {
+          const int rr = row < 0 ? 0 : row;
+          cp_async4(st + 2 * kTile * kRow + lane * 4, c.ks + rr, row < 0 ? 0 : 4);
+          cp_async4(st + 2 * kTile * kRow + kTile * 4 + lane * 4, c.vs + rr, row < 0 ? 0 : 4);
+        }
       }
       if (lane == 0) *reinterpret_cast<unsigned*>(ring + put * S::kStage + 2 * kTile * kRow + 2 * kTile * 4) = mask;
       put = put + 1 == kStages ? 0 : put + 1;
@@ -330,6 +349,18 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   look();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
+  if (!g.whole) {
+    // empty contexts, and contexts longer than their tables
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const int n = a.ctx_len[b];
+      if (a.err && threadIdx.x == 0 && n > g.cap) atomicCAS(a.err, 0, 1);
+      if (n <= 0) {
+        T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
+        for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
+          o[static_cast<long long>(i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
+      }
+    }
+  }
 
   // ---- portions of this warp, one (sequence, group) each
   int get = 0;
@@ -393,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
 
-    for (long long t = cur.t; t < cur.end; ++t) {
+    for (int t = cur.t; t < cur.end; ++t) {
       cp_wait<kStages - 2>();
       __syncwarp();
       const uint8_t* st = ring + get * S::kStage;
@@ -410,7 +441,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t a0 = f16x2_of(xs[j]), a1 = f16x2_of(ys[j]), a2 = f16x2_of(xs[j] >> 16), a3 = f16x2_of(ys[j] >> 16);
+          uint32_t a0, a1, a2, a3;
+          widen(xs[j], a0, a2);
+          widen(ys[j], a1, a3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const uint2 b = S::kQRegs ? qf[S::kQRegs ? (i * 4 + j) * NT + n : 0] : q_smem[((i * 4 + j) * NT + n) * 32 + lane];
@@ -421,41 +454,49 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       // weights of tokens gq and gq + 8 for heads 2 tq and 2 tq + 1
       const float k0 = scales[gq], k1 = scales[gq + 8], v0 = scales[kTile + gq], v1 = scales[kTile + gq + 8];
       const bool in0 = mask >> gq & 1, in1 = mask >> (gq + 8) & 1;
-      const int x0 = static_cast<int>(__float_as_uint(v0) >> 23 & 255) - 127;
-      const int x1 = static_cast<int>(__float_as_uint(v1) >> 23 & 255) - 127;
-      const float e0 = static_cast<float>(max(x0, kMinVsExp)), e1 = static_cast<float>(max(x1, kMinVsExp));
-      uint32_t wb[NT][2];
+      const float e0 = fmaxf(log2_fast(v0), kMinVsLog), e1 = fmaxf(log2_fast(v1), kMinVsLog);
       bool grew = false;
-      float cor[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[n][e] = s[n][e] * ch[n][e] * k0;
+          s[n][2 + e] = s[n][2 + e] * ch[n][e] * k1;
+          grew |= (in0 && s[n][e] + e0 > m[n][e] + kSlack) || (in1 && s[n][2 + e] + e1 > m[n][e] + kSlack);
+        }
+      if (__any_sync(0xffffffffu, grew)) {  // the maximum outran the reference: move it, and what was summed with it
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(in0 ? s[n][e] + e0 : -INFINITY, in1 ? s[n][2 + e] + e1 : -INFINITY);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[n][e]);
+            const float cor = top == -INFINITY ? 1.f : exp2_fast(m[n][e] - top);
+            m[n][e] = top;
+            l[n][e] *= cor;
+#pragma unroll
+            for (int i = 0; i < 2 * NW; ++i) {
+              acc[i][n][e] *= cor;
+              acc[i][n][2 + e] *= cor;
+            }
+          }
+      }
+      uint32_t wb[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float p[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float lo = s[n][e] * ch[n][e] * k0, hi = s[n][2 + e] * ch[n][e] * k1;
-          float top = fmaxf(in0 ? lo + e0 : -INFINITY, in1 ? hi + e1 : -INFINITY);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float mn = fmaxf(m[n][e], top), mr = mn == -INFINITY ? 0.f : mn;
-          cor[n][e] = exp2_fast(m[n][e] - mr);
-          grew |= mn != m[n][e];
-          m[n][e] = mn;
-          p[e] = in0 ? exp2_fast(lo - mr) : 0.f;
-          p[2 + e] = in1 ? exp2_fast(hi - mr) : 0.f;
+          const float mr = m[n][e] == -INFINITY ? 0.f : m[n][e];
+          p[e] = in0 ? exp2_fast(s[n][e] - mr) : 0.f;
+          p[2 + e] = in1 ? exp2_fast(s[n][2 + e] - mr) : 0.f;
+          l[n][e] += p[e] + p[2 + e];
         }
         wb[n][0] = transpose8x8(pack_f16(in0 ? p[0] * v0 : 0.f, in0 ? p[1] * v0 : 0.f));
         wb[n][1] = transpose8x8(pack_f16(in1 ? p[2] * v1 : 0.f, in1 ? p[3] * v1 : 0.f));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) l[n][e] = l[n][e] * cor[n][e] + (p[e] + p[2 + e]);
-      }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int i = 0; i < 2 * NW; ++i)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][n][e] *= cor[n][e & 1];
       }
       // O^T [16 dimensions, heads] += V^T w: bytes of neighbouring tokens are paired before they are widened
       const uint8_t* vr = st + kTile * kRow + 2 * tq * kRow;
@@ -475,8 +516,11 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
         for (int u = 0; u < U; ++u) {
           const uint32_t lo0 = __byte_perm(rw[0][u], rw[1][u], 0x5140), hi0 = __byte_perm(rw[0][u], rw[1][u], 0x7362);
           const uint32_t lo1 = __byte_perm(rw[2][u], rw[3][u], 0x5140), hi1 = __byte_perm(rw[2][u], rw[3][u], 0x7362);
-          const uint32_t a0 = f16x2_of(lo0), a1 = f16x2_of(lo0 >> 16), a2 = f16x2_of(lo1), a3 = f16x2_of(lo1 >> 16);
-          const uint32_t c0 = f16x2_of(hi0), c1 = f16x2_of(hi0 >> 16), c2 = f16x2_of(hi1), c3 = f16x2_of(hi1 >> 16);
+          uint32_t a0, a1, a2, a3, c0, c1, c2, c3;
+          widen(lo0, a0, a1);
+          widen(lo1, a2, a3);
+          widen(hi0, c0, c1);
+          widen(hi1, c2, c3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816(acc[2 * (kk + u)][n], a0, a1, a2, a3, wb[n][0], wb[n][1]);
@@ -491,9 +535,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 
     // ---- the end of the portion: a whole context is written out, a part kept for the CTA's merge
     const bool opens = cur.t == 0;
-    const int behind = static_cast<int>((cur.tokens + kTile - 1) / kTile - cur.end);
+    const int behind = tiles(cur.tokens) - cur.end;
     const bool closes = behind == 0;
-    const int b = cur.b, r = cur.r;
+    const int b = cur.b, r = cur.r, begun = cur.t;
     going = next_portion(a, g, cur);
     float* part = first_portion ? first_part : reinterpret_cast<float*>(ring);
     if (!first_portion && !(opens && closes)) {  // the list's last portion: the ring is done with
@@ -526,11 +570,12 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           *reinterpret_cast<float2*>(part + kHeads * D + 2 * h) = make_float2(m[n][e], v);
       }
     if (!(opens && closes) && lane == 0)
-      meta[2 * w + (first_portion ? 0 : 1)] = make_int4(b, r, (opens ? 1 : 0) | (closes ? 2 : 0), behind);
+      meta[2 * w + (first_portion ? 0 : 1)] = make_int4(b, r, (opens ? 1 : 0) | (closes ? 2 : 0) | begun << 2, behind);
     first_portion = false;
   }
   cp_wait<0>();
   __syncthreads();
+  tb::pdl_trigger();
 
   // ---- merge the parts of this CTA: runs of the same (sequence, group)
   bool first_run = true;
@@ -547,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       if (o.x >= 0) {
         if (o.x != at.x || o.y != at.y) break;
         set |= 1u << y;
-        bits |= o.z;
+        bits |= o.z & 3;
         behind = o.w;
       }
       ++y;
@@ -557,14 +602,19 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     const int h0 = at.y / g.NG * g.G + at.y % g.NG * kHeads;
     const int left = g.G - at.y % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
     const long long slot = 2ll * blockIdx.x + (first_run ? 0 : 1);
-    if (bits == 1 && threadIdx.x == 0) {
-      // the first part of a context that goes on: the others are in the CTAs up to the one with its last tile
+    if (!whole && threadIdx.x == 0) {
+      // a part of a context that other CTAs share: list position p belongs to worker ((p + 1) workers - 1) / total
       const long long all = static_cast<long long>(N) * kWarps;
-      const long long last_tile = (blockIdx.x + 1ll) * kWarps * total / all + behind - 1;
-      int* rec = P::record(a.ws, gridDim.x, blockIdx.x);
-      rec[0] = at.x * g.HG + at.y;
-      rec[1] = static_cast<int>(slot);
-      rec[2] = static_cast<int>(((last_tile + 1) * all - 1) / total / kWarps - blockIdx.x) + 1;
+      int4* rec = P::record(a.ws, gridDim.x, blockIdx.x);
+      if (bits & 1) {
+        const long long last_tile = (blockIdx.x + 1ll) * kWarps * total / all + behind - 1;
+        rec->x = at.x * g.HG + at.y;
+        rec->y = static_cast<int>(slot);
+        rec->z = static_cast<int>(((last_tile + 1) * all - 1) / total / kWarps - blockIdx.x) + 1;
+      } else {
+        const long long first_tile = blockIdx.x * static_cast<long long>(kWarps) * total / all - (at.z >> 2);
+        rec->w = static_cast<int>(((first_tile + 1) * all - 1) / total / kWarps);
+      }
     }
     for (int i = threadIdx.x; i < nh * (D / 4); i += kThreads) {
       const int h = i / (D / 4), d = i % (D / 4) * 4;
@@ -604,55 +654,108 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   }
 }
 
-// Joins the parts of the contexts that were split: one CTA per first part and
-// query head, a warp every eighth part.
+// Joins the contexts that were split over CTAs.  Up to kFewParts parts: the CTA
+// of the first part joins them, a warp for each query head.  More: CTA i of
+// those that share the context joins query head i, each warp every eighth part.
+constexpr int kFewParts = 16, kJoinWarps = 8;
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) decode_attn_quant_join_kernel(TbDecodeAttnQuantArgs a, Geometry g, int grid) {
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    decode_attn_quant_join_kernel(TbDecodeAttnQuantArgs a, Geometry g, int grid, bool out4) {
   using P = Partials<D, NT>;
-  constexpr int kW = 8, E = D / 32;
-  __shared__ float red[kW], sl[kW], so[kW][D];
+  static_assert(P::kHeads <= kFewParts + 1, "a CTA for each head of a context with many parts");
+  constexpr int E = D / 32, V = E < 4 ? E : 4;
+  __shared__ float red[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
   tb::pdl_wait();
-  const int* rec = P::record(a.ws, grid, blockIdx.x);
-  const int n = rec[2];
-  if (n == 0) return;
-  const int h = blockIdx.y, seg = rec[0], r = seg % g.HG, b = seg / g.HG;
-  const int h0 = r % g.NG * P::kHeads;
-  if (h0 + h >= g.G) return;
+  const int4 mine = *P::record(a.ws, grid, blockIdx.x);
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long long own = rec[1], next = 2ll * blockIdx.x;
-  auto slot = [&](int p) { return p == 0 ? own : next + 2ll * p; };
-  float M = -INFINITY;
-  for (int p = threadIdx.x; p < n; p += blockDim.x) M = fmaxf(M, P::stat(a.ws, slot(p), h)[0]);
-  M = tb::warp_max(M);
-  if (lane == 0) red[w] = M;
-  __syncthreads();
+  auto add = [&](float (&o)[E], float f, const float* v) {
 #pragma unroll
-  for (int i = 0; i < kW; ++i) M = fmaxf(M, red[i]);
-  if (M == -INFINITY) M = 0.f;
-  float L = 0.f, o[E] = {};
-#pragma unroll 4
-  for (int p = w; p < n; p += kW) {
-    const float* st = P::stat(a.ws, slot(p), h);
-    const float* v = P::out(a.ws, slot(p), h);
-    const float f = exp2_fast(st[0] - M);
-    L += f * st[1];
+    for (int i = 0; i < E; i += V) {
+      float x[V];
+      tb::load_vec<float, V>(v + lane * E + i, x);
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] += f * v[i * 32 + lane];
-  }
-  if (lane == 0) sl[w] = L;
-#pragma unroll
-  for (int i = 0; i < E; ++i) so[w][i * 32 + lane] = o[i];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float l = 0.f, v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kW; ++i) {
-      l += sl[i];
-      v += so[i][threadIdx.x];
+      for (int e = 0; e < V; ++e) o[i + e] += f * x[e];
     }
-    T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b +
-             static_cast<long long>(r / g.NG * g.G + h0 + h) * a.os_h;
-    out[threadIdx.x] = tb::from_f32<T>(l == 0.f ? 0.f : v / l);
+  };
+  auto write = [&](int seg, int h, float L, const float (&o)[E]) {
+    const int r = seg % g.HG, head = r / g.NG * g.G + r % g.NG * P::kHeads + h;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* p = static_cast<T*>(a.out) + static_cast<long long>(seg / g.HG) * a.os_b + static_cast<long long>(head) * a.os_h +
+           lane * E;
+#pragma unroll
+    for (int i = 0; i < E; i += V) {
+      float x[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = o[i + e] * inv;
+      if (out4) {
+        tb::store_vec<T, V>(p + i, x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[i + e] = tb::from_f32<T>(x[e]);
+      }
+    }
+  };
+  auto heads_of = [&](int seg) {
+    const int left = g.G - seg % g.HG % g.NG * P::kHeads;
+    return left < P::kHeads ? left : P::kHeads;
+  };
+  if (mine.z > 0 && mine.z <= kFewParts) {
+    const int nh = heads_of(mine.x);
+    for (int h = w; h < nh; h += kJoinWarps) {
+      const long long slot = lane == 0 ? mine.y : 2ll * (blockIdx.x + lane);
+      const float* st = P::stat(a.ws, slot, h);
+      const float m = lane < mine.z ? st[0] : -INFINITY;
+      const float M = tb::warp_max(m);
+      const float f = lane < mine.z ? exp2_fast(m - (M == -INFINITY ? 0.f : M)) : 0.f;
+      const float L = tb::warp_sum(lane < mine.z ? f * st[1] : 0.f);
+      float o[E] = {};
+#pragma unroll 4
+      for (int p = 0; p < mine.z; ++p)
+        add(o, __shfl_sync(0xffffffffu, f, p), P::out(a.ws, p == 0 ? mine.y : 2ll * (blockIdx.x + p), h));
+      write(mine.x, h, L, o);
+    }
+  }
+#pragma unroll 1
+  for (int role = 0; role < 2; ++role) {  // the first of a long run; one of the others
+    const int lead = role == 0 ? static_cast<int>(blockIdx.x) : mine.w;
+    if (lead < 0) continue;
+    const int4 rec = role == 0 ? mine : *P::record(a.ws, grid, lead);
+    const int h = blockIdx.x - lead;
+    if (rec.z <= kFewParts || h >= heads_of(rec.x)) continue;  // the same for the whole CTA
+    auto slot = [&](int p) { return p == 0 ? static_cast<long long>(rec.y) : 2ll * (lead + p); };
+    float M = -INFINITY;
+    for (int p = threadIdx.x; p < rec.z; p += kJoinWarps * 32) M = fmaxf(M, P::stat(a.ws, slot(p), h)[0]);
+    M = tb::warp_max(M);
+    __syncthreads();
+    if (lane == 0) red[w] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) M = fmaxf(M, red[i]);
+    if (M == -INFINITY) M = 0.f;
+    float L = 0.f, o[E] = {};
+#pragma unroll 8
+    for (int p = w; p < rec.z; p += kJoinWarps) {
+      const float2 st = *reinterpret_cast<const float2*>(P::stat(a.ws, slot(p), h));
+      const float f = exp2_fast(st.x - M);
+      L += f * st.y;
+      add(o, f, P::out(a.ws, slot(p), h));
+    }
+    if (lane == 0) sl[w] = L;
+#pragma unroll
+    for (int i = 0; i < E; ++i) so[w][lane * E + i] = o[i];
+    __syncthreads();
+    if (w == 0) {
+      L = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] = 0.f;
+      for (int x = 0; x < kJoinWarps; ++x) {
+        L += sl[x];
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] += so[x][lane * E + i];
+      }
+      write(rec.x, h, L, o);
+    }
   }
 }
 
@@ -669,7 +772,11 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a) {
   g.G = a.Hq / a.cache.Hk;
   g.NG = (g.G + 8 * NT - 1) / (8 * NT);
   g.HG = a.cache.Hk * g.NG;
-  g.cap = static_cast<long long>(a.cache.max_blocks) * a.cache.bs;
+  g.cap = a.cache.max_blocks * a.cache.bs;
+  g.shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a.cache.bs == 1 << i) g.shift = i;
+  g.tile_pages = a.cache.bs % kTile == 0;
   g.whole = g.cap <= kWholeTokens;
   return g;
 }
@@ -692,8 +799,17 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, q8, out4);
   const cudaError_t e1 = cudaGetLastError();
   if (e1 != cudaSuccess) return static_cast<int>(e1);
-  decode_attn_quant_join_kernel<T, D, NT><<<dim3(grid, 8 * NT), 256, 0, s>>>(a, g, grid);
-  return static_cast<int>(cudaGetLastError());
+  // programmatic launch: the joining CTAs are in place when the last list ends
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_attn_quant_join_kernel<T, D, NT>, a, g, grid, out4));
 }
 
 // 16 columns where more than 8 query heads share a KV head, else 8.
@@ -727,7 +843,8 @@ extern "C" size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int 
 extern "C" int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s) {
   const TbDecodeAttnQuantArgs& a = *args;
   if (a.B <= 0 || a.Hq <= 0) return 0;
-  if (a.cache.Hk <= 0 || a.Hq % a.cache.Hk || a.cache.bs <= 0 || a.cache.num_seqs != a.B)
+  if (a.cache.Hk <= 0 || a.Hq % a.cache.Hk || a.cache.bs <= 0 || a.cache.num_seqs != a.B ||
+      a.cache.max_blocks < 0 || a.cache.max_blocks > 0x7fffffff / a.cache.bs)
     return static_cast<int>(cudaErrorInvalidValue);
   if (a.dtype == TB_BF16) return launch_type<__nv_bfloat16>(a, s);
   if (a.dtype == TB_F16) return launch_type<__half>(a, s);
