@@ -42,6 +42,9 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;       // tokens per tile
 constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that many
+constexpr int kWaveTiles = 64;  // tiles per CTA where there are more CTAs than fit at once
+constexpr int kMostWaves = 4;
+constexpr int kStart = 1;       // what beginning a (sequence, group) costs a warp, in tiles
 constexpr int kWholeTokens = 256;  // contexts that cannot be longer are not split
 constexpr float kMinVsLog = -100.f;
 constexpr float kSlack = 8.f;   // the reference of the weights may lag behind their maximum by a factor of 2^8
@@ -106,7 +109,7 @@ struct Smem {
   static constexpr bool kQRegs = D * NT <= 256;  // q fragments in registers, else per warp in shared memory
   static constexpr int kQ = kQRegs ? 0 : (D / 16) * NT * 32 * 8;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kScan = (2 * kWarps + 2 * kWarps) * 8;
+  static constexpr int kScan = (3 * kWarps + 4) * 8;
   static constexpr int kBytes = kWarps * (kRing + kPart + kQ) + kScan + 2 * kWarps * 16;
   static_assert(kRing >= kPart && kRing % 16 == 0 && kPart % 16 == 0, "a part fits a ring");
 };
@@ -141,6 +144,7 @@ struct Geometry {
   int shift;       // log2 of the page size, or -1
   int tile_pages;  // pages hold whole tiles
   int whole;       // one CTA per (sequence, group), nothing to join
+  int fit;         // CTAs that fit at once
 };
 
 __device__ __forceinline__ int tokens_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
@@ -148,13 +152,29 @@ __device__ __forceinline__ int tokens_of(const TbDecodeAttnQuantArgs& a, const G
   return n < 0 ? 0 : n < g.cap ? n : g.cap;
 }
 
+__device__ __forceinline__ int tiles(int tokens) { return tokens / kTile + (tokens % kTile != 0); }
+
+// The list is counted in units: kStart for beginning a (sequence, group), then
+// its tiles.  Of n workers the first `more` take each + 1 units, the others each.
+__device__ __forceinline__ int units(int tokens) { return tokens > 0 ? tiles(tokens) + kStart : 0; }
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+struct Shares {
+  long long each, more;
+  __device__ __forceinline__ long long start(long long i) const { return i * each + (i < more ? i : more); }
+  __device__ __forceinline__ long long owner(long long unit) const {
+    const long long head = more * (each + 1);
+    return unit < head ? divide(unit, each + 1) : more + divide(unit - head, each);
+  }
+};
+
 // Where a warp (or its prefetch) stands in its list of tiles: in sequence b,
-// group r, at tile t of the portion [.., end), with `rest` tiles behind it.
+// group r, at tile t of the portion [.., end), with `rest` units behind it.
 struct Cursor {
   int b, r, tokens, t, end;
   long long rest;
 };
-__device__ __forceinline__ int tiles(int tokens) { return tokens / kTile + (tokens % kTile != 0); }
 
 // Moves on to the next portion; false at the end of the list.
 __device__ __forceinline__ bool next_portion(const TbDecodeAttnQuantArgs& a, const Geometry& g, Cursor& c) {
@@ -166,11 +186,11 @@ __device__ __forceinline__ bool next_portion(const TbDecodeAttnQuantArgs& a, con
       c.tokens = tokens_of(a, g, c.b);
     } while (c.tokens == 0);
   }
-  const int n = tiles(c.tokens);
+  const int n = units(c.tokens), take = n < c.rest ? n : static_cast<int>(c.rest);
   c.t = 0;
-  c.end = n < c.rest ? n : static_cast<int>(c.rest);
-  c.rest -= c.end;
-  return true;
+  c.end = take - kStart;
+  c.rest -= take;
+  return c.end > 0;  // (nothing is behind a portion without a tile)
 }
 
 template <typename T>
@@ -201,12 +221,23 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   float* first_part = reinterpret_cast<float*>(smem + kWarps * S::kRing + w * S::kPart);
   uint2* q_smem = reinterpret_cast<uint2*>(smem + kWarps * (S::kRing + S::kPart) + w * S::kQ);
   long long* scan = reinterpret_cast<long long*>(smem + kWarps * (S::kRing + S::kPart + S::kQ));
-  int4* meta = reinterpret_cast<int4*>(scan + 4 * kWarps);  // of the 2 kWarps parts: (sequence, group, opens | closes << 1 | first tile << 2, tiles behind it)
+  int* shared = reinterpret_cast<int*>(scan + 3 * kWarps + 2);  // first CTA of the list's first context, last one of its last
+  int4* meta = reinterpret_cast<int4*>(scan + 3 * kWarps + 4);  // of the 2 kWarps parts: (sequence, group, opens | closes << 1, -)
 
   // ---- this warp's list of tiles
   Cursor cur;
-  long long total = 0;
-  int N = gridDim.x;
+  int ctas = 0;  // that have a list
+  // zeros for empty contexts, and word of contexts longer than their tables, each by one of n CTAs
+  auto empty_rows = [&](int n) {
+    for (int b = blockIdx.x; b < a.B; b += n) {
+      const int ctx = a.ctx_len[b];
+      if (a.err && threadIdx.x == 0 && ctx > g.cap) atomicCAS(a.err, 0, 1);
+      if (ctx > 0) continue;
+      T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
+      for (int i = threadIdx.x; i < a.Hq * (D / 4); i += kThreads)
+        store_out4<T>(o + static_cast<long long>(i / (D / 4)) * a.os_h + i % (D / 4) * 4, out4, 0.f, 0.f, 0.f, 0.f);
+    }
+  };
   if (g.whole) {
     cur.b = blockIdx.x / g.HG;
     cur.r = blockIdx.x % g.HG;
@@ -224,12 +255,12 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     cur.end = n * (w + 1) / kWarps;
     cur.rest = 0;
   } else {
-    // prefix sums of the sequences' tiles: each thread a run of sequences
+    // prefix sums of the sequences' units: each thread a run of sequences
     const int per = (a.B + kThreads - 1) / kThreads, b0 = threadIdx.x * per;
     const int b1 = b0 + per < a.B ? b0 + per : a.B;
     long long mine = 0;
 #pragma unroll 4
-    for (int b = b0; b < b1; ++b) mine += tiles(tokens_of(a, g, b));
+    for (int b = b0; b < b1; ++b) mine += units(tokens_of(a, g, b));
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -237,8 +268,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       if (lane >= o) inc += y;
     }
     if (lane == 31) scan[w] = inc;
+    if (threadIdx.x == 0) *P::record(a.ws, gridDim.x, blockIdx.x) = make_int4(0, 0, 0, -1);
     __syncthreads();
-    long long before = inc - mine;
+    long long before = inc - mine, total = 0;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       if (i < w) before += scan[i];
@@ -247,36 +279,55 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     total *= g.HG;
     before *= g.HG;
     mine *= g.HG;
-    const long long want = (total + kMinTiles - 1) / kMinTiles;
-    if (want < N) N = static_cast<int>(want);
-    if (threadIdx.x == 0) *P::record(a.ws, gridDim.x, blockIdx.x) = make_int4(0, 0, 0, -1);
-    if (static_cast<int>(blockIdx.x) >= N) return;
+    // as many CTAs as fit at once, unless that leaves them less than kMinTiles, or more than kWaveTiles
+    long long N = g.fit;
+    if (total < N * kMinTiles) N = (total + kMinTiles - 1) / kMinTiles;
+    if (total > N * kWaveTiles) N = total / kWaveTiles;
+    if (N > gridDim.x) N = gridDim.x;
+    if (N == 0) empty_rows(gridDim.x);
+    if (blockIdx.x >= N) return;
+    ctas = static_cast<int>(N);
+    Shares sh;
+    sh.each = divide(total, N * kWarps);
+    sh.more = total - sh.each * (N * kWarps);
+    const long long me = static_cast<long long>(blockIdx.x) * kWarps;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const long long f = (static_cast<long long>(blockIdx.x) * kWarps + i) * total / (static_cast<long long>(N) * kWarps);
+    for (int i = 0; i <= kWarps; ++i) {  // where the warps' lists start, and the last unit of this CTA
+      const long long at_unit = sh.start(me + i) - (i == kWarps ? 1 : 0);
+      const long long f = at_unit < total ? at_unit : total - 1;  // (a worker without units starts behind the last one)
       if (f >= before && f < before + mine) {
         int b = b0;
-        long long at = before, n = static_cast<long long>(tiles(tokens_of(a, g, b))) * g.HG;
+        long long at = before, n = static_cast<long long>(units(tokens_of(a, g, b))) * g.HG;
         while (f >= at + n) {
           at += n;
-          n = static_cast<long long>(tiles(tokens_of(a, g, ++b))) * g.HG;
+          n = static_cast<long long>(units(tokens_of(a, g, ++b))) * g.HG;
         }
-        scan[2 * kWarps + 2 * i] = b;
-        scan[2 * kWarps + 2 * i + 1] = f - at;
+        scan[kWarps + 2 * i] = b;
+        scan[kWarps + 2 * i + 1] = f - at;
       }
     }
     __syncthreads();
-    const long long me = static_cast<long long>(blockIdx.x) * kWarps + w, all = static_cast<long long>(N) * kWarps;
-    const long long first = me * total / all, last = (me + 1) * total / all;
-    cur.b = static_cast<int>(scan[2 * kWarps + 2 * w]);
-    const long long off = scan[2 * kWarps + 2 * w + 1];
+    const long long first = sh.start(me + w);
+    cur.b = static_cast<int>(scan[kWarps + 2 * w]);
+    const long long off = scan[kWarps + 2 * w + 1];
     cur.tokens = tokens_of(a, g, cur.b);
-    const int n = tiles(cur.tokens);
-    cur.r = static_cast<int>(off / n);
-    cur.t = static_cast<int>(off - static_cast<long long>(cur.r) * n);
-    cur.rest = last - first;
-    cur.end = n - cur.t < cur.rest ? n : cur.t + static_cast<int>(cur.rest);
-    cur.rest -= cur.end - cur.t;
+    const int n = units(cur.tokens);
+    cur.r = static_cast<int>(divide(off, n));
+    const int at = static_cast<int>(off - static_cast<long long>(cur.r) * n);
+    cur.t = at > kStart ? at - kStart : 0;
+    cur.rest = sh.start(me + w + 1) - first;
+    const int take = n - at < cur.rest ? n - at : static_cast<int>(cur.rest);
+    cur.end = at + take - kStart;
+    cur.rest -= take;
+    // which CTAs share the contexts at the two ends of this CTA's list (used by the merge, if they are split)
+    if (threadIdx.x == 0) {
+      shared[0] = static_cast<int>(sh.owner(first - cur.t) / kWarps);
+    } else if (threadIdx.x == kThreads - 1) {
+      const long long e = scan[kWarps + 2 * kWarps + 1];
+      const int ne = units(tokens_of(a, g, static_cast<int>(scan[kWarps + 2 * kWarps])));
+      const long long behind = ne - 1 - (e - divide(e, ne) * ne);
+      shared[1] = static_cast<int>(sh.owner(sh.start(me + kWarps) - 1 + behind) / kWarps);
+    }
   }
   if (lane == 0) meta[2 * w] = meta[2 * w + 1] = make_int4(-1, 0, 0, 0);
 
@@ -349,18 +400,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   look();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
-  if (!g.whole) {
-    // empty contexts, and contexts longer than their tables
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-      const int n = a.ctx_len[b];
-      if (a.err && threadIdx.x == 0 && n > g.cap) atomicCAS(a.err, 0, 1);
-      if (n <= 0) {
-        T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
-        for (int i = threadIdx.x; i < a.Hq * D; i += kThreads)
-          o[static_cast<long long>(i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
-      }
-    }
-  }
+  if (!g.whole) empty_rows(ctas);
 
   // ---- portions of this warp, one (sequence, group) each
   int get = 0;
@@ -535,9 +575,8 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 
     // ---- the end of the portion: a whole context is written out, a part kept for the CTA's merge
     const bool opens = cur.t == 0;
-    const int behind = tiles(cur.tokens) - cur.end;
-    const bool closes = behind == 0;
-    const int b = cur.b, r = cur.r, begun = cur.t;
+    const bool closes = cur.end == tiles(cur.tokens);
+    const int b = cur.b, r = cur.r;
     going = next_portion(a, g, cur);
     float* part = first_portion ? first_part : reinterpret_cast<float*>(ring);
     if (!first_portion && !(opens && closes)) {  // the list's last portion: the ring is done with
@@ -570,87 +609,95 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           *reinterpret_cast<float2*>(part + kHeads * D + 2 * h) = make_float2(m[n][e], v);
       }
     if (!(opens && closes) && lane == 0)
-      meta[2 * w + (first_portion ? 0 : 1)] = make_int4(b, r, (opens ? 1 : 0) | (closes ? 2 : 0) | begun << 2, behind);
+      meta[2 * w + (first_portion ? 0 : 1)] = make_int4(b, r, (opens ? 1 : 0) | (closes ? 2 : 0), 0);
     first_portion = false;
   }
   cp_wait<0>();
   __syncthreads();
   tb::pdl_trigger();
 
-  // ---- merge the parts of this CTA: runs of the same (sequence, group)
+  // ---- merge the parts of this CTA: runs of the same (sequence, group), a warp for each query head
+  constexpr int E = D / 32, V = E < 4 ? E : 4;
   bool first_run = true;
+#pragma unroll 1
   for (int x = 0; x < 2 * kWarps;) {
     const int4 at = meta[x];
     if (at.x < 0) {
       ++x;
       continue;
     }
-    int y = x, bits = 0, behind = 0;  // behind: tiles of the context after the run
+    int bits = 0;
     unsigned set = 0;
-    while (y < 2 * kWarps) {
-      const int4 o = meta[y];
-      if (o.x >= 0) {
-        if (o.x != at.x || o.y != at.y) break;
-        set |= 1u << y;
-        bits |= o.z & 3;
-        behind = o.w;
-      }
-      ++y;
+    for (; x < 2 * kWarps; ++x) {
+      const int4 o = meta[x];
+      if (o.x < 0) continue;
+      if (o.x != at.x || o.y != at.y) break;
+      set |= 1u << x;
+      bits |= o.z & 3;
     }
-    x = y;
     const bool whole = bits == 3;
     const int h0 = at.y / g.NG * g.G + at.y % g.NG * kHeads;
     const int left = g.G - at.y % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
     const long long slot = 2ll * blockIdx.x + (first_run ? 0 : 1);
-    if (!whole && threadIdx.x == 0) {
-      // a part of a context that other CTAs share: list position p belongs to worker ((p + 1) workers - 1) / total
-      const long long all = static_cast<long long>(N) * kWarps;
+    first_run = false;
+    if (!whole && threadIdx.x == 0) {  // a part of a context that other CTAs share
       int4* rec = P::record(a.ws, gridDim.x, blockIdx.x);
       if (bits & 1) {
-        const long long last_tile = (blockIdx.x + 1ll) * kWarps * total / all + behind - 1;
         rec->x = at.x * g.HG + at.y;
         rec->y = static_cast<int>(slot);
-        rec->z = static_cast<int>(((last_tile + 1) * all - 1) / total / kWarps - blockIdx.x) + 1;
+        rec->z = shared[1] - static_cast<int>(blockIdx.x) + 1;
       } else {
-        const long long first_tile = blockIdx.x * static_cast<long long>(kWarps) * total / all - (at.z >> 2);
-        rec->w = static_cast<int>(((first_tile + 1) * all - 1) / total / kWarps);
+        rec->w = shared[0];
       }
     }
-    for (int i = threadIdx.x; i < nh * (D / 4); i += kThreads) {
-      const int h = i / (D / 4), d = i % (D / 4) * 4;
-      auto part_of = [&](int p) {
-        return p % 2 ? reinterpret_cast<const float*>(smem + p / 2 * S::kRing)
-                     : reinterpret_cast<const float*>(smem + kWarps * S::kRing + p / 2 * S::kPart);
-      };
-      float M = -INFINITY;
-      for (unsigned r = set; r; r &= r - 1) M = fmaxf(M, part_of(__ffs(r) - 1)[kHeads * D + 2 * h]);
-      const float mr = M == -INFINITY ? 0.f : M;
-      float L = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+    auto part_of = [&](int p) {
+      return reinterpret_cast<const float*>(p % 2 ? smem + p / 2 * S::kRing : smem + kWarps * S::kRing + p / 2 * S::kPart);
+    };
+#pragma unroll 1
+    for (int h = w; h < nh; h += kWarps) {
+      float2 st = make_float2(-INFINITY, 0.f);
+      if (lane < 2 * kWarps && set >> lane & 1) st = *reinterpret_cast<const float2*>(part_of(lane) + kHeads * D + 2 * h);
+      float M = st.x;
+#pragma unroll
+      for (int o = 1; o < 2 * kWarps; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      M = __shfl_sync(0xffffffffu, M, 0);
+      const float f = st.x == -INFINITY ? 0.f : exp2_fast(st.x - M);
+      float L = f * st.y;
+#pragma unroll
+      for (int o = 1; o < 2 * kWarps; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      L = __shfl_sync(0xffffffffu, L, 0);
+      const float inv = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
+      float o[E] = {};
       for (unsigned r = set; r; r &= r - 1) {
-        const float* p = part_of(__ffs(r) - 1);
-        const float2 st = *reinterpret_cast<const float2*>(p + kHeads * D + 2 * h);
-        const float f = exp2_fast(st.x - mr);
-        const float4 v = *reinterpret_cast<const float4*>(p + h * D + d);
-        L += f * st.y;
-        o0 += f * v.x;
-        o1 += f * v.y;
-        o2 += f * v.z;
-        o3 += f * v.w;
-      }
-      if (whole) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        store_out4<T>(static_cast<T*>(a.out) + static_cast<long long>(at.x) * a.os_b +
-                          static_cast<long long>(h0 + h) * a.os_h + d,
-                      out4, o0 * inv, o1 * inv, o2 * inv, o3 * inv);
-      } else {
-        *reinterpret_cast<float4*>(P::out(a.ws, slot, h) + d) = make_float4(o0, o1, o2, o3);
-        if (d == 0) {
-          P::stat(a.ws, slot, h)[0] = M;
-          P::stat(a.ws, slot, h)[1] = L;
+        const int p = __ffs(r) - 1;
+        const float fp = __shfl_sync(0xffffffffu, f, p);
+        const float* v = part_of(p) + h * D + lane * V;
+#pragma unroll
+        for (int i = 0; i < E; i += V) {
+          float y[V];
+          tb::load_vec<float, V>(v + i * 32, y);
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[i + e] += fp * y[e];
         }
       }
+      T* out = static_cast<T*>(a.out) + static_cast<long long>(at.x) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
+      float* part = P::out(a.ws, slot, h);
+#pragma unroll
+      for (int i = 0; i < E; i += V) {
+        float y[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = o[i + e] * inv;
+        if (!whole) {
+          tb::store_vec<float, V>(part + i * 32 + lane * V, y);
+        } else if (out4) {
+          tb::store_vec<T, V>(out + i * 32 + lane * V, y);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) out[i * 32 + lane * V + e] = tb::from_f32<T>(y[e]);
+        }
+      }
+      if (!whole && lane == 0) *reinterpret_cast<float2*>(P::stat(a.ws, slot, h)) = make_float2(M, L);
     }
-    first_run = false;
   }
 }
 
@@ -673,7 +720,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 #pragma unroll
     for (int i = 0; i < E; i += V) {
       float x[V];
-      tb::load_vec<float, V>(v + lane * E + i, x);
+      tb::load_vec<float, V>(v + i * 32 + lane * V, x);
 #pragma unroll
       for (int e = 0; e < V; ++e) o[i + e] += f * x[e];
     }
@@ -682,17 +729,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const int r = seg % g.HG, head = r / g.NG * g.G + r % g.NG * P::kHeads + h;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     T* p = static_cast<T*>(a.out) + static_cast<long long>(seg / g.HG) * a.os_b + static_cast<long long>(head) * a.os_h +
-           lane * E;
+           lane * V;
 #pragma unroll
     for (int i = 0; i < E; i += V) {
       float x[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) x[e] = o[i + e] * inv;
       if (out4) {
-        tb::store_vec<T, V>(p + i, x);
+        tb::store_vec<T, V>(p + i * 32, x);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) p[i + e] = tb::from_f32<T>(x[e]);
+        for (int e = 0; e < V; ++e) p[i * 32 + e] = tb::from_f32<T>(x[e]);
       }
     }
   };
@@ -767,8 +814,9 @@ int sm_count() {
 }
 
 template <int D, int NT>
-Geometry geometry(const TbDecodeAttnQuantArgs& a) {
+Geometry geometry(const TbDecodeAttnQuantArgs& a, int sms) {
   Geometry g;
+  g.fit = sms * resident<D, NT>();
   g.G = a.Hq / a.cache.Hk;
   g.NG = (g.G + 8 * NT - 1) / (8 * NT);
   g.HG = a.cache.Hk * g.NG;
@@ -781,10 +829,20 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a) {
   return g;
 }
 
+// CTAs to launch for contexts of at most `cap` tokens: those that fit at once,
+// more (up to kMostWaves times) where each could still take kWaveTiles.
+template <int D, int NT>
+int grid_of(int B, int Hq, int Hk, int cap) {
+  const int fit = sm_count() * resident<D, NT>(), G = Hq / Hk;
+  const long long most = static_cast<long long>(B) * Hk * ((G + 8 * NT - 1) / (8 * NT)) * (cap / kTile + 1 + kStart);
+  const long long n = most / kWaveTiles;
+  return n <= fit ? fit : n < kMostWaves * fit ? static_cast<int>(n) : kMostWaves * fit;
+}
+
 template <typename T, int D, int NT>
 int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   using S = Smem<D, NT>;
-  const Geometry g = geometry<D, NT>(a);
+  const Geometry g = geometry<D, NT>(a, sm_count());
   auto kernel = decode_attn_quant_kernel<T, D, NT>;
   const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -794,7 +852,7 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
     kernel<<<a.B * g.HG, kThreads, S::kBytes, s>>>(a, g, q8, out4);
     return static_cast<int>(cudaGetLastError());
   }
-  const int grid = sm_count() * resident<D, NT>();
+  const int grid = grid_of<D, NT>(a.B, a.Hq, a.cache.Hk, g.cap);
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
   kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, q8, out4);
   const cudaError_t e1 = cudaGetLastError();
@@ -829,13 +887,16 @@ int launch_type(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
 extern "C" size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens) {
   if (B <= 0 || Hk <= 0 || max_tokens <= kWholeTokens) return 0;
   const bool two = Hq / Hk > 8;
-  const int n = sm_count();
   switch (D) {
-    case 64: return two ? Partials<64, 2>::bytes(n * resident<64, 2>()) : Partials<64, 1>::bytes(n * resident<64, 1>());
+    case 64:
+      return two ? Partials<64, 2>::bytes(grid_of<64, 2>(B, Hq, Hk, max_tokens))
+                 : Partials<64, 1>::bytes(grid_of<64, 1>(B, Hq, Hk, max_tokens));
     case 128:
-      return two ? Partials<128, 2>::bytes(n * resident<128, 2>()) : Partials<128, 1>::bytes(n * resident<128, 1>());
+      return two ? Partials<128, 2>::bytes(grid_of<128, 2>(B, Hq, Hk, max_tokens))
+                 : Partials<128, 1>::bytes(grid_of<128, 1>(B, Hq, Hk, max_tokens));
     case 256:
-      return two ? Partials<256, 2>::bytes(n * resident<256, 2>()) : Partials<256, 1>::bytes(n * resident<256, 1>());
+      return two ? Partials<256, 2>::bytes(grid_of<256, 2>(B, Hq, Hk, max_tokens))
+                 : Partials<256, 1>::bytes(grid_of<256, 1>(B, Hq, Hk, max_tokens));
   }
   return 0;
 }

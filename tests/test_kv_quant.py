@@ -242,6 +242,20 @@ LENS = [[1], [33], [0, 1, 2, 15], [16, 17, 31, 0, 32, 129], [500, 3, 0, 257], [2
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cap", [0, 64, 4096])
+def test_attention_all_empty(cap, device):
+    """Nothing but empty contexts, in tables without a column, short and long: zeros over what out held."""
+    c = quant_kv_cache(3, 2, 16, 128, device)
+    q = torch.randn(700, 6, 128, device=device).bfloat16()
+    out = torch.full_like(q, float("nan"))
+    table = torch.zeros(700, cap // 16, dtype=torch.int32, device=device)
+    ctx = torch.zeros(700, dtype=torch.int32, device=device)
+    ctx[5] = -3
+    decode_attention_quant(q, *c, table, ctx, out=out)
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("Hq,Hk,D,bs", [(12, 2, 128, 16), (32, 8, 128, 16), (4, 4, 64, 1), (8, 1, 256, 64),
                                         (9, 3, 128, 7), (16, 1, 64, 24), (20, 1, 128, 16), (34, 2, 256, 16),
@@ -253,7 +267,8 @@ def test_attention(Hq, Hk, D, bs, dtype, device):
         c = random_cache(nb, Hk, bs, D, device, g)
         q = (torch.randn(len(lens), Hq, D, generator=g) * 2).to(dtype).to(device)
         ctx = torch.tensor(lens, dtype=torch.int32, device=device)
-        out = decode_attention_quant(q, *c, table, ctx)
+        out = torch.full_like(q, float("nan"))
+        assert decode_attention_quant(q, *c, table, ctx, out=out) is out
         check_attention(out, q, c, table, lens, D ** -0.5)
 
 
@@ -441,11 +456,11 @@ def test_attention_split_and_joined(lens, Hq, Hk, D, bs, dev):
     c = random_cache(nb, Hk, bs, D, dev, g)
     q = torch.randn(len(lens), Hq, D, generator=g).bfloat16().to(dev)
     ctx = torch.tensor(lens, dtype=torch.int32, device=dev)
-    out = decode_attention_quant(q, *c, table, ctx)
+    out = decode_attention_quant(q, *c, table, ctx, out=torch.full_like(q, float("nan")))
     some = list(range(0, len(lens), max(1, len(lens) // 12)))
     check_attention(out[some], q[some], c, table[some], [lens[i] for i in some], D ** -0.5)
     for _ in range(3):  # the joins have a fixed order
-        assert torch.equal(decode_attention_quant(q, *c, table, ctx), out)
+        assert torch.equal(decode_attention_quant(q, *c, table, ctx, out=torch.full_like(q, float("nan"))), out)
 
 
 @pytest.mark.gpu
