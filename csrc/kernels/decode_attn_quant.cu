@@ -43,7 +43,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;       // tokens per tile
 constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that many
 constexpr int kWaveTiles = 64;  // tiles per CTA where there are more CTAs than fit at once
-constexpr int kMostWaves = 4;
+constexpr int kMostWaves = 1;
 constexpr int kStart = 1;       // what beginning a (sequence, group) costs a warp, in tiles
 constexpr int kWholeTokens = 256;  // contexts that cannot be longer are not split
 constexpr float kMinVsLog = -100.f;
@@ -109,8 +109,8 @@ struct Smem {
   static constexpr bool kQRegs = D * NT <= 256;  // q fragments in registers, else per warp in shared memory
   static constexpr int kQ = kQRegs ? 0 : (D / 16) * NT * 32 * 8;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kScan = (3 * kWarps + 4) * 8;
-  static constexpr int kBytes = kWarps * (kRing + kPart + kQ) + kScan + 2 * kWarps * 16;
+  static constexpr int kScan = (kThreads + kWarps + 2) * 4 + 2 * kWarps * 8;
+  static constexpr int kBytes = kWarps * (kRing + kPart + kQ) + kScan;
   static_assert(kRing >= kPart && kRing % 16 == 0 && kPart % 16 == 0, "a part fits a ring");
 };
 
@@ -157,23 +157,19 @@ __device__ __forceinline__ int tiles(int tokens) { return tokens / kTile + (toke
 // The list is counted in units: kStart for beginning a (sequence, group), then
 // its tiles.  Of n workers the first `more` take each + 1 units, the others each.
 __device__ __forceinline__ int units(int tokens) { return tokens > 0 ? tiles(tokens) + kStart : 0; }
-__device__ __forceinline__ long long divide(long long a, long long b) {
-  return (a | b) >> 32 ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
-}
 struct Shares {
-  long long each, more;
-  __device__ __forceinline__ long long start(long long i) const { return i * each + (i < more ? i : more); }
-  __device__ __forceinline__ long long owner(long long unit) const {
-    const long long head = more * (each + 1);
-    return unit < head ? divide(unit, each + 1) : more + divide(unit - head, each);
+  uint32_t each, more;
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ uint32_t owner(uint32_t unit) const {
+    const uint32_t head = more * (each + 1);
+    return unit < head ? unit / (each + 1) : more + (unit - head) / each;
   }
 };
 
 // Where a warp (or its prefetch) stands in its list of tiles: in sequence b,
 // group r, at tile t of the portion [.., end), with `rest` units behind it.
 struct Cursor {
-  int b, r, tokens, t, end;
-  long long rest;
+  int b, r, tokens, t, end, rest;
 };
 
 // Moves on to the next portion; false at the end of the list.
@@ -186,7 +182,7 @@ __device__ __forceinline__ bool next_portion(const TbDecodeAttnQuantArgs& a, con
       c.tokens = tokens_of(a, g, c.b);
     } while (c.tokens == 0);
   }
-  const int n = units(c.tokens), take = n < c.rest ? n : static_cast<int>(c.rest);
+  const int n = units(c.tokens), take = n < c.rest ? n : c.rest;
   c.t = 0;
   c.end = take - kStart;
   c.rest -= take;
@@ -220,9 +216,10 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   uint8_t* ring = smem + w * S::kRing;
   float* first_part = reinterpret_cast<float*>(smem + kWarps * S::kRing + w * S::kPart);
   uint2* q_smem = reinterpret_cast<uint2*>(smem + kWarps * (S::kRing + S::kPart) + w * S::kQ);
-  long long* scan = reinterpret_cast<long long*>(smem + kWarps * (S::kRing + S::kPart + S::kQ));
-  int* shared = reinterpret_cast<int*>(scan + 3 * kWarps + 2);  // first CTA of the list's first context, last one of its last
-  int4* meta = reinterpret_cast<int4*>(scan + 3 * kWarps + 4);  // of the 2 kWarps parts: (sequence, group, opens | closes << 1, -)
+  uint32_t* before = reinterpret_cast<uint32_t*>(smem + kWarps * (S::kRing + S::kPart + S::kQ));  // [threads]
+  uint32_t* sums = before + kThreads;                                                          // [warps]
+  int* shared = reinterpret_cast<int*>(sums + kWarps);  // first CTA of the list's first context, last one of its last
+  int2* meta = reinterpret_cast<int2*>(shared + 2);     // [2 warps] parts: (sequence x group or -1, opens | closes << 1)
 
   // ---- this warp's list of tiles
   Cursor cur;
@@ -236,6 +233,48 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b;
       for (int i = threadIdx.x; i < a.Hq * (D / 4); i += kThreads)
         store_out4<T>(o + static_cast<long long>(i / (D / 4)) * a.os_h + i % (D / 4) * 4, out4, 0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  uint32_t total = 0;
+  Shares sh = {};
+  // the sequence b of a unit and its place in the sequence: the run of sequences that holds it (the last one that does
+  // not begin behind it; a lane looks at four), then the sequence in the run
+  auto find = [&](uint32_t unit, int& b, uint32_t& off) {
+    const int per = (a.B + kThreads - 1) / kThreads;
+    uint32_t base = 0;
+    for (int i = 0; i < lane * 4 / 32; ++i) base += sums[i];
+    const uint4 x = *reinterpret_cast<const uint4*>(before + lane * 4);
+    const uint32_t at[4] = {(base + x.x) * g.HG, (base + x.y) * g.HG, (base + x.z) * g.HG, (base + x.w) * g.HG};
+    int n = 0;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at[i] <= unit) {
+        ++n;
+        top = at[i];
+      }
+    const int run = __reduce_add_sync(0xffffffffu, n) - 1;
+    off = unit - __reduce_max_sync(0xffffffffu, top);
+    b = run * per;
+    if (per == 1) return;
+    for (int i = 0; i < per; i += 32) {
+      const int c = b + lane;
+      uint32_t inc = i + lane < per && c < a.B ? units(tokens_of(a, g, c)) * g.HG : 0;
+      const uint32_t mine = inc;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const unsigned behind = __ballot_sync(0xffffffffu, off < inc);
+      if (behind) {
+        const int l = __ffs(behind) - 1;
+        b += l;
+        off -= __shfl_sync(0xffffffffu, inc - mine, l);
+        return;
+      }
+      b += 32;
+      off -= __shfl_sync(0xffffffffu, inc, 31);
     }
   };
   if (g.whole) {
@@ -257,79 +296,48 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   } else {
     // prefix sums of the sequences' units: each thread a run of sequences
     const int per = (a.B + kThreads - 1) / kThreads, b0 = threadIdx.x * per;
-    const int b1 = b0 + per < a.B ? b0 + per : a.B;
-    long long mine = 0;
+    const int b1 = min(b0 + per, a.B);
+    uint32_t mine = 0;
 #pragma unroll 4
     for (int b = b0; b < b1; ++b) mine += units(tokens_of(a, g, b));
-    long long inc = mine;
+    uint32_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+      const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    if (lane == 31) scan[w] = inc;
+    before[threadIdx.x] = inc - mine;  // within the warp
+    if (lane == 31) sums[w] = inc;
     if (threadIdx.x == 0) *P::record(a.ws, gridDim.x, blockIdx.x) = make_int4(0, 0, 0, -1);
     __syncthreads();
-    long long before = inc - mine, total = 0;
+    total = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < w) before += scan[i];
-      total += scan[i];
-    }
+    for (int i = 0; i < kWarps; ++i) total += sums[i];
     total *= g.HG;
-    before *= g.HG;
-    mine *= g.HG;
     // as many CTAs as fit at once, unless that leaves them less than kMinTiles, or more than kWaveTiles
-    long long N = g.fit;
+    uint32_t N = g.fit;
     if (total < N * kMinTiles) N = (total + kMinTiles - 1) / kMinTiles;
     if (total > N * kWaveTiles) N = total / kWaveTiles;
     if (N > gridDim.x) N = gridDim.x;
     if (N == 0) empty_rows(gridDim.x);
     if (blockIdx.x >= N) return;
     ctas = static_cast<int>(N);
-    Shares sh;
-    sh.each = divide(total, N * kWarps);
+    sh.each = total / (N * kWarps);
     sh.more = total - sh.each * (N * kWarps);
-    const long long me = static_cast<long long>(blockIdx.x) * kWarps;
-#pragma unroll
-    for (int i = 0; i <= kWarps; ++i) {  // where the warps' lists start, and the last unit of this CTA
-      const long long at_unit = sh.start(me + i) - (i == kWarps ? 1 : 0);
-      const long long f = at_unit < total ? at_unit : total - 1;  // (a worker without units starts behind the last one)
-      if (f >= before && f < before + mine) {
-        int b = b0;
-        long long at = before, n = static_cast<long long>(units(tokens_of(a, g, b))) * g.HG;
-        while (f >= at + n) {
-          at += n;
-          n = static_cast<long long>(units(tokens_of(a, g, ++b))) * g.HG;
-        }
-        scan[kWarps + 2 * i] = b;
-        scan[kWarps + 2 * i + 1] = f - at;
-      }
-    }
-    __syncthreads();
-    const long long first = sh.start(me + w);
-    cur.b = static_cast<int>(scan[kWarps + 2 * w]);
-    const long long off = scan[kWarps + 2 * w + 1];
+    const uint32_t me = blockIdx.x * kWarps + w, first = sh.start(me);
+    uint32_t off;
+    find(min(first, total - 1), cur.b, off);  // (a warp without units starts behind the last one)
     cur.tokens = tokens_of(a, g, cur.b);
     const int n = units(cur.tokens);
-    cur.r = static_cast<int>(divide(off, n));
-    const int at = static_cast<int>(off - static_cast<long long>(cur.r) * n);
+    cur.r = off / n;
+    const int at = off - cur.r * n;
     cur.t = at > kStart ? at - kStart : 0;
-    cur.rest = sh.start(me + w + 1) - first;
-    const int take = n - at < cur.rest ? n - at : static_cast<int>(cur.rest);
+    cur.rest = sh.start(me + 1) - first;
+    const int take = min(n - at, cur.rest);
     cur.end = at + take - kStart;
     cur.rest -= take;
-    // which CTAs share the contexts at the two ends of this CTA's list (used by the merge, if they are split)
-    if (threadIdx.x == 0) {
-      shared[0] = static_cast<int>(sh.owner(first - cur.t) / kWarps);
-    } else if (threadIdx.x == kThreads - 1) {
-      const long long e = scan[kWarps + 2 * kWarps + 1];
-      const int ne = units(tokens_of(a, g, static_cast<int>(scan[kWarps + 2 * kWarps])));
-      const long long behind = ne - 1 - (e - divide(e, ne) * ne);
-      shared[1] = static_cast<int>(sh.owner(sh.start(me + kWarps) - 1 + behind) / kWarps);
-    }
   }
-  if (lane == 0) meta[2 * w] = meta[2 * w + 1] = make_int4(-1, 0, 0, 0);
+  if (lane == 0) meta[2 * w] = meta[2 * w + 1] = make_int2(-1, 0);
 
   // ---- prefetch: a cursor that runs ahead, and where its next tile lies: with pages of whole tiles the tile's first row
   // and its number of tokens, else (lanes 0-15) each token's row
@@ -400,7 +408,20 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   look();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
-  if (!g.whole) empty_rows(ctas);
+  if (!g.whole) {
+    empty_rows(ctas);
+    // which CTAs share the contexts at the two ends of this CTA's list (used by the merge, if they are split)
+    if (w == 0) {
+      if (lane == 0) shared[0] = sh.owner(sh.start(blockIdx.x * kWarps) - cur.t) / kWarps;
+    } else if (w == kWarps - 1) {
+      const uint32_t last = sh.start((blockIdx.x + 1) * kWarps) - 1;
+      int b;
+      uint32_t off;
+      find(last, b, off);
+      const uint32_t n = units(tokens_of(a, g, b));
+      if (lane == 0) shared[1] = sh.owner(last + n - 1 - off % n) / kWarps;
+    }
+  }
 
   // ---- portions of this warp, one (sequence, group) each
   int get = 0;
@@ -609,41 +630,32 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           *reinterpret_cast<float2*>(part + kHeads * D + 2 * h) = make_float2(m[n][e], v);
       }
     if (!(opens && closes) && lane == 0)
-      meta[2 * w + (first_portion ? 0 : 1)] = make_int4(b, r, (opens ? 1 : 0) | (closes ? 2 : 0), 0);
+      meta[2 * w + (first_portion ? 0 : 1)] = make_int2(b * g.HG + r, (opens ? 1 : 0) | (closes ? 2 : 0));
     first_portion = false;
   }
   cp_wait<0>();
   __syncthreads();
   tb::pdl_trigger();
 
-  // ---- merge the parts of this CTA: runs of the same (sequence, group), a warp for each query head
+  // ---- merge the parts of this CTA: those of the same (sequence, group), a warp for each query head
   constexpr int E = D / 32, V = E < 4 ? E : 4;
+  const int2 mt = lane < 2 * kWarps ? meta[lane] : make_int2(-1, 0);
   bool first_run = true;
 #pragma unroll 1
-  for (int x = 0; x < 2 * kWarps;) {
-    const int4 at = meta[x];
-    if (at.x < 0) {
-      ++x;
-      continue;
-    }
-    int bits = 0;
-    unsigned set = 0;
-    for (; x < 2 * kWarps; ++x) {
-      const int4 o = meta[x];
-      if (o.x < 0) continue;
-      if (o.x != at.x || o.y != at.y) break;
-      set |= 1u << x;
-      bits |= o.z & 3;
-    }
-    const bool whole = bits == 3;
-    const int h0 = at.y / g.NG * g.G + at.y % g.NG * kHeads;
-    const int left = g.G - at.y % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
+  for (unsigned parts = __ballot_sync(0xffffffffu, mt.x >= 0); parts != 0;) {
+    const int seg = __shfl_sync(0xffffffffu, mt.x, __ffs(parts) - 1);
+    const unsigned set = __ballot_sync(0xffffffffu, mt.x == seg);
+    const bool opens = __any_sync(0xffffffffu, mt.x == seg && mt.y & 1);
+    const bool whole = __any_sync(0xffffffffu, mt.x == seg && mt.y & 2) && opens;
+    parts &= ~set;
+    const int b = seg / g.HG, r = seg - b * g.HG, kh = r / g.NG, left = g.G - (r - kh * g.NG) * kHeads;
+    const int nh = min(left, kHeads), h0 = kh * g.G + g.G - left;
     const long long slot = 2ll * blockIdx.x + (first_run ? 0 : 1);
     first_run = false;
     if (!whole && threadIdx.x == 0) {  // a part of a context that other CTAs share
       int4* rec = P::record(a.ws, gridDim.x, blockIdx.x);
-      if (bits & 1) {
-        rec->x = at.x * g.HG + at.y;
+      if (opens) {
+        rec->x = seg;
         rec->y = static_cast<int>(slot);
         rec->z = shared[1] - static_cast<int>(blockIdx.x) + 1;
       } else {
@@ -651,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       }
     }
     auto part_of = [&](int p) {
-      return reinterpret_cast<const float*>(p % 2 ? smem + p / 2 * S::kRing : smem + kWarps * S::kRing + p / 2 * S::kPart);
+      return reinterpret_cast<const float*>(smem + (p % 2 ? p / 2 * S::kRing : kWarps * S::kRing + p / 2 * S::kPart));
     };
 #pragma unroll 1
     for (int h = w; h < nh; h += kWarps) {
@@ -680,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           for (int e = 0; e < V; ++e) o[i + e] += fp * y[e];
         }
       }
-      T* out = static_cast<T*>(a.out) + static_cast<long long>(at.x) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
+      T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
       float* part = P::out(a.ws, slot, h);
 #pragma unroll
       for (int i = 0; i < E; i += V) {
@@ -813,6 +825,18 @@ int sm_count() {
   return n;
 }
 
+// Units of B sequences with HG groups and contexts of `cap` tokens.
+long long most_units(int B, int HG, int cap) { return static_cast<long long>(B) * HG * (cap / kTile + 1 + kStart); }
+
+// CTAs to launch for contexts of at most `cap` tokens: those that fit at once,
+// more (up to kMostWaves times) where each could still take kWaveTiles.
+template <int D, int NT>
+int grid_of(int B, int Hq, int Hk, int cap) {
+  const int fit = sm_count() * resident<D, NT>(), G = Hq / Hk;
+  const long long n = most_units(B, Hk * ((G + 8 * NT - 1) / (8 * NT)), cap) / kWaveTiles;
+  return n <= fit ? fit : n < kMostWaves * fit ? static_cast<int>(n) : kMostWaves * fit;
+}
+
 template <int D, int NT>
 Geometry geometry(const TbDecodeAttnQuantArgs& a, int sms) {
   Geometry g;
@@ -825,18 +849,9 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a, int sms) {
   for (int i = 0; i < 31; ++i)
     if (a.cache.bs == 1 << i) g.shift = i;
   g.tile_pages = a.cache.bs % kTile == 0;
-  g.whole = g.cap <= kWholeTokens;
+  // (units are counted in 32 bits)
+  g.whole = g.cap <= kWholeTokens || most_units(a.B, g.HG, g.cap) > 0x7fffffff;
   return g;
-}
-
-// CTAs to launch for contexts of at most `cap` tokens: those that fit at once,
-// more (up to kMostWaves times) where each could still take kWaveTiles.
-template <int D, int NT>
-int grid_of(int B, int Hq, int Hk, int cap) {
-  const int fit = sm_count() * resident<D, NT>(), G = Hq / Hk;
-  const long long most = static_cast<long long>(B) * Hk * ((G + 8 * NT - 1) / (8 * NT)) * (cap / kTile + 1 + kStart);
-  const long long n = most / kWaveTiles;
-  return n <= fit ? fit : n < kMostWaves * fit ? static_cast<int>(n) : kMostWaves * fit;
 }
 
 template <typename T, int D, int NT>
