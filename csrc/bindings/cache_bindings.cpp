@@ -1,13 +1,16 @@
 // torch-tensor entry points of the general rotary positions and the 8-bit
 // paged KV cache.  Each checks its arguments completely, whatever device they
-// are on, then launches on the current stream of their device and returns
-// true; for CPU tensors it returns false and the caller computes on the host.
+// are on, then launches on the current stream of their device and returns its
+// result (a new tensor where no output was given); for CPU tensors it returns
+// None and the caller computes on the host.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/pybind11.h>
 #include <torch/extension.h>
 
 #include <climits>
+#include <cmath>
+#include <optional>
 
 #include "kernels.h"
 #include "turbol/common.hpp"
@@ -85,12 +88,11 @@ void index1(const at::Tensor& t, int64_t n, const char* op, const char* m) {
   chk(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), op, m);
 }
 
-int* error_of(const py::object& e, const at::Device& dev, const char* op, at::Tensor& hold) {
-  if (e.is_none()) return nullptr;
-  hold = e.cast<at::Tensor>();
-  chk(hold.scalar_type() == at::kInt && hold.numel() >= 1 && hold.is_contiguous() && hold.device() == dev, op,
+int* error_of(const std::optional<at::Tensor>& e, const at::Device& dev, const char* op) {
+  if (!e) return nullptr;
+  chk(e->scalar_type() == at::kInt && e->numel() >= 1 && e->is_contiguous() && e->device() == dev, op,
       "error is an int32 tensor on the same device");
-  return hold.data_ptr<int>();
+  return e->data_ptr<int>();
 }
 
 // The table's dimensions: R / 2 pairs for max_pos positions.
@@ -101,25 +103,31 @@ void table_of(const at::Tensor& t, int64_t D, const char* op) {
   chk(reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0, op, "table is 8-byte aligned");
 }
 
-bool rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, const at::Tensor& out, bool interleaved,
-            bool transpose, const py::object& error) {
+using Opt = std::optional<at::Tensor>;
+
+Opt rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, const Opt& out_, bool interleaved,
+           bool transpose, const Opt& error) {
   const char* op = "rotary";
   rows3(x, op, "x is [T, H, D] with a contiguous last dimension");
   const int dt = type_of(x, op);
-  rows3(out, op, "out is [T, H, D] with a contiguous last dimension");
-  chk(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type(), op, "out has x's shape and type");
   chk(x.size(2) % 2 == 0 && x.size(2) <= INT_MAX, op, "an even head dimension");
   index1(pos, x.size(0), op, "pos is a contiguous int32 [T]");
   table_of(table, x.size(2), op);
   const at::Device dev = x.device();
-  chk(out.device() == dev && pos.device() == dev && table.device() == dev, op, "all tensors on one device");
-  chk(rows_distinct(out), op, "out has overlapping rows");
-  chk(same_view(x, out) || columns_apart(x, out), op, "out is x itself or does not overlap it");
-  at::Tensor hold;
-  int* err = error_of(error, dev, op, hold);
-  if (!x.is_cuda()) return false;
-  if (x.numel() == 0) return true;
+  chk(pos.device() == dev && table.device() == dev, op, "all tensors on one device");
+  if (out_) {
+    rows3(*out_, op, "out is [T, H, D] with a contiguous last dimension");
+    chk(out_->sizes() == x.sizes() && out_->scalar_type() == x.scalar_type(), op, "out has x's shape and type");
+    chk(out_->device() == dev, op, "all tensors on one device");
+    chk(rows_distinct(*out_), op, "out has overlapping rows");
+    chk(same_view(x, *out_) || columns_apart(x, *out_), op, "out is x itself or does not overlap it");
+    for (const at::Tensor* t : {&pos, &table}) chk(apart(*out_, *t), op, "out overlaps an input");
+  }
+  int* err = error_of(error, dev, op);
+  if (!x.is_cuda()) return std::nullopt;
   c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out = out_ ? *out_ : at::empty(x.sizes(), x.options());
+  if (x.numel() == 0) return out;
   TbRotaryArgs a{};
   a.x = x.data_ptr();
   a.y = out.data_ptr();
@@ -139,7 +147,40 @@ bool rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table,
   a.transpose = transpose;
   a.err = err;
   cuda_ok(tb_rotary(&a, turbol::StreamFor(x)), op);
-  return true;
+  return out;
+}
+
+// The differentiable form (CUDA tensors): the gradient of a rotation is the
+// rotation by the negative angles (times the table's factor), itself
+// differentiable.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& pos,
+                            const at::Tensor& table, bool interleaved, bool transpose, const Opt& error) {
+    at::Tensor out = *rotary(x, pos, table, std::nullopt, interleaved, transpose, error);
+    ctx->save_for_backward({pos, table});
+    ctx->saved_data["how"] = (interleaved ? 1 : 0) | (transpose ? 2 : 0);
+    if (error) ctx->saved_data["error"] = *error;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 const torch::autograd::variable_list& grads) {
+    at::Tensor dx;
+    if (grads[0].defined()) {
+      const auto saved = ctx->get_saved_variables();
+      const int64_t how = ctx->saved_data["how"].toInt();
+      Opt error;
+      if (ctx->saved_data.count("error")) error = ctx->saved_data["error"].toTensor();
+      const at::Tensor dy = grads[0].stride(2) == 1 ? grads[0] : grads[0].contiguous();  // a broadcast gradient
+      dx = RotaryFunction::apply(dy, saved[0], saved[1], (how & 1) != 0, (how & 2) == 0, error);
+    }
+    return {dx, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor rotary_grad(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, bool interleaved,
+                       bool transpose, const Opt& error) {
+  chk(x.is_cuda(), "rotary_grad", "CUDA tensors");
+  return RotaryFunction::apply(x, pos, table, interleaved, transpose, error);
 }
 
 TbQuantCache cache_of(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
@@ -176,10 +217,9 @@ TbQuantCache cache_of(const at::Tensor& kc, const at::Tensor& vc, const at::Tens
   return c;
 }
 
-bool kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& seq, const at::Tensor& pos,
-                    const at::Tensor& block_table, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
-                    const py::object& q_, const py::object& q_out_, const py::object& table_, bool interleaved,
-                    const py::object& error) {
+Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& seq, const at::Tensor& pos,
+                   const at::Tensor& block_table, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
+                   const Opt& q_, const Opt& q_out_, const Opt& table_, bool interleaved, const Opt& error) {
   const char* op = "kv_quant_write";
   TbKvQuantWriteArgs a{};
   a.cache = cache_of(kc, vc, ks, vs, block_table, op);
@@ -199,10 +239,9 @@ bool kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
     for (const at::Tensor* t : {&k, &v, &seq, &pos, &block_table})
       chk(apart(*caches[i], *t), op, "an input overlaps the cache");
   }
-  at::Tensor q, q_out, table, hold;
-  a.rot.err = error_of(error, dev, op, hold);
-  if (!table_.is_none()) {
-    table = table_.cast<at::Tensor>();
+  a.rot.err = error_of(error, dev, op);
+  if (table_) {
+    const at::Tensor& table = *table_;
     table_of(table, a.cache.D, op);
     chk(table.size(1) % 4 == 0, op, "a multiple of 8 rotated dimensions");
     chk(table.device() == dev, op, "all tensors on one device");
@@ -211,32 +250,40 @@ bool kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
     a.rot.max_pos = static_cast<int>(table.size(0));
     a.rot.interleaved = interleaved;
   }
-  chk(q_.is_none() == q_out_.is_none(), op, "q and q_out come together");
-  if (!q_.is_none()) {
-    q = q_.cast<at::Tensor>();
-    q_out = q_out_.cast<at::Tensor>();
-    chk(!table_.is_none(), op, "q needs a table");
-    rows3(q, op, "q is [T, Hq, D] with a contiguous last dimension");
-    rows3(q_out, op, "q_out is [T, Hq, D] with a contiguous last dimension");
-    chk(q.size(0) == T && q.size(2) == a.cache.D && q.scalar_type() == k.scalar_type(), op,
+  chk(q_ || !q_out_, op, "q_out needs q");
+  if (q_) {
+    chk(table_.has_value(), op, "q needs a table");
+    rows3(*q_, op, "q is [T, Hq, D] with a contiguous last dimension");
+    chk(q_->size(0) == T && q_->size(2) == a.cache.D && q_->scalar_type() == k.scalar_type(), op,
         "q has k's rows, head dimension and type");
-    chk(q_out.sizes() == q.sizes() && q_out.scalar_type() == q.scalar_type(), op, "q_out has q's shape and type");
-    chk(q.device() == dev && q_out.device() == dev, op, "all tensors on one device");
-    chk(rows_distinct(q_out), op, "q_out has overlapping rows");
-    chk(same_view(q, q_out) || columns_apart(q, q_out), op, "q_out is q itself or does not overlap it");
-    chk(columns_apart(q_out, k) && columns_apart(q_out, v), op, "q_out overlaps k or v");
-    for (int i = 0; i < 4; ++i) chk(apart(*caches[i], q) && apart(*caches[i], q_out), op, "q overlaps the cache");
-    a.rot.x = q.data_ptr();
-    a.rot.y = q_out.data_ptr();
-    a.rot.H = static_cast<int>(q.size(1));
-    a.rot.xs_t = q.stride(0);
-    a.rot.xs_h = q.stride(1);
-    a.rot.ys_t = q_out.stride(0);
-    a.rot.ys_h = q_out.stride(1);
+    chk(q_->device() == dev, op, "all tensors on one device");
+    for (int i = 0; i < 4; ++i) chk(apart(*caches[i], *q_), op, "q overlaps the cache");
   }
-  if (!kc.is_cuda()) return false;
-  if (T == 0) return true;
+  if (q_out_) {
+    rows3(*q_out_, op, "q_out is [T, Hq, D] with a contiguous last dimension");
+    chk(q_out_->sizes() == q_->sizes() && q_out_->scalar_type() == q_->scalar_type(), op,
+        "q_out has q's shape and type");
+    chk(q_out_->device() == dev, op, "all tensors on one device");
+    chk(rows_distinct(*q_out_), op, "q_out has overlapping rows");
+    chk(same_view(*q_, *q_out_) || columns_apart(*q_, *q_out_), op, "q_out is q itself or does not overlap it");
+    chk(columns_apart(*q_out_, k) && columns_apart(*q_out_, v), op, "q_out overlaps k or v");
+    for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &seq, &pos, &block_table, &*table_})
+      chk(apart(*t, *q_out_), op, "q_out overlaps an input");
+  }
+  if (!kc.is_cuda()) return std::nullopt;
   c10::cuda::CUDAGuard guard(dev);
+  Opt q_out = q_out_;
+  if (q_ && !q_out) q_out = at::empty(q_->sizes(), q_->options());
+  if (T == 0) return q_out;
+  if (q_) {
+    a.rot.x = q_->data_ptr();
+    a.rot.y = q_out->data_ptr();
+    a.rot.H = static_cast<int>(q_->size(1));
+    a.rot.xs_t = q_->stride(0);
+    a.rot.xs_h = q_->stride(1);
+    a.rot.ys_t = q_out->stride(0);
+    a.rot.ys_h = q_out->stride(1);
+  }
   a.k = k.data_ptr();
   a.v = v.data_ptr();
   a.ks_t = k.stride(0);
@@ -247,12 +294,12 @@ bool kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
   a.pos = pos.data_ptr<int>();
   a.T = static_cast<int>(T);
   cuda_ok(tb_kv_quant_write(&a, turbol::StreamFor(kc)), op);
-  return true;
+  return q_out;
 }
 
 bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs,
                    const at::Tensor& seq, const at::Tensor& pos, const at::Tensor& block_table, const at::Tensor& k_out,
-                   const at::Tensor& v_out, const py::object& error) {
+                   const at::Tensor& v_out, const Opt& error) {
   const char* op = "kv_quant_read";
   TbKvQuantReadArgs a{};
   a.cache = cache_of(kc, vc, ks, vs, block_table, op);
@@ -271,8 +318,7 @@ bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
   chk(columns_apart(k_out, v_out), op, "the two outputs overlap");
   for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &seq, &pos, &block_table})
     chk(apart(k_out, *t) && apart(v_out, *t), op, "out overlaps an input");
-  at::Tensor hold;
-  a.err = error_of(error, dev, op, hold);
+  a.err = error_of(error, dev, op);
   if (!kc.is_cuda()) return false;
   if (T == 0) return true;
   c10::cuda::CUDAGuard guard(dev);
@@ -289,35 +335,39 @@ bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
   return true;
 }
 
-bool decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
                             const at::Tensor& vs, const at::Tensor& block_table, const at::Tensor& ctx_len,
-                            const at::Tensor& out, double scale, const py::object& error) {
+                           const Opt& out_, std::optional<double> scale_, const Opt& error) {
   const char* op = "decode_attention_quant";
   TbDecodeAttnQuantArgs a{};
   a.cache = cache_of(kc, vc, ks, vs, block_table, op);
   const at::Device dev = kc.device();
   rows3(q, op, "q is [B, Hq, D] with a contiguous last dimension");
-  rows3(out, op, "out is [B, Hq, D] with a contiguous last dimension");
   a.dtype = type_of(q, op);
   chk(a.dtype != TB_F32, op, "bf16 or fp16 q");
-  chk(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), op, "out has q's shape and type");
   chk(q.size(2) == a.cache.D, op, "q has the cache's head dimension");
   chk(q.size(1) >= 1 && q.size(1) % a.cache.Hk == 0, op, "the query heads are a multiple of the KV heads");
   const int64_t B = q.size(0);
   chk(block_table.size(0) == B, op, "one block_table row per sequence");
   chk(B * q.size(1) <= INT_MAX, op, "at most 2^31 - 1 query rows");
   index1(ctx_len, B, op, "ctx_len is a contiguous int32 [B]");
-  for (const at::Tensor* t : {&q, &out, &ctx_len}) chk(t->device() == dev, op, "all tensors on one device");
-  chk(rows_distinct(out), op, "out has overlapping rows");
-  chk(columns_apart(out, q), op, "out overlaps q");
-  for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &ctx_len, &block_table})
-    chk(apart(out, *t), op, "out overlaps an input");
+  for (const at::Tensor* t : {&q, &ctx_len}) chk(t->device() == dev, op, "all tensors on one device");
+  if (out_) {
+    rows3(*out_, op, "out is [B, Hq, D] with a contiguous last dimension");
+    chk(out_->sizes() == q.sizes() && out_->scalar_type() == q.scalar_type(), op, "out has q's shape and type");
+    chk(out_->device() == dev, op, "all tensors on one device");
+    chk(rows_distinct(*out_), op, "out has overlapping rows");
+    chk(columns_apart(*out_, q), op, "out overlaps q");
+    for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &ctx_len, &block_table})
+      chk(apart(*out_, *t), op, "out overlaps an input");
+  }
+  const double scale = scale_ ? *scale_ : 1.0 / std::sqrt(static_cast<double>(a.cache.D));
   chk(std::isfinite(scale), op, "a finite scale");
-  at::Tensor hold, ws;
-  a.err = error_of(error, dev, op, hold);
-  if (!kc.is_cuda()) return false;
-  if (B == 0) return true;
+  a.err = error_of(error, dev, op);
+  if (!kc.is_cuda()) return std::nullopt;
   c10::cuda::CUDAGuard guard(dev);
+  at::Tensor ws, out = out_ ? *out_ : at::empty(q.sizes(), q.options());
+  if (B == 0) return out;
   a.q = q.data_ptr();
   a.out = out.data_ptr();
   a.qs_b = q.stride(0);
@@ -336,15 +386,17 @@ bool decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at:
     a.ws = ws.data_ptr<float>();
   }
   cuda_ok(tb_decode_attention_quant(&a, turbol::StreamFor(kc)), op);
-  return true;
+  return out;
 }
 
 }  // namespace
 
 void register_cache_ops(py::module_& m) {
-  m.def("rotary", &rotary, py::arg("x"), py::arg("pos"), py::arg("table"), py::arg("out"),
+  m.def("rotary", &rotary, py::arg("x"), py::arg("pos"), py::arg("table"), py::arg("out") = py::none(),
         py::arg("interleaved") = false, py::arg("transpose") = false, py::arg("error") = py::none(),
-        "out = rotary positions of x [T, H, D] (general form); false for CPU tensors, after the checks");
+        "rotary positions of x [T, H, D] (general form); None for CPU tensors, after the checks");
+  m.def("rotary_grad", &rotary_grad, py::arg("x"), py::arg("pos"), py::arg("table"), py::arg("interleaved") = false,
+        py::arg("transpose") = false, py::arg("error") = py::none(), "the same, differentiable in x (CUDA tensors)");
   m.def("kv_quant_write", &kv_quant_write, py::arg("k"), py::arg("v"), py::arg("seq_of_token"), py::arg("pos"),
         py::arg("block_table"), py::arg("kc"), py::arg("vc"), py::arg("ks"), py::arg("vs"), py::arg("q") = py::none(),
         py::arg("q_out") = py::none(), py::arg("table") = py::none(), py::arg("interleaved") = false,
@@ -354,6 +406,6 @@ void register_cache_ops(py::module_& m) {
         py::arg("seq_of_token"), py::arg("pos"), py::arg("block_table"), py::arg("k_out"), py::arg("v_out"),
         py::arg("error") = py::none(), "reads rows of the 8-bit paged cache back");
   m.def("decode_attention_quant", &decode_attention_quant, py::arg("q"), py::arg("kc"), py::arg("vc"), py::arg("ks"),
-        py::arg("vs"), py::arg("block_table"), py::arg("ctx_len"), py::arg("out"), py::arg("scale"),
-        py::arg("error") = py::none(), "attention of one token per sequence over the 8-bit paged cache");
+        py::arg("vs"), py::arg("block_table"), py::arg("ctx_len"), py::arg("out") = py::none(),
+        py::arg("scale") = py::none(), py::arg("error") = py::none(), "attention of one token per sequence over the 8-bit paged cache");
 }

@@ -18,61 +18,73 @@
 
 namespace {
 
-// One thread: one unit of one head, two vectors of NP elements.  Rotated units
-// hold NP pairs (half layout: NP elements of each half; interleaved: 2 NP
-// neighbours), the others 2 NP copied elements.
-template <typename T, int NP, bool INTER>
-__global__ void rotary_kernel(TbRotaryArgs a, int rot_units, int units) {
-  const long long total = static_cast<long long>(a.T) * a.H * units;
+// A thread holds one unit, two vectors of NP elements, of HU heads of a token
+// (every HS-th), so it reads its table entries once: of 40 heads read anew they
+// were 2.5 times the traffic of the rows themselves, in L1.  Rotated units hold NP
+// pairs (half layout: NP elements of each half; interleaved: 2 NP neighbours), the
+// others 2 NP copied elements.  All loads are issued before the first product.
+template <typename T, int NP, int HU, bool INTER>
+__global__ void __launch_bounds__(256, HU > 1 ? 3 : 4) rotary_kernel(TbRotaryArgs a, int rot_units, int units, int HS, int tokens) {
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
-  const float2* table = reinterpret_cast<const float2*>(a.table);
-  const int half = a.R / 2;
+  const int half = a.R / 2, per = units * HS;
+  const int tk = threadIdx.x / per;
+  const long long t = blockIdx.x * static_cast<long long>(tokens) + tk;
+  if (tk >= tokens || t >= a.T) return;
+  const int p = a.pos[t];
+  const bool bad = p >= a.max_pos;
+  if (bad && a.err && threadIdx.x == tk * per) atomicCAS(a.err, 0, 1);
   const float sgn = a.transpose ? -1.f : 1.f;
-  for (long long e = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; e < total;
-       e += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const int u = static_cast<int>(e % units);
-    const long long r = e / units;
-    const int h = static_cast<int>(r % a.H);
-    const long long t = r / a.H;
-    const int p = a.pos[t];
-    const bool bad = p >= a.max_pos;
-    if (bad && a.err && u == 0 && h == 0) atomicCAS(a.err, 0, 1);
+  for (int i = threadIdx.x - tk * per; i < per; i += blockDim.x) {  // (more than one round only where per > 256)
+    const int u = i % units, h0 = i / units;
+    const bool turn = u < rot_units && p >= 0 && !bad;
     const int o1 = INTER || u >= rot_units ? u * 2 * NP : u * NP;
     const int o2 = INTER || u >= rot_units ? o1 + NP : o1 + half;
-    const T* xr = x + t * a.xs_t + static_cast<long long>(h) * a.xs_h;
-    T* yr = y + t * a.ys_t + static_cast<long long>(h) * a.ys_h;
-    float f[NP], g[NP];
-    tb::load_vec<T, NP>(xr + o1, f);
-    tb::load_vec<T, NP>(xr + o2, g);
-    if (bad) {
+    const T* xr = x + t * a.xs_t;
+    T* yr = y + t * a.ys_t;
+    tb::Packed<T, NP> lo[HU], hi[HU];
+    float cs[2 * NP];
+    if (turn) tb::load_vec<float, 2 * NP>(a.table + (static_cast<long long>(p) * half + u * NP) * 2, cs);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) f[i] = g[i] = NAN;
-    } else if (u < rot_units && p >= 0) {
-      const float2* tab = table + static_cast<long long>(p) * half + u * NP;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const float2 cs = tab[i];
-        const float sn = sgn * cs.y;
-        float& v = INTER ? (2 * i < NP ? f[2 * i % NP] : g[2 * i % NP]) : f[i];
-        float& w = INTER ? (2 * i + 1 < NP ? f[(2 * i + 1) % NP] : g[(2 * i + 1) % NP]) : g[i];
-        const float nv = v * cs.x - w * sn;
-        w = w * cs.x + v * sn;
-        v = nv;
+    for (int k = 0; k < HU; ++k)
+      if (h0 + k * HS < a.H) {
+        lo[k].load(xr + (h0 + k * HS) * a.xs_h + o1);
+        hi[k].load(xr + (h0 + k * HS) * a.xs_h + o2);
       }
-    }
-    tb::store_vec<T, NP>(yr + o1, f);
-    tb::store_vec<T, NP>(yr + o2, g);
+#pragma unroll
+    for (int k = 0; k < HU; ++k)
+      if (h0 + k * HS < a.H) {
+        float f[NP], g[NP];
+        lo[k].unpack(f);
+        hi[k].unpack(g);
+        if (bad) {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) f[j] = g[j] = NAN;
+        } else if (turn) {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            const float c = cs[2 * j], sn = sgn * cs[2 * j + 1];
+            float& v = INTER ? (2 * j < NP ? f[2 * j % NP] : g[2 * j % NP]) : f[j];
+            float& w = INTER ? (2 * j + 1 < NP ? f[(2 * j + 1) % NP] : g[(2 * j + 1) % NP]) : g[j];
+            const float nv = v * c - w * sn;
+            w = w * c + v * sn;
+            v = nv;
+          }
+        }
+        tb::store_vec<T, NP>(yr + (h0 + k * HS) * a.ys_h + o1, f);
+        tb::store_vec<T, NP>(yr + (h0 + k * HS) * a.ys_h + o2, g);
+      }
   }
 }
 
-template <typename T, int NP, bool INTER>
+template <typename T, int NP, int HU, bool INTER>
 int launch_vec(const TbRotaryArgs& a, cudaStream_t s) {
   const int rot_units = a.R / 2 / NP;
   const int units = rot_units + (a.x == a.y ? 0 : (a.D - a.R) / (2 * NP));
-  const long long total = static_cast<long long>(a.T) * a.H * units;
-  const long long blocks = (total + 255) / 256;
-  rotary_kernel<T, NP, INTER><<<static_cast<int>(blocks < 1184 ? blocks : 1184), 256, 0, s>>>(a, rot_units, units);
+  const int HS = (a.H + HU - 1) / HU;
+  const long long per = static_cast<long long>(units) * HS;
+  const int tokens = per >= 256 ? 1 : static_cast<int>(256 / per);
+  rotary_kernel<T, NP, HU, INTER><<<(a.T + tokens - 1) / tokens, 256, 0, s>>>(a, rot_units, units, HS, tokens);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -81,12 +93,17 @@ template <typename T, int NP>
 bool fits(const TbRotaryArgs& a) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y);
   return a.R / 2 % NP == 0 && (a.D - a.R) % (2 * NP) == 0 && a.xs_t % NP == 0 && a.xs_h % NP == 0 &&
-         a.ys_t % NP == 0 && a.ys_h % NP == 0 && at % (NP * sizeof(T)) == 0;
+         a.ys_t % NP == 0 && a.ys_h % NP == 0 && at % (NP * sizeof(T)) == 0 &&
+         reinterpret_cast<uintptr_t>(a.table) % 16 == 0;
 }
 
+// Four heads per thread where that still fills the machine (16 K units of a
+// head per head of the four: 148 SMs x 1,024 threads in flight and more).
 template <typename T, int NP>
 int launch_layout(const TbRotaryArgs& a, cudaStream_t s) {
-  return a.interleaved ? launch_vec<T, NP, true>(a, s) : launch_vec<T, NP, false>(a, s);
+  const bool many = static_cast<long long>(a.T) * a.H * (a.D / (2 * NP)) >= 4ll * 148 * 1024;
+  if (many) return a.interleaved ? launch_vec<T, NP, 4, true>(a, s) : launch_vec<T, NP, 4, false>(a, s);
+  return a.interleaved ? launch_vec<T, NP, 1, true>(a, s) : launch_vec<T, NP, 1, false>(a, s);
 }
 
 // The widest vectors that fit: 16 bytes, 8 bytes, or single elements.

@@ -60,4 +60,17 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
   }
 }
 
+// N values as they lie in memory (N * sizeof(T) at most 16 bytes), so that loads
+// can be kept in flight in few registers.
+template <typename T, int N>
+struct Packed {
+  typename RawOf<N * sizeof(T)>::type raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const decltype(raw)*>(p); }
+  __device__ __forceinline__ void unpack(float (&f)[N]) const {
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f32(e[i]);
+  }
+};
+
 }  // namespace tb

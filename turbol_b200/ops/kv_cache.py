@@ -22,7 +22,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import reference as ref
-from .rotary import _launch
+from .rotary import _call
 
 
 class QuantKV(NamedTuple):
@@ -60,12 +60,11 @@ def kv_quant_write(k: torch.Tensor, v: torch.Tensor, seq_of_token: torch.Tensor,
     and its q row is copied.  A sequence, position or block out of range writes
     nothing and sets ``error``; a position beyond the table also makes the q row
     NaN.  No two tokens of a call may name the same slot.  Not differentiable."""
-    if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if not _launch("kv_quant_write", k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q, q_out, table,
-                   interleaved, error):
-        ref.kv_quant_write(k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q, table, interleaved, q_out, error)
-    return q_out
+    y = _call("kv_quant_write", k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q, q_out, table, interleaved, error)
+    if not kc.is_cuda:
+        y = torch.empty_like(q) if q is not None and q_out is None else q_out
+        ref.kv_quant_write(k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q, table, interleaved, y, error)
+    return y if q_out is None else q_out
 
 
 def kv_quant_read(kc: torch.Tensor, vc: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor, seq_of_token: torch.Tensor,
@@ -79,7 +78,7 @@ def kv_quant_read(kc: torch.Tensor, vc: torch.Tensor, ks: torch.Tensor, vs: torc
     if out is None:
         shape = (pos.shape[0], kc.shape[1], kc.shape[3])
         out = (torch.zeros(shape, dtype=dtype, device=kc.device), torch.zeros(shape, dtype=dtype, device=kc.device))
-    if not _launch("kv_quant_read", kc, vc, ks, vs, seq_of_token, pos, block_table, out[0], out[1], error):
+    if not _call("kv_quant_read", kc, vc, ks, vs, seq_of_token, pos, block_table, out[0], out[1], error):
         ref.kv_quant_read(kc, vc, ks, vs, seq_of_token, pos, block_table, out, error)
     return out
 
@@ -94,10 +93,9 @@ def decode_attention_quant(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, 
     blocks out of range are left out and set ``error``.  The result does not
     depend on what the pages hold behind a context; it can depend, within
     rounding, on the other sequences of the batch (where contexts are split)."""
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1])
-    if not _launch("decode_attention_quant", q, kc, vc, ks, vs, block_table, ctx_len, out, scale, error):
-        ref.decode_attention_quant(q, kc, vc, ks, vs, block_table, ctx_len, scale, out, error)
-    return out
+    y = _call("decode_attention_quant", q, kc, vc, ks, vs, block_table, ctx_len, out, scale, error)
+    if y is None:
+        y = ref.decode_attention_quant(q, kc, vc, ks, vs, block_table, ctx_len,
+                                       1.0 / math.sqrt(q.shape[-1]) if scale is None else scale,
+                                       torch.empty_like(q) if out is None else out, error)
+    return y if out is None else out

@@ -83,24 +83,27 @@ def rotary_table(rot_dim: int, max_pos: int, theta: float = 1e4, scaling: Option
     return (torch.stack([torch.cos(ang), torch.sin(ang)], -1) * m).to(device=device, dtype=torch.float32).contiguous()
 
 
-def _launch(name: str, *args, **kw) -> bool:
-    """Checks and launches a kernel; False for CPU tensors (or a CPU-only build)."""
+def _call(name: str, *args):
+    """A kernel entry point: checks, launches and returns its result; None for CPU tensors (or a CPU-only build)."""
     o = getattr(_core(), "ops", None)
-    return False if o is None else getattr(o, name)(*args, **kw)
+    return None if o is None else getattr(o, name)(*args)
 
 
 def _apply(x, pos, table, interleaved, transpose, out, error):
-    if not _launch("rotary", x, pos, table, out, interleaved, transpose, error):
-        ref.rotary(x, pos, table, interleaved, transpose, out, error)
-    return out
+    y = _call("rotary", x, pos, table, out, interleaved, transpose, error)
+    if y is None:
+        y = ref.rotary(x, pos, table, interleaved, transpose, torch.empty_like(x) if out is None else out, error)
+    return y if out is None else out
 
 
 class _Rotary(torch.autograd.Function):
+    """The differentiable form for CPU tensors."""
+
     @staticmethod
     def forward(ctx, x, pos, table, interleaved, transpose, error):
         ctx.save_for_backward(pos, table)
         ctx.how = (interleaved, transpose, error)
-        return _apply(x, pos, table, interleaved, transpose, torch.empty(x.shape, dtype=x.dtype, device=x.device), error)
+        return _apply(x, pos, table, interleaved, transpose, None, error)
 
     @staticmethod
     def backward(ctx, dy):
@@ -128,8 +131,9 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, interleaved:
     (an int32 device tensor, optional) to 1."""
     if out is None:
         if x.requires_grad and torch.is_grad_enabled():
+            if x.is_cuda:
+                return _core().ops.rotary_grad(x, pos, table, interleaved, transpose, error)
             return _Rotary.apply(x, pos, table, interleaved, transpose, error)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
         raise ValueError("rotary: out= has no gradient")
     return _apply(x, pos, table, interleaved, transpose, out, error)
