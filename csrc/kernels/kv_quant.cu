@@ -70,161 +70,262 @@ __device__ __forceinline__ void store4(T* p, bool aligned, const float (&f)[4]) 
   }
 }
 
-// One pass over the rows: D / 8 lanes per row, eight elements each, U rows per
-// lane (all loaded before the first is reduced).  ROT: q and k rows are rotated; a
-// lane then holds both members of its pairs (half layout: two vectors of four),
-// else eight neighbours.  Rows of a token: Hk of k, Hk of v, then Hq of q.
-template <typename T, int D, int U, bool ROT>
-__global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs a, int slots, bool aligned) {
-  constexpr int L = D / 8, kRows = 256 / L;  // lanes per row, rows per block and round
-  const int l = threadIdx.x % L;
-  const int Hk = a.cache.Hk, R = ROT ? a.rot.R : 0;
-  const long long rows = static_cast<long long>(a.T) * slots;
-  const long long r0 = blockIdx.x * static_cast<long long>(U * kRows) + threadIdx.x / L;
-  int p[U], seq[U], slot[U];
-  long long t[U];
+// A warp takes G tokens side by side, a row of each per round, and of their
+// slots (k heads, v heads, then q heads) the rounds [part, part + 1) / parts: the
+// head is the same for the whole warp, and a row costs an addition.
+struct Split {
+  int parts, slots;
+};
+
+// Word j of an array that starts anywhere, and element j of such words.
+__device__ __forceinline__ uint32_t word_at(const float* p, int j) { return __float_as_uint(p[j]); }
+template <typename T>
+__device__ __forceinline__ uint32_t word_at(const T* p, int j) {
+  const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+  return h[2 * j] | static_cast<uint32_t>(h[2 * j + 1]) << 16;
+}
+__device__ __forceinline__ float element(const float*, const uint32_t (&w)[8], int j) { return __uint_as_float(w[j]); }
+__device__ __forceinline__ float element(const __nv_bfloat16*, const uint32_t (&w)[4], int j) {
+  return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+}
+__device__ __forceinline__ float element(const __half*, const uint32_t (&w)[4], int j) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(w[j / 2] >> (j % 2 * 16))));
+}
+
+// The largest |x| of a lane's values, two at a time where they have 16 bits; a
+// NaN wins.
+__device__ __forceinline__ uint32_t max_two(const float*, uint32_t a, uint32_t b) {
+  return max(a, b);  // absolute values compare like their bits, and NaN is above infinity
+}
+__device__ __forceinline__ uint32_t max_two(const __nv_bfloat16*, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_two(const __half*, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <typename T, int W>
+__device__ __forceinline__ uint32_t top_of(const T* tag, const uint32_t (&w)[W]) {
+  constexpr uint32_t kAbs = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  uint32_t m = w[0] & kAbs;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long r = r0 + u * kRows;
-    t[u] = r >> 32 ? r / slots : static_cast<uint32_t>(r) / static_cast<uint32_t>(slots);
-    slot[u] = static_cast<int>(r - t[u] * slots);
-    p[u] = seq[u] = -1;
-    if (r < rows) {
-      p[u] = a.pos[t[u]];
-      seq[u] = a.seq[t[u]];
-    } else {
-      t[u] = -1;
-    }
-  }
-  tb::Packed<T, 4> x0[U], x1[U];
-  long long row[U];
+  for (int i = 1; i < W; ++i) m = max_two(tag, m, w[i] & kAbs);
+  return m;
+}
+// ... as the bits of an fp32 number
+__device__ __forceinline__ uint32_t top_bits(const float*, uint32_t m) { return m; }
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const T*, uint32_t m) {
+  const unsigned short h = static_cast<unsigned short>(max(m & 0xffffu, m >> 16));
+  return __float_as_uint(tb::to_f32(*reinterpret_cast<const T*>(&h)));
+}
+
+// Rows as they come: D / 8 lanes per row, eight neighbouring elements each, four
+// heads in flight.  The four rows are reduced together (5 shuffles at D = 128, 16
+// apart), and the two divisions of a row are done once per lane.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
+  constexpr int L = D / 8, G = 32 / L, U = 4, W = 2 * sizeof(T);  // lanes per row, tokens, rounds in flight, words
+  const T* tag = nullptr;
+  const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
+  const long long item = blockIdx.x * 8ll + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
+  const int row0 = t < a.T ? static_cast<int>(slot_row(a.cache, a.seq[t], a.pos[t], l == 0 ? a.rot.err : nullptr)) : -1;
+  if (!__any_sync(0xffffffffu, row0 >= 0)) return;
+  const T* kp = static_cast<const T*>(a.k) + t * a.ks_t + 8 * l;
+  const T* vp = static_cast<const T*>(a.v) + t * a.vs_t + 8 * l;
+  const int part = static_cast<int>(item - group * sp.parts), batches = (sp.slots + U - 1) / U;
+  const int hi_slot = min((part + 1) * batches / sp.parts * U, sp.slots);
+  for (int s0 = part * batches / sp.parts * U; s0 < hi_slot; s0 += U) {
+    uint32_t x[U][W], m[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int kind = slot[u] < Hk ? 0 : slot[u] < 2 * Hk ? 1 : 2, h = slot[u] - kind * Hk;  // k, v, q
-    const bool turn = ROT && kind != 1 && 8 * l < R, half = turn && !a.rot.interleaved;
-    const int o1 = half ? 4 * l : 8 * l, o2 = half ? 4 * l + R / 2 : 8 * l + 4;
-    const bool past = ROT && p[u] >= a.rot.max_pos;
-    const T* x = kind == 0   ? static_cast<const T*>(a.k) + t[u] * a.ks_t + h * a.ks_h
-                 : kind == 1 ? static_cast<const T*>(a.v) + t[u] * a.vs_t + h * a.vs_h
-                             : static_cast<const T*>(a.rot.x) + t[u] * a.rot.xs_t + h * a.rot.xs_h;
-    const bool need = t[u] >= 0 && (kind == 2 || (p[u] >= 0 && seq[u] >= 0));
-    if (need && aligned) {
-      x0[u].load(x + o1);
-      x1[u].load(x + o2);
-    } else if (need) {
-      T* e0 = reinterpret_cast<T*>(&x0[u].raw);
-      T* e1 = reinterpret_cast<T*>(&x1[u].raw);
+    for (int u = 0; u < U; ++u) {
+      const int slot = s0 + u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e0[i] = x[o1 + i];
-        e1[i] = x[o2 + i];
+      for (int j = 0; j < W; ++j) x[u][j] = 0;
+      if (slot < hi_slot && row0 >= 0) {
+        const T* p = slot < Hk ? kp + slot * a.ks_h : vp + (slot - Hk) * a.vs_h;
+        if (aligned) {
+#pragma unroll
+          for (int j = 0; j < W; j += 4) {
+            const uint4 y = reinterpret_cast<const uint4*>(p)[j / 4];
+            x[u][j] = y.x;
+            x[u][j + 1] = y.y;
+            x[u][j + 2] = y.z;
+            x[u][j + 3] = y.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < W; ++j) x[u][j] = word_at(p, j);
+        }
       }
-    } else {
-      x0[u].raw = x1[u].raw = {};
     }
-    row[u] = -1;
-    if (need && kind < 2 && !past) row[u] = slot_row(a.cache, seq[u], p[u], l == 0 ? a.rot.err : nullptr);
-    if (row[u] >= 0) row[u] += static_cast<long long>(h) * a.cache.bs;
-  }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int kind = slot[u] < Hk ? 0 : slot[u] < 2 * Hk ? 1 : 2, h = slot[u] - kind * Hk;
-    const bool turn = ROT && kind != 1 && 8 * l < R, half = turn && !a.rot.interleaved;
-    const int o1 = half ? 4 * l : 8 * l, o2 = half ? 4 * l + R / 2 : 8 * l + 4;
-    const bool past = ROT && p[u] >= a.rot.max_pos;
-    float f[4], g[4];
-    x0[u].unpack(f);
-    x1[u].unpack(g);
-    if (turn && p[u] >= 0 && !past) {
-      const float2* tab = reinterpret_cast<const float2*>(a.rot.table) + static_cast<long long>(p[u]) * (R / 2) + 4 * l;
+    for (int u = 0; u < U; ++u) m[u] = top_of(tag, x[u]);
+    // reduce and deal out: a quarter of a row's lanes ends with the maximum of one of the four rows each
+    const bool hi = l & L / 2, mid = l & L / 4;
+    uint32_t m0 = hi ? m[2] : m[0], m1 = hi ? m[3] : m[1];
+    m0 = max_two(tag, m0, __shfl_xor_sync(0xffffffffu, hi ? m[0] : m[2], L / 2));
+    m1 = max_two(tag, m1, __shfl_xor_sync(0xffffffffu, hi ? m[1] : m[3], L / 2));
+    uint32_t top = max_two(tag, mid ? m1 : m0, __shfl_xor_sync(0xffffffffu, mid ? m0 : m1, L / 4));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 cs = tab[i];
-        float& v = half ? f[i] : i < 2 ? f[2 * i] : g[2 * i - 4];
-        float& w = half ? g[i] : i < 2 ? f[2 * i + 1] : g[2 * i - 3];
-        const float nv = v * cs.x - w * cs.y;
-        w = w * cs.x + v * cs.y;
-        v = nv;
-      }
+    for (int o = L / 8; o > 0; o >>= 1) top = max_two(tag, top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float amax = __uint_as_float(max(top_bits(tag, top), kMinAmaxBits)), inv = __fdiv_rn(kMaxCode, amax);
+    const int own = s0 + (hi ? 2 : 0) + (mid ? 1 : 0);  // the slot of this lane's maximum
+    if (l % (L / 4) == 0 && own < hi_slot && row0 >= 0)
+      (own < Hk ? a.cache.ks + own * a.cache.bs : a.cache.vs + (own - Hk) * a.cache.bs)[row0] = __fdiv_rn(amax, kMaxCode);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int slot = s0 + u;
+      const float f = __shfl_sync(0xffffffffu, inv, (lane & ~(L - 1)) + (u / 2) * (L / 2) + (u % 2) * (L / 4));
+      if (slot >= hi_slot || row0 < 0) continue;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = element(tag, x[u], j) * f;
+      uint8_t* c = slot < Hk ? static_cast<uint8_t*>(a.cache.kc) + static_cast<long long>(slot) * a.cache.bs * D
+                             : static_cast<uint8_t*>(a.cache.vc) + static_cast<long long>(slot - Hk) * a.cache.bs * D;
+      *reinterpret_cast<uint2*>(c + static_cast<long long>(row0) * D + 8 * l) =
+          make_uint2(to_e4m3x4(v[0], v[1], v[2], v[3]), to_e4m3x4(v[4], v[5], v[6], v[7]));
     }
-    // absolute values compare like their bits, and NaN is above infinity
-    uint32_t m = kMinAmaxBits;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, max(__float_as_uint(f[i]) & 0x7fffffffu, __float_as_uint(g[i]) & 0x7fffffffu));
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (ROT && t[u] >= 0 && past && l == 0 && a.rot.err) atomicCAS(a.rot.err, 0, 1);
-    if (ROT && t[u] >= 0 && kind == 2) {
-      T* y = static_cast<T*>(a.rot.y) + t[u] * a.rot.ys_t + h * a.rot.ys_h;
-      if (past) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = g[i] = NAN;
-      }
-      store4<T>(y + o1, aligned, f);
-      store4<T>(y + o2, aligned, g);
-    }
-    if (row[u] < 0) continue;
-    const float amax = __uint_as_float(m), inv = __fdiv_rn(kMaxCode, amax);
-    uint8_t* c = static_cast<uint8_t*>(kind == 0 ? a.cache.kc : a.cache.vc) + row[u] * D;
-    const uint32_t c0 = to_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-    const uint32_t c1 = to_e4m3x4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
-    if (ROT) {
-      *reinterpret_cast<uint32_t*>(c + o1) = c0;
-      *reinterpret_cast<uint32_t*>(c + o2) = c1;
-    } else {
-      *reinterpret_cast<uint2*>(c + o1) = make_uint2(c0, c1);
-    }
-    if (l == 0) (kind == 0 ? a.cache.ks : a.cache.vs)[row[u]] = __fdiv_rn(amax, kMaxCode);
   }
 }
 
-// D / 16 lanes per row, sixteen codes each, U rows per lane.
-template <typename T, int D, int U>
-__global__ void __launch_bounds__(256) kv_quant_read_kernel(TbKvQuantReadArgs a, bool aligned) {
-  constexpr int L = D / 16, kRows = 256 / L;
-  const int l = threadIdx.x % L, Hk = a.cache.Hk, slots = 2 * Hk;
-  const long long rows = static_cast<long long>(a.T) * slots;
-  const long long r0 = blockIdx.x * static_cast<long long>(U * kRows) + threadIdx.x / L;
-  long long t[U], row[U];
-  int slot[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long r = r0 + u * kRows;
-    t[u] = r >> 32 ? r / slots : static_cast<uint32_t>(r) / static_cast<uint32_t>(slots);
-    slot[u] = static_cast<int>(r - t[u] * slots);
-    row[u] = -1;
-    if (r < rows) row[u] = slot_row(a.cache, a.seq[t[u]], a.pos[t[u]], l == 0 ? a.err : nullptr);
-    if (row[u] >= 0) row[u] += static_cast<long long>(slot[u] < Hk ? slot[u] : slot[u] - Hk) * a.cache.bs;
+// One token's q and k rows rotated first: G heads of it per round, its table
+// entries in registers for all of them.  A lane holds both members of its pairs
+// (half layout: two vectors of four), else eight neighbours.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_quant_write_rot_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
+  constexpr int L = D / 8, G = 32 / L, U = 2;
+  const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk, R = a.rot.R;
+  const long long item = blockIdx.x * 8ll + threadIdx.x / 32, t = item / sp.parts;
+  if (t >= a.T) return;
+  const int part = static_cast<int>(item - t * sp.parts), rounds = (sp.slots + G - 1) / G;
+  const int lo = part * rounds / sp.parts, hi = (part + 1) * rounds / sp.parts;
+  const int p = a.pos[t];
+  const bool past = p >= a.rot.max_pos, turn = 8 * l < R, half = turn && !a.rot.interleaved;
+  float cs[8];
+  if (turn && p >= 0 && !past) tb::load_vec<float, 8>(a.rot.table + (static_cast<long long>(p) * (R / 2) + 4 * l) * 2, cs);
+  int base = -1;
+  if (past) {
+    if (a.rot.err && lane == 0) atomicCAS(a.rot.err, 0, 1);
+  } else {
+    base = static_cast<int>(slot_row(a.cache, a.seq[t], p, lane == 0 ? a.rot.err : nullptr));
   }
-  uint4 w[U];
-  float s[U];
+  for (int i = lo; i < hi; i += U) {
+    tb::Packed<T, 4> x0[U], x1[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (row[u] >= 0) {
-      w[u] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(slot[u] < Hk ? a.cache.kc : a.cache.vc) +
-                                             row[u] * D + 16 * l);
-      s[u] = (slot[u] < Hk ? a.cache.ks : a.cache.vs)[row[u]];
+    for (int u = 0; u < U; ++u) {
+      const int slot = (i + u) * G + lane / L, kind = slot < Hk ? 0 : slot < 2 * Hk ? 1 : 2, h = slot - kind * Hk;
+      const bool pairs = half && kind != 1;
+      const T* x = kind == 0   ? static_cast<const T*>(a.k) + t * a.ks_t + h * a.ks_h
+                   : kind == 1 ? static_cast<const T*>(a.v) + t * a.vs_t + h * a.vs_h
+                               : static_cast<const T*>(a.rot.x) + t * a.rot.xs_t + h * a.rot.xs_h;
+      const int o1 = pairs ? 4 * l : 8 * l, o2 = pairs ? 4 * l + R / 2 : 8 * l + 4;
+      x0[u].raw = x1[u].raw = {};
+      if (i + u < hi && slot < sp.slots && (kind == 2 || base >= 0)) {
+        if (aligned) {
+          x0[u].load(x + o1);
+          x1[u].load(x + o2);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            reinterpret_cast<T*>(&x0[u].raw)[j] = x[o1 + j];
+            reinterpret_cast<T*>(&x1[u].raw)[j] = x[o2 + j];
+          }
+        }
+      }
     }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (row[u] < 0) continue;
-    T* y = (slot[u] < Hk ? static_cast<T*>(a.k) + t[u] * a.ks_t + slot[u] * a.ks_h
-                         : static_cast<T*>(a.v) + t[u] * a.vs_t + (slot[u] - Hk) * a.vs_h) +
-           16 * l;
-    const uint32_t ww[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-    float f[16];
+    for (int u = 0; u < U; ++u) {
+      const int slot = (i + u) * G + lane / L, kind = slot < Hk ? 0 : slot < 2 * Hk ? 1 : 2, h = slot - kind * Hk;
+      const bool live = i + u < hi && slot < sp.slots, pairs = half && kind != 1;
+      const int o1 = pairs ? 4 * l : 8 * l, o2 = pairs ? 4 * l + R / 2 : 8 * l + 4;
+      float f[4], g[4];
+      x0[u].unpack(f);
+      x1[u].unpack(g);
+      if (turn && kind != 1 && p >= 0 && !past) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float q[4];
-      from_e4m3x4(ww[i], q);
+        for (int j = 0; j < 4; ++j) {
+          float& v = pairs ? f[j] : j < 2 ? f[2 * j] : g[2 * j - 4];
+          float& w = pairs ? g[j] : j < 2 ? f[2 * j + 1] : g[2 * j - 3];
+          const float nv = v * cs[2 * j] - w * cs[2 * j + 1];
+          w = w * cs[2 * j] + v * cs[2 * j + 1];
+          v = nv;
+        }
+      }
+      uint32_t m = kMinAmaxBits;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[4 * i + e] = q[e] * s[u];
+      for (int j = 0; j < 4; ++j)
+        m = max(m, max(__float_as_uint(f[j]) & 0x7fffffffu, __float_as_uint(g[j]) & 0x7fffffffu));
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (live && kind == 2) {
+        T* y = static_cast<T*>(a.rot.y) + t * a.rot.ys_t + h * a.rot.ys_h;
+        if (past) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] = g[j] = NAN;
+        }
+        store4<T>(y + o1, aligned, f);
+        store4<T>(y + o2, aligned, g);
+      } else if (live && base >= 0) {
+        const long long row = base + static_cast<long long>(h) * a.cache.bs;
+        const float amax = __uint_as_float(m), inv = __fdiv_rn(kMaxCode, amax);
+        uint8_t* c = static_cast<uint8_t*>(kind == 0 ? a.cache.kc : a.cache.vc) + row * D;
+        *reinterpret_cast<uint32_t*>(c + o1) = to_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+        *reinterpret_cast<uint32_t*>(c + o2) = to_e4m3x4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
+        if (l == 0) (kind == 0 ? a.cache.ks : a.cache.vs)[row] = __fdiv_rn(amax, kMaxCode);
+      }
     }
-    if (aligned) {
-      tb::store_vec<T, 16>(y, f);
-    } else {
+  }
+}
+
+// D / 16 lanes per row, sixteen codes each, four heads in flight.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_quant_read_kernel(TbKvQuantReadArgs a, Split sp, bool aligned) {
+  constexpr int L = D / 16, G = 32 / L, U = 4;
+  const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
+  const long long item = blockIdx.x * 8ll + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
+  if (t >= a.T) return;
+  const int row0 = static_cast<int>(slot_row(a.cache, a.seq[t], a.pos[t], l == 0 ? a.err : nullptr));
+  if (row0 < 0) return;
+  const uint8_t* kc = static_cast<const uint8_t*>(a.cache.kc) + static_cast<long long>(row0) * D + 16 * l;
+  const uint8_t* vc = static_cast<const uint8_t*>(a.cache.vc) + static_cast<long long>(row0) * D + 16 * l;
+  T* kp = static_cast<T*>(a.k) + t * a.ks_t + 16 * l;
+  T* vp = static_cast<T*>(a.v) + t * a.vs_t + 16 * l;
+  const int part = static_cast<int>(item - group * sp.parts), batches = (sp.slots + U - 1) / U;
+  const int hi_slot = min((part + 1) * batches / sp.parts * U, sp.slots);
+  for (int s0 = part * batches / sp.parts * U; s0 < hi_slot; s0 += U) {
+    uint4 w[U];
+    float s[U];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = tb::from_f32<T>(f[i]);
+    for (int u = 0; u < U; ++u) {
+      const int slot = s0 + u, h = slot < Hk ? slot : slot - Hk;
+      if (slot >= hi_slot) continue;
+      w[u] = *reinterpret_cast<const uint4*>((slot < Hk ? kc : vc) + static_cast<long long>(h) * a.cache.bs * D);
+      s[u] = ((slot < Hk ? a.cache.ks : a.cache.vs) + h * a.cache.bs)[row0];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int slot = s0 + u;
+      if (slot >= hi_slot) continue;
+      T* y = slot < Hk ? kp + slot * a.ks_h : vp + (slot - Hk) * a.vs_h;
+      const uint32_t ww[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+      float f[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float q[4];
+        from_e4m3x4(ww[j], q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * j + e] = q[e] * s[u];
+      }
+      if (aligned) {
+        tb::store_vec<T, 16>(y, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = tb::from_f32<T>(f[j]);
+      }
     }
   }
 }
@@ -235,45 +336,47 @@ bool rows_aligned(const void* p, long long st, long long sh, int dtype, int byte
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && st * e % bytes == 0 && sh * e % bytes == 0;
 }
 
-// Rows per lane: as many as leave every SM 2,048 threads, at most four.
-constexpr long long kFullMachine = 148 * 2048;
+// Warps that share the slots of their tokens: as long as that leaves each four
+// rounds, or (few tokens: latency counts) fills 16 warps per SM.
+int parts_of(long long groups, int rounds) {
+  int n = 1;
+  while (2 * n <= rounds && 2 * n * groups <= 148 * 16) n *= 2;
+  return n;
+}
+int blocks_of(long long warps) { return static_cast<int>((warps + 7) / 8); }
 
-template <typename T, int D, bool ROT>
-int write_rot(const TbKvQuantWriteArgs& a, cudaStream_t s) {
-  constexpr int kRows = 256 / (D / 8);
-  const int slots = 2 * a.cache.Hk + (a.rot.x ? a.rot.H : 0), v = 4 * (a.rot.dtype == TB_F32 ? 4 : 2);
+template <typename T, int D>
+int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
+  constexpr int G = 32 / (D / 8);  // rows per warp and round
+  const bool rot = a.rot.R > 0;
+  const int v = rot ? 4 * static_cast<int>(sizeof(T)) : 16;
   bool al = rows_aligned(a.k, a.ks_t, a.ks_h, a.rot.dtype, v) && rows_aligned(a.v, a.vs_t, a.vs_h, a.rot.dtype, v);
-  if (a.rot.x)
+  Split sp = {1, 2 * a.cache.Hk};
+  if (!rot) {
+    const long long groups = (a.T + G - 1ll) / G;
+    sp.parts = parts_of(groups, (sp.slots + 3) / 4);
+    kv_quant_write_kernel<T, D><<<blocks_of(groups * sp.parts), 256, 0, s>>>(a, sp, al);
+    return static_cast<int>(cudaGetLastError());
+  }
+  if (a.rot.x) {
+    sp.slots += a.rot.H;
     al = al && rows_aligned(a.rot.x, a.rot.xs_t, a.rot.xs_h, a.rot.dtype, v) &&
          rows_aligned(a.rot.y, a.rot.ys_t, a.rot.ys_h, a.rot.dtype, v);
-  const long long rows = static_cast<long long>(a.T) * slots;
-  const int u = rows * (D / 8) >= 4 * kFullMachine ? 4 : 1;
-  const long long grid = (rows + u * kRows - 1) / (u * kRows);
-  if (grid > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
-  if (u == 4)
-    kv_quant_write_kernel<T, D, 4, ROT><<<static_cast<int>(grid), 256, 0, s>>>(a, slots, al);
-  else
-    kv_quant_write_kernel<T, D, 1, ROT><<<static_cast<int>(grid), 256, 0, s>>>(a, slots, al);
+  }
+  al = al && reinterpret_cast<uintptr_t>(a.rot.table) % 16 == 0;
+  sp.parts = parts_of(a.T, (sp.slots + G - 1) / G);
+  kv_quant_write_rot_kernel<T, D><<<blocks_of(static_cast<long long>(a.T) * sp.parts), 256, 0, s>>>(a, sp, al);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T, int D>
-int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
-  return a.rot.R > 0 ? write_rot<T, D, true>(a, s) : write_rot<T, D, false>(a, s);
-}
-
-template <typename T, int D>
 int read_as(const TbKvQuantReadArgs& a, cudaStream_t s) {
-  constexpr int kRows = 256 / (D / 16);
+  constexpr int G = 32 / (D / 16);
   const bool al = rows_aligned(a.k, a.ks_t, a.ks_h, a.dtype, 16) && rows_aligned(a.v, a.vs_t, a.vs_h, a.dtype, 16);
-  const long long rows = static_cast<long long>(a.T) * 2 * a.cache.Hk;
-  const int u = rows * (D / 16) >= 4 * kFullMachine ? 4 : 1;
-  const long long grid = (rows + u * kRows - 1) / (u * kRows);
-  if (grid > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
-  if (u == 4)
-    kv_quant_read_kernel<T, D, 4><<<static_cast<int>(grid), 256, 0, s>>>(a, al);
-  else
-    kv_quant_read_kernel<T, D, 1><<<static_cast<int>(grid), 256, 0, s>>>(a, al);
+  const long long groups = (a.T + G - 1ll) / G;
+  Split sp = {1, 2 * a.cache.Hk};
+  sp.parts = parts_of(groups, (sp.slots + 3) / 4);
+  kv_quant_read_kernel<T, D><<<blocks_of(groups * sp.parts), 256, 0, s>>>(a, sp, al);
   return static_cast<int>(cudaGetLastError());
 }
 
