@@ -131,26 +131,27 @@ __global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs 
   constexpr int L = D / 8, G = 32 / L, U = 4, W = 2 * sizeof(T);  // lanes per row, tokens, rounds in flight, words
   const T* tag = nullptr;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
-  const long long item = blockIdx.x * 8ll + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
-  const int row0 = t < a.T ? static_cast<int>(slot_row(a.cache, a.seq[t], a.pos[t], l == 0 ? a.rot.err : nullptr)) : -1;
-  if (!__any_sync(0xffffffffu, row0 >= 0)) return;
+  const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
+  const int p = t < a.T ? a.pos[t] : -1, seq = t < a.T ? a.seq[t] : -1;
+  const bool need = p >= 0 && seq >= 0;  // (the rows are loaded while their slots are still looked up)
+  if (!__any_sync(0xffffffffu, need)) return;
+  const int row0 = static_cast<int>(slot_row(a.cache, seq, p, l == 0 ? a.rot.err : nullptr));
   const T* kp = static_cast<const T*>(a.k) + t * a.ks_t + 8 * l;
   const T* vp = static_cast<const T*>(a.v) + t * a.vs_t + 8 * l;
-  const int part = static_cast<int>(item - group * sp.parts), batches = (sp.slots + U - 1) / U;
-  const int hi_slot = min((part + 1) * batches / sp.parts * U, sp.slots);
-  for (int s0 = part * batches / sp.parts * U; s0 < hi_slot; s0 += U) {
+  const int part = static_cast<int>(item - group * sp.parts), hi_slot = (part + 1) * sp.slots / sp.parts;
+  for (int s0 = part * sp.slots / sp.parts; s0 < hi_slot; s0 += U) {
     uint32_t x[U][W], m[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int slot = s0 + u;
 #pragma unroll
       for (int j = 0; j < W; ++j) x[u][j] = 0;
-      if (slot < hi_slot && row0 >= 0) {
-        const T* p = slot < Hk ? kp + slot * a.ks_h : vp + (slot - Hk) * a.vs_h;
+      if (slot < hi_slot && need) {
+        const T* row = slot < Hk ? kp + slot * a.ks_h : vp + (slot - Hk) * a.vs_h;
         if (aligned) {
 #pragma unroll
           for (int j = 0; j < W; j += 4) {
-            const uint4 y = reinterpret_cast<const uint4*>(p)[j / 4];
+            const uint4 y = reinterpret_cast<const uint4*>(row)[j / 4];
             x[u][j] = y.x;
             x[u][j + 1] = y.y;
             x[u][j + 2] = y.z;
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs 
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < W; ++j) x[u][j] = word_at(p, j);
+          for (int j = 0; j < W; ++j) x[u][j] = word_at(row, j);
         }
       }
     }
@@ -199,11 +200,11 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_quant_write_rot_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
   constexpr int L = D / 8, G = 32 / L, U = 2;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk, R = a.rot.R;
-  const long long item = blockIdx.x * 8ll + threadIdx.x / 32, t = item / sp.parts;
+  const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, t = item / sp.parts;
   if (t >= a.T) return;
   const int part = static_cast<int>(item - t * sp.parts), rounds = (sp.slots + G - 1) / G;
   const int lo = part * rounds / sp.parts, hi = (part + 1) * rounds / sp.parts;
-  const int p = a.pos[t];
+  const int p = a.pos[t], seq = a.seq[t];
   const bool past = p >= a.rot.max_pos, turn = 8 * l < R, half = turn && !a.rot.interleaved;
   float cs[8];
   if (turn && p >= 0 && !past) tb::load_vec<float, 8>(a.rot.table + (static_cast<long long>(p) * (R / 2) + 4 * l) * 2, cs);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(256) kv_quant_write_rot_kernel(TbKvQuantWriteA
   if (past) {
     if (a.rot.err && lane == 0) atomicCAS(a.rot.err, 0, 1);
   } else {
-    base = static_cast<int>(slot_row(a.cache, a.seq[t], p, lane == 0 ? a.rot.err : nullptr));
+    base = static_cast<int>(slot_row(a.cache, seq, p, lane == 0 ? a.rot.err : nullptr));
   }
   for (int i = lo; i < hi; i += U) {
     tb::Packed<T, 4> x0[U], x1[U];
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(256) kv_quant_write_rot_kernel(TbKvQuantWriteA
                                : static_cast<const T*>(a.rot.x) + t * a.rot.xs_t + h * a.rot.xs_h;
       const int o1 = pairs ? 4 * l : 8 * l, o2 = pairs ? 4 * l + R / 2 : 8 * l + 4;
       x0[u].raw = x1[u].raw = {};
-      if (i + u < hi && slot < sp.slots && (kind == 2 || base >= 0)) {
+      if (i + u < hi && slot < sp.slots && (kind == 2 || (p >= 0 && seq >= 0))) {
         if (aligned) {
           x0[u].load(x + o1);
           x1[u].load(x + o2);
@@ -286,7 +287,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_quant_read_kernel(TbKvQuantReadArgs a, Split sp, bool aligned) {
   constexpr int L = D / 16, G = 32 / L, U = 4;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
-  const long long item = blockIdx.x * 8ll + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
+  const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
   if (t >= a.T) return;
   const int row0 = static_cast<int>(slot_row(a.cache, a.seq[t], a.pos[t], l == 0 ? a.err : nullptr));
   if (row0 < 0) return;
@@ -294,9 +295,8 @@ __global__ void __launch_bounds__(256) kv_quant_read_kernel(TbKvQuantReadArgs a,
   const uint8_t* vc = static_cast<const uint8_t*>(a.cache.vc) + static_cast<long long>(row0) * D + 16 * l;
   T* kp = static_cast<T*>(a.k) + t * a.ks_t + 16 * l;
   T* vp = static_cast<T*>(a.v) + t * a.vs_t + 16 * l;
-  const int part = static_cast<int>(item - group * sp.parts), batches = (sp.slots + U - 1) / U;
-  const int hi_slot = min((part + 1) * batches / sp.parts * U, sp.slots);
-  for (int s0 = part * batches / sp.parts * U; s0 < hi_slot; s0 += U) {
+  const int part = static_cast<int>(item - group * sp.parts), hi_slot = (part + 1) * sp.slots / sp.parts;
+  for (int s0 = part * sp.slots / sp.parts; s0 < hi_slot; s0 += U) {
     uint4 w[U];
     float s[U];
 #pragma unroll
@@ -336,14 +336,20 @@ bool rows_aligned(const void* p, long long st, long long sh, int dtype, int byte
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && st * e % bytes == 0 && sh * e % bytes == 0;
 }
 
-// Warps that share the slots of their tokens: as long as that leaves each four
-// rounds, or (few tokens: latency counts) fills 16 warps per SM.
+// Warps that share the rounds of their tokens (few tokens: latency counts), as
+// many as fill 16 warps per SM (512 tokens of 16 rows: 3.7 us so, 4.6 with 8 or 32);
+// in blocks of two warps, over more SMs, where there are few.
+constexpr int kFewWarps = 148 * 16, kSpread = 148 * 8;
 int parts_of(long long groups, int rounds) {
   int n = 1;
-  while (2 * n <= rounds && 2 * n * groups <= 148 * 16) n *= 2;
+  while (2 * n <= rounds && 2 * n * groups <= kFewWarps) n *= 2;
   return n;
 }
-int blocks_of(long long warps) { return static_cast<int>((warps + 7) / 8); }
+struct Shape {
+  int grid, block;
+  explicit Shape(long long warps)
+      : grid(static_cast<int>(warps <= kSpread ? (warps + 1) / 2 : (warps + 7) / 8)), block(warps <= kSpread ? 64 : 256) {}
+};
 
 template <typename T, int D>
 int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
@@ -354,8 +360,9 @@ int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
   Split sp = {1, 2 * a.cache.Hk};
   if (!rot) {
     const long long groups = (a.T + G - 1ll) / G;
-    sp.parts = parts_of(groups, (sp.slots + 3) / 4);
-    kv_quant_write_kernel<T, D><<<blocks_of(groups * sp.parts), 256, 0, s>>>(a, sp, al);
+    sp.parts = parts_of(groups, sp.slots);
+    const Shape g(groups * sp.parts);
+    kv_quant_write_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, al);
     return static_cast<int>(cudaGetLastError());
   }
   if (a.rot.x) {
@@ -365,7 +372,8 @@ int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
   }
   al = al && reinterpret_cast<uintptr_t>(a.rot.table) % 16 == 0;
   sp.parts = parts_of(a.T, (sp.slots + G - 1) / G);
-  kv_quant_write_rot_kernel<T, D><<<blocks_of(static_cast<long long>(a.T) * sp.parts), 256, 0, s>>>(a, sp, al);
+  const Shape g(static_cast<long long>(a.T) * sp.parts);
+  kv_quant_write_rot_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, al);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -375,8 +383,9 @@ int read_as(const TbKvQuantReadArgs& a, cudaStream_t s) {
   const bool al = rows_aligned(a.k, a.ks_t, a.ks_h, a.dtype, 16) && rows_aligned(a.v, a.vs_t, a.vs_h, a.dtype, 16);
   const long long groups = (a.T + G - 1ll) / G;
   Split sp = {1, 2 * a.cache.Hk};
-  sp.parts = parts_of(groups, (sp.slots + 3) / 4);
-  kv_quant_read_kernel<T, D><<<blocks_of(groups * sp.parts), 256, 0, s>>>(a, sp, al);
+  sp.parts = parts_of(groups, sp.slots);
+  const Shape g(groups * sp.parts);
+  kv_quant_read_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, al);
   return static_cast<int>(cudaGetLastError());
 }
 
