@@ -31,6 +31,7 @@ def main():
     ap.add_argument("--warmup", type=int, default=1)
     ap.add_argument("--prompts", type=int, default=64, help="prompts per rank")
     ap.add_argument("--group", type=int, default=8)
+    ap.add_argument("--kv-dtype", choices=["bf16", "fp8"], default="bf16", help="KV cache of the rollout")
     ap.add_argument("--prompt-len", type=int, default=256)
     ap.add_argument("--response-len", type=int, default=512)
     ap.add_argument("--micro-batch", type=int, default=8)
@@ -57,7 +58,7 @@ def main():
     rank = dist.get_rank() if world > 1 else 0
     cfg = GRPOConfig(model=LMConfig.tiny() if a.tiny else LMConfig.qwen2_1p5b(), num_prompts=a.prompts,
                      group_size=a.group, prompt_len=a.prompt_len, response_len=a.response_len,
-                     micro_batch=a.micro_batch)
+                     micro_batch=a.micro_batch, kv_dtype=a.kv_dtype)
     if a.tp > 1 and (world < 2 or world % a.tp):
         raise SystemExit("--tp needs a world size that is a multiple of it")
     tr = GRPOTrainer(cfg, str(dev), dp=dp, tp=a.tp, tp_mode=a.tp_mode)

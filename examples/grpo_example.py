@@ -53,6 +53,7 @@ def parse_args(argv=None):
     p.add_argument("--micro-batch", type=int, default=8)
     p.add_argument("--clip", type=float, default=0.2)
     p.add_argument("--seed", type=int, default=0)
+    p.add_argument("--kv-dtype", choices=["bf16", "fp8"], default="bf16", help="KV cache of the rollout")
     p.add_argument("--dp", choices=["fused", "nccl"], default="fused",
                    help="data-parallel gradient reduction when launched on several GPUs (torchrun)")
     p.add_argument("--tp", type=int, default=1, help="tensor-parallel group size (rollout and training)")
@@ -72,7 +73,8 @@ def main(argv=None):
              "llama3-8b": LMConfig.llama3_8b()}[args.model]
     cfg = GRPOConfig(model=model, num_prompts=args.num_prompts, group_size=args.group_size,
                      prompt_len=args.prompt_len, response_len=args.max_tokens, temperature=args.temperature,
-                     lr=args.lr, clip=args.clip, kl_coef=args.kl_coef, micro_batch=args.micro_batch, seed=args.seed)
+                     lr=args.lr, clip=args.clip, kl_coef=args.kl_coef, micro_batch=args.micro_batch, seed=args.seed,
+                     kv_dtype=args.kv_dtype)
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = 0
     if world > 1:  # launched by torchrun: one process per GPU, TP groups of --tp ranks, DP over the rest

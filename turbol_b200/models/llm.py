@@ -31,6 +31,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .._native import ops as _ops
+from ..ops.rotary import rotary, rotary_table
 
 ALIGN = 64  # elements; every parameter offset is 128-byte aligned in bf16
 
@@ -50,6 +51,17 @@ class LMConfig:
     qkv_bias: bool = True
     max_seq: int = 4096
     init_std: float = 0.02
+    # rotary positions other than the default (rotate-half over the whole head,
+    # unscaled): the rotated dimensions (a multiple of 8; None = head_dim), pairs
+    # of neighbours instead of halves, and a scaling for long contexts (the forms
+    # of ops.rotary.rotary_inv_freq)
+    rotary_dim: Optional[int] = None
+    rope_interleaved: bool = False
+    rope_scaling: Optional[dict] = None
+
+    @property
+    def rope_default(self) -> bool:
+        return self.rotary_dim in (None, self.head_dim) and not self.rope_interleaved and not self.rope_scaling
 
     @property
     def q_dim(self) -> int:
@@ -86,11 +98,27 @@ class LMConfig:
 
 
 def rope_table(cfg: LMConfig, device) -> torch.Tensor:
-    """[max_seq, head_dim/2, 2] fp32 (cos, sin) for rotate-half RoPE."""
+    """[max_seq, rotary_dim/2, 2] fp32 (cos, sin)."""
     D = cfg.head_dim
+    if not cfg.rope_default:
+        R = D if cfg.rotary_dim is None else cfg.rotary_dim
+        if R % 8 or not 0 < R <= D:
+            raise ValueError(f"rotary_dim: a multiple of 8 up to the head dimension {D}, not {R}")
+        return rotary_table(R, cfg.max_seq, cfg.rope_theta, cfg.rope_scaling, device)
     inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D, 2, dtype=torch.float64) / D))
     ang = torch.arange(cfg.max_seq, dtype=torch.float64)[:, None] * inv[None, :]
     return torch.stack([torch.cos(ang), torch.sin(ang)], -1).to(device=device, dtype=torch.float32).contiguous()
+
+
+def apply_rope(cfg: LMConfig, table: torch.Tensor, qkv: torch.Tensor, pos: torch.Tensor, heads: int,
+               inverse: bool = False):
+    """Rotates the first ``heads`` heads of fused QKV rows in place (inverse: the backward's rotation)."""
+    D = cfg.head_dim
+    if cfg.rope_default:
+        _ops().rope(qkv, pos, table, heads, D, inverse)
+    else:
+        x = qkv[:, : heads * D].unflatten(1, (heads, D))
+        rotary(x, pos, table, cfg.rope_interleaved, inverse, out=x)
 
 
 class DecoderLM:
@@ -254,7 +282,7 @@ class DecoderLM:
                 o.gemm(a["h1"], self.s[P + "wqkv"], qkv, bias=self.f32[P + "bqkv"], epi=o.EPI_BIAS)
             else:
                 o.gemm(a["h1"], self.s[P + "wqkv"], qkv)
-            o.rope(qkv, pos, self.table, cfg.n_heads + cfg.n_kv_heads, D)
+            apply_rope(cfg, self.table, qkv, pos, cfg.n_heads + cfg.n_kv_heads)
             if kv_hook is not None:
                 kv_hook(i, qkv)
             q, k, v = qkv[:, : cfg.q_dim], qkv[:, cfg.q_dim:cfg.q_dim + cfg.kv_dim], qkv[:, cfg.q_dim + cfg.kv_dim:]
@@ -324,7 +352,7 @@ class DecoderLM:
             dv = d_qkv[:, cfg.q_dim + cfg.kv_dim:]
             o.flash_attn_bwd(q, k, v, a["attn"], d_attn, a["lse"], delta, dq, dk, dv, B, T, cfg.n_heads,
                              cfg.n_kv_heads, scale, ws=attn_ws)
-            o.rope(d_qkv, pos, self.table, cfg.n_heads + cfg.n_kv_heads, D, True)   # inverse rotation
+            apply_rope(cfg, self.table, d_qkv, pos, cfg.n_heads + cfg.n_kv_heads, True)   # inverse rotation
             o.gemm(d_qkv, self.s[P + "wqkv"], dh, False, True)                      # dh1 = dQKV Wqkv
             o.gemm(d_qkv, a["h1"], G[P + "wqkv"], True, True, accumulate=True, split_k=1)  # dWqkv += dQKV^T h1
             if cfg.qkv_bias:

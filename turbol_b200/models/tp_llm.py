@@ -53,7 +53,7 @@ from typing import Optional
 import torch
 
 from .._native import ops as _ops
-from .llm import ALIGN, DecoderLM
+from .llm import ALIGN, DecoderLM, apply_rope
 
 
 class TPDecoderLM:
@@ -128,7 +128,7 @@ class TPDecoderLM:
             qkv = c.all_gather_gemm(h1, w[P + "wqkv"], bias=w[P + "bqkv"], epi=o.EPI_BIAS)
         else:
             qkv = c.all_gather_gemm(h1, w[P + "wqkv"])
-        o.rope(qkv, pos_full, self.table, self.hq + self.hk, cfg.head_dim)
+        apply_rope(cfg, self.table, qkv, pos_full, self.hq + self.hk)
         if kv_hook is not None:
             kv_hook(i, qkv)
         attn = torch.empty(N, self.q_dim, device=x.device, dtype=torch.bfloat16)
@@ -442,7 +442,7 @@ class TPTrainLM(TPDecoderLM):
             else:
                 c.all_gather_gemm(a["h1"], w[P + "wqkv"], out=a["qkv"], gather_out=a["h1f"])
             qkv = a["qkv"]
-            o.rope(qkv, pos_full, self.table, self.hq + self.hk, D)
+            apply_rope(cfg, self.table, qkv, pos_full, self.hq + self.hk)
             q, k, v = qkv[:, : self.q_dim], qkv[:, self.q_dim:self.q_dim + self.kv_dim], qkv[:, self.q_dim + self.kv_dim:]
             o.flash_attn_fwd(q, k, v, a["attn"], a["lse"], B, T, self.hq, self.hk, scale)
             a["x2"] = c.gemm_reduce_scatter(a["attn"], w[P + "wo"], residual=x)
@@ -490,7 +490,7 @@ class TPTrainLM(TPDecoderLM):
             dv = d_qkv[:, self.q_dim + self.kv_dim:]
             o.flash_attn_bwd(q, k, v, a["attn"], d_attn, a["lse"], delta, dq, dk, dv, B, T, self.hq, self.hk, scale,
                              ws=attn_ws)
-            o.rope(d_qkv, pos_full, self.table, self.hq + self.hk, D, True)              # inverse rotation
+            apply_rope(cfg, self.table, d_qkv, pos_full, self.hq + self.hk, True)        # inverse rotation
             dh1 = c.gemm_reduce_scatter(d_qkv, w[P + "wqkv"], b_mn=True)                   # dh1_r = RS(dQKV Wqkv_r)
             o.gemm(d_qkv, a["h1f"], G[P + "wqkv"], True, True, accumulate=True, split_k=1)  # dWqkv_r += dQKV^T h1
             if cfg.qkv_bias:

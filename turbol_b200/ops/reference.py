@@ -164,7 +164,12 @@ def lm_forward_ref(model, ids, params=None):
         q = qkv[..., : cfg.q_dim].view(B, T, cfg.n_heads, D)
         k = qkv[..., cfg.q_dim:cfg.q_dim + cfg.kv_dim].view(B, T, cfg.n_kv_heads, D)
         v = qkv[..., cfg.q_dim + cfg.kv_dim:].view(B, T, cfg.n_kv_heads, D)
-        q, k = rope(q, pos, cfg.rope_theta), rope(k, pos, cfg.rope_theta)
+        if cfg.rope_default:
+            q, k = rope(q, pos, cfg.rope_theta), rope(k, pos, cfg.rope_theta)
+        else:
+            flat_pos = pos.repeat(B)
+            q, k = (rotary(x.reshape(B * T, -1, D), flat_pos, model.table, cfg.rope_interleaved).view(x.shape)
+                    for x in (q, k))
         a = causal_attention(q, k, v).reshape(B, T, cfg.q_dim)
         x = x + a @ P[p + "wo"].t()
         h = rmsnorm(x, P[p + "ln2"], cfg.rms_eps)

@@ -48,6 +48,7 @@ class GRPOConfig:
     kl_coef: float = 0.04
     micro_batch: int = 8  # sequences per forward/backward
     seed: int = 0
+    kv_dtype: str = "bf16"  # rollout KV cache: "bf16" or "fp8" (not with a tensor-parallel decode)
 
     @property
     def batch(self) -> int:
@@ -94,6 +95,10 @@ class GRPOTrainer:
         self.rollout_mode = rollout if tp > 1 and tp_mode == "train" else "local"
         if self.rollout_mode not in ("replica", "tp", "local"):
             raise ValueError(f"unknown rollout mode {rollout!r}")
+        if cfg.kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype: 'bf16' or 'fp8', not {cfg.kv_dtype!r}")
+        if cfg.kv_dtype != "bf16" and tp > 1 and self.rollout_mode != "replica":
+            raise ValueError("kv_dtype 'fp8' needs a rollout on whole models (tp=1, or rollout='replica')")
         self.sync = None
         self.device = torch.device(device)
         self.dp, self.group = dp, group
@@ -147,7 +152,8 @@ class GRPOTrainer:
             self.tpm = TPDecoderLM(self.model, self.comm)
             self.gen = TPLLMGenerator(self.tpm, cfg.batch, cfg.seq_len, seed=cfg.seed + 17 + 7919 * self.group_index)
         else:
-            self.gen = LLMGenerator(self.model, cfg.batch, cfg.seq_len, seed=cfg.seed + 17 + 7919 * self.rank)
+            self.gen = LLMGenerator(self.model, cfg.batch, cfg.seq_len, seed=cfg.seed + 17 + 7919 * self.rank,
+                                    kv_dtype=cfg.kv_dtype)
         self.stats = torch.zeros(4, device=self.device)
         self.step_count = 0
         self.last_times = {}
@@ -211,7 +217,8 @@ class GRPOTrainer:
             self.sync = TPReplicaSync(self.model, mesh.tp_group)
             self.sync()
             self.gen = LLMGenerator(self.sync.full, cfg.batch // tp, cfg.seq_len,
-                                    seed=cfg.seed + 17 + 7919 * self.group_index + 104729 * self.tp_rank)
+                                    seed=cfg.seed + 17 + 7919 * self.group_index + 104729 * self.tp_rank,
+                                    kv_dtype=cfg.kv_dtype)
         else:
             self.gen = TPLLMGenerator(self.model, cfg.batch, cfg.seq_len,
                                       seed=cfg.seed + 17 + 7919 * self.group_index)

@@ -54,6 +54,7 @@ class RLHFConfig:
     temperature: float = 1.0
     seed: int = 0
     recompute: bool = False     # activation recomputation in the pipeline stages
+    kv_dtype: str = "bf16"      # rollout KV cache: "bf16" or "fp8"
 
     @property
     def seq_len(self) -> int:
@@ -130,7 +131,7 @@ class PPORLHFTrainer:
         # bf16 rollout copy of the whole policy on every rank
         self.rollout = DecoderLM(cfg.model, self.device, seed=cfg.seed, master=False)
         self.gen = LLMGenerator(self.rollout, cfg.num_prompts // self.world, cfg.seq_len,
-                                seed=cfg.seed + 31 + 7919 * self.rank)
+                                seed=cfg.seed + 31 + 7919 * self.rank, kv_dtype=cfg.kv_dtype)
         self.step_count = 0
         self.sync_weights()
 

@@ -32,12 +32,24 @@ from typing import List, Optional
 import torch
 
 from .._native import core as _core, ops as _ops
-from ..models.llm import DecoderLM, LMConfig
+from ..models.llm import DecoderLM, LMConfig, apply_rope
+from ..ops.kv_cache import decode_attention_quant, kv_quant_read, kv_quant_write, quant_kv_cache
 
 
 class LLMGenerator:
+    """kv_dtype: "bf16", or "fp8" for e4m3 codes with a scale per token and KV
+    head (0.52 of the bytes at head dimension 128: more sequences or longer
+    contexts in the same memory, and less to read per decoded token).  Kernels
+    set ``kv_error`` [1] if they meet a cache index out of range (fp8)."""
+
+    kv_dtype = "bf16"
+
     def __init__(self, model: DecoderLM, max_batch: int, max_len: int, block_size: int = 16, seed: int = 0,
-                 cuda_graph: bool = True, decode_gemm: Optional[bool] = None, attn_split: int = 1):
+                 cuda_graph: bool = True, decode_gemm: Optional[bool] = None, attn_split: int = 1,
+                 kv_dtype: str = "bf16"):
+        if kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype: 'bf16' or 'fp8', not {kv_dtype!r}")
+        self.kv_dtype = kv_dtype
         self.m = model
         self.cfg = model.cfg
         self.device = model.device
@@ -62,11 +74,73 @@ class LLMGenerator:
         self.num_blocks = max_batch * self.blocks_per_seq + 1
         self.kv = _core().KVBlockManager(self.num_blocks, block_size)
         shape = (self.num_blocks, cfg.n_kv_heads, block_size, cfg.head_dim)
-        self.kc = [torch.empty(shape, device=self.device, dtype=torch.bfloat16) for _ in model.layers]
-        self.vc = [torch.empty(shape, device=self.device, dtype=torch.bfloat16) for _ in model.layers]
+        if kv_dtype == "fp8":
+            self.kvq = [quant_kv_cache(*shape, device=self.device) for _ in model.layers]
+            self.kv_error = torch.zeros(1, device=self.device, dtype=torch.int32)
+        else:
+            self.kc = [torch.empty(shape, device=self.device, dtype=torch.bfloat16) for _ in model.layers]
+            self.vc = [torch.empty(shape, device=self.device, dtype=torch.bfloat16) for _ in model.layers]
         self._graph = None
         self._graph_B = None
         self.calls = 0
+
+    # ------------------------------------------------------------ cache access
+    def _heads(self, qkv: torch.Tensor):
+        """The q, k and v heads of fused QKV rows, [T, heads, head_dim] views."""
+        cfg = self.cfg
+        x = qkv.unflatten(1, (cfg.n_heads + 2 * cfg.n_kv_heads, cfg.head_dim))
+        return x.split((cfg.n_heads, cfg.n_kv_heads, cfg.n_kv_heads), 1)
+
+    def _cache_rows(self, li: int, qkv, seq_of_tok, pos, table):
+        """Writes the k and v rows (already rotated) of a prefill into layer li's pages."""
+        cfg = self.cfg
+        if self.kv_dtype == "fp8":
+            _, k, v = self._heads(qkv)
+            kv_quant_write(k, v, seq_of_tok, pos, table, *self.kvq[li], error=self.kv_error)
+        else:
+            _ops().kv_write(qkv, cfg.q_dim, cfg.q_dim + cfg.kv_dim, seq_of_tok, pos, table, self.kc[li], self.vc[li],
+                            cfg.n_kv_heads, cfg.head_dim, self.bs)
+
+    def _copy_blocks(self, li: int, dst: torch.Tensor, src: torch.Tensor):
+        """Copies whole blocks of layer li."""
+        for t in self.kvq[li] if self.kv_dtype == "fp8" else (self.kc[li], self.vc[li]):
+            t = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+            t[dst] = t[src]
+
+    def _rope_write_attend(self, li: int, qkv, attn, st, scale: float):
+        """One decode token per sequence: rotary positions, its k and v into layer li's pages, attention over them."""
+        o, cfg, m = _ops(), self.cfg, self.m
+        D = cfg.head_dim
+        if self.kv_dtype == "fp8":
+            q, k, v = self._heads(qkv)
+            kv_quant_write(k, v, st["seq"], st["pos"], st["table"], *self.kvq[li], q=q, table=m.table,
+                           interleaved=cfg.rope_interleaved, q_out=q, error=self.kv_error)
+            decode_attention_quant(q, *self.kvq[li], st["table"], st["ctx"], scale,
+                                   out=attn.unflatten(1, (cfg.n_heads, D)), error=self.kv_error)
+            return
+        if cfg.rope_default:
+            o.rope_kv_write(qkv, st["pos"], m.table, cfg.n_heads, cfg.n_kv_heads, D, st["seq"], st["table"],
+                            self.kc[li], self.vc[li], self.bs)
+        else:
+            apply_rope(cfg, m.table, qkv, st["pos"], cfg.n_heads + cfg.n_kv_heads)
+            self._cache_rows(li, qkv, st["seq"], st["pos"], st["table"])
+        o.decode_attention(qkv, self.kc[li], self.vc[li], st["table"], st["ctx"], attn, cfg.n_heads,
+                           cfg.n_kv_heads, D, self.bs, scale, st["attn_split"], st.get("attn_part"),
+                           st.get("attn_cnt"))
+
+    def cached_kv(self, layer: int, seq: int, n: int):
+        """The first n cached (rotated) keys and values of sequence ``seq`` of the
+        last ``generate`` call, as attention sees them: two bf16 [n, kv_heads,
+        head_dim] tensors."""
+        li = self.m.layers.index(layer)
+        if not 0 <= seq < self.state["table"].shape[0] or not 0 <= n <= self.max_len:
+            raise ValueError("cached_kv: no such sequence or length")
+        pos = torch.arange(n, device=self.device, dtype=torch.int32)
+        if self.kv_dtype == "fp8":
+            return kv_quant_read(*self.kvq[li], torch.full_like(pos, seq), pos, self.state["table"],
+                                 error=self.kv_error)
+        blk, slot = self.state["table"][seq, (pos // self.bs).long()].long(), (pos % self.bs).long()
+        return self.kc[li][blk, :, slot], self.vc[li][blk, :, slot]
 
     def reset_graph(self):
         """Drops the captured decode step.  The capture holds the model's weight
@@ -131,11 +205,7 @@ class LLMGenerator:
                 o.gemm(h, m.s[P + "wqkv"], qkv, bias=m.f32[P + "bqkv"], epi=o.EPI_BIAS, **kw)
             else:
                 o.gemm(h, m.s[P + "wqkv"], qkv, **kw)
-            o.rope_kv_write(qkv, st["pos"], m.table, cfg.n_heads, cfg.n_kv_heads, D, st["seq"], st["table"],
-                            self.kc[li], self.vc[li], self.bs)
-            o.decode_attention(qkv, self.kc[li], self.vc[li], st["table"], st["ctx"], attn, cfg.n_heads,
-                               cfg.n_kv_heads, D, self.bs, scale, st["attn_split"], st.get("attn_part"),
-                               st.get("attn_cnt"))
+            self._rope_write_attend(li, qkv, attn, st, scale)
             if dg:
                 o.gemm_decode(attn, m.s[P + "wo"], x2, aux=x, epi=o.EPI_RESIDUAL)
                 o.rmsnorm_fwd(x2, m.f32[P + "ln2"], h, None, cfg.rms_eps)
@@ -213,7 +283,7 @@ class LLMGenerator:
         cfg, o = self.cfg, _ops()
         G = cfg.n_heads // cfg.n_kv_heads
         want = getattr(self, "attn_split", 1)
-        if want == 1 or self.bs != 16 or cfg.head_dim != 128 or G > 8 or cfg.n_heads % cfg.n_kv_heads:
+        if self.kv_dtype == "fp8" or want == 1 or self.bs != 16 or cfg.head_dim != 128 or G > 8 or cfg.n_heads % cfg.n_kv_heads:
             return {"attn_split": 1}
         n = int(o.decode_attention_splits(B, cfg.n_kv_heads)) if want == 0 else int(want)
         if n <= 1:
@@ -273,12 +343,9 @@ class LLMGenerator:
         # ---- prefill the P prompts once; K/V land in the shared prompt blocks
         pos = torch.arange(Lp, device=self.device, dtype=torch.int32).repeat(P)
         seq_of_tok = torch.arange(P, device=self.device, dtype=torch.int32).repeat_interleave(Lp)
-        kcs, vcs = self.kc, self.vc
 
         def hook(i, qkv):
-            li = m.layers.index(i)
-            o.kv_write(qkv, cfg.q_dim, cfg.q_dim + cfg.kv_dim, seq_of_tok, pos, pre_table, kcs[li], vcs[li],
-                       cfg.n_kv_heads, cfg.head_dim, self.bs)
+            self._cache_rows(m.layers.index(i), qkv, seq_of_tok, pos, pre_table)
 
         x = m.embed(prompts)
         x, _ = m.forward(x, P, Lp, pos, save=False, kv_hook=hook)
@@ -288,8 +355,7 @@ class LLMGenerator:
             src_blocks = pre_table[:, n_shared].long()
             dst_blocks = table[:, n_shared].long()
             for li in range(len(m.layers)):
-                kcs[li][dst_blocks] = kcs[li][src_blocks.repeat_interleave(G)]
-                vcs[li][dst_blocks] = vcs[li][src_blocks.repeat_interleave(G)]
+                self._copy_blocks(li, dst_blocks, src_blocks.repeat_interleave(G))
         # ---- decode state: first token sampled from the prompt's last position
         if self._graph is None or self._graph_B != (B, max_new):
             self.state = self._alloc_state(B, max_new)
@@ -367,6 +433,7 @@ class RolloutConfig:
     model: str = "tiny"  # "tiny" | "qwen2-1.5b" | "llama3-8b" (random-init architectures)
     device: str = "cuda:0"
     seed: int = 0
+    kv_dtype: str = "bf16"  # "bf16" | "fp8" (the native engine's KV cache)
 
 
 class RolloutEngine:
@@ -385,7 +452,8 @@ class RolloutEngine:
             cfg = {"tiny": LMConfig.tiny(vocab=512), "qwen2-1.5b": LMConfig.qwen2_1p5b(),
                    "llama3-8b": LMConfig.llama3_8b()}[c.model]
             model = DecoderLM(cfg, c.device, seed=c.seed, master=False)
-            self._gen = LLMGenerator(model, c.max_batch_size, min(cfg.max_seq, 4096), seed=c.seed)
+            self._gen = LLMGenerator(model, c.max_batch_size, min(cfg.max_seq, 4096), seed=c.seed,
+                                     kv_dtype=c.kv_dtype)
         elif c.inference_backend == "vllm":
             from ..vllm_inference import VLLMInferenceConfig, VLLMInferenceEngine
 
