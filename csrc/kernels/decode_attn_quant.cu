@@ -45,7 +45,7 @@ constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that
 constexpr int kWaveTiles = 64;  // tiles per CTA where there are more CTAs than fit at once
 constexpr int kMostWaves = 1;
 constexpr int kStart = 1;       // what beginning a (sequence, group) costs a warp, in tiles
-constexpr int kWholeTokens = 256;  // contexts that cannot be longer are not split
+constexpr int kMostCluster = 8;   // CTAs of a cluster (the portable bound)
 constexpr float kMinVsLog = -100.f;
 constexpr float kSlack = 8.f;   // the reference of the weights may lag behind their maximum by a factor of 2^8
 
@@ -135,7 +135,7 @@ struct Partials {
   __device__ static int4* record(float* ws, int grid, int c) {
     return reinterpret_cast<int4*>(ws + 2ll * grid * kSlot) + c;
   }
-  static size_t bytes(int grid) { return (2 * grid * kSlot + 4 * static_cast<size_t>(grid)) * 4; }
+  static size_t bytes(int grid) { return grid == 0 ? 0 : (2 * grid * kSlot + 4 * static_cast<size_t>(grid)) * 4; }
 };
 
 struct Geometry {
@@ -143,7 +143,7 @@ struct Geometry {
   int cap;         // tokens that a table row can name
   int shift;       // log2 of the page size, or -1
   int tile_pages;  // pages hold whole tiles
-  int whole;       // one CTA per (sequence, group), nothing to join
+  int cs;          // CTAs (a cluster) for each (sequence, group), or 0: work dealt out evenly
   int fit;         // CTAs that fit at once
 };
 
@@ -200,6 +200,133 @@ __device__ __forceinline__ void store_out4(T* p, bool aligned, float x, float y,
     p[2] = tb::from_f32<T>(z);
     p[3] = tb::from_f32<T>(w);
   }
+}
+
+// A value in the shared memory of CTA `rank` of the cluster, at the place that p has here.
+__device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  return d;
+}
+__device__ __forceinline__ float peer_load(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer_load4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Joins the parts of a (sequence, group) that a cluster shares: each CTA its
+// warps', then a warp of the cluster for each query head the CTAs', over
+// distributed shared memory.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, const Geometry& g, uint8_t* smem, int2* meta,
+                                             bool out4) {
+  using S = Smem<D, NT>;
+  constexpr int kHeads = S::kHeads, E = D / 32, V = E < 4 ? E : 4;
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32, rank = blockIdx.x % g.cs, seg = blockIdx.x / g.cs;
+  const int b = seg / g.HG, r = seg - b * g.HG, kh = r / g.NG, left = g.G - (r - kh * g.NG) * kHeads;
+  const int nh = min(left, kHeads), h0 = kh * g.G + g.G - left;
+  float* sum = reinterpret_cast<float*>(smem);  // the CTA's part, in the ring of warp 0 (drained)
+  __syncthreads();
+  for (int h = w; h < nh; h += kWarps) {
+    float m[kWarps], l[kWarps], M = -INFINITY, L = 0.f, o[E] = {};
+    const float* part[kWarps];
+    bool any = false;
+#pragma unroll
+    for (int p = 0; p < kWarps; ++p) {
+      part[p] = reinterpret_cast<const float*>(smem + kWarps * S::kRing + p * S::kPart);
+      const bool have = meta[2 * p].x >= 0;
+      any |= have;
+      m[p] = have ? part[p][kHeads * D + 2 * h] : -INFINITY;
+      l[p] = have ? part[p][kHeads * D + 2 * h + 1] : 0.f;
+      M = fmaxf(M, m[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < kWarps; ++p) {
+      const float f = m[p] == -INFINITY ? 0.f : exp2_fast(m[p] - M);
+      L += f * l[p];
+      if (meta[2 * p].x < 0) continue;
+#pragma unroll
+      for (int i = 0; i < E; i += V) {
+        float y[V];
+        tb::load_vec<float, V>(part[p] + h * D + i * 32 + lane * V, y);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[i + e] += f * y[e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; i += V) {
+      float y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = o[i + e];
+      tb::store_vec<float, V>(sum + h * D + i * 32 + lane * V, y);
+    }
+    if (lane == 0) *reinterpret_cast<float2*>(sum + kHeads * D + 2 * h) = make_float2(M, any ? L : -1.f);  // -1: no part
+  }
+  cluster_barrier();
+  for (int h = rank + g.cs * w; h < nh; h += g.cs * kWarps) {
+    float m = -INFINITY, l = -1.f;
+    if (lane < g.cs) {
+      const uint32_t at = peer_address(sum + kHeads * D + 2 * h, lane);
+      m = peer_load(at);
+      l = peer_load(at + 4);
+    }
+    if (!__any_sync(0xffffffffu, l != -1.f)) break;  // one warp had the whole context, and wrote it
+    float o[kMostCluster][E];
+#pragma unroll
+    for (int p = 0; p < kMostCluster; ++p) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[p][i] = 0.f;
+      if (p >= g.cs) continue;
+      const uint32_t at = peer_address(sum + h * D + lane * V, p);
+#pragma unroll
+      for (int i = 0; i < E; i += V) {
+        if constexpr (V == 4) {
+          const float4 y = peer_load4(at + i * 32 * 4);
+          o[p][i] = y.x;
+          o[p][i + 1] = y.y;
+          o[p][i + 2] = y.z;
+          o[p][i + 3] = y.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[p][i + e] = peer_load(at + e * 4);
+        }
+      }
+    }
+    const float M = tb::warp_max(m), f = m == -INFINITY ? 0.f : exp2_fast(m - M);
+    const float L = tb::warp_sum(f * l), inv = L == 0.f ? 0.f : 1.f / L;
+    float y[E] = {};
+#pragma unroll
+    for (int p = 0; p < kMostCluster; ++p) {
+      const float fp = __shfl_sync(0xffffffffu, f, p);
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] += fp * o[p][i];
+    }
+    T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
+#pragma unroll
+    for (int i = 0; i < E; i += V) {
+      float z[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[e] = y[i + e] * inv;
+      if (out4) {
+        tb::store_vec<T, V>(out + i * 32 + lane * V, z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[i * 32 + lane * V + e] = tb::from_f32<T>(z[e]);
+      }
+    }
+  }
+  cluster_barrier();  // nobody leaves while another still reads its shared memory
 }
 
 template <typename T, int D, int NT>
@@ -277,21 +404,23 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       off -= __shfl_sync(0xffffffffu, inc, 31);
     }
   };
-  if (g.whole) {
-    cur.b = blockIdx.x / g.HG;
-    cur.r = blockIdx.x % g.HG;
+  if (g.cs) {
+    const int seg = blockIdx.x / g.cs, part = blockIdx.x % g.cs * kWarps + w, parts = g.cs * kWarps;
+    cur.b = seg / g.HG;
+    cur.r = seg % g.HG;
     cur.tokens = tokens_of(a, g, cur.b);
     const int n = tiles(cur.tokens);
     if (a.err && threadIdx.x == 0 && a.ctx_len[cur.b] > g.cap) atomicCAS(a.err, 0, 1);
-    if (n == 0) {
+    if (n == 0) {  // (the whole cluster)
       T* o = static_cast<T*>(a.out) + static_cast<long long>(cur.b) * a.os_b;
       const int h0 = cur.r / g.NG * g.G + cur.r % g.NG * kHeads, left = g.G - cur.r % g.NG * kHeads;
-      for (int i = threadIdx.x; i < (left < kHeads ? left : kHeads) * D; i += kThreads)
-        o[static_cast<long long>(h0 + i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
+      if (part < kWarps)
+        for (int i = threadIdx.x; i < (left < kHeads ? left : kHeads) * D; i += kThreads)
+          o[static_cast<long long>(h0 + i / D) * a.os_h + i % D] = tb::from_f32<T>(0.f);
       return;
     }
-    cur.t = n * w / kWarps;
-    cur.end = n * (w + 1) / kWarps;
+    cur.t = static_cast<int>(static_cast<long long>(n) * part / parts);
+    cur.end = static_cast<int>(static_cast<long long>(n) * (part + 1) / parts);
     cur.rest = 0;
   } else {
     // prefix sums of the sequences' units: each thread a run of sequences
@@ -405,10 +534,31 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     }
     cp_commit();
   };
+  // q of a portion as it lies in memory: asked for before what stands between the portions
+  tb::Packed<T, 8> q_raw[NT][D / 32];
+  auto ask_q = [&]() {
+    const int h0 = cur.r / g.NG * g.G + cur.r % g.NG * kHeads, left = g.G - cur.r % g.NG * kHeads;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const T* q = static_cast<const T*>(a.q) + static_cast<long long>(cur.b) * a.qs_b +
+                   static_cast<long long>(h0 + (n * 8 + gq < left ? n * 8 + gq : 0)) * a.qs_h + tq * (D / 4);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        if (q8) {
+          q_raw[n][i].load(q + 8 * i);
+        } else {
+          const unsigned short* e = reinterpret_cast<const unsigned short*>(q + 8 * i);
+          q_raw[n][i].raw = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        }
+      }
+    }
+  };
+  bool going = cur.t < cur.end;
+  if (S::kQRegs && going) ask_q();
   look();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
-  if (!g.whole) {
+  if (!g.cs) {
     empty_rows(ctas);
     // which CTAs share the contexts at the two ends of this CTA's list (used by the merge, if they are split)
     if (w == 0) {
@@ -425,12 +575,13 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 
   // ---- portions of this warp, one (sequence, group) each
   int get = 0;
-  bool first_portion = true, going = cur.t < cur.end;
+  bool first_portion = true;
   while (going) {
     const int h0 = cur.r / g.NG * g.G + cur.r % g.NG * kHeads;  // first query head of the group
     const int left = g.G - cur.r % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
     // q as B fragments: lane (head gq, tq) holds, for k step (i, j), the dimensions (tq NCH + i) 16 + 4 j .. + 3, the
     // same that it reads of a K row.  A power of two per head brings them into fp16's range.
+    if (!S::kQRegs) ask_q();
     uint2 qf[S::kQRegs ? NT * (D / 16) : 1];
     float ch[NT][2], m[NT][2], l[NT][2], acc[2 * NW][NT][4];
 #pragma unroll
@@ -438,19 +589,12 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       float v[D / 4];
       uint32_t top = 0;
       const bool live = n * 8 + gq < nh;
-      const T* q = static_cast<const T*>(a.q) + static_cast<long long>(cur.b) * a.qs_b +
-                   static_cast<long long>(h0 + (live ? n * 8 + gq : 0)) * a.qs_h + tq * (D / 4);
-      if (q8) {
 #pragma unroll
-        for (int i = 0; i < D / 4; i += 8) {
-          float f[8];
-          tb::load_vec<T, 8>(q + i, f);
+      for (int i = 0; i < D / 32; ++i) {
+        float f[8];
+        q_raw[n][i].unpack(f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i + e] = f[e];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 4; ++i) v[i] = tb::to_f32(q[i]);
+        for (int e = 0; e < 8; ++e) v[8 * i + e] = f[e];
       }
 #pragma unroll
       for (int i = 0; i < D / 4; ++i) {
@@ -599,6 +743,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     const bool closes = cur.end == tiles(cur.tokens);
     const int b = cur.b, r = cur.r;
     going = next_portion(a, g, cur);
+    if (S::kQRegs && going) ask_q();
     float* part = first_portion ? first_part : reinterpret_cast<float*>(ring);
     if (!first_portion && !(opens && closes)) {  // the list's last portion: the ring is done with
       cp_wait<0>();
@@ -634,6 +779,10 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     first_portion = false;
   }
   cp_wait<0>();
+  if (g.cs > 1) {
+    cluster_join<T, D, NT>(a, g, smem, meta, out4);
+    return;
+  }
   __syncthreads();
   tb::pdl_trigger();
 
@@ -825,15 +974,32 @@ int sm_count() {
   return n;
 }
 
-// Units of B sequences with HG groups and contexts of `cap` tokens.
-long long most_units(int B, int HG, int cap) { return static_cast<long long>(B) * HG * (cap / kTile + 1 + kStart); }
+// How the work of `segs` (sequence, group) pairs with contexts of up to `cap`
+// tokens is dealt out: a cluster of so many CTAs for each pair, or 0, the even
+// lists.  The lists pay for their start and for the joining kernel, a cluster for
+// the longest context, with a warp's latency per tile.  Measured on one B200 (D =
+// 128): lists 10.5 us and 0.76 ns per tile, of which contexts of mixed lengths have
+// half of `cap`; clusters 6.5 us and 0.85 us per tile of a warp.  1 x 1,000 tokens x
+// 8 KV heads: clusters 7.5 us, lists 10.3; 37 ragged contexts up to 1,536 tokens:
+// clusters 27 us, lists 22.
+// Lists count their units in 31 bits; more take the clusters.
+int cluster_of(int segs, int cap, int fit) {
+  const long long tiles = cap / kTile + 1, units = (tiles + kStart) * segs;
+  if (units > 0x7fffffff) return 1;
+  if (segs > fit) return 0;
+  int cs = 1;
+  while (cs < kMostCluster && 2 * cs * segs <= fit && cs * kWarps < tiles) cs *= 2;
+  return 6.5 + 0.85 * ((tiles + cs * kWarps - 1) / (cs * kWarps)) < 10.5 + segs * tiles * 0.0004 ? cs : 0;
+}
 
 // CTAs to launch for contexts of at most `cap` tokens: those that fit at once,
 // more (up to kMostWaves times) where each could still take kWaveTiles.
 template <int D, int NT>
 int grid_of(int B, int Hq, int Hk, int cap) {
   const int fit = sm_count() * resident<D, NT>(), G = Hq / Hk;
-  const long long n = most_units(B, Hk * ((G + 8 * NT - 1) / (8 * NT)), cap) / kWaveTiles;
+  const int segs = B * Hk * ((G + 8 * NT - 1) / (8 * NT));
+  if (cluster_of(segs, cap, fit)) return 0;
+  const long long n = static_cast<long long>(segs) * (cap / kTile + 1 + kStart) / kWaveTiles;
   return n <= fit ? fit : n < kMostWaves * fit ? static_cast<int>(n) : kMostWaves * fit;
 }
 
@@ -849,8 +1015,7 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a, int sms) {
   for (int i = 0; i < 31; ++i)
     if (a.cache.bs == 1 << i) g.shift = i;
   g.tile_pages = a.cache.bs % kTile == 0;
-  // (units are counted in 32 bits)
-  g.whole = g.cap <= kWholeTokens || most_units(a.B, g.HG, g.cap) > 0x7fffffff;
+  g.cs = cluster_of(a.B * g.HG, g.cap, g.fit);
   return g;
 }
 
@@ -863,9 +1028,18 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   if (e != cudaSuccess) return static_cast<int>(e);
   const bool q8 = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.qs_b % 8 == 0 && a.qs_h % 8 == 0;
   const bool out4 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.os_b % 4 == 0 && a.os_h % 4 == 0;
-  if (g.whole) {
-    kernel<<<a.B * g.HG, kThreads, S::kBytes, s>>>(a, g, q8, out4);
-    return static_cast<int>(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  if (g.cs) {
+    cfg.gridDim = dim3(a.B * g.HG * g.cs);
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(g.cs), 1, 1};
+    cfg.numAttrs = g.cs > 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, g, q8, out4));
   }
   const int grid = grid_of<D, NT>(a.B, a.Hq, a.cache.Hk, g.cap);
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
@@ -873,14 +1047,11 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   const cudaError_t e1 = cudaGetLastError();
   if (e1 != cudaSuccess) return static_cast<int>(e1);
   // programmatic launch: the joining CTAs are in place when the last list ends
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_attn_quant_join_kernel<T, D, NT>, a, g, grid, out4));
 }
@@ -900,7 +1071,7 @@ int launch_type(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
 }  // namespace
 
 extern "C" size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens) {
-  if (B <= 0 || Hk <= 0 || max_tokens <= kWholeTokens) return 0;
+  if (B <= 0 || Hk <= 0) return 0;
   const bool two = Hq / Hk > 8;
   switch (D) {
     case 64:

@@ -109,9 +109,9 @@ def test_gradients(interleaved, device):
     v = torch.randn(T, H, D, device=device)
     with torch.no_grad():
         step = rotary(x + v, pos, table, interleaved=interleaved).double() - y.double()
-    lhs, rhs = (dy.double() * step).sum(), (dx.double() * v.double()).sum()
+    lhs, rhs = float((dy.double() * step).sum()), float((dx.double() * v.double()).sum())
     n = T * H * D
-    assert abs(lhs - rhs) <= 2.0 ** -20 * math.sqrt(n) * float((dy.abs().max() * (x.abs().max() + v.abs().max())) * 4)
+    assert abs(lhs - rhs) <= 2.0 ** -20 * math.sqrt(n) * 4 * float(dy.abs().max() * (x.detach().abs().max() + v.abs().max()))
     # a broadcast gradient, a strided input, and the gradient of the gradient
     wide = torch.randn(T, H, 2 * D, device=device, requires_grad=True)
     rotary(wide[..., ::1][..., :D], pos, table, interleaved=interleaved).sum().backward()
