@@ -8,15 +8,21 @@
 // The pages are the traffic (2 (D + 4) bytes per token and KV head), read once:
 //
 //  * Work is cut into tiles of 16 tokens and dealt out evenly over the warps of
-//    a resident grid, whatever the contexts' lengths: worker i of n takes the
-//    tiles [i T / n, (i + 1) T / n) of the list (sequence, KV head, tile), read
-//    off ctx_len on the device, so one captured call serves contexts that grow.
+//    a resident grid, whatever the contexts' lengths: worker i of n takes its
+//    share of the list (sequence, KV head, tile), read off ctx_len on the
+//    device, so one captured call serves contexts that grow.  (Equal shares end
+//    up to 15% apart, SMs of different GPCs reaching memory at different rates;
+//    that, the 5 us until the first tile is there and the 5 us of joining are
+//    what separates the kernel from its bytes: with every product left out it
+//    took 96% of its time.)
 //  * A warp fills a ring of tiles in its shared memory with cp.async, running
 //    ahead over the borders of contexts, and waits for no other warp before
 //    the end of its list.  Contexts that end inside its list it writes out; the
 //    parts at the list's two ends (maximum, sum, unnormalised output) the CTA
 //    merges, and what is split over CTAs a second kernel joins, all in a fixed
 //    order: no atomics, the same bits every time.
+//  * Few or short contexts go to clusters instead, one per (sequence, KV head),
+//    joined over distributed shared memory in the one launch.
 //  * Products run on mma.sync m16n8k16 in fp16 (every e4m3 value is an fp16
 //    value) with the tokens, then the head's dimensions, as the 16 rows and the
 //    query heads as the 8 columns: with 5 to 8 query heads per KV head hardly a
@@ -30,6 +36,10 @@
 //    m moves only once the maximum is 2^8 above it, so weights stay below 2^8
 //    and most tiles need no reduction over the warp and no rescaling.  q is
 //    brought into fp16 range by a power of two per head (exact).
+//
+// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 100 us,
+// 5.5 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 31 us; 1 x
+// 1,000 tokens x 8 KV heads 7.4 us.
 #include <math.h>
 
 #include "device_common.cuh"
@@ -42,9 +52,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;       // tokens per tile
 constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that many
-constexpr int kWaveTiles = 64;  // tiles per CTA where there are more CTAs than fit at once
-constexpr int kMostWaves = 1;
-constexpr int kStart = 1;       // what beginning a (sequence, group) costs a warp, in tiles
+constexpr int kStart = 3;       // what beginning a (sequence, group) costs a warp, in tiles
 constexpr int kMostCluster = 8;   // CTAs of a cluster (the portable bound)
 constexpr float kMinVsLog = -100.f;
 constexpr float kSlack = 8.f;   // the reference of the weights may lag behind their maximum by a factor of 2^8
@@ -144,7 +152,6 @@ struct Geometry {
   int shift;       // log2 of the page size, or -1
   int tile_pages;  // pages hold whole tiles
   int cs;          // CTAs (a cluster) for each (sequence, group), or 0: work dealt out evenly
-  int fit;         // CTAs that fit at once
 };
 
 __device__ __forceinline__ int tokens_of(const TbDecodeAttnQuantArgs& a, const Geometry& g, int b) {
@@ -443,11 +450,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) total += sums[i];
     total *= g.HG;
-    // as many CTAs as fit at once, unless that leaves them less than kMinTiles, or more than kWaveTiles
-    uint32_t N = g.fit;
+    // all CTAs, unless that leaves them less than kMinTiles
+    uint32_t N = gridDim.x;
     if (total < N * kMinTiles) N = (total + kMinTiles - 1) / kMinTiles;
-    if (total > N * kWaveTiles) N = total / kWaveTiles;
-    if (N > gridDim.x) N = gridDim.x;
     if (N == 0) empty_rows(gridDim.x);
     if (blockIdx.x >= N) return;
     ctas = static_cast<int>(N);
@@ -548,7 +553,8 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           q_raw[n][i].load(q + 8 * i);
         } else {
           const unsigned short* e = reinterpret_cast<const unsigned short*>(q + 8 * i);
-          q_raw[n][i].raw = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+          auto two = [&](int j) { return e[j] | static_cast<uint32_t>(e[j + 1]) << 16; };
+          q_raw[n][i].raw = make_uint4(two(0), two(2), two(4), two(6));
         }
       }
     }
@@ -790,6 +796,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   constexpr int E = D / 32, V = E < 4 ? E : 4;
   const int2 mt = lane < 2 * kWarps ? meta[lane] : make_int2(-1, 0);
   bool first_run = true;
+  int turn = 0;  // (set of parts, head) pairs so far: they go round the warps
 #pragma unroll 1
   for (unsigned parts = __ballot_sync(0xffffffffu, mt.x >= 0); parts != 0;) {
     const int seg = __shfl_sync(0xffffffffu, mt.x, __ffs(parts) - 1);
@@ -815,32 +822,23 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       return reinterpret_cast<const float*>(smem + (p % 2 ? p / 2 * S::kRing : kWarps * S::kRing + p / 2 * S::kPart));
     };
 #pragma unroll 1
-    for (int h = w; h < nh; h += kWarps) {
-      float2 st = make_float2(-INFINITY, 0.f);
-      if (lane < 2 * kWarps && set >> lane & 1) st = *reinterpret_cast<const float2*>(part_of(lane) + kHeads * D + 2 * h);
-      float M = st.x;
-#pragma unroll
-      for (int o = 1; o < 2 * kWarps; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      M = __shfl_sync(0xffffffffu, M, 0);
-      const float f = st.x == -INFINITY ? 0.f : exp2_fast(st.x - M);
-      float L = f * st.y;
-#pragma unroll
-      for (int o = 1; o < 2 * kWarps; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      L = __shfl_sync(0xffffffffu, L, 0);
-      const float inv = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
-      float o[E] = {};
+    for (int h = (w - turn) & (kWarps - 1); h < nh; h += kWarps) {
+      float M = -INFINITY, L = 0.f, o[E] = {};
+      for (unsigned r = set; r; r &= r - 1) M = fmaxf(M, part_of(__ffs(r) - 1)[kHeads * D + 2 * h]);
       for (unsigned r = set; r; r &= r - 1) {
-        const int p = __ffs(r) - 1;
-        const float fp = __shfl_sync(0xffffffffu, f, p);
-        const float* v = part_of(p) + h * D + lane * V;
+        const float* p = part_of(__ffs(r) - 1);
+        const float2 st = *reinterpret_cast<const float2*>(p + kHeads * D + 2 * h);
+        const float f = st.x == -INFINITY ? 0.f : exp2_fast(st.x - M);
+        L += f * st.y;
 #pragma unroll
         for (int i = 0; i < E; i += V) {
           float y[V];
-          tb::load_vec<float, V>(v + i * 32, y);
+          tb::load_vec<float, V>(p + h * D + i * 32 + lane * V, y);
 #pragma unroll
-          for (int e = 0; e < V; ++e) o[i + e] += fp * y[e];
+          for (int e = 0; e < V; ++e) o[i + e] += f * y[e];
         }
       }
+      const float inv = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
       T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
       float* part = P::out(a.ws, slot, h);
 #pragma unroll
@@ -859,6 +857,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       }
       if (!whole && lane == 0) *reinterpret_cast<float2*>(P::stat(a.ws, slot, h)) = make_float2(M, L);
     }
+    turn += nh;
   }
 }
 
@@ -992,21 +991,16 @@ int cluster_of(int segs, int cap, int fit) {
   return 6.5 + 0.85 * ((tiles + cs * kWarps - 1) / (cs * kWarps)) < 10.5 + segs * tiles * 0.0004 ? cs : 0;
 }
 
-// CTAs to launch for contexts of at most `cap` tokens: those that fit at once,
-// more (up to kMostWaves times) where each could still take kWaveTiles.
+// CTAs of the even lists (0: clusters).
 template <int D, int NT>
-int grid_of(int B, int Hq, int Hk, int cap) {
+int list_grid(int B, int Hq, int Hk, int cap) {
   const int fit = sm_count() * resident<D, NT>(), G = Hq / Hk;
-  const int segs = B * Hk * ((G + 8 * NT - 1) / (8 * NT));
-  if (cluster_of(segs, cap, fit)) return 0;
-  const long long n = static_cast<long long>(segs) * (cap / kTile + 1 + kStart) / kWaveTiles;
-  return n <= fit ? fit : n < kMostWaves * fit ? static_cast<int>(n) : kMostWaves * fit;
+  return cluster_of(B * Hk * ((G + 8 * NT - 1) / (8 * NT)), cap, fit) ? 0 : fit;
 }
 
 template <int D, int NT>
-Geometry geometry(const TbDecodeAttnQuantArgs& a, int sms) {
+Geometry geometry(const TbDecodeAttnQuantArgs& a) {
   Geometry g;
-  g.fit = sms * resident<D, NT>();
   g.G = a.Hq / a.cache.Hk;
   g.NG = (g.G + 8 * NT - 1) / (8 * NT);
   g.HG = a.cache.Hk * g.NG;
@@ -1015,14 +1009,14 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a, int sms) {
   for (int i = 0; i < 31; ++i)
     if (a.cache.bs == 1 << i) g.shift = i;
   g.tile_pages = a.cache.bs % kTile == 0;
-  g.cs = cluster_of(a.B * g.HG, g.cap, g.fit);
+  g.cs = cluster_of(a.B * g.HG, g.cap, sm_count() * resident<D, NT>());
   return g;
 }
 
 template <typename T, int D, int NT>
 int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   using S = Smem<D, NT>;
-  const Geometry g = geometry<D, NT>(a, sm_count());
+  const Geometry g = geometry<D, NT>(a);
   auto kernel = decode_attn_quant_kernel<T, D, NT>;
   const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -1041,7 +1035,7 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
     cfg.numAttrs = g.cs > 1;
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, g, q8, out4));
   }
-  const int grid = grid_of<D, NT>(a.B, a.Hq, a.cache.Hk, g.cap);
+  const int grid = list_grid<D, NT>(a.B, a.Hq, a.cache.Hk, g.cap);
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
   kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, q8, out4);
   const cudaError_t e1 = cudaGetLastError();
@@ -1075,14 +1069,14 @@ extern "C" size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int 
   const bool two = Hq / Hk > 8;
   switch (D) {
     case 64:
-      return two ? Partials<64, 2>::bytes(grid_of<64, 2>(B, Hq, Hk, max_tokens))
-                 : Partials<64, 1>::bytes(grid_of<64, 1>(B, Hq, Hk, max_tokens));
+      return two ? Partials<64, 2>::bytes(list_grid<64, 2>(B, Hq, Hk, max_tokens))
+                 : Partials<64, 1>::bytes(list_grid<64, 1>(B, Hq, Hk, max_tokens));
     case 128:
-      return two ? Partials<128, 2>::bytes(grid_of<128, 2>(B, Hq, Hk, max_tokens))
-                 : Partials<128, 1>::bytes(grid_of<128, 1>(B, Hq, Hk, max_tokens));
+      return two ? Partials<128, 2>::bytes(list_grid<128, 2>(B, Hq, Hk, max_tokens))
+                 : Partials<128, 1>::bytes(list_grid<128, 1>(B, Hq, Hk, max_tokens));
     case 256:
-      return two ? Partials<256, 2>::bytes(grid_of<256, 2>(B, Hq, Hk, max_tokens))
-                 : Partials<256, 1>::bytes(grid_of<256, 1>(B, Hq, Hk, max_tokens));
+      return two ? Partials<256, 2>::bytes(list_grid<256, 2>(B, Hq, Hk, max_tokens))
+                 : Partials<256, 1>::bytes(list_grid<256, 1>(B, Hq, Hk, max_tokens));
   }
   return 0;
 }
