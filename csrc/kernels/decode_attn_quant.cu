@@ -862,8 +862,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 }
 
 // Joins the contexts that were split over CTAs.  Up to kFewParts parts: the CTA
-// of the first part joins them, a warp for each query head.  More: CTA i of
-// those that share the context joins query head i, each warp every eighth part.
+// of the first part joins them, a warp for each query head.  More: each of the CTAs
+// that share the context joins a slice of a query head, its lanes and warps
+// different parts.
 constexpr int kFewParts = 16, kJoinWarps = 8;
 
 template <typename T, int D, int NT>
@@ -928,11 +929,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const int lead = role == 0 ? static_cast<int>(blockIdx.x) : mine.w;
     if (lead < 0) continue;
     const int4 rec = role == 0 ? mine : *P::record(a.ws, grid, lead);
-    const int h = blockIdx.x - lead;
-    if (rec.z <= kFewParts || h >= heads_of(rec.x)) continue;  // the same for the whole CTA
+    if (rec.z <= kFewParts) continue;
+    // slices of a head's dimensions, so that more of the CTAs that share the context take part
+    const int nh = heads_of(rec.x), n = rec.z;
+    int slices = 1;
+    while (2 * slices <= D / 32 && 2 * slices * nh <= n) slices *= 2;
+    const int item = blockIdx.x - lead, h = item / slices, size = D / slices;
+    if (h >= nh) continue;  // the same for the whole CTA
     auto slot = [&](int p) { return p == 0 ? static_cast<long long>(rec.y) : 2ll * (lead + p); };
     float M = -INFINITY;
-    for (int p = threadIdx.x; p < rec.z; p += kJoinWarps * 32) M = fmaxf(M, P::stat(a.ws, slot(p), h)[0]);
+    for (int p = threadIdx.x; p < n; p += kJoinWarps * 32) M = fmaxf(M, P::stat(a.ws, slot(p), h)[0]);
     M = tb::warp_max(M);
     __syncthreads();
     if (lane == 0) red[w] = M;
@@ -940,28 +946,49 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 #pragma unroll
     for (int i = 0; i < kJoinWarps; ++i) M = fmaxf(M, red[i]);
     if (M == -INFINITY) M = 0.f;
-    float L = 0.f, o[E] = {};
-#pragma unroll 8
-    for (int p = w; p < rec.z; p += kJoinWarps) {
+    // `lanes` lanes hold a part's slice, four dimensions each (at D = 256 in one slice: and the four 128 further)
+    const int lanes = min(size / 4, 32), at_once = 32 / lanes, d = item % slices * size + lane % lanes * 4;
+    const bool wide = D == 256 && size == 256;
+    float L = 0.f, o[8] = {};
+#pragma unroll 4
+    for (int p = w * at_once + lane / lanes; p < n; p += kJoinWarps * at_once) {
       const float2 st = *reinterpret_cast<const float2*>(P::stat(a.ws, slot(p), h));
-      const float f = exp2_fast(st.x - M);
+      const float f = exp2_fast(st.x - M), *v = P::out(a.ws, slot(p), h) + d;
       L += f * st.y;
-      add(o, f, P::out(a.ws, slot(p), h));
+      float x[4];
+      tb::load_vec<float, 4>(v, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+      if (wide) {
+        tb::load_vec<float, 4>(v + 128, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 + e] += f * x[e];
+      }
+    }
+    for (int x = lanes; x < 32; x *= 2) {
+      L += __shfl_xor_sync(0xffffffffu, L, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], x);
     }
     if (lane == 0) sl[w] = L;
+    if (lane < lanes) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) so[w][lane * E + i] = o[i];
-    __syncthreads();
-    if (w == 0) {
-      L = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = 0.f;
-      for (int x = 0; x < kJoinWarps; ++x) {
-        L += sl[x];
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] += so[x][lane * E + i];
+      for (int e = 0; e < 4; ++e) {
+        so[w][lane * 4 + e] = o[e];
+        if (wide) so[w][128 + lane * 4 + e] = o[4 + e];
       }
-      write(rec.x, h, L, o);
+    }
+    __syncthreads();
+    if (threadIdx.x < size) {
+      float sum = 0.f, l = 0.f;
+#pragma unroll
+      for (int x = 0; x < kJoinWarps; ++x) {
+        l += sl[x];
+        sum += so[x][threadIdx.x];
+      }
+      const int r = rec.x % g.HG, head = r / g.NG * g.G + r % g.NG * P::kHeads + h;
+      static_cast<T*>(a.out)[static_cast<long long>(rec.x / g.HG) * a.os_b + static_cast<long long>(head) * a.os_h +
+                             item % slices * size + threadIdx.x] = tb::from_f32<T>(l == 0.f ? 0.f : sum / l);
     }
   }
 }

@@ -449,7 +449,9 @@ def test_write_attend_read_in_a_row(device):
 # ------------------------------------------------------------------ GPU only
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens,Hq,Hk,D,bs", [([40000, 7], 8, 2, 128, 16), ([9000], 32, 1, 64, 64), ([20000], 2, 2, 256, 16),
-                                             ([768] * 300, 12, 2, 128, 16), ([0, 5, 900] * 100, 20, 1, 128, 16)])
+                                             ([768] * 300, 12, 2, 128, 16), ([0, 5, 900] * 100, 20, 1, 128, 16),
+                                                ([60000, 0, 2000], 16, 1, 256, 16), ([100000], 1, 1, 128, 64),
+                                                ([30000, 30000], 12, 1, 64, 7), ([3000] * 40, 16, 1, 256, 64)])
 def test_attention_split_and_joined(lens, Hq, Hk, D, bs, dev):
     g = torch.Generator().manual_seed(2)
     table, nb = pages(lens, bs, dev)
