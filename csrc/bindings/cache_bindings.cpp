@@ -45,15 +45,23 @@ struct Range {
   uintptr_t lo, hi;
 };
 Range range_of(const at::Tensor& t) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-  if (t.numel() == 0) return {p, p};
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  const auto sizes = t.sizes(), strides = t.strides();
   int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  for (size_t i = 0; i < sizes.size(); ++i) {
+    if (sizes[i] == 0) return {p, p};
+    last += (sizes[i] - 1) * strides[i];
+  }
   return {p, p + static_cast<uintptr_t>(last + 1) * t.element_size()};
 }
-bool apart(const at::Tensor& a, const at::Tensor& b) {
-  const Range x = range_of(a), y = range_of(b);
-  return x.hi <= y.lo || y.hi <= x.lo || x.lo == x.hi || y.lo == y.hi;
+bool apart(const Range& x, const Range& y) { return x.hi <= y.lo || y.hi <= x.lo || x.lo == x.hi || y.lo == y.hi; }
+bool apart(const at::Tensor& a, const at::Tensor& b) { return apart(range_of(a), range_of(b)); }
+// Whether `t` is apart from every one of `others`.
+template <size_t N>
+bool apart_from_all(const Range& t, const Range (&others)[N]) {
+  for (const Range& o : others)
+    if (!apart(t, o)) return false;
+  return true;
 }
 // Whether two [T, H, D] views share no element: disjoint ranges, or column
 // slices of rows with the same stride.
@@ -63,7 +71,7 @@ bool columns_apart(const at::Tensor& a, const at::Tensor& b) {
   const int64_t e = a.element_size(), row = a.stride(0) * e;
   const int64_t wa = ((a.size(1) - 1) * a.stride(1) + a.size(2)) * e, wb = ((b.size(1) - 1) * b.stride(1) + b.size(2)) * e;
   if (row <= 0) return false;
-  int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr()));
+  int64_t d = static_cast<int64_t>(range_of(b).lo - range_of(a).lo);
   d %= row;
   if (d < 0) d += row;
   return d >= wa && d + wb <= row;
@@ -233,12 +241,11 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
   index1(seq, T, op, "seq_of_token is a contiguous int32 [T]");
   index1(pos, T, op, "pos is a contiguous int32 [T]");
   for (const at::Tensor* t : {&k, &v, &seq, &pos}) chk(t->device() == dev, op, "all tensors on one device");
-  const at::Tensor* caches[4] = {&kc, &vc, &ks, &vs};
-  for (int i = 0; i < 4; ++i) {
-    for (int j = i + 1; j < 4; ++j) chk(apart(*caches[i], *caches[j]), op, "the cache tensors overlap");
-    for (const at::Tensor* t : {&k, &v, &seq, &pos, &block_table})
-      chk(apart(*caches[i], *t), op, "an input overlaps the cache");
-  }
+  const Range caches[4] = {range_of(kc), range_of(vc), range_of(ks), range_of(vs)};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 4; ++j) chk(apart(caches[i], caches[j]), op, "the cache tensors overlap");
+  for (const at::Tensor* t : {&k, &v, &seq, &pos, &block_table})
+    chk(apart_from_all(range_of(*t), caches), op, "an input overlaps the cache");
   a.rot.err = error_of(error, dev, op);
   if (table_) {
     const at::Tensor& table = *table_;
@@ -257,7 +264,7 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
     chk(q_->size(0) == T && q_->size(2) == a.cache.D && q_->scalar_type() == k.scalar_type(), op,
         "q has k's rows, head dimension and type");
     chk(q_->device() == dev, op, "all tensors on one device");
-    for (int i = 0; i < 4; ++i) chk(apart(*caches[i], *q_), op, "q overlaps the cache");
+    chk(apart_from_all(range_of(*q_), caches), op, "q overlaps the cache");
   }
   if (q_out_) {
     rows3(*q_out_, op, "q_out is [T, Hq, D] with a contiguous last dimension");
@@ -267,8 +274,10 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
     chk(rows_distinct(*q_out_), op, "q_out has overlapping rows");
     chk(same_view(*q_, *q_out_) || columns_apart(*q_, *q_out_), op, "q_out is q itself or does not overlap it");
     chk(columns_apart(*q_out_, k) && columns_apart(*q_out_, v), op, "q_out overlaps k or v");
-    for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &seq, &pos, &block_table, &*table_})
-      chk(apart(*t, *q_out_), op, "q_out overlaps an input");
+    const Range out = range_of(*q_out_);
+    chk(apart_from_all(out, caches), op, "q_out overlaps the cache");
+    for (const at::Tensor* t : {&seq, &pos, &block_table, &*table_})
+      chk(apart(out, range_of(*t)), op, "q_out overlaps an input");
   }
   if (!kc.is_cuda()) return std::nullopt;
   c10::cuda::CUDAGuard guard(dev);
@@ -316,8 +325,9 @@ bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
   for (const at::Tensor* t : {&k_out, &v_out, &seq, &pos}) chk(t->device() == dev, op, "all tensors on one device");
   chk(rows_distinct(k_out) && rows_distinct(v_out), op, "out has overlapping rows");
   chk(columns_apart(k_out, v_out), op, "the two outputs overlap");
+  const Range outs[2] = {range_of(k_out), range_of(v_out)};
   for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &seq, &pos, &block_table})
-    chk(apart(k_out, *t) && apart(v_out, *t), op, "out overlaps an input");
+    chk(apart_from_all(range_of(*t), outs), op, "out overlaps an input");
   a.err = error_of(error, dev, op);
   if (!kc.is_cuda()) return false;
   if (T == 0) return true;
@@ -358,8 +368,9 @@ Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::
     chk(out_->device() == dev, op, "all tensors on one device");
     chk(rows_distinct(*out_), op, "out has overlapping rows");
     chk(columns_apart(*out_, q), op, "out overlaps q");
+    const Range out = range_of(*out_);
     for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &ctx_len, &block_table})
-      chk(apart(*out_, *t), op, "out overlaps an input");
+      chk(apart(out, range_of(*t)), op, "out overlaps an input");
   }
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt(static_cast<double>(a.cache.D));
   chk(std::isfinite(scale), op, "a finite scale");

@@ -7,6 +7,7 @@ in-place kernel of the decoder's default (bf16, half layout, whole head).
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -83,10 +84,15 @@ def rotary_table(rot_dim: int, max_pos: int, theta: float = 1e4, scaling: Option
     return (torch.stack([torch.cos(ang), torch.sin(ang)], -1) * m).to(device=device, dtype=torch.float32).contiguous()
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    o = getattr(_core(), "ops", None)
+    return (lambda *args: None) if o is None else getattr(o, name)
+
+
 def _call(name: str, *args):
     """A kernel entry point: checks, launches and returns its result; None for CPU tensors (or a CPU-only build)."""
-    o = getattr(_core(), "ops", None)
-    return None if o is None else getattr(o, name)(*args)
+    return _entry(name)(*args)
 
 
 def _apply(x, pos, table, interleaved, transpose, out, error):
