@@ -42,6 +42,8 @@
 // 1,000 tokens x 8 KV heads 7.4 us.
 #include <math.h>
 
+#include <atomic>
+
 #include "device_common.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
@@ -232,8 +234,8 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Joins the parts of a (sequence, group) that a cluster shares: each CTA its
-// warps', then a warp of the cluster for each query head the CTAs', over
+// Joins the parts of a (sequence, group) that a cluster (or one CTA) shares: each
+// CTA its warps', then a warp of the cluster for each query head the CTAs', over
 // distributed shared memory.
 template <typename T, int D, int NT>
 __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, const Geometry& g, uint8_t* smem, int2* meta,
@@ -244,6 +246,21 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
   const int b = seg / g.HG, r = seg - b * g.HG, kh = r / g.NG, left = g.G - (r - kh * g.NG) * kHeads;
   const int nh = min(left, kHeads), h0 = kh * g.G + g.G - left;
   float* sum = reinterpret_cast<float*>(smem);  // the CTA's part, in the ring of warp 0 (drained)
+  auto write = [&](int h, const float (&o)[E], float inv) {
+    T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
+#pragma unroll
+    for (int i = 0; i < E; i += V) {
+      float z[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[e] = o[i + e] * inv;
+      if (out4) {
+        tb::store_vec<T, V>(out + i * 32 + lane * V, z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[i * 32 + lane * V + e] = tb::from_f32<T>(z[e]);
+      }
+    }
+  };
   __syncthreads();
   for (int h = w; h < nh; h += kWarps) {
     float m[kWarps], l[kWarps], M = -INFINITY, L = 0.f, o[E] = {};
@@ -271,6 +288,10 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
         for (int e = 0; e < V; ++e) o[i + e] += f * y[e];
       }
     }
+    if (g.cs == 1) {
+      if (any) write(h, o, L == 0.f ? 0.f : 1.f / L);  // (else one warp had the whole context, and wrote it)
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < E; i += V) {
       float y[V];
@@ -280,6 +301,7 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
     }
     if (lane == 0) *reinterpret_cast<float2*>(sum + kHeads * D + 2 * h) = make_float2(M, any ? L : -1.f);  // -1: no part
   }
+  if (g.cs == 1) return;
   cluster_barrier();
   for (int h = rank + g.cs * w; h < nh; h += g.cs * kWarps) {
     float m = -INFINITY, l = -1.f;
@@ -319,19 +341,7 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
 #pragma unroll
       for (int i = 0; i < E; ++i) y[i] += fp * o[p][i];
     }
-    T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
-#pragma unroll
-    for (int i = 0; i < E; i += V) {
-      float z[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[e] = y[i + e] * inv;
-      if (out4) {
-        tb::store_vec<T, V>(out + i * 32 + lane * V, z);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[i * 32 + lane * V + e] = tb::from_f32<T>(z[e]);
-      }
-    }
+    write(h, y, inv);
   }
   cluster_barrier();  // nobody leaves while another still reads its shared memory
 }
@@ -415,6 +425,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     const int seg = blockIdx.x / g.cs, part = blockIdx.x % g.cs * kWarps + w, parts = g.cs * kWarps;
     cur.b = seg / g.HG;
     cur.r = seg % g.HG;
+    // the table row (its first 1,024 entries) comes nearer while the context's length is read
+    if (lane * 32 < c.max_blocks)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(c.block_table + static_cast<long long>(cur.b) * c.max_blocks + lane * 32));
     cur.tokens = tokens_of(a, g, cur.b);
     const int n = tiles(cur.tokens);
     if (a.err && threadIdx.x == 0 && a.ctx_len[cur.b] > g.cap) atomicCAS(a.err, 0, 1);
@@ -785,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     first_portion = false;
   }
   cp_wait<0>();
-  if (g.cs > 1) {
+  if (g.cs) {
     cluster_join<T, D, NT>(a, g, smem, meta, out4);
     return;
   }
@@ -993,10 +1006,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   }
 }
 
-int sm_count() {
+int sm_count() {  // of the current device, asked for once
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148;
+  if (dev < kDevices) n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (dev < kDevices) known[dev].store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 
@@ -1059,8 +1078,10 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
     cfg.gridDim = dim3(a.B * g.HG * g.cs);
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {static_cast<unsigned>(g.cs), 1, 1};
-    cfg.numAttrs = g.cs > 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, g, q8, out4));
+    cfg.numAttrs = 1;
+    if (g.cs > 1) return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, g, q8, out4));
+    kernel<<<cfg.gridDim, kThreads, S::kBytes, s>>>(a, g, q8, out4);
+    return static_cast<int>(cudaGetLastError());
   }
   const int grid = list_grid<D, NT>(a.B, a.Hq, a.cache.Hk, g.cap);
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
