@@ -371,7 +371,8 @@ int tb_rotary(const TbRotaryArgs* args, cudaStream_t s);
 // ---------------- 8-bit paged KV cache (kv_quant.cu, decode_attn_quant.cu) ----------------
 // Codes: e4m3 [num_blocks, Hk, bs, D], D in {64, 128, 256}; scales: fp32
 // [num_blocks, Hk, bs]; a value is code * scale.  A token's slot is
-// (block_table[seq, pos / bs], pos % bs).
+// (block_table[seq, pos / bs], pos % bs).  The four arrays are 16-byte aligned,
+// and num_blocks * Hk * bs and max_blocks * bs are below 2^31.
 typedef struct {
   void *kc, *vc;
   float *ks, *vs;
@@ -421,6 +422,7 @@ typedef struct {
   size_t ws_bytes;
   int* err;
 } TbDecodeAttnQuantArgs;
+// max_tokens: max_blocks * bs.  For the current device.
 size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens);
 int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s);
 

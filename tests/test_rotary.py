@@ -217,3 +217,31 @@ def test_large_offsets_streams_and_capture(dev):
     x.copy_(torch.randn(300, 4, 64, device=dev))
     g.replay()
     check(out, x, pos, table)
+
+
+@pytest.mark.gpu
+def test_forward_and_backward_in_a_graph(dev):
+    """A captured forward and backward, replayed on new values; an eager pass over the same leaf afterwards."""
+    table = rotary_table(64, 64, device=dev)
+    x = torch.randn(50, 4, 64, device=dev).bfloat16().requires_grad_()
+    dy = torch.randn(50, 4, 64, device=dev).bfloat16()
+    pos = torch.randint(0, 64, (50,), dtype=torch.int32, device=dev)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            torch.autograd.grad(rotary(x, pos, table), x, dy)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = rotary(x, pos, table)
+        (dx,) = torch.autograd.grad(y, x, dy)
+    with torch.no_grad():
+        x.copy_(torch.randn(50, 4, 64, device=dev))
+        dy.copy_(torch.randn(50, 4, 64, device=dev))
+        pos.copy_(torch.randint(0, 64, (50,), dtype=torch.int32, device=dev))
+    g.replay()
+    check(y.detach(), x.detach(), pos, table)
+    check(dx, dy, pos, table, transpose=True)
+    (again,) = torch.autograd.grad(rotary(x, pos, table), x, dy)
+    assert torch.equal(again, dx)
