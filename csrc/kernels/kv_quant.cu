@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t top_bits(const T*, uint32_t m) {
 // heads in flight.  The four rows are reduced together (5 shuffles at D = 128, 16
 // apart), and the two divisions of a row are done once per lane.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 6 : 10) kv_quant_write_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
   constexpr int L = D / 8, G = 32 / L, U = 4, W = 2 * sizeof(T);  // lanes per row, tokens, rounds in flight, words
   const T* tag = nullptr;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
@@ -139,18 +139,28 @@ __global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs 
   const bool need = p >= 0 && seq >= 0;  // (the rows are loaded while their slots are still looked up)
   if (!__any_sync(0xffffffffu, need)) return;
   const int row0 = static_cast<int>(slot_row(a.cache, seq, p, l == 0 ? a.rot.err : nullptr));
-  const T* kp = static_cast<const T*>(a.k) + t * a.ks_t + 8 * l;
-  const T* vp = static_cast<const T*>(a.v) + t * a.vs_t + 8 * l;
   const int part = static_cast<int>(item - group * sp.parts), hi_slot = (part + 1) * sp.slots / sp.parts;
-  for (int s0 = part * sp.slots / sp.parts; s0 < hi_slot; s0 += U) {
+  const int lo_slot = part * sp.slots / sp.parts;
+  // where the next row is read and its codes go; both jump to v behind the last k head
+  const T* vp = static_cast<const T*>(a.v) + t * a.vs_t + 8 * l;
+  uint8_t* vc = static_cast<uint8_t*>(a.cache.vc) + static_cast<long long>(row0) * D + 8 * l;
+  const long long head = static_cast<long long>(a.cache.bs) * D;
+  const T* from = lo_slot < Hk ? static_cast<const T*>(a.k) + t * a.ks_t + lo_slot * a.ks_h + 8 * l
+                               : vp + (lo_slot - Hk) * a.vs_h;
+  uint8_t* to = lo_slot < Hk
+                    ? static_cast<uint8_t*>(a.cache.kc) + static_cast<long long>(row0) * D + lo_slot * head + 8 * l
+                    : vc + (lo_slot - Hk) * head;
+  for (int s0 = lo_slot; s0 < hi_slot; s0 += U) {
     uint32_t x[U][W], m[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int slot = s0 + u;
 #pragma unroll
       for (int j = 0; j < W; ++j) x[u][j] = 0;
+      if (slot == Hk) from = vp;
+      const T* row = from;
+      from += slot < Hk ? a.ks_h : a.vs_h;
       if (slot < hi_slot && need) {
-        const T* row = slot < Hk ? kp + slot * a.ks_h : vp + (slot - Hk) * a.vs_h;
         if (aligned) {
 #pragma unroll
           for (int j = 0; j < W; j += 4) {
@@ -184,13 +194,14 @@ __global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs 
     for (int u = 0; u < U; ++u) {
       const int slot = s0 + u;
       const float f = __shfl_sync(0xffffffffu, inv, (lane & ~(L - 1)) + (u / 2) * (L / 2) + (u % 2) * (L / 4));
+      if (slot == Hk) to = vc;
+      uint8_t* c = to;
+      to += head;
       if (slot >= hi_slot || row0 < 0) continue;
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = element(tag, x[u], j) * f;
-      uint8_t* c = slot < Hk ? static_cast<uint8_t*>(a.cache.kc) + static_cast<long long>(slot) * a.cache.bs * D
-                             : static_cast<uint8_t*>(a.cache.vc) + static_cast<long long>(slot - Hk) * a.cache.bs * D;
-      *reinterpret_cast<uint2*>(c + static_cast<long long>(row0) * D + 8 * l) =
+      *reinterpret_cast<uint2*>(c) =
           make_uint2(to_e4m3x4(v[0], v[1], v[2], v[3]), to_e4m3x4(v[4], v[5], v[6], v[7]));
     }
   }
@@ -200,7 +211,7 @@ __global__ void __launch_bounds__(256) kv_quant_write_kernel(TbKvQuantWriteArgs 
 // entries in registers for all of them.  A lane holds both members of its pairs
 // (half layout: two vectors of four), else eight neighbours.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_quant_write_rot_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
+__global__ void __launch_bounds__(128) kv_quant_write_rot_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
   constexpr int L = D / 8, G = 32 / L, U = 2;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk, R = a.rot.R;
   const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, t = item / sp.parts;
@@ -287,7 +298,7 @@ __global__ void __launch_bounds__(256) kv_quant_write_rot_kernel(TbKvQuantWriteA
 
 // D / 16 lanes per row, sixteen codes each, four heads in flight.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_quant_read_kernel(TbKvQuantReadArgs a, Split sp, bool aligned) {
+__global__ void __launch_bounds__(128) kv_quant_read_kernel(TbKvQuantReadArgs a, Split sp, bool aligned) {
   constexpr int L = D / 16, G = 32 / L, U = 4;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
   const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
@@ -341,7 +352,8 @@ bool rows_aligned(const void* p, long long st, long long sh, int dtype, int byte
 
 // Warps that share the rounds of their tokens (few tokens: latency counts), as
 // many as fill 16 warps per SM (512 tokens of 16 rows: 3.7 us so, 4.6 with 8 or 32);
-// in blocks of two warps, over more SMs, where there are few.
+// in blocks of two warps, over more SMs, where there are few, else of four (ragged
+// batches: 1 us in 33 less than with eight).
 constexpr int kFewWarps = 148 * 16, kSpread = 148 * 8;
 int parts_of(long long groups, int rounds) {
   int n = 1;
@@ -351,7 +363,7 @@ int parts_of(long long groups, int rounds) {
 struct Shape {
   int grid, block;
   explicit Shape(long long warps)
-      : grid(static_cast<int>(warps <= kSpread ? (warps + 1) / 2 : (warps + 7) / 8)), block(warps <= kSpread ? 64 : 256) {}
+      : grid(static_cast<int>(warps <= kSpread ? (warps + 1) / 2 : (warps + 3) / 4)), block(warps <= kSpread ? 64 : 128) {}
 };
 
 template <typename T, int D>
