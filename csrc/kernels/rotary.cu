@@ -9,8 +9,8 @@
 // the table.  Dimensions behind R are copied (in place: left alone).
 //
 // The kernel moves every element once in and once out and does 3 flops per
-// element, so memory bounds it: 16,383 rows x 40 heads x 128 in bf16 take 58 us on
-// one B200, 5.8 TB/s (88% of its copy rate).
+// element, so memory bounds it: 16,383 rows x 40 heads x 128 in bf16 take 54 us on
+// one B200, 6.2 TB/s (95% of its copy rate).
 #include <math.h>
 
 #include "device_common.cuh"
@@ -19,14 +19,18 @@
 
 namespace {
 
+// Threads of a block, and the blocks of an SM that the registers have to allow.
+constexpr int threads_of(int hu) { return hu == 8 ? 128 : 256; }
+constexpr int blocks_of(int hu) { return hu == 4 ? 3 : 4; }
+
 // A thread holds one unit, two vectors of NP elements, of HU heads of a token
 // (every HS-th), so it reads its table entries once: read anew for each head they
-// are twice the bytes of a bf16 row, out of L1 (81 us instead of 58 at the size
-// above).  Rotated units hold NP
-// pairs (half layout: NP elements of each half; interleaved: 2 NP neighbours), the
-// others 2 NP copied elements.  All loads are issued before the first product.
+// are twice the bytes of a bf16 row, out of L1 (81 us with HU = 1, 58 with 4, 54
+// with 8 at the size above).  Rotated units hold NP pairs (half layout: NP elements
+// of each half; interleaved: 2 NP neighbours), the others 2 NP copied elements.  All loads are issued before the first product.
 template <typename T, int NP, int HU, bool INTER>
-__global__ void __launch_bounds__(256, HU > 1 ? 3 : 4) rotary_kernel(TbRotaryArgs a, int rot_units, int units, int HS, int tokens) {
+__global__ void __launch_bounds__(threads_of(HU), blocks_of(HU))
+    rotary_kernel(TbRotaryArgs a, int rot_units, int units, int HS, int tokens) {
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
   const int half = a.R / 2, per = units * HS;
@@ -37,7 +41,7 @@ __global__ void __launch_bounds__(256, HU > 1 ? 3 : 4) rotary_kernel(TbRotaryArg
   const bool bad = p >= a.max_pos;
   if (bad && a.err && threadIdx.x == tk * per) atomicCAS(a.err, 0, 1);
   const float sgn = a.transpose ? -1.f : 1.f;
-  for (int i = threadIdx.x - tk * per; i < per; i += blockDim.x) {  // (more than one round only where per > 256)
+  for (int i = threadIdx.x - tk * per; i < per; i += blockDim.x) {  // (more than one round only where per > blockDim.x)
     const int u = i % units, h0 = i / units;
     const bool turn = u < rot_units && p >= 0 && !bad;
     const int o1 = INTER || u >= rot_units ? u * 2 * NP : u * NP;
@@ -85,8 +89,9 @@ int launch_vec(const TbRotaryArgs& a, cudaStream_t s) {
   const int units = rot_units + (a.x == a.y ? 0 : (a.D - a.R) / (2 * NP));
   const int HS = (a.H + HU - 1) / HU;
   const long long per = static_cast<long long>(units) * HS;
-  const int tokens = per >= 256 ? 1 : static_cast<int>(256 / per);
-  rotary_kernel<T, NP, HU, INTER><<<(a.T + tokens - 1) / tokens, 256, 0, s>>>(a, rot_units, units, HS, tokens);
+  constexpr int kThreads = threads_of(HU);
+  const int tokens = per >= kThreads ? 1 : static_cast<int>(kThreads / per);
+  rotary_kernel<T, NP, HU, INTER><<<(a.T + tokens - 1) / tokens, kThreads, 0, s>>>(a, rot_units, units, HS, tokens);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -99,13 +104,24 @@ bool fits(const TbRotaryArgs& a) {
          reinterpret_cast<uintptr_t>(a.table) % 16 == 0;
 }
 
-// Four heads per thread where that still leaves each of 148 SMs 1,024 threads;
-// else one: 64 rows x 14 heads take 2.2 us so, mostly launch.
+// Heads per thread.  One where more would leave an SM (of 148) fewer than 1,024
+// threads (64 rows x 14 heads take 2.2 us so, mostly launch) or find no heads to hold
+// (100,000 rows x 1 head x 128: 15.4 us, with four 19.4).  Else four, and eight in
+// smaller blocks for 8 or more heads in vectors of 16 bytes: 54 against 58 us at the
+// size above, 40 against 44 for 60,000 rows x 8 heads x 128, but 23 against 21 for
+// 16,000 rows x 16 heads x 80 (40 rotated), which are in vectors of 8 bytes.
+template <typename T, int NP, bool INTER>
+int launch_heads(const TbRotaryArgs& a, cudaStream_t s) {
+  const bool few = static_cast<long long>(a.T) * a.H * (a.D / (2 * NP)) < 4ll * 148 * 1024;
+  if (few || a.H == 1) return launch_vec<T, NP, 1, INTER>(a, s);
+  if constexpr (NP * sizeof(T) == 16)
+    if (a.H >= 8) return launch_vec<T, NP, 8, INTER>(a, s);
+  return launch_vec<T, NP, 4, INTER>(a, s);
+}
+
 template <typename T, int NP>
 int launch_layout(const TbRotaryArgs& a, cudaStream_t s) {
-  const bool many = static_cast<long long>(a.T) * a.H * (a.D / (2 * NP)) >= 4ll * 148 * 1024;
-  if (many) return a.interleaved ? launch_vec<T, NP, 4, true>(a, s) : launch_vec<T, NP, 4, false>(a, s);
-  return a.interleaved ? launch_vec<T, NP, 1, true>(a, s) : launch_vec<T, NP, 1, false>(a, s);
+  return a.interleaved ? launch_heads<T, NP, true>(a, s) : launch_heads<T, NP, false>(a, s);
 }
 
 // The widest vectors that fit: 16 bytes, 8 bytes, or single elements.

@@ -51,6 +51,20 @@ def test_matches_64_bits(T, H, D, R, interleaved, dtype, device):
         assert torch.equal(z, y)  # in place: the same bits
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,H,D,R,shift", [(76001, 1, 128, 128, 0), (26003, 3, 128, 64, 0), (8501, 9, 128, 128, 0),
+                                           (4003, 19, 128, 96, 0), (4801, 16, 128, 128, 4), (6007, 17, 96, 40, 1)])
+def test_many_rows(T, H, D, R, shift, interleaved, dtype):
+    """Enough rows for several heads per thread, whose last share is short; vectors of every width."""
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T * H * D + 8, generator=g).to(dtype).to("cuda:0")[shift:shift + T * H * D].view(T, H, D)
+    table = rotary_table(R, 500, device="cuda:0")
+    pos = torch.randint(-1, 500, (T,), generator=g, dtype=torch.int32).to("cuda:0")
+    check(rotary(x, pos, table, interleaved=interleaved), x, pos, table, interleaved)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_strided_rows_and_heads(interleaved, device):
