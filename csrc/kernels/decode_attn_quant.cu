@@ -37,9 +37,9 @@
 //    and most tiles need no reduction over the warp and no rescaling.  q is
 //    brought into fp16 range by a power of two per head (exact).
 //
-// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 100 us,
-// 5.5 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 31 us; 1 x
-// 1,000 tokens x 8 KV heads 7.4 us.
+// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 97 us,
+// 5.7 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 30 us; 1 x
+// 1,000 tokens x 8 KV heads 7.5 us.
 #include <math.h>
 
 #include <atomic>
@@ -106,28 +106,31 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 
 // Shared memory.  A ring stage holds 16 K rows and 16 V rows of codes (rows
 // padded by 16 bytes against bank conflicts), their scales and a mask of the
-// tokens that count.  A part is heads x D outputs, then heads x (maximum, sum):
+// tokens that count.  Two stages are enough at D = 128 and 256, the next tile being
+// asked for before one is used (2 x 131,072 tokens x 8 KV heads x 128: 97 us, with
+// three 103); small tiles and two sets of heads take three.  A part is heads x D outputs, then heads x (maximum, sum):
 // a warp's first one goes to its place behind the rings, its last one into its
 // own ring, drained by then.
 template <int D, int NT>
 struct Smem {
-  static constexpr int kStages = D == 256 ? 2 : D == 128 ? 3 : 4;
+  static constexpr int kStages = D == 64 || NT == 2 ? 3 : 2;
   static constexpr int kRow = D + 16;
   static constexpr int kStage = 2 * kTile * kRow + 2 * kTile * 4 + 16;
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPart = kHeads * (D + 2) * 4;
-  static constexpr bool kQRegs = D * NT <= 256;  // q fragments in registers, else per warp in shared memory
-  static constexpr int kQ = kQRegs ? 0 : (D / 16) * NT * 32 * 8;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kScan = (kThreads + kWarps + 2) * 4 + 2 * kWarps * 8;
-  static constexpr int kBytes = kWarps * (kRing + kPart + kQ) + kScan;
+  static constexpr int kBytes = kWarps * (kRing + kPart) + kScan;
   static_assert(kRing >= kPart && kRing % 16 == 0 && kPart % 16 == 0, "a part fits a ring");
 };
 
-// CTAs per SM that shared memory (228 KB, 1 KB of it per CTA the system's) leaves room for.
+// CTAs per SM: those that shared memory (228 KB, 1 KB of it per CTA the system's)
+// leaves room for, up to 3, or 4 for D = 64.  (A fourth at D = 128: 2 x 131,072
+// tokens x 8 KV heads 101 us for 97, 37 ragged contexts up to 1,536 22 for 21.)
 template <int D, int NT>
 constexpr int resident() {
-  return 233472 / (Smem<D, NT>::kBytes + 1024) < 8 ? 233472 / (Smem<D, NT>::kBytes + 1024) : 8;
+  constexpr int kFit = 233472 / (Smem<D, NT>::kBytes + 1024), kMost = D == 64 ? 4 : 3;
+  return kFit < kMost ? kFit : kMost;
 }
 
 // Workspace: two parts per CTA (what its list's ends leave), then one record per
@@ -145,7 +148,7 @@ struct Partials {
   __device__ static int4* record(float* ws, int grid, int c) {
     return reinterpret_cast<int4*>(ws + 2ll * grid * kSlot) + c;
   }
-  static size_t bytes(int grid) { return grid == 0 ? 0 : (2 * grid * kSlot + 4 * static_cast<size_t>(grid)) * 4; }
+  static size_t bytes(int grid) { return (2 * grid * kSlot + 4 * static_cast<size_t>(grid)) * 4; }
 };
 
 struct Geometry {
@@ -237,10 +240,10 @@ __device__ __forceinline__ void cluster_barrier() {
 // Joins the parts of a (sequence, group) that a cluster (or one CTA) shares: each
 // CTA its warps', then a warp of the cluster for each query head the CTAs', over
 // distributed shared memory.
-template <typename T, int D, int NT>
+template <typename T, int D>
 __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, const Geometry& g, uint8_t* smem, int2* meta,
                                              bool out4) {
-  using S = Smem<D, NT>;
+  using S = Smem<D, 1>;
   constexpr int kHeads = S::kHeads, E = D / 32, V = E < 4 ? E : 4;
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32, rank = blockIdx.x % g.cs, seg = blockIdx.x / g.cs;
   const int b = seg / g.HG, r = seg - b * g.HG, kh = r / g.NG, left = g.G - (r - kh * g.NG) * kHeads;
@@ -359,9 +362,8 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32, gq = lane / 4, tq = lane % 4;
   uint8_t* ring = smem + w * S::kRing;
   float* first_part = reinterpret_cast<float*>(smem + kWarps * S::kRing + w * S::kPart);
-  uint2* q_smem = reinterpret_cast<uint2*>(smem + kWarps * (S::kRing + S::kPart) + w * S::kQ);
-  uint32_t* before = reinterpret_cast<uint32_t*>(smem + kWarps * (S::kRing + S::kPart + S::kQ));  // [threads]
-  uint32_t* sums = before + kThreads;                                                          // [warps]
+  uint32_t* before = reinterpret_cast<uint32_t*>(smem + kWarps * (S::kRing + S::kPart));  // [threads]
+  uint32_t* sums = before + kThreads;                                                     // [warps]
   int* shared = reinterpret_cast<int*>(sums + kWarps);  // first CTA of the list's first context, last one of its last
   int2* meta = reinterpret_cast<int2*>(shared + 2);     // [2 warps] parts: (sequence x group or -1, opens | closes << 1)
 
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       off -= __shfl_sync(0xffffffffu, inc, 31);
     }
   };
-  if (g.cs) {
+  if (NT == 1 && g.cs) {
     const int seg = blockIdx.x / g.cs, part = blockIdx.x % g.cs * kWarps + w, parts = g.cs * kWarps;
     cur.b = seg / g.HG;
     cur.r = seg % g.HG;
@@ -573,11 +575,11 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     }
   };
   bool going = cur.t < cur.end;
-  if (S::kQRegs && going) ask_q();
+  if (going) ask_q();
   look();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
-  if (!g.cs) {
+  if (NT == 2 || !g.cs) {
     empty_rows(ctas);
     // which CTAs share the contexts at the two ends of this CTA's list (used by the merge, if they are split)
     if (w == 0) {
@@ -600,8 +602,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     const int left = g.G - cur.r % g.NG * kHeads, nh = left < kHeads ? left : kHeads;
     // q as B fragments: lane (head gq, tq) holds, for k step (i, j), the dimensions (tq NCH + i) 16 + 4 j .. + 3, the
     // same that it reads of a K row.  A power of two per head brings them into fp16's range.
-    if (!S::kQRegs) ask_q();
-    uint2 qf[S::kQRegs ? NT * (D / 16) : 1];
+    uint2 qf[NT * (D / 16)];
     float ch[NT][2], m[NT][2], l[NT][2], acc[2 * NW][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -625,13 +626,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       const int e2 = max(static_cast<int>(top >> 23) - 127, -100);
       const float f = pow2i(13 - e2);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint2 x = make_uint2(pack_f16(v[4 * i] * f, v[4 * i + 1] * f), pack_f16(v[4 * i + 2] * f, v[4 * i + 3] * f));
-        if constexpr (S::kQRegs)
-          qf[i * NT + n] = x;
-        else
-          q_smem[(i * NT + n) * 32 + lane] = x;  // read by this lane only
-      }
+      for (int i = 0; i < D / 16; ++i)
+        qf[i * NT + n] =
+            make_uint2(pack_f16(v[4 * i] * f, v[4 * i + 1] * f), pack_f16(v[4 * i + 2] * f, v[4 * i + 3] * f));
       // 2^(e2 - 13), times the scale in units of log 2; a lane's columns are heads 2 tq and 2 tq + 1
       const float mine = a.scale * 1.4426950408889634f * pow2i(e2 - 13);
 #pragma unroll
@@ -651,6 +648,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     for (int t = cur.t; t < cur.end; ++t) {
       cp_wait<kStages - 2>();
       __syncwarp();
+      issue();  // into the stage of the tile before
       const uint8_t* st = ring + get * S::kStage;
       const float* scales = reinterpret_cast<const float*>(st + 2 * kTile * kRow);
       const unsigned mask = *reinterpret_cast<const unsigned*>(st + 2 * kTile * kRow + 2 * kTile * 4);
@@ -670,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           widen(ys[j], a1, a3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint2 b = S::kQRegs ? qf[S::kQRegs ? (i * 4 + j) * NT + n : 0] : q_smem[((i * 4 + j) * NT + n) * 32 + lane];
+            const uint2 b = qf[(i * 4 + j) * NT + n];
             mma16816(s[n], a0, a1, a2, a3, b.x, b.y);
           }
         }
@@ -753,8 +751,6 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
         }
       }
       get = get + 1 == kStages ? 0 : get + 1;
-      __syncwarp();
-      issue();
     }
 
     // ---- the end of the portion: a whole context is written out, a part kept for the CTA's merge
@@ -762,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     const bool closes = cur.end == tiles(cur.tokens);
     const int b = cur.b, r = cur.r;
     going = next_portion(a, g, cur);
-    if (S::kQRegs && going) ask_q();
+    if (going) ask_q();
     float* part = first_portion ? first_part : reinterpret_cast<float*>(ring);
     if (!first_portion && !(opens && closes)) {  // the list's last portion: the ring is done with
       cp_wait<0>();
@@ -798,10 +794,11 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     first_portion = false;
   }
   cp_wait<0>();
-  if (g.cs) {
-    cluster_join<T, D, NT>(a, g, smem, meta, out4);
-    return;
-  }
+  if constexpr (NT == 1)
+    if (g.cs) {
+      cluster_join<T, D>(a, g, smem, meta, out4);
+      return;
+    }
   __syncthreads();
   tb::pdl_trigger();
 
@@ -1037,11 +1034,10 @@ int cluster_of(int segs, int cap, int fit) {
   return 6.5 + 0.85 * ((tiles + cs * kWarps - 1) / (cs * kWarps)) < 10.5 + segs * tiles * 0.0004 ? cs : 0;
 }
 
-// CTAs of the even lists (0: clusters).
-template <int D, int NT>
-int list_grid(int B, int Hq, int Hk, int cap) {
-  const int fit = sm_count() * resident<D, NT>(), G = Hq / Hk;
-  return cluster_of(B * Hk * ((G + 8 * NT - 1) / (8 * NT)), cap, fit) ? 0 : fit;
+// CTAs of a cluster for each (sequence, eight query heads), or 0: even lists.
+template <int D>
+int clusters(int B, int Hq, int Hk, int cap) {
+  return cluster_of(B * Hk * ((Hq / Hk + 7) / 8), cap, sm_count() * resident<D, 1>());
 }
 
 template <int D, int NT>
@@ -1055,7 +1051,7 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a) {
   for (int i = 0; i < 31; ++i)
     if (a.cache.bs == 1 << i) g.shift = i;
   g.tile_pages = a.cache.bs % kTile == 0;
-  g.cs = cluster_of(a.B * g.HG, g.cap, sm_count() * resident<D, NT>());
+  g.cs = NT == 1 ? clusters<D>(a.B, a.Hq, a.cache.Hk, g.cap) : 0;
   return g;
 }
 
@@ -1083,7 +1079,7 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
     kernel<<<cfg.gridDim, kThreads, S::kBytes, s>>>(a, g, q8, out4);
     return static_cast<int>(cudaGetLastError());
   }
-  const int grid = list_grid<D, NT>(a.B, a.Hq, a.cache.Hk, g.cap);
+  const int grid = sm_count() * resident<D, NT>();
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
   kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, q8, out4);
   const cudaError_t e1 = cudaGetLastError();
@@ -1098,33 +1094,48 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_attn_quant_join_kernel<T, D, NT>, a, g, grid, out4));
 }
 
-// 16 columns where more than 8 query heads share a KV head, else 8.
+// Query heads that a warp takes, in eights: two where more than 8 share a KV head,
+// which widens the pages once for both (64 x 1,000 tokens x 8 KV heads, 16 query heads
+// on each: 49 us against 56 with one), but in clusters one, for the shorter way of a
+// tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2), and for D = 256 one, whose
+// output fills the registers (64 x 1,000 x 4 KV heads, 16 on each: 53 against 59).
+template <int D>
+bool take_two(int B, int Hq, int Hk, int cap) {
+  return D < 256 && Hq / Hk > 8 && clusters<D>(B, Hq, Hk, cap) == 0;
+}
+
+template <typename T, int D>
+int launch_dim(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
+  if constexpr (D < 256)
+    if (take_two<D>(a.B, a.Hq, a.cache.Hk, a.cache.max_blocks * a.cache.bs)) return launch<T, D, 2>(a, s);
+  return launch<T, D, 1>(a, s);
+}
+
 template <typename T>
 int launch_type(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
-  const bool two = a.Hq / a.cache.Hk > 8;
   switch (a.cache.D) {
-    case 64: return two ? launch<T, 64, 2>(a, s) : launch<T, 64, 1>(a, s);
-    case 128: return two ? launch<T, 128, 2>(a, s) : launch<T, 128, 1>(a, s);
-    case 256: return two ? launch<T, 256, 2>(a, s) : launch<T, 256, 1>(a, s);
+    case 64: return launch_dim<T, 64>(a, s);
+    case 128: return launch_dim<T, 128>(a, s);
+    case 256: return launch_dim<T, 256>(a, s);
   }
   return static_cast<int>(cudaErrorInvalidValue);
+}
+
+template <int D>
+size_t ws_bytes(int B, int Hq, int Hk, int cap) {
+  if (clusters<D>(B, Hq, Hk, cap)) return 0;
+  return take_two<D>(B, Hq, Hk, cap) ? Partials<D, 2>::bytes(sm_count() * resident<D, 2>())
+                                     : Partials<D, 1>::bytes(sm_count() * resident<D, 1>());
 }
 
 }  // namespace
 
 extern "C" size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens) {
   if (B <= 0 || Hk <= 0) return 0;
-  const bool two = Hq / Hk > 8;
   switch (D) {
-    case 64:
-      return two ? Partials<64, 2>::bytes(list_grid<64, 2>(B, Hq, Hk, max_tokens))
-                 : Partials<64, 1>::bytes(list_grid<64, 1>(B, Hq, Hk, max_tokens));
-    case 128:
-      return two ? Partials<128, 2>::bytes(list_grid<128, 2>(B, Hq, Hk, max_tokens))
-                 : Partials<128, 1>::bytes(list_grid<128, 1>(B, Hq, Hk, max_tokens));
-    case 256:
-      return two ? Partials<256, 2>::bytes(list_grid<256, 2>(B, Hq, Hk, max_tokens))
-                 : Partials<256, 1>::bytes(list_grid<256, 1>(B, Hq, Hk, max_tokens));
+    case 64: return ws_bytes<64>(B, Hq, Hk, max_tokens);
+    case 128: return ws_bytes<128>(B, Hq, Hk, max_tokens);
+    case 256: return ws_bytes<256>(B, Hq, Hk, max_tokens);
   }
   return 0;
 }

@@ -466,6 +466,30 @@ def test_attention_split_and_joined(lens, Hq, Hk, D, bs, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,Hq,Hk,D,bs", [([0, 1, 17, 900, 31] * 60, 16, 1, 128, 16), ([0, 1, 17, 900, 31] * 60, 40, 2, 64, 7),
+                                             ([0, 3, 400] * 120, 33, 1, 256, 64), ([50000, 3, 0], 32, 1, 128, 16),
+                                             ([70000], 9, 1, 64, 8), ([20000, 20000], 17, 1, 256, 24),
+                                             ([90000], 24, 1, 64, 64), ([5000] * 30, 128, 2, 128, 128)])
+def test_attention_many_heads_on_one(lens, Hq, Hk, D, bs, dtype, dev):
+    """9 and more query heads on a KV head, with fewer than eight for some of the warps that share its pages."""
+    g = torch.Generator().manual_seed(3)
+    table, nb = pages(lens, bs, dev)
+    c = random_cache(nb, Hk, bs, D, dev, g)
+    q = torch.randn(len(lens), Hq, D, generator=g).to(dtype).to(dev)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=dev)
+    out = decode_attention_quant(q, *c, table, ctx, out=torch.full_like(q, float("nan")))
+    some = list(range(0, len(lens), max(1, len(lens) // 12)))
+    check_attention(out[some], q[some], c, table[some], [lens[i] for i in some], D ** -0.5)
+    assert torch.isfinite(out).all()
+    # the same bits again, and from rows without alignment
+    row = torch.zeros(len(lens), Hq * D + 1, dtype=dtype, device=dev)
+    row[:, 1:] = q.view(len(lens), -1)
+    for x in (q, row[:, 1:].view(len(lens), Hq, D)):
+        assert torch.equal(decode_attention_quant(x, *c, table, ctx, out=torch.full_like(q, float("nan"))), out)
+
+
+@pytest.mark.gpu
 def test_streams_and_two_captured_graphs(dev):
     """Two graphs of the same call on different data, replayed in turn and at once on two streams; contexts that grow
     between replays are read from the device."""
