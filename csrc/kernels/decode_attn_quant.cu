@@ -108,9 +108,9 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 // padded by 16 bytes against bank conflicts), their scales and a mask of the
 // tokens that count.  Two stages are enough at D = 128 and 256, the next tile being
 // asked for before one is used (2 x 131,072 tokens x 8 KV heads x 128: 97 us, with
-// three 103); small tiles and two sets of heads take three.  A part is heads x D outputs, then heads x (maximum, sum):
-// a warp's first one goes to its place behind the rings, its last one into its
-// own ring, drained by then.
+// three 103); small tiles and two sets of heads take three.  A part is heads x D
+// outputs, then heads x (maximum, sum): a warp's first one goes to its place behind
+// the rings, its last one into its own ring, drained by then.
 template <int D, int NT>
 struct Smem {
   static constexpr int kStages = D == 64 || NT == 2 ? 3 : 2;

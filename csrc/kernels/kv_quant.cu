@@ -12,10 +12,9 @@
 // the row read back NaN or infinite: nothing is silently clipped.
 //
 // Reads and writes are one pass over the rows and a few operations per element.
-// On one B200 at D = 128 in bf16: read of 84 K tokens x 8 KV heads (522 MB) 97 us,
-// 5.4 TB/s; write of 23 K tokens among 49 K rows x 8 KV heads (143 MB) 34 us, bound by
-// instruction issue (2.5 of 4 per cycle); a decode step of 512 tokens with rotary 4
-// us, launch and one chain of loads.
+// On one B200 at D = 128 in bf16: read of 84 K tokens x 8 KV heads (522 MB) 94 us,
+// 5.5 TB/s; write of 23 K tokens among 49 K rows x 8 KV heads (143 MB) 28 us, 5.1 TB/s;
+// a decode step of 512 tokens with rotary 4 us, launch and one chain of loads.
 #include <math.h>
 
 #include "device_common.cuh"
