@@ -37,7 +37,8 @@ int type_of(const at::Tensor& t, const char* op) {
 
 // [T, H, D] rows with a contiguous last dimension.
 void rows3(const at::Tensor& t, const char* op, const char* m) {
-  chk(t.dim() == 3 && (t.size(2) <= 1 || t.stride(2) == 1) && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX, op, m);
+  chk(t.dim() == 3 && (t.size(2) <= 1 || t.stride(2) == 1) && t.size(0) <= INT_MAX, op, m);
+  chk(t.size(2) == 0 || t.size(1) <= INT_MAX / t.size(2), op, "at most 2^31 - 1 elements per row");
 }
 
 // Bytes [lo, hi) that a view touches (empty: lo == hi).
@@ -202,6 +203,7 @@ TbQuantCache cache_of(const at::Tensor& kc, const at::Tensor& vc, const at::Tens
   const int64_t D = kc.size(3);
   chk(D == 64 || D == 128 || D == 256, op, "head dimension 64, 128 or 256");
   chk(kc.size(1) >= 1 && kc.size(2) >= 1, op, "at least one KV head and one slot per block");
+  chk(kc.size(1) <= INT_MAX / D && kc.size(2) <= INT_MAX, op, "at most 2^31 - 1 elements per token, slots per block");
   chk(kc.size(0) * kc.size(1) * kc.size(2) <= INT_MAX, op, "at most 2^31 - 1 rows (blocks x heads x slots)");
   chk(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.is_contiguous() &&
           block_table.size(0) <= INT_MAX && block_table.size(1) <= INT_MAX / kc.size(2),

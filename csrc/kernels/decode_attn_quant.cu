@@ -1146,7 +1146,7 @@ extern "C" int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cuda
   if (a.cache.Hk <= 0 || a.Hq % a.cache.Hk || a.cache.bs <= 0 || a.cache.num_seqs != a.B ||
       a.cache.max_blocks < 0 || a.cache.max_blocks > 0x7fffffff / a.cache.bs || a.cache.num_blocks < 0 ||
       static_cast<long long>(a.cache.num_blocks) * a.cache.Hk > 0x7fffffff / a.cache.bs ||
-      a.B > 0x7fffffff / a.Hq)
+      a.B > 0x7fffffff / a.Hq || static_cast<long long>(a.Hq) * a.cache.D > 0x7fffffff)
     return static_cast<int>(cudaErrorInvalidValue);
   if (a.dtype == TB_BF16) return launch_type<__nv_bfloat16>(a, s);
   if (a.dtype == TB_F16) return launch_type<__half>(a, s);

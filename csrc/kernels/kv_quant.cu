@@ -356,7 +356,7 @@ bool rows_aligned(const void* p, long long st, long long sh, int dtype, int byte
 constexpr int kFewWarps = 148 * 16, kSpread = 148 * 8;
 int parts_of(long long groups, int rounds) {
   int n = 1;
-  while (2 * n <= rounds && 2 * n * groups <= kFewWarps) n *= 2;
+  while (2 * n <= rounds && 2 * n * groups <= kFewWarps && 2ll * n * rounds <= 0x7fffffff) n *= 2;
   return n;
 }
 struct Shape {
@@ -405,6 +405,7 @@ int read_as(const TbKvQuantReadArgs& a, cudaStream_t s) {
 
 bool cache_ok(const TbQuantCache& c) {
   return c.Hk > 0 && c.bs > 0 && c.num_blocks >= 0 && (c.D == 64 || c.D == 128 || c.D == 256) &&
+         c.Hk <= 0x7fffffff / c.D &&
          static_cast<long long>(c.num_blocks) * c.Hk <= 0x7fffffff / c.bs;
 }
 

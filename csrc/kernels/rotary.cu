@@ -138,7 +138,8 @@ int launch_type(const TbRotaryArgs& a, cudaStream_t s) {
 extern "C" int tb_rotary(const TbRotaryArgs* args, cudaStream_t s) {
   const TbRotaryArgs& a = *args;
   if (a.T <= 0 || a.H <= 0) return 0;
-  if (a.R <= 0 || a.R % 2 || a.D % 2 || a.R > a.D || a.max_pos <= 0) return static_cast<int>(cudaErrorInvalidValue);
+  if (a.R <= 0 || a.R % 2 || a.D % 2 || a.R > a.D || a.H > 0x7fffffff / a.D || a.max_pos <= 0)
+    return static_cast<int>(cudaErrorInvalidValue);
   switch (a.dtype) {
     case TB_BF16: return launch_type<__nv_bfloat16>(a, s);
     case TB_F16: return launch_type<__half>(a, s);

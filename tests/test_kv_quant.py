@@ -6,7 +6,7 @@ import torch
 
 from turbol_b200.ops import reference as ref
 from turbol_b200.ops.kv_cache import decode_attention_quant, kv_quant_read, kv_quant_write, quant_kv_cache
-from turbol_b200.ops.rotary import rotary_table
+from turbol_b200.ops.rotary import rotary, rotary_table
 
 F8 = torch.float8_e4m3fn
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
@@ -463,6 +463,24 @@ def test_attention_split_and_joined(lens, Hq, Hk, D, bs, dev):
     check_attention(out[some], q[some], c, table[some], [lens[i] for i in some], D ** -0.5)
     for _ in range(3):  # the joins have a fixed order
         assert torch.equal(decode_attention_quant(q, *c, table, ctx, out=torch.full_like(q, float("nan"))), out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sizes_past_31_bits_are_refused(device):
+    """Views and empty tensors of sizes that the kernels do not count to; nothing of them is in memory."""
+    i32 = dict(dtype=torch.int32, device=device)
+    c = quant_kv_cache(2, 1, 16, 64, device)
+    one, table = torch.zeros(1, **i32), torch.zeros(1, 2, **i32)
+    many = torch.zeros(1, 1, 64, device=device).bfloat16().expand(1, 1 << 25, 64)
+    with pytest.raises(ValueError, match="2\\^31"):
+        decode_attention_quant(many, *c, table, one)
+    with pytest.raises(ValueError, match="2\\^31"):
+        rotary(torch.zeros(1, 1, 2, device=device).expand(1, 1 << 30, 2), one, rotary_table(2, 4, device=device))
+    none = torch.zeros(0, device=device)
+    for shape in ((0, 1 << 32, 16, 64), (0, 1 << 25, 16, 64), (0, 1, 1 << 31, 64)):
+        kc, ks = none.to(F8).expand(0).reshape(shape), none.reshape(shape[:3])
+        with pytest.raises(ValueError, match="2\\^31"):
+            decode_attention_quant(torch.zeros(1, 2, 64, device=device).bfloat16(), kc, kc.clone(), ks, ks.clone(), table, one)
 
 
 @pytest.mark.gpu
