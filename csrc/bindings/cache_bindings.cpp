@@ -41,6 +41,12 @@ void rows3(const at::Tensor& t, const char* op, const char* m) {
   chk(t.size(2) == 0 || t.size(1) <= INT_MAX / t.size(2), op, "at most 2^31 - 1 elements per row");
 }
 
+// What has no backward pass refuses tensors that would want one.
+void no_grad(std::initializer_list<const at::Tensor*> ts, const char* op) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts) chk(!t->requires_grad(), op, "has no gradient (call it under torch.no_grad)");
+}
+
 // Bytes [lo, hi) that a view touches (empty: lo == hi).
 struct Range {
   uintptr_t lo, hi;
@@ -238,6 +244,7 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
   rows3(v, op, "v is [T, Hk, D] with a contiguous last dimension");
   a.rot.dtype = type_of(k, op);
   chk(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), op, "k and v have the same shape and type");
+  no_grad({&k, &v}, op);
   chk(k.size(1) == a.cache.Hk && k.size(2) == a.cache.D, op, "k has the cache's heads and head dimension");
   const int64_t T = k.size(0);
   index1(seq, T, op, "seq_of_token is a contiguous int32 [T]");
@@ -267,6 +274,7 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
         "q has k's rows, head dimension and type");
     chk(q_->device() == dev, op, "all tensors on one device");
     chk(apart_from_all(range_of(*q_), caches), op, "q overlaps the cache");
+    no_grad({&*q_}, op);
   }
   if (q_out_) {
     rows3(*q_out_, op, "q_out is [T, Hq, D] with a contiguous last dimension");
@@ -274,6 +282,7 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
         "q_out has q's shape and type");
     chk(q_out_->device() == dev, op, "all tensors on one device");
     chk(rows_distinct(*q_out_), op, "q_out has overlapping rows");
+    no_grad({&*q_out_}, op);
     chk(same_view(*q_, *q_out_) || columns_apart(*q_, *q_out_), op, "q_out is q itself or does not overlap it");
     chk(columns_apart(*q_out_, k) && columns_apart(*q_out_, v), op, "q_out overlaps k or v");
     const Range out = range_of(*q_out_);
@@ -326,6 +335,7 @@ bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
   index1(pos, T, op, "pos is a contiguous int32 [T]");
   for (const at::Tensor* t : {&k_out, &v_out, &seq, &pos}) chk(t->device() == dev, op, "all tensors on one device");
   chk(rows_distinct(k_out) && rows_distinct(v_out), op, "out has overlapping rows");
+  no_grad({&k_out, &v_out}, op);
   chk(columns_apart(k_out, v_out), op, "the two outputs overlap");
   const Range outs[2] = {range_of(k_out), range_of(v_out)};
   for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &seq, &pos, &block_table})
@@ -358,6 +368,7 @@ Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::
   a.dtype = type_of(q, op);
   chk(a.dtype != TB_F32, op, "bf16 or fp16 q");
   chk(q.size(2) == a.cache.D, op, "q has the cache's head dimension");
+  no_grad({&q}, op);
   chk(q.size(1) >= 1 && q.size(1) % a.cache.Hk == 0, op, "the query heads are a multiple of the KV heads");
   const int64_t B = q.size(0);
   chk(block_table.size(0) == B, op, "one block_table row per sequence");
@@ -370,6 +381,7 @@ Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::
     chk(out_->device() == dev, op, "all tensors on one device");
     chk(rows_distinct(*out_), op, "out has overlapping rows");
     chk(columns_apart(*out_, q), op, "out overlaps q");
+    no_grad({&*out_}, op);
     const Range out = range_of(*out_);
     for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &ctx_len, &block_table})
       chk(apart(out, range_of(*t)), op, "out overlaps an input");

@@ -466,6 +466,27 @@ def test_attention_split_and_joined(lens, Hq, Hk, D, bs, dev):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_gradients_are_refused(device):
+    """No silent break in an autograd graph: outside no_grad, what requires a gradient raises, and inside it runs."""
+    i32 = dict(dtype=torch.int32, device=device)
+    c = quant_kv_cache(2, 1, 16, 64, device)
+    table, seq, pos, ctx = torch.zeros(2, 1, **i32), torch.zeros(2, **i32), torch.arange(2, **i32), torch.ones(2, **i32)
+    x, q = torch.ones(2, 1, 64, device=device).bfloat16(), torch.ones(2, 4, 64, device=device).bfloat16()
+    rt, leaf = rotary_table(64, 8, device=device), lambda t: t.clone().requires_grad_()
+    calls = [lambda: kv_quant_write(leaf(x), x, seq, pos, table, *c), lambda: kv_quant_write(x, leaf(x), seq, pos, table, *c),
+             lambda: kv_quant_write(x, x, seq, pos, table, *c, q=leaf(q), table=rt),
+             lambda: kv_quant_write(x, x, seq, pos, table, *c, q=q, q_out=leaf(q), table=rt),
+             lambda: kv_quant_read(*c, seq, pos, table, out=(leaf(x), x.clone())),
+             lambda: decode_attention_quant(leaf(q), *c, table, ctx),
+             lambda: decode_attention_quant(q, *c, table, ctx, out=leaf(q))]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_sizes_past_31_bits_are_refused(device):
     """Views and empty tensors of sizes that the kernels do not count to; nothing of them is in memory."""
     i32 = dict(dtype=torch.int32, device=device)

@@ -59,7 +59,8 @@ def kv_quant_write(k: torch.Tensor, v: torch.Tensor, seq_of_token: torch.Tensor,
     A token with a negative position or sequence is padding: nothing is written
     and its q row is copied.  A sequence, position or block out of range writes
     nothing and sets ``error``; a position beyond the table also makes the q row
-    NaN.  No two tokens of a call may name the same slot.  Not differentiable."""
+    NaN.  No two tokens of a call may name the same slot.  Not differentiable:
+    tensors that require a gradient are refused outside torch.no_grad."""
     y = _call("kv_quant_write", k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q, q_out, table, interleaved, error)
     if not kc.is_cuda:
         y = torch.empty_like(q) if q is not None and q_out is None else q_out
@@ -88,11 +89,11 @@ def decode_attention_quant(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, 
                            out: Optional[torch.Tensor] = None, error: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one token per sequence, q [B, Hq, D] (bf16 or fp16), over the
     first ctx_len[b] (int32) tokens of row b of ``block_table``: [B, Hq, D], q's
-    type.  Query head h reads KV head h // (Hq / Hk).  scale: default
-    1 / sqrt(D).  An empty context gives zeros.  Tokens behind the table or in
-    blocks out of range are left out and set ``error``.  Weights are rounded to
-    fp16 (sums stay in fp32).  The result does not
-    depend on what the pages hold behind a context; it can depend, within
+    type, without a backward pass (as :func:`kv_quant_write`).  Query head h reads
+    KV head h // (Hq / Hk).  scale: default 1 / sqrt(D).  An empty context gives
+    zeros.  Tokens behind the table or in blocks out of range are left out and set
+    ``error``.  Weights are rounded to fp16 (sums stay in fp32).  The result does
+    not depend on what the pages hold behind a context; it can depend, within
     rounding, on the other sequences of the batch (where contexts are split)."""
     y = _call("decode_attention_quant", q, kc, vc, ks, vs, block_table, ctx_len, out, scale, error)
     if y is None:
