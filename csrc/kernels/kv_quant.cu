@@ -12,8 +12,8 @@
 // the row read back NaN or infinite: nothing is silently clipped.
 //
 // Reads and writes are one pass over the rows and a few operations per element.
-// On one B200 at D = 128 in bf16: read of 84 K tokens x 8 KV heads (522 MB) 94 us,
-// 5.5 TB/s; write of 23 K tokens among 49 K rows x 8 KV heads (143 MB) 28 us, 5.1 TB/s;
+// On one B200 at D = 128 in bf16: read of 84 K tokens x 8 KV heads (522 MB) 86 us,
+// 6.0 TB/s; write of 23 K tokens among 49 K rows x 8 KV heads (143 MB) 28 us, 5.1 TB/s;
 // a decode step of 512 tokens with rotary 4 us, launch and one chain of loads.
 #include <math.h>
 
@@ -295,9 +295,27 @@ __global__ void __launch_bounds__(128) kv_quant_write_rot_kernel(TbKvQuantWriteA
   }
 }
 
-// D / 16 lanes per row, sixteen codes each, four heads in flight.
+// Sixteen values to a multiple of 32 bytes: whole sectors per store (two stores of
+// 16 bytes leave each sector to be put together: 84 K tokens x 8 KV heads x 128 in
+// bf16 94 us for 86, in fp32 168 for 140).
+template <typename T>
+__device__ __forceinline__ void store_sectors(T* p, const float (&f)[16]) {
+  constexpr int W = 4 * sizeof(T);
+  uint32_t w[W];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) reinterpret_cast<T*>(w)[i] = tb::from_f32<T>(f[i]);
+#pragma unroll
+  for (int i = 0; i < W; i += 8)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(p) + i),
+                 "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
+                 "r"(w[i + 7])
+                 : "memory");
+}
+
+// D / 16 lanes per row, sixteen codes each, four heads in flight (as fast as two or
+// eight).  align: what rows start on a multiple of, 32, 16 or fewer bytes.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv_quant_read_kernel(TbKvQuantReadArgs a, Split sp, bool aligned) {
+__global__ void __launch_bounds__(128) kv_quant_read_kernel(TbKvQuantReadArgs a, Split sp, int align) {
   constexpr int L = D / 16, G = 32 / L, U = 4;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk;
   const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, group = item / sp.parts, t = group * G + lane / L;
@@ -333,7 +351,9 @@ __global__ void __launch_bounds__(128) kv_quant_read_kernel(TbKvQuantReadArgs a,
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[4 * j + e] = q[e] * s[u];
       }
-      if (aligned) {
+      if (align == 32) {
+        store_sectors<T>(y, f);
+      } else if (align == 16) {
         tb::store_vec<T, 16>(y, f);
       } else {
 #pragma unroll
@@ -394,12 +414,14 @@ int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
 template <typename T, int D>
 int read_as(const TbKvQuantReadArgs& a, cudaStream_t s) {
   constexpr int G = 32 / (D / 16);
-  const bool al = rows_aligned(a.k, a.ks_t, a.ks_h, a.dtype, 16) && rows_aligned(a.v, a.vs_t, a.vs_h, a.dtype, 16);
+  auto on = [&](int bytes) {
+    return rows_aligned(a.k, a.ks_t, a.ks_h, a.dtype, bytes) && rows_aligned(a.v, a.vs_t, a.vs_h, a.dtype, bytes);
+  };
   const long long groups = (a.T + G - 1ll) / G;
   Split sp = {1, 2 * a.cache.Hk};
   sp.parts = parts_of(groups, sp.slots);
   const Shape g(groups * sp.parts);
-  kv_quant_read_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, al);
+  kv_quant_read_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, on(32) ? 32 : on(16) ? 16 : 0);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -466,6 +466,28 @@ def test_attention_split_and_joined(lens, Hq, Hk, D, bs, dev):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_read_at_every_alignment(D, dtype, device):
+    """Rows that start on multiples of 32, 16 and fewer bytes: code * scale rounded once, and the gaps as they were."""
+    lens, Hk, bs = [37, 5], 3, 8
+    table, nb = pages(lens, bs, device)
+    c = random_cache(nb, Hk, bs, D, device, torch.Generator().manual_seed(6))
+    seq, pos = tokens_of(lens, device)
+    blk, slot = where(seq, pos, table, bs)
+    want = [(bits(x)[blk, :, slot].view(F8).double() * s[blk, :, slot].double()[..., None]).float().to(dtype)
+            for x, s in ((c.kc, c.ks), (c.vc, c.vs))]
+    T, pad = pos.numel(), 32
+    for shift in (0, 1, 2, 4, 8, 12, 16):
+        buf = [torch.full((T * Hk * (D + pad) + shift,), 7.0, dtype=dtype, device=device) for _ in range(2)]
+        rows = [b[shift:].view(T, Hk, D + pad) for b in buf]
+        kv_quant_read(*c, seq, pos, table, out=(rows[0][..., :D], rows[1][..., :D]))
+        for b, r, w in zip(buf, rows, want):
+            assert torch.equal(r[..., :D], w)
+            assert (r[..., D:] == 7).all() and (b[:shift] == 7).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradients_are_refused(device):
     """No silent break in an autograd graph: outside no_grad, what requires a gradient raises, and inside it runs."""
     i32 = dict(dtype=torch.int32, device=device)
