@@ -488,6 +488,27 @@ def test_read_at_every_alignment(D, dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_write_at_every_alignment(D, dtype, device):
+    """Rows that start on multiples of 32, 16 and fewer bytes: the formula's bits, with 1 to 9 KV heads in flight."""
+    for Hk, shift in ((1, 0), (2, 1), (3, 2), (5, 4), (9, 8), (4, 12), (2, 16)):
+        lens, bs = [37, 1, 5], 8
+        table, nb = pages(lens, bs, device)
+        seq, pos = tokens_of(lens, device)
+        T, pad = pos.numel(), 32
+        g = torch.Generator().manual_seed(D + shift)
+        rows = [torch.randn(T * Hk * (D + pad) + shift, generator=g).to(dtype).to(device)[shift:].view(T, Hk, D + pad)
+                for _ in range(2)]
+        c = quant_kv_cache(nb, Hk, bs, D, device)
+        kv_quant_write(rows[0][..., :D], rows[1][..., :D], seq, pos, table, *c)
+        blk, slot = where(seq, pos, table, bs)
+        for r, code, scale in ((rows[0], c.kc, c.ks), (rows[1], c.vc, c.vs)):
+            cc, ss = ref.kv_quantise(r[..., :D].cpu())
+            assert torch.equal(bits(code)[blk, :, slot].cpu(), bits(cc)) and torch.equal(scale[blk, :, slot].cpu(), ss)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradients_are_refused(device):
     """No silent break in an autograd graph: outside no_grad, what requires a gradient raises, and inside it runs."""
     i32 = dict(dtype=torch.int32, device=device)
