@@ -37,9 +37,10 @@
 //    and most tiles need no reduction over the warp and no rescaling.  q is
 //    brought into fp16 range by a power of two per head (exact).
 //
-// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 97 us,
-// 5.7 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 30 us; 1 x
+// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 96 us,
+// 5.8 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 30 us; 1 x
 // 1,000 tokens x 8 KV heads 7.5 us.
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -57,6 +58,7 @@ constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that
 constexpr int kStart = 3;       // what beginning a (sequence, group) costs a warp, in tiles
 constexpr int kMostCluster = 8;   // CTAs of a cluster (the portable bound)
 constexpr float kMinVsLog = -100.f;
+constexpr float kLowest = -FLT_MAX;  // the reference before the first token: below every score, and finite
 constexpr float kSlack = 8.f;   // the reference of the weights may lag behind their maximum by a factor of 2^8
 
 // The four codes of a word as two fp16 pairs.
@@ -489,27 +491,37 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   if (lane == 0) meta[2 * w] = meta[2 * w + 1] = make_int2(-1, 0);
 
   // ---- prefetch: a cursor that runs ahead, and where its next tile lies: with pages of whole tiles the tile's first row
-  // and its number of tokens, else (lanes 0-15) each token's row
+  // and its number of tokens (32 tiles looked up at once), else (lanes 0-15) each token's row
   Cursor pre = cur;
   bool more = true;
   int row = -1, count = 0, pre_kh = cur.r / g.NG;
+  int rows = -1, first = 0, last = 0;  // with pages of whole tiles: a lane for each of the tiles [first, last)
+  auto row_of = [&](int tok) {
+    const int pb = g.shift >= 0 ? tok >> g.shift : tok / c.bs;
+    const int blk = c.block_table[static_cast<long long>(pre.b) * c.max_blocks + pb];
+    if (blk >= 0 && blk < c.num_blocks) return (blk * c.Hk + pre_kh) * c.bs + (tok - pb * c.bs);
+    if (a.err) atomicCAS(a.err, 0, 1);
+    return -1;
+  };
   auto look = [&]() {
     if (more && pre.t >= pre.end) {
       more = next_portion(a, g, pre);
       pre_kh = pre.r / g.NG;
+      last = 0;
     }
     if (!more) return;
-    const int tok = pre.t * kTile + (g.tile_pages ? 0 : lane);
-    row = -1;
-    if (g.tile_pages || (lane < kTile && tok < pre.tokens)) {
-      const int pb = g.shift >= 0 ? tok >> g.shift : tok / c.bs;
-      const int blk = c.block_table[static_cast<long long>(pre.b) * c.max_blocks + pb];
-      if (blk >= 0 && blk < c.num_blocks)
-        row = (blk * c.Hk + pre_kh) * c.bs + (tok - pb * c.bs);
-      else if (a.err)
-        atomicCAS(a.err, 0, 1);
+    if (g.tile_pages) {
+      if (pre.t >= last) {
+        first = pre.t;
+        last = min(first + 32, pre.end);
+        rows = first + lane < last ? row_of((first + lane) * kTile) : -1;
+      }
+      row = __shfl_sync(0xffffffffu, rows, pre.t - first);
+      count = row < 0 ? 0 : min(pre.tokens - pre.t * kTile, kTile);
+    } else {
+      const int tok = pre.t * kTile + lane;
+      row = lane < kTile && tok < pre.tokens ? row_of(tok) : -1;
     }
-    if (g.tile_pages) count = row < 0 ? 0 : min(pre.tokens - tok, kTile);
   };
   const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   constexpr int kChunks = D / 16, kRows = 32 / kChunks;  // chunks per row, rows per instruction
@@ -634,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         ch[n][e] = __shfl_sync(0xffffffffu, mine, (2 * tq + e) * 4);
-        m[n][e] = -INFINITY;
+        m[n][e] = kLowest;
         l[n][e] = 0.f;
       }
     }
@@ -673,30 +685,31 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
           }
         }
       }
-      // weights of tokens gq and gq + 8 for heads 2 tq and 2 tq + 1
-      const float k0 = scales[gq], k1 = scales[gq + 8], v0 = scales[kTile + gq], v1 = scales[kTile + gq + 8];
+      // weights of tokens gq and gq + 8 for heads 2 tq and 2 tq + 1; tokens that do not count have a score of -inf
       const bool in0 = mask >> gq & 1, in1 = mask >> (gq + 8) & 1;
+      const float k0 = scales[gq], k1 = scales[gq + 8];
+      const float v0 = in0 ? scales[kTile + gq] : 0.f, v1 = in1 ? scales[kTile + gq + 8] : 0.f;
       const float e0 = fmaxf(log2_fast(v0), kMinVsLog), e1 = fmaxf(log2_fast(v1), kMinVsLog);
       bool grew = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[n][e] = s[n][e] * ch[n][e] * k0;
-          s[n][2 + e] = s[n][2 + e] * ch[n][e] * k1;
-          grew |= (in0 && s[n][e] + e0 > m[n][e] + kSlack) || (in1 && s[n][2 + e] + e1 > m[n][e] + kSlack);
+          s[n][e] = in0 ? s[n][e] * ch[n][e] * k0 : -INFINITY;
+          s[n][2 + e] = in1 ? s[n][2 + e] * ch[n][e] * k1 : -INFINITY;
+          grew |= fmaxf(s[n][e] + e0, s[n][2 + e] + e1) > m[n][e] + kSlack;
         }
       if (__any_sync(0xffffffffu, grew)) {  // the maximum outran the reference: move it, and what was summed with it
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(in0 ? s[n][e] + e0 : -INFINITY, in1 ? s[n][2 + e] + e1 : -INFINITY);
+            float top = fmaxf(s[n][e] + e0, s[n][2 + e] + e1);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             top = fmaxf(top, m[n][e]);
-            const float cor = top == -INFINITY ? 1.f : exp2_fast(m[n][e] - top);
+            const float cor = exp2_fast(m[n][e] - top);
             m[n][e] = top;
             l[n][e] *= cor;
 #pragma unroll
@@ -712,13 +725,12 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
         float p[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float mr = m[n][e] == -INFINITY ? 0.f : m[n][e];
-          p[e] = in0 ? exp2_fast(s[n][e] - mr) : 0.f;
-          p[2 + e] = in1 ? exp2_fast(s[n][2 + e] - mr) : 0.f;
+          p[e] = exp2_fast(s[n][e] - m[n][e]);
+          p[2 + e] = exp2_fast(s[n][2 + e] - m[n][e]);
           l[n][e] += p[e] + p[2 + e];
         }
-        wb[n][0] = transpose8x8(pack_f16(in0 ? p[0] * v0 : 0.f, in0 ? p[1] * v0 : 0.f));
-        wb[n][1] = transpose8x8(pack_f16(in1 ? p[2] * v1 : 0.f, in1 ? p[3] * v1 : 0.f));
+        wb[n][0] = transpose8x8(pack_f16(p[0] * v0, p[1] * v0));
+        wb[n][1] = transpose8x8(pack_f16(p[2] * v1, p[3] * v1));
       }
       // O^T [16 dimensions, heads] += V^T w: bytes of neighbouring tokens are paired before they are widened
       const uint8_t* vr = st + kTile * kRow + 2 * tq * kRow;
@@ -1096,9 +1108,9 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
 
 // Query heads that a warp takes, in eights: two where more than 8 share a KV head,
 // which widens the pages once for both (64 x 1,000 tokens x 8 KV heads, 16 query heads
-// on each: 49 us against 56 with one), but in clusters one, for the shorter way of a
+// on each: 43 us against 56 with one), but in clusters one, for the shorter way of a
 // tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2), and for D = 256 one, whose
-// output fills the registers (64 x 1,000 x 4 KV heads, 16 on each: 53 against 59).
+// output fills the registers (64 x 1,000 x 4 KV heads, 16 on each: 50 against 59).
 template <int D>
 bool take_two(int B, int Hq, int Hk, int cap) {
   return D < 256 && Hq / Hk > 8 && clusters<D>(B, Hq, Hk, cap) == 0;
