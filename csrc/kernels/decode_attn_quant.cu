@@ -127,12 +127,16 @@ struct Smem {
 };
 
 // CTAs per SM: those that shared memory (228 KB, 1 KB of it per CTA the system's)
-// leaves room for, up to 3, or 4 for D = 64.  (A fourth at D = 128: 2 x 131,072
-// tokens x 8 KV heads 101 us for 97, 37 ragged contexts up to 1,536 22 for 21.)
+// leaves room for, up to 4.  Lists at D = 128 have three of them: with four, 2 x
+// 131,072 tokens x 8 KV heads took 101 us for 96, and no mix of contexts gained over 2%.
 template <int D, int NT>
 constexpr int resident() {
-  constexpr int kFit = 233472 / (Smem<D, NT>::kBytes + 1024), kMost = D == 64 ? 4 : 3;
-  return kFit < kMost ? kFit : kMost;
+  constexpr int kFit = 233472 / (Smem<D, NT>::kBytes + 1024);
+  return kFit < 4 ? kFit : 4;
+}
+template <int D, int NT>
+constexpr int list_ctas() {
+  return D == 128 && resident<D, NT>() > 3 ? 3 : resident<D, NT>();
 }
 
 // Workspace: two parts per CTA (what its list's ends leave), then one record per
@@ -351,8 +355,11 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
   cluster_barrier();  // nobody leaves while another still reads its shared memory
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, resident<D, NT>())
+// kClusters: a cluster (or one CTA) for each (sequence, eight query heads), else even
+// lists: two kernels, since what a CTA does not need costs it instruction fetches (one
+// short context: 4.3 us, from one kernel for both 5.1).
+template <typename T, int D, int NT, bool kClusters>
+__global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list_ctas<D, NT>())
     decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool q8, bool out4) {
   using S = Smem<D, NT>;
   using P = Partials<D, NT>;
@@ -425,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
       off -= __shfl_sync(0xffffffffu, inc, 31);
     }
   };
-  if (NT == 1 && g.cs) {
+  if constexpr (kClusters) {
     const int seg = blockIdx.x / g.cs, part = blockIdx.x % g.cs * kWarps + w, parts = g.cs * kWarps;
     cur.b = seg / g.HG;
     cur.r = seg % g.HG;
@@ -591,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
   look();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue();
-  if (NT == 2 || !g.cs) {
+  if constexpr (!kClusters) {
     empty_rows(ctas);
     // which CTAs share the contexts at the two ends of this CTA's list (used by the merge, if they are split)
     if (w == 0) {
@@ -806,11 +813,10 @@ __global__ void __launch_bounds__(kThreads, resident<D, NT>())
     first_portion = false;
   }
   cp_wait<0>();
-  if constexpr (NT == 1)
-    if (g.cs) {
-      cluster_join<T, D>(a, g, smem, meta, out4);
-      return;
-    }
+  if constexpr (kClusters) {
+    cluster_join<T, D>(a, g, smem, meta, out4);
+    return;
+  }
   __syncthreads();
   tb::pdl_trigger();
 
@@ -1031,11 +1037,13 @@ int sm_count() {  // of the current device, asked for once
 // How the work of `segs` (sequence, group) pairs with contexts of up to `cap`
 // tokens is dealt out: a cluster of so many CTAs for each pair, or 0, the even
 // lists.  The lists pay for their start and for the joining kernel, a cluster for
-// the longest context, with a warp's latency per tile.  Measured on one B200 (D =
-// 128): lists 10.5 us and 0.76 ns per tile, of which contexts of mixed lengths have
-// half of `cap`; clusters 6.5 us and 0.85 us per tile of a warp.  1 x 1,000 tokens x
-// 8 KV heads: clusters 7.5 us, lists 10.3; 37 ragged contexts up to 1,536 tokens:
-// clusters 27 us, lists 22.
+// the longest context, with a warp's latency per tile, and for the memory that all
+// of them share.  Measured on one B200 (D = 128): lists 10.5 us and 0.76 ns per tile, of
+// which contexts of mixed lengths have half of `cap`; clusters 5.7 us, 0.85 us per
+// tile of a warp and a fifth of the lists' time for the tiles.  Clusters and lists: 1 x
+// 1,000 tokens x 8 KV heads 6.6 and 10.3 us, 8 x 4,096 x 8 18.3 and 22.7, 37 ragged up to
+// 1,536 x 8 18.7 and 20.8, 64 x 1,000 x 8 27.4 and 33.8 (ragged 21.8 and 22.4), 16 ragged
+// up to 8,000 x 8 37.0 and 32.8.
 // Lists count their units in 31 bits; more take the clusters.
 int cluster_of(int segs, int cap, int fit) {
   const long long tiles = cap / kTile + 1, units = (tiles + kStart) * segs;
@@ -1043,7 +1051,8 @@ int cluster_of(int segs, int cap, int fit) {
   if (segs > fit) return 0;
   int cs = 1;
   while (cs < kMostCluster && 2 * cs * segs <= fit && cs * kWarps < tiles) cs *= 2;
-  return 6.5 + 0.85 * ((tiles + cs * kWarps - 1) / (cs * kWarps)) < 10.5 + segs * tiles * 0.0004 ? cs : 0;
+  const double all = segs * tiles * 0.0004;
+  return 5.7 + 0.85 * ((tiles + cs * kWarps - 1) / (cs * kWarps)) + 0.2 * all < 10.5 + all ? cs : 0;
 }
 
 // CTAs of a cluster for each (sequence, eight query heads), or 0: even lists.
@@ -1071,9 +1080,6 @@ template <typename T, int D, int NT>
 int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   using S = Smem<D, NT>;
   const Geometry g = geometry<D, NT>(a);
-  auto kernel = decode_attn_quant_kernel<T, D, NT>;
-  const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
-  if (e != cudaSuccess) return static_cast<int>(e);
   const bool q8 = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.qs_b % 8 == 0 && a.qs_h % 8 == 0;
   const bool out4 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.os_b % 4 == 0 && a.os_h % 4 == 0;
   cudaLaunchConfig_t cfg = {};
@@ -1082,16 +1088,24 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = s;
   cfg.attrs = attr;
-  if (g.cs) {
-    cfg.gridDim = dim3(a.B * g.HG * g.cs);
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {static_cast<unsigned>(g.cs), 1, 1};
-    cfg.numAttrs = 1;
-    if (g.cs > 1) return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, g, q8, out4));
-    kernel<<<cfg.gridDim, kThreads, S::kBytes, s>>>(a, g, q8, out4);
-    return static_cast<int>(cudaGetLastError());
+  if constexpr (NT == 1) {
+    if (g.cs) {
+      auto kernel = decode_attn_quant_kernel<T, D, 1, true>;
+      const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
+      if (e != cudaSuccess) return static_cast<int>(e);
+      cfg.gridDim = dim3(a.B * g.HG * g.cs);
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim = {static_cast<unsigned>(g.cs), 1, 1};
+      cfg.numAttrs = 1;
+      if (g.cs > 1) return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, g, q8, out4));
+      kernel<<<cfg.gridDim, kThreads, S::kBytes, s>>>(a, g, q8, out4);
+      return static_cast<int>(cudaGetLastError());
+    }
   }
-  const int grid = sm_count() * resident<D, NT>();
+  auto kernel = decode_attn_quant_kernel<T, D, NT, false>;
+  const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int grid = sm_count() * list_ctas<D, NT>();
   if (a.ws == nullptr || a.ws_bytes < Partials<D, NT>::bytes(grid)) return static_cast<int>(cudaErrorInvalidValue);
   kernel<<<grid, kThreads, S::kBytes, s>>>(a, g, q8, out4);
   const cudaError_t e1 = cudaGetLastError();
@@ -1136,8 +1150,8 @@ int launch_type(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
 template <int D>
 size_t ws_bytes(int B, int Hq, int Hk, int cap) {
   if (clusters<D>(B, Hq, Hk, cap)) return 0;
-  return take_two<D>(B, Hq, Hk, cap) ? Partials<D, 2>::bytes(sm_count() * resident<D, 2>())
-                                     : Partials<D, 1>::bytes(sm_count() * resident<D, 1>());
+  return take_two<D>(B, Hq, Hk, cap) ? Partials<D, 2>::bytes(sm_count() * list_ctas<D, 2>())
+                                     : Partials<D, 1>::bytes(sm_count() * list_ctas<D, 1>());
 }
 
 }  // namespace
