@@ -38,8 +38,8 @@
 //    brought into fp16 range by a power of two per head (exact).
 //
 // On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 96 us,
-// 5.8 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 30 us; 1 x
-// 1,000 tokens x 8 KV heads 7.5 us.
+// 5.8 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 28 us; 1 x
+// 1,000 tokens x 8 KV heads 6.1 us.
 #include <float.h>
 #include <math.h>
 
@@ -357,10 +357,13 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
 
 // kClusters: a cluster (or one CTA) for each (sequence, eight query heads), else even
 // lists: two kernels, since what a CTA does not need costs it instruction fetches (one
-// short context: 4.3 us, from one kernel for both 5.1).
-template <typename T, int D, int NT, bool kClusters>
+// short context: 4.3 us, from one kernel for both 5.1).  kPlain: pages of whole tiles,
+// and q and out aligned for vectors, else as the flags say (with the flags: 512 ragged
+// contexts up to 768 x 2 KV heads 29.5 us for 28.5, 37 up to 1,536 x 8 18.7 for 17.6).
+template <typename T, int D, int NT, bool kClusters, bool kPlain>
 __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list_ctas<D, NT>())
-    decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool q8, bool out4) {
+    decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool q_aligned, bool out_aligned) {
+  const bool q8 = kPlain || q_aligned, out4 = kPlain || out_aligned, tile_pages = kPlain || g.tile_pages;
   using S = Smem<D, NT>;
   using P = Partials<D, NT>;
   constexpr int kStages = S::kStages, kHeads = S::kHeads, kRow = S::kRow;
@@ -517,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
       last = 0;
     }
     if (!more) return;
-    if (g.tile_pages) {
+    if (tile_pages) {
       if (pre.t >= last) {
         first = pre.t;
         last = min(first + 32, pre.end);
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
     if (more) {
       const uint32_t st = ring_s + put * S::kStage, dst = to_lane + put * S::kStage;
       unsigned mask;
-      if (g.tile_pages) {
+      if (tile_pages) {
         // rows behind the context are copied as K (their scores are masked), but not as V: a NaN there times a weight of 0
         const long long at = static_cast<long long>(count > 0 ? row : 0) * D + lane * 16;
         const uint8_t *kp = static_cast<const uint8_t*>(c.kc) + at, *vp = static_cast<const uint8_t*>(c.vc) + at;
@@ -596,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
   bool going = cur.t < cur.end;
   if (going) ask_q();
   look();
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) issue();
   if constexpr (!kClusters) {
     empty_rows(ctas);
@@ -1076,12 +1079,9 @@ Geometry geometry(const TbDecodeAttnQuantArgs& a) {
   return g;
 }
 
-template <typename T, int D, int NT>
-int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
+template <typename T, int D, int NT, bool kPlain>
+int launch_as(const TbDecodeAttnQuantArgs& a, const Geometry& g, bool q8, bool out4, cudaStream_t s) {
   using S = Smem<D, NT>;
-  const Geometry g = geometry<D, NT>(a);
-  const bool q8 = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.qs_b % 8 == 0 && a.qs_h % 8 == 0;
-  const bool out4 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.os_b % 4 == 0 && a.os_h % 4 == 0;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.blockDim = dim3(kThreads);
@@ -1090,7 +1090,7 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   cfg.attrs = attr;
   if constexpr (NT == 1) {
     if (g.cs) {
-      auto kernel = decode_attn_quant_kernel<T, D, 1, true>;
+      auto kernel = decode_attn_quant_kernel<T, D, 1, true, kPlain>;
       const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
       if (e != cudaSuccess) return static_cast<int>(e);
       cfg.gridDim = dim3(a.B * g.HG * g.cs);
@@ -1102,7 +1102,7 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
       return static_cast<int>(cudaGetLastError());
     }
   }
-  auto kernel = decode_attn_quant_kernel<T, D, NT, false>;
+  auto kernel = decode_attn_quant_kernel<T, D, NT, false, kPlain>;
   const cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::kBytes);
   if (e != cudaSuccess) return static_cast<int>(e);
   const int grid = sm_count() * list_ctas<D, NT>();
@@ -1120,11 +1120,21 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
   return static_cast<int>(cudaLaunchKernelEx(&cfg, decode_attn_quant_join_kernel<T, D, NT>, a, g, grid, out4));
 }
 
+template <typename T, int D, int NT>
+int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
+  const Geometry g = geometry<D, NT>(a);
+  const bool q8 = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.qs_b % 8 == 0 && a.qs_h % 8 == 0;
+  const bool out4 = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.os_b % 4 == 0 && a.os_h % 4 == 0;
+  return g.tile_pages && q8 && out4 ? launch_as<T, D, NT, true>(a, g, q8, out4, s)
+                                    : launch_as<T, D, NT, false>(a, g, q8, out4, s);
+}
+
 // Query heads that a warp takes, in eights: two where more than 8 share a KV head,
 // which widens the pages once for both (64 x 1,000 tokens x 8 KV heads, 16 query heads
-// on each: 43 us against 56 with one), but in clusters one, for the shorter way of a
-// tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2), and for D = 256 one, whose
-// output fills the registers (64 x 1,000 x 4 KV heads, 16 on each: 50 against 59).
+// on each: 41 us; before other steps 49 against 56 with one), but in clusters one, for
+// the shorter way of a tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2 then),
+// and for D = 256 one, whose output fills the registers (64 x 1,000 x 4 KV heads, 16 on
+// each: 59 against 66 then, 49 now).
 template <int D>
 bool take_two(int B, int Hq, int Hk, int cap) {
   return D < 256 && Hq / Hk > 8 && clusters<D>(B, Hq, Hk, cap) == 0;
