@@ -1131,10 +1131,10 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
 
 // Query heads that a warp takes, in eights: two where more than 8 share a KV head,
 // which widens the pages once for both (64 x 1,000 tokens x 8 KV heads, 16 query heads
-// on each: 41 us; before other steps 49 against 56 with one), but in clusters one, for
-// the shorter way of a tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2 then),
-// and for D = 256 one, whose output fills the registers (64 x 1,000 x 4 KV heads, 16 on
-// each: 59 against 66 then, 49 now).
+// on each: 41 us against 49 with one; D = 64: 45 against 59), but in clusters one, for the
+// shorter way of a tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2), and for D =
+// 256 one, whose output fills the registers (64 x 1,000 x 4 KV heads, 16 on each: 59 against
+// 66, both before tiles were looked up 32 at a time; 49 now).
 template <int D>
 bool take_two(int B, int Hq, int Hk, int cap) {
   return D < 256 && Hq / Hk > 8 && clusters<D>(B, Hq, Hk, cap) == 0;
