@@ -12,9 +12,10 @@
 //    share of the list (sequence, KV head, tile), read off ctx_len on the
 //    device, so one captured call serves contexts that grow.  (Equal shares end
 //    up to 15% apart, SMs of different GPCs reaching memory at different rates;
-//    that, the 5 us until the first tile is there and the 5 us of joining are
-//    what separates the kernel from its bytes: with every product left out it
-//    took 96% of its time.)
+//    that, the 4 us until the first tile is there and the 5 us of joining are
+//    what separates the kernel from its bytes: with every product and widening
+//    left out lists take 98 to 99% of their time, clusters 91%, and lists with 16
+//    query heads on a KV head 96%.)
 //  * A warp fills a ring of tiles in its shared memory with cp.async, running
 //    ahead over the borders of contexts, and waits for no other warp before
 //    the end of its list.  Contexts that end inside its list it writes out; the
