@@ -225,9 +225,12 @@ __global__ void __launch_bounds__(128, 8)  // (64 registers: all of a round's lo
 
 // One token's q and k rows rotated first: G heads of it per round, its table
 // entries in registers for all of them.  A lane holds both members of its pairs
-// (half layout: two vectors of four), else eight neighbours.
+// (half layout: two vectors of four), else eight neighbours.  wide_table: the table
+// starts on a multiple of 16 bytes (it may start on any multiple of 8; its rows are
+// multiples of 32 long).
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv_quant_write_rot_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned) {
+__global__ void __launch_bounds__(128)
+    kv_quant_write_rot_kernel(TbKvQuantWriteArgs a, Split sp, bool aligned, bool wide_table) {
   constexpr int L = D / 8, G = 32 / L, U = 2;
   const int lane = threadIdx.x % 32, l = lane % L, Hk = a.cache.Hk, R = a.rot.R;
   const long long item = blockIdx.x * (blockDim.x / 32ll) + threadIdx.x / 32, t = item / sp.parts;
@@ -237,7 +240,19 @@ __global__ void __launch_bounds__(128) kv_quant_write_rot_kernel(TbKvQuantWriteA
   const int p = a.pos[t], seq = a.seq[t];
   const bool past = p >= a.rot.max_pos, turn = 8 * l < R, half = turn && !a.rot.interleaved;
   float cs[8];
-  if (turn && p >= 0 && !past) tb::load_vec<float, 8>(a.rot.table + (static_cast<long long>(p) * (R / 2) + 4 * l) * 2, cs);
+  if (turn && p >= 0 && !past) {
+    const float* entry = a.rot.table + (static_cast<long long>(p) * (R / 2) + 4 * l) * 2;
+    if (wide_table) {
+      tb::load_vec<float, 8>(entry, cs);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float2 e = *reinterpret_cast<const float2*>(entry + j);
+        cs[j] = e.x;
+        cs[j + 1] = e.y;
+      }
+    }
+  }
   int base = -1;
   if (past) {
     if (a.rot.err && lane == 0) atomicCAS(a.rot.err, 0, 1);
@@ -423,10 +438,10 @@ int write_as(const TbKvQuantWriteArgs& a, cudaStream_t s) {
     al = al && rows_aligned(a.rot.x, a.rot.xs_t, a.rot.xs_h, a.rot.dtype, v) &&
          rows_aligned(a.rot.y, a.rot.ys_t, a.rot.ys_h, a.rot.dtype, v);
   }
-  al = al && reinterpret_cast<uintptr_t>(a.rot.table) % 16 == 0;
+  const bool wide_table = reinterpret_cast<uintptr_t>(a.rot.table) % 16 == 0;
   sp.parts = parts_of(a.T, (sp.slots + G - 1) / G);
   const Shape g(static_cast<long long>(a.T) * sp.parts);
-  kv_quant_write_rot_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, al);
+  kv_quant_write_rot_kernel<T, D><<<g.grid, g.block, 0, s>>>(a, sp, al, wide_table);
   return static_cast<int>(cudaGetLastError());
 }
 

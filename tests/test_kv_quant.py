@@ -624,3 +624,37 @@ def test_offsets_beyond_32_bits(dev):
     q = torch.randn(1, Hq, D, device=dev).bfloat16()
     out = decode_attention_quant(q, *c, table, torch.tensor([n], dtype=torch.int32, device=dev))
     check_attention(out, q, c, table, [n], D ** -0.5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("Hq,Hk,D,R", [(5, 2, 128, 128), (3, 1, 64, 24), (2, 2, 256, 128)])
+def test_write_with_rotary_at_every_alignment(Hq, Hk, D, R, interleaved, dtype, device):
+    """A table on any multiple of 8 bytes, rows on any multiple of their elements, in every combination: the bits that
+    aligned ones give."""
+    lens, bs = [19, 1, 6], 16
+    table, nb = pages(lens, bs, device)
+    seq, pos = tokens_of(lens, device)
+    T, H = seq.numel(), Hq + 2 * Hk
+    g = torch.Generator().manual_seed(R)
+    rt = rotary_table(R, 19, 1e4, device=device)
+    x = torch.randn(T, H, D, generator=g).to(dtype).to(device)
+    c = quant_kv_cache(nb, Hk, bs, D, device)
+    want = kv_quant_write(x[:, Hq:Hq + Hk], x[:, Hq + Hk:], seq, pos, table, *c, q=x[:, :Hq], table=rt,
+                          interleaved=interleaved)
+    for floats, shift in ((2, 0), (4, 0), (6, 0), (0, 1), (2, 1), (2, 4), (0, 3)):
+        t = torch.zeros(rt.numel() + 8, device=device)[floats:floats + rt.numel()].view(rt.shape)
+        t.copy_(rt)
+        assert t.data_ptr() % 16 == floats * 4 % 16
+        row = torch.zeros(T * H * D + shift, dtype=dtype, device=device)[shift:].view(T, H, D)
+        row.copy_(x)
+        d = quant_kv_cache(nb, Hk, bs, D, device)
+        q = kv_quant_write(row[:, Hq:Hq + Hk], row[:, Hq + Hk:], seq, pos, table, *d, q=row[:, :Hq], table=t,
+                           interleaved=interleaved)
+        assert torch.equal(q, want) and all(torch.equal(bits(a), bits(b)) for a, b in zip(c, d))
+        # rotary takes other vectors then, whose products may be fused with the other sum: two results, each within three
+        # roundings of 2^-24 of the two products (2 amax at most) and half a step of the exact one
+        a, b = (rotary(y, pos, z, interleaved=interleaved).double() for y, z in ((row[:, :Hq], t), (x[:, :Hq], rt)))
+        amax = x[:, :Hq].double().abs().amax(-1, keepdim=True)
+        assert ((a - b).abs() <= 2 * (HALF_STEP[dtype] * 1.01 * a.abs().maximum(b.abs()) + 6 * 2.0 ** -24 * amax)).all()
