@@ -353,7 +353,8 @@ enum { TB_BF16 = 0, TB_F16 = 1, TB_F32 = 2 };
 // y = the rotation of x [T, H, D] by the table rows of pos (transpose: its
 // backward).  R (even) of D (even) dimensions rotate, the others are copied
 // (x == y: left alone).  A negative position marks padding, copied as it is; a
-// position >= max_pos makes the row NaN and sets *err (optional) to 1.
+// position >= max_pos makes the whole row NaN, in place too, and sets *err
+// (optional) to 1.
 // Strides in elements; x == y needs equal strides, else the two do not overlap.
 typedef struct {
   const void* x;

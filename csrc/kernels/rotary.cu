@@ -6,7 +6,8 @@
 //   y_a = c a - s b,   y_b = c b + s a        (backward: s -> -s),
 //
 // in fp32 with one rounding at the store; scaling for long contexts lives in
-// the table.  Dimensions behind R are copied (in place: left alone).
+// the table.  Dimensions behind R are copied (in place: left alone, but NaN like the
+// others in rows whose position is past the table).
 //
 // The kernel moves every element once in and once out and does 3 flops per
 // element, so memory bounds it: 16,383 rows x 40 heads x 128 in bf16 take 54 us on
@@ -39,7 +40,6 @@ __global__ void __launch_bounds__(threads_of(HU), blocks_of(HU))
   if (tk >= tokens || t >= a.T) return;
   const int p = a.pos[t];
   const bool bad = p >= a.max_pos;
-  if (bad && a.err && threadIdx.x == tk * per) atomicCAS(a.err, 0, 1);
   const float sgn = a.transpose ? -1.f : 1.f;
   for (int i = threadIdx.x - tk * per; i < per; i += blockDim.x) {  // (more than one round only where per > blockDim.x)
     const int u = i % units, h0 = i / units;
@@ -57,16 +57,14 @@ __global__ void __launch_bounds__(threads_of(HU), blocks_of(HU))
         lo[k].load(xr + (h0 + k * HS) * a.xs_h + o1);
         hi[k].load(xr + (h0 + k * HS) * a.xs_h + o2);
       }
+    if (bad) break;  // (here, so that the loads do not wait for the position)
 #pragma unroll
     for (int k = 0; k < HU; ++k)
       if (h0 + k * HS < a.H) {
         float f[NP], g[NP];
         lo[k].unpack(f);
         hi[k].unpack(g);
-        if (bad) {
-#pragma unroll
-          for (int j = 0; j < NP; ++j) f[j] = g[j] = NAN;
-        } else if (turn) {
+        if (turn) {
 #pragma unroll
           for (int j = 0; j < NP; ++j) {
             const float c = cs[2 * j], sn = sgn * cs[2 * j + 1];
@@ -80,6 +78,15 @@ __global__ void __launch_bounds__(threads_of(HU), blocks_of(HU))
         tb::store_vec<T, NP>(yr + (h0 + k * HS) * a.ys_h + o1, f);
         tb::store_vec<T, NP>(yr + (h0 + k * HS) * a.ys_h + o2, g);
       }
+  }
+  if (bad) {  // the whole row becomes NaN, with the dimensions that have no unit in place
+    if (a.err && threadIdx.x == tk * per) atomicCAS(a.err, 0, 1);
+    float f[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) f[j] = NAN;
+    const int row = a.D / NP, step = min(per, static_cast<int>(blockDim.x));
+    for (int i = threadIdx.x - tk * per; i < a.H * row; i += step)
+      tb::store_vec<T, NP>(y + t * a.ys_t + i / row * a.ys_h + i % row * NP, f);
   }
 }
 

@@ -259,3 +259,29 @@ def test_forward_and_backward_in_a_graph(dev):
     check(dx, dy, pos, table, transpose=True)
     (again,) = torch.autograd.grad(rotary(x, pos, table), x, dy)
     assert torch.equal(again, dx)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,H,D,R", [(7, 3, 128, 64), (5, 2, 80, 20), (4, 2, 10, 6), (9, 1, 256, 32), (6, 4, 64, 64),
+                                     (5003, 9, 128, 32), (26003, 3, 128, 64)])
+def test_positions_out_of_range_in_place(T, H, D, R, interleaved, dtype, device):
+    """In place on part of the head: a row past the table becomes NaN in all its dimensions, the others and what lies
+    between the rows stay as a new output has them."""
+    if device == "cpu" and T > 1000:
+        pytest.skip("the same math on the host, whatever the number of rows")
+    g = torch.Generator().manual_seed(T + R)
+    table = rotary_table(R, 50, device=device)
+    buf = torch.randn(T, H * D + 16, generator=g).to(dtype).to(device)
+    x = buf[:, 8:8 + H * D].view(T, H, D)
+    pos = torch.randint(-1, 50, (T,), generator=g, dtype=torch.int32)
+    pos[::3] = torch.randint(50, 2 ** 31 - 1, (len(pos[::3]),), generator=g, dtype=torch.int32)
+    pos = pos.to(device)
+    before, bad = buf.clone(), pos >= 50
+    want = rotary(x, pos, table, interleaved=interleaved)
+    err = torch.zeros(1, dtype=torch.int32, device=device)
+    assert rotary(x, pos, table, interleaved=interleaved, out=x, error=err) is x
+    assert int(err) == 1 and x[bad].isnan().all() and want[bad].isnan().all()
+    assert torch.equal(x[~bad], want[~bad])
+    assert torch.equal(buf[:, :8], before[:, :8]) and torch.equal(buf[:, 8 + H * D:], before[:, 8 + H * D:])
