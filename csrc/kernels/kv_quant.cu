@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(128)
   if (t >= a.T) return;
   const int part = static_cast<int>(item - t * sp.parts), rounds = (sp.slots + G - 1) / G;
   const int lo = part * rounds / sp.parts, hi = (part + 1) * rounds / sp.parts;
-  const int p = a.pos[t], seq = a.seq[t];
+  const int seq = a.seq[t], p = seq < 0 ? -1 : a.pos[t];  // (padding, whatever its position)
   const bool past = p >= a.rot.max_pos, turn = 8 * l < R, half = turn && !a.rot.interleaved;
   float cs[8];
   if (turn && p >= 0 && !past) {

@@ -658,3 +658,29 @@ def test_write_with_rotary_at_every_alignment(Hq, Hk, D, R, interleaved, dtype, 
         a, b = (rotary(y, pos, z, interleaved=interleaved).double() for y, z in ((row[:, :Hq], t), (x[:, :Hq], rt)))
         amax = x[:, :Hq].double().abs().amax(-1, keepdim=True)
         assert ((a - b).abs() <= 2 * (HALF_STEP[dtype] * 1.01 * a.abs().maximum(b.abs()) + 6 * 2.0 ** -24 * amax)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("max_pos", [64, 8])
+def test_write_padding_by_sequence(max_pos, interleaved, device):
+    """A negative sequence is padding whatever its position, even one past the table: its q row is copied, nothing is
+    written, and it is no error."""
+    Hq, Hk, D, bs, nb = 3, 2, 64, 16, 4
+    g = torch.Generator().manual_seed(max_pos)
+    seq = torch.tensor([0, -1, 0, -1, -2 ** 31, -1], dtype=torch.int32, device=device)
+    pos = torch.tensor([3, 5, 7, 20, 63, 2 ** 31 - 1], dtype=torch.int32, device=device)
+    table = torch.tensor([[2, 1]], dtype=torch.int32, device=device)
+    q, k, v = (torch.randn(6, h, D, generator=g).bfloat16().to(device) for h in (Hq, Hk, Hk))
+    rt = rotary_table(D, max_pos, device=device)
+    c, err = quant_kv_cache(nb, Hk, bs, D, device), torch.zeros(1, dtype=torch.int32, device=device)
+    out = kv_quant_write(k, v, seq, pos, table, *c, q=q, table=rt, interleaved=interleaved, error=err)
+    pad = seq < 0
+    assert torch.equal(out[pad], q[pad]) and int(err) == 0
+    assert torch.equal(out[~pad], rotary(q, pos.clamp_max(7), rt, interleaved=interleaved)[~pad])
+    assert not torch.equal(out[~pad], q[~pad])
+    for s in (c.ks, c.vs):
+        assert s.transpose(1, 2).ne(0).any(-1).nonzero().tolist() == [[2, 3], [2, 7]]
+    # in place
+    assert kv_quant_write(k, v, seq, pos, table, *c, q=q, table=rt, interleaved=interleaved, q_out=q, error=err) is q
+    assert torch.equal(q, out) and int(err) == 0

@@ -248,7 +248,7 @@ def _slots(seq_of_token, pos, block_table, num_blocks, bs, error):
 
 def kv_quant_write(k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q=None, table=None, interleaved=False,
                    q_out=None, error=None):
-    p = pos
+    p = pos = torch.where(seq_of_token < 0, -1, pos)  # a negative sequence is padding, whatever its position
     if table is not None:
         if q is not None:
             rotary(q, pos, table, interleaved, out=q_out, error=error)
