@@ -60,7 +60,9 @@ constexpr int kStart = 3;       // what beginning a (sequence, group) costs a wa
 constexpr int kMostCluster = 8;   // CTAs of a cluster (the portable bound)
 constexpr float kMinVsLog = -100.f;
 constexpr float kLowest = -FLT_MAX;  // the reference before the first token: below every score, and finite
-constexpr float kSlack = 8.f;   // the reference of the weights may lag behind their maximum by a factor of 2^8
+// The reference of the weights may lag behind their maximum by a factor of 2^8.  Added to it rounding down: where
+// neighbouring scores are 16 apart, half way rounds up to the next one and lets weights of 2^16 through, past fp16.
+constexpr float kSlack = 8.f;
 
 // The four codes of a word as two fp16 pairs.
 __device__ __forceinline__ void widen(uint32_t codes, uint32_t& lo, uint32_t& hi) {
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
         for (int e = 0; e < 2; ++e) {
           s[n][e] = in0 ? s[n][e] * ch[n][e] * k0 : -INFINITY;
           s[n][2 + e] = in1 ? s[n][2 + e] * ch[n][e] * k1 : -INFINITY;
-          grew |= fmaxf(s[n][e] + e0, s[n][2 + e] + e1) > m[n][e] + kSlack;
+          grew |= fmaxf(s[n][e] + e0, s[n][2 + e] + e1) > __fadd_rd(m[n][e], kSlack);
         }
       if (__any_sync(0xffffffffu, grew)) {  // the maximum outran the reference: move it, and what was summed with it
 #pragma unroll

@@ -684,3 +684,29 @@ def test_write_padding_by_sequence(max_pos, interleaved, device):
     # in place
     assert kv_quant_write(k, v, seq, pos, table, *c, q=q, table=rt, interleaved=interleaved, q_out=q, error=err) is q
     assert torch.equal(q, out) and int(err) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("Hq,D,n", [(4, 64, 4000), (8, 128, 700), (20, 128, 4000), (3, 256, 2000)])
+@pytest.mark.parametrize("B,v_scale", [(1, 1 / 448), (600, 1 / 448), (1, 128.0), (600, 128.0)])
+def test_attention_huge_scores(B, v_scale, Hq, D, n, device):
+    """Scores near 2^27, where neighbouring fp32 numbers are 16 apart, that creep up from tile to tile: the weights stay
+    finite, so equal values average to themselves."""
+    if device == "cpu" and B > 1:
+        pytest.skip("the host's plain math, sequence by sequence")
+    Hk, bs = 1, 16
+    nb = -(-n // bs)
+    c = quant_kv_cache(nb, Hk, bs, D, device)
+    bits(c.kc).fill_(0x7E), bits(c.vc).fill_(0x7E)  # 448
+    step = torch.arange(nb, device=device, dtype=torch.float64)[:, None, None] * 2.0 ** -23
+    c.ks.copy_(((1 + step) / 512).expand_as(c.ks))
+    c.vs.fill_(v_scale)
+    table = torch.arange(nb, dtype=torch.int32, device=device).repeat(B, 1)
+    ctx = torch.full((B,), n, dtype=torch.int32, device=device)
+    for dtype in (torch.bfloat16, torch.float16):
+        q = torch.ones(B, Hq, D, dtype=dtype, device=device)
+        for top in (1.0, 1.37, 1.9):  # several places between two powers of two
+            scale = top * 2.0 ** 27 / math.log2(math.e) / (448 / 512 * D)
+            out = decode_attention_quant(q, *c, table, ctx, scale=scale)
+            # values 448 * fl(1 / 448), off by 2^-24; rounded weights over their unrounded sum, and the output's rounding
+            assert ((out.double() / (448 * v_scale) - 1).abs() <= HALF_STEP[dtype] * 1.01 + 2.0 ** -11 + n * 2.0 ** -22).all()
