@@ -31,11 +31,11 @@
 //    codes widened through shared memory first.  S^T = K q, whose accumulator,
 //    transposed in registers (movmatrix), is the operand of O^T = V^T w.
 //  * The weights' reference m follows the running maximum of a_j + log2 vs_j
-//    (a_j in units of log 2): then w_j = exp2(a_j - m) vs_j fits fp16 however
-//    much the scales of tokens differ (rounded to 2^-11 relative, 2^-25 absolute
-//    at the small end), while the sum l of exp2(a_j - m) stays in fp32 range.
-//    m moves only once the maximum is 2^8 above it, so weights stay below 2^8
-//    and most tiles need no reduction over the warp and no rescaling.  q is
+//    (a_j in units of log 2), 7 below it: then w_j = exp2(a_j - m) vs_j fits fp16
+//    however much the scales of tokens differ (rounded to 2^-11 relative, 2^-32 of
+//    the largest at the small end), while the sum l of exp2(a_j - m) stays in fp32
+//    range.  m moves only once the maximum is 15 above it, so weights stay below
+//    2^15 and most tiles need no reduction over the warp and no rescaling.  q is
 //    brought into fp16 range by a power of two per head (exact).
 //
 // On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 96 us,
@@ -58,11 +58,13 @@ constexpr int kTile = 16;       // tokens per tile
 constexpr int kMinTiles = 8;    // tiles per CTA, at least, where there are that many
 constexpr int kStart = 3;       // what beginning a (sequence, group) costs a warp, in tiles
 constexpr int kMostCluster = 8;   // CTAs of a cluster (the portable bound)
-constexpr float kMinVsLog = -100.f;
+constexpr float kMinVsLog = -92.f;   // keeps the sum of exp2(a - m), 2^(15 + 92) per token at most, in fp32 range
 constexpr float kLowest = -FLT_MAX;  // the reference before the first token: below every score, and finite
-// The reference of the weights may lag behind their maximum by a factor of 2^8.  Added to it rounding down: where
-// neighbouring scores are 16 apart, half way rounds up to the next one and lets weights of 2^16 through, past fp16.
-constexpr float kSlack = 8.f;
+// The reference of the weights is set 2^7 below their maximum, and left until that is 2^15 above it: the weights use
+// fp16's upper range, so that a token has to be 2^-32 of the largest one before its weight rounds to 0 (with the
+// reference at the maximum 2^-25, and 2^18 such tokens of a context lost 2^-7 of the sum).  The slack is added rounding
+// down: where neighbouring scores are 8 or 16 apart, it could round up and let weights of 2^16 through, past fp16.
+constexpr float kAhead = 7.f, kSlack = 15.f;
 
 // The four codes of a word as two fp16 pairs.
 __device__ __forceinline__ void widen(uint32_t codes, uint32_t& lo, uint32_t& hi) {
@@ -721,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, m[n][e]);
+            top = fmaxf(top - kAhead, m[n][e]);
             const float cor = exp2_fast(m[n][e] - top);
             m[n][e] = top;
             l[n][e] *= cor;

@@ -710,3 +710,40 @@ def test_attention_huge_scores(B, v_scale, Hq, D, n, device):
             out = decode_attention_quant(q, *c, table, ctx, scale=scale)
             # values 448 * fl(1 / 448), off by 2^-24; rounded weights over their unrounded sum, and the output's rounding
             assert ((out.double() / (448 * v_scale) - 1).abs() <= HALF_STEP[dtype] * 1.01 + 2.0 ** -11 + n * 2.0 ** -22).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,D", [(1, 64), (12, 64), (2, 128)])
+def test_attention_keeps_a_long_faint_tail(Hq, D, dev):
+    """One loud token, whose value is zero but in dimension 0, and 2^18 faint ones, each 2^-25 of it: they make up the
+    other dimensions.  Every sequence reads the same pages, and there are as many as warps, so that the loud token and
+    nearly all of its tail are one warp's."""
+    n, bs, Hk = 1 << 18, 64, 1
+    B = 2368 if D == 64 else 1776
+    nb = n // bs
+    g = torch.Generator().manual_seed(D)
+    c = quant_kv_cache(nb, Hk, bs, D, dev)
+    tail = math.log(2.0) * (25.02 + 0.2 * torch.rand(nb, Hk, bs, generator=g))  # how far below the loud token's score
+    bits(c.kc).fill_(0xFE)  # -448
+    c.ks.copy_(tail / 448)
+    c.ks[0, 0, 0] = 0.0
+    v = 1.5 + torch.rand(nb, Hk, bs, D, generator=g) / 2
+    v[0, 0, 0] = 0.0
+    v[..., 0] = 2.0  # one scale for all
+    cc, ss = ref.kv_quantise(v)
+    bits(c.vc).copy_(bits(cc))
+    c.vs.copy_(ss)
+    table = torch.arange(nb, dtype=torch.int32, device=dev).repeat(B, 1)
+    ctx = torch.full((B,), n, dtype=torch.int32, device=dev)
+    q = torch.ones(B, Hq, D, dtype=torch.float16, device=dev)
+    out = decode_attention_quant(q, *c, table, ctx, scale=1.0 / D).double()
+    p = torch.softmax(-448 * c.ks.double().view(-1), 0)
+    e = p @ (bits(c.vc).view(F8).double().view(n, D) * c.vs.double().view(n, 1))
+    # The output's rounding and the weights' to fp16: 2^-11 relative, or where they are below 2^-14 absolute, 2^-25 for a
+    # largest weight of at least 2^7, so n * 2^-32 in all for values up to 2.  Scores near 18, off by 2^-24 (D / 2 + 8)
+    # of that.  Sums in fp32 of n / 16 steps: 16 products are added to the numerator in one, each perhaps cut off at 2^-24
+    # of the sum, and two weights to a denominator in two roundings of 2^-24.
+    tol = e * (2.0 ** -11 * 2.01 + 3 * 2.0 ** -24 * (D / 2 + 8) * 18 + n / 16 * (17 + 2) * 2.0 ** -24) + n * 2.0 ** -32 * 2
+    assert (e[1:] > 20 * tol[1:]).all()  # a lost tail would be seen
+    over = (out - e).abs() - tol
+    assert not (over > 0).any(), (float(over.max()), float(tol.max()))
