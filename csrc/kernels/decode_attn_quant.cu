@@ -98,6 +98,9 @@ __device__ __forceinline__ float log2_fast(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What a sum of 0 over a context stands for, M being the reference it was taken with: no token (M = -inf: zeros), or
+// scores that are all -inf (NaN, as 0 / 0).
+__device__ __forceinline__ float of_nothing(float M) { return M == -INFINITY ? 0.f : NAN; }
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -303,7 +306,7 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
       }
     }
     if (g.cs == 1) {
-      if (any) write(h, o, L == 0.f ? 0.f : 1.f / L);  // (else one warp had the whole context, and wrote it)
+      if (any) write(h, o, L == 0.f ? of_nothing(M) : 1.f / L);  // (else one warp had the whole context, and wrote it)
       continue;
     }
 #pragma unroll
@@ -347,7 +350,7 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
       }
     }
     const float M = tb::warp_max(m), f = m == -INFINITY ? 0.f : exp2_fast(m - M);
-    const float L = tb::warp_sum(f * l), inv = L == 0.f ? 0.f : 1.f / L;
+    const float L = tb::warp_sum(f * l), inv = L == 0.f ? of_nothing(M) : 1.f / L;
     float y[E] = {};
 #pragma unroll
     for (int p = 0; p < kMostCluster; ++p) {
@@ -672,6 +675,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
 
+    unsigned seen = 0;  // whether any token counted
     for (int t = cur.t; t < cur.end; ++t) {
       cp_wait<kStages - 2>();
       __syncwarp();
@@ -679,6 +683,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
       const uint8_t* st = ring + get * S::kStage;
       const float* scales = reinterpret_cast<const float*>(st + 2 * kTile * kRow);
       const unsigned mask = *reinterpret_cast<const unsigned*>(st + 2 * kTile * kRow + 2 * kTile * 4);
+      seen |= mask;
       // S^T [16 tokens, heads] = K q
       float s[NT][4];
 #pragma unroll
@@ -786,6 +791,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
     const int b = cur.b, r = cur.r;
     going = next_portion(a, g, cur);
     if (going) ask_q();
+    const float nothing = seen ? NAN : 0.f;
     float* part = first_portion ? first_part : reinterpret_cast<float*>(ring);
     if (!first_portion && !(opens && closes)) {  // the list's last portion: the ring is done with
       cp_wait<0>();
@@ -800,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const float inv = v == 0.f ? 0.f : 1.f / v;
+        const float inv = v == 0.f ? nothing : 1.f / v;
         T* o = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
@@ -814,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
           }
         }
         if (!(opens && closes) && gq == 0)
-          *reinterpret_cast<float2*>(part + kHeads * D + 2 * h) = make_float2(m[n][e], v);
+          *reinterpret_cast<float2*>(part + kHeads * D + 2 * h) = make_float2(seen ? m[n][e] : -INFINITY, v);
       }
     if (!(opens && closes) && lane == 0)
       meta[2 * w + (first_portion ? 0 : 1)] = make_int2(b * g.HG + r, (opens ? 1 : 0) | (closes ? 2 : 0));
@@ -874,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list
           for (int e = 0; e < V; ++e) o[i + e] += f * y[e];
         }
       }
-      const float inv = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
+      const float inv = !whole ? 1.f : L == 0.f ? of_nothing(M) : 1.f / L;
       T* out = static_cast<T*>(a.out) + static_cast<long long>(b) * a.os_b + static_cast<long long>(h0 + h) * a.os_h;
       float* part = P::out(a.ws, slot, h);
 #pragma unroll
@@ -922,9 +928,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
       for (int e = 0; e < V; ++e) o[i + e] += f * x[e];
     }
   };
-  auto write = [&](int seg, int h, float L, const float (&o)[E]) {
+  auto write = [&](int seg, int h, float inv, const float (&o)[E]) {
     const int r = seg % g.HG, head = r / g.NG * g.G + r % g.NG * P::kHeads + h;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
     T* p = static_cast<T*>(a.out) + static_cast<long long>(seg / g.HG) * a.os_b + static_cast<long long>(head) * a.os_h +
            lane * V;
 #pragma unroll
@@ -957,7 +962,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 #pragma unroll 4
       for (int p = 0; p < mine.z; ++p)
         add(o, __shfl_sync(0xffffffffu, f, p), P::out(a.ws, p == 0 ? mine.y : 2ll * (blockIdx.x + p), h));
-      write(mine.x, h, L, o);
+      write(mine.x, h, L == 0.f ? of_nothing(M) : 1.f / L, o);
     }
   }
 #pragma unroll 1
@@ -981,7 +986,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kJoinWarps; ++i) M = fmaxf(M, red[i]);
-    if (M == -INFINITY) M = 0.f;
+    const float m0 = M == -INFINITY ? 0.f : M;
     // `lanes` lanes hold a part's slice, four dimensions each (at D = 256 in one slice: and the four 128 further)
     const int lanes = min(size / 4, 32), at_once = 32 / lanes, d = item % slices * size + lane % lanes * 4;
     const bool wide = D == 256 && size == 256;
@@ -989,7 +994,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 #pragma unroll 4
     for (int p = w * at_once + lane / lanes; p < n; p += kJoinWarps * at_once) {
       const float2 st = *reinterpret_cast<const float2*>(P::stat(a.ws, slot(p), h));
-      const float f = exp2_fast(st.x - M), *v = P::out(a.ws, slot(p), h) + d;
+      const float f = exp2_fast(st.x - m0), *v = P::out(a.ws, slot(p), h) + d;
       L += f * st.y;
       float x[4];
       tb::load_vec<float, 4>(v, x);
@@ -1024,7 +1029,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
       }
       const int r = rec.x % g.HG, head = r / g.NG * g.G + r % g.NG * P::kHeads + h;
       static_cast<T*>(a.out)[static_cast<long long>(rec.x / g.HG) * a.os_b + static_cast<long long>(head) * a.os_h +
-                             item % slices * size + threadIdx.x] = tb::from_f32<T>(l == 0.f ? 0.f : sum / l);
+                             item % slices * size + threadIdx.x] = tb::from_f32<T>(l == 0.f ? of_nothing(M) : sum / l);
     }
   }
 }

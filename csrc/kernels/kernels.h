@@ -409,8 +409,9 @@ typedef struct {
 } TbKvQuantReadArgs;
 int tb_kv_quant_read(const TbKvQuantReadArgs* args, cudaStream_t s);
 // out[b] = attention of the one token q[b] over the first ctx_len[b] tokens of
-// sequence b (zeros where ctx_len[b] <= 0).  Tokens in blocks out of range, or
-// behind the table, are left out and set *err to 1.
+// sequence b (zeros where ctx_len[b] <= 0, NaN where all its scores are -inf).
+// Tokens in blocks out of range, or behind the table, are left out and set *err
+// to 1.
 typedef struct {
   TbQuantCache cache;
   const void* q;  // [B, Hq, D] bf16 / fp16

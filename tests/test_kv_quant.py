@@ -747,3 +747,40 @@ def test_attention_keeps_a_long_faint_tail(Hq, D, dev):
     assert (e[1:] > 20 * tol[1:]).all()  # a lost tail would be seen
     over = (out - e).abs() - tol
     assert not (over > 0).any(), (float(over.max()), float(tol.max()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("Hq,Hk,D,bs", [(12, 2, 128, 16), (4, 4, 64, 7), (8, 1, 256, 64), (20, 1, 128, 16)])
+def test_attention_infinite_scores(Hq, Hk, D, bs, device):
+    """Scores of -inf: a token of weight zero beside finite ones; NaN, as the formula's 0 / 0, where a context has no
+    other; and zeros still for contexts without a token that counts."""
+    for lens in ([1], [40, 0, 1], [5000, 3], [300] * 160 if device != "cpu" else [300, 2]):
+        table, nb = pages(lens, bs, device)
+        g = torch.Generator().manual_seed(len(lens))
+        c = random_cache(nb, Hk, bs, D, device, g)
+        q = (torch.randn(len(lens), Hq, D, generator=g).abs() + 0.01).bfloat16().to(device)
+        ctx = torch.tensor(lens, dtype=torch.int32, device=device)
+        loud = quant_kv_cache(nb, Hk, bs, D, device)
+        for a, b in zip(loud, c):
+            bits(a).copy_(bits(b))
+        # the keys of every context but its last token: all dimensions negative, times infinity
+        seq, pos = tokens_of(lens, device)
+        first = pos < ctx[seq.long()] - 1
+        blk, slot = where(seq, pos, table, bs)
+        code = bits(loud.kc).transpose(1, 2)[blk, slot]
+        bits(loud.kc).transpose(1, 2)[blk, slot] = torch.where(code & 0x7F == 0, 0x81, code | 0x80).to(torch.uint8)
+        loud.ks.transpose(1, 2)[blk[first], slot[first]] = float("inf")
+        out = decode_attention_quant(q, *loud, table, ctx)
+        last = (ctx - 1).clamp_min(0)
+        lb, ls = where(torch.arange(len(lens), device=device), last, table, bs)
+        v = bits(loud.vc)[lb, :, ls].view(F8).double() * loud.vs[lb, :, ls].double()[..., None]
+        v = v.repeat_interleave(Hq // Hk, 1)
+        # one weight, exact but for its rounding to fp16 and the output's
+        tol = v.abs() * (2.0 ** -8 * 1.01 + 2.0 ** -11 + 2.0 ** -20)
+        assert ((out.double() - v).abs() <= tol)[ctx > 0].all() and (out[ctx == 0] == 0).all()
+        loud.ks.transpose(1, 2)[blk, slot] = float("inf")
+        out = decode_attention_quant(q, *loud, table, ctx)
+        assert out[ctx > 0].isnan().all() and (out[ctx == 0] == 0).all()
+        err = torch.zeros(1, dtype=torch.int32, device=device)
+        out = decode_attention_quant(q, *loud, torch.full_like(table, -1), ctx, error=err)
+        assert (out == 0).all() and int(err) == 1

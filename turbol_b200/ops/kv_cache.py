@@ -91,10 +91,11 @@ def decode_attention_quant(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, 
     first ctx_len[b] (int32) tokens of row b of ``block_table``: [B, Hq, D], q's
     type, without a backward pass (as :func:`kv_quant_write`).  Query head h reads
     KV head h // (Hq / Hk).  scale: default 1 / sqrt(D).  An empty context gives
-    zeros.  Tokens behind the table or in blocks out of range are left out and set
-    ``error``.  Weights are rounded to fp16 (sums stay in fp32).  The result does
-    not depend on what the pages hold behind a context; it can depend, within
-    rounding, on the other sequences of the batch (where contexts are split)."""
+    zeros, one whose scores are all -inf gives NaN.  Tokens behind the table or in
+    blocks out of range are left out and set ``error``.  Weights are rounded to
+    fp16 (sums stay in fp32).  The result does not depend on what the pages hold
+    behind a context; it can depend, within rounding, on the other sequences of the
+    batch (where contexts are split)."""
     y = _call("decode_attention_quant", q, kc, vc, ks, vs, block_table, ctx_len, out, scale, error)
     if y is None:
         y = ref.decode_attention_quant(q, kc, vc, ks, vs, block_table, ctx_len,
