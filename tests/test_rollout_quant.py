@@ -177,3 +177,20 @@ def test_fp8_rollout_in_the_trainer_and_engine(dev):
     e.initialize()
     assert len(e.generate_batch(["one", "another prompt"])) == 2
     e.shutdown()
+
+
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+def test_positions_past_the_model_are_refused(kv_dtype):
+    """A prompt and answer longer than the model's table of positions: refused by generate before anything runs."""
+    from turbol_b200.rl.rollout import LLMGenerator, TPLLMGenerator
+
+    m = DecoderLM(tiny(max_seq=32), "cpu", master=False)
+    gen = LLMGenerator(m, 2, 64, kv_dtype=kv_dtype)
+    tp = TPLLMGenerator.__new__(TPLLMGenerator)
+    tp.m, tp.cfg, tp.tpm, tp.max_batch, tp.max_len = m, m.cfg, type("TP", (), {"tp": 1, "rank": 0}), 2, 64
+    for g in (gen, tp):
+        for Lp, new in ((33, 1), (32, 2), (16, 18), (1, 33)):
+            with pytest.raises(ValueError, match="max_seq"):
+                g.generate(torch.zeros(1, Lp, dtype=torch.int32), 2, new)
+        with pytest.raises(ValueError, match="capacity"):
+            g.generate(torch.zeros(1, 16, dtype=torch.int32), 3, 4)

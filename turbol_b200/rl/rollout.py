@@ -314,6 +314,13 @@ class LLMGenerator:
         return {"ws": torch.zeros(n, device=self.device)}
 
     # ------------------------------------------------------------ generate
+    def _check_sizes(self, B: int, Lp: int, max_new: int):
+        if B > self.max_batch or Lp + max_new > self.max_len:
+            raise ValueError("generate: batch or length beyond the engine's capacity")
+        # the last sampled token is never embedded, so its position needs no row
+        if max(Lp, Lp + max_new - 1) > self.m.table.shape[0]:
+            raise ValueError(f"generate: positions beyond the model's max_seq ({self.m.table.shape[0]})")
+
     @torch.no_grad()
     def generate(self, prompts: torch.Tensor, group: int = 1, max_new: int = 16, temperature: float = 1.0,
                  top_k: int = -1, top_p: float = 1.0, eos_id: int = -1, pad_id: int = 0, stop_check: int = 16):
@@ -330,8 +337,7 @@ class LLMGenerator:
         P, Lp = prompts.shape
         G = group
         B = P * G
-        if B > self.max_batch or Lp + max_new > self.max_len:
-            raise ValueError("generate: batch or length beyond the engine's capacity")
+        self._check_sizes(B, Lp, max_new)
         sampling = (int(top_k), float(top_p), int(eos_id), int(pad_id))
         if sampling != self.sampling:
             self.sampling = sampling
@@ -601,8 +607,7 @@ class TPLLMGenerator(LLMGenerator):
         P, Lp = prompts.shape
         G = group
         B = P * G
-        if B > self.max_batch or Lp + max_new > self.max_len:
-            raise ValueError("generate: batch or length beyond the engine's capacity")
+        self._check_sizes(B, Lp, max_new)
         if P % tp:
             raise ValueError("generate: the prompt count must divide by the tensor-parallel size")
         self.temperature = float(temperature)
