@@ -194,3 +194,29 @@ def test_positions_past_the_model_are_refused(kv_dtype):
                 g.generate(torch.zeros(1, Lp, dtype=torch.int32), 2, new)
         with pytest.raises(ValueError, match="capacity"):
             g.generate(torch.zeros(1, 16, dtype=torch.int32), 3, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [True, False])
+def test_generate_reports_cache_errors(graph, dev):
+    """A block out of range in the table of one sequence: the kernels skip it, and generate says so instead of
+    returning; the next call, on sound tables, runs."""
+    from turbol_b200.rl.rollout import LLMGenerator
+
+    m = DecoderLM(tiny(), dev, seed=3)
+    gen = LLMGenerator(m, 4, 64, cuda_graph=graph, kv_dtype="fp8")
+    prompts = torch.arange(32, dtype=torch.int32, device=dev).view(2, 16)
+    want = gen.generate(prompts, 2, 12, temperature=0.0)
+    tables = gen._tables
+
+    def broken(*args):
+        table, *rest = tables(*args)
+        table[3, 1] = gen.num_blocks + 7  # the block of the first decoded tokens
+        return (table, *rest)
+
+    gen._tables = broken
+    with pytest.raises(RuntimeError, match="out of range"):
+        gen.generate(prompts, 2, 12, temperature=0.0)
+    gen._tables = tables
+    again = gen.generate(prompts, 2, 12, temperature=0.0)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])

@@ -39,8 +39,9 @@ from ..ops.kv_cache import decode_attention_quant, kv_quant_read, kv_quant_write
 class LLMGenerator:
     """kv_dtype: "bf16", or "fp8" for e4m3 codes with a scale per token and KV
     head (0.52 of the bytes at head dimension 128: more sequences or longer
-    contexts in the same memory, and less to read per decoded token).  Kernels
-    set ``kv_error`` [1] if they meet a cache index out of range (fp8)."""
+    contexts in the same memory, and less to read per decoded token).  Its kernels
+    set ``kv_error`` [1] if they meet a cache index out of range: ``generate``
+    clears it, and raises RuntimeError if it is set at the end."""
 
     kv_dtype = "bf16"
 
@@ -345,6 +346,8 @@ class LLMGenerator:
         self.temperature = float(temperature)
         self.calls += 1
         table, pre_table, n_shared, tail = self._tables(P, G, Lp, max_new)
+        if self.kv_dtype == "fp8":
+            self.kv_error.zero_()
         prompts = prompts.to(self.device, torch.int32).contiguous()
         # ---- prefill the P prompts once; K/V land in the shared prompt blocks
         pos = torch.arange(Lp, device=self.device, dtype=torch.int32).repeat(P)
@@ -420,6 +423,8 @@ class LLMGenerator:
                 done_steps += n
                 if eos and int(st["n_done"].item()) >= B:  # every sequence has stopped
                     break
+        if self.kv_dtype == "fp8" and int(self.kv_error.item()):
+            raise RuntimeError("generate: the KV cache's kernels met an index out of range")
         self.last_lengths = st["lengths"].clone() if eos else None
         seqs = torch.cat([prompts.repeat_interleave(G, 0), st["tok_mat"]], 1)
         return seqs, st["lp_mat"].clone()
