@@ -41,8 +41,13 @@ void rows3(const at::Tensor& t, const char* op, const char* m) {
   chk(t.size(2) == 0 || t.size(1) <= INT_MAX / t.size(2), op, "at most 2^31 - 1 elements per row");
 }
 
-// What has no backward pass refuses tensors that would want one.
+// Whether t carries a forward-mode tangent.
+bool is_dual(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
+// What has no derivative refuses tensors that would want one (forward mode has no
+// switch: torch.no_grad() leaves it on).
 void no_grad(std::initializer_list<const at::Tensor*> ts, const char* op) {
+  for (const at::Tensor* t : ts) chk(!is_dual(*t), op, "has no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor* t : ts) chk(!t->requires_grad(), op, "has no gradient (call it under torch.no_grad)");
 }
@@ -135,6 +140,7 @@ Opt rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, 
     chk(out_->sizes() == x.sizes() && out_->scalar_type() == x.scalar_type(), op, "out has x's shape and type");
     chk(out_->device() == dev, op, "all tensors on one device");
     chk(rows_distinct(*out_), op, "out has overlapping rows");
+    chk(!is_dual(x) && !is_dual(*out_), op, "out= has no forward-mode derivative");
     chk(same_view(x, *out_) || columns_apart(x, *out_), op, "out is x itself or does not overlap it");
     for (const at::Tensor* t : {&pos, &table}) chk(apart(*out_, *t), op, "out overlaps an input");
   }
@@ -162,6 +168,11 @@ Opt rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, 
   a.transpose = transpose;
   a.err = err;
   cuda_ok(tb_rotary(&a, turbol::StreamFor(x)), op);
+  if (is_dual(x)) {  // the rotation is linear: the tangent turns like x
+    at::Tensor t = x._fw_grad(0);
+    if (t._is_zerotensor() || t.stride(2) != 1) t = at::empty(x.sizes(), x.options()).copy_(t);
+    out._set_fw_grad(*rotary(t, pos, table, std::nullopt, interleaved, transpose, error), 0, /*is_inplace_op=*/false);
+  }
   return out;
 }
 

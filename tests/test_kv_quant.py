@@ -784,3 +784,26 @@ def test_attention_infinite_scores(Hq, Hk, D, bs, device):
         err = torch.zeros(1, dtype=torch.int32, device=device)
         out = decode_attention_quant(q, *loud, torch.full_like(table, -1), ctx, error=err)
         assert (out == 0).all() and int(err) == 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_is_refused(device):
+    """A tangent would get lost, and torch.no_grad() leaves forward mode on: refused, inside it too."""
+    fw = torch.autograd.forward_ad
+    i32 = dict(dtype=torch.int32, device=device)
+    c = quant_kv_cache(2, 1, 16, 64, device)
+    table, seq, pos, ctx = torch.zeros(2, 1, **i32), torch.zeros(2, **i32), torch.arange(2, **i32), torch.ones(2, **i32)
+    x, q = torch.ones(2, 1, 64, device=device).bfloat16(), torch.ones(2, 4, 64, device=device).bfloat16()
+    rt = rotary_table(64, 8, device=device)
+    with fw.dual_level(), torch.no_grad():
+        def dual(t):
+            return fw.make_dual(t.clone(), torch.ones_like(t))
+
+        for call in (lambda: kv_quant_write(dual(x), x, seq, pos, table, *c),
+                     lambda: kv_quant_write(x, dual(x), seq, pos, table, *c),
+                     lambda: kv_quant_write(x, x, seq, pos, table, *c, q=dual(q), table=rt),
+                     lambda: kv_quant_read(*c, seq, pos, table, out=(dual(x), x.clone())),
+                     lambda: decode_attention_quant(dual(q), *c, table, ctx),
+                     lambda: decode_attention_quant(q, *c, table, ctx, out=dual(q))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()

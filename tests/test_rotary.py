@@ -285,3 +285,30 @@ def test_positions_out_of_range_in_place(T, H, D, R, interleaved, dtype, device)
     assert int(err) == 1 and x[bad].isnan().all() and want[bad].isnan().all()
     assert torch.equal(x[~bad], want[~bad])
     assert torch.equal(buf[:, :8], before[:, :8]) and torch.equal(buf[:, 8 + H * D:], before[:, 8 + H * D:])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_forward_mode(interleaved, device):
+    """A tangent is rotated like the value, with or without a gradient switch; where it would get lost, it is refused."""
+    fw = torch.autograd.forward_ad
+    T, H, D, R = 9, 3, 64, 32
+    table = rotary_table(R, 40, device=device)
+    pos = torch.randint(0, 40, (T,), dtype=torch.int32, device=device)
+    pos[3] = -1
+    x = torch.randn(T, H, D, device=device)
+    with fw.dual_level():
+        for t in (torch.randn(T, H, D, device=device), torch.randn(1, 1, 1, device=device).expand(T, H, D),
+                  torch.randn(D, H, T, device=device).permute(2, 1, 0)):
+            with torch.no_grad():
+                y, dy = fw.unpack_dual(rotary(fw.make_dual(x, t), pos, table, interleaved=interleaved))
+            check(y, x, pos, table, interleaved)
+            check(dy, t, pos, table, interleaved)
+            y, dy = fw.unpack_dual(rotary(fw.make_dual(x, t), pos, table, interleaved=interleaved, transpose=True))
+            check(dy, t, pos, table, interleaved, transpose=True)
+        assert fw.unpack_dual(rotary(x, pos, table)).tangent is None
+        dual = fw.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError, match="forward-mode"):
+            rotary(dual, pos, table, out=torch.empty_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):  # both modes at once
+            rotary(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), pos, table)

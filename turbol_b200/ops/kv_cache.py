@@ -60,7 +60,8 @@ def kv_quant_write(k: torch.Tensor, v: torch.Tensor, seq_of_token: torch.Tensor,
     and its q row is copied.  A sequence, position or block out of range writes
     nothing and sets ``error``; a position beyond the table also makes the q row
     NaN.  No two tokens of a call may name the same slot.  Not differentiable:
-    tensors that require a gradient are refused outside torch.no_grad."""
+    tensors that require a gradient are refused outside torch.no_grad, tangents of
+    forward mode always."""
     y = _call("kv_quant_write", k, v, seq_of_token, pos, block_table, kc, vc, ks, vs, q, q_out, table, interleaved, error)
     if not kc.is_cuda:
         y = torch.empty_like(q) if q is not None and q_out is None else q_out

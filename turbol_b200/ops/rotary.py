@@ -130,9 +130,9 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, interleaved:
     with one rounding; the other dimensions are copied.
 
     interleaved: pairs (2i, 2i + 1) instead of (i, i + R / 2).  transpose: the
-    backward's rotation (by the negative angles).  Differentiable in x, unless
-    ``out`` is given (x itself for in-place use, or a tensor that does not
-    overlap it).  A row with a negative position is padding and copied
+    backward's rotation (by the negative angles).  Differentiable in x, backward or
+    in forward mode (not both at once), unless ``out`` is given (x itself for
+    in-place use, or a tensor that does not overlap it).  A row with a negative position is padding and copied
     unrotated; one at or beyond the table's end becomes NaN and sets ``error``
     (an int32 device tensor, optional) to 1."""
     if out is None:
