@@ -46,10 +46,13 @@ bool is_dual(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 
 // What has no derivative refuses tensors that would want one (forward mode has no
 // switch: torch.no_grad() leaves it on).
-void no_grad(std::initializer_list<const at::Tensor*> ts, const char* op) {
-  for (const at::Tensor* t : ts) chk(!is_dual(*t), op, "has no forward-mode derivative");
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : ts) chk(!t->requires_grad(), op, "has no gradient (call it under torch.no_grad)");
+void no_grad(std::initializer_list<const at::Tensor*> ts, const char* op, const char* what = nullptr) {
+  const bool on = at::GradMode::is_enabled();
+  for (const at::Tensor* t : ts)
+    if (is_dual(*t) || (on && t->requires_grad()))
+      throw std::invalid_argument(std::string(op) + ": " + (what ? std::string(what) + " " : std::string()) +
+                                  (is_dual(*t) ? "has no forward-mode derivative"
+                                               : "has no gradient (call it under torch.no_grad)"));
 }
 
 // Bytes [lo, hi) that a view touches (empty: lo == hi).
@@ -121,6 +124,7 @@ void table_of(const at::Tensor& t, int64_t D, const char* op) {
           t.size(0) <= INT_MAX && t.size(1) >= 1 && 2 * t.size(1) <= D,
       op, "table is a contiguous fp32 [max_pos, R / 2, 2] with 1 <= R / 2 <= D / 2");
   chk(reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0, op, "table is 8-byte aligned");
+  no_grad({&t}, op, "the table");
 }
 
 using Opt = std::optional<at::Tensor>;
@@ -206,6 +210,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 at::Tensor rotary_grad(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, bool interleaved,
                        bool transpose, const Opt& error) {
   chk(x.is_cuda(), "rotary_grad", "CUDA tensors");
+  no_grad({&table}, "rotary", "the table");  // (inside the node gradients are off)
   return RotaryFunction::apply(x, pos, table, interleaved, transpose, error);
 }
 
@@ -217,6 +222,7 @@ TbQuantCache cache_of(const at::Tensor& kc, const at::Tensor& vc, const at::Tens
   chk(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.dim() == 3 && ks.sizes() == vs.sizes() &&
           ks.is_contiguous() && vs.is_contiguous() && ks.sizes() == kc.sizes().slice(0, 3),
       op, "ks and vs are contiguous fp32 [num_blocks, Hk, block_size]");
+  no_grad({&kc, &vc, &ks, &vs}, op, "the cache");
   const int64_t D = kc.size(3);
   chk(D == 64 || D == 128 || D == 256, op, "head dimension 64, 128 or 256");
   chk(kc.size(1) >= 1 && kc.size(2) >= 1, op, "at least one KV head and one slot per block");

@@ -807,3 +807,21 @@ def test_forward_mode_is_refused(device):
                      lambda: decode_attention_quant(q, *c, table, ctx, out=dual(q))):
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_of_scales_and_table_are_refused(device):
+    i32 = dict(dtype=torch.int32, device=device)
+    c = quant_kv_cache(2, 1, 16, 64, device)
+    table, seq, pos, ctx = torch.zeros(2, 1, **i32), torch.zeros(2, **i32), torch.arange(2, **i32), torch.ones(2, **i32)
+    x, q = torch.ones(2, 1, 64, device=device).bfloat16(), torch.ones(2, 4, 64, device=device).bfloat16()
+    rt = rotary_table(64, 8, device=device).requires_grad_()
+    scales = [(c.kc, c.vc, c.ks.clone().requires_grad_(), c.vs), (c.kc, c.vc, c.ks, c.vs.clone().requires_grad_())]
+    for call in [lambda: kv_quant_write(x, x, seq, pos, table, *c, q=q, table=rt)] + \
+            [f for s in scales for f in (lambda s=s: kv_quant_write(x, x, seq, pos, table, *s),
+                                         lambda s=s: kv_quant_read(*s, seq, pos, table),
+                                         lambda s=s: decode_attention_quant(q, *s, table, ctx))]:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()

@@ -312,3 +312,18 @@ def test_forward_mode(interleaved, device):
             rotary(dual, pos, table, out=torch.empty_like(x))
         with pytest.raises((RuntimeError, NotImplementedError)):  # both modes at once
             rotary(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), pos, table)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_of_the_table_are_refused(device):
+    """The table's gradient would be dropped without a word: refused, with and without a gradient of x."""
+    x, pos = torch.randn(3, 2, 64, device=device), torch.arange(3, dtype=torch.int32, device=device)
+    table = rotary_table(64, 8, device=device).requires_grad_()
+    for a in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="table"):
+            rotary(a, pos, table)
+        with torch.no_grad():
+            check(rotary(a, pos, table), x, pos, table.detach())
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError, match="table"):
+            rotary(x, pos, torch.autograd.forward_ad.make_dual(table.detach(), torch.ones_like(table)))

@@ -132,13 +132,16 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, interleaved:
     interleaved: pairs (2i, 2i + 1) instead of (i, i + R / 2).  transpose: the
     backward's rotation (by the negative angles).  Differentiable in x, backward or
     in forward mode (not both at once), unless ``out`` is given (x itself for
-    in-place use, or a tensor that does not overlap it).  A row with a negative position is padding and copied
+    in-place use, or a tensor that does not overlap it); a table that requires a
+    gradient is refused.  A row with a negative position is padding and copied
     unrotated; one at or beyond the table's end becomes NaN and sets ``error``
     (an int32 device tensor, optional) to 1."""
     if out is None:
         if x.requires_grad and torch.is_grad_enabled():
             if x.is_cuda:
                 return _core().ops.rotary_grad(x, pos, table, interleaved, transpose, error)
+            if table.requires_grad:
+                raise ValueError("rotary: the table has no gradient (call it under torch.no_grad)")
             return _Rotary.apply(x, pos, table, interleaved, transpose, error)
     elif torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
         raise ValueError("rotary: out= has no gradient")
