@@ -98,7 +98,8 @@ int launch_vec(const TbRotaryArgs& a, cudaStream_t s) {
   const long long per = static_cast<long long>(units) * HS;
   constexpr int kThreads = threads_of(HU);
   const int tokens = per >= kThreads ? 1 : static_cast<int>(kThreads / per);
-  rotary_kernel<T, NP, HU, INTER><<<(a.T + tokens - 1) / tokens, kThreads, 0, s>>>(a, rot_units, units, HS, tokens);
+  const int grid = static_cast<int>((a.T + (tokens - 1ll)) / tokens);  // (T + tokens can pass 31 bits)
+  rotary_kernel<T, NP, HU, INTER><<<grid, kThreads, 0, s>>>(a, rot_units, units, HS, tokens);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -327,3 +327,16 @@ def test_gradients_of_the_table_are_refused(device):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(ValueError, match="table"):
             rotary(x, pos, torch.autograd.forward_ad.make_dual(table.detach(), torch.ones_like(table)))
+
+
+@pytest.mark.gpu
+def test_rows_up_to_31_bits(dev):
+    """2^31 - 1 rows: the number of blocks does not overflow."""
+    T = 2 ** 31 - 1
+    table = rotary_table(2, 4, device=dev)
+    pos = torch.ones(T, dtype=torch.int32, device=dev)
+    pos[-1] = 3
+    x = torch.tensor([[[1.0, 0.5]]], dtype=torch.bfloat16, device=dev).expand(T, 1, 2)
+    y = rotary(x, pos, table)
+    for rows in (slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)):
+        check(y[rows], x[rows], pos[rows], table)
