@@ -220,3 +220,36 @@ def test_generate_reports_cache_errors(graph, dev):
     gen._tables = tables
     again = gen.generate(prompts, 2, 12, temperature=0.0)
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+def test_cached_kv_before_generate(kv_dtype):
+    from turbol_b200.rl.rollout import LLMGenerator
+
+    gen = LLMGenerator(DecoderLM(tiny(), "cpu", master=False), 2, 32, kv_dtype=kv_dtype)
+    for layer in (0, 99):
+        with pytest.raises(ValueError):
+            gen.cached_kv(layer, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+def test_cached_kv_ends_where_the_cache_does(kv_dtype, dev):
+    """No rows past the tokens that were written (they would come from other sequences' blocks): the last sampled token
+    is not among them, nor is what an early stop left out."""
+    from turbol_b200.rl.rollout import LLMGenerator
+
+    gen = LLMGenerator(DecoderLM(tiny(), dev, seed=3), 4, 64, kv_dtype=kv_dtype)
+    prompts = torch.arange(40, dtype=torch.int32, device=dev).view(2, 20)
+    for new, eos, want in ((1, -1, 20), (9, -1, 28), (30, None, None)):
+        if eos is None:  # a token that every sequence samples at once: stops at the first check
+            eos = int(gen.generate(prompts[:1], 1, 1, temperature=0.0)[0][0, -1])
+            gen.generate(prompts[:1], 2, new, temperature=0.0, eos_id=eos, stop_check=4)
+            want = 24
+        else:
+            gen.generate(prompts, 2, new, temperature=0.0)
+        assert gen.cached == want
+        assert gen.cached_kv(1, 1, want)[0].shape == (want, gen.cfg.n_kv_heads, gen.cfg.head_dim)
+        for seq, n in ((0, want + 1), (0, -1), (4, 1), (-1, 1)):
+            with pytest.raises(ValueError):
+                gen.cached_kv(0, seq, n)

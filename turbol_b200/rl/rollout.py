@@ -44,6 +44,7 @@ class LLMGenerator:
     clears it, and raises RuntimeError if it is set at the end."""
 
     kv_dtype = "bf16"
+    cached = 0  # tokens of each sequence that the cache holds since the last generate call
 
     def __init__(self, model: DecoderLM, max_batch: int, max_len: int, block_size: int = 16, seed: int = 0,
                  cuda_graph: bool = True, decode_gemm: Optional[bool] = None, attn_split: int = 1,
@@ -132,10 +133,13 @@ class LLMGenerator:
     def cached_kv(self, layer: int, seq: int, n: int):
         """The first n cached (rotated) keys and values of sequence ``seq`` of the
         last ``generate`` call, as attention sees them: two bf16 [n, kv_heads,
-        head_dim] tensors."""
+        head_dim] tensors.  n is at most ``self.cached``: the prompt and all
+        generated tokens but the last, which is sampled and not decoded."""
+        if self.cached == 0 or layer not in self.m.layers:
+            raise ValueError("cached_kv: no such layer, or nothing generated yet")
         li = self.m.layers.index(layer)
-        if not 0 <= seq < self.state["table"].shape[0] or not 0 <= n <= self.max_len:
-            raise ValueError("cached_kv: no such sequence or length")
+        if not 0 <= seq < self.state["table"].shape[0] or not 0 <= n <= self.cached:
+            raise ValueError("cached_kv: no such sequence, or beyond what is cached")
         pos = torch.arange(n, device=self.device, dtype=torch.int32)
         if self.kv_dtype == "fp8":
             return kv_quant_read(*self.kvq[li], torch.full_like(pos, seq), pos, self.state["table"],
@@ -345,6 +349,7 @@ class LLMGenerator:
             self._graph = None  # the captured step holds the sampler's kind
         self.temperature = float(temperature)
         self.calls += 1
+        self.cached = 0
         table, pre_table, n_shared, tail = self._tables(P, G, Lp, max_new)
         if self.kv_dtype == "fp8":
             self.kv_error.zero_()
@@ -390,6 +395,7 @@ class LLMGenerator:
         st["pos"].fill_(Lp)
         st["ctx"].fill_(Lp + 1)
         steps = max_new - 1
+        done_steps = 0
         if steps > 0:
             if self.cuda_graph:
                 # capture one decode step once per (batch, length) shape, then
@@ -415,7 +421,6 @@ class LLMGenerator:
             else:
                 def step_fn():
                     self._decode_step(B)
-            done_steps = 0
             while done_steps < steps:
                 n = min(stop_check if eos else steps, steps - done_steps)
                 for _ in range(n):
@@ -425,6 +430,7 @@ class LLMGenerator:
                     break
         if self.kv_dtype == "fp8" and int(self.kv_error.item()):
             raise RuntimeError("generate: the KV cache's kernels met an index out of range")
+        self.cached = Lp + done_steps
         self.last_lengths = st["lengths"].clone() if eos else None
         seqs = torch.cat([prompts.repeat_interleave(G, 0), st["tok_mat"]], 1)
         return seqs, st["lp_mat"].clone()
@@ -617,6 +623,7 @@ class TPLLMGenerator(LLMGenerator):
             raise ValueError("generate: the prompt count must divide by the tensor-parallel size")
         self.temperature = float(temperature)
         self.calls += 1
+        self.cached = 0
         table, pre_table, n_shared, tail = self._tables(P, G, Lp, max_new)
         prompts = prompts.to(self.device, torch.int32).contiguous()
         pos = torch.arange(Lp, device=self.device, dtype=torch.int32).repeat(P)
@@ -679,6 +686,7 @@ class TPLLMGenerator(LLMGenerator):
             else:
                 for _ in range(steps):
                     self._decode_step(B)
+        self.cached = Lp + max(steps, 0)
         group_pg = getattr(tpm.comm, "group", None)
         tok_all = torch.empty(B, max_new, device=self.device, dtype=torch.int32)
         lp_all = torch.empty(B, max_new, device=self.device, dtype=torch.float32)
