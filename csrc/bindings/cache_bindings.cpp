@@ -404,7 +404,7 @@ Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::
       chk(apart(out, range_of(*t)), op, "out overlaps an input");
   }
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt(static_cast<double>(a.cache.D));
-  chk(std::isfinite(scale), op, "a finite scale");
+  chk(std::isfinite(static_cast<float>(scale * M_LOG2E)), op, "a scale that is finite in fp32, times log2(e) too");
   a.err = error_of(error, dev, op);
   if (!kc.is_cuda()) return std::nullopt;
   c10::cuda::CUDAGuard guard(dev);

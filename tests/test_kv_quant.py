@@ -825,3 +825,17 @@ def test_gradients_of_scales_and_table_are_refused(device):
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scales_past_fp32_are_refused(device):
+    """A scale that is finite in 64 bits and infinite in the kernel's 32."""
+    i32 = dict(dtype=torch.int32, device=device)
+    c = quant_kv_cache(1, 1, 16, 64, device)
+    q = torch.zeros(1, 1, 64, device=device).bfloat16()
+    args = (q, *c, torch.zeros(1, 1, **i32), torch.ones(1, **i32))
+    for scale in (1e39, -1e300, 3e38):  # (3e38 overflows with the factor log2(e))
+        with pytest.raises(ValueError, match="scale"):
+            decode_attention_quant(*args, scale=scale)
+    for scale in (2e38, -2e38, 0.0, 1e-300):
+        assert (decode_attention_quant(*args, scale=scale) == 0).all()
