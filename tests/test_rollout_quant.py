@@ -253,3 +253,19 @@ def test_cached_kv_ends_where_the_cache_does(kv_dtype, dev):
         for seq, n in ((0, want + 1), (0, -1), (4, 1), (-1, 1)):
             with pytest.raises(ValueError):
                 gen.cached_kv(0, seq, n)
+
+
+@pytest.mark.parametrize("backend", ["native", "echo", "vllm"])
+def test_engine_checks_its_kv_dtype(backend):
+    """Unknown caches are refused whatever the backend, and an 8-bit one where the backend would not use it."""
+    from turbol_b200.rl.rollout import RolloutConfig, RolloutEngine
+
+    with pytest.raises(ValueError, match="kv_dtype"):
+        RolloutEngine(RolloutConfig(inference_backend=backend, kv_dtype="int3", device="cpu")).initialize()
+    if backend == "vllm":
+        with pytest.raises(ValueError, match="kv_dtype"):
+            RolloutEngine(RolloutConfig(inference_backend=backend, kv_dtype="fp8", device="cpu")).initialize()
+    elif backend == "echo":
+        e = RolloutEngine(RolloutConfig(inference_backend=backend, kv_dtype="fp8"))
+        e.initialize()
+        assert e.generate("x") == "[RolloutEngine] x"

@@ -463,6 +463,10 @@ class RolloutEngine:
 
     def initialize(self):
         c = self.config
+        if c.kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype: 'bf16' or 'fp8', not {c.kv_dtype!r}")
+        if c.kv_dtype != "bf16" and c.inference_backend == "vllm":
+            raise ValueError("kv_dtype is the native engine's; the vllm backend has its own cache")
         self._tok = _core().ByteTokenizer()
         Status = _core().Status
         if c.inference_backend == "native" and torch.cuda.is_available():
