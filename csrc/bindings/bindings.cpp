@@ -798,5 +798,9 @@ PYBIND11_MODULE(turbol_core, m) {
   py::module_ dist = m.def_submodule("dist", "C++ distributed runtime: NcclCommunicator, DistributedTrainer, "
                                                "PipelineTrainer (turbol/distributed.hpp)");
   register_dist(dist);
+#else
+  py::module_ host_ops = m.def_submodule("host_ops", "operators that check their arguments here and leave CPU tensors "
+                                                     "to plain math");
+  register_cache_ops(host_ops);
 #endif
 }

@@ -2,9 +2,10 @@
 // paged KV cache.  Each checks its arguments completely, whatever device they
 // are on, then launches on the current stream of their device and returns its
 // result (a new tensor where no output was given); for CPU tensors it returns
-// None and the caller computes on the host.
+// None and the caller computes on the host.  The CPU-only build has them too, for
+// the checks.
 #include <ATen/ATen.h>
-#include <c10/cuda/CUDAGuard.h>
+#include <c10/core/DeviceGuard.h>
 #include <pybind11/pybind11.h>
 #include <torch/extension.h>
 
@@ -150,7 +151,7 @@ Opt rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, 
   }
   int* err = error_of(error, dev, op);
   if (!x.is_cuda()) return std::nullopt;
-  c10::cuda::CUDAGuard guard(dev);
+  c10::DeviceGuard guard(dev);
   at::Tensor out = out_ ? *out_ : at::empty(x.sizes(), x.options());
   if (x.numel() == 0) return out;
   TbRotaryArgs a{};
@@ -308,7 +309,7 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
       chk(apart(out, range_of(*t)), op, "q_out overlaps an input");
   }
   if (!kc.is_cuda()) return std::nullopt;
-  c10::cuda::CUDAGuard guard(dev);
+  c10::DeviceGuard guard(dev);
   Opt q_out = q_out_;
   if (q_ && !q_out) q_out = at::empty(q_->sizes(), q_->options());
   if (T == 0) return q_out;
@@ -360,7 +361,7 @@ bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
   a.err = error_of(error, dev, op);
   if (!kc.is_cuda()) return false;
   if (T == 0) return true;
-  c10::cuda::CUDAGuard guard(dev);
+  c10::DeviceGuard guard(dev);
   a.k = k_out.data_ptr();
   a.v = v_out.data_ptr();
   a.ks_t = k_out.stride(0);
@@ -407,7 +408,7 @@ Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::
   chk(std::isfinite(static_cast<float>(scale * M_LOG2E)), op, "a scale that is finite in fp32, times log2(e) too");
   a.err = error_of(error, dev, op);
   if (!kc.is_cuda()) return std::nullopt;
-  c10::cuda::CUDAGuard guard(dev);
+  c10::DeviceGuard guard(dev);
   at::Tensor ws, out = out_ ? *out_ : at::empty(q.sizes(), q.options());
   if (B == 0) return out;
   a.q = q.data_ptr();

@@ -64,4 +64,22 @@ int tb_sample_indices(int* idx, int n, long long size, unsigned long long seed, 
   return static_cast<int>(cudaErrorNoDevice);
 }
 
+int tb_rotary(const TbRotaryArgs* args, cudaStream_t s) {
+  return static_cast<int>(cudaErrorNoDevice);
+}
+
+int tb_kv_quant_write(const TbKvQuantWriteArgs* args, cudaStream_t s) {
+  return static_cast<int>(cudaErrorNoDevice);
+}
+
+int tb_kv_quant_read(const TbKvQuantReadArgs* args, cudaStream_t s) {
+  return static_cast<int>(cudaErrorNoDevice);
+}
+
+size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens) { return 0; }
+
+int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s) {
+  return static_cast<int>(cudaErrorNoDevice);
+}
+
 }  // extern "C"

@@ -6,8 +6,9 @@
 CPU-only build (TURBOL_CPU_ONLY=1): the host runtime (Tensor/Config/engines on
 CPU tensors/profiler/writers/tokenizer/dataset/store/schedules/KV allocator and
 the pybind11 module) compiled with the C++ compiler alone against torch's CPU
-headers: no nvcc, no CUDA runtime, no kernels (the ``ops`` submodule is absent
-and ``built_for()`` returns "cpu").  It is for machines without a GPU and for
+headers: no nvcc, no CUDA runtime, no kernels (the ``ops`` submodule is absent,
+``host_ops`` has what only checks arguments there, and ``built_for()`` returns
+"cpu").  It is for machines without a GPU and for
 CI; write it to its own --build-lib so it does not replace the CUDA build.
 
 One extension, ``turbol_b200.turbol_core``, holds both the C++ host runtime
@@ -72,7 +73,8 @@ CPU_ONLY = os.environ.get("TURBOL_CPU_ONLY", "") not in ("", "0")
 
 
 def cpu_sources():
-    pats = ["csrc/core/*.cpp", "csrc/engines/*.cpp", "csrc/bindings/bindings.cpp", "csrc/cpu_only/*.cpp"]
+    pats = ["csrc/core/*.cpp", "csrc/engines/*.cpp", "csrc/bindings/bindings.cpp", "csrc/bindings/cache_bindings.cpp",
+            "csrc/cpu_only/*.cpp"]
     out = []
     for p in pats:
         out += sorted(glob.glob(os.path.join(ROOT, p)))

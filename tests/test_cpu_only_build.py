@@ -76,3 +76,54 @@ def test_cpu_only_core_builds_and_runs(tmp_path):
     code = f"REPO = {ROOT!r}\nLIB = {str(lib)!r}\n" + CHECK
     r = subprocess.run([sys.executable, "-c", code], cwd=str(tmp_path), capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "CPU_ONLY_OK" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]
+
+
+CACHE_CHECK = r'''
+import sys, os
+sys.path = [p for p in sys.path if os.path.abspath(p or ".") != REPO]
+sys.path.insert(0, LIB)
+import torch
+import turbol_b200
+from turbol_b200 import turbol_core as C
+from turbol_b200.ops.kv_cache import decode_attention_quant, kv_quant_read, kv_quant_write, quant_kv_cache
+from turbol_b200.ops.rotary import rotary, rotary_table
+assert os.path.abspath(turbol_b200.__file__).startswith(os.path.abspath(LIB)), turbol_b200.__file__
+assert C.built_for() == "cpu" and not hasattr(C, "ops")
+i32 = dict(dtype=torch.int32)
+c = quant_kv_cache(2, 1, 16, 64, "cpu")
+table, seq, pos, ctx = torch.zeros(3, 1, **i32), torch.zeros(3, **i32), torch.arange(3, **i32), torch.ones(3, **i32)
+x, q, rt = torch.randn(3, 1, 64).bfloat16(), torch.randn(3, 4, 64).bfloat16(), rotary_table(64, 8, device="cpu")
+refused = [lambda: rotary(x, pos.long(), rt), lambda: rotary(x.double(), pos, rt), lambda: rotary(x, pos, rt, out=x[:, :, ::1].expand(3, 1, 64)[:2]),
+           lambda: rotary(x.clone().requires_grad_(), pos[:2], rt),
+           lambda: kv_quant_write(x, x[:2], seq, pos, table, *c), lambda: kv_quant_write(x, x, seq.long(), pos, table, *c),
+           lambda: kv_quant_write(x, x, seq, pos, table, c.kc, c.kc, c.ks, c.vs), lambda: kv_quant_read(*c, seq[:2], pos, table),
+           lambda: decode_attention_quant(q.float(), *c, table, ctx), lambda: decode_attention_quant(q, *c, table, ctx, out=q),
+           lambda: decode_attention_quant(q, *c, table, ctx, scale=float("nan")),
+           lambda: decode_attention_quant(q.clone().requires_grad_(), *c, table, ctx)]
+for i, call in enumerate(refused):
+    try:
+        call()
+    except ValueError:
+        continue
+    raise AssertionError(f"call {i} was not refused")
+assert rotary(x, pos, rt).shape == x.shape
+assert torch.equal(kv_quant_write(x, x, seq, pos, table, *c, q=q, table=rt)[:1], q[:1])
+assert kv_quant_read(*c, seq, pos, table)[0].shape == x.shape
+assert decode_attention_quant(q, *c, table, ctx).shape == q.shape
+print("CACHE_CHECKS_OK")
+'''
+
+
+@pytest.mark.skipif(shutil.which("g++") is None and shutil.which("c++") is None, reason="no C++ compiler")
+def test_cpu_only_operators_check_their_arguments(tmp_path):
+    """The operators with a plain form on the host refuse there what they refuse in the CUDA build."""
+    lib, tmp = tmp_path / "lib", tmp_path / "tmp"
+    env = dict(os.environ, TURBOL_CPU_ONLY="1", MAX_JOBS=str(max(1, os.cpu_count() or 1)))
+    b = subprocess.run([sys.executable, "setup.py", "build_ext", "--build-lib", str(lib), "--build-temp", str(tmp)],
+                       cwd=ROOT, env=env, capture_output=True, text=True, timeout=1200)
+    assert b.returncode == 0, b.stdout[-3000:] + b.stderr[-3000:]
+    shutil.copytree(os.path.join(ROOT, "turbol_b200"), lib / "turbol_b200", dirs_exist_ok=True,
+                    ignore=shutil.ignore_patterns("*.so", "__pycache__"))
+    code = f"REPO = {ROOT!r}\nLIB = {str(lib)!r}\n" + CACHE_CHECK
+    r = subprocess.run([sys.executable, "-c", code], cwd=str(tmp_path), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "CACHE_CHECKS_OK" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]

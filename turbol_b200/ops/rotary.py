@@ -86,12 +86,12 @@ def rotary_table(rot_dim: int, max_pos: int, theta: float = 1e4, scaling: Option
 
 @functools.lru_cache(maxsize=None)
 def _entry(name: str):
-    o = getattr(_core(), "ops", None)
-    return (lambda *args: None) if o is None else getattr(o, name)
+    c = _core()
+    return getattr(c.ops if hasattr(c, "ops") else c.host_ops, name)
 
 
 def _call(name: str, *args):
-    """A kernel entry point: checks, launches and returns its result; None for CPU tensors (or a CPU-only build)."""
+    """A kernel entry point: checks, launches and returns its result; None for CPU tensors."""
     return _entry(name)(*args)
 
 
