@@ -839,3 +839,19 @@ def test_scales_past_fp32_are_refused(device):
             decode_attention_quant(*args, scale=scale)
     for scale in (2e38, -2e38, 0.0, 1e-300):
         assert (decode_attention_quant(*args, scale=scale) == 0).all()
+
+
+def test_attention_far_behind_its_table_on_the_host():
+    """A context of 2^31 - 1 tokens over a table of 12: the host does not walk (or hold) the missing ones."""
+    Hq, Hk, D, bs, nb = 4, 2, 64, 4, 8
+    g = torch.Generator().manual_seed(9)
+    c = random_cache(nb, Hk, bs, D, "cpu", g)
+    q = torch.randn(2, Hq, D, generator=g).bfloat16()
+    table = torch.tensor([[4, 5, 6], [1, 2, 3]], dtype=torch.int32)
+    err = torch.zeros(1, dtype=torch.int32)
+    out = decode_attention_quant(q, *c, table, torch.tensor([2 ** 31 - 1, 12], dtype=torch.int32), error=err)
+    assert int(err) == 1
+    check_attention(out, q, c, table, [12, 12], D ** -0.5)
+    err.zero_()
+    decode_attention_quant(q, *c, table, torch.tensor([12, 12], dtype=torch.int32), error=err)
+    assert int(err) == 0

@@ -276,7 +276,8 @@ def decode_attention_quant(q, kc, vc, ks, vs, block_table, ctx_len, scale, out=N
     num_blocks, Hk, bs, _ = kc.shape
     y = torch.zeros(B, Hq, D, dtype=dtype, device=q.device)
     for b, n in enumerate(ctx_len.tolist()):
-        idx = torch.arange(max(n, 0), device=q.device)
+        # (one token behind the table is enough to tell of all)
+        idx = torch.arange(min(max(n, 0), block_table.shape[1] * bs + 1), device=q.device)
         t, blk, slot = _slots(torch.full_like(idx, b), idx, block_table, num_blocks, bs, error)
         if t.numel() == 0:
             continue
