@@ -56,6 +56,13 @@ void no_grad(std::initializer_list<const at::Tensor*> ts, const char* op, const 
                                                : "has no gradient (call it under torch.no_grad)"));
 }
 
+// Tells autograd that a kernel writes to `ts`, so that a backward pass that needs
+// what was there raises.
+void written(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // Bytes [lo, hi) that a view touches (empty: lo == hi).
 struct Range {
   uintptr_t lo, hi;
@@ -173,6 +180,7 @@ Opt rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, 
   a.transpose = transpose;
   a.err = err;
   cuda_ok(tb_rotary(&a, turbol::StreamFor(x)), op);
+  if (out_) written({&*out_});
   if (is_dual(x)) {  // the rotation is linear: the tangent turns like x
     at::Tensor t = x._fw_grad(0);
     if (t._is_zerotensor() || t.stride(2) != 1) t = at::empty(x.sizes(), x.options()).copy_(t);
@@ -332,6 +340,8 @@ Opt kv_quant_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& s
   a.pos = pos.data_ptr<int>();
   a.T = static_cast<int>(T);
   cuda_ok(tb_kv_quant_write(&a, turbol::StreamFor(kc)), op);
+  written({&kc, &vc, &ks, &vs});
+  if (q_out_) written({&*q_out_});
   return q_out;
 }
 
@@ -372,6 +382,7 @@ bool kv_quant_read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
   a.pos = pos.data_ptr<int>();
   a.T = static_cast<int>(T);
   cuda_ok(tb_kv_quant_read(&a, turbol::StreamFor(kc)), op);
+  written({&k_out, &v_out});
   return true;
 }
 
@@ -429,6 +440,7 @@ Opt decode_attention_quant(const at::Tensor& q, const at::Tensor& kc, const at::
     a.ws = ws.data_ptr<float>();
   }
   cuda_ok(tb_decode_attention_quant(&a, turbol::StreamFor(kc)), op);
+  if (out_) written({&*out_});
   return out;
 }
 

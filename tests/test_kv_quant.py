@@ -855,3 +855,32 @@ def test_attention_far_behind_its_table_on_the_host():
     err.zero_()
     decode_attention_quant(q, *c, table, torch.tensor([12, 12], dtype=torch.int32), error=err)
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_writes_are_told_to_autograd(device):
+    """A backward pass over what a call has overwritten raises, as after torch's own in-place operations."""
+    i32 = dict(dtype=torch.int32, device=device)
+    c = quant_kv_cache(2, 1, 16, 64, device)
+    table, seq, pos, ctx = torch.zeros(2, 1, **i32), torch.zeros(2, **i32), torch.arange(2, **i32), torch.ones(2, **i32)
+    x, q = torch.ones(2, 1, 64, device=device), torch.ones(2, 4, 64, device=device)
+    rt, half = rotary_table(64, 8, device=device), torch.ones(2, 4, 64, device=device).bfloat16()
+    w = torch.ones(1, device=device, requires_grad=True)
+    out = (torch.zeros_like(x), torch.zeros_like(x))
+    for call, changed in ((lambda: rotary(q, pos, rt, out=q), [q]),
+                          (lambda: kv_quant_write(x, x, seq, pos, table, *c), [c.ks, c.vs]),
+                          (lambda: kv_quant_write(x, x, seq, pos, table, *c, q=q, table=rt, q_out=q), [c.ks, c.vs, q]),
+                          (lambda: kv_quant_read(*c, seq, pos, table, out=out), list(out)),
+                          (lambda: decode_attention_quant(half.clone(), *c, table, ctx, out=half), [half])):
+        losses = [(t * w).sum() for t in changed]
+        codes = [t._version for t in c[:2]]
+        call()
+        for loss in losses:
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                loss.backward()
+        if changed[0] is c.ks:
+            assert all(t._version > v for t, v in zip(c[:2], codes))
+    with torch.inference_mode():
+        z = torch.ones(2, 4, 64, device=device)
+    with torch.inference_mode():
+        rotary(z, pos, rt, out=z)
