@@ -55,16 +55,16 @@ def rotary_inv_freq(rot_dim: int, theta: float = 1e4, scaling: Optional[dict] = 
             raise ValueError(f"rotary: {kind} scaling needs original_max_pos")
     if kind == "llama3":
         lo, hi = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
-        if not (hi > lo > 0 and n > 0):
-            raise ValueError("rotary: llama3 scaling needs high_freq_factor above low_freq_factor above 0 and a positive "
+        if not (hi > lo and n > 0):
+            raise ValueError("rotary: llama3 scaling needs high_freq_factor above low_freq_factor and a positive "
                              "original_max_pos")
         keep = ((n * inv / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
         return inv * (keep + (1 - keep) / f), 1.0
     if kind == "yarn":
         fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
-        if not (fast > slow > 0 and theta > 1 and n > 0):
-            raise ValueError("rotary: yarn scaling needs beta_fast above beta_slow above 0, theta above 1 and a positive "
-                             "original_max_pos")
+        if not (fast >= slow > 0 and theta > 1 and n > 0):
+            raise ValueError("rotary: yarn scaling needs beta_slow above 0 and not above beta_fast, theta above 1 and a "
+                             "positive original_max_pos")
 
         def index_of(turns):  # the (fractional) pair index that makes this many turns over n positions
             return rot_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(theta))
