@@ -38,9 +38,9 @@
 //    2^15 and most tiles need no reduction over the warp and no rescaling.  q is
 //    brought into fp16 range by a power of two per head (exact).
 //
-// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 96 us,
-// 5.8 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 28 us; 1 x
-// 1,000 tokens x 8 KV heads 6.1 us.
+// On one B200, D = 128, in a graph: 2 x 131,072 tokens x 8 KV heads (554 MB) 97 us,
+// 5.7 TB/s; 512 ragged contexts up to 768 tokens x 2 KV heads (96 MB) 29 us; 1 x
+// 1,000 tokens x 8 KV heads 6.2 us.
 #include <float.h>
 #include <math.h>
 
@@ -117,8 +117,8 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 // Shared memory.  A ring stage holds 16 K rows and 16 V rows of codes (rows
 // padded by 16 bytes against bank conflicts), their scales and a mask of the
 // tokens that count.  Two stages are enough at D = 128 and 256, the next tile being
-// asked for before one is used (2 x 131,072 tokens x 8 KV heads x 128: 97 us, with
-// three 103); small tiles and two sets of heads take three.  A part is heads x D
+// asked for before one is used (2 x 131,072 tokens x 8 KV heads x 128: 98 us, with
+// three 104); small tiles and two sets of heads take three.  A part is heads x D
 // outputs, then heads x (maximum, sum): a warp's first one goes to its place behind
 // the rings, its last one into its own ring, drained by then.
 template <int D, int NT>
@@ -136,7 +136,7 @@ struct Smem {
 
 // CTAs per SM: those that shared memory (228 KB, 1 KB of it per CTA the system's)
 // leaves room for, up to 4.  Lists at D = 128 have three of them: with four, 2 x
-// 131,072 tokens x 8 KV heads took 101 us for 96, and no mix of contexts gained over 2%.
+// 131,072 tokens x 8 KV heads took 100 us for 98, and no mix of contexts gained over 2%.
 template <int D, int NT>
 constexpr int resident() {
   constexpr int kFit = 233472 / (Smem<D, NT>::kBytes + 1024);
@@ -365,9 +365,9 @@ __device__ __forceinline__ void cluster_join(const TbDecodeAttnQuantArgs& a, con
 
 // kClusters: a cluster (or one CTA) for each (sequence, eight query heads), else even
 // lists: two kernels, since what a CTA does not need costs it instruction fetches (one
-// short context: 4.3 us, from one kernel for both 5.1).  kPlain: pages of whole tiles,
+// short context: 4.2 us, from one kernel for both 5.1).  kPlain: pages of whole tiles,
 // and q and out aligned for vectors, else as the flags say (with the flags: 512 ragged
-// contexts up to 768 x 2 KV heads 29.5 us for 28.5, 37 up to 1,536 x 8 18.7 for 17.6).
+// contexts up to 768 x 2 KV heads 29.5 us for 29.0, 37 up to 1,536 x 8 18.7 for 18.1).
 template <typename T, int D, int NT, bool kClusters, bool kPlain>
 __global__ void __launch_bounds__(kThreads, kClusters ? resident<D, NT>() : list_ctas<D, NT>())
     decode_attn_quant_kernel(TbDecodeAttnQuantArgs a, Geometry g, bool q_aligned, bool out_aligned) {
@@ -1054,9 +1054,14 @@ int sm_count() {  // of the current device, asked for once
 // of them share.  Measured on one B200 (D = 128): lists 10.5 us and 0.76 ns per tile, of
 // which contexts of mixed lengths have half of `cap`; clusters 5.7 us, 0.85 us per
 // tile of a warp and a fifth of the lists' time for the tiles.  Clusters and lists: 1 x
-// 1,000 tokens x 8 KV heads 6.6 and 10.3 us, 8 x 4,096 x 8 18.3 and 22.7, 37 ragged up to
-// 1,536 x 8 18.7 and 20.8, 64 x 1,000 x 8 27.4 and 33.8 (ragged 21.8 and 22.4), 16 ragged
-// up to 8,000 x 8 37.0 and 32.8.
+// 1,000 tokens x 8 KV heads 6.2 and 10.4 us, 8 x 4,096 x 8 17.9 and 22.2, 37 ragged up to
+// 1,536 x 8 18.3 and 20.2, 64 x 1,000 x 8 26.9 and 33.1 (ragged 21.2 and 21.8), 16 ragged
+// up to 8,000 x 8 35.1 and 32.3.  The numbers were fitted there and serve D = 64 and 256
+// too, where the same contexts take 5.6 and 9.9, 13.6 and 17.4, 14.0 and 15.9, 18.6 and
+// 23.8 (16.0 and 17.1), 26.1 and 23.9 us at 64; 7.9 and 11.8, 29.2 and 33.4 (lists are
+// taken), 32.5 and 29.6, 55 either way (32.1 and 32.2), 70 and 52 us at 256.  Where it is
+// farthest off, lists are taken for contexts of one length that just fill the machine:
+// 100 x 1,600 x 4 in 38 us for 32 (D = 64: 27 for 22).
 // Lists count their units in 31 bits; more take the clusters.
 int cluster_of(int segs, int cap, int fit) {
   const long long tiles = cap / kTile + 1, units = (tiles + kStart) * segs;
@@ -1141,7 +1146,7 @@ int launch(const TbDecodeAttnQuantArgs& a, cudaStream_t s) {
 
 // Query heads that a warp takes, in eights: two where more than 8 share a KV head,
 // which widens the pages once for both (64 x 1,000 tokens x 8 KV heads, 16 query heads
-// on each: 41 us against 49 with one; D = 64: 45 against 59), but in clusters one, for the
+// on each: 41 us against 50 with one; D = 64: 46 against 59), but in clusters one, for the
 // shorter way of a tile (1 x 2,000 tokens, 16 heads on 1: 9.2 us against 11.2), and for D =
 // 256 one, whose output fills the registers (64 x 1,000 x 4 KV heads, 16 on each: 59 against
 // 66, both before tiles were looked up 32 at a time; 49 now).

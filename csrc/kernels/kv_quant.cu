@@ -133,7 +133,7 @@ __device__ __forceinline__ void load_sector(const void* p, uint32_t (&w)[8]) {
 }
 
 // Rows as they come: a lane holds 32 neighbouring bytes of a row (with 16, 16,384
-// tokens x 2 KV heads x 128 in bf16 took 7.3 us for 6.0), and four heads of it are in
+// tokens x 2 KV heads x 128 in bf16 took 7.3 us for 5.7), and four heads of it are in
 // flight.  The four rows are reduced together (4 shuffles at D = 128 in 16 bits, 12
 // apart), and the two divisions of a row are done once per lane.  align: what rows
 // start on a multiple of, 32, 16 or fewer bytes.
@@ -402,7 +402,7 @@ bool rows_aligned(const void* p, long long st, long long sh, int dtype, int byte
 }
 
 // Warps that share the rounds of their tokens (few tokens: latency counts), as
-// many as fill 16 warps per SM (512 tokens of 16 rows: 3.7 us so, 4.6 with 8 or 32);
+// many as fill 16 warps per SM (512 tokens of 16 rows: 3.9 us so, 4.6 with 8 or 32);
 // in blocks of two warps, over more SMs, where there are few, else of four (ragged
 // batches: 1 us in 33 less than with eight).
 constexpr int kFewWarps = 148 * 16, kSpread = 148 * 8;

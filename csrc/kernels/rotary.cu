@@ -10,8 +10,8 @@
 // others in rows whose position is past the table).
 //
 // The kernel moves every element once in and once out and does 3 flops per
-// element, so memory bounds it: 16,383 rows x 40 heads x 128 in bf16 take 54 us on
-// one B200, 6.2 TB/s (95% of its copy rate).
+// element, so memory bounds it: 16,383 rows x 40 heads x 128 in bf16 take 53 us on
+// one B200, 6.3 TB/s (97% of its copy rate).
 #include <math.h>
 
 #include "device_common.cuh"
@@ -26,7 +26,7 @@ constexpr int blocks_of(int hu) { return hu == 4 ? 3 : 4; }
 
 // A thread holds one unit, two vectors of NP elements, of HU heads of a token
 // (every HS-th), so it reads its table entries once: read anew for each head they
-// are twice the bytes of a bf16 row, out of L1 (81 us with HU = 1, 58 with 4, 54
+// are twice the bytes of a bf16 row, out of L1 (88 us with HU = 1, 58 with 4, 53
 // with 8 at the size above).  Rotated units hold NP pairs (half layout: NP elements
 // of each half; interleaved: 2 NP neighbours), the others 2 NP copied elements.  All loads are issued before the first product.
 template <typename T, int NP, int HU, bool INTER>
@@ -113,10 +113,10 @@ bool fits(const TbRotaryArgs& a) {
 }
 
 // Heads per thread.  One where more would leave an SM (of 148) fewer than 1,024
-// threads (64 rows x 14 heads take 2.2 us so, mostly launch) or find no heads to hold
-// (100,000 rows x 1 head x 128: 15.4 us, with four 19.4).  Else four, and eight in
-// smaller blocks for 8 or more heads in vectors of 16 bytes: 54 against 58 us at the
-// size above, 40 against 44 for 60,000 rows x 8 heads x 128, but 23 against 21 for
+// threads (64 rows x 14 heads take 2.2 us so, mostly launch, with four 2.9) or find no
+// heads to hold (100,000 rows x 1 head x 128: 15.4 us, with four 20.4).  Else four, and
+// eight in smaller blocks for 8 or more heads in vectors of 16 bytes: 53 against 58 us
+// at the size above, 40 against 46 for 60,000 rows x 8 heads x 128, and 20 either way for
 // 16,000 rows x 16 heads x 80 (40 rotated), which are in vectors of 8 bytes.
 template <typename T, int NP, bool INTER>
 int launch_heads(const TbRotaryArgs& a, cudaStream_t s) {
