@@ -28,6 +28,7 @@ using namespace turbol;
 void register_kernel_ops(py::module_& ops);  // ops_bindings.cpp
 void register_llm_ops(py::module_& ops);      // llm_bindings.cpp
 void register_cache_ops(py::module_& ops);    // cache_bindings.cpp
+void register_vocab_ops(py::module_& ops);    // vocab_bindings.cpp
 void register_comm_ops(py::module_& ops);     // comm_bindings.cpp
 void register_dist(py::module_& m);           // dist_bindings.cpp
 
@@ -794,6 +795,7 @@ PYBIND11_MODULE(turbol_core, m) {
   register_kernel_ops(ops);
   register_llm_ops(ops);
   register_cache_ops(ops);
+  register_vocab_ops(ops);
   register_comm_ops(ops);
   py::module_ dist = m.def_submodule("dist", "C++ distributed runtime: NcclCommunicator, DistributedTrainer, "
                                                "PipelineTrainer (turbol/distributed.hpp)");
@@ -802,5 +804,6 @@ PYBIND11_MODULE(turbol_core, m) {
   py::module_ host_ops = m.def_submodule("host_ops", "operators that check their arguments here and leave CPU tensors "
                                                      "to plain math");
   register_cache_ops(host_ops);
+  register_vocab_ops(host_ops);
 #endif
 }

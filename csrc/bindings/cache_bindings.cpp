@@ -14,27 +14,13 @@
 #include <optional>
 
 #include "kernels.h"
+#include "op_checks.hpp"
 #include "turbol/common.hpp"
 
 namespace py = pybind11;
+using namespace turbol::checks;
 
 namespace {
-
-void chk(bool c, const char* op, const char* m) {
-  if (!c) throw std::invalid_argument(std::string(op) + ": " + m);
-}
-void cuda_ok(int e, const char* what) {
-  if (e != 0) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(static_cast<cudaError_t>(e)));
-}
-
-int type_of(const at::Tensor& t, const char* op) {
-  switch (t.scalar_type()) {
-    case at::kBFloat16: return TB_BF16;
-    case at::kHalf: return TB_F16;
-    case at::kFloat: return TB_F32;
-    default: throw std::invalid_argument(std::string(op) + ": bf16, fp16 or fp32 values");
-  }
-}
 
 // [T, H, D] rows with a contiguous last dimension.
 void rows3(const at::Tensor& t, const char* op, const char* m) {
@@ -42,50 +28,6 @@ void rows3(const at::Tensor& t, const char* op, const char* m) {
   chk(t.size(2) == 0 || t.size(1) <= INT_MAX / t.size(2), op, "at most 2^31 - 1 elements per row");
 }
 
-// Whether t carries a forward-mode tangent.
-bool is_dual(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
-
-// What has no derivative refuses tensors that would want one (forward mode has no
-// switch: torch.no_grad() leaves it on).
-void no_grad(std::initializer_list<const at::Tensor*> ts, const char* op, const char* what = nullptr) {
-  const bool on = at::GradMode::is_enabled();
-  for (const at::Tensor* t : ts)
-    if (is_dual(*t) || (on && t->requires_grad()))
-      throw std::invalid_argument(std::string(op) + ": " + (what ? std::string(what) + " " : std::string()) +
-                                  (is_dual(*t) ? "has no forward-mode derivative"
-                                               : "has no gradient (call it under torch.no_grad)"));
-}
-
-// Tells autograd that a kernel writes to `ts`, so that a backward pass that needs
-// what was there raises.
-void written(std::initializer_list<const at::Tensor*> ts) {
-  for (const at::Tensor* t : ts)
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
-}
-
-// Bytes [lo, hi) that a view touches (empty: lo == hi).
-struct Range {
-  uintptr_t lo, hi;
-};
-Range range_of(const at::Tensor& t) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-  const auto sizes = t.sizes(), strides = t.strides();
-  int64_t last = 0;
-  for (size_t i = 0; i < sizes.size(); ++i) {
-    if (sizes[i] == 0) return {p, p};
-    last += (sizes[i] - 1) * strides[i];
-  }
-  return {p, p + static_cast<uintptr_t>(last + 1) * t.element_size()};
-}
-bool apart(const Range& x, const Range& y) { return x.hi <= y.lo || y.hi <= x.lo || x.lo == x.hi || y.lo == y.hi; }
-bool apart(const at::Tensor& a, const at::Tensor& b) { return apart(range_of(a), range_of(b)); }
-// Whether `t` is apart from every one of `others`.
-template <size_t N>
-bool apart_from_all(const Range& t, const Range (&others)[N]) {
-  for (const Range& o : others)
-    if (!apart(t, o)) return false;
-  return true;
-}
 // Whether two [T, H, D] views share no element: disjoint ranges, or column
 // slices of rows with the same stride.
 bool columns_apart(const at::Tensor& a, const at::Tensor& b) {
@@ -111,21 +53,6 @@ bool rows_distinct(const at::Tensor& t) {
   }
   return s1 >= t.size(2) && s0 >= (n1 - 1) * s1 + t.size(2);
 }
-bool same_view(const at::Tensor& a, const at::Tensor& b) {
-  return a.data_ptr() == b.data_ptr() && a.strides() == b.strides() && a.sizes() == b.sizes();
-}
-
-void index1(const at::Tensor& t, int64_t n, const char* op, const char* m) {
-  chk(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), op, m);
-}
-
-int* error_of(const std::optional<at::Tensor>& e, const at::Device& dev, const char* op) {
-  if (!e) return nullptr;
-  chk(e->scalar_type() == at::kInt && e->numel() >= 1 && e->is_contiguous() && e->device() == dev, op,
-      "error is an int32 tensor on the same device");
-  return e->data_ptr<int>();
-}
-
 // The table's dimensions: R / 2 pairs for max_pos positions.
 void table_of(const at::Tensor& t, int64_t D, const char* op) {
   chk(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(2) == 2 && t.is_contiguous() && t.size(0) >= 1 &&
@@ -134,8 +61,6 @@ void table_of(const at::Tensor& t, int64_t D, const char* op) {
   chk(reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0, op, "table is 8-byte aligned");
   no_grad({&t}, op, "the table");
 }
-
-using Opt = std::optional<at::Tensor>;
 
 Opt rotary(const at::Tensor& x, const at::Tensor& pos, const at::Tensor& table, const Opt& out_, bool interleaved,
            bool transpose, const Opt& error) {

@@ -82,4 +82,14 @@ int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s)
   return static_cast<int>(cudaErrorNoDevice);
 }
 
+int tb_topk_logprobs(const TbTopkLogprobsArgs* args, cudaStream_t s) { return static_cast<int>(cudaErrorNoDevice); }
+
+int tb_distill(const TbDistillArgs* args, cudaStream_t s) { return static_cast<int>(cudaErrorNoDevice); }
+
+int tb_embedding(const TbEmbeddingArgs* args, cudaStream_t s) { return static_cast<int>(cudaErrorNoDevice); }
+
+size_t tb_embedding_grad_ws_bytes(int N, int H, int V) { return 0; }
+
+int tb_embedding_grad(const TbEmbeddingGradArgs* args, cudaStream_t s) { return static_cast<int>(cudaErrorNoDevice); }
+
 }  // extern "C"

@@ -428,6 +428,82 @@ typedef struct {
 size_t tb_decode_attention_quant_ws_bytes(int B, int Hq, int Hk, int D, int max_tokens);
 int tb_decode_attention_quant(const TbDecodeAttnQuantArgs* args, cudaStream_t s);
 
+// ---------------- distillation (topk_logprobs.cu, distill.cu) ----------------
+// The k largest of each row of logits [R, V] (ties: the lowest index first; NaN
+// ranks as -inf) as log-probabilities log_softmax(z / temperature), and the rows'
+// log-sum-exps.  1 <= k <= 256, k <= V <= 2^20, any row stride.  Rows without a
+// logit above -inf: all -inf.
+typedef struct {
+  const void* logits;
+  long long ld;
+  int R, V, k;
+  int dtype;  // TB_BF16 / TB_F16 / TB_F32
+  double temperature;
+  float* logp;  // [R, k]
+  int* ids;     // [R, k]
+  float* lse;   // [R]
+} TbTopkLogprobsArgs;
+int tb_topk_logprobs(const TbTopkLogprobsArgs* args, cudaStream_t s);
+
+// Per row of logits [R, V]: weight * KL to a teacher's list of K ids and
+// log-probabilities, plus target_weight * -log p[target], and its gradient.
+enum { TB_DISTILL_FORWARD = 0, TB_DISTILL_FORWARD_REST = 1, TB_DISTILL_REVERSE = 2 };
+enum { TB_DISTILL_STATS = 8 };  // floats kept of a row for a backward pass of its own
+typedef struct {
+  const void* logits;
+  long long ld;
+  void* grad;  // [R, V], logits' type, may be logits itself; NULL: the loss alone
+  long long ld_grad;
+  const int* ids;      // [R, K], 1 <= K <= 256
+  const float* logp;   // [R, K]
+  const float* weight;         // [R], NULL: ones
+  const int* target;           // [R], NULL: none; negative: none in this row
+  const float* target_weight;  // [R], NULL: ones
+  float* loss;         // [R]; NULL: a backward pass from `stats`
+  float* stats;        // [R, TB_DISTILL_STATS]: written with the loss (may be NULL then), or read
+  const float* dloss;  // [R]: the loss's gradient in a backward pass
+  int R, V, K;
+  int dtype, kind;
+  double temperature;
+  int* err;
+} TbDistillArgs;
+int tb_distill(const TbDistillArgs* args, cudaStream_t s);
+
+// ---------------- embedding (embedding.cu) ----------------
+// out[t] = scale * weight[ids[t]] (one rounding; negative ids: zeros; ids past V:
+// NaN and *err = 1).
+typedef struct {
+  const void* ids;  // int32 or int64
+  int ids64;
+  const void* weight;
+  long long ld_w;
+  void* out;
+  long long ld_out;
+  int N, H, V;
+  int dtype;
+  float scale;
+  int* err;
+} TbEmbeddingArgs;
+int tb_embedding(const TbEmbeddingArgs* args, cudaStream_t s);
+// grad[v] += scale * sum of the rows dy[t] with ids[t] == v, in token order (zero: =,
+// and zeros where no id is v).  The sums are fp32, rounded once.
+typedef struct {
+  const void* ids;
+  int ids64;
+  const void* dy;
+  long long ld_dy;
+  void* grad;
+  long long ld_grad;
+  int N, H, V;
+  int dtype, grad_dtype;  // of dy, of grad
+  float scale;
+  int zero;
+  int* err;
+  void* ws;
+} TbEmbeddingGradArgs;
+size_t tb_embedding_grad_ws_bytes(int N, int H, int V);
+int tb_embedding_grad(const TbEmbeddingGradArgs* args, cudaStream_t s);
+
 // ---------------- NVLink peer-memory collectives ----------------
 #define TB_MAX_PEERS 8
 typedef struct {

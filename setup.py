@@ -74,7 +74,7 @@ CPU_ONLY = os.environ.get("TURBOL_CPU_ONLY", "") not in ("", "0")
 
 def cpu_sources():
     pats = ["csrc/core/*.cpp", "csrc/engines/*.cpp", "csrc/bindings/bindings.cpp", "csrc/bindings/cache_bindings.cpp",
-            "csrc/cpu_only/*.cpp"]
+            "csrc/bindings/vocab_bindings.cpp", "csrc/cpu_only/*.cpp"]
     out = []
     for p in pats:
         out += sorted(glob.glob(os.path.join(ROOT, p)))

@@ -289,3 +289,109 @@ def decode_attention_quant(q, kc, vc, ks, vs, block_table, ctx_len, scale, out=N
         return y
     out.copy_(y)
     return out
+
+
+# ------------------------------------------------------------------ distillation
+def topk_logprobs(logits, k, temperature=1.0, dtype=torch.float32):
+    """(log-probabilities, ids int32, log-sum-exps) of each row's k largest logits; the numbers in ``dtype``."""
+    z = logits.double()
+    # NaN ranks as -inf, equal values (+-0 too) by the lowest id
+    key = torch.where(z.isnan(), torch.full_like(z, -math.inf), z) + 0.0
+    ids = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :k]
+    lse = torch.logsumexp(z / temperature, 1)
+    top = key.amax(1, keepdim=True)
+    top = torch.where(top.isinf(), 0.0, top)  # (differences first: next to the type's lowest value lse loses log V)
+    logp = (z.gather(1, ids) - top) / temperature - torch.logsumexp((z - top) / temperature, 1, keepdim=True)
+    logp = torch.where(lse[:, None].isneginf(), lse[:, None], logp)
+    logp = torch.where(lse[:, None].isnan(), lse[:, None], logp)
+    return logp.to(dtype), ids.to(torch.int32), lse.to(dtype)
+
+
+DISTILL_REST_MIN = 2.0 ** -20
+
+
+def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, temperature=1.0, target=None,
+            target_weight=None, error=None, dtype=None):
+    """(loss fp32 [R], gradient in ``dtype``, default logits') of the distillation loss, computed in 64 bits."""
+    R, V = logits.shape
+    f64 = dict(dtype=torch.float64, device=logits.device)
+    w = torch.ones(R, **f64) if weight is None else weight.double()
+    c = torch.zeros(R, **f64) if target is None else torch.ones(R, **f64) if target_weight is None else \
+        target_weight.double()
+    y = torch.full((R,), -1, device=logits.device) if target is None else target.long()
+    live = (w != 0) | ((c != 0) & (y >= 0))
+    bad = ((ids >= V) & ~logprobs.isneginf() & (w != 0)[:, None]).any() | ((y >= V) & live).any()
+    if error is not None and bool(bad):
+        error[0] = 1
+    c = torch.where((y >= 0) & (y < V), c, 0.0)
+    live = (w != 0) | (c != 0)
+    y = y.clamp(0, V - 1)[:, None]
+    z = torch.where(live[:, None], logits.double() / temperature, 0.0)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    lse = torch.where(lse.isinf(), math.nan, lse)
+    logp = z - lse
+    p = logp.exp()
+    here = (ids >= 0) & (ids < V) & ~logprobs.isneginf()
+    at = torch.where(here, ids.long(), V)  # (what is left out: a column behind the last)
+    mass = torch.where(here, logprobs.double().exp(), 0.0)
+    t = torch.zeros(R, V + 1, **f64).scatter_add_(1, at, mass)[:, :V]
+    inside = torch.zeros(R, V + 1, dtype=torch.bool, device=logits.device).scatter_(1, at, True)[:, :V]
+    total = mass.sum(1, keepdim=True)
+
+    def plogq(a, b, on):  # a (log a - log b) where it counts
+        return torch.where(on & (a > 0), a * (a.log() - b), 0.0).sum(1, keepdim=True) + \
+            torch.where(on & a.isnan(), a, 0.0).sum(1, keepdim=True)
+
+    if not rest:
+        t = torch.where(total != 0, t / total, 0.0)
+        kl = plogq(t, logp, inside)
+        d = torch.where(total != 0, p - t, 0.0)
+    else:
+        lr = torch.logsumexp(torch.where(inside, -math.inf, logp), 1, keepdim=True)
+        pr, empty = lr.exp(), lr.isneginf()
+        q = torch.where(empty | inside, 0.0, (logp - lr).exp())
+        if kind == "forward":
+            tr = (1 - total).clamp_min(0)
+            kl = plogq(t, logp, inside) + torch.where(empty | (tr == 0), 0.0, tr * (tr.clamp_min(1e-300).log() - lr))
+            a = total + torch.where(empty, 0.0, tr)  # 1, but for a student without mass outside (or a list with more than 1)
+            d = torch.where(inside, a * p - t, (a * pr - tr) * q)
+        else:
+            f = torch.where(inside & (p > 0), logp - t.clamp_min(1e-300).log(), 0.0)
+            fr = torch.where(empty, 0.0, lr - (1 - total).clamp_min(DISTILL_REST_MIN).log())
+            kl = (p * f).sum(1, keepdim=True) + pr * fr
+            d = torch.where(inside, p * (f - kl), pr * q * (fr - kl))
+    on, c = (w != 0)[:, None], c[:, None]
+    loss = torch.where(on, w[:, None] * kl, 0.0) + torch.where(c != 0, -c * logp.gather(1, y), 0.0)
+    d = torch.where(on, w[:, None] * d, 0.0) + torch.where(c != 0, c * p, 0.0)
+    d.scatter_add_(1, y, -c)
+    return loss.squeeze(1).float(), (d / temperature).to(logits.dtype if dtype is None else dtype)
+
+
+# ------------------------------------------------------------------ embedding
+def embedding(ids, weight, scale=1.0, out=None, error=None):
+    """scale * weight[ids], padding (negative ids) zero, ids past the table NaN."""
+    i = ids.long()
+    bad = i >= weight.shape[0]
+    if error is not None and bool(bad.any()):
+        error[0] = 1
+    y = weight[i.clamp(0, weight.shape[0] - 1)].double() * scale
+    y = y.masked_fill((i < 0)[..., None], 0.0).masked_fill(bad[..., None], math.nan).to(weight.dtype)
+    if out is None:
+        return y
+    out.copy_(y)
+    return out
+
+
+def embedding_grad(ids, dy, grad, scale=1.0, accumulate=True, error=None):
+    """grad[v] (+)= scale * sum of dy over the tokens v, summed in fp32 in token order."""
+    i = ids.reshape(-1).long()
+    if error is not None and bool((i >= grad.shape[0]).any()):
+        error[0] = 1
+    t = torch.nonzero((i >= 0) & (i < grad.shape[0])).squeeze(1)
+    rows, at = torch.unique(i[t], return_inverse=True)
+    s = torch.zeros(rows.numel(), grad.shape[1], device=grad.device)
+    s.index_add_(0, at, dy.reshape(i.numel(), grad.shape[1])[t].float())
+    if not accumulate:
+        grad.zero_()
+    grad[rows] = (grad[rows].float() + s * scale).to(grad.dtype)
+    return grad
