@@ -54,6 +54,10 @@ def parse_args(argv=None):
     p.add_argument("--clip", type=float, default=0.2)
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--kv-dtype", choices=["bf16", "fp8"], default="bf16", help="KV cache of the rollout")
+    p.add_argument("--distill-coef", type=float, default=0.0,
+                   help="weight of the distillation loss on the frozen reference's most likely tokens")
+    p.add_argument("--distill-topk", type=int, default=64)
+    p.add_argument("--distill-kind", choices=["forward", "reverse"], default="forward")
     p.add_argument("--dp", choices=["fused", "nccl"], default="fused",
                    help="data-parallel gradient reduction when launched on several GPUs (torchrun)")
     p.add_argument("--tp", type=int, default=1, help="tensor-parallel group size (rollout and training)")
@@ -74,7 +78,8 @@ def main(argv=None):
     cfg = GRPOConfig(model=model, num_prompts=args.num_prompts, group_size=args.group_size,
                      prompt_len=args.prompt_len, response_len=args.max_tokens, temperature=args.temperature,
                      lr=args.lr, clip=args.clip, kl_coef=args.kl_coef, micro_batch=args.micro_batch, seed=args.seed,
-                     kv_dtype=args.kv_dtype)
+                     kv_dtype=args.kv_dtype, distill_coef=args.distill_coef, distill_topk=args.distill_topk,
+                     distill_kind=args.distill_kind)
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = 0
     if world > 1:  # launched by torchrun: one process per GPU, TP groups of --tp ranks, DP over the rest
@@ -108,6 +113,8 @@ def main(argv=None):
                    "grpo/pg_loss": st["pg_loss"], "grpo/kl": st["kl"], "grpo/kl_coef": cfg.kl_coef,
                    "grpo/gen_ms": st["rollout_s"] * 1e3, "grpo/reward_ms": st["reward_ref_s"] * 1e3,
                    "grpo/policy_ms": st["train_s"] * 1e3, "grpo/train_tokens_per_s": tok_s}
+        if "distill_kl" in st:
+            scalars["grpo/distill_kl"] = st["distill_kl"]
         for k, v in scalars.items():
             tb.add_scalar(k, float(v), step + 1)
         if (step + 1) % args.print_every == 0 or step + 1 == args.num_steps:

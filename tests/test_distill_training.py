@@ -1,0 +1,145 @@
+"""The distillation and the scaled embedding where the framework uses them: GRPO with a
+teacher, the decoder's embedding in training and in the rollout."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+from turbol_b200.models.llm import DecoderLM, LMConfig
+from turbol_b200.ops import reference as ref
+from turbol_b200.rl.grpo import GRPOConfig, GRPOTrainer
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+
+
+def tiny(**kw):
+    cfg = LMConfig.tiny()
+    for k, v in kw.items():
+        setattr(cfg, k, v)
+    return cfg
+
+
+def config(**kw):
+    return GRPOConfig(**{**dict(model=tiny(), num_prompts=2, group_size=4, prompt_len=20, response_len=12, micro_batch=4), **kw})
+
+
+def test_refusals():
+    for kw in (dict(distill_coef=0.1, distill_kind="both"), dict(distill_coef=0.1, distill_topk=0),
+               dict(distill_coef=0.1, distill_topk=257), dict(distill_coef=-1.0), dict(distill_coef=math.nan)):
+        with pytest.raises(ValueError, match="distill"):
+            GRPOTrainer(config(**kw), "cpu")
+    with pytest.raises(ValueError, match="tensor parallelism"):
+        GRPOTrainer(config(distill_coef=0.1), "cpu", tp=2)
+    teacher = DecoderLM(tiny(), "cpu", master=False)
+    with pytest.raises(ValueError, match="needs distill_coef"):
+        GRPOTrainer(config(), "cpu", teacher=teacher)
+    for t in (DecoderLM(tiny(vocab=1000), "cpu", master=False), DecoderLM(tiny(max_seq=16), "cpu", master=False)):
+        with pytest.raises(ValueError, match="teacher"):
+            GRPOTrainer(config(distill_coef=0.1), "cpu", teacher=t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["forward", "reverse"])
+@pytest.mark.parametrize("tie", [True, False])
+def test_gradient_of_the_training_loss(kind, tie, dev):
+    """The micro-batched update's gradient (policy loss, KL penalty, distillation; scaled embedding) against autograd on
+    the fp32 model."""
+    cfg = config(model=tiny(embed_scale=4.0, tie_embeddings=tie), distill_coef=0.7, distill_topk=24, distill_kind=kind, kl_coef=0.1)
+    tr = GRPOTrainer(cfg, dev, teacher=DecoderLM(tiny(tie_embeddings=tie), dev, seed=11, master=False))
+    g = torch.Generator(device=dev).manual_seed(2)
+    seqs = torch.randint(0, cfg.model.vocab, (cfg.batch, cfg.seq_len), generator=g, device=dev, dtype=torch.int32)
+    adv = torch.randn(cfg.batch, generator=g, device=dev)
+    lists = tr._teacher_lists(cfg.batch)
+    tr._score(tr.teacher, seqs, lists=lists)
+    ref_lp = tr.ref_logprobs(seqs) + 0.1 * torch.randn(cfg.batch, cfg.response_len, generator=g, device=dev)
+    tr.model.zero_grad()
+    tr.stats.zero_()
+    tr._train(seqs, ref_lp, adv, lists)
+    m = tr.model
+    leaves = {n: (m.p[n] if n.endswith(("ln1", "ln2", "norm", "bqkv")) else m.s[n].float()).clone().requires_grad_()
+              for n in m.offsets}
+    Lp, B, L = cfg.prompt_len, cfg.batch, cfg.response_len
+    logits = ref.lm_forward_ref(m, seqs, leaves)[:, Lp - 1:-1]
+    lsm = torch.log_softmax(logits, -1)
+    lp = lsm.gather(2, seqs[:, Lp:].long()[..., None]).squeeze(2)
+    pg = -(torch.exp(lp - lp.detach()) * adv[:, None])
+    k3 = torch.exp(ref_lp - lp) - (ref_lp - lp) - 1
+    ids, l = lists[0].long(), lists[1]
+    top = lsm.gather(2, ids)
+    inside = torch.zeros_like(lsm, dtype=torch.bool).scatter_(2, ids, True)
+    rest = torch.logsumexp(lsm.masked_fill(inside, -math.inf), -1)
+    t_rest = 1 - l.double().exp().sum(-1).float()
+    if kind == "forward":
+        kl = (l.exp() * (l - top)).sum(-1) + t_rest * (t_rest.log() - rest)
+    else:
+        kl = (top.exp() * (top - l)).sum(-1) + rest.exp() * (rest - t_rest.log())
+    (pg + cfg.kl_coef * k3 + cfg.distill_coef * kl).mean().backward()
+    mean = float(kl.detach().mean())
+    assert abs(float(tr.distill_kl) - mean) <= 0.03 * mean
+    for n in m.offsets:
+        e = leaves[n].grad
+        assert (m.g[n] - e).norm() / e.norm() < 5e-2, n
+
+
+@pytest.mark.gpu
+def test_steps(dev):
+    """The frozen reference as teacher: no distance in the first step; another teacher: some; the same seeds, the same
+    gradients of the embedding."""
+    tr = GRPOTrainer(config(distill_coef=0.1, distill_topk=16), dev)
+    assert tr.teacher is tr.ref
+    st = [tr.step() for _ in range(2)]
+    assert abs(st[0]["distill_kl"]) < 1e-4 and all(math.isfinite(s["distill_kl"]) for s in st)
+    tr = GRPOTrainer(config(distill_coef=0.1, distill_kind="reverse"), dev, teacher=DecoderLM(tiny(), dev, seed=5, master=False))
+    st = tr.step()
+    assert math.isfinite(st["pg_loss"]) and st["distill_kl"] > 1e-3
+    assert "distill_kl" not in GRPOTrainer(config(), dev).step()
+
+
+@pytest.mark.gpu
+def test_scaled_embedding_in_the_rollout(dev):
+    """Greedy tokens of a model with scaled embeddings are those of its fp32 forward (up to its bf16 rounding)."""
+    from turbol_b200.rl.rollout import LLMGenerator
+
+    m = DecoderLM(tiny(embed_scale=16.0), dev, seed=3)
+    prompts = torch.randint(0, m.cfg.vocab, (2, 21), device=dev, dtype=torch.int32)
+    for graph in (True, False):
+        seqs, lp = LLMGenerator(m, 4, 64, cuda_graph=graph).generate(prompts, 2, 10, temperature=0.0)
+        lg = ref.lm_forward_ref(m, seqs)[:, 20:-1]
+        picked = lg.gather(2, seqs[:, 21:].long()[..., None]).squeeze(2)
+        spread = lg.amax(-1) - lg.mean(-1)
+        assert ((lg.amax(-1) - picked) <= 0.2 * spread).all()
+    x, plain = m.embed(prompts), m.s["embed"][prompts.reshape(-1).long()]
+    assert torch.equal(x, plain * 16)
+
+
+@pytest.mark.gpu
+def test_embedding_gradient_is_reproducible(dev):
+    """Many tokens of few kinds: the same bits every time, and the sums of the older kernel within rounding."""
+    from turbol_b200._native import ops
+
+    m = DecoderLM(tiny(), dev)
+    ids = torch.randint(0, 9, (8, 300), device=dev, dtype=torch.int32)
+    dx = torch.randn(2400, m.cfg.hidden, device=dev).bfloat16()
+    got = []
+    for _ in range(3):
+        m.zero_grad()
+        m.embed_backward(ids, dx)
+        got.append(m.g["embed"].clone())
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    old = torch.zeros_like(got[0])
+    ops().embed_bwd(ids.reshape(-1), dx, old)
+    # two fp32 sums of some 270 terms each in different orders
+    mag = torch.zeros_like(old).index_add_(0, ids.reshape(-1).long(), dx.float().abs())
+    assert ((old - got[0]).abs() <= 2 * 400 * 2.0 ** -24 * mag).all()
+
+
+@pytest.mark.gpu
+def test_example(tmp_path, dev):
+    import grpo_example
+
+    tr = grpo_example.main(["--num-prompts", "2", "--group-size", "4", "--prompt-len", "16", "--max-tokens", "16",
+                            "--num-steps", "2", "--print-every", "1", "--micro-batch", "4", "--distill-coef", "0.2",
+                            "--distill-topk", "20", "--distill-kind", "reverse", "--log-dir", str(tmp_path)])
+    assert tr.step_count == 2 and math.isfinite(float(tr.distill_kl))

@@ -31,6 +31,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .._native import ops as _ops
+from ..ops.embedding import embedding, embedding_grad
 from ..ops.rotary import rotary, rotary_table
 
 ALIGN = 64  # elements; every parameter offset is 128-byte aligned in bf16
@@ -58,6 +59,7 @@ class LMConfig:
     rotary_dim: Optional[int] = None
     rope_interleaved: bool = False
     rope_scaling: Optional[dict] = None
+    embed_scale: float = 1.0  # factor on the embedding's rows as they enter the first layer (not on a tied head)
 
     @property
     def rope_default(self) -> bool:
@@ -119,6 +121,14 @@ def apply_rope(cfg: LMConfig, table: torch.Tensor, qkv: torch.Tensor, pos: torch
     else:
         x = qkv[:, : heads * D].unflatten(1, (heads, D))
         rotary(x, pos, table, cfg.rope_interleaved, inverse, out=x)
+
+
+def embed_into(cfg: LMConfig, ids: torch.Tensor, weight: torch.Tensor, out: torch.Tensor):
+    """Writes the (scaled) embedding rows of the int32 ids [N] to out [N, hidden]."""
+    if cfg.embed_scale == 1.0:
+        _ops().embed_fwd(ids, weight, out)
+    else:
+        embedding(ids, weight, cfg.embed_scale, out=out)
 
 
 class DecoderLM:
@@ -243,7 +253,7 @@ class DecoderLM:
     def embed(self, ids: torch.Tensor) -> torch.Tensor:
         N = ids.numel()
         x = torch.empty(N, self.cfg.hidden, device=self.device, dtype=torch.bfloat16)
-        _ops().embed_fwd(ids.reshape(-1).to(torch.int32).contiguous(), self.s["embed"], x)
+        embed_into(self.cfg, ids.reshape(-1).to(torch.int32).contiguous(), self.s["embed"], x)
         return x
 
     def forward(self, x: torch.Tensor, B: int, T: int, pos: torch.Tensor, save: bool = False, kv_hook=None):
@@ -363,7 +373,7 @@ class DecoderLM:
         return dx
 
     def embed_backward(self, ids: torch.Tensor, dx: torch.Tensor):
-        _ops().embed_bwd(ids.reshape(-1).to(torch.int32).contiguous(), dx, self.g["embed"])
+        embedding_grad(ids.reshape(-1).to(torch.int32).contiguous(), dx, self.g["embed"], self.cfg.embed_scale)
 
     # ------------------------------------------------------------------ utilities
     def zero_grad(self):

@@ -53,6 +53,7 @@ from typing import Optional
 import torch
 
 from .._native import ops as _ops
+from ..ops.embedding import embedding_grad
 from .llm import ALIGN, DecoderLM, apply_rope
 
 
@@ -504,7 +505,7 @@ class TPTrainLM(TPDecoderLM):
         """Embedding gradient of this rank's rows (partial; summed over the group
         by :meth:`reduce_replicated_grads`)."""
         r0, m = self.rows_of(ids_flat.numel())
-        _ops().embed_bwd(ids_flat[r0:r0 + m].to(torch.int32).contiguous(), dx, self.g["embed"])
+        embedding_grad(ids_flat[r0:r0 + m].to(torch.int32).contiguous(), dx, self.g["embed"], self.cfg.embed_scale)
 
     def state_dict(self):
         return {"cfg": self.cfg.__dict__, "layers": self.layers, "tp": self.tp, "rank": self.rank,

@@ -153,7 +153,7 @@ def lm_forward_ref(model, ids, params=None):
                 P[n] = model.p[n].float()
     B, T = ids.shape
     H, D, F = cfg.hidden, cfg.head_dim, cfg.ffn
-    x = P["embed"][ids.long()]
+    x = P["embed"][ids.long()] * cfg.embed_scale
     pos = torch.arange(T, device=ids.device)
     for i in model.layers:
         p = f"l{i}."

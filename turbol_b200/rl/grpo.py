@@ -16,6 +16,13 @@ One step:
 With one update per rollout the behaviour policy equals the current policy,
 so the ratio is 1 and the clip is inactive (the GRPO setting with mu = 1).
 
+On-policy distillation (``distill_coef`` > 0): a teacher (the frozen reference,
+or a given model) lists its ``distill_topk`` most likely tokens at every response
+position, and the loss gets distill_coef x the mean KL between its distribution and
+the policy's over the list and the rest (``distill_kind``: "forward" KL(teacher ||
+policy) or "reverse").  Its gradient and the policy gradient's are written in one
+pass over the logits.
+
 Train tokens per step = P * G * (prompt_len + response_len).
 
 The reference's grpo_example.py (turbol_vllm/examples/py/grpo_example.py:124-151)
@@ -26,11 +33,13 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass, field
+from typing import Optional
 
 import torch
 
 from .._native import ops as _ops
 from ..models.llm import DecoderLM, LMConfig
+from ..ops.distill import distill_loss_grad, topk_logprobs
 from ..ops.rl import FusedAdam
 from .rollout import LLMGenerator
 
@@ -49,6 +58,9 @@ class GRPOConfig:
     micro_batch: int = 8  # sequences per forward/backward
     seed: int = 0
     kv_dtype: str = "bf16"  # rollout KV cache: "bf16" or "fp8" (not with a tensor-parallel decode)
+    distill_coef: float = 0.0  # weight of the distillation loss (0: none; not with tensor parallelism)
+    distill_topk: int = 64
+    distill_kind: str = "forward"  # "forward" or "reverse"
 
     @property
     def batch(self) -> int:
@@ -84,8 +96,10 @@ class GRPOTrainer:
       rank re-slices its rollout shard from the updated weights."""
 
     def __init__(self, cfg: GRPOConfig, device="cuda:0", optimizer=None, dp: str = "none", group=None,
-                 tp: int = 1, tp_mode: str = "train", rollout: str = "replica"):
-        """rollout (tp_mode "train"): "replica" - each rank decodes its share of
+                 tp: int = 1, tp_mode: str = "train", rollout: str = "replica", teacher: Optional[DecoderLM] = None):
+        """teacher: the model that ``cfg.distill_coef`` pulls towards (default: the frozen
+        reference), with the policy's vocabulary, on the same device.
+        rollout (tp_mode "train"): "replica" - each rank decodes its share of
         the group's sequences on a full bf16 copy of the model that a fused
         all-gather kernel refreshes after every optimizer step
         (:class:`~turbol_b200.parallel.weight_sync.TPReplicaSync`); "tp" - the
@@ -99,6 +113,22 @@ class GRPOTrainer:
             raise ValueError(f"kv_dtype: 'bf16' or 'fp8', not {cfg.kv_dtype!r}")
         if cfg.kv_dtype != "bf16" and tp > 1 and self.rollout_mode != "replica":
             raise ValueError("kv_dtype 'fp8' needs a rollout on whole models (tp=1, or rollout='replica')")
+        if cfg.distill_coef:
+            if not 0 < cfg.distill_coef < float("inf"):
+                raise ValueError(f"distill_coef: a finite weight of at least 0, not {cfg.distill_coef}")
+            if tp > 1:
+                raise ValueError("distill_coef: not with tensor parallelism")
+            if cfg.distill_kind not in ("forward", "reverse"):
+                raise ValueError(f"distill_kind: 'forward' or 'reverse', not {cfg.distill_kind!r}")
+            if not 1 <= cfg.distill_topk <= min(256, cfg.model.vocab):
+                raise ValueError(f"distill_topk: 1 to 256 and to the vocabulary, not {cfg.distill_topk}")
+        if teacher is not None:
+            if not cfg.distill_coef:
+                raise ValueError("a teacher needs distill_coef")
+            if teacher.cfg.vocab != cfg.model.vocab or teacher.device != torch.device(device):
+                raise ValueError("the teacher has the policy's vocabulary and device")
+            if teacher.cfg.max_seq < cfg.seq_len:
+                raise ValueError("the teacher's positions do not cover the sequences")
         self.sync = None
         self.device = torch.device(device)
         self.dp, self.group = dp, group
@@ -136,6 +166,7 @@ class GRPOTrainer:
             elif dp != "none":
                 raise ValueError(f"unknown data-parallel mode {dp!r}")
         self.ref = self.model.frozen_copy()
+        self.teacher = teacher if teacher is not None else self.ref
         if tp > 1:
             from ..models.tp_llm import TPDecoderLM
             from ..parallel.dist import build_mesh
@@ -291,25 +322,38 @@ class GRPOTrainer:
         return (base[:, None] + torch.arange(Lp - 1, Lp - 1 + Lr, device=self.device)[None, :]).reshape(-1)
 
     @torch.no_grad()
-    def ref_logprobs(self, seqs: torch.Tensor) -> torch.Tensor:
-        """Log-probs of the response tokens under the frozen reference model."""
+    def ref_logprobs(self, seqs: torch.Tensor, lists=None) -> torch.Tensor:
+        """Log-probs of the response tokens under the frozen reference model (and its lists, as in _score)."""
+        out = torch.empty(seqs.shape[0], self.cfg.response_len, device=self.device)
+        self._score(self.ref, seqs, out, lists)
+        return out
+
+    def _score(self, model: DecoderLM, seqs: torch.Tensor, out=None, lists=None):
+        """A frozen model's view of the response tokens: their log-probs into ``out`` [B, Lr], and its most likely
+        tokens into ``lists`` (ids int32 and log-probs fp32 [B, Lr, K])."""
         cfg = self.cfg
-        o = _ops()
-        B, T, Lr = seqs.shape[0], cfg.seq_len, cfg.response_len
-        out = torch.empty(B, Lr, device=self.device)
+        T = cfg.seq_len
         mb = cfg.micro_batch
         pos = torch.arange(T, device=self.device, dtype=torch.int32).repeat(mb)
-        for s0 in range(0, B, mb):
+        for s0 in range(0, seqs.shape[0], mb):
             ids = seqs[s0:s0 + mb].contiguous()
             m = ids.shape[0]
-            x = self.ref.embed(ids)
-            x, _ = self.ref.forward(x, m, T, pos[: m * T], save=False)
-            hf = self.ref.final_norm(x)
+            x = model.embed(ids)
+            x, _ = model.forward(x, m, T, pos[: m * T], save=False)
+            hf = model.final_norm(x)
             rows = hf.index_select(0, self._response_rows(m))
-            logits = self.ref.logits(rows)
-            tgt = ids[:, cfg.prompt_len:].reshape(-1).contiguous()
-            o.logprob(logits, tgt, out[s0:s0 + m].view(-1))
-        return out
+            logits = model.logits(rows)
+            if out is not None:
+                tgt = ids[:, cfg.prompt_len:].reshape(-1).contiguous()
+                _ops().logprob(logits, tgt, out[s0:s0 + m].view(-1))
+            if lists is not None:
+                top = topk_logprobs(logits, lists[0].shape[2])
+                lists[0][s0:s0 + m] = top.ids.view(m, -1, top.ids.shape[1])
+                lists[1][s0:s0 + m] = top.logprobs.view(m, -1, top.ids.shape[1])
+
+    def _teacher_lists(self, n: int):
+        shape = (n, self.cfg.response_len, self.cfg.distill_topk)
+        return (torch.empty(shape, device=self.device, dtype=torch.int32), torch.empty(shape, device=self.device))
 
     # ------------------------------------------------------------------ step
     def step(self) -> dict:
@@ -342,7 +386,10 @@ class GRPOTrainer:
             ref_lp = (self.ref_logprobs(seqs.index_select(0, own).contiguous()) if self.rollout_mode == "replica"
                       else self._tp_ref_logprobs(seqs))
         else:
-            ref_lp = self.ref_logprobs(seqs)
+            lists = self._teacher_lists(seqs.shape[0]) if cfg.distill_coef else None
+            ref_lp = self.ref_logprobs(seqs, lists if self.teacher is self.ref else None)
+            if lists is not None and self.teacher is not self.ref:
+                self._score(self.teacher, seqs, lists=lists)
         torch.cuda.synchronize(dev)
         t2 = time.perf_counter()
         # 4. update
@@ -355,7 +402,7 @@ class GRPOTrainer:
 
             dist.all_reduce(self.stats, group=self.mesh.tp_group)
         else:
-            self._train(seqs, ref_lp, adv)
+            self._train(seqs, ref_lp, adv, lists)
         if self.grad_sync is not None:
             self.opt.step(grad_scale=self.grad_sync(self.model.grad))
         else:
@@ -370,12 +417,13 @@ class GRPOTrainer:
         self.step_count += 1
         st = self.stats.cpu().tolist()
         self.last_times = {"rollout_s": t1 - t0, "reward_ref_s": t2 - t1, "train_s": t3 - t2, "step_s": t3 - t0}
-        return {"reward_mean": float(rewards.mean()), "reward_std": float(rewards.std()),
+        extra = {"distill_kl": float(self.distill_kl)} if cfg.distill_coef else {}
+        return {**extra, "reward_mean": float(rewards.mean()), "reward_std": float(rewards.std()),
                 "pg_loss": st[0], "kl": st[1], "clipped_tokens": st[2], "tokens": st[3],
                 "rollout_logp_mean": float(roll_lp.mean()), **self.last_times,
                 "train_tokens": train_tokens}
 
-    def _train(self, seqs, ref_lp, adv):
+    def _train(self, seqs, ref_lp, adv, lists=None):
         cfg = self.cfg
         o = _ops()
         m_ = self.model
@@ -385,6 +433,9 @@ class GRPOTrainer:
         pos = torch.arange(T, device=self.device, dtype=torch.int32).repeat(mb)
         mask = torch.ones(mb, Lr, device=self.device)
         nb = seqs.shape[0]
+        if lists is not None:  # per token: coefficient / (sequences x response tokens), as the policy loss's mean
+            weight = torch.full((mb * Lr,), cfg.distill_coef / (nb * Lr), device=self.device)
+            self.distill_kl = torch.zeros((), device=self.device)
         for s0 in range(0, nb, mb):
             ids = seqs[s0:s0 + mb].contiguous()
             m = ids.shape[0]
@@ -403,7 +454,13 @@ class GRPOTrainer:
             dlp = torch.empty_like(lp)
             o.grpo_loss(lp.view(m, Lr), old.view(m, Lr), ref_lp[s0:s0 + m].contiguous(), adv[s0:s0 + m].contiguous(),
                         mask[:m], dlp.view(m, Lr), self.stats, cfg.clip, cfg.kl_coef, 1.0 / nb)
-            o.logprob(logits, tgt, None, dlp)                          # logits <- d loss / d logits
+            if lists is None:
+                o.logprob(logits, tgt, None, dlp)                      # logits <- d loss / d logits
+            else:  # with the distillation's: dlp is the gradient of log p[tgt], so -dlp weighs -log p[tgt]
+                loss, _ = distill_loss_grad(logits, lists[0][s0:s0 + m].view(m * Lr, -1),
+                                            lists[1][s0:s0 + m].view(m * Lr, -1), weight[: m * Lr],
+                                            kind=cfg.distill_kind, target=tgt, target_weight=-dlp, out=logits)
+                self.distill_kl += (loss - dlp * lp).sum() / cfg.distill_coef
             dhr = torch.empty(m * Lr, H, device=self.device, dtype=torch.bfloat16)
             o.gemm(logits, m_.head_weight(), dhr, False, True)          # d h = dLogits W_head
             o.gemm(logits, hr, m_.head_grad(), True, True, accumulate=True, split_k=1)  # dW_head += dLogits^T h

@@ -32,7 +32,7 @@ from typing import List, Optional
 import torch
 
 from .._native import core as _core, ops as _ops
-from ..models.llm import DecoderLM, LMConfig, apply_rope
+from ..models.llm import DecoderLM, LMConfig, apply_rope, embed_into
 from ..ops.kv_cache import decode_attention_quant, kv_quant_read, kv_quant_write, quant_kv_cache
 
 
@@ -188,7 +188,7 @@ class LLMGenerator:
         H, D = cfg.hidden, cfg.head_dim
         st = self.state
         x = st["x"]
-        o.embed_fwd(st["tok"], m.s["embed"], x)
+        embed_into(cfg, st["tok"], m.s["embed"], x)
         h, qkv, attn, x2, act = st["h"], st["qkv"], st["attn"], st["x2"], st["act"]
         # few sequences: the projections have few output tiles and long K, so
         # split K over the SMs (partials in this workspace); many sequences:
@@ -590,7 +590,7 @@ class TPLLMGenerator(LLMGenerator):
         st = self.state
         D = cfg.head_dim
         scale = 1.0 / math.sqrt(D)
-        o.embed_fwd(st["tok"], self.m.s["embed"], st["x"])
+        embed_into(cfg, st["tok"], self.m.s["embed"], st["x"])
         x = st["x"]
         for li, i in enumerate(tpm.layers):
             def attn_fn(qkv, out, li=li):
