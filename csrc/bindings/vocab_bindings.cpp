@@ -24,6 +24,7 @@ namespace {
 
 constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int64_t kMaxList = 256;
+constexpr int64_t kMaxTokens = 1 << 30, kMaxColumns = 1 << 24;  // of an embedding
 
 // [R, V] rows with a contiguous last dimension.
 int rows2(const at::Tensor& t, const char* op, const char* m) {
@@ -240,8 +241,8 @@ at::Tensor distill_loss_autograd(const at::Tensor& logits, const at::Tensor& ids
 // ------------------------------------------------------------------ embedding
 int ids_of(const at::Tensor& ids, const char* op) {
   chk((ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) && ids.is_contiguous() &&
-          ids.numel() <= INT_MAX,
-      op, "ids are contiguous int32 or int64, at most 2^31 - 1");
+          ids.numel() <= kMaxTokens,
+      op, "ids are contiguous int32 or int64, at most 2^30");
   return ids.scalar_type() == at::kLong;
 }
 void scale_of(double scale, const char* op) {
@@ -258,7 +259,8 @@ Opt embedding(const at::Tensor& ids, const at::Tensor& weight, double scale, con
   TbEmbeddingArgs a{};
   a.ids64 = ids_of(ids, op);
   a.dtype = rows2(weight, op, "weight is [V, H] with a contiguous last dimension");
-  chk(weight.size(0) >= 1 && weight.size(1) >= 1 && weight.size(1) <= INT_MAX, op, "at least one row and one column");
+  chk(weight.size(0) >= 1 && weight.size(1) >= 1 && weight.size(1) <= kMaxColumns, op,
+      "at least one row, and 1 to 2^24 columns");
   scale_of(scale, op);
   const at::Device dev = weight.device();
   chk(ids.device() == dev, op, "all tensors on one device");
@@ -303,7 +305,8 @@ bool embedding_grad(const at::Tensor& ids, const at::Tensor& dy, const at::Tenso
   TbEmbeddingGradArgs a{};
   a.ids64 = ids_of(ids, op);
   a.grad_dtype = rows2(grad, op, "grad is [V, H] with a contiguous last dimension");
-  chk(grad.size(0) >= 1 && grad.size(1) >= 1 && grad.size(1) <= INT_MAX, op, "at least one row and one column");
+  chk(grad.size(0) >= 1 && grad.size(1) >= 1 && grad.size(1) <= kMaxColumns, op,
+      "at least one row, and 1 to 2^24 columns");
   const int64_t H = grad.size(1), N = ids.numel();
   a.dtype = type_of(dy, op);
   chk(dy.sizes() == at::IntArrayRef(rows_shape(ids, H)), op, "dy has ids' shape and grad's row length");
