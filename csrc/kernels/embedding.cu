@@ -7,17 +7,16 @@
 //
 // * Few tokens: one CTA for each token and slab of columns.  The first token of an id
 //   finds the others by comparing all ids and sums their rows; one launch, no workspace.
-// * More: the tokens are sorted by id (stable, so by token within an id), then threads
-//   sum pieces of a fixed number of sorted tokens, a vector of columns each.  An id whose
-//   tokens lie within a piece is finished there; what an id has in the pieces that it
-//   shares with other pieces is left in a workspace, and a last launch adds those up.  A
-//   token that fills a third of the batch is thus as well spread as any other.
+// * More: the tokens are sorted by id (stable, so by token within an id); then each CTA
+//   sums a piece of 128 sorted tokens for 256 columns, a warp 16 of them.  An id whose
+//   tokens lie within a warp's share is finished there, one within the piece after an
+//   exchange over shared memory; what goes on into other pieces is left in a workspace, and
+//   a last launch adds it up.  A token that fills a third of the batch is thus spread over
+//   the machine like any other.
 //
-// The sort is a radix sort of one thread-block cluster (digits of up to 9 bits, counts
-// per warp in shared memory, totals exchanged over distributed shared memory), because
-// one launch with cluster barriers is shorter than the six launches of a sort over the
-// whole machine; a dense gradient's zeros are written by the other clusters meanwhile.
-#include <cooperative_groups.h>
+// Up to 8,192 tokens the sort counts, for each token, the ones before it (N^2 comparisons
+// in one launch); above it is a radix sort in digits of up to 9 bits, one launch to count
+// the first digit and one for each digit, which also counts the next one.
 #include <limits.h>
 #include <math.h>
 
@@ -28,14 +27,14 @@
 
 namespace {
 
-namespace cg = cooperative_groups;
-
 __device__ __forceinline__ long long id_of(const void* ids, int ids64, long long t) {
   return ids64 ? static_cast<const long long*>(ids)[t] : static_cast<const int*>(ids)[t];
 }
 
 // ------------------------------------------------------------------ lookup
-constexpr int kUnroll = 4;
+// Vectors of N elements that a lane has in flight.
+template <typename T, int N>
+constexpr int kUnroll = N * sizeof(T) == 16 ? 4 : 8;
 
 template <typename T, int N>
 __device__ __forceinline__ void scaled_row(const TbEmbeddingArgs& a, long long id, float (&x)[N]) {
@@ -48,25 +47,26 @@ __device__ __forceinline__ void scaled_row(const TbEmbeddingArgs& a, long long i
   }
 }
 
-// A warp takes 32 x kUnroll vectors of N elements of a row (rows of 32 vectors and more).
+// A warp takes 32 x U vectors of N elements of a row (rows of 32 vectors and more).
 template <typename T, int N>
 __global__ void __launch_bounds__(256) lookup_wide_kernel(TbEmbeddingArgs a, int segs) {
+  constexpr int U = kUnroll<T, N>;
   const int lane = threadIdx.x & 31, per = a.H / N;
   const long long tasks = static_cast<long long>(a.N) * segs;
   for (long long task = blockIdx.x * 8ll + threadIdx.x / 32; task < tasks; task += gridDim.x * 8ll) {
     const long long t = segs == 1 ? task : task / segs;
-    const int first = static_cast<int>(task - t * segs) * 32 * kUnroll + lane;
+    const int first = static_cast<int>(task - t * segs) * 32 * U + lane;
     const long long id = id_of(a.ids, a.ids64, t);
     const bool good = id >= 0 && id < a.V;
     if (id >= a.V && a.err && lane == 0) *a.err = 1;
     const T* src = static_cast<const T*>(a.weight) + (good ? id : 0) * a.ld_w;
     T* dst = static_cast<T*>(a.out) + t * a.ld_out;
-    tb::Packed<T, N> p[kUnroll];
+    tb::Packed<T, N> p[U];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < U; ++u)
       if (first + u * 32 < per && good) p[u].load(src + (first + u * 32) * N);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < U; ++u)
       if (first + u * 32 < per) {
         float x[N];
         p[u].unpack(x);
@@ -199,288 +199,446 @@ __global__ void __launch_bounds__(256) grad_few_kernel(TbEmbeddingGradArgs a, in
 }
 
 // ---- the sort
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxBins = 512;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxBins = 512, kMaxBlocks = 64, kMaxPasses = 4;
+constexpr int kCompared = 8192;  // tokens that are sorted by comparing them all
 
-struct SortPlan {
-  int N, V, bits, passes, L, pieces;  // L: tokens of a piece
+struct Plan {
+  int N, V;
+  int bits, passes, blocks, share;  // radix: bits of a digit; blocks of `share` tokens
+  int P, pieces;                    // sums: pieces of P tokens
+  int slabs, width;                 // slabs of `width` vectors of columns
+  long long row;                    // floats of a row of `part`
 };
-struct SortWork {  // in the workspace; pairs are (id, token)
+struct Work {  // in the workspace; pairs are (id, token), ids without a row are V
   uint2 *a, *b;
-  int* owners;  // [0]: how many; then the pieces where an id begins that goes on in the next one
-  float* part;  // [pieces][2][H]: the sums of the id that came in, and of the one that goes on
+  unsigned* counts;  // [passes][blocks][bins]
+  int* owners;       // [0]: how many; then the pieces where an id begins that goes on in the next one
+  float* part;       // [pieces][2][row]: the sums of the id that came in, and of the one that goes on
 };
 
-__device__ __forceinline__ uint2 ld_pair(const uint2* p) { return __ldcg(p); }
-
-// 16-byte stores of zeros over rows of `bytes` bytes, `stride` apart.
-__device__ void fill_zero(char* base, long long rows, long long bytes, long long stride, long long thread, long long threads) {
-  if (bytes == stride) {
-    bytes *= rows;
-    rows = 1;
-  }
-  if (rows == 1) {
-    const long long head = min(bytes, static_cast<long long>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15));
-    const long long body = (bytes - head) / 16;
-    uint4* p = reinterpret_cast<uint4*>(base + head);
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    long long i = thread;
-    for (; i + 3 * threads < body; i += 4 * threads) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) p[i + u * threads] = z;
-    }
-    for (; i < body; i += threads) p[i] = z;
-    const long long tail = bytes - head - body * 16;
-    if (thread < head) base[thread] = 0;
-    if (thread < tail) base[head + body * 16 + thread] = 0;
-    return;
-  }
-  for (long long i = thread; i < rows * (bytes / 2); i += threads)  // (rows with gaps; elements of 2 or 4 bytes)
-    reinterpret_cast<uint16_t*>(base + i / (bytes / 2) * stride)[i % (bytes / 2)] = 0;
+__device__ __forceinline__ unsigned key_of(const TbEmbeddingGradArgs& a, long long t) {
+  const long long id = id_of(a.ids, a.ids64, t);
+  if (id >= a.V && a.err) *a.err = 1;
+  return id < 0 || id >= a.V ? static_cast<unsigned>(a.V) : static_cast<unsigned>(id);
 }
 
-// Cluster 0 sorts; the others (a dense gradient) write the zeros.
-__global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(TbEmbeddingGradArgs a, SortPlan plan, SortWork work, int elem) {
-  extern __shared__ unsigned hist[];  // [warps][bins], then offsets
-  __shared__ unsigned total[kMaxBins], scan[kMaxBins];
-  __shared__ unsigned warp_sum[32];
-  cg::cluster_group cl = cg::this_cluster();
-  const int rank = cl.block_rank(), ranks = cl.num_blocks();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// A token's place is the number of tokens with smaller ids, and of earlier ones with the
+// same: 32 tokens per CTA, their comparisons shared by the lanes of 16 warps.
+__global__ void __launch_bounds__(512) compare_sort_kernel(TbEmbeddingGradArgs a, Plan plan, Work work) {
+  extern __shared__ unsigned keys[];  // [N], padded to a multiple of 4 with keys above all
+  __shared__ int place[32];
   tb::pdl_trigger();
-  if (blockIdx.x >= static_cast<unsigned>(ranks)) {
-    fill_zero(static_cast<char*>(a.grad), a.V, static_cast<long long>(a.H) * elem, a.ld_grad * elem,
-              (blockIdx.x - ranks) * static_cast<long long>(kSortThreads) + tid,
-              (gridDim.x - ranks) * static_cast<long long>(kSortThreads));
-    return;
+  const int n4 = (plan.N + 3) / 4 * 4;
+  for (int t = threadIdx.x; t < n4; t += 512) keys[t] = t < plan.N ? key_of(a, t) : 0xffffffffu;
+  if (threadIdx.x < 32) place[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) work.owners[0] = 0;
+  __syncthreads();
+  const int t = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
+  const unsigned key = t < plan.N ? keys[t] : 0;
+  const uint4* all = reinterpret_cast<const uint4*>(keys);
+  // four keys at a time; before the CTA's tokens equal ones count, behind them they do not
+  const int first = blockIdx.x * 8, last = first + 8;  // the CTA's own, in fours
+  int n = 0;
+#pragma unroll 4
+  for (int i = warp; i < n4 / 4; i += 16) {
+    const uint4 k = all[i];
+    if (i < first) {
+      n += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+    } else if (i >= last) {
+      n += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
+    } else {
+      const int u = i * 4;
+      n += (k.x < key || (k.x == key && u < t)) + (k.y < key || (k.y == key && u + 1 < t)) +
+           (k.z < key || (k.z == key && u + 2 < t)) + (k.w < key || (k.w == key && u + 3 < t));
+    }
   }
-  const int N = plan.N, bins = 1 << plan.bits;
-  // a warp's tokens: consecutive, a multiple of 32 of them
-  const int per = (N + ranks * kSortThreads - 1) / (ranks * kSortThreads) * 32;
-  const int lo = min(N, (rank * kSortWarps + warp) * per), hi = min(N, lo + per);
-  if (rank == 0 && tid == 0) work.owners[0] = 0;
-  uint2* in = nullptr;
-  for (int pass = 0; pass < plan.passes; ++pass) {
-    uint2* out = (plan.passes - pass) % 2 ? work.a : work.b;  // the last pass writes a
-    const int shift = pass * plan.bits;
-    const auto pair_at = [&](int i) {
-      if (pass) return ld_pair(in + i);
-      const long long id = id_of(a.ids, a.ids64, i);
-      if (id >= a.V && a.err) *a.err = 1;
-      return make_uint2(id < 0 || id >= a.V ? plan.V : static_cast<unsigned>(id), i);
-    };
-    for (int i = tid; i < kSortWarps * bins; i += kSortThreads) hist[i] = 0;
-    __syncthreads();
-    unsigned* mine = hist + warp * bins;
-    // ---- counts of each warp
-    for (int i0 = lo; i0 < hi; i0 += 128) {
-      unsigned key[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) key[u] = i0 + u * 32 + lane < hi ? pair_at(i0 + u * 32 + lane).x : 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool on = i0 + u * 32 + lane < hi;
-        const unsigned d = on ? key[u] >> shift & (bins - 1) : 0xffffffffu;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        if (on && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
-        __syncwarp();
-      }
+  atomicAdd(&place[threadIdx.x & 31], n);
+  __syncthreads();
+  if (threadIdx.x < 32 && t < plan.N) work.a[place[threadIdx.x]] = make_uint2(key, t);
+}
+
+// Counts of the first digit, a block of tokens per CTA.
+__global__ void __launch_bounds__(kSortThreads) count_kernel(TbEmbeddingGradArgs a, Plan plan, Work work) {
+  __shared__ unsigned hist[kMaxBins];
+  const int bins = 1 << plan.bits, tid = threadIdx.x;
+  tb::pdl_trigger();
+  if (tid < bins) {
+    hist[tid] = 0;
+    for (int p = 1; p < plan.passes; ++p) work.counts[(p * plan.blocks + blockIdx.x) * bins + tid] = 0;
+  }
+  if (blockIdx.x == 0 && tid == 0) work.owners[0] = 0;
+  __syncthreads();
+  const long long lo = static_cast<long long>(blockIdx.x) * plan.share;
+  const long long hi = min(static_cast<long long>(plan.N), lo + plan.share);
+  for (long long t = lo + tid; t < hi; t += kSortThreads) atomicAdd(&hist[key_of(a, t) & (bins - 1)], 1u);
+  __syncthreads();
+  if (tid < bins) work.counts[blockIdx.x * bins + tid] = hist[tid];
+}
+
+// One digit: the pairs of a block to their places (stable), and the next digit counted
+// for the blocks that they come to.
+__global__ void __launch_bounds__(kSortThreads, 1) scatter_kernel(TbEmbeddingGradArgs a, Plan plan, Work work, int pass) {
+  extern __shared__ unsigned hist[];  // [warps][bins]: counts, then places
+  __shared__ unsigned scan[kMaxBins], warp_sum[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bins = 1 << plan.bits, shift = pass * plan.bits;
+  tb::pdl_trigger();
+  for (int i = tid; i < kSortWarps * bins; i += kSortThreads) hist[i] = 0;
+  __syncthreads();
+  tb::pdl_wait();
+  const uint2* in = (plan.passes - pass) % 2 ? work.b : work.a;  // the last pass writes a
+  uint2* out = (plan.passes - pass) % 2 ? work.a : work.b;
+  // a warp's pairs: consecutive, a multiple of 32 of them
+  const long long end = min(static_cast<long long>(plan.N), (blockIdx.x + 1ll) * plan.share);
+  const int per = (plan.share + kSortThreads - 1) / kSortThreads * 32;
+  const long long lo = min(end, static_cast<long long>(blockIdx.x) * plan.share + warp * static_cast<long long>(per));
+  const long long hi = min(end, lo + per);
+  const auto pair_at = [&](long long i) {
+    if (pass) return __ldcg(in + i);
+    return make_uint2(key_of(a, i), static_cast<unsigned>(i));
+  };
+  // lanes with the same digit (a ballot for each bit)
+  const auto peers_of = [&](unsigned d, bool on) {
+    unsigned peers = __ballot_sync(0xffffffffu, on);
+    for (int b = 0; b < plan.bits; ++b) {
+      const unsigned x = __ballot_sync(0xffffffffu, d >> b & 1);
+      peers &= d >> b & 1 ? x : ~x;
     }
-    __syncthreads();
-    // ---- where each warp's tokens of a digit go
-    if (tid < bins) {
-      unsigned s = 0;
-      for (int w = 0; w < kSortWarps; ++w) {
-        const unsigned c = hist[w * bins + tid];
-        hist[w * bins + tid] = s;
-        s += c;
-      }
-      total[tid] = s;
+    return peers;
+  };
+  unsigned* mine = hist + warp * bins;
+  uint2 p = make_uint2(0, 0);
+  unsigned peers = 0;
+  for (long long i = lo + lane; i - lane < hi; i += 32) {
+    const bool on = i < hi;
+    if (on) p = pair_at(i);
+    const unsigned d = p.x >> shift & (bins - 1);
+    peers = peers_of(d, on);
+    if (on && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+    __syncwarp();
+  }
+  // ---- the digit's places over all blocks
+  unsigned all = 0, before = 0;
+  if (tid < bins) {
+    const unsigned* counts = work.counts + pass * plan.blocks * bins + tid;
+#pragma unroll 8
+    for (int b = 0; b < plan.blocks; ++b) {
+      const unsigned c = __ldcg(counts + b * bins);
+      if (b < static_cast<int>(blockIdx.x)) before += c;
+      all += c;
     }
-    cl.sync();
-    unsigned all = 0, before = 0;
-    if (tid < bins)
-      for (int r = 0; r < ranks; ++r) {
-        const unsigned c = *cl.map_shared_rank(&total[tid], r);
-        if (r < rank) before += c;
-        all += c;
-      }
-    unsigned incl = all;  // inclusive sum over the digits (threads past the last digit hold 0)
+  }
+  unsigned incl = all;  // inclusive sum over the digits (threads past the last digit hold 0)
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    unsigned x = warp_sum[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
+      const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    if (lane == 31) warp_sum[warp] = incl;
-    __syncthreads();
-    if (warp == 0) {
-      unsigned x = warp_sum[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      warp_sum[lane] = x;
-    }
-    __syncthreads();
-    if (tid < bins) scan[tid] = incl - all + (warp ? warp_sum[warp - 1] : 0) + before;
-    __syncthreads();
-    for (int i = tid; i < kSortWarps * bins; i += kSortThreads) hist[i] += scan[i & (bins - 1)];
-    __syncthreads();
-    // ---- to their places
-    for (int i0 = lo; i0 < hi; i0 += 128) {
-      uint2 p[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) p[u] = i0 + u * 32 + lane < hi ? pair_at(i0 + u * 32 + lane) : make_uint2(0, 0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool on = i0 + u * 32 + lane < hi;
-        const unsigned d = on ? p[u].x >> shift & (bins - 1) : 0xffffffffu;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const unsigned at = on ? mine[d] + __popc(peers & ((1u << lane) - 1)) : 0;
-        __syncwarp();
-        if (on) {
-          if (lane == __ffs(peers) - 1) mine[d] += __popc(peers);
-          __stcg(out + at, p[u]);
-        }
-        __syncwarp();
-      }
-    }
-    cl.sync();
-    in = out;
+    warp_sum[lane] = x;
   }
-  // ---- pieces where an id begins that the next piece goes on with
-  for (int c = rank * kSortThreads + tid; c + 1 < plan.pieces; c += ranks * kSortThreads) {
-    const int e = (c + 1) * plan.L;
-    const unsigned id = ld_pair(in + e).x;
-    if (id < static_cast<unsigned>(plan.V) && ld_pair(in + e - 1).x == id &&
-        (c == 0 || ld_pair(in + c * plan.L - 1).x != id))
-      work.owners[1 + atomicAdd(&work.owners[0], 1)] = c;
+  __syncthreads();
+  // ---- and over the warps of this one (two halves of the warps per digit)
+  const int half = tid >> plan.bits, w0 = half * (kSortWarps / 2);
+  const unsigned digit = tid & (bins - 1);
+  unsigned c[kSortWarps / 2], sum = 0;
+  if (half < 2) {
+#pragma unroll
+    for (int w = 0; w < kSortWarps / 2; ++w) c[w] = hist[(w0 + w) * bins + digit];
+#pragma unroll
+    for (int w = 0; w < kSortWarps / 2; ++w) sum += c[w];
+    if (half == 0) scan[digit] = incl - all + (warp ? warp_sum[warp - 1] : 0) + before + sum;  // where the second half begins
+  }
+  __syncthreads();
+  if (half < 2) {
+    unsigned at = scan[digit] - (half == 0 ? sum : 0);
+#pragma unroll
+    for (int w = 0; w < kSortWarps / 2; ++w) {
+      hist[(w0 + w) * bins + digit] = at;
+      at += c[w];
+    }
+  }
+  __syncthreads();
+  // ---- to their places
+  const bool once = per == 32;
+  for (long long i = lo + lane; i - lane < hi; i += 32) {
+    const bool on = i < hi;
+    if (!once && on) p = pair_at(i);
+    const unsigned d = p.x >> shift & (bins - 1);
+    if (!once) peers = peers_of(d, on);
+    const unsigned at = on ? mine[d] + __popc(peers & ((1u << lane) - 1)) : 0;
+    __syncwarp();
+    if (on) {
+      if (lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+      __stcg(out + at, p);
+      if (pass + 1 < plan.passes)
+        atomicAdd(&work.counts[((pass + 1) * plan.blocks + at / plan.share) * bins + (p.x >> (shift + plan.bits) & (bins - 1))], 1u);
+    }
+    __syncwarp();
   }
 }
 
-// ---- sums of pieces: a thread takes N columns of a piece
-template <typename T, typename G, int N>
-__global__ void __launch_bounds__(256) pieces_kernel(TbEmbeddingGradArgs a, SortPlan plan, SortWork work, bool vec) {
-  constexpr int U = 8;
-  const int per = a.H / N;
-  const unsigned V = plan.V;
+// ---- a dense gradient's zeros
+constexpr int kFillBytes = 32768;
+__global__ void __launch_bounds__(128) fill_kernel(char* base, long long bytes) {  // base and bytes: multiples of 16
+  extern __shared__ __align__(128) uint4 zeros[];
   tb::pdl_trigger();
-  tb::pdl_wait();
-  const long long i = blockIdx.x * 256ll + threadIdx.x;
-  const long long c = static_cast<long long>(plan.pieces) * per <= UINT_MAX ? static_cast<unsigned>(i) / static_cast<unsigned>(per) : i / per;
-  if (c >= plan.pieces) return;
-  const int h = static_cast<int>(i - c * per) * N;
+  for (int i = threadIdx.x; i < kFillBytes / 16; i += 128) zeros[i] = make_uint4(0, 0, 0, 0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x) return;
+  const unsigned src = static_cast<unsigned>(__cvta_generic_to_shared(zeros));
+  for (long long at = blockIdx.x * static_cast<long long>(kFillBytes); at < bytes; at += gridDim.x * static_cast<long long>(kFillBytes)) {
+    const unsigned n = static_cast<unsigned>(min(static_cast<long long>(kFillBytes), bytes - at));
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + at), "r"(src), "r"(n) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group.read 4;" ::: "memory");
+  }
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  tb::pdl_wait();  // so that whoever waits for this kernel also waits for the one before
+}
+
+// ---- the sums.  A lane has eight columns of a slab, as M vectors of N.
+template <typename T, typename G, int N>
+struct Tile {
+  static constexpr int M = 8 / N;
+  int h[M];  // first column of each vector; -1: none
+  __device__ __forceinline__ Tile(const TbEmbeddingGradArgs& a, const Plan& plan, int slab) {
+    const int lane = threadIdx.x & 31, per = a.H / N, end = min(per, (slab + 1) * plan.width);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int v = slab * plan.width + m * 32 + lane;
+      h[m] = m * 32 + lane < plan.width && v < end ? v * N : -1;
+    }
+  }
+  __device__ __forceinline__ void finish_row(const TbEmbeddingGradArgs& a, bool vec, long long id, const float (&sum)[M][N]) const {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+      if (h[m] >= 0) finish<G, N>(a, vec, id, h[m], sum[m]);
+  }
+  __device__ __forceinline__ void leave(float* row, const float (&sum)[M][N]) const {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+      if (h[m] >= 0) tb::store_vec<float, N>(row + h[m], sum[m]);
+  }
+  __device__ __forceinline__ static void zero(float (&sum)[M][N]) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum[m][j] = 0.f;
+  }
+  __device__ __forceinline__ static void put(float* s, const float (&sum)[M][N]) {  // 256 floats of shared memory
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < N; ++j) s[(m * N + j) * 32 + (threadIdx.x & 31)] = sum[m][j];
+  }
+  __device__ __forceinline__ static void add(const float* s, float (&sum)[M][N]) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum[m][j] += s[(m * N + j) * 32 + (threadIdx.x & 31)];
+  }
+};
+
+constexpr int kWarps = 8;
+
+template <typename T, typename G, int N>
+__global__ void __launch_bounds__(kWarps * 32, 3) pieces_kernel(TbEmbeddingGradArgs a, Plan plan, Work work, bool vec) {
+  using Sum = Tile<T, G, N>;
+  constexpr int M = Sum::M, U = N * sizeof(T) == 16 ? 8 / M : 4;
+  __shared__ float in[kWarps][256], on[kWarps][256];  // sums of the ids that came in, that go on
+  __shared__ bool through[kWarps];                    // the id that came in goes on
+  tb::pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x / plan.slabs, slab = blockIdx.x % plan.slabs;
+  const Sum tile(a, plan, slab);
+  const unsigned V = plan.V;
+  const T* dy = static_cast<const T*>(a.dy);
+  float* part = work.part + static_cast<long long>(c) * 2 * plan.row;
   const uint2* pairs = work.a;
-  const int lo = static_cast<int>(c) * plan.L, hi = min(plan.N, lo + plan.L);
-  unsigned id = ld_pair(pairs + lo).x;
-  if (id >= V) return;
-  bool came = lo > 0 && ld_pair(pairs + lo - 1).x == id;  // the id began in an earlier piece
-  float* part = work.part + c * 2 * a.H + h;
-  const T* dy = static_cast<const T*>(a.dy) + h;
-  float sum[N];
+  const int lo = min(static_cast<long long>(plan.N), static_cast<long long>(c) * plan.P + warp * (plan.P / kWarps));
+  const int hi = min(static_cast<long long>(plan.N), static_cast<long long>(c) * plan.P + (warp + 1) * (plan.P / kWarps));
+  float sum[M][N];
+  Sum::zero(sum);
+  bool came = false, goes = false, ends = false;  // ends: what came in has its end here
+  unsigned id = V;
+  tb::pdl_wait();
+  if (lo < hi) {
+    const unsigned prev = lo > 0 ? __ldcg(pairs + lo - 1).x : V, next = hi < plan.N ? __ldcg(pairs + hi).x : V;
+    uint2 mine = lo + lane < hi ? __ldcg(pairs + lo + lane) : make_uint2(V, 0);
+    id = __shfl_sync(0xffffffffu, mine.x, 0);
+    came = id < V && prev == id;
+    bool first = came;  // the sum is of what came in
+    for (int i0 = lo; i0 < hi && id < V; i0 += 32) {
+      if (i0 != lo) mine = i0 + lane < hi ? __ldcg(pairs + i0 + lane) : make_uint2(V, 0);
+      const int n = min(32, hi - i0);
+      for (int u0 = 0; u0 < n; u0 += U) {
+        unsigned key[U];
+        tb::Packed<T, N> x[U][M];
 #pragma unroll
-  for (int j = 0; j < N; ++j) sum[j] = 0.f;
-  const auto leave = [&](int which) {
-    float* p = part + static_cast<long long>(which) * a.H;
+        for (int u = 0; u < U; ++u) {  // (u0 + u < 32: U divides 32; lanes behind the end hold V)
+          key[u] = __shfl_sync(0xffffffffu, mine.x, u0 + u);
+          const T* row = dy + static_cast<long long>(__shfl_sync(0xffffffffu, mine.y, u0 + u)) * a.ld_dy;
 #pragma unroll
-    for (int j = 0; j < N; ++j) p[j] = sum[j];
-  };
-  for (int i0 = lo; i0 < hi && id < V; i0 += U) {
-    uint2 p[U];
-    tb::Packed<T, N> x[U];
+          for (int m = 0; m < M; ++m)
+            if (key[u] < V && tile.h[m] >= 0) x[u][m].load(row + tile.h[m]);
+        }
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u] = i0 + u < hi ? ld_pair(pairs + i0 + u) : make_uint2(V, 0);
+        for (int u = 0; u < U; ++u) {
+          if (u0 + u >= n) break;
+          if (key[u] != id) {
+            if (id < V) {
+              if (first) {
+                Sum::put(in[warp], sum);
+                ends = true;
+              } else {
+                tile.finish_row(a, vec, id, sum);
+              }
+            }
+            first = false;
+            id = key[u];
+            Sum::zero(sum);
+          }
+          if (id < V) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (p[u].x < V) x[u].load(dy + static_cast<long long>(p[u].y) * a.ld_dy);
+            for (int m = 0; m < M; ++m) {
+              float f[N];
+              x[u][m].unpack(f);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i0 + u >= hi) break;
-      if (p[u].x != id) {
-        if (id < V) {
-          if (came) {
-            leave(0);
-          } else {
-            finish<G, N>(a, vec, id, h, sum);
+              for (int j = 0; j < N; ++j) sum[m][j] += f[j];
+            }
           }
         }
-        came = false;
-        id = p[u].x;
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] = 0.f;
-      }
-      if (id < V) {
-        float f[N];
-        x[u].unpack(f);
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] += f[j];
       }
     }
+    goes = id < V && next == id;
+    if (first) {
+      Sum::put(in[warp], sum);
+      ends = !goes;
+    } else if (goes) {
+      Sum::put(on[warp], sum);
+    } else if (id < V) {
+      tile.finish_row(a, vec, id, sum);
+    }
   }
-  if (id >= V) return;
-  if (came) {
-    leave(0);
-  } else if (hi < plan.N && ld_pair(pairs + hi).x == id) {
-    leave(1);
-  } else {
-    finish<G, N>(a, vec, id, h, sum);
+  if (lane == 0) through[warp] = came && !ends;
+  __syncthreads();
+  // ---- what goes on within the piece
+  if (warp == 0 && came) {  // and what came into it
+    Sum::zero(sum);
+    for (int w = 0;; ++w) {
+      Sum::add(in[w], sum);
+      if (!through[w] || w + 1 == kWarps) break;
+    }
+    tile.leave(part, sum);
+  }
+  if (goes && !(came && !ends)) {
+    Sum::zero(sum);
+    Sum::add(on[warp], sum);
+    for (int w = warp + 1;; ++w) {
+      if (w == kWarps) {  // into the next piece
+        tile.leave(part + plan.row, sum);
+        if (slab == 0 && lane == 0) work.owners[1 + atomicAdd(&work.owners[0], 1)] = c;
+        break;
+      }
+      Sum::add(in[w], sum);
+      if (!through[w]) {
+        tile.finish_row(a, vec, id, sum);
+        break;
+      }
+    }
   }
 }
 
-// ---- ids over several pieces: a CTA takes 32 vectors of columns of one; its warps share
-// the pieces, the first one's sum comes first
-constexpr int kJoinWarps = 16;
+// ---- ids over several pieces: a warp takes a slab of one; over many pieces the CTA's warps
+// share them (the order of the additions follows from the number of pieces alone)
+constexpr int kShared = 32;
 template <typename G, int N>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(TbEmbeddingGradArgs a, SortPlan plan, SortWork work, int slabs, bool vec) {
-  constexpr int U = 8;
-  __shared__ float buf[kJoinWarps][32 * N];
+__global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a, Plan plan, Work work, bool vec) {
+  using Sum = Tile<float, G, N>;
+  constexpr int M = Sum::M, U = 4;
+  __shared__ float buf[kWarps][256];
+  __shared__ int count[kWarps], begin[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tb::pdl_wait();
-  const long long tasks = static_cast<long long>(work.owners[0]) * slabs;
-  for (long long task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int c = work.owners[1 + task / slabs];
-    const int h = static_cast<int>(task % slabs) * 32 * N + lane * N;
-    const unsigned id = ld_pair(work.a + (c + 1ll) * plan.L).x;
-    int n = 0;  // pieces that the id comes into
-    for (;;) {
-      const long long p = c + 1ll + n + threadIdx.x;
-      const int on = __syncthreads_count(p < plan.pieces && ld_pair(work.a + p * plan.L).x == id);
-      n += on;
-      if (on < kJoinWarps * 32) break;
+  const long long tasks = static_cast<long long>(__ldcg(work.owners)) * plan.slabs;
+  const auto sum_of = [&](const Sum& tile, long long first, int n, float (&sum)[M][N]) {
+    for (int i = 0; i < n; i += U) {
+      float x[U][M][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          if (i + u < n && tile.h[m] >= 0) tb::load_vec<float, N>(work.part + (first + i + u) * 2 * plan.row + tile.h[m], x[u][m]);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u < n) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[m][j] += x[u][m][j];
+        }
     }
-    float sum[N];
+  };
+  const auto first_of = [&](const Sum& tile, long long c, float (&sum)[M][N]) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] = 0.f;
-    if (h < a.H) {
-      const int lo = static_cast<int>(static_cast<long long>(n) * warp / kJoinWarps);
-      const int hi = static_cast<int>(static_cast<long long>(n) * (warp + 1) / kJoinWarps);
-      const float* p = work.part + (c + 1ll) * 2 * a.H + h;
-      if (warp == 0) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] = p[-static_cast<long long>(a.H) + j];
+    for (int m = 0; m < M; ++m)
+      if (tile.h[m] >= 0) tb::load_vec<float, N>(work.part + (c * 2 + 1) * plan.row + tile.h[m], sum[m]);
+  };
+  for (long long base = blockIdx.x * static_cast<long long>(kWarps); base < tasks; base += gridDim.x * static_cast<long long>(kWarps)) {
+    const long long task = base + warp;
+    if (task < tasks) {
+      const int c = __ldcg(work.owners + 1 + task / plan.slabs);
+      const unsigned id = __ldcg(work.a + (c + 1ll) * plan.P).x;
+      int n = 0;  // pieces that the id comes into
+      for (;;) {
+        const long long p = c + 1ll + n + lane;
+        const int k = __popc(__ballot_sync(0xffffffffu, p < plan.pieces && __ldcg(work.a + min(p, plan.pieces - 1ll) * plan.P).x == id));
+        n += k;
+        if (k < 32) break;
       }
-      for (int i = lo; i < hi; i += U) {
-        float x[U][N];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int j = 0; j < N; ++j) x[u][j] = i + u < hi ? p[(i + u) * 2ll * a.H + j] : 0.f;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int j = 0; j < N; ++j) sum[j] += x[u][j];
+      if (lane == 0) {
+        count[warp] = n;
+        begin[warp] = c;
       }
+      if (n <= kShared) {
+        const Sum tile(a, plan, static_cast<int>(task % plan.slabs));
+        float sum[M][N];
+        Sum::zero(sum);
+        first_of(tile, c, sum);
+        sum_of(tile, c + 1ll, n, sum);
+        tile.finish_row(a, vec, id, sum);
+      }
+    } else if (lane == 0) {
+      count[warp] = 0;
     }
-#pragma unroll
-    for (int j = 0; j < N; ++j) buf[warp][j * 32 + lane] = sum[j];
     __syncthreads();
-    if (warp == 0 && h < a.H) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        sum[j] = 0.f;
-        for (int w = 0; w < kJoinWarps; ++w) sum[j] += buf[w][j * 32 + lane];
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = count[w];
+      if (n <= kShared) continue;
+      const Sum tile(a, plan, static_cast<int>((base + w) % plan.slabs));
+      const int c = begin[w], lo = static_cast<int>(static_cast<long long>(n) * warp / kWarps);
+      const int hi = static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
+      float sum[M][N];
+      Sum::zero(sum);
+      if (warp == 0) first_of(tile, c, sum);
+      sum_of(tile, c + 1ll + lo, hi - lo, sum);
+      Sum::put(buf[warp], sum);
+      __syncthreads();
+      if (warp == 0) {
+        for (int v = 1; v < kWarps; ++v) Sum::add(buf[v], sum);
+        tile.finish_row(a, vec, __ldcg(work.a + (c + 1ll) * plan.P).x, sum);
       }
-      finish<G, N>(a, vec, id, h, sum);
+      __syncthreads();
     }
     __syncthreads();
   }
@@ -495,7 +653,8 @@ template <typename T, int N>
 cudaError_t lookup(const TbEmbeddingArgs& a, cudaStream_t s) {
   const int per = a.H / N;
   if (per >= 32) {
-    const int segs = (per + 32 * kUnroll - 1) / (32 * kUnroll);
+    constexpr int kRow = 32 * kUnroll<T, N>;
+    const int segs = (per + kRow - 1) / kRow;
     const long long ctas = (static_cast<long long>(a.N) * segs + 7) / 8;
     lookup_wide_kernel<T, N><<<static_cast<unsigned>(ctas < (1 << 24) ? ctas : 1 << 24), 256, 0, s>>>(a, segs);
   } else {
@@ -519,79 +678,109 @@ cudaError_t lookup_of(const TbEmbeddingArgs& a, cudaStream_t s) {
   return lookup<T, 1>(a, s);
 }
 
-SortPlan plan_of(int N, int V) {
-  SortPlan p{};
+size_t up16(size_t b) { return (b + 15) / 16 * 16; }
+
+Plan plan_of(int N, int H, int V, int vec) {
+  Plan p{};
   p.N = N;
   p.V = V;
   int bits = 1;
   while (bits < 31 && (V >> bits) != 0) ++bits;  // keys 0 .. V
   p.passes = (bits + 8) / 9;
   p.bits = (bits + p.passes - 1) / p.passes;
-  // pieces of at least 16 tokens, at most 4,096 of them (and of the workspace's rows)
-  p.L = 16;
-  while ((N + p.L - 1) / p.L > 4096) p.L *= 2;
-  p.pieces = (N + p.L - 1) / p.L;
+  // radix: a token per thread, up to the blocks whose counts a block adds up by itself
+  p.blocks = (N + kSortThreads - 1) / kSortThreads;
+  if (p.blocks > kMaxBlocks) p.blocks = kMaxBlocks;
+  p.share = ((N + p.blocks - 1) / p.blocks + 31) / 32 * 32;
+  // pieces of 128 tokens, at most 8,192 of them (and of the workspace's rows)
+  p.P = 128;
+  while ((N + p.P - 1) / p.P > 8192) p.P *= 2;
+  p.pieces = (N + p.P - 1) / p.P;
+  const int per = H / vec, most = 256 / vec;
+  p.slabs = (per + most - 1) / most;
+  p.width = ((per + p.slabs - 1) / p.slabs + 31) / 32 * 32;
+  p.row = (H + 3) / 4 * 4;
   return p;
 }
-size_t up16(size_t b) { return (b + 15) / 16 * 16; }
 
-template <typename K, typename... Args>
-cudaError_t launch_after(K kernel, unsigned grid, unsigned block, cudaStream_t s, Args... args) {
+size_t work_of(const Plan& p, char* w, Work* out) {
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    char* q = w + at;
+    at += up16(bytes);
+    return q;
+  };
+  Work k;
+  k.a = reinterpret_cast<uint2*>(take(p.N * sizeof(uint2)));
+  k.b = reinterpret_cast<uint2*>(take(p.N * sizeof(uint2)));
+  k.counts = reinterpret_cast<unsigned*>(take(static_cast<size_t>(kMaxPasses) * kMaxBlocks * kMaxBins * sizeof(unsigned)));
+  k.owners = reinterpret_cast<int*>(take((p.pieces + 1) * sizeof(int)));
+  k.part = reinterpret_cast<float*>(take(static_cast<size_t>(p.pieces) * 2 * p.row * sizeof(float)));
+  if (out) *out = k;
+  return at;
+}
+
+template <typename... P, typename... Args>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, bool after, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Zeros in all rows of grad.  Large rows without gaps: by a kernel, beside the launch before
+// it (`after`); others before that.
+template <typename G>
+bool by_kernel(const TbEmbeddingGradArgs& a) {
+  const size_t all = a.H * sizeof(G) * a.V;
+  return (a.ld_grad == a.H || a.V == 1) && all >= (1 << 20) && (reinterpret_cast<uintptr_t>(a.grad) | all) % 16 == 0;
+}
+template <typename G>
+cudaError_t fill(const TbEmbeddingGradArgs& a, cudaStream_t s, bool after) {
+  const size_t row = a.H * sizeof(G), all = row * a.V;
+  if (by_kernel<G>(a))
+    return launch(fill_kernel, 148u * 2, 128u, kFillBytes, s, after, static_cast<char*>(a.grad), static_cast<long long>(all));
+  if (a.ld_grad == a.H || a.V == 1) return cudaMemsetAsync(a.grad, 0, all, s);
+  return cudaMemset2DAsync(a.grad, a.ld_grad * sizeof(G), 0, row, a.V, s);
 }
 
 template <typename T, typename G, int N>
 cudaError_t grad(const TbEmbeddingGradArgs& a, cudaStream_t s) {
   const bool vec = aligned(a.grad, a.ld_grad * sizeof(G), N * sizeof(G) < 16 ? N * sizeof(G) : 16);
-  const int slabs = (a.H + 32 * N - 1) / (32 * N);
-  if (a.N <= kFew) {
-    if (a.zero) {
-      const size_t row = a.H * sizeof(G);
-      const cudaError_t e = a.ld_grad == a.H ? cudaMemsetAsync(a.grad, 0, row * a.V, s)
-                                             : cudaMemset2DAsync(a.grad, a.ld_grad * sizeof(G), 0, row, a.V, s);
-      if (e != cudaSuccess) return e;
-    }
-    if (a.N > 0) grad_few_kernel<T, G, N><<<static_cast<unsigned>(a.N) * slabs, 256, 0, s>>>(a, slabs, vec);
+  const bool few = a.N <= kFew, beside = a.zero && !few && by_kernel<G>(a);
+  cudaError_t e = cudaSuccess;
+  if (a.zero && !beside) e = fill<G>(a, s, false);
+  if (e != cudaSuccess || a.N == 0) return e;
+  if (few) {
+    const int slabs = (a.H + 32 * N - 1) / (32 * N);
+    grad_few_kernel<T, G, N><<<static_cast<unsigned>(a.N) * slabs, 256, 0, s>>>(a, slabs, vec);
     return cudaGetLastError();
   }
-  const SortPlan plan = plan_of(a.N, a.V);
-  SortWork work;
-  char* w = static_cast<char*>(a.ws);
-  work.a = reinterpret_cast<uint2*>(w);
-  work.b = reinterpret_cast<uint2*>(w += up16(a.N * sizeof(uint2)));
-  work.owners = reinterpret_cast<int*>(w += up16(a.N * sizeof(uint2)));
-  work.part = reinterpret_cast<float*>(w += up16((plan.pieces + 1) * sizeof(int)));
-  const int ranks = a.N <= 2048 ? 1 : a.N <= 4096 ? 2 : a.N <= 8192 ? 4 : 8;
-  const int smem = kSortWarps * (1 << plan.bits) * static_cast<int>(sizeof(unsigned));
-  cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&sort_kernel), kSortWarps * kMaxBins * 4);
+  const Plan plan = plan_of(a.N, a.H, a.V, N);
+  Work work;
+  work_of(plan, static_cast<char*>(a.ws), &work);
+  if (a.N <= kCompared) {
+    e = launch(compare_sort_kernel, (a.N + 31) / 32, 512u, (a.N + 3) / 4 * 16, s, false, a, plan, work);
+  } else {
+    e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&scatter_kernel), kSortWarps * kMaxBins * 4);
+    if (e == cudaSuccess) e = launch(count_kernel, plan.blocks, kSortThreads, 0, s, false, a, plan, work);
+    for (int p = 0; p < plan.passes && e == cudaSuccess; ++p)
+      e = launch(scatter_kernel, plan.blocks, kSortThreads, (kSortWarps << plan.bits) * sizeof(unsigned), s, true, a, plan, work, p);
+  }
+  if (e == cudaSuccess && beside) e = fill<G>(a, s, true);  // (the sort neither reads nor writes grad)
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ranks + (a.zero ? (148 - ranks) / ranks * ranks : 0));
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sort_kernel, a, plan, work, static_cast<int>(sizeof(G)));
+  e = launch(pieces_kernel<T, G, N>, static_cast<unsigned>(plan.pieces) * plan.slabs, kWarps * 32, 0, s, true, a, plan, work, vec);
   if (e != cudaSuccess) return e;
-  const long long threads = static_cast<long long>(plan.pieces) * (a.H / N);
-  e = launch_after(pieces_kernel<T, G, N>, static_cast<unsigned>((threads + 255) / 256), 256, s, a, plan, work, vec);
-  if (e != cudaSuccess) return e;
-  const long long tasks = static_cast<long long>(plan.pieces) * slabs;
-  return launch_after(join_kernel<G, N>, static_cast<unsigned>(tasks < 296 ? tasks : 296), kJoinWarps * 32, s, a, plan, work, slabs, vec);
+  const long long tasks = static_cast<long long>(plan.pieces) * plan.slabs;
+  const long long ctas = (tasks + kWarps - 1) / kWarps;
+  return launch(join_kernel<G, N>, static_cast<unsigned>(ctas < 592 ? ctas : 592), kWarps * 32, 0, s, true, a, plan, work, vec);
 }
 
 template <typename T, typename G>
@@ -631,8 +820,7 @@ extern "C" int tb_embedding(const TbEmbeddingArgs* args, cudaStream_t s) {
 
 extern "C" size_t tb_embedding_grad_ws_bytes(int N, int H, int V) {
   if (N <= kFew) return 0;
-  const SortPlan p = plan_of(N, V);
-  return 2 * up16(N * sizeof(uint2)) + up16((p.pieces + 1) * sizeof(int)) + static_cast<size_t>(p.pieces) * 2 * H * sizeof(float);
+  return work_of(plan_of(N, H, V, 1), nullptr, nullptr);
 }
 
 extern "C" int tb_embedding_grad(const TbEmbeddingGradArgs* args, cudaStream_t s) {
