@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(256) grad_few_kernel(TbEmbeddingGradArgs a, in
 
 // ---- the sort
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxBins = 512, kMaxBlocks = 64, kMaxPasses = 4;
+constexpr int kSms = 148;
 constexpr int kCompared = 8192;  // tokens that are sorted by comparing them all
 
 struct Plan {
@@ -216,45 +217,68 @@ struct Work {  // in the workspace; pairs are (id, token), ids without a row are
   float* part;       // [pieces][2][row]: the sums of the id that came in, and of the one that goes on
 };
 
-__device__ __forceinline__ unsigned key_of(const TbEmbeddingGradArgs& a, long long t) {
-  const long long id = id_of(a.ids, a.ids64, t);
+__device__ __forceinline__ unsigned key_from(const TbEmbeddingGradArgs& a, long long id) {
   if (id >= a.V && a.err) *a.err = 1;
   return id < 0 || id >= a.V ? static_cast<unsigned>(a.V) : static_cast<unsigned>(id);
 }
+__device__ __forceinline__ unsigned key_of(const TbEmbeddingGradArgs& a, long long t) {
+  return key_from(a, id_of(a.ids, a.ids64, t));
+}
 
 // A token's place is the number of tokens with smaller ids, and of earlier ones with the
-// same: 32 tokens per CTA, their comparisons shared by the lanes of 16 warps.
-__global__ void __launch_bounds__(512) compare_sort_kernel(TbEmbeddingGradArgs a, Plan plan, Work work) {
-  extern __shared__ unsigned keys[];  // [N], padded to a multiple of 4 with keys above all
-  __shared__ int place[32];
+// same.  A CTA places `own` tokens (N over the SMs); its threads share each one's
+// comparisons, kSortThreads / own to a token.
+__global__ void __launch_bounds__(kSortThreads) compare_sort_kernel(TbEmbeddingGradArgs a, Plan plan, Work work, int own) {
+  extern __shared__ unsigned keys[];  // [N], padded to a multiple of 4 with keys above all; then [own] places
+  constexpr int U = 8;
   tb::pdl_trigger();
-  const int n4 = (plan.N + 3) / 4 * 4;
-  for (int t = threadIdx.x; t < n4; t += 512) keys[t] = t < plan.N ? key_of(a, t) : 0xffffffffu;
-  if (threadIdx.x < 32) place[threadIdx.x] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) work.owners[0] = 0;
-  __syncthreads();
-  const int t = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
-  const unsigned key = t < plan.N ? keys[t] : 0;
-  const uint4* all = reinterpret_cast<const uint4*>(keys);
-  // four keys at a time; before the CTA's tokens equal ones count, behind them they do not
-  const int first = blockIdx.x * 8, last = first + 8;  // the CTA's own, in fours
-  int n = 0;
-#pragma unroll 4
-  for (int i = warp; i < n4 / 4; i += 16) {
-    const uint4 k = all[i];
-    if (i < first) {
-      n += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
-    } else if (i >= last) {
-      n += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
-    } else {
-      const int u = i * 4;
-      n += (k.x < key || (k.x == key && u < t)) + (k.y < key || (k.y == key && u + 1 < t)) +
-           (k.z < key || (k.z == key && u + 2 < t)) + (k.w < key || (k.w == key && u + 3 < t));
+  const int tid = threadIdx.x, N = plan.N, n4 = (N + 3) / 4;
+  int* place = reinterpret_cast<int*>(keys + n4 * 4);
+  for (int t0 = tid; t0 < n4 * 4; t0 += U * kSortThreads) {
+    long long id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = t0 + u * kSortThreads < N ? id_of(a.ids, a.ids64, t0 + u * kSortThreads) : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * kSortThreads;
+      if (t < n4 * 4) keys[t] = t < N ? key_from(a, id[u]) : 0xffffffffu;
     }
   }
-  atomicAdd(&place[threadIdx.x & 31], n);
+  for (int i = tid; i < own; i += kSortThreads) place[i] = 0;
+  if (blockIdx.x == 0 && tid == 0) work.owners[0] = 0;
   __syncthreads();
-  if (threadIdx.x < 32 && t < plan.N) work.a[place[threadIdx.x]] = make_uint2(key, t);
+  const int slices = kSortThreads / own, slice = tid / own, i = tid - slice * own, first = blockIdx.x * own;
+  const int t = first + i;
+  const bool on = slice < slices && t < N;
+  const unsigned key = on ? keys[t] : 0;
+  if (on) {
+    const uint4* all = reinterpret_cast<const uint4*>(keys);
+    // four keys at a time: equal ones count before the token and not behind it
+    const int lo = static_cast<int>(static_cast<long long>(n4) * slice / slices), hi = static_cast<int>(static_cast<long long>(n4) * (slice + 1) / slices);
+    const int mid = min(max(t / 4, lo), hi);
+    int n = 0;
+#pragma unroll 4
+    for (int k = lo; k < mid; ++k) {
+      const uint4 x = all[k];
+      n += (x.x <= key) + (x.y <= key) + (x.z <= key) + (x.w <= key);
+    }
+    int k = mid;
+    if (k < hi && k == t / 4) {
+      const uint4 x = all[k];
+      const int r = t & 3;
+      n += (x.x < key || (x.x == key && r > 0)) + (x.y < key || (x.y == key && r > 1)) + (x.z < key || (x.z == key && r > 2)) +
+           (x.w < key);
+      ++k;
+    }
+#pragma unroll 4
+    for (; k < hi; ++k) {
+      const uint4 x = all[k];
+      n += (x.x < key) + (x.y < key) + (x.z < key) + (x.w < key);
+    }
+    atomicAdd(&place[i], n);
+  }
+  __syncthreads();
+  if (on && slice == 0) work.a[place[i]] = make_uint2(key, t);
 }
 
 // Counts of the first digit, a block of tokens per CTA.
@@ -308,26 +332,28 @@ __global__ void __launch_bounds__(kSortThreads, 1) scatter_kernel(TbEmbeddingGra
   };
   unsigned* mine = hist + warp * bins;
   uint2 p = make_uint2(0, 0);
-  unsigned peers = 0;
-  for (long long i = lo + lane; i - lane < hi; i += 32) {
-    const bool on = i < hi;
-    if (on) p = pair_at(i);
-    const unsigned d = p.x >> shift & (bins - 1);
-    peers = peers_of(d, on);
-    if (on && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
-    __syncwarp();
-  }
-  // ---- the digit's places over all blocks
+  if (lo + lane < hi) p = pair_at(lo + lane);
+  // ---- the digit's counts in all blocks, and in the ones before (asked for beside the pairs)
   unsigned all = 0, before = 0;
   if (tid < bins) {
     const unsigned* counts = work.counts + pass * plan.blocks * bins + tid;
-#pragma unroll 8
+#pragma unroll 16
     for (int b = 0; b < plan.blocks; ++b) {
       const unsigned c = __ldcg(counts + b * bins);
       if (b < static_cast<int>(blockIdx.x)) before += c;
       all += c;
     }
   }
+  unsigned peers = 0;
+  for (long long i = lo + lane; i - lane < hi; i += 32) {
+    const bool on = i < hi;
+    if (on && i >= lo + 32) p = pair_at(i);
+    const unsigned d = p.x >> shift & (bins - 1);
+    peers = peers_of(d, on);
+    if (on && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+    __syncwarp();
+  }
+  // ---- the digit's places over all blocks
   unsigned incl = all;  // inclusive sum over the digits (threads past the last digit hold 0)
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -570,7 +596,8 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
   __shared__ int count[kWarps], begin[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tb::pdl_wait();
-  const long long tasks = static_cast<long long>(__ldcg(work.owners)) * plan.slabs;
+  const int owners = __ldcg(work.owners);
+  const long long tasks = static_cast<long long>(owners) * plan.slabs;
   const auto sum_of = [&](const Sum& tile, long long first, int n, float (&sum)[M][N]) {
     for (int i = 0; i < n; i += U) {
       float x[U][M][N];
@@ -597,7 +624,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
   for (long long base = blockIdx.x * static_cast<long long>(kWarps); base < tasks; base += gridDim.x * static_cast<long long>(kWarps)) {
     const long long task = base + warp;
     if (task < tasks) {
-      const int c = __ldcg(work.owners + 1 + task / plan.slabs);
+      const int c = __ldcg(work.owners + 1 + task % owners);  // (slabs of one id in different CTAs)
       const unsigned id = __ldcg(work.a + (c + 1ll) * plan.P).x;
       int n = 0;  // pieces that the id comes into
       for (;;) {
@@ -611,7 +638,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
         begin[warp] = c;
       }
       if (n <= kShared) {
-        const Sum tile(a, plan, static_cast<int>(task % plan.slabs));
+        const Sum tile(a, plan, static_cast<int>(task / owners));
         float sum[M][N];
         Sum::zero(sum);
         first_of(tile, c, sum);
@@ -625,7 +652,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
     for (int w = 0; w < kWarps; ++w) {
       const int n = count[w];
       if (n <= kShared) continue;
-      const Sum tile(a, plan, static_cast<int>((base + w) % plan.slabs));
+      const Sum tile(a, plan, static_cast<int>((base + w) / owners));
       const int c = begin[w], lo = static_cast<int>(static_cast<long long>(n) * warp / kWarps);
       const int hi = static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
       float sum[M][N];
@@ -746,7 +773,7 @@ template <typename G>
 cudaError_t fill(const TbEmbeddingGradArgs& a, cudaStream_t s, bool after) {
   const size_t row = a.H * sizeof(G), all = row * a.V;
   if (by_kernel<G>(a))
-    return launch(fill_kernel, 148u * 2, 128u, kFillBytes, s, after, static_cast<char*>(a.grad), static_cast<long long>(all));
+    return launch(fill_kernel, kSms * 2, 128u, kFillBytes, s, after, static_cast<char*>(a.grad), static_cast<long long>(all));
   if (a.ld_grad == a.H || a.V == 1) return cudaMemsetAsync(a.grad, 0, all, s);
   return cudaMemset2DAsync(a.grad, a.ld_grad * sizeof(G), 0, row, a.V, s);
 }
@@ -767,7 +794,8 @@ cudaError_t grad(const TbEmbeddingGradArgs& a, cudaStream_t s) {
   Work work;
   work_of(plan, static_cast<char*>(a.ws), &work);
   if (a.N <= kCompared) {
-    e = launch(compare_sort_kernel, (a.N + 31) / 32, 512u, (a.N + 3) / 4 * 16, s, false, a, plan, work);
+    const int own = (a.N + kSms - 1) / kSms;
+    e = launch(compare_sort_kernel, (a.N + own - 1) / own, kSortThreads, (a.N + 3) / 4 * 16 + own * 4, s, false, a, plan, work, own);
   } else {
     e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&scatter_kernel), kSortWarps * kMaxBins * 4);
     if (e == cudaSuccess) e = launch(count_kernel, plan.blocks, kSortThreads, 0, s, false, a, plan, work);

@@ -9,9 +9,9 @@
 // by (maximum descending, index ascending): for an element outside them, each of those
 // groups holds one that comes before it.  So the selection looks at V / 64 maxima in
 // shared memory and reads some k groups again, whatever the data (all equal, ascending).
-// Both selections search the k-th place by bisection over unique keys (value, index) with
-// counts over the block, and stop at the first threshold that leaves few more than k;
-// what is left is ordered by counting.
+// Both selections search the k-th place by bisection with counts over the block, first of
+// the value and, where too many are equal, of the index, and stop at the first threshold
+// that leaves few more than k; what is left is ordered by counting.
 #include "kernels.h"
 #include "vocab_rows.cuh"
 
@@ -20,76 +20,155 @@ namespace {
 namespace cg = cooperative_groups;
 using tb::Row;
 using tb::SoftSum;
+using tb::Vec;
 
+constexpr int kThreads = 256;
 constexpr int kMaxK = 256;
 constexpr int kIndexBits = 21;  // indexes below 2^20 elements (and the row's offset in its vectors)
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
 constexpr int kRank = 512;  // elements that are ordered by counting
 using Key = unsigned long long;
 
-// Keeps the order of the values; +0 and -0 are equal, NaN is -inf.
-__device__ __forceinline__ uint32_t order_of(float x) {
-  const uint32_t b = __float_as_uint(isnan(x) ? -INFINITY : x + 0.f);
-  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
-}
-// Larger keys come first: larger values, then lower indexes.
-__device__ __forceinline__ Key key_of(uint32_t order, int index) {
-  return (static_cast<Key>(order) << kIndexBits) | (kIndexMask - static_cast<uint32_t>(index));
+__host__ __device__ constexpr int most_groups(int k) { return k + k / 4 + 16; }
+
+// Whole numbers in the order of the values: +0 and -0 are equal, NaN is -inf, 0 is below all.
+template <typename T>
+struct Order;
+template <>
+struct Order<float> {
+  using Type = uint32_t;
+  __device__ __forceinline__ static uint32_t of(float x) {
+    const uint32_t b = __float_as_uint(isnan(x) ? -INFINITY : x + 0.f);
+    return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+  }
+  __device__ __forceinline__ static float value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+};
+template <uint32_t INF>
+struct Order16 {  // INF: the bits of infinity
+  using Type = uint16_t;
+  __device__ __forceinline__ static uint32_t of_bits(uint32_t b) {
+    if ((b & 0x7fffu) > INF) b = 0x8000u | INF;
+    if (b == 0x8000u) b = 0;
+    return b & 0x8000u ? b ^ 0xffffu : b | 0x8000u;
+  }
+  __device__ __forceinline__ static uint32_t bits(uint32_t o) { return o & 0x8000u ? o ^ 0x8000u : o ^ 0xffffu; }
+};
+template <>
+struct Order<__nv_bfloat16> : Order16<0x7f80u> {
+  __device__ __forceinline__ static uint32_t of(float x) { return of_bits(__float_as_uint(x) >> 16); }  // (a bf16 value)
+  __device__ __forceinline__ static float value(uint32_t o) { return __uint_as_float(bits(o) << 16); }
+};
+template <>
+struct Order<__half> : Order16<0x7c00u> {
+  __device__ __forceinline__ static uint32_t of(float x) { return of_bits(__half_as_ushort(__float2half_rn(x))); }
+  __device__ __forceinline__ static float value(uint32_t o) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits(o)))); }
+};
+
+// The orders of a vector's elements, 0 outside the row, and how many are at or above `floor`.
+template <typename T>
+__device__ __forceinline__ uint4 orders_of(const Row<T>& row, int v, const uint4& p, uint32_t floor, int& above) {
+  constexpr int E = Row<T>::E;
+  uint32_t o[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      o[j] = Order<T>::of(__uint_as_float(j == 0 ? p.x : j == 1 ? p.y : j == 2 ? p.z : p.w));
+    } else {
+      const uint32_t w = j < 2 ? p.x : j < 4 ? p.y : j < 6 ? p.z : p.w;
+      o[j] = Order<T>::of_bits(j & 1 ? w >> 16 : w & 0xffffu);
+    }
+  }
+  if (v >= row.v1 || !row.inside(v, v + 1)) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int e = v * E - row.mis + j;
+      if (v >= row.v1 || e < 0 || e >= row.V) o[j] = 0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < E; ++j) above += o[j] >= floor;
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  } else {
+    return make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
+  }
 }
 
 struct Shared {
   Key cand[kRank];
   Key sorted[kMaxK];  // this CTA's own list, read by the others of its cluster
-  float merge[64];
+  float part[2][kThreads / 32];
   float mine[2];
   uint32_t lo, hi;
   int count[3];
   int groups, cands, own;
-  int list[kMaxK + kMaxK / 4 + 16];
+  int list[most_groups(kMaxK)];
 };
 
-__host__ __device__ constexpr int most_groups(int k) { return k + k / 4 + 16; }
-
 // Sum of `c` over the block; `turn` counts the calls.
-__device__ __forceinline__ int block_count(Shared& s, int c, int turn) {
+__device__ __forceinline__ int block_count(Shared& s, int c, int& turn) {
   c = __reduce_add_sync(0xffffffffu, c);
-  if ((threadIdx.x & 31) == 0 && c) atomicAdd(&s.count[turn % 3], c);
+  int* slot = &s.count[turn % 3];
+  if ((threadIdx.x & 31) == 0 && c) atomicAdd(slot, c);
   __syncthreads();
   if (threadIdx.x == 0) s.count[(turn + 2) % 3] = 0;
-  return s.count[turn % 3];
+  ++turn;
+  return *slot;
 }
 
-// A key with at least k and at most `most` of the n orders (index = position, or the
-// element that `index_of` names) at or above it; n >= k.  `order` is in shared memory.
-template <typename IndexOf>
-__device__ Key threshold(Shared& s, const uint32_t* order, int n, int k, int most, Key lo, Key hi, int& turn,
-                         IndexOf index_of) {
-  int at_lo = n;
-  while (at_lo > most && hi - lo > 1) {
-    const Key mid = lo + (hi - lo) / 2;
+// A place in the order (value descending, index ascending): at least k and at most `most`
+// of the n orders in shared memory are at or before it.  n >= k of them are at or above lo,
+// none at or above hi; `index_of` gives the index of position i, ascending or not.
+struct Place {
+  uint32_t order;
+  int index;
+  __device__ __forceinline__ bool takes(uint32_t o, int i) const { return o > order || (o == order && i <= index); }
+};
+template <typename O, typename IndexOf>
+__device__ Place place_of(Shared& s, const O* orders, int n, int k, int most, int at_lo, uint32_t lo, Key hi, int last, int& turn,
+                          IndexOf index_of) {
+  int at_hi = 0;
+  Place p{lo, last};
+  while (at_lo > most && hi - p.order > 1) {
+    const uint32_t mid = p.order + static_cast<uint32_t>((hi - p.order) / 2);
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) c += key_of(order[i], index_of(i)) >= mid;
-    c = block_count(s, c, turn++);
+    for (int i = threadIdx.x; i < n; i += kThreads) c += orders[i] >= mid;
+    c = block_count(s, c, turn);
     if (c >= k) {
-      lo = mid;
+      p.order = mid;
       at_lo = c;
     } else {
       hi = mid;
+      at_hi = c;
     }
   }
-  return lo;
+  int low = -1;  // too many equal ones: the first of them
+  while (at_lo > most && p.index - low > 1) {
+    const int mid = low + (p.index - low) / 2;
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) c += orders[i] == p.order && index_of(i) <= mid;
+    c = block_count(s, c, turn) + at_hi;
+    if (c >= k) {
+      p.index = mid;
+      at_lo = c;
+    } else {
+      low = mid;
+    }
+  }
+  return p;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(512, 2) topk_kernel(TbTopkLogprobsArgs a, float k1) {
+__global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1) {
+  using O = typename Order<T>::Type;
   constexpr int E = Row<T>::E, GE = 8 * E;
-  extern __shared__ uint32_t orders[];  // the groups' maxima, then the chosen groups' elements
+  extern __shared__ uint4 dynamic[];  // the groups' maxima, then the chosen groups' elements, then the cluster's lists
+  O* orders = reinterpret_cast<O*>(dynamic);
   __shared__ Shared s;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ranks = cl.num_blocks();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int k = a.k;
-  int turn = 0;
   for (long long r = blockIdx.x / ranks; r < a.R; r += gridDim.x / ranks) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.V, rank, ranks);
     const int g0 = row.v0 / 8, ng = (row.v1 - row.v0 + 7) / 8;
@@ -99,153 +178,158 @@ __global__ void __launch_bounds__(512, 2) topk_kernel(TbTopkLogprobsArgs a, floa
       s.groups = s.cands = 0;
       s.count[0] = s.count[1] = s.count[2] = 0;
     }
-    __syncthreads();
-    turn = 0;
-    // ---- the pass: a warp takes 32 groups, lane l one vector of groups l / 8, 4 + l / 8, ...
-    SoftSum sum;
+    int turn = 0;
+    // ---- the pass
+    tb::RunningSum<T> running;
     uint32_t olo = 0xffffffffu, ohi = 0;
-    for (int c = row.v0 + warp * 256; c < row.v1; c += nwarps * 256) {
-      float x[8][E], top[8];
+    for (int c = row.v0 + warp * tb::kChunk; c < row.v1; c += kThreads / 32 * tb::kChunk) {
+      uint4 p[8];
+      row.load_chunk(c, p);
+      typename Vec<T>::Max top[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int v = c + i * 32 + lane;
-        if (v < row.v1) {
-          row.load(v, x[i]);
-        } else {
+      for (int i = 0; i < 8; ++i) top[i] = Vec<T>::top(p[i]);
+      typename Vec<T>::Max all = top[0];
 #pragma unroll
-          for (int j = 0; j < E; ++j) x[i][j] = -INFINITY;
-        }
-      }
-      float all = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        top[i] = x[i][0];
-#pragma unroll
-        for (int j = 1; j < E; ++j) top[i] = fmaxf(top[i], x[i][j]);
-        all = fmaxf(all, top[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum.add(x[i], all, k1);
-      // maxima over eight lanes of eight vectors: lane l ends with those of vector l % 8
+      for (int i = 1; i < 8; ++i) all = Vec<T>::max(all, top[i]);
+      running.add(p, Vec<T>::value(all), k1);
+      // maxima over eight lanes of eight vectors: lane l ends with those of its vector l % 8
 #pragma unroll
       for (int h = 4; h > 0; h >>= 1) {
         const bool up = lane & h;
 #pragma unroll
         for (int i = 0; i < h; ++i) {
-          const float send = up ? top[i] : top[i + h], keep = up ? top[i + h] : top[i];
-          top[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, h));
+          const auto send = up ? top[i] : top[i + h], keep = up ? top[i + h] : top[i];
+          top[i] = Vec<T>::max(keep, __shfl_xor_sync(0xffffffffu, send, h));
         }
       }
       const int g = c / 8 - g0 + (lane & 7) * 4 + lane / 8;
       if (g < ng) {
-        const uint32_t o = order_of(top[0]);
-        orders[g] = o;
+        const uint32_t o = Order<T>::of(Vec<T>::value(top[0]));
+        orders[g] = static_cast<O>(o);
         olo = min(olo, o);
         ohi = max(ohi, o);
       }
     }
+    SoftSum sum = running.done(k1);
+    sum.merge_lanes(k1);
     olo = __reduce_min_sync(0xffffffffu, olo);
     ohi = __reduce_max_sync(0xffffffffu, ohi);
+    __syncthreads();
     if (lane == 0) {
+      s.part[0][warp] = sum.m;
+      s.part[1][warp] = sum.s;
       atomicMin(&s.lo, olo);
       atomicMax(&s.hi, ohi);
     }
-    sum = tb::block_merge(sum, k1, s.merge);  // (synchronises)
+    __syncthreads();
+    sum.m = lane < kThreads / 32 ? s.part[0][lane] : -INFINITY;
+    sum.s = lane < kThreads / 32 ? s.part[1][lane] : 0.f;
+    sum.merge_lanes(k1);
     // ---- the first k groups, and a few more
-    uint32_t floor_order = 0;
-    const uint32_t last = s.hi;
+    uint32_t floor = 1;
+    const Key above_all = static_cast<Key>(s.hi) + 1;
     if (ng > k) {
-      const Key t = threshold(s, orders, ng, k, most_groups(k), static_cast<Key>(s.lo) << kIndexBits,
-                              static_cast<Key>(last + 1ull) << kIndexBits, turn, [](int i) { return i; });
-      floor_order = static_cast<uint32_t>(t >> kIndexBits);  // k elements are at or above it
-      for (int i = threadIdx.x; i < ng; i += blockDim.x)
-        if (key_of(orders[i], i) >= t) s.list[atomicAdd(&s.groups, 1)] = i;
+      const Place t = place_of(s, orders, ng, k, most_groups(k), ng, s.lo, above_all, ng - 1, turn, [](int i) { return i; });
+      floor = t.order;  // k elements are at or above it
+      for (int i = threadIdx.x; i < ng; i += kThreads)
+        if (t.takes(orders[i], i)) s.list[atomicAdd(&s.groups, 1)] = i;
     } else {
-      for (int i = threadIdx.x; i < ng; i += blockDim.x) s.list[i] = i;
+      for (int i = threadIdx.x; i < ng; i += kThreads) s.list[i] = i;
       if (threadIdx.x == 0) s.groups = ng;
     }
     __syncthreads();
     // ---- their elements
     const int groups = s.groups, n = groups * GE;
     int above = 0;
-    for (int i = threadIdx.x; i < groups * 8; i += blockDim.x) {
-      const int v = (g0 + s.list[i >> 3]) * 8 + (i & 7);
-      float x[E];
-      if (v < row.v1) {
-        row.load(v, x);
-      } else {
+    for (int i0 = threadIdx.x; i0 < groups * 8; i0 += 4 * kThreads) {
+      uint4 p[4];
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = -INFINITY;
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kThreads;
+        if (i < groups * 8) p[u] = row.load((g0 + s.list[i >> 3]) * 8 + (i & 7));
       }
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int e = v * E - row.mis + j;  // outside the row: 0, below every order
-        const uint32_t o = e >= 0 && e < a.V ? order_of(x[j]) : 0;
-        orders[i * E + j] = o;
-        above += o >= max(floor_order, 1u);
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kThreads;
+        if (i < groups * 8) dynamic[i] = orders_of(row, (g0 + s.list[i >> 3]) * 8 + (i & 7), p[u], floor, above);
       }
     }
-    const auto element = [&](int i) {
-      return (g0 + s.list[i / GE]) * GE + i % GE - row.mis;
-    };
-    above = block_count(s, above, turn++);
+    const auto element = [&](int i) { return (g0 + s.list[i / GE]) * GE + i % GE - row.mis; };
+    above = block_count(s, above, turn);
     const int own = min(k, above);  // (fewer than k: a short part of a row)
-    Key t = static_cast<Key>(max(floor_order, 1u)) << kIndexBits;
-    if (above > kRank) {
-      t = threshold(s, orders, n, own, kRank, t, static_cast<Key>(last + 1ull) << kIndexBits, turn,
-                    [&](int i) { return max(element(i), 0); });
-    }
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      if (orders[i] == 0) continue;
-      const Key x = key_of(orders[i], element(i));
-      if (x >= t) s.cand[atomicAdd(&s.cands, 1)] = x;
+    Place t{floor, 0x7fffffff};
+    if (above > kRank) t = place_of(s, orders, n, own, kRank, above, floor, above_all, a.V, turn, element);
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint32_t o = orders[i];
+      if (o < t.order) continue;
+      const int e = element(i);
+      if (t.takes(o, e)) s.cand[atomicAdd(&s.cands, 1)] = static_cast<Key>(o) << kIndexBits | (kIndexMask - static_cast<uint32_t>(e));
     }
     __syncthreads();
     const int cands = s.cands;
-    for (int i = threadIdx.x; i < cands; i += blockDim.x) {
+    for (int i = threadIdx.x; i < cands; i += kThreads) {
       const Key x = s.cand[i];
       int place = 0;
+#pragma unroll 8
       for (int j = 0; j < cands; ++j) place += s.cand[j] > x;
       if (place < own) s.sorted[place] = x;
     }
-    if (threadIdx.x == 0) s.own = own;
+    if (ranks > 1) {
+      if (threadIdx.x == 0) {
+        s.own = own;
+        s.mine[0] = sum.m;
+        s.mine[1] = sum.s;
+      }
+      cl.sync();
+      // ---- the cluster's sums, and its lists side by side
+      SoftSum whole;
+      for (int o = 0; o < ranks; ++o) {
+        const float* m = cl.map_shared_rank(s.mine, o);
+        whole.merge(m[0], m[1], k1);
+      }
+      sum = whole;
+      Key* lists = reinterpret_cast<Key*>(dynamic);
+      for (int i = threadIdx.x; i < ranks * k; i += kThreads) {
+        const int o = i / k, j = i - o * k;
+        lists[i] = j < *cl.map_shared_rank(&s.own, o) ? cl.map_shared_rank(s.sorted, o)[j] : 0;
+      }
+    }
     __syncthreads();
-    // ---- the cluster's lists joined: a place is the sum of the places in every list
-    sum = tb::cluster_merge(sum, k1, s.mine);
-    const double inv_t = 1.0 / a.temperature, lns = log(static_cast<double>(sum.s));
+    // ---- a place is the sum of the places in every list
+    const double inv_t = 1.0 / a.temperature;
+    const bool plain = !isinf(sum.m) && !isnan(sum.s);
+    const double lns = plain ? tb::log_of(sum.s) : 0.0;
     if (rank == 0 && threadIdx.x == 0)
-      a.lse[r] = isinf(sum.m) && !isnan(sum.s) ? sum.m : static_cast<float>(sum.m * inv_t + lns);
-    for (int i = threadIdx.x; i < own; i += blockDim.x) {
+      a.lse[r] = plain ? static_cast<float>(sum.m * inv_t + lns) : isnan(sum.s) ? NAN : sum.m;
+    for (int i = threadIdx.x; i < own; i += kThreads) {
       const Key x = s.sorted[i];
       int place = i;
-      for (int o = 0; o < ranks; ++o) {
-        if (o == rank) continue;
-        const Key* theirs = cl.map_shared_rank(s.sorted, o);
-        int lo = 0, hi = *cl.map_shared_rank(&s.own, o);
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (theirs[mid] > x) {
-            lo = mid + 1;
-          } else {
-            hi = mid;
+      if (ranks > 1) {
+        const Key* lists = reinterpret_cast<const Key*>(dynamic);
+        for (int o = 0; o < ranks; ++o) {
+          if (o == rank) continue;
+          int lo = 0, hi = k;
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (lists[o * k + mid] > x) {
+              lo = mid + 1;
+            } else {
+              hi = mid;
+            }
           }
+          place += lo;
         }
-        place += lo;
+        if (place >= k) continue;
       }
-      if (place >= k) continue;
-      const int e = static_cast<int>(kIndexMask - (static_cast<uint32_t>(x) & kIndexMask));
-      // the element's own value (the order has NaN as -inf)
-      const float z = tb::to_f32(row.row[e]);
+      const float z = Order<T>::value(static_cast<uint32_t>(x >> kIndexBits));
       float y;
-      if (isnan(sum.s)) {
-        y = NAN;
-      } else if (isinf(sum.m)) {
-        y = sum.m > 0 && z == sum.m ? NAN : -INFINITY;
-      } else {
+      if (plain) {
         y = static_cast<float>((static_cast<double>(z) - sum.m) * inv_t - lns);
+      } else {
+        y = isnan(sum.s) || (sum.m > 0 && z == sum.m) ? NAN : -INFINITY;
       }
       a.logp[r * k + place] = y;
-      a.ids[r * k + place] = e;
+      a.ids[r * k + place] = static_cast<int>(kIndexMask - (static_cast<uint32_t>(x) & kIndexMask));
     }
     if (ranks > 1) {
       cl.sync();
@@ -255,21 +339,28 @@ __global__ void __launch_bounds__(512, 2) topk_kernel(TbTopkLogprobsArgs a, floa
   }
 }
 
+// CTAs of a cluster: as many as the machine has room for beside the other rows, a chunk at
+// least to each; enough of them that the maxima of a part fit its shared memory.
+int ranks_of(int R, int groups) {
+  int ranks = 1;
+  while (ranks < 8 && ((groups + ranks - 1) / ranks > 8192 || (R * 2ll * ranks <= 148 * 4 && groups >= 64 * ranks))) ranks *= 2;
+  return ranks;
+}
+
 template <typename T>
 cudaError_t launch(const TbTopkLogprobsArgs& a, cudaStream_t stream) {
   constexpr int E = Row<T>::E;
-  const int groups = (a.V + E - 2 + 8 * E) / (8 * E);
-  int ranks = 1;
-  while (ranks < 8 && (groups + ranks - 1) / ranks > 8192) ranks *= 2;
-  const int per = (groups + ranks - 1) / ranks;
-  const int chosen = (per > a.k ? (per < most_groups(a.k) ? per : most_groups(a.k)) : per) * 8 * E;
-  const size_t smem = sizeof(uint32_t) * static_cast<size_t>(per > chosen ? per : chosen);
-  cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&topk_kernel<T>), 128 * 1024);
+  using O = typename Order<T>::Type;
+  const int groups = (a.V + E - 2 + 8 * E) / (8 * E), ranks = ranks_of(a.R, groups), per = (groups + ranks - 1) / ranks;
+  const int chosen = per > a.k && per > most_groups(a.k) ? most_groups(a.k) : per;
+  size_t smem = sizeof(O) * static_cast<size_t>(per > chosen * 8 * E ? per : chosen * 8 * E);
+  if (ranks > 1 && smem < ranks * a.k * sizeof(Key)) smem = ranks * a.k * sizeof(Key);
+  cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&topk_kernel<T>), 64 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   const int rows = a.R < (1 << 20) ? a.R : 1 << 20;
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * ranks);
-  cfg.blockDim = dim3(512);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
