@@ -32,6 +32,7 @@ using tb::Vec;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxList = kThreads;  // a thread for each entry
+constexpr int kSlots = 148 * 4;  // CTAs that the machine holds
 constexpr double kRestMin = 1.0 / (1 << 20);
 enum { kLoss, kBoth, kGrad };  // what a launch computes (kGrad: from the numbers that kLoss kept)
 
@@ -61,7 +62,7 @@ struct Entry {
 };
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, float k1, int part) {
+__global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, float k1, double inv_t, int part) {
   constexpr int E = Row<T>::E;
   extern __shared__ uint4 dynamic[];  // [part]: a byte for each vector of this CTA's part, its elements in the list
   unsigned char* bytes = reinterpret_cast<unsigned char*>(dynamic);
@@ -70,8 +71,6 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, f
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ranks = cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
-  const double inv_t = 1.0 / a.temperature;
-  bool clear = false;
   for (long long r = blockIdx.x / ranks; r < a.R; r += gridDim.x / ranks) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.V, rank, ranks);
     T* grad = MODE == kLoss ? nullptr : static_cast<T*>(a.grad) + r * a.ld_grad;
@@ -138,10 +137,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, f
     };
     Numbers n;
     if (MODE != kGrad) {
-      if (!clear) {
-        for (int i = tid; i < part; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
-        clear = true;
-      }
+      for (int i = tid; i < part; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
       const uint32_t bit = here ? 1u << ((at / E - row.v0) % 4 * 8 + at % E) : 0;
       uint32_t* word = bits + (here ? (at / E - row.v0) / 4 : 0);
@@ -196,7 +192,6 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, f
         in.merge(s.part[2][i], s.part[3][i], k1);
         mass += s.mass[i];
       }
-      if (here) *word = 0;  // for the next row
       int twice = s.twice;
       if (ranks > 1) {
         if (tid == 0) {
@@ -359,10 +354,16 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, f
 }
 
 // CTAs of a cluster: as many as the machine has room for beside the other rows, a chunk at
-// least to each; enough of them that a part's bitmap fits its shared memory.
-int ranks_of(int R, int groups) {
+// least to each; enough of them that a part's bitmap fits its shared memory; and, where rows
+// are read twice, that the rows in work fit the L2 cache beside what is written.
+int ranks_of(int R, int groups, bool twice) {
+  const auto more = [&](int ranks) {
+    if ((groups + ranks - 1) / ranks > 4096) return true;
+    if (groups < 64 * ranks) return false;
+    return R * 2ll * ranks <= kSlots || (twice && static_cast<long long>(min(R, kSlots / ranks)) * groups * 128 > (48 << 20));
+  };
   int ranks = 1;
-  while (ranks < 8 && ((groups + ranks - 1) / ranks > 4096 || (R * 2ll * ranks <= 148 * 4 && groups >= 64 * ranks))) ranks *= 2;
+  while (ranks < 8 && more(ranks)) ranks *= 2;
   return ranks;
 }
 
@@ -370,12 +371,12 @@ template <typename T, int MODE>
 cudaError_t launch(const TbDistillArgs& a, cudaStream_t stream) {
   constexpr int E = Row<T>::E;
   const int groups = (a.V + E - 2 + 8 * E) / (8 * E);
-  const int ranks = ranks_of(a.R, groups);
+  const int ranks = ranks_of(a.R, groups, MODE == kBoth);
   const size_t smem = MODE == kGrad ? 0 : (static_cast<size_t>((groups + ranks - 1) / ranks) * 8 + 15) / 16 * 16;
   cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&distill_kernel<T, MODE>), 64 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  const int slots = 148 * 4 / ranks, rows = a.R < slots ? a.R : slots;
+  const int rows = a.R < (1 << 20) ? a.R : 1 << 20;
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * ranks);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
@@ -387,7 +388,7 @@ cudaError_t launch(const TbDistillArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE>, a, static_cast<float>(tb::kLog2e / a.temperature),
-                            static_cast<int>(smem / 16));
+                            1.0 / a.temperature, static_cast<int>(smem / 16));
 }
 
 template <typename T>

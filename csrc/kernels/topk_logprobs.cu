@@ -9,9 +9,10 @@
 // by (maximum descending, index ascending): for an element outside them, each of those
 // groups holds one that comes before it.  So the selection looks at V / 64 maxima in
 // shared memory and reads some k groups again, whatever the data (all equal, ascending).
-// Both selections search the k-th place by bisection with counts over the block, first of
-// the value and, where too many are equal, of the index, and stop at the first threshold
-// that leaves few more than k; what is left is ordered by counting.
+// A histogram of the maxima, filled during the pass, gives a value that k groups reach and
+// few more; of those groups the elements that reach it, some k, are ordered by counting.
+// Where too many do (equal values, the largest side by side), the k-th place is searched by
+// bisection with counts over the block, first of the value and then of the index.
 #include "kernels.h"
 #include "vocab_rows.cuh"
 
@@ -27,6 +28,7 @@ constexpr int kMaxK = 256;
 constexpr int kIndexBits = 21;  // indexes below 2^20 elements (and the row's offset in its vectors)
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
 constexpr int kRank = 512;  // elements that are ordered by counting
+constexpr int kBins = 16384;  // of the histogram, two to a word
 using Key = unsigned long long;
 
 __host__ __device__ constexpr int most_groups(int k) { return k + k / 4 + 16; }
@@ -159,16 +161,20 @@ __device__ Place place_of(Shared& s, const O* orders, int n, int k, int most, in
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1) {
+__global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1, double inv_t) {
   using O = typename Order<T>::Type;
   constexpr int E = Row<T>::E, GE = 8 * E;
   extern __shared__ uint4 dynamic[];  // the groups' maxima, then the chosen groups' elements, then the cluster's lists
   O* orders = reinterpret_cast<O*>(dynamic);
   __shared__ Shared s;
+  __shared__ uint4 hist4[kBins / 8];
+  uint32_t* hist = reinterpret_cast<uint32_t*>(hist4);
+  constexpr int kShift = sizeof(T) == 2 ? 2 : 18;  // orders of a bin
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ranks = cl.num_blocks();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int k = a.k;
+  for (int i = threadIdx.x; i < kBins / 8; i += kThreads) hist4[i] = make_uint4(0, 0, 0, 0);
   for (long long r = blockIdx.x / ranks; r < a.R; r += gridDim.x / ranks) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.V, rank, ranks);
     const int g0 = row.v0 / 8, ng = (row.v1 - row.v0 + 7) / 8;
@@ -178,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
       s.groups = s.cands = 0;
       s.count[0] = s.count[1] = s.count[2] = 0;
     }
+    __syncthreads();
     int turn = 0;
     // ---- the pass
     tb::RunningSum<T> running;
@@ -206,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
       if (g < ng) {
         const uint32_t o = Order<T>::of(Vec<T>::value(top[0]));
         orders[g] = static_cast<O>(o);
+        atomicAdd(&hist[o >> (kShift + 1)], 1u << (o >> kShift & 1) * 16);
         olo = min(olo, o);
         ohi = max(ohi, o);
       }
@@ -214,7 +222,6 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     sum.merge_lanes(k1);
     olo = __reduce_min_sync(0xffffffffu, olo);
     ohi = __reduce_max_sync(0xffffffffu, ohi);
-    __syncthreads();
     if (lane == 0) {
       s.part[0][warp] = sum.m;
       s.part[1][warp] = sum.s;
@@ -225,48 +232,95 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     sum.m = lane < kThreads / 32 ? s.part[0][lane] : -INFINITY;
     sum.s = lane < kThreads / 32 ? s.part[1][lane] : 0.f;
     sum.merge_lanes(k1);
-    // ---- the first k groups, and a few more
+    // ---- the first k groups, and a few more: from the highest bin down (each warp for itself)
     uint32_t floor = 1;
     const Key above_all = static_cast<Key>(s.hi) + 1;
+    Place t{1, 0x7fffffff};
     if (ng > k) {
-      const Place t = place_of(s, orders, ng, k, most_groups(k), ng, s.lo, above_all, ng - 1, turn, [](int i) { return i; });
+      int at = 0;  // groups in the words above
+      int word = static_cast<int>(s.hi >> (kShift + 1));
+      for (;; word -= 32) {
+        const uint32_t h = word - lane >= 0 ? hist[word - lane] : 0;
+        const int c = (h >> 16) + (h & 0xffffu);
+        int incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
+        }
+        const unsigned enough = __ballot_sync(0xffffffffu, at + incl >= k);
+        if (!enough) {
+          at += __shfl_sync(0xffffffffu, incl, 31);
+          continue;
+        }
+        const int l = __ffs(enough) - 1;
+        const int before = at + __shfl_sync(0xffffffffu, incl - c, l);
+        const uint32_t w = __shfl_sync(0xffffffffu, h, l);
+        const bool upper = before + static_cast<int>(w >> 16) >= k;
+        floor = static_cast<uint32_t>((word - l) * 2 + (upper ? 1 : 0)) << kShift;
+        at = before + static_cast<int>(w >> 16) + (upper ? 0 : static_cast<int>(w & 0xffffu));
+        break;
+      }
+      floor = max(floor, 1u);
+      t.order = floor;
+      if (at > most_groups(k)) t = place_of(s, orders, ng, k, most_groups(k), at, floor, above_all, ng - 1, turn, [](int i) { return i; });
       floor = t.order;  // k elements are at or above it
-      for (int i = threadIdx.x; i < ng; i += kThreads)
-        if (t.takes(orders[i], i)) s.list[atomicAdd(&s.groups, 1)] = i;
-    } else {
-      for (int i = threadIdx.x; i < ng; i += kThreads) s.list[i] = i;
-      if (threadIdx.x == 0) s.groups = ng;
     }
+    for (int i = threadIdx.x; i < ng; i += kThreads)
+      if (t.takes(orders[i], i)) s.list[atomicAdd(&s.groups, 1)] = i;
     __syncthreads();
-    // ---- their elements
-    const int groups = s.groups, n = groups * GE;
-    int above = 0;
+    // ---- their elements at or above it
+    const int groups = s.groups;
+    const auto vector_of = [&](int i) { return (g0 + s.list[i >> 3]) * 8 + (i & 7); };
+    const auto push = [&](uint32_t o, int e) {
+      const int at = atomicAdd(&s.cands, 1);
+      if (at < kRank) s.cand[at] = static_cast<Key>(o) << kIndexBits | (kIndexMask - static_cast<uint32_t>(e));
+    };
     for (int i0 = threadIdx.x; i0 < groups * 8; i0 += 4 * kThreads) {
       uint4 p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kThreads;
-        if (i < groups * 8) p[u] = row.load((g0 + s.list[i >> 3]) * 8 + (i & 7));
-      }
+      for (int u = 0; u < 4; ++u) p[u] = i0 + u * kThreads < groups * 8 ? row.load(vector_of(i0 + u * kThreads)) : Row<T>::lowest();
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * kThreads;
-        if (i < groups * 8) dynamic[i] = orders_of(row, (g0 + s.list[i >> 3]) * 8 + (i & 7), p[u], floor, above);
+        if (i >= groups * 8 || Order<T>::of(Vec<T>::value(Vec<T>::top(p[u]))) < floor) continue;
+        const int v = vector_of(i);
+        int above = 0;
+        const uint4 q = orders_of(row, v, p[u], floor, above);
+        if (above) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const uint32_t word = j / (E / 4) == 0 ? q.x : j / (E / 4) == 1 ? q.y : j / (E / 4) == 2 ? q.z : q.w;
+            const uint32_t o = sizeof(T) == 4 ? word : j & 1 ? word >> 16 : word & 0xffffu;
+            if (o >= floor) push(o, v * E - row.mis + j);
+          }
+        }
       }
     }
-    const auto element = [&](int i) { return (g0 + s.list[i / GE]) * GE + i % GE - row.mis; };
-    above = block_count(s, above, turn);
-    const int own = min(k, above);  // (fewer than k: a short part of a row)
-    Place t{floor, 0x7fffffff};
-    if (above > kRank) t = place_of(s, orders, n, own, kRank, above, floor, above_all, a.V, turn, element);
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint32_t o = orders[i];
-      if (o < t.order) continue;
-      const int e = element(i);
-      if (t.takes(o, e)) s.cand[atomicAdd(&s.cands, 1)] = static_cast<Key>(o) << kIndexBits | (kIndexMask - static_cast<uint32_t>(e));
-    }
     __syncthreads();
-    const int cands = s.cands;
+    int cands = s.cands;
+    const int own = min(k, cands);  // (fewer than k: a short part of a row)
+    if (cands > kRank) {  // ---- too many: all the groups' elements in shared memory, and the first `own` of them
+      const int n = groups * GE;
+      int above = 0;
+      for (int i = threadIdx.x; i < groups * 8; i += kThreads) {
+        const int v = vector_of(i);
+        dynamic[i] = orders_of(row, v, row.load(v), floor, above);
+      }
+      __syncthreads();
+      const auto element = [&](int i) { return (g0 + s.list[i / GE]) * GE + i % GE - row.mis; };
+      const Place e = place_of(s, orders, n, own, kRank, cands, floor, above_all, a.V, turn, element);
+      if (threadIdx.x == 0) s.cands = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint32_t o = orders[i];
+        if (o >= e.order && e.takes(o, element(i))) push(o, element(i));
+      }
+      __syncthreads();
+      cands = s.cands;
+    }
+    // the bins that were in use, for the next row
+    for (int i = static_cast<int>(s.lo >> (kShift + 1)) + threadIdx.x; i <= static_cast<int>(s.hi >> (kShift + 1)); i += kThreads) hist[i] = 0;
     for (int i = threadIdx.x; i < cands; i += kThreads) {
       const Key x = s.cand[i];
       int place = 0;
@@ -296,7 +350,6 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     }
     __syncthreads();
     // ---- a place is the sum of the places in every list
-    const double inv_t = 1.0 / a.temperature;
     const bool plain = !isinf(sum.m) && !isnan(sum.s);
     const double lns = plain ? tb::log_of(sum.s) : 0.0;
     if (rank == 0 && threadIdx.x == 0)
@@ -369,7 +422,8 @@ cudaError_t launch(const TbTopkLogprobsArgs& a, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, topk_kernel<T>, a, static_cast<float>(tb::kLog2e / a.temperature));
+  return cudaLaunchKernelEx(&cfg, topk_kernel<T>, a, static_cast<float>(tb::kLog2e / a.temperature),
+                            1.0 / a.temperature);
 }
 
 }  // namespace
