@@ -189,7 +189,7 @@ Opt distill_loss(const at::Tensor& logits, const at::Tensor& ids, const at::Tens
   return loss_of(a, logits, logprobs, nullptr);
 }
 
-// The differentiable form (CUDA tensors).  The forward pass keeps eight numbers per
+// The differentiable form (CUDA tensors).  The forward pass keeps a few numbers per
 // row; the backward pass reads the logits again.
 struct DistillFunction : torch::autograd::Function<DistillFunction> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids,

@@ -17,9 +17,11 @@
 //
 // The pass over the row leaves the elements of S out (a bitmap in shared memory, a byte
 // per vector), so that p_R is a sum of its own terms and not a difference from 1; the
-// elements of S join afterwards, a thread to each.  A second pass writes the gradient, then
-// the elements of S are written over.  Numbers of the row (logarithms, t_R, KL) are formed
-// in 64 bits: the loss is a small difference of large ones.
+// elements of S join afterwards.  A second pass writes the gradient, then the elements of S
+// are written over.  Where both passes are one launch, the second finds most of the row in
+// the L2 cache, by the policy that the first one read it with.  Masses are summed in 64 bits
+// (t_R is 1 less their sum), and log S is kept as the sum of two fp32 numbers: the loss is a
+// small difference of large ones.
 #include "kernels.h"
 #include "vocab_rows.cuh"
 
@@ -30,356 +32,378 @@ using tb::Row;
 using tb::SoftSum;
 using tb::Vec;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxList = kThreads;  // a thread for each entry
-constexpr int kSlots = 148 * 4;  // CTAs that the machine holds
+constexpr int kMaxList = 256;  // (a thread for each entry)
+constexpr int kMaxWarps = 16;
+constexpr int kLane = 8;  // vectors of a lane at a time
 constexpr double kRestMin = 1.0 / (1 << 20);
 enum { kLoss, kBoth, kGrad };  // what a launch computes (kGrad: from the numbers that kLoss kept)
 
-struct Shared {
-  float part[4][kWarps];
-  double mass[kWarps], term[kWarps];
-  float mine[2];
-  int twice;     // an id of this CTA's part occurs twice in the list
-  int y_listed;  // the target is in the list
-  int id[kMaxList];
-  float l[kMaxList];
-};
-
-// What a row's passes share, the same in all threads.
+// What a row's passes share.
 struct Numbers {
   float origin, factor;  // the gradient outside the list: factor x 2^((z - origin) k1)
-  float top, lns;        // log p = (z - top) / T - lns
-  float kl, whole;       // whole: sum t + t_R
-  float mass;            // sum t as listed
+  float top;
+  float2 lns;       // log p = (z - top) / T - lns
+  float kl, whole;  // whole: sum t + t_R
 };
 
-// The entry of a list that a thread has.
-struct Entry {
-  int id = -1;  // -1: padding, or not the id's first entry
-  float z = 0.f, l = 0.f;
-  double t = 0.0, lt = 0.0;  // mass of the class, and its logarithm
+// The weights of the KL and of the target, and the target (-1: none).
+struct Weights {
+  float w, c;
+  int y;
+  bool bad;  // a target past the vocabulary
+  __device__ __forceinline__ Weights(const TbDistillArgs& a, float w_, float c_, int y_) : w(w_), c(y_ < 0 ? 0.f : c_), y(y_) {
+    bad = y >= a.V && live();
+    if (y >= a.V) {
+      y = -1;
+      c = 0.f;
+    }
+  }
+  __device__ __forceinline__ bool live() const { return w != 0.f || c != 0.f; }
 };
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads, 4) distill_kernel(TbDistillArgs a, float k1, double inv_t, int part) {
-  constexpr int E = Row<T>::E;
+struct Shared {
+  float part[2][kMaxWarps];
+  float mine[2][2];  // of rows in turn, read by the others of the cluster
+  Numbers n;
+  // the row's weights and list: what lives over the passes is here, not in registers
+  float w, c, z_y;
+  int y, y_listed, twice;
+  __align__(16) int id[kMaxList];  // -1: padding
+  float z[kMaxList], l[kMaxList];
+  double t[kMaxList];  // mass of the class; -1 where the entry is not its id's first
+  // the softmax sum of the list's elements, the masses' sum, t_R, and their logarithms
+  float in_m, in_s;
+  float mass, log_mass, t_rest, log_t_rest;
+};
+
+// Warp 0: the list's sums.
+__device__ __forceinline__ void list_sums(const TbDistillArgs& a, Shared& s, float k1) {
+  const int lane = threadIdx.x & 31;
+  SoftSum in;
+  double mass = 0.0;
+  for (int k = lane; k < a.K; k += 32) {
+    if (s.id[k] < 0 || s.t[k] < 0.0) continue;
+    const float x = s.z[k];
+    in.merge(isnan(x) ? -INFINITY : x, isnan(x) ? NAN : 1.f, k1);
+    mass += s.t[k];
+  }
+  in.merge_lanes(k1);
+  mass = tb::warp_sum(mass);
+  if (lane) return;
+  s.in_m = in.m;
+  s.in_s = in.s;
+  s.mass = static_cast<float>(mass);
+  s.log_mass = a.kind == TB_DISTILL_FORWARD && s.mass != 0.f ? logf(s.mass) : 0.f;
+  const double t = fmax(1.0 - mass, a.kind == TB_DISTILL_REVERSE ? kRestMin : 0.0);
+  s.t_rest = isnan(mass) ? NAN : static_cast<float>(t);
+  s.log_t_rest = s.t_rest > 0.f ? logf(s.t_rest) : 0.f;
+}
+
+// Warp 0, when the row's sums are known: the loss, and what the gradient needs.
+__device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, long long r, const SoftSum& sum, float k1, float inv_t,
+                                           bool write) {
+  const int lane = threadIdx.x & 31;
+  const float w = s.w, c = s.c;
+  const bool listed = w != 0.f, twice = s.twice;
+  SoftSum all = sum;
+  all.merge(s.in_m, s.in_s, k1);
+  const bool good = !isnan(all.s) && !isinf(all.m);
+  const float2 lns = good ? tb::log_of(all.s) : make_float2(0.f, 0.f);
+  const tb::Scaled log_p{inv_t};
+  // log p of the elements outside; none there: their terms are left out
+  const bool none = sum.m == -INFINITY || !good;
+  float lp_rest = 0.f, p_rest = 0.f;
+  if (!none) {
+    const float2 l = tb::log_of(sum.s);
+    lp_rest = fmaf(sum.m - all.m, inv_t, l.x - lns.x) + (l.y - lns.y);
+    p_rest = tb::ex2(lp_rest * static_cast<float>(tb::kLog2e));
+  }
+  float kl = 0.f, h = 0.f, whole = 1.f;  // h: factor of q_j outside the list
+  if (listed) {
+    for (int k = lane; k < a.K; k += 32) {
+      const float t = static_cast<float>(s.t[k]);
+      if (s.id[k] < 0 || t < 0.f) continue;
+      const float lp = log_p(s.z[k], all.m, lns);
+      const float lt = (twice ? logf(t) : s.l[k]) - s.log_mass;
+      if (a.kind == TB_DISTILL_REVERSE) {
+        const float p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
+        if (p != 0.f) kl += p * (lp - lt);
+      } else if (t != 0.f) {
+        kl += (a.kind == TB_DISTILL_FORWARD ? t / s.mass : t) * (lt - lp);
+      }
+    }
+    kl = tb::warp_sum(kl);
+    if (a.kind == TB_DISTILL_FORWARD) {
+      whole = s.mass != 0.f ? 1.f : 0.f;
+      h = whole * p_rest;
+    } else if (a.kind == TB_DISTILL_FORWARD_REST) {
+      const float t_out = none ? 0.f : s.t_rest;
+      if (t_out > 0.f) kl += t_out * (s.log_t_rest - lp_rest);
+      whole = s.mass + t_out;
+      h = whole * p_rest - t_out;
+    } else {
+      const float f_rest = none ? 0.f : lp_rest - s.log_t_rest;
+      if (p_rest != 0.f) kl += p_rest * f_rest;
+      if (p_rest != 0.f) h = p_rest * (f_rest - kl);
+    }
+  }
+  if (lane) return;
+  const tb::Exponent ex(sum.m, k1);
+  const float f = (listed ? w * h : 0.f) + (c != 0.f ? c * p_rest : 0.f);
+  const float factor = !good ? NAN : none ? 0.f : f * inv_t / sum.s * ex.fix;
+  s.n = {ex.m, factor, all.m, good ? lns : make_float2(NAN, NAN), kl, whole};
+  if (!write) return;
+  a.loss[r] = good ? (listed ? w * kl : 0.f) + (c != 0.f ? -c * log_p(s.z_y, all.m, lns) : 0.f) : NAN;
+  if (a.stats) {
+    float4* st = reinterpret_cast<float4*>(a.stats + r * TB_DISTILL_STATS);
+    st[0] = make_float4(s.n.origin, s.n.factor, s.n.top, s.n.lns.x);
+    st[1] = make_float4(s.n.lns.y, s.n.kl, s.n.whole, s.mass);
+    st[2] = make_float4(twice ? 1.f : 0.f, 0.f, 0.f, 0.f);
+  }
+}
+
+template <typename T, int MODE, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDistillArgs a, float k1, float inv_t, int part) {
+  constexpr int E = Row<T>::E, kWarps = kThreads / 32, kStep = kLane * 32;
   extern __shared__ uint4 dynamic[];  // [part]: a byte for each vector of this CTA's part, its elements in the list
   unsigned char* bytes = reinterpret_cast<unsigned char*>(dynamic);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(dynamic);
   __shared__ Shared s;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ranks = cl.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
+  int live = 0;  // live rows so far
   for (long long r = blockIdx.x / ranks; r < a.R; r += gridDim.x / ranks) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.V, rank, ranks);
     T* grad = MODE == kLoss ? nullptr : static_cast<T*>(a.grad) + r * a.ld_grad;
     const bool same = MODE != kLoss && ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
-    // ---- the weights, and the thread's entry of the list
-    const float w = a.weight ? a.weight[r] : 1.f;
-    int y = a.target ? a.target[r] : -1;
-    float c = y < 0 ? 0.f : a.target_weight ? a.target_weight[r] : 1.f;
-    Entry mine;
-    if (tid < K) {
-      mine.id = a.ids[r * K + tid];
-      mine.l = a.logp[r * K + tid];
-    }
-    if (y >= a.V) {
-      if (MODE != kGrad && a.err && tid == 0 && (c != 0.f || w != 0.f)) *a.err = 1;
-      y = -1;
-      c = 0.f;
-    }
-    const bool live = w != 0.f || c != 0.f, listed = w != 0.f;
-    if (!live) {
-      if (MODE != kGrad && rank == 0 && tid == 0) a.loss[r] = 0.f;
-      if (MODE != kLoss) {
-        for (int v = row.v0 + tid; v < row.v1; v += kThreads) {
-          const int e = v * E - row.mis;
-          if (same && row.inside(v, v + 1)) {
-            *reinterpret_cast<uint4*>(grad + e) = make_uint4(0, 0, 0, 0);
-          } else {
-            for (int j = max(0, -e); j < min(E, a.V - e); ++j) grad[e + j] = tb::from_f32<T>(0.f);
+    {
+      // ---- the weights, and a thread for each entry of the list (all asked for at once)
+      int id = -1;
+      float l = 0.f;
+      if (tid < K) {
+        id = a.ids[r * K + tid];
+        l = a.logp[r * K + tid];
+      }
+      const Weights q(a, a.weight ? a.weight[r] : 1.f, a.target_weight ? a.target_weight[r] : 1.f, a.target ? a.target[r] : -1);
+      if (MODE != kGrad && a.err && q.bad && tid == 0) *a.err = 1;
+      if (!q.live()) {
+        if (MODE != kGrad && rank == 0 && tid == 0) a.loss[r] = 0.f;
+        if (MODE != kLoss) {
+          for (int v = row.v0 + tid; v < row.v1; v += kThreads) {
+            const int e = v * E - row.mis;
+            if (same && row.inside(v, v + 1)) {
+              __stcs(reinterpret_cast<uint4*>(grad + e), make_uint4(0, 0, 0, 0));
+            } else {
+              for (int j = max(0, -e); j < min(E, a.V - e); ++j) grad[e + j] = tb::from_f32<T>(0.f);
+            }
           }
         }
+        continue;
       }
-      continue;
-    }
-    if (!listed || mine.l == -INFINITY || mine.id < 0) mine.id = -1;
-    if (mine.id >= a.V) {
-      if (MODE != kGrad && a.err) *a.err = 1;
-      mine.id = -1;
-    }
-    if (mine.id >= 0) {
-      mine.z = tb::to_f32(row.row[mine.id]);
-      mine.t = exp(static_cast<double>(mine.l));
-      mine.lt = mine.l;
-    }
-    float z_y = 0.f;
-    if (tid == 0 && y >= 0) z_y = tb::to_f32(row.row[y]);
-    const int at = mine.id + row.mis;  // the entry's place among this CTA's vectors
-    const bool here = mine.id >= 0 && at / E >= row.v0 && at / E < row.v1;
-    s.id[tid] = mine.id;
-    s.l[tid] = mine.l;
-    if (tid == 0) s.twice = s.y_listed = 0;
-    // an id that occurs twice counts once, with the sum of its masses
-    const auto unite = [&] {
-      if (mine.id < 0) return;
-      bool first = true;
-      double t = 0.0;
-      for (int j = 0; j < K; ++j) {
-        if (s.id[j] != mine.id) continue;
-        if (j < tid) first = false;
-        t += exp(static_cast<double>(s.l[j]));
+      if (q.w == 0.f || id < 0 || l == -INFINITY) id = -1;
+      if (id >= a.V) {
+        if (MODE != kGrad && a.err) *a.err = 1;
+        id = -1;
       }
-      mine.t = t;
-      mine.lt = log(t);
-      if (!first) mine.id = -1;
-    };
+      if (tid < kMaxList) {
+        s.id[tid] = id;
+        s.l[tid] = l;
+        if (id >= 0) s.z[tid] = tb::to_f32(row.row[id]);
+        s.t[tid] = id >= 0 ? exp(static_cast<double>(l)) : 0.0;
+      }
+      if (tid == 0) {
+        s.w = q.w;
+        s.c = q.c;
+        s.y = q.y;
+        s.z_y = q.y >= 0 ? tb::to_f32(row.row[q.y]) : 0.f;
+      }
+      if (MODE != kGrad)
+        for (int i = tid; i < part; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
+      const int y_listed = __syncthreads_or(id >= 0 && id == q.y);
+      if (tid == 0) s.y_listed = y_listed;
+      // ---- an id that occurs twice counts once, with the sum of its masses
+      int seen = 0;
+      if (MODE == kGrad) {
+        seen = a.stats[r * TB_DISTILL_STATS + 8] != 0.f;
+      } else if (id >= 0) {
+        const int4* ids = reinterpret_cast<const int4*>(s.id);
+#pragma unroll 4
+        for (int j = 0; j < tid / 4; ++j) {
+          const int4 x = ids[j];
+          seen |= x.x == id || x.y == id || x.z == id || x.w == id;
+        }
+        for (int j = tid & ~3; j < tid; ++j) seen |= s.id[j] == id;
+        const int v = (id + row.mis) / E - row.v0, b = (id + row.mis) % E;
+        if (v >= 0 && v < row.v1 - row.v0) atomicOr(reinterpret_cast<uint32_t*>(bytes) + v / 4, 1u << (v % 4 * 8 + b));
+      }
+      const int twice = __syncthreads_or(seen);
+      if (tid == 0) s.twice = twice;
+      if (twice) {
+        if (id >= 0) {
+          bool first = true;
+          double m = 0.0;
+          for (int j = 0; j < K; ++j) {
+            if (s.id[j] != id) continue;
+            if (j < tid) first = false;
+            m += exp(static_cast<double>(s.l[j]));
+          }
+          s.t[tid] = first ? m : -1.0;
+        }
+        __syncthreads();
+      }
+    }
     Numbers n;
     if (MODE != kGrad) {
-      for (int i = tid; i < part; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-      const uint32_t bit = here ? 1u << ((at / E - row.v0) % 4 * 8 + at % E) : 0;
-      uint32_t* word = bits + (here ? (at / E - row.v0) / 4 : 0);
-      if (here && atomicOr(word, bit) & bit) s.twice = 1;
-      if (mine.id >= 0 && mine.id == y) s.y_listed = 1;
-      __syncthreads();
       // ---- the pass over what is outside the list
       tb::RunningSum<T> running;
-      for (int v = row.v0 + warp * tb::kChunk; v < row.v1; v += kWarps * tb::kChunk) {
-        uint4 p[8];
-        row.load_chunk(v, p);
-        uint32_t in[8], any = 0;
+      const uint64_t again = MODE == kBoth ? tb::read_again() : tb::read_once();
+      for (int v = row.v0 + warp * kStep; v < row.v1; v += kWarps * kStep) {
+        uint4 p[kLane];
+        row.template load_some<kLane>(v, p, again);
+        uint32_t in[kLane], any = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = v + i * 32 + lane;
-          in[i] = j < row.v1 ? bytes[j - row.v0] : 0;
-          any |= in[i];
+        for (int j = 0; j < kLane; ++j) {
+          const int u = v + j * 32 + lane;
+          in[j] = u < row.v1 ? bytes[u - row.v0] : 0;
+          any |= in[j];
         }
         if (any) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (in[i]) p[i] = tb::without<T>(p[i], in[i]);
+          for (int j = 0; j < kLane; ++j)
+            if (in[j]) p[j] = tb::without<T>(p[j], in[j]);
         }
         typename Vec<T>::Max top = Vec<T>::top(p[0]);
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = Vec<T>::max(top, Vec<T>::top(p[i]));
+        for (int j = 1; j < kLane; ++j) top = Vec<T>::max(top, Vec<T>::top(p[j]));
         running.add(p, Vec<T>::value(top), k1);
       }
-      // ---- sums over the block: outside the list, the list's first entries, the masses
-      SoftSum sum = running.done(k1), in;
-      if (mine.id >= 0 && !s.twice) {
-        in.m = mine.z;
-        in.s = isnan(mine.z) ? NAN : 1.f;
-        if (isnan(mine.z)) in.m = -INFINITY;
-      }
+      SoftSum sum = running.done(k1);
       sum.merge_lanes(k1);
-      in.merge_lanes(k1);
-      const double mass_w = tb::warp_sum(mine.id >= 0 ? mine.t : 0.0);
       if (lane == 0) {
         s.part[0][warp] = sum.m;
         s.part[1][warp] = sum.s;
-        s.part[2][warp] = in.m;
-        s.part[3][warp] = in.s;
-        s.mass[warp] = mass_w;
       }
+      if (warp == kWarps - 1) list_sums(a, s, k1);  // (the warp with the fewest vectors)
       __syncthreads();
-      sum = in = SoftSum();
-      double mass = 0.0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        sum.merge(s.part[0][i], s.part[1][i], k1);
-        in.merge(s.part[2][i], s.part[3][i], k1);
-        mass += s.mass[i];
+      if (warp == 0) {
+        sum = SoftSum();
+        if (lane < kWarps) {
+          sum.m = s.part[0][lane];
+          sum.s = s.part[1][lane];
+        }
+        sum.merge_lanes(k1);
       }
-      int twice = s.twice;
       if (ranks > 1) {
         if (tid == 0) {
-          s.mine[0] = sum.m;
-          s.mine[1] = sum.s;
+          s.mine[live & 1][0] = sum.m;
+          s.mine[live & 1][1] = sum.s;
         }
         cl.sync();
-        sum = SoftSum();
-        twice = 0;
-        for (int o = 0; o < ranks; ++o) {
-          const float* m = cl.map_shared_rank(s.mine, o);
-          sum.merge(m[0], m[1], k1);
-          twice |= *cl.map_shared_rank(&s.twice, o);
-        }
-      }
-      if (twice) {  // (the same in the whole cluster)
-        unite();
-        in = SoftSum();
-        if (mine.id >= 0) {
-          in.m = isnan(mine.z) ? -INFINITY : mine.z;
-          in.s = isnan(mine.z) ? NAN : 1.f;
-        }
-        in.merge_lanes(k1);
-        __syncthreads();
-        if (lane == 0) {
-          s.part[2][warp] = in.m;
-          s.part[3][warp] = in.s;
-        }
-        __syncthreads();
-        in = SoftSum();
-        for (int i = 0; i < kWarps; ++i) in.merge(s.part[2][i], s.part[3][i], k1);
-      }
-      if (a.kind == TB_DISTILL_FORWARD) {
-        mine.t = mass != 0.0 ? mine.t / mass : 0.0;
-        mine.lt -= log(mass);
-      }
-      // ---- the whole row
-      SoftSum all = sum;
-      all.merge(in.m, in.s, k1);
-      const bool good = !isnan(all.s) && !isinf(all.m);
-      const double lns = good ? tb::log_of(all.s) : 0.0;
-      // log p of the elements outside; none there: their terms are left out
-      const bool none = sum.m == -INFINITY || !good;
-      const double lp_rest = none ? 0.0 : (static_cast<double>(sum.m) - all.m) * inv_t + tb::log_of(sum.s) - lns;
-      const double p_rest = none ? 0.0 : tb::exp_of(lp_rest);
-      const double t_rest = 1.0 - mass;
-      double kl = 0.0, h = 0.0;  // h: factor of q_j outside the list
-      n.whole = 1.f;
-      if (listed) {
-        double term = 0.0;
-        if (mine.id >= 0) {
-          const double lp = (static_cast<double>(mine.z) - all.m) * inv_t - lns;
-          if (a.kind == TB_DISTILL_REVERSE) {
-            const float p = tb::exp_of(lp);
-            if (p != 0.f) term = p * (lp - mine.lt);
-          } else if (mine.t != 0.0) {
-            term = mine.t * (mine.lt - lp);
+        if (warp == 0) {
+          sum = SoftSum();
+          if (lane < ranks) {
+            const float* m = cl.map_shared_rank(s.mine[live & 1], lane);
+            sum.m = m[0];
+            sum.s = m[1];
           }
-        }
-        term = tb::warp_sum(term);
-        if (lane == 0) s.term[warp] = term;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) kl += s.term[i];
-        if (a.kind == TB_DISTILL_FORWARD) {
-          n.whole = mass != 0.0 ? 1.f : 0.f;
-          h = n.whole * p_rest;
-        } else if (a.kind == TB_DISTILL_FORWARD_REST) {
-          const double t_out = none ? 0.0 : fmax(t_rest, 0.0);
-          if (t_out > 0.0) kl += t_out * (log(t_out) - lp_rest);
-          n.whole = static_cast<float>(mass + t_out);
-          h = (mass + t_out) * p_rest - t_out;
-        } else {
-          const double f_rest = none ? 0.0 : lp_rest - log(fmax(t_rest, kRestMin));
-          kl += p_rest * f_rest;
-          h = p_rest * (f_rest - kl);
+          sum.merge_lanes(k1);
         }
       }
-      if (rank == 0 && tid == 0) {
-        const double ce = lns - (static_cast<double>(z_y) - all.m) * inv_t;
-        a.loss[r] = good ? static_cast<float>((listed ? w * kl : 0.0) + (c != 0.f ? c * ce : 0.0)) : NAN;
-      }
-      const tb::Exponent ex(sum.m, k1);
-      const double f = (listed ? w * h : 0.0) + (c != 0.f ? c * p_rest : 0.0);
-      n.origin = ex.m;
-      n.factor = !good ? NAN : none ? 0.f : static_cast<float>(f * inv_t / sum.s * ex.fix);
-      n.top = all.m;
-      n.lns = good ? static_cast<float>(lns) : NAN;
-      n.kl = static_cast<float>(kl);
-      n.mass = static_cast<float>(mass);
-      if (MODE == kLoss && a.stats && rank == 0 && tid == 0) {
-        float4* st = reinterpret_cast<float4*>(a.stats + r * TB_DISTILL_STATS);
-        st[0] = make_float4(n.origin, n.factor, n.top, n.lns);
-        st[1] = make_float4(n.kl, n.whole, n.mass, twice ? 1.f : 0.f);
-      }
+      if (warp == 0) numbers_of(a, s, r, sum, k1, inv_t, rank == 0);
+      __syncthreads();
+      n = s.n;
     } else {
       const float4* st = reinterpret_cast<const float4*>(a.stats + r * TB_DISTILL_STATS);
-      const float4 x = st[0], z = st[1];
-      const float g = a.dloss[r];
-      n = {x.x, x.y * g, x.z, x.w, z.x, z.y, z.z};
-      __syncthreads();
-      if (mine.id >= 0 && mine.id == y) s.y_listed = 1;
-      if (z.w != 0.f) unite();
-      if (a.kind == TB_DISTILL_FORWARD) mine.t = n.mass != 0.f ? mine.t / n.mass : 0.0;
+      const float4 x = st[0], y = st[1];
+      n = {x.x, x.y * a.dloss[r], x.z, make_float2(x.w, y.x), y.y, y.z};
+      if (tid == 0) s.mass = y.w;
     }
+    ++live;
     if (MODE != kLoss) {
       // ---- the gradient outside the list (in place: every element is read by its writer)
       const tb::Exponent ex(n.origin, k1);
       const float2 factor = make_float2(n.factor, n.factor);
-      for (int v = row.v0 + warp * tb::kChunk; v < row.v1; v += kWarps * tb::kChunk) {
-        uint4 p[8];
-        row.load_chunk(v, p);
-        if (same && v + tb::kChunk <= row.v1 && row.inside(v, v + tb::kChunk)) {
+      const uint64_t once = tb::read_once();
+      for (int v = row.v0 + warp * kStep; v < row.v1; v += kWarps * kStep) {
+        uint4 p[kLane];
+        row.template load_some<kLane>(v, p, once);
+        if (same && v + kStep <= row.v1 && row.inside(v, v + kStep)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(grad + (v + i * 32 + lane) * E - row.mis) = tb::scaled_powers<T>(p[i], ex, factor);
+          for (int j = 0; j < kLane; ++j)
+            __stcs(reinterpret_cast<uint4*>(grad + (v + j * 32 + lane) * E - row.mis), tb::scaled_powers<T>(p[j], ex, factor));
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int j = v + i * 32 + lane, e = j * E - row.mis;
-            if (j >= row.v1) continue;
+          for (int j = 0; j < kLane; ++j) {
+            const int u = v + j * 32 + lane, e = u * E - row.mis;
+            if (u >= row.v1) continue;
             union {
               uint4 q;
               T x[E];
-            } u;
-            u.q = tb::scaled_powers<T>(p[i], ex, factor);
-            if (same && row.inside(j, j + 1)) {
-              *reinterpret_cast<uint4*>(grad + e) = u.q;
+            } x;
+            x.q = tb::scaled_powers<T>(p[j], ex, factor);
+            if (same && row.inside(u, u + 1)) {
+              __stcs(reinterpret_cast<uint4*>(grad + e), x.q);
             } else {
 #pragma unroll
-              for (int q = 0; q < E; ++q)
-                if (e + q >= 0 && e + q < a.V) grad[e + q] = u.x[q];
+              for (int b = 0; b < E; ++b)
+                if (e + b >= 0 && e + b < a.V) grad[e + b] = x.x[b];
             }
           }
         }
       }
       __syncthreads();
       // ---- the list's elements, and the target
-      const float scale = static_cast<float>(inv_t) * (MODE == kGrad ? a.dloss[r] : 1.f);
-      if (mine.id >= 0 && here) {
-        const double lp = (static_cast<double>(mine.z) - n.top) * inv_t - n.lns;
-        const float p = isnan(lp) ? NAN : tb::exp_of(lp), t = static_cast<float>(mine.t);
-        float d = p * n.whole - t;
-        if (a.kind == TB_DISTILL_REVERSE)
-          d = p == 0.f ? 0.f : p * static_cast<float>(lp - mine.lt - n.kl);
-        d *= w;
-        if (c != 0.f) d += c * (mine.id == y ? p - 1.f : p);
-        grad[mine.id] = tb::from_f32<T>(d * scale);
+      const float scale = inv_t * (MODE == kGrad ? a.dloss[r] : 1.f), c = s.c;
+      const int y = s.y;
+      const auto mine = [&](int id) {
+        const int v = (id + row.mis) / E;
+        return v >= row.v0 && v < row.v1;
+      };
+      if (tid < K) {
+        const int id = s.id[tid];
+        const float t = static_cast<float>(s.t[tid]);
+        if (id >= 0 && t >= 0.f && mine(id)) {
+          const float lp = tb::Scaled{inv_t}(s.z[tid], n.top, n.lns), p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
+          float d;
+          if (a.kind == TB_DISTILL_REVERSE) {
+            d = p == 0.f ? 0.f : p * (lp - (s.twice ? logf(t) : s.l[tid]) - n.kl);
+          } else {
+            d = p * n.whole - (a.kind == TB_DISTILL_FORWARD ? (s.mass != 0.f ? t / s.mass : 0.f) : t);
+          }
+          d *= s.w;
+          if (c != 0.f) d += c * (id == y ? p - 1.f : p);
+          grad[id] = tb::from_f32<T>(d * scale);
+        }
       }
-      const int vy = (y + row.mis) / E;
-      if (tid == 0 && c != 0.f && !s.y_listed && vy >= row.v0 && vy < row.v1)
-        grad[y] = tb::from_f32<T>(ex.power(z_y) * n.factor - c * scale);
+      if (tid == 0 && c != 0.f && !s.y_listed && mine(y)) grad[y] = tb::from_f32<T>(ex.power(s.z_y) * n.factor - c * scale);
     }
-    if (ranks > 1) {
-      cl.sync();
-    } else {
-      __syncthreads();
-    }
+    __syncthreads();
   }
+  if (ranks > 1) cl.sync();  // the others have read this CTA's numbers
 }
 
-// CTAs of a cluster: as many as the machine has room for beside the other rows, a chunk at
-// least to each; enough of them that a part's bitmap fits its shared memory; and, where rows
-// are read twice, that the rows in work fit the L2 cache beside what is written.
-int ranks_of(int R, int groups, bool twice) {
-  const auto more = [&](int ranks) {
-    if ((groups + ranks - 1) / ranks > 4096) return true;
-    if (groups < 64 * ranks) return false;
-    return R * 2ll * ranks <= kSlots || (twice && static_cast<long long>(min(R, kSlots / ranks)) * groups * 128 > (48 << 20));
-  };
+constexpr int kSms = 148;
+constexpr int kPart = 32 * 1024;  // vectors of a part at most (of its bitmap, bytes)
+
+// CTAs of a cluster: as many as the machine has room for beside the other rows, 64 groups at
+// least to each; and enough of them that a part's bitmap fits its shared memory.
+int ranks_of(int R, int groups, int slots) {
   int ranks = 1;
-  while (ranks < 8 && more(ranks)) ranks *= 2;
+  while (ranks < 8 && ((groups + ranks - 1) / ranks * 8 > kPart || (R * 2ll * ranks <= slots && groups >= 64 * ranks))) ranks *= 2;
   return ranks;
 }
 
-template <typename T, int MODE>
-cudaError_t launch(const TbDistillArgs& a, cudaStream_t stream) {
-  constexpr int E = Row<T>::E;
-  const int groups = (a.V + E - 2 + 8 * E) / (8 * E);
-  const int ranks = ranks_of(a.R, groups, MODE == kBoth);
-  const size_t smem = MODE == kGrad ? 0 : (static_cast<size_t>((groups + ranks - 1) / ranks) * 8 + 15) / 16 * 16;
-  cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&distill_kernel<T, MODE>), 64 * 1024);
+template <typename T, int MODE, int kThreads>
+cudaError_t launch(const TbDistillArgs& a, int groups, cudaStream_t stream) {
+  const int ranks = ranks_of(a.R, groups, kSms * (1024 / kThreads));
+  const int part = MODE == kGrad ? 0 : ((groups + ranks - 1) / ranks * 8 + 15) / 16;
+  cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&distill_kernel<T, MODE, kThreads>), 2 * kPart);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   const int rows = a.R < (1 << 20) ? a.R : 1 << 20;
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * ranks);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = static_cast<size_t>(part) * 16;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -387,14 +411,19 @@ cudaError_t launch(const TbDistillArgs& a, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE>, a, static_cast<float>(tb::kLog2e / a.temperature),
-                            1.0 / a.temperature, static_cast<int>(smem / 16));
+  return cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE, kThreads>, a, static_cast<float>(tb::kLog2e / a.temperature),
+                            static_cast<float>(1.0 / a.temperature), part);
 }
 
+// Both passes in one launch: the rows in work, read twice, have to fit the L2 cache beside
+// what is written, so long rows get two CTAs of 512 threads on an SM instead of four of 256.
 template <typename T>
 cudaError_t launch_mode(const TbDistillArgs& a, cudaStream_t s) {
-  if (!a.loss) return launch<T, kGrad>(a, s);
-  return a.grad ? launch<T, kBoth>(a, s) : launch<T, kLoss>(a, s);
+  constexpr int E = Row<T>::E;
+  const int groups = (a.V + E - 2 + 8 * E) / (8 * E);
+  if (!a.loss) return launch<T, kGrad, 256>(a, groups, s);
+  if (!a.grad) return launch<T, kLoss, 256>(a, groups, s);
+  return groups > 768 ? launch<T, kBoth, 512>(a, groups, s) : launch<T, kBoth, 256>(a, groups, s);
 }
 
 }  // namespace

@@ -448,7 +448,7 @@ int tb_topk_logprobs(const TbTopkLogprobsArgs* args, cudaStream_t s);
 // Per row of logits [R, V]: weight * KL to a teacher's list of K ids and
 // log-probabilities, plus target_weight * -log p[target], and its gradient.
 enum { TB_DISTILL_FORWARD = 0, TB_DISTILL_FORWARD_REST = 1, TB_DISTILL_REVERSE = 2 };
-enum { TB_DISTILL_STATS = 8 };  // floats kept of a row for a backward pass of its own
+enum { TB_DISTILL_STATS = 12 };  // floats kept of a row for a backward pass of its own
 typedef struct {
   const void* logits;
   long long ld;

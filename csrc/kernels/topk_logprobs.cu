@@ -161,7 +161,7 @@ __device__ Place place_of(Shared& s, const O* orders, int n, int k, int most, in
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1, double inv_t) {
+__global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1, float inv_t) {
   using O = typename Order<T>::Type;
   constexpr int E = Row<T>::E, GE = 8 * E;
   extern __shared__ uint4 dynamic[];  // the groups' maxima, then the chosen groups' elements, then the cluster's lists
@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     __syncthreads();
     // ---- a place is the sum of the places in every list
     const bool plain = !isinf(sum.m) && !isnan(sum.s);
-    const double lns = plain ? tb::log_of(sum.s) : 0.0;
+    const float2 lns = plain ? tb::log_of(sum.s) : make_float2(0.f, 0.f);
     if (rank == 0 && threadIdx.x == 0)
-      a.lse[r] = plain ? static_cast<float>(sum.m * inv_t + lns) : isnan(sum.s) ? NAN : sum.m;
+      a.lse[r] = plain ? fmaf(sum.m, inv_t, lns.x) + lns.y : isnan(sum.s) ? NAN : sum.m;
     for (int i = threadIdx.x; i < own; i += kThreads) {
       const Key x = s.sorted[i];
       int place = i;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
       const float z = Order<T>::value(static_cast<uint32_t>(x >> kIndexBits));
       float y;
       if (plain) {
-        y = static_cast<float>((static_cast<double>(z) - sum.m) * inv_t - lns);
+        y = tb::Scaled{inv_t}(z, sum.m, lns);
       } else {
         y = isnan(sum.s) || (sum.m > 0 && z == sum.m) ? NAN : -INFINITY;
       }
@@ -423,7 +423,7 @@ cudaError_t launch(const TbTopkLogprobsArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, topk_kernel<T>, a, static_cast<float>(tb::kLog2e / a.temperature),
-                            1.0 / a.temperature);
+                            static_cast<float>(1.0 / a.temperature));
 }
 
 }  // namespace

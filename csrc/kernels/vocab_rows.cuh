@@ -21,7 +21,7 @@
 namespace tb {
 
 constexpr double kLog2e = 1.4426950408889634;
-constexpr double kLn2 = 0.6931471805599453;
+constexpr float kLn2 = 0.69314718f;
 constexpr int kChunk = 256;  // vectors of a chunk
 
 __device__ __forceinline__ float ex2(float x) {
@@ -29,19 +29,25 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// exp of a 64-bit number as fp32: the integral power of two exactly, the rest by ex2.
-__device__ __forceinline__ float exp_of(double x) {
-  const double y = fmin(fmax(x * kLog2e, -1000.0), 1000.0);  // (NaN becomes -1000: the callers check)
-  const double n = rint(y);
-  return ldexpf(ex2(static_cast<float>(y - n)), static_cast<int>(n));
-}
-// log of a positive finite fp32 number, off by 2^-26 or so: the exponent's share exactly.
-__device__ __forceinline__ double log_of(float x) {
+// log of a positive finite number as the sum of two, off by 2^-25 or so: the exponent's
+// share exactly (its factor ln 2 in two parts, the first of 12 bits).
+__device__ __forceinline__ float2 log_of(float x) {
   int e;
-  const float f = frexpf(x, &e);  // [0.5, 1)
-  const bool low = f < 0.70710678f;
-  return (e - (low ? 1 : 0)) * kLn2 + static_cast<double>(logf(low ? 2.f * f : f));
+  float f = frexpf(x, &e);  // [0.5, 1)
+  if (f < 0.70710678f) {
+    f *= 2.f;
+    --e;
+  }
+  constexpr float kHigh = 0.693115234375f, kLow = 3.19461846e-5f;  // ln 2
+  return make_float2(e * kHigh, fmaf(static_cast<float>(e), kLow, logf(f)));
 }
+// 1 / T, and log p of a logit.
+struct Scaled {
+  float inv_t;
+  __device__ __forceinline__ float operator()(float z, float top, float2 lns) const {
+    return fmaf(z - top, inv_t, -lns.x) - lns.y;
+  }
+};
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -147,6 +153,15 @@ struct Row {
                  : "memory");
     return p;
   }
+  // With a policy for the L2 cache.
+  __device__ __forceinline__ uint4 load_inside(int v, uint64_t policy) const {
+    uint4 p;
+    asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+                 : "=r"(p.x), "=r"(p.y), "=r"(p.z), "=r"(p.w)
+                 : "l"(base + static_cast<long long>(v) * E), "l"(policy)
+                 : "memory");
+    return p;
+  }
   __device__ __forceinline__ static uint4 lowest() {
     return make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
   }
@@ -178,7 +193,31 @@ struct Row {
       for (int i = 0; i < 8; ++i) p[i] = load(c + i * 32 + lane);
     }
   }
+  // The same for N vectors of a lane, with a policy.
+  template <int N>
+  __device__ __forceinline__ void load_some(int c, uint4 (&p)[N], uint64_t policy) const {
+    const int lane = threadIdx.x & 31;
+    if (c + N * 32 <= v1 && inside(c, c + N * 32)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) p[i] = load_inside(c + i * 32 + lane, policy);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) p[i] = load(c + i * 32 + lane);
+    }
+  }
 };
+
+// What is read again soon stays in the L2 cache before all else; what is not goes first.
+__device__ __forceinline__ uint64_t read_again() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t read_once() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
 
 // A maximum m and the sum s of 2^((x - m) k1); an infinite m counts as 0 in the exponent
 // (s is then 0, inf or NaN).
@@ -209,7 +248,7 @@ struct Exponent {
     m = isinf(m_) ? 0.f : m_;
     c = -(m * k1);
     near = fabsf(c) < 1e37f;
-    fix = near ? 1.f - fmaf(m, k1, c) * static_cast<float>(kLn2) : 1.f;
+    fix = near ? 1.f - fmaf(m, k1, c) * kLn2 : 1.f;
   }
   __device__ __forceinline__ float2 powers(float2 x) const {
     const float2 a = near ? fma2(x, make_float2(k1, k1), make_float2(c, c)) : make_float2((x.x - m) * k1, (x.y - m) * k1);
@@ -260,7 +299,8 @@ template <typename T>
 struct RunningSum {
   float m = -INFINITY;
   float2 s0 = {0.f, 0.f}, s1 = {0.f, 0.f};
-  __device__ __forceinline__ void add(const uint4 (&p)[8], float top, float k1) {
+  template <int N>
+  __device__ __forceinline__ void add(const uint4 (&p)[N], float top, float k1) {
     if (top > m) {
       const float f = m == -INFINITY ? 0.f : Exponent(m, k1).fix * ex2((m - top) * k1);
       s0 = mul2(s0, make_float2(f, f));
@@ -271,7 +311,7 @@ struct RunningSum {
     if (e.near) {
       const float2 k2 = make_float2(k1, k1), c2 = make_float2(e.c, e.c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < Row<T>::kPairs; ++j) {
           const float2 a = fma2(Vec<T>::pair(p[i], j), k2, c2);
@@ -280,7 +320,7 @@ struct RunningSum {
         }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < Row<T>::kPairs; ++j) s0 = add2(s0, e.powers(Vec<T>::pair(p[i], j)));
     }

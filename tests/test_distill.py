@@ -226,8 +226,8 @@ def run_both(x, ids, logp, w, kind, rest, T, y, c):
     assert out is z and torch.equal(l2, loss) and torch.equal(z.nan_to_num(7.0), d.nan_to_num(7.0))
     leaf = x.detach().clone().requires_grad_()
     l3 = distill_loss(leaf, ids, logp, w, **how)
-    assert torch.equal(l3.detach().nan_to_num(7.0), loss.nan_to_num(7.0))
-    assert torch.equal(distill_loss(x, ids, logp, w, **how).nan_to_num(7.0), loss.nan_to_num(7.0))
+    # (the loss alone may be summed in another order: compared with the definition below)
+    assert torch.equal(distill_loss(x, ids, logp, w, **how).nan_to_num(7.0), l3.detach().nan_to_num(7.0))
     g = torch.rand(x.shape[0], generator=torch.Generator().manual_seed(1)).to(x.device) + 0.5
     d3, = torch.autograd.grad(l3, leaf, g)
     compare(l3, d3, x, want, g)
