@@ -13,6 +13,8 @@
 // few more; of those groups the elements that reach it, some k, are ordered by counting.
 // Where too many do (equal values, the largest side by side), the k-th place is searched by
 // bisection with counts over the block, first of the value and then of the index.
+#include <type_traits>
+
 #include "kernels.h"
 #include "vocab_rows.cuh"
 
@@ -28,10 +30,13 @@ constexpr int kMaxK = 256;
 constexpr int kIndexBits = 21;  // indexes below 2^20 elements (and the row's offset in its vectors)
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
 constexpr int kRank = 512;  // elements that are ordered by counting
-constexpr int kBins = 16384;  // of the histogram, two to a word
+constexpr int kBins = 8192;   // of the histogram, two to a word
 using Key = unsigned long long;
 
-__host__ __device__ constexpr int most_groups(int k) { return k + k / 4 + 16; }
+// Groups that are looked at again: by the histogram, whose bins hold several values, and by
+// the exact search.
+__host__ __device__ constexpr int most_groups(int k) { return 2 * k + 32; }
+__host__ __device__ constexpr int few_groups(int k) { return k + k / 4 + 16; }
 
 // Whole numbers in the order of the values: +0 and -0 are equal, NaN is -inf, 0 is below all.
 template <typename T>
@@ -164,17 +169,23 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1, float inv_t) {
   using O = typename Order<T>::Type;
   constexpr int E = Row<T>::E, GE = 8 * E;
-  extern __shared__ uint4 dynamic[];  // the groups' maxima, then the chosen groups' elements, then the cluster's lists
-  O* orders = reinterpret_cast<O*>(dynamic);
+  // the histogram and the groups' maxima; in their place, where too many elements are equal,
+  // the chosen groups' elements; then the cluster's lists.  (Little of it: what shared memory
+  // leaves of the L1 cache holds the loads in flight.)
+  extern __shared__ uint4 dynamic[];
+  uint32_t* hist = reinterpret_cast<uint32_t*>(dynamic);
+  O* orders = reinterpret_cast<O*>(dynamic + kBins / 8);
   __shared__ Shared s;
-  __shared__ uint4 hist4[kBins / 8];
-  uint32_t* hist = reinterpret_cast<uint32_t*>(hist4);
-  constexpr int kShift = sizeof(T) == 2 ? 2 : 18;  // orders of a bin
+  // A bin has one order of bf16 (two of fp16, 2^16 of fp32), and again the orders 8,192 bins
+  // away: some 64 powers of two (fp16: 16), further than a row's maxima lie apart.  Where they
+  // do not, too few groups are found, and the search starts over.
+  constexpr int kShift = std::is_same<T, float>::value ? 16 : std::is_same<T, __half>::value ? 1 : 0;
+  constexpr uint32_t kWords = kBins / 2 - 1;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ranks = cl.num_blocks();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int k = a.k;
-  for (int i = threadIdx.x; i < kBins / 8; i += kThreads) hist4[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < kBins / 8; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
   for (long long r = blockIdx.x / ranks; r < a.R; r += gridDim.x / ranks) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.V, rank, ranks);
     const int g0 = row.v0 / 8, ng = (row.v1 - row.v0 + 7) / 8;
@@ -213,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
       if (g < ng) {
         const uint32_t o = Order<T>::of(Vec<T>::value(top[0]));
         orders[g] = static_cast<O>(o);
-        atomicAdd(&hist[o >> (kShift + 1)], 1u << (o >> kShift & 1) * 16);
+        atomicAdd(&hist[o >> (kShift + 1) & kWords], 1u << (o >> kShift & 1) * 16);
         olo = min(olo, o);
         ohi = max(ohi, o);
       }
@@ -234,13 +245,14 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     sum.merge_lanes(k1);
     // ---- the first k groups, and a few more: from the highest bin down (each warp for itself)
     uint32_t floor = 1;
+    int at_floor = ng;
     const Key above_all = static_cast<Key>(s.hi) + 1;
     Place t{1, 0x7fffffff};
     if (ng > k) {
       int at = 0;  // groups in the words above
       int word = static_cast<int>(s.hi >> (kShift + 1));
-      for (;; word -= 32) {
-        const uint32_t h = word - lane >= 0 ? hist[word - lane] : 0;
+      for (const int end = word - kBins / 2; word > end; word -= 32) {
+        const uint32_t h = word - lane > end ? hist[(word - lane) & kWords] : 0;
         const int c = (h >> 16) + (h & 0xffffu);
         int incl = c;
 #pragma unroll
@@ -257,20 +269,38 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
         const int before = at + __shfl_sync(0xffffffffu, incl - c, l);
         const uint32_t w = __shfl_sync(0xffffffffu, h, l);
         const bool upper = before + static_cast<int>(w >> 16) >= k;
-        floor = static_cast<uint32_t>((word - l) * 2 + (upper ? 1 : 0)) << kShift;
+        if (word >= l) floor = static_cast<uint32_t>((word - l) * 2 + (upper ? 1 : 0)) << kShift;
         at = before + static_cast<int>(w >> 16) + (upper ? 0 : static_cast<int>(w & 0xffffu));
         break;
       }
-      floor = max(floor, 1u);
-      t.order = floor;
-      if (at > most_groups(k)) t = place_of(s, orders, ng, k, most_groups(k), at, floor, above_all, ng - 1, turn, [](int i) { return i; });
-      floor = t.order;  // k elements are at or above it
+      t.order = floor = max(floor, s.lo);
+      at_floor = at;
     }
-    for (int i = threadIdx.x; i < ng; i += kThreads)
-      if (t.takes(orders[i], i)) s.list[atomicAdd(&s.groups, 1)] = i;
-    __syncthreads();
-    // ---- their elements at or above it
-    const int groups = s.groups;
+    const auto choose = [&] {
+      for (int i = threadIdx.x; i < ng; i += kThreads)
+        if (t.takes(orders[i], i)) s.list[atomicAdd(&s.groups, 1)] = i;
+      __syncthreads();
+    };
+    const bool fits = at_floor <= most_groups(k);
+    if (fits) choose();
+    int groups = s.groups;
+    if (fits) at_floor = groups;
+    if (ng > k && (!fits || groups < k)) {  // (see the histogram's bins)
+      int c = 0;
+      for (int i = threadIdx.x; i < ng; i += kThreads) c += orders[i] >= floor;
+      at_floor = block_count(s, c, turn);
+      if (at_floor < k) {
+        floor = s.lo;
+        at_floor = ng;
+      }
+      t = place_of(s, orders, ng, k, few_groups(k), at_floor, floor, above_all, ng - 1, turn, [](int i) { return i; });
+      if (threadIdx.x == 0) s.groups = 0;
+      __syncthreads();
+      choose();
+      groups = s.groups;
+      floor = t.order;
+    }
+    // ---- their elements at or above it: k of them at least
     const auto vector_of = [&](int i) { return (g0 + s.list[i >> 3]) * 8 + (i & 7); };
     const auto push = [&](uint32_t o, int e) {
       const int at = atomicAdd(&s.cands, 1);
@@ -299,15 +329,25 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     }
     __syncthreads();
     int cands = s.cands;
+    bool trashed = ranks > 1;  // (the lists come to lie there)
     const int own = min(k, cands);  // (fewer than k: a short part of a row)
-    if (cands > kRank) {  // ---- too many: all the groups' elements in shared memory, and the first `own` of them
+    if (cands > kRank) {  // ---- too many: the first k groups' elements in shared memory, and the first `own` of them
+      if (groups > few_groups(k) && ng > k) {
+        t = place_of(s, orders, ng, k, few_groups(k), at_floor, floor, above_all, ng - 1, turn, [](int i) { return i; });
+        if (threadIdx.x == 0) s.groups = 0;
+        __syncthreads();
+        choose();
+        groups = s.groups;
+      }
+      floor = t.order;
       const int n = groups * GE;
       int above = 0;
       for (int i = threadIdx.x; i < groups * 8; i += kThreads) {
         const int v = vector_of(i);
         dynamic[i] = orders_of(row, v, row.load(v), floor, above);
       }
-      __syncthreads();
+      cands = block_count(s, above, turn);
+      orders = reinterpret_cast<O*>(dynamic);
       const auto element = [&](int i) { return (g0 + s.list[i / GE]) * GE + i % GE - row.mis; };
       const Place e = place_of(s, orders, n, own, kRank, cands, floor, above_all, a.V, turn, element);
       if (threadIdx.x == 0) s.cands = 0;
@@ -318,9 +358,12 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
       }
       __syncthreads();
       cands = s.cands;
+      orders = reinterpret_cast<O*>(dynamic + kBins / 8);
+      trashed = true;
+    } else if (!trashed) {  // the bins that were in use, for the next row
+      const int lo = static_cast<int>(s.lo >> (kShift + 1)), hi = static_cast<int>(s.hi >> (kShift + 1));
+      for (int i = lo + threadIdx.x; i <= min(hi, lo + static_cast<int>(kWords)); i += kThreads) hist[i & kWords] = 0;
     }
-    // the bins that were in use, for the next row
-    for (int i = static_cast<int>(s.lo >> (kShift + 1)) + threadIdx.x; i <= static_cast<int>(s.hi >> (kShift + 1)); i += kThreads) hist[i] = 0;
     for (int i = threadIdx.x; i < cands; i += kThreads) {
       const Key x = s.cand[i];
       int place = 0;
@@ -389,10 +432,12 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     } else {
       __syncthreads();
     }
+    if (trashed)
+      for (int i = threadIdx.x; i < kBins / 8; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// CTAs of a cluster: as many as the machine has room for beside the other rows, a chunk at
+// CTAs of a cluster: as many as the machine has room for beside the other rows, 64 groups at
 // least to each; enough of them that the maxima of a part fit its shared memory.
 int ranks_of(int R, int groups) {
   int ranks = 1;
@@ -405,9 +450,10 @@ cudaError_t launch(const TbTopkLogprobsArgs& a, cudaStream_t stream) {
   constexpr int E = Row<T>::E;
   using O = typename Order<T>::Type;
   const int groups = (a.V + E - 2 + 8 * E) / (8 * E), ranks = ranks_of(a.R, groups), per = (groups + ranks - 1) / ranks;
-  const int chosen = per > a.k && per > most_groups(a.k) ? most_groups(a.k) : per;
-  size_t smem = sizeof(O) * static_cast<size_t>(per > chosen * 8 * E ? per : chosen * 8 * E);
-  if (ranks > 1 && smem < ranks * a.k * sizeof(Key)) smem = ranks * a.k * sizeof(Key);
+  const int chosen = (per > a.k && per > few_groups(a.k) ? few_groups(a.k) : per) * 8 * E;
+  size_t smem = kBins * 2 + (sizeof(O) * per + 15) / 16 * 16;
+  if (smem < sizeof(O) * chosen) smem = sizeof(O) * chosen;
+  if (smem < ranks * a.k * sizeof(Key)) smem = ranks * a.k * sizeof(Key);
   cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&topk_kernel<T>), 64 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
