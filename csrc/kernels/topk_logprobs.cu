@@ -5,7 +5,7 @@
 // a_1 .. a_k the ids in order of (z descending, id ascending).
 //
 // One pass over the row forms the softmax's running maximum and sum, and the maximum of
-// every group of 8 vectors (128 bytes).  The k largest elements lie in the k first groups
+// every group of 8 vectors (128 bytes; of every vector in short rows).  The k largest elements lie in the k first groups
 // by (maximum descending, index ascending): for an element outside them, each of those
 // groups holds one that comes before it.  So the selection looks at V / 64 maxima in
 // shared memory and reads some k groups again, whatever the data (all equal, ascending).
@@ -30,6 +30,7 @@ constexpr int kMaxK = 256;
 constexpr int kIndexBits = 21;  // indexes below 2^20 elements (and the row's offset in its vectors)
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
 constexpr int kRank = 512;  // elements that are ordered by counting
+constexpr int kSingle = 2048;  // vectors of a part up to which each is a group of its own
 constexpr int kBins = 8192;   // of the histogram, two to a word
 using Key = unsigned long long;
 
@@ -101,6 +102,31 @@ __device__ __forceinline__ uint4 orders_of(const Row<T>& row, int v, const uint4
   }
 }
 
+// The histogram's bins, ascending with the order's upper 16 bits: single bf16 values from
+// 2^-8 to 2^24 (8 fp16 values), 16 of them below and above and of the negative ones.
+template <typename T>
+struct Bin {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr int kShift = sizeof(T) == 4 ? 16 : 0;
+  __device__ __forceinline__ static int of(uint32_t order) {
+    const uint32_t h = order >> kShift, p = h - 0x8000u;
+    if (h < 0x8000u) return h >> 4;
+    if (kHalf) return 2048 + (p >> 3);
+    return p < 0x3b80u ? 2048 + (p >> 4) : p < 0x4b80u ? 3000 + (p - 0x3b80u) : 7096 + ((p - 0x4b80u) >> 4);
+  }
+  __device__ __forceinline__ static uint32_t lowest(int b) {
+    uint32_t h;
+    if (b < 2048) {
+      h = b << 4;
+    } else if (kHalf) {
+      h = 0x8000u + ((b - 2048) << 3);
+    } else {
+      h = 0x8000u + (b < 3000 ? (b - 2048) << 4 : b < 7096 ? 0x3b80 + (b - 3000) : 0x4b80 + ((b - 7096) << 4));
+    }
+    return h << kShift;
+  }
+};
+
 struct Shared {
   Key cand[kRank];
   Key sorted[kMaxK];  // this CTA's own list, read by the others of its cluster
@@ -168,7 +194,7 @@ __device__ Place place_of(Shared& s, const O* orders, int n, int k, int most, in
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a, float k1, float inv_t) {
   using O = typename Order<T>::Type;
-  constexpr int E = Row<T>::E, GE = 8 * E;
+  constexpr int E = Row<T>::E;
   // the histogram and the groups' maxima; in their place, where too many elements are equal,
   // the chosen groups' elements; then the cluster's lists.  (Little of it: what shared memory
   // leaves of the L1 cache holds the loads in flight.)
@@ -176,11 +202,6 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
   uint32_t* hist = reinterpret_cast<uint32_t*>(dynamic);
   O* orders = reinterpret_cast<O*>(dynamic + kBins / 8);
   __shared__ Shared s;
-  // A bin has one order of bf16 (two of fp16, 2^16 of fp32), and again the orders 8,192 bins
-  // away: some 64 powers of two (fp16: 16), further than a row's maxima lie apart.  Where they
-  // do not, too few groups are found, and the search starts over.
-  constexpr int kShift = std::is_same<T, float>::value ? 16 : std::is_same<T, __half>::value ? 1 : 0;
-  constexpr uint32_t kWords = kBins / 2 - 1;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), ranks = cl.num_blocks();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -188,7 +209,8 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
   for (int i = threadIdx.x; i < kBins / 8; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
   for (long long r = blockIdx.x / ranks; r < a.R; r += gridDim.x / ranks) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.V, rank, ranks);
-    const int g0 = row.v0 / 8, ng = (row.v1 - row.v0 + 7) / 8;
+    const bool single = row.v1 - row.v0 <= kSingle;
+    const int GV = single ? 1 : 8, ng = (row.v1 - row.v0 + GV - 1) / GV;  // vectors of a group, groups
     if (threadIdx.x == 0) {
       s.lo = 0xffffffffu;
       s.hi = 0;
@@ -200,6 +222,14 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     // ---- the pass
     tb::RunningSum<T> running;
     uint32_t olo = 0xffffffffu, ohi = 0;
+    const auto keep = [&](int g, typename Vec<T>::Max top) {
+      const uint32_t o = Order<T>::of(Vec<T>::value(top));
+      orders[g] = static_cast<O>(o);
+      const int bin = Bin<T>::of(o);
+      atomicAdd(&hist[bin >> 1], 1u << (bin & 1) * 16);
+      olo = min(olo, o);
+      ohi = max(ohi, o);
+    };
     for (int c = row.v0 + warp * tb::kChunk; c < row.v1; c += kThreads / 32 * tb::kChunk) {
       uint4 p[8];
       row.load_chunk(c, p);
@@ -210,6 +240,14 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
 #pragma unroll
       for (int i = 1; i < 8; ++i) all = Vec<T>::max(all, top[i]);
       running.add(p, Vec<T>::value(all), k1);
+      if (single) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int g = c - row.v0 + i * 32 + lane;
+          if (g < ng) keep(g, top[i]);
+        }
+        continue;
+      }
       // maxima over eight lanes of eight vectors: lane l ends with those of its vector l % 8
 #pragma unroll
       for (int h = 4; h > 0; h >>= 1) {
@@ -220,14 +258,8 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
           top[i] = Vec<T>::max(keep, __shfl_xor_sync(0xffffffffu, send, h));
         }
       }
-      const int g = c / 8 - g0 + (lane & 7) * 4 + lane / 8;
-      if (g < ng) {
-        const uint32_t o = Order<T>::of(Vec<T>::value(top[0]));
-        orders[g] = static_cast<O>(o);
-        atomicAdd(&hist[o >> (kShift + 1) & kWords], 1u << (o >> kShift & 1) * 16);
-        olo = min(olo, o);
-        ohi = max(ohi, o);
-      }
+      const int g = (c - row.v0) / 8 + (lane & 7) * 4 + lane / 8;
+      if (g < ng) keep(g, top[0]);
     }
     SoftSum sum = running.done(k1);
     sum.merge_lanes(k1);
@@ -250,9 +282,8 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     Place t{1, 0x7fffffff};
     if (ng > k) {
       int at = 0;  // groups in the words above
-      int word = static_cast<int>(s.hi >> (kShift + 1));
-      for (const int end = word - kBins / 2; word > end; word -= 32) {
-        const uint32_t h = word - lane > end ? hist[(word - lane) & kWords] : 0;
+      for (int word = Bin<T>::of(s.hi) >> 1; word >= 0; word -= 32) {
+        const uint32_t h = word >= lane ? hist[word - lane] : 0;
         const int c = (h >> 16) + (h & 0xffffu);
         int incl = c;
 #pragma unroll
@@ -269,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
         const int before = at + __shfl_sync(0xffffffffu, incl - c, l);
         const uint32_t w = __shfl_sync(0xffffffffu, h, l);
         const bool upper = before + static_cast<int>(w >> 16) >= k;
-        if (word >= l) floor = static_cast<uint32_t>((word - l) * 2 + (upper ? 1 : 0)) << kShift;
+        floor = Bin<T>::lowest((word - l) * 2 + (upper ? 1 : 0));
         at = before + static_cast<int>(w >> 16) + (upper ? 0 : static_cast<int>(w & 0xffffu));
         break;
       }
@@ -281,39 +312,26 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
         if (t.takes(orders[i], i)) s.list[atomicAdd(&s.groups, 1)] = i;
       __syncthreads();
     };
-    const bool fits = at_floor <= most_groups(k);
-    if (fits) choose();
-    int groups = s.groups;
-    if (fits) at_floor = groups;
-    if (ng > k && (!fits || groups < k)) {  // (see the histogram's bins)
-      int c = 0;
-      for (int i = threadIdx.x; i < ng; i += kThreads) c += orders[i] >= floor;
-      at_floor = block_count(s, c, turn);
-      if (at_floor < k) {
-        floor = s.lo;
-        at_floor = ng;
-      }
+    if (at_floor > most_groups(k) && ng > k) {
       t = place_of(s, orders, ng, k, few_groups(k), at_floor, floor, above_all, ng - 1, turn, [](int i) { return i; });
-      if (threadIdx.x == 0) s.groups = 0;
-      __syncthreads();
-      choose();
-      groups = s.groups;
       floor = t.order;
     }
+    choose();
+    int groups = s.groups;
     // ---- their elements at or above it: k of them at least
-    const auto vector_of = [&](int i) { return (g0 + s.list[i >> 3]) * 8 + (i & 7); };
+    const auto vector_of = [&](int i) { return row.v0 + (single ? s.list[i] : s.list[i >> 3] * 8 + (i & 7)); };
     const auto push = [&](uint32_t o, int e) {
       const int at = atomicAdd(&s.cands, 1);
       if (at < kRank) s.cand[at] = static_cast<Key>(o) << kIndexBits | (kIndexMask - static_cast<uint32_t>(e));
     };
-    for (int i0 = threadIdx.x; i0 < groups * 8; i0 += 4 * kThreads) {
+    for (int i0 = threadIdx.x; i0 < groups * GV; i0 += 4 * kThreads) {
       uint4 p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) p[u] = i0 + u * kThreads < groups * 8 ? row.load(vector_of(i0 + u * kThreads)) : Row<T>::lowest();
+      for (int u = 0; u < 4; ++u) p[u] = i0 + u * kThreads < groups * GV ? row.load(vector_of(i0 + u * kThreads)) : Row<T>::lowest();
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * kThreads;
-        if (i >= groups * 8 || Order<T>::of(Vec<T>::value(Vec<T>::top(p[u]))) < floor) continue;
+        if (i >= groups * GV || Order<T>::of(Vec<T>::value(Vec<T>::top(p[u]))) < floor) continue;
         const int v = vector_of(i);
         int above = 0;
         const uint4 q = orders_of(row, v, p[u], floor, above);
@@ -340,15 +358,15 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
         groups = s.groups;
       }
       floor = t.order;
-      const int n = groups * GE;
+      const int n = groups * GV * E;
       int above = 0;
-      for (int i = threadIdx.x; i < groups * 8; i += kThreads) {
+      for (int i = threadIdx.x; i < groups * GV; i += kThreads) {
         const int v = vector_of(i);
         dynamic[i] = orders_of(row, v, row.load(v), floor, above);
       }
       cands = block_count(s, above, turn);
       orders = reinterpret_cast<O*>(dynamic);
-      const auto element = [&](int i) { return (g0 + s.list[i / GE]) * GE + i % GE - row.mis; };
+      const auto element = [&](int i) { return vector_of(i / E) * E + i % E - row.mis; };
       const Place e = place_of(s, orders, n, own, kRank, cands, floor, above_all, a.V, turn, element);
       if (threadIdx.x == 0) s.cands = 0;
       __syncthreads();
@@ -361,8 +379,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
       orders = reinterpret_cast<O*>(dynamic + kBins / 8);
       trashed = true;
     } else if (!trashed) {  // the bins that were in use, for the next row
-      const int lo = static_cast<int>(s.lo >> (kShift + 1)), hi = static_cast<int>(s.hi >> (kShift + 1));
-      for (int i = lo + threadIdx.x; i <= min(hi, lo + static_cast<int>(kWords)); i += kThreads) hist[i & kWords] = 0;
+      for (int i = (Bin<T>::of(s.lo) >> 1) + threadIdx.x; i <= Bin<T>::of(s.hi) >> 1; i += kThreads) hist[i] = 0;
     }
     for (int i = threadIdx.x; i < cands; i += kThreads) {
       const Key x = s.cand[i];
@@ -437,11 +454,13 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
   }
 }
 
-// CTAs of a cluster: as many as the machine has room for beside the other rows, 64 groups at
-// least to each; enough of them that the maxima of a part fit its shared memory.
+// CTAs of a cluster: as many as the machine has room for beside the other rows, 512 groups at
+// least to each (joining the lists costs 3 us: one row of 500 groups takes 8.2 us with one CTA
+// and 11.3 with eight, of 2,374 groups 18.4, 12.3 with four and with eight); enough of them
+// that the maxima of a part fit its shared memory.
 int ranks_of(int R, int groups) {
   int ranks = 1;
-  while (ranks < 8 && ((groups + ranks - 1) / ranks > 8192 || (R * 2ll * ranks <= 148 * 4 && groups >= 64 * ranks))) ranks *= 2;
+  while (ranks < 8 && ((groups + ranks - 1) / ranks > 8192 || (R * 2ll * ranks <= 148 * 4 && groups >= 1024 * ranks))) ranks *= 2;
   return ranks;
 }
 
@@ -451,7 +470,8 @@ cudaError_t launch(const TbTopkLogprobsArgs& a, cudaStream_t stream) {
   using O = typename Order<T>::Type;
   const int groups = (a.V + E - 2 + 8 * E) / (8 * E), ranks = ranks_of(a.R, groups), per = (groups + ranks - 1) / ranks;
   const int chosen = (per > a.k && per > few_groups(a.k) ? few_groups(a.k) : per) * 8 * E;
-  size_t smem = kBins * 2 + (sizeof(O) * per + 15) / 16 * 16;
+  const int maxima = per * 8 < kSingle ? per * 8 : per > kSingle ? per : kSingle;
+  size_t smem = kBins * 2 + (sizeof(O) * maxima + 15) / 16 * 16;
   if (smem < sizeof(O) * chosen) smem = sizeof(O) * chosen;
   if (smem < ranks * a.k * sizeof(Key)) smem = ranks * a.k * sizeof(Key);
   cudaError_t e = tb::ensure_dyn_smem(reinterpret_cast<const void*>(&topk_kernel<T>), 64 * 1024);
