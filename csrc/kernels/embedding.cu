@@ -31,52 +31,117 @@ __device__ __forceinline__ long long id_of(const void* ids, int ids64, long long
   return ids64 ? static_cast<const long long*>(ids)[t] : static_cast<const int*>(ids)[t];
 }
 
-// ------------------------------------------------------------------ lookup
-// Vectors of N elements that a lane has in flight.
-template <typename T, int N>
-constexpr int kUnroll = N * sizeof(T) == 16 ? 4 : 8;
-
-template <typename T, int N>
-__device__ __forceinline__ void scaled_row(const TbEmbeddingArgs& a, long long id, float (&x)[N]) {
-  if (id >= 0 && id < a.V) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] *= a.scale;
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = id < 0 ? 0.f : NAN;
+// ---- rows of any alignment: 16 bytes that begin `shift` bytes into the first of two vectors.
+// (What lies beside a row within its tensor is read along and not used.)
+template <typename T>
+struct Two {
+  static constexpr int E = 16 / sizeof(T);
+  uint4 a, b;
+  __device__ __forceinline__ static unsigned shift_of(const T* p) { return static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) & 15); }
+  // Whether the vectors that hold the elements [p, p + n) lie between first and last.
+  __device__ __forceinline__ static bool inside(const T* p, int n, const T* first, const T* last) {
+    return p - shift_of(p) / sizeof(T) >= first && p + (n + E - 1) / E * E + E <= last;
   }
-}
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4* v = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+    a = v[0];
+    b = v[1];
+  }
+  __device__ __forceinline__ void values(unsigned s, float (&x)[E]) const {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = s & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = s & 4 ? w[i + 1] : w[i];
+    uint4 q;
+    q.x = __funnelshift_r(w[0], w[1], (s & 3) * 8);
+    q.y = __funnelshift_r(w[1], w[2], (s & 3) * 8);
+    q.z = __funnelshift_r(w[2], w[3], (s & 3) * 8);
+    q.w = __funnelshift_r(w[3], w[4], (s & 3) * 8);
+    const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = tb::to_f32(e[j]);
+  }
+};
 
-// A warp takes 32 x U vectors of N elements of a row (rows of 32 vectors and more).
-template <typename T, int N>
+// ------------------------------------------------------------------ lookup
+constexpr int kUnroll = 4;  // vectors that a lane has in flight
+
+// A warp takes 32 x kUnroll vectors of a row (aligned rows of 32 vectors and more).
+template <typename T>
 __global__ void __launch_bounds__(256) lookup_wide_kernel(TbEmbeddingArgs a, int segs) {
-  constexpr int U = kUnroll<T, N>;
-  const int lane = threadIdx.x & 31, per = a.H / N;
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, per = a.H / E;
   const long long tasks = static_cast<long long>(a.N) * segs;
   for (long long task = blockIdx.x * 8ll + threadIdx.x / 32; task < tasks; task += gridDim.x * 8ll) {
     const long long t = segs == 1 ? task : task / segs;
-    const int first = static_cast<int>(task - t * segs) * 32 * U + lane;
+    const int first = static_cast<int>(task - t * segs) * 32 * kUnroll + lane;
     const long long id = id_of(a.ids, a.ids64, t);
     const bool good = id >= 0 && id < a.V;
     if (id >= a.V && a.err && lane == 0) *a.err = 1;
     const T* src = static_cast<const T*>(a.weight) + (good ? id : 0) * a.ld_w;
     T* dst = static_cast<T*>(a.out) + t * a.ld_out;
-    tb::Packed<T, N> p[U];
+    tb::Packed<T, E> p[kUnroll];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (first + u * 32 < per && good) p[u].load(src + (first + u * 32) * N);
+    for (int u = 0; u < kUnroll; ++u)
+      if (first + u * 32 < per && good) p[u].load(src + (first + u * 32) * E);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < kUnroll; ++u)
       if (first + u * 32 < per) {
-        float x[N];
+        float x[E];
         p[u].unpack(x);
-        scaled_row<T, N>(a, id, x);
-        tb::store_vec<T, N>(dst + (first + u * 32) * N, x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = good ? x[j] * a.scale : id < 0 ? 0.f : NAN;
+        tb::store_vec<T, E>(dst + (first + u * 32) * E, x);
       }
   }
 }
 
-// A thread for every vector (shorter rows).
+// The same for rows of any alignment, a row per warp: the output's whole vectors, then the
+// elements before and behind them.
+template <typename T>
+__global__ void __launch_bounds__(256) lookup_shift_kernel(TbEmbeddingArgs a) {
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const T* table = static_cast<const T*>(a.weight);
+  const T* end = table + (a.V - 1) * a.ld_w + a.H;
+  for (long long t = blockIdx.x * 8ll + threadIdx.x / 32; t < a.N; t += gridDim.x * 8ll) {
+    const long long id = id_of(a.ids, a.ids64, t);
+    const bool good = id >= 0 && id < a.V;
+    if (id >= a.V && a.err && lane == 0) *a.err = 1;
+    const T* src = table + (good ? id : 0) * a.ld_w;
+    T* dst = static_cast<T*>(a.out) + t * a.ld_out;
+    const auto one = [&](int h) { dst[h] = tb::from_f32<T>(good ? tb::to_f32(src[h]) * a.scale : id < 0 ? 0.f : NAN); };
+    const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / static_cast<int>(sizeof(T));
+    const int per = (a.H - head) / E;
+    if (!good || !Two<T>::inside(src + head, per * E, table, end)) {
+#pragma unroll 4
+      for (int h = lane; h < a.H; h += 32) one(h);
+      continue;
+    }
+    const unsigned s = Two<T>::shift_of(src + head);
+    for (int v = lane; v < per; v += 32 * kUnroll) {
+      Two<T> p[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (v + u * 32 < per) p[u].load(src + head + (v + u * 32) * E);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (v + u * 32 < per) {
+          float x[E];
+          p[u].values(s, x);
+#pragma unroll
+          for (int j = 0; j < E; ++j) x[j] *= a.scale;
+          tb::store_vec<T, E>(dst + head + (v + u * 32) * E, x);
+        }
+    }
+    const int tail = head + per * E;
+    if (lane < head) one(lane);
+    if (tail + lane < a.H) one(tail + lane);
+  }
+}
+
+// A thread for every N elements (shorter rows).
 template <typename T, int N>
 __global__ void __launch_bounds__(256) lookup_narrow_kernel(TbEmbeddingArgs a) {
   const int per = a.H / N;
@@ -85,10 +150,12 @@ __global__ void __launch_bounds__(256) lookup_narrow_kernel(TbEmbeddingArgs a) {
     const long long t = total <= UINT_MAX ? static_cast<unsigned>(i) / static_cast<unsigned>(per) : i / per;
     const int h = static_cast<int>(i - t * per) * N;
     const long long id = id_of(a.ids, a.ids64, t);
+    const bool good = id >= 0 && id < a.V;
     if (id >= a.V && a.err) *a.err = 1;
     float x[N];
-    if (id >= 0 && id < a.V) tb::load_vec<T, N>(static_cast<const T*>(a.weight) + id * a.ld_w + h, x);
-    scaled_row<T, N>(a, id, x);
+    if (good) tb::load_vec<T, N>(static_cast<const T*>(a.weight) + id * a.ld_w + h, x);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = good ? x[j] * a.scale : id < 0 ? 0.f : NAN;
     tb::store_vec<T, N>(static_cast<T*>(a.out) + t * a.ld_out + h, x);
   }
 }
@@ -676,33 +743,34 @@ bool aligned(const void* p, long long stride_bytes, long long to) {
   return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride_bytes)) % to == 0;
 }
 
+unsigned grid_of(long long ctas) { return static_cast<unsigned>(ctas < (1 << 24) ? ctas : 1 << 24); }
+
 template <typename T, int N>
-cudaError_t lookup(const TbEmbeddingArgs& a, cudaStream_t s) {
-  const int per = a.H / N;
-  if (per >= 32) {
-    constexpr int kRow = 32 * kUnroll<T, N>;
-    const int segs = (per + kRow - 1) / kRow;
-    const long long ctas = (static_cast<long long>(a.N) * segs + 7) / 8;
-    lookup_wide_kernel<T, N><<<static_cast<unsigned>(ctas < (1 << 24) ? ctas : 1 << 24), 256, 0, s>>>(a, segs);
-  } else {
-    const long long ctas = (static_cast<long long>(a.N) * per + 255) / 256;
-    lookup_narrow_kernel<T, N><<<static_cast<unsigned>(ctas < (1 << 24) ? ctas : 1 << 24), 256, 0, s>>>(a);
-  }
+cudaError_t lookup_narrow(const TbEmbeddingArgs& a, cudaStream_t s) {
+  lookup_narrow_kernel<T, N><<<grid_of((static_cast<long long>(a.N) * (a.H / N) + 255) / 256), 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 
-// Vectors of 16 bytes, of 4, or single elements, as the rows' lengths and places allow.
 template <typename T>
 cudaError_t lookup_of(const TbEmbeddingArgs& a, cudaStream_t s) {
-  constexpr long long e = sizeof(T);
-  const auto fits = [&](long long b) {
-    return a.H * e % b == 0 && aligned(a.weight, a.ld_w * e, b) && aligned(a.out, a.ld_out * e, b);
-  };
-  if (fits(16)) return lookup<T, 16 / e>(a, s);
-  if constexpr (e == 2) {
-    if (fits(4)) return lookup<T, 2>(a, s);
+  constexpr int e = sizeof(T), E = 16 / e;
+  const auto fits = [&](int b) { return a.H * e % b == 0 && aligned(a.weight, a.ld_w * e, b) && aligned(a.out, a.ld_out * e, b); };
+  const bool whole = fits(16);
+  if (a.H < 32 * E) {
+    if (whole) return lookup_narrow<T, E>(a, s);
+    if (fits(8)) return lookup_narrow<T, E / 2>(a, s);
+    if constexpr (e == 2) {
+      if (fits(4)) return lookup_narrow<T, 2>(a, s);
+    }
+    return lookup_narrow<T, 1>(a, s);
   }
-  return lookup<T, 1>(a, s);
+  if (whole) {
+    const int segs = (a.H / E + 32 * kUnroll - 1) / (32 * kUnroll);
+    lookup_wide_kernel<T><<<grid_of((static_cast<long long>(a.N) * segs + 7) / 8), 256, 0, s>>>(a, segs);
+  } else {
+    lookup_shift_kernel<T><<<grid_of((static_cast<long long>(a.N) + 7) / 8), 256, 0, s>>>(a);
+  }
+  return cudaGetLastError();
 }
 
 size_t up16(size_t b) { return (b + 15) / 16 * 16; }
