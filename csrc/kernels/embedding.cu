@@ -274,7 +274,7 @@ struct Plan {
   int N, V;
   int bits, passes, blocks, share;  // radix: bits of a digit; blocks of `share` tokens
   int P, pieces;                    // sums: pieces of P tokens
-  int slabs, width;                 // slabs of `width` vectors of columns
+  int slabs;                        // of 256 columns
   long long row;                    // floats of a row of `part`
 };
 struct Work {  // in the workspace; pairs are (id, token), ids without a row are V
@@ -502,25 +502,32 @@ __global__ void __launch_bounds__(128) fill_kernel(char* base, long long bytes) 
 // ---- the sums.  A lane has eight columns of a slab, as M vectors of N.
 template <typename T, typename G, int N>
 struct Tile {
-  static constexpr int M = 8 / N;
-  int h[M];  // first column of each vector; -1: none
-  __device__ __forceinline__ Tile(const TbEmbeddingGradArgs& a, const Plan& plan, int slab) {
-    const int lane = threadIdx.x & 31, per = a.H / N, end = min(per, (slab + 1) * plan.width);
+  static constexpr int M = 8 / N, kNext = 32 * N;  // columns between a lane's vectors
+  int h;     // the lane's first column
+  int n;     // its vectors
+  bool all;  // every lane has M
+  __device__ __forceinline__ Tile(const TbEmbeddingGradArgs& a, int slab) {
+    const int lane = threadIdx.x & 31, count = min(a.H / N - slab * (256 / N), 256 / N);
+    h = (slab * (256 / N) + lane) * N;
+    n = min(M, max(0, count - lane + 31) / 32);
+    all = count == 256 / N;
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {  // f(vector, its first column)
+    if (all) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const int v = slab * plan.width + m * 32 + lane;
-      h[m] = m * 32 + lane < plan.width && v < end ? v * N : -1;
+      for (int m = 0; m < M; ++m) f(m, h + m * kNext);
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        if (m < n) f(m, h + m * kNext);
     }
   }
   __device__ __forceinline__ void finish_row(const TbEmbeddingGradArgs& a, bool vec, long long id, const float (&sum)[M][N]) const {
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-      if (h[m] >= 0) finish<G, N>(a, vec, id, h[m], sum[m]);
+    each([&](int m, int column) { finish<G, N>(a, vec, id, column, sum[m]); });
   }
   __device__ __forceinline__ void leave(float* row, const float (&sum)[M][N]) const {
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-      if (h[m] >= 0) tb::store_vec<float, N>(row + h[m], sum[m]);
+    each([&](int m, int column) { tb::store_vec<float, N>(row + column, sum[m]); });
   }
   __device__ __forceinline__ static void zero(float (&sum)[M][N]) {
 #pragma unroll
@@ -553,7 +560,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) pieces_kernel(TbEmbeddingGradA
   tb::pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x / plan.slabs, slab = blockIdx.x % plan.slabs;
-  const Sum tile(a, plan, slab);
+  const Sum tile(a, slab);
   const unsigned V = plan.V;
   const T* dy = static_cast<const T*>(a.dy);
   float* part = work.part + static_cast<long long>(c) * 2 * plan.row;
@@ -581,9 +588,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) pieces_kernel(TbEmbeddingGradA
         for (int u = 0; u < U; ++u) {  // (u0 + u < 32: U divides 32; lanes behind the end hold V)
           key[u] = __shfl_sync(0xffffffffu, mine.x, u0 + u);
           const T* row = dy + static_cast<long long>(__shfl_sync(0xffffffffu, mine.y, u0 + u)) * a.ld_dy;
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-            if (key[u] < V && tile.h[m] >= 0) x[u][m].load(row + tile.h[m]);
+          if (key[u] < V) tile.each([&](int m, int column) { x[u][m].load(row + column); });
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -670,9 +675,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
       float x[U][M][N];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-          if (i + u < n && tile.h[m] >= 0) tb::load_vec<float, N>(work.part + (first + i + u) * 2 * plan.row + tile.h[m], x[u][m]);
+        if (i + u < n) tile.each([&](int m, int column) { tb::load_vec<float, N>(work.part + (first + i + u) * 2 * plan.row + column, x[u][m]); });
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i + u < n) {
@@ -684,9 +687,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
     }
   };
   const auto first_of = [&](const Sum& tile, long long c, float (&sum)[M][N]) {
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-      if (tile.h[m] >= 0) tb::load_vec<float, N>(work.part + (c * 2 + 1) * plan.row + tile.h[m], sum[m]);
+    tile.each([&](int m, int column) { tb::load_vec<float, N>(work.part + (c * 2 + 1) * plan.row + column, sum[m]); });
   };
   for (long long base = blockIdx.x * static_cast<long long>(kWarps); base < tasks; base += gridDim.x * static_cast<long long>(kWarps)) {
     const long long task = base + warp;
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
         begin[warp] = c;
       }
       if (n <= kShared) {
-        const Sum tile(a, plan, static_cast<int>(task / owners));
+        const Sum tile(a, static_cast<int>(task / owners));
         float sum[M][N];
         Sum::zero(sum);
         first_of(tile, c, sum);
@@ -719,7 +720,7 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(TbEmbeddingGradArgs a
     for (int w = 0; w < kWarps; ++w) {
       const int n = count[w];
       if (n <= kShared) continue;
-      const Sum tile(a, plan, static_cast<int>((base + w) / owners));
+      const Sum tile(a, static_cast<int>((base + w) / owners));
       const int c = begin[w], lo = static_cast<int>(static_cast<long long>(n) * warp / kWarps);
       const int hi = static_cast<int>(static_cast<long long>(n) * (warp + 1) / kWarps);
       float sum[M][N];
@@ -775,7 +776,7 @@ cudaError_t lookup_of(const TbEmbeddingArgs& a, cudaStream_t s) {
 
 size_t up16(size_t b) { return (b + 15) / 16 * 16; }
 
-Plan plan_of(int N, int H, int V, int vec) {
+Plan plan_of(int N, int H, int V) {
   Plan p{};
   p.N = N;
   p.V = V;
@@ -791,9 +792,7 @@ Plan plan_of(int N, int H, int V, int vec) {
   p.P = 128;
   while ((N + p.P - 1) / p.P > 8192) p.P *= 2;
   p.pieces = (N + p.P - 1) / p.P;
-  const int per = H / vec, most = 256 / vec;
-  p.slabs = (per + most - 1) / most;
-  p.width = ((per + p.slabs - 1) / p.slabs + 31) / 32 * 32;
+  p.slabs = (H + 255) / 256;
   p.row = (H + 3) / 4 * 4;
   return p;
 }
@@ -858,7 +857,7 @@ cudaError_t grad(const TbEmbeddingGradArgs& a, cudaStream_t s) {
     grad_few_kernel<T, G, N><<<static_cast<unsigned>(a.N) * slabs, 256, 0, s>>>(a, slabs, vec);
     return cudaGetLastError();
   }
-  const Plan plan = plan_of(a.N, a.H, a.V, N);
+  const Plan plan = plan_of(a.N, a.H, a.V);
   Work work;
   work_of(plan, static_cast<char*>(a.ws), &work);
   if (a.N <= kCompared) {
@@ -916,7 +915,7 @@ extern "C" int tb_embedding(const TbEmbeddingArgs* args, cudaStream_t s) {
 
 extern "C" size_t tb_embedding_grad_ws_bytes(int N, int H, int V) {
   if (N <= kFew) return 0;
-  return work_of(plan_of(N, H, V, 1), nullptr, nullptr);
+  return work_of(plan_of(N, H, V), nullptr, nullptr);
 }
 
 extern "C" int tb_embedding_grad(const TbEmbeddingGradArgs* args, cudaStream_t s) {
