@@ -128,7 +128,9 @@ TbDistillArgs distill_args(const at::Tensor& logits, const at::Tensor& ids, cons
 at::Tensor grad_like(const at::Tensor& logits) {
   const int64_t R = logits.size(0), V = logits.size(1), e = 16 / logits.element_size();
   const int64_t more = R > 1 ? ((logits.stride(0) - V) % e + e) % e : 0;
-  return more ? at::empty_strided({R, V}, {V + more, 1}, logits.options()) : at::empty({R, V}, logits.options());
+  const int64_t first = static_cast<int64_t>(reinterpret_cast<uintptr_t>(logits.const_data_ptr()) & 15) / logits.element_size();
+  if (R == 0 || (more == 0 && first == 0)) return at::empty({R, V}, logits.options());
+  return at::empty({first + R * (V + more)}, logits.options()).as_strided({R, V}, {V + more, 1}, first);
 }
 
 using LossAndGrad = std::optional<std::tuple<at::Tensor, at::Tensor>>;

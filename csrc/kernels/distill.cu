@@ -70,7 +70,7 @@ struct Shared {
   int y, y_listed, twice;
   __align__(16) int id[kMaxList];  // -1: padding
   float z[kMaxList], l[kMaxList];
-  double t[kMaxList];  // mass of the class; -1 where the entry is not its id's first
+  double t[kMaxList];  // mass of the class (l: its logarithm); -1 where the entry is not its id's first
   // the softmax sum of the list's elements, the masses' sum, t_R, and their logarithms
   float in_m, in_s;
   float mass, log_mass, t_rest, log_t_rest;
@@ -104,7 +104,7 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
                                            bool write) {
   const int lane = threadIdx.x & 31;
   const float w = s.w, c = s.c;
-  const bool listed = w != 0.f, twice = s.twice;
+  const bool listed = w != 0.f;
   SoftSum all = sum;
   all.merge(s.in_m, s.in_s, k1);
   const bool good = !isnan(all.s) && !isinf(all.m);
@@ -124,7 +124,7 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
       const float t = static_cast<float>(s.t[k]);
       if (s.id[k] < 0 || t < 0.f) continue;
       const float lp = log_p(s.z[k], all.m, lns);
-      const float lt = (twice ? logf(t) : s.l[k]) - s.log_mass;
+      const float lt = s.l[k] - s.log_mass;
       if (a.kind == TB_DISTILL_REVERSE) {
         const float p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
         if (p != 0.f) kl += p * (lp - lt);
@@ -158,7 +158,7 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
     float4* st = reinterpret_cast<float4*>(a.stats + r * TB_DISTILL_STATS);
     st[0] = make_float4(s.n.origin, s.n.factor, s.n.top, s.n.lns.x);
     st[1] = make_float4(s.n.lns.y, s.n.kl, s.n.whole, s.mass);
-    st[2] = make_float4(twice ? 1.f : 0.f, 0.f, 0.f, 0.f);
+    st[2] = make_float4(s.twice ? 1.f : 0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -248,7 +248,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
             m += exp(static_cast<double>(s.l[j]));
           }
           s.t[tid] = first ? m : -1.0;
+          l = static_cast<float>(log(m));
         }
+        __syncthreads();
+        if (id >= 0) s.l[tid] = l;
         __syncthreads();
       }
     }
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
           const float lp = tb::Scaled{inv_t}(s.z[tid], n.top, n.lns), p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
           float d;
           if (a.kind == TB_DISTILL_REVERSE) {
-            d = p == 0.f ? 0.f : p * (lp - (s.twice ? logf(t) : s.l[tid]) - n.kl);
+            d = p == 0.f ? 0.f : p * (lp - s.l[tid] - n.kl);
           } else {
             d = p * n.whole - (a.kind == TB_DISTILL_FORWARD ? (s.mass != 0.f ? t / s.mass : 0.f) : t);
           }
@@ -385,11 +388,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
 constexpr int kSms = 148;
 constexpr int kPart = 32 * 1024;  // vectors of a part at most (of its bitmap, bytes)
 
-// CTAs of a cluster: as many as the machine has room for beside the other rows, 64 groups at
-// least to each; and enough of them that a part's bitmap fits its shared memory.
+// CTAs of a cluster: as many as half the machine holds beside the other rows (clusters that
+// would fill it wait for one another: loss and gradient of 36 rows of 2,374 groups take 20.9 us
+// with one CTA, 14.8 with four, 21.0 with eight; 4 rows 20.4, 12.3 and 9.3), some 100 groups at
+// least to each (4 rows of 250 groups take 8.7 us with one and 9.1 with two, of 500 groups 10.7,
+// and 8.8 with four); and enough of them that a part's bitmap fits its shared memory.
 int ranks_of(int R, int groups, int slots) {
   int ranks = 1;
-  while (ranks < 8 && ((groups + ranks - 1) / ranks * 8 > kPart || (R * 2ll * ranks <= slots && groups >= 64 * ranks))) ranks *= 2;
+  while (ranks < 8 && ((groups + ranks - 1) / ranks * 8 > kPart || (R * 4ll * ranks <= slots && groups >= 128 * (ranks + 1)))) ranks *= 2;
   return ranks;
 }
 

@@ -5,9 +5,9 @@
 // a_1 .. a_k the ids in order of (z descending, id ascending).
 //
 // One pass over the row forms the softmax's running maximum and sum, and the maximum of
-// every group of 8 vectors (128 bytes; of every vector in short rows).  The k largest elements lie in the k first groups
-// by (maximum descending, index ascending): for an element outside them, each of those
-// groups holds one that comes before it.  So the selection looks at V / 64 maxima in
+// every group of 8 vectors (128 bytes; of every vector in short rows).  The k largest
+// elements lie in the k first groups by (maximum descending, index ascending): for an element
+// outside them, each of those groups holds one that comes before it.  So the selection looks at V / 64 maxima in
 // shared memory and reads some k groups again, whatever the data (all equal, ascending).
 // A histogram of the maxima, filled during the pass, gives a value that k groups reach and
 // few more; of those groups the elements that reach it, some k, are ordered by counting.
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
     const bool plain = !isinf(sum.m) && !isnan(sum.s);
     const float2 lns = plain ? tb::log_of(sum.s) : make_float2(0.f, 0.f);
     if (rank == 0 && threadIdx.x == 0)
-      a.lse[r] = plain ? fmaf(sum.m, inv_t, lns.x) + lns.y : isnan(sum.s) ? NAN : sum.m;
+      a.lse[r] = plain ? fmaf(sum.m, inv_t, lns.x + lns.y) : isnan(sum.s) ? NAN : sum.m;
     for (int i = threadIdx.x; i < own; i += kThreads) {
       const Key x = s.sorted[i];
       int place = i;
@@ -454,13 +454,15 @@ __global__ void __launch_bounds__(kThreads, 4) topk_kernel(TbTopkLogprobsArgs a,
   }
 }
 
-// CTAs of a cluster: as many as the machine has room for beside the other rows, 512 groups at
-// least to each (joining the lists costs 3 us: one row of 500 groups takes 8.2 us with one CTA
-// and 11.3 with eight, of 2,374 groups 18.4, 12.3 with four and with eight); enough of them
-// that the maxima of a part fit its shared memory.
+// CTAs of a cluster: as many as half the machine holds beside the other rows (clusters that
+// would fill it wait for one another: 74 rows of 2,374 groups take 18.5 us with one CTA, 15.6
+// with four, 25.1 with eight), 512 groups at least to each (joining the lists costs 3 us: four
+// rows of 500 groups take 8.1 us with one CTA and 9.2 with two, of 1,024 groups 10.9 and 9.4,
+// of 2,374 groups 18.1, and 11.5 with four); enough of them that the maxima of a part fit its
+// shared memory.
 int ranks_of(int R, int groups) {
   int ranks = 1;
-  while (ranks < 8 && ((groups + ranks - 1) / ranks > 8192 || (R * 2ll * ranks <= 148 * 4 && groups >= 1024 * ranks))) ranks *= 2;
+  while (ranks < 8 && ((groups + ranks - 1) / ranks > 8192 || (R * 4ll * ranks <= 148 * 4 && groups >= 1024 * ranks))) ranks *= 2;
   return ranks;
 }
 

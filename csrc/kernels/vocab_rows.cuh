@@ -238,16 +238,16 @@ struct SoftSum {
 };
 
 // The exponent x k1 + c of 2^((x - m) k1) in one operation: c = -m k1 rounded, whose
-// rounding `fix` takes out of a sum of such powers.  Where that product comes near the end
-// of fp32 (masks of the type's lowest value are the only values of a row), the difference is
-// formed first.
+// rounding d `fix` takes out of a sum of such powers, as 1 - d ln 2 (below 2^11, where d is
+// at most 2^-14, off by 2^-29).  Where that product is larger (up to masks of the type's
+// lowest value as the only values of a row), the difference is formed first.
 struct Exponent {
   float m, k1, c, fix;
   bool near;
   __device__ __forceinline__ Exponent(float m_, float k1_) : k1(k1_) {
     m = isinf(m_) ? 0.f : m_;
     c = -(m * k1);
-    near = fabsf(c) < 1e37f;
+    near = fabsf(c) < 2048.f;
     fix = near ? 1.f - fmaf(m, k1, c) * kLn2 : 1.f;
   }
   __device__ __forceinline__ float2 powers(float2 x) const {
@@ -301,8 +301,8 @@ struct RunningSum {
   float2 s0 = {0.f, 0.f}, s1 = {0.f, 0.f};
   template <int N>
   __device__ __forceinline__ void add(const uint4 (&p)[N], float top, float k1) {
-    if (top > m) {
-      const float f = m == -INFINITY ? 0.f : Exponent(m, k1).fix * ex2((m - top) * k1);
+    if (top > m) {  // (what is there gets the new maximum's rounding, which done() takes out)
+      const float f = m == -INFINITY ? 0.f : Exponent(m, k1).fix * (2.f - Exponent(top, k1).fix) * ex2((m - top) * k1);
       s0 = mul2(s0, make_float2(f, f));
       s1 = mul2(s1, make_float2(f, f));
       m = top;

@@ -551,3 +551,55 @@ def test_list_to_loss(device):
         a, d = distill_loss_grad(other, top.ids, top.logprobs, kind=kind, rest=rest)
         b = distill_loss(other - 0.1 * d, top.ids, top.logprobs, kind=kind, rest=rest)
         assert (b < a).all()
+
+
+def far_rows(V, device):
+    """fp32 rows around 2^20 whose differences are whole numbers up to 8: ascending, so that the running maximum rises
+    often; descending; shuffled.  And the same around 0, shifted in exact steps."""
+    g = torch.Generator().manual_seed(V)
+    z = torch.randint(0, 9, (3, V), generator=g).float()
+    z[0], z[1] = z[0].sort().values, z[1].sort(descending=True).values
+    return (z + 2.0 ** 20).to(device), z.to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [1.0, 2.0 ** -10, 2.0 ** 8])
+def test_logits_far_from_zero(T, device):
+    """Maxima whose product with 1 / T is coarse in fp32: what counts are the differences.  (1 / T exact.)"""
+    far, near = far_rows(40000, device)
+    for z in (far, -far, near * 1000.0):
+        check_top(z, 20, T)
+    if T != 1.0:
+        return
+    ids, logp = lists(near, 40)
+    y = torch.tensor([5, 39999, 20000], dtype=torch.int32, device=device)
+    for kind, rest in KINDS:
+        run_both(far, ids, logp, None, kind, rest, 1.0, y, None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind,rest", KINDS)
+def test_faint_entries(kind, rest, device):
+    """Masses below 2^-149, once and twice in the list."""
+    x = rows(4, 200, torch.float32, device, spread=1.0)
+    ids, logp = lists(x, 6)
+    logp = logp.clone()
+    logp[:2, 3:] = -200.0
+    ids[1, 4], ids[2, 1], logp[2, :2] = ids[1, 3], ids[2, 0], -300.0
+    run_both(x, ids, logp, None, kind, rest, 1.0, None, None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [777, 40003])
+def test_gradient_of_slices(V, dtype, device):
+    """Rows that begin behind the first element of an odd row (shifted tokens of a batch)."""
+    x = rows(7, V, dtype, device, pad=0)[1:]
+    ids, logp = lists(x, 10)
+    loss, d = distill_loss_grad(x, ids, logp)
+    compare(loss, d, x, definition(x, ids, logp, None, "forward", True, 1.0, None, None))
+    leaf = x.detach().requires_grad_()
+    l = distill_loss(leaf, ids, logp)
+    l.sum().backward()
+    compare(l, leaf.grad, x, definition(x, ids, logp, None, "forward", True, 1.0, None, None))
+    assert leaf.grad.shape == x.shape
