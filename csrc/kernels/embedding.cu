@@ -17,6 +17,13 @@
 // Up to 8,192 tokens the sort counts, for each token, the ones before it (N^2 comparisons
 // in one launch); above it is a radix sort in digits of up to 9 bits, one launch to count
 // the first digit and one for each digit, which also counts the next one.
+//
+// What bounds it, measured with bf16 rows: the lookup moves its bytes (16,384 rows of 4,096:
+// 32 us, 268 MB); the sums do where rows are 16-byte vectors (the same batch: 48 us beside no
+// zeros, 134 MB read and as much written), while rows of odd length take an element per lane
+// (65,537 of 1,025 fp16: 59 us, 134 MB read, 40% of the copy rate) and small batches the chain
+// of launches (6,144 tokens of 1,536: sort 11, sums 16, join 5 us, of 19 MB).  The sort
+// waits on shared memory and on its own launches: 11 us for 6,144 tokens, 24 for 65,537.
 #include <limits.h>
 #include <math.h>
 
@@ -282,6 +289,7 @@ struct Work {  // in the workspace; pairs are (id, token), ids without a row are
   unsigned* counts;  // [passes][blocks][bins]
   int* owners;       // [0]: how many; then the pieces where an id begins that goes on in the next one
   float* part;       // [pieces][2][row]: the sums of the id that came in, and of the one that goes on
+  unsigned* named;   // a bit for each row of grad that an id names
 };
 
 __device__ __forceinline__ unsigned key_from(const TbEmbeddingGradArgs& a, long long id) {
@@ -479,24 +487,45 @@ __global__ void __launch_bounds__(kSortThreads, 1) scatter_kernel(TbEmbeddingGra
   }
 }
 
-// ---- a dense gradient's zeros
-constexpr int kFillBytes = 32768;
-__global__ void __launch_bounds__(128) fill_kernel(char* base, long long bytes) {  // base and bytes: multiples of 16
-  extern __shared__ __align__(128) uint4 zeros[];
-  tb::pdl_trigger();
-  for (int i = threadIdx.x; i < kFillBytes / 16; i += 128) zeros[i] = make_uint4(0, 0, 0, 0);
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x) return;
-  const unsigned src = static_cast<unsigned>(__cvta_generic_to_shared(zeros));
-  for (long long at = blockIdx.x * static_cast<long long>(kFillBytes); at < bytes; at += gridDim.x * static_cast<long long>(kFillBytes)) {
-    const unsigned n = static_cast<unsigned>(min(static_cast<long long>(kFillBytes), bytes - at));
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + at), "r"(src), "r"(n) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    asm volatile("cp.async.bulk.wait_group.read 4;" ::: "memory");
+// ---- a dense gradient's zeros: by CTAs beside those of the sums, which write the rows that
+// an id names; these write the runs of others, a warp `unit` rows at a time.  The rows' bits
+// were set before the sort began, so nothing is waited for: the stores go on beside the sort,
+// too.  (8,192 tokens of 151,936 rows of 1,536 bf16, 467 MB: 94 us, 5.0 TB/s, and 193 with
+// zeros in all rows before the sums; 16,384 of 128,256 rows of 4,096: 205 and 252.)
+__global__ void __launch_bounds__(256) mark_kernel(TbEmbeddingGradArgs a, unsigned* named) {
+  const long long t = blockIdx.x * 256ll + threadIdx.x;
+  if (t >= a.N) return;
+  const long long id = id_of(a.ids, a.ids64, t);
+  if (id < 0 || id >= a.V) return;
+  const unsigned bit = 1u << (id & 31);
+  if (!(__ldcg(named + (id >> 5)) & bit)) atomicOr(named + (id >> 5), bit);  // (a token may fill the batch)
+}
+constexpr int kFillers = 4 * 148;  // CTAs (with 3 x 148 the same tokens take 99 us, with 8 x 148 90)
+// Rows of a task (a power of two): 8, so that even a small table has one for every warp (1,024
+// tokens of 32,000 rows of 1,024: 24.6 us, and 36.8 with 32); short rows 32.
+__device__ __forceinline__ int unit_of(long long row) { return row < 1024 ? 32 : 8; }
+template <typename G>
+__device__ __forceinline__ void fill_others(G* grad, int H, int V, const unsigned* named) {
+  const int lane = threadIdx.x & 31, unit = unit_of(H * static_cast<long long>(sizeof(G))), tasks = (V - 1) / unit + 1;
+  for (int task = blockIdx.x * 8 + threadIdx.x / 32; task < tasks; task += kFillers * 8) {
+    const long long v = static_cast<long long>(task) * unit;
+    const int rows = static_cast<int>(min(static_cast<long long>(unit), V - v));
+    unsigned left = ~__ldcg(named + (v >> 5)) >> (v & 31);
+    if (rows < 32) left &= (1u << rows) - 1;
+    while (left) {
+      const int first = __ffs(left) - 1, end = __ffs(~(left >> first)), n = end ? end - 1 : 32;
+      G* p = grad + (v + first) * H;
+      const long long count = static_cast<long long>(n) * H;
+      const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(G));
+      const long long vecs = count > head ? (count - head) * sizeof(G) / 16 : 0, tail = head + vecs * (16 / sizeof(G));
+      if (lane < head && lane < count) p[lane] = tb::from_f32<G>(0.f);
+      uint4* q = reinterpret_cast<uint4*>(p + head);
+#pragma unroll 4
+      for (long long i = lane; i < vecs; i += 32) __stcs(q + i, make_uint4(0, 0, 0, 0));
+      if (tail + lane < count) p[tail + lane] = tb::from_f32<G>(0.f);
+      left = first + n < 32 ? left >> (first + n) << (first + n) : 0u;
+    }
   }
-  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  tb::pdl_wait();  // so that whoever waits for this kernel also waits for the one before
 }
 
 // ---- the sums.  A lane has eight columns of a slab, as M vectors of N.
@@ -552,14 +581,18 @@ struct Tile {
 constexpr int kWarps = 8;
 
 template <typename T, typename G, int N>
-__global__ void __launch_bounds__(kWarps * 32, 3) pieces_kernel(TbEmbeddingGradArgs a, Plan plan, Work work, bool vec) {
+__global__ void __launch_bounds__(kWarps * 32, 3) pieces_kernel(TbEmbeddingGradArgs a, Plan plan, Work work, bool vec, int fillers) {
   using Sum = Tile<T, G, N>;
   constexpr int M = Sum::M, U = N * sizeof(T) == 16 ? 8 / M : 4;
   __shared__ float in[kWarps][256], on[kWarps][256];  // sums of the ids that came in, that go on
   __shared__ bool through[kWarps];                    // the id that came in goes on
   tb::pdl_trigger();
+  if (static_cast<int>(blockIdx.x) < fillers) {
+    fill_others(static_cast<G*>(a.grad), a.H, plan.V, work.named);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x / plan.slabs, slab = blockIdx.x % plan.slabs;
+  const int c = (blockIdx.x - fillers) / plan.slabs, slab = (blockIdx.x - fillers) % plan.slabs;
   const Sum tile(a, slab);
   const unsigned V = plan.V;
   const T* dy = static_cast<const T*>(a.dy);
@@ -810,6 +843,7 @@ size_t work_of(const Plan& p, char* w, Work* out) {
   k.counts = reinterpret_cast<unsigned*>(take(static_cast<size_t>(kMaxPasses) * kMaxBlocks * kMaxBins * sizeof(unsigned)));
   k.owners = reinterpret_cast<int*>(take((p.pieces + 1) * sizeof(int)));
   k.part = reinterpret_cast<float*>(take(static_cast<size_t>(p.pieces) * 2 * p.row * sizeof(float)));
+  k.named = reinterpret_cast<unsigned*>(take((static_cast<size_t>(p.V) + 31) / 32 * sizeof(unsigned)));
   if (out) *out = k;
   return at;
 }
@@ -829,28 +863,23 @@ cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t s
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Zeros in all rows of grad.  Large rows without gaps: by a kernel, beside the launch before
-// it (`after`); others before that.
+// Zeros in all rows of grad.
 template <typename G>
-bool by_kernel(const TbEmbeddingGradArgs& a) {
-  const size_t all = a.H * sizeof(G) * a.V;
-  return (a.ld_grad == a.H || a.V == 1) && all >= (1 << 20) && (reinterpret_cast<uintptr_t>(a.grad) | all) % 16 == 0;
-}
-template <typename G>
-cudaError_t fill(const TbEmbeddingGradArgs& a, cudaStream_t s, bool after) {
-  const size_t row = a.H * sizeof(G), all = row * a.V;
-  if (by_kernel<G>(a))
-    return launch(fill_kernel, kSms * 2, 128u, kFillBytes, s, after, static_cast<char*>(a.grad), static_cast<long long>(all));
-  if (a.ld_grad == a.H || a.V == 1) return cudaMemsetAsync(a.grad, 0, all, s);
+cudaError_t fill(const TbEmbeddingGradArgs& a, cudaStream_t s) {
+  const size_t row = a.H * sizeof(G);
+  if (a.ld_grad == a.H || a.V == 1) return cudaMemsetAsync(a.grad, 0, row * a.V, s);
   return cudaMemset2DAsync(a.grad, a.ld_grad * sizeof(G), 0, row, a.V, s);
 }
+// Zeros beside the sums (rows without gaps): the rows' bits cost two launches, which pay from
+// some 32 MB on (4,096 tokens of 33.6 MB: 25 us beside, and 32 before; 600 of 4.2 MB: 16.5 and 12).
+constexpr size_t kBeside = 32 << 20;
 
 template <typename T, typename G, int N>
 cudaError_t grad(const TbEmbeddingGradArgs& a, cudaStream_t s) {
   const bool vec = aligned(a.grad, a.ld_grad * sizeof(G), N * sizeof(G) < 16 ? N * sizeof(G) : 16);
-  const bool few = a.N <= kFew, beside = a.zero && !few && by_kernel<G>(a);
+  const bool few = a.N <= kFew, beside = a.zero && !few && a.ld_grad == a.H && a.H * sizeof(G) * a.V >= kBeside;
   cudaError_t e = cudaSuccess;
-  if (a.zero && !beside) e = fill<G>(a, s, false);
+  if (a.zero && !beside) e = fill<G>(a, s);
   if (e != cudaSuccess || a.N == 0) return e;
   if (few) {
     const int slabs = (a.H + 32 * N - 1) / (32 * N);
@@ -858,8 +887,14 @@ cudaError_t grad(const TbEmbeddingGradArgs& a, cudaStream_t s) {
     return cudaGetLastError();
   }
   const Plan plan = plan_of(a.N, a.H, a.V);
+  const int fillers = beside ? kFillers : 0;
   Work work;
   work_of(plan, static_cast<char*>(a.ws), &work);
+  if (beside) {
+    e = cudaMemsetAsync(work.named, 0, (static_cast<size_t>(a.V) + 31) / 32 * sizeof(unsigned), s);
+    if (e == cudaSuccess) e = launch(mark_kernel, (a.N + 255) / 256, 256u, 0, s, false, a, work.named);
+    if (e != cudaSuccess) return e;
+  }
   if (a.N <= kCompared) {
     const int own = (a.N + kSms - 1) / kSms;
     e = launch(compare_sort_kernel, (a.N + own - 1) / own, kSortThreads, (a.N + 3) / 4 * 16 + own * 4, s, false, a, plan, work, own);
@@ -869,9 +904,9 @@ cudaError_t grad(const TbEmbeddingGradArgs& a, cudaStream_t s) {
     for (int p = 0; p < plan.passes && e == cudaSuccess; ++p)
       e = launch(scatter_kernel, plan.blocks, kSortThreads, (kSortWarps << plan.bits) * sizeof(unsigned), s, true, a, plan, work, p);
   }
-  if (e == cudaSuccess && beside) e = fill<G>(a, s, true);  // (the sort neither reads nor writes grad)
   if (e != cudaSuccess) return e;
-  e = launch(pieces_kernel<T, G, N>, static_cast<unsigned>(plan.pieces) * plan.slabs, kWarps * 32, 0, s, true, a, plan, work, vec);
+  e = launch(pieces_kernel<T, G, N>, static_cast<unsigned>(plan.pieces) * plan.slabs + fillers, kWarps * 32, 0, s, true, a, plan, work, vec,
+             fillers);
   if (e != cudaSuccess) return e;
   const long long tasks = static_cast<long long>(plan.pieces) * plan.slabs;
   const long long ctas = (tasks + kWarps - 1) / kWarps;

@@ -329,3 +329,26 @@ def test_large_offsets(dev):
     assert float(y[-1, -1]) == 2.0 and float(y[-2, -1]) == 1.0
     g = embedding_grad(many, y, torch.zeros(2, H, device=dev))
     assert (g[0] == V - 1).all() and (g[1] == 2.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,H", [(513, 70001, 128), (700, 8191, 1025), (9000, 40, 300000), (20000, 300007, 31), (4096, 3, 2900001)])
+def test_zeros_beside_the_sums(N, V, H, dtype, dev):
+    """Large dense gradients: every row that no id names is zero, whatever was there, the others as if added to zeros;
+    the same when an id past the table or a filler token is among them."""
+    g = torch.Generator().manual_seed(N)
+    ids = torch.randint(0, V, (N,), generator=g)
+    ids[:: 7], ids[1], ids[2] = V - 1, -1, V + 5
+    if V > 1000:
+        ids[(ids >= 96) & (ids < 700)] = 0  # whole stretches without a name
+    ids = ids.to(dev)
+    dy = torch.randn(1, H, device=dev).to(dtype).expand(N, H) if H > 10000 else torch.randn(N, H, device=dev).to(dtype)
+    out = torch.full((V, H), math.nan, device=dev, dtype=dtype)
+    embedding_grad(ids, dy, out, scale=0.5, accumulate=False)
+    want = torch.zeros_like(out)
+    embedding_grad(ids, dy, want, scale=0.5)
+    assert torch.equal(out, want)
+    named = torch.zeros(V, dtype=torch.bool, device=dev)
+    named[ids[(ids >= 0) & (ids < V)]] = True
+    assert not out[~named].any() and out[named].any(1).all()
