@@ -201,7 +201,9 @@ __device__ __forceinline__ void finish(const TbEmbeddingGradArgs& a, bool vec, l
   tb::store_vec<G, N>(p, x);
 }
 
-constexpr int kFew = 512;  // tokens of the one-launch form
+// Tokens of the one-launch form (512 of 1,536 bf16 take 11.5 us with it and 15.4 sorted, 64 take
+// 3.0 and 9.5; of 4,096 columns 25.8 and 20.4: there every slab compares the ids again).
+constexpr int kFew = 512;
 
 template <typename T, typename G, int N>
 __global__ void __launch_bounds__(256) grad_few_kernel(TbEmbeddingGradArgs a, int slabs, bool vec) {
@@ -275,7 +277,9 @@ __global__ void __launch_bounds__(256) grad_few_kernel(TbEmbeddingGradArgs a, in
 // ---- the sort
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxBins = 512, kMaxBlocks = 64, kMaxPasses = 4;
 constexpr int kSms = 148;
-constexpr int kCompared = 8192;  // tokens that are sorted by comparing them all
+// Tokens that are sorted by comparing them all (6,144 tokens of 1,536 bf16: 29.3 us, and 33.8 by
+// the radix sort in two digits, 36.0 in three; 8,192: 38.1 and 36.7, 38.8; 2,048: 22.2 and 19.7, 21.4).
+constexpr int kCompared = 8192;
 
 struct Plan {
   int N, V;
