@@ -22,6 +22,14 @@
 // the L2 cache, by the policy that the first one read it with.  Masses are summed in 64 bits
 // (t_R is 1 less their sum), and log S is kept as the sum of two fp32 numbers: the loss is a
 // small difference of large ones.
+//
+// The floor is one read of the live rows and one write of the gradient.  4,096 rows of 151,936
+// bf16 (all live) take 530 us, 4.7 TB/s: a third of the rows' second reads misses the L2 cache
+// (495 MB read for 360 of 1,184 rows), whose writes pass through it.  Rows kept in shared
+// memory, rings of bulk loads and the next row's first loads ahead gained nothing: then too few
+// loads are in flight, or the sums wait for the stores.  The loss alone, 1,184 rows: 76 us, 4.7
+// TB/s.  Short rows (777 of 32,003 fp16, odd: 37 us for a floor of 14) wait four times per row
+// for all warps: list, repeats, sums, numbers.
 #include "kernels.h"
 #include "vocab_rows.cuh"
 

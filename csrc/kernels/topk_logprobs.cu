@@ -13,6 +13,11 @@
 // few more; of those groups the elements that reach it, some k, are ordered by counting.
 // Where too many do (equal values, the largest side by side), the k-th place is searched by
 // bisection with counts over the block, first of the value and then of the index.
+//
+// The floor is one read of the logits.  4,096 rows of 151,936 bf16 take 251 us (4.9 TB/s, 77%
+// of the copy rate): the exponentials keep their unit 59% busy, and while one CTA selects, the
+// other three of its SM load.  512 rows, one wave, take 40 us (3.8 TB/s): all CTAs select at
+// the same time.
 #include <type_traits>
 
 #include "kernels.h"
