@@ -97,6 +97,22 @@ def test_steps(dev):
     assert "distill_kl" not in GRPOTrainer(config(), dev).step()
 
 
+def test_device_names():
+    """A teacher on the trainer's device under another of its names passes the checks (what comes after them needs a GPU)."""
+    try:
+        GRPOTrainer(config(distill_coef=0.1), "cpu", teacher=DecoderLM(tiny(), "cpu:0", master=False))
+    except Exception as e:
+        assert "teacher" not in str(e)
+
+
+@pytest.mark.gpu
+def test_device_names_on_the_gpu(dev):
+    here = torch.cuda.current_device()
+    for name, teachers in ((f"cuda:{here}", "cuda"), ("cuda", f"cuda:{here}")):
+        tr = GRPOTrainer(config(distill_coef=0.1), name, teacher=DecoderLM(tiny(), teachers, seed=5, master=False))
+        assert math.isfinite(tr.step()["distill_kl"])
+
+
 @pytest.mark.gpu
 def test_scaled_embedding_in_the_rollout(dev):
     """Greedy tokens of a model with scaled embeddings are those of its fp32 forward (up to its bf16 rounding)."""

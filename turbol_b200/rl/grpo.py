@@ -125,7 +125,8 @@ class GRPOTrainer:
         if teacher is not None:
             if not cfg.distill_coef:
                 raise ValueError("a teacher needs distill_coef")
-            if teacher.cfg.vocab != cfg.model.vocab or teacher.device != torch.device(device):
+            # (by tensors: "cuda" is the current device's name as well)
+            if teacher.cfg.vocab != cfg.model.vocab or teacher.shadow.device != torch.empty(0, device=device).device:
                 raise ValueError("the teacher has the policy's vocabulary and device")
             if teacher.cfg.max_seq < cfg.seq_len:
                 raise ValueError("the teacher's positions do not cover the sequences")
