@@ -247,16 +247,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
       const int twice = __syncthreads_or(seen);
       if (tid == 0) s.twice = twice;
       if (twice) {
-        if (id >= 0) {
+        if (id >= 0) {  // (the logarithm from the largest of its entries: the mass itself may be below 2^-1074)
           bool first = true;
-          double m = 0.0;
+          float top = l;
           for (int j = 0; j < K; ++j) {
             if (s.id[j] != id) continue;
             if (j < tid) first = false;
-            m += exp(static_cast<double>(s.l[j]));
+            top = fmaxf(top, s.l[j]);
           }
-          s.t[tid] = first ? m : -1.0;
-          l = static_cast<float>(log(m));
+          double m = 0.0;
+          for (int j = 0; j < K; ++j)
+            if (s.id[j] == id) m += exp(static_cast<double>(s.l[j]) - top);
+          s.t[tid] = first ? m * exp(static_cast<double>(top)) : -1.0;
+          l = static_cast<float>(top + log(m));
         }
         __syncthreads();
         if (id >= 0) s.l[tid] = l;

@@ -603,3 +603,66 @@ def test_gradient_of_slices(V, dtype, device):
     l.sum().backward()
     compare(l, leaf.grad, x, definition(x, ids, logp, None, "forward", True, 1.0, None, None))
     assert leaf.grad.shape == x.shape
+
+
+def by_log_masses(x, ids, logp, kind, rest):
+    """(loss, gradient, scale of the errors [R, V], factor of the loss's), as `definition` gives them, in 64 bits from the
+    logarithms of the classes' masses: no mass itself is formed where only its logarithm counts."""
+    loss, grads, mags, facs = [], [], [], []
+    for r in range(x.shape[0]):
+        z = x[r].cpu().double().requires_grad_()
+        lp = torch.log_softmax(z, 0)
+        entries = {}
+        for a, l in zip(ids[r].tolist(), logp[r].double().tolist()):
+            if a >= 0 and l > -INF:
+                entries.setdefault(a, []).append(l)
+        at = torch.tensor(sorted(entries), dtype=torch.long)
+        lt = torch.stack([torch.logsumexp(torch.tensor(entries[a], dtype=torch.float64), 0) for a in sorted(entries)])
+        outside = torch.ones(len(z), dtype=torch.bool)
+        outside[at] = False
+        lr = torch.logsumexp(lp[outside], 0)
+        F = (lp.detach()[at] - lt).abs()
+        if not rest:
+            lt = lt - torch.logsumexp(lt, 0)
+            F = (lp.detach()[at] - lt).abs()
+            kl = (lt.exp() * (lt - lp[at])).sum()
+        elif kind == "forward":
+            tr = max(0.0, 1 - float(lt.exp().sum()))
+            kl = (lt.exp() * (lt - lp[at])).sum() + (tr * (math.log(tr) - lr) if tr > 0 else 0.0)
+        else:
+            tr = max(1 - float(lt.exp().sum()), 2.0 ** -20)
+            kl = (lp[at].exp() * (lp[at] - lt)).sum() + lr.exp() * (lr - math.log(tr))
+        d, = torch.autograd.grad(kl, z)
+        p = lp.detach().exp()
+        mag = p + torch.where(outside, p / p[outside].sum(), 0.0)
+        mag[at] += lt.exp()
+        f = 2 + float(F.max())
+        loss.append(float(kl.detach())), grads.append(d), mags.append(mag * f), facs.append(f)
+    return torch.tensor(loss, dtype=torch.float64), torch.stack(grads), torch.stack(mags), torch.tensor(facs).double()
+
+
+def check_list(x, ids, logp, kind, rest):
+    """The fused form and the differentiable one against the logarithms' form."""
+    want = by_log_masses(x, ids, logp, kind, rest)
+    assert want[0].isfinite().all() and want[1].isfinite().all()
+    loss, d = distill_loss_grad(x, ids, logp, kind=kind, rest=rest)
+    compare(loss, d, x, want)
+    leaf = x.detach().clone().requires_grad_()
+    l = distill_loss(leaf, ids, logp, kind=kind, rest=rest)
+    g, = torch.autograd.grad(l, leaf, torch.ones_like(l))
+    compare(l, g, x, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind,rest", KINDS)
+@pytest.mark.parametrize("low", [-700.0, -800.0, -1e4])
+def test_faint_entries_beside_a_repeated_id(low, kind, rest, device):
+    """Masses that 64 bits hold as zero: of an id that occurs once beside one that occurs twice, and of the repeated id
+    itself.  (Reverse: their logarithms count.)"""
+    x = rows(4, 200, torch.float32, device, spread=1.0)
+    ids, logp = lists(x, 6)
+    logp = logp.clone()
+    logp[:3, 5] = low
+    ids[1, 1] = ids[1, 0]
+    ids[2, 4], logp[2, 4] = ids[2, 5], low - 0.5
+    check_list(x, ids, logp, kind, rest)

@@ -333,18 +333,21 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
     p = logp.exp()
     here = (ids >= 0) & (ids < V) & ~logprobs.isneginf()
     at = torch.where(here, ids.long(), V)  # (what is left out: a column behind the last)
-    mass = torch.where(here, logprobs.double().exp(), 0.0)
-    t = torch.zeros(R, V + 1, **f64).scatter_add_(1, at, mass)[:, :V]
+    l = torch.where(here, logprobs.double(), -math.inf)
+    top = torch.full((R, V + 1), -math.inf, **f64).scatter_reduce_(1, at, l, "amax")
+    lt = torch.zeros(R, V + 1, **f64).scatter_add_(1, at, torch.where(here, (l - top.gather(1, at)).exp(), 0.0))
+    lt = (top + lt.log())[:, :V]  # the classes' log-masses: of faint ones nothing else is left
+    t = torch.where(lt.isneginf(), 0.0, lt.exp())
     inside = torch.zeros(R, V + 1, dtype=torch.bool, device=logits.device).scatter_(1, at, True)[:, :V]
-    total = mass.sum(1, keepdim=True)
+    total = torch.where(here, l.exp(), 0.0).sum(1, keepdim=True)
 
-    def plogq(a, b, on):  # a (log a - log b) where it counts
-        return torch.where(on & (a > 0), a * (a.log() - b), 0.0).sum(1, keepdim=True) + \
+    def plogq(a, la, b, on):  # a (la - log b) where it counts
+        return torch.where(on & (a > 0), a * (la - b), 0.0).sum(1, keepdim=True) + \
             torch.where(on & a.isnan(), a, 0.0).sum(1, keepdim=True)
 
     if not rest:
         t = torch.where(total != 0, t / total, 0.0)
-        kl = plogq(t, logp, inside)
+        kl = plogq(t, t.log(), logp, inside)
         d = torch.where(total != 0, p - t, 0.0)
     else:
         lr = torch.logsumexp(torch.where(inside, -math.inf, logp), 1, keepdim=True)
@@ -352,11 +355,11 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
         q = torch.where(empty | inside, 0.0, (logp - lr).exp())
         if kind == "forward":
             tr = (1 - total).clamp_min(0)
-            kl = plogq(t, logp, inside) + torch.where(empty | (tr == 0), 0.0, tr * (tr.clamp_min(1e-300).log() - lr))
+            kl = plogq(t, lt, logp, inside) + torch.where(empty | (tr == 0), 0.0, tr * (tr.clamp_min(1e-300).log() - lr))
             a = total + torch.where(empty, 0.0, tr)  # 1, but for a student without mass outside (or a list with more than 1)
             d = torch.where(inside, a * p - t, (a * pr - tr) * q)
         else:
-            f = torch.where(inside & (p > 0), logp - t.clamp_min(1e-300).log(), 0.0)
+            f = torch.where(inside & (p > 0), logp - lt, 0.0)
             fr = torch.where(empty, 0.0, lr - (1 - total).clamp_min(DISTILL_REST_MIN).log())
             kl = (p * f).sum(1, keepdim=True) + pr * fr
             d = torch.where(inside, p * (f - kl), pr * q * (fr - kl))
