@@ -4,7 +4,7 @@
 // p = softmax(z / T), the row's loss is w KL + c (-log p_y), with
 //
 //   forward:        KL = sum_S t (log t - log p),                 T dKL/dz_j = p_j - t_j
-//                   (t divided by its sum)
+//                   (t divided by its sum: by the sum of exp(l - max l), whatever the list's own scale)
 //   forward, rest:  ... + t_R (log t_R - log p_R),                T dKL/dz_j = p_j - t_j in S,
 //                                                                 (p_R - t_R) q_j outside
 //                   (p times sum t + t_R where that is not 1)
@@ -78,7 +78,8 @@ struct Shared {
   int y, y_listed, twice;
   __align__(16) int id[kMaxList];  // -1: padding
   float z[kMaxList], l[kMaxList];
-  double t[kMaxList];  // mass of the class (l: its logarithm); -1 where the entry is not its id's first
+  double t[kMaxList];  // mass of the class (l: its logarithm), without the rest relative to the largest entry;
+                       // -1 where the entry is not its id's first
   // the softmax sum of the list's elements, the masses' sum, t_R, and their logarithms
   float in_m, in_s;
   float mass, log_mass, t_rest, log_t_rest;
@@ -130,14 +131,14 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
   if (listed) {
     for (int k = lane; k < a.K; k += 32) {
       const float t = static_cast<float>(s.t[k]);
-      if (s.id[k] < 0 || t < 0.f) continue;
+      if (s.id[k] < 0 || s.t[k] < 0.0) continue;
       const float lp = log_p(s.z[k], all.m, lns);
       const float lt = s.l[k] - s.log_mass;
       if (a.kind == TB_DISTILL_REVERSE) {
         const float p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
         if (p != 0.f) kl += p * (lp - lt);
-      } else if (t != 0.f) {
-        kl += (a.kind == TB_DISTILL_FORWARD ? t / s.mass : t) * (lt - lp);
+      } else if (s.t[k] != 0.0) {  // (a mass below 2^-149 counts where the student has none)
+        kl += lp == -INFINITY ? INFINITY : (a.kind == TB_DISTILL_FORWARD ? t / s.mass : t) * (lt - lp);
       }
     }
     kl = tb::warp_sum(kl);
@@ -215,9 +216,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
       }
       if (tid < kMaxList) {
         s.id[tid] = id;
-        s.l[tid] = l;
+        s.l[tid] = id >= 0 ? l : -INFINITY;
         if (id >= 0) s.z[tid] = tb::to_f32(row.row[id]);
-        s.t[tid] = id >= 0 ? exp(static_cast<double>(l)) : 0.0;
+        if (a.kind != TB_DISTILL_FORWARD) s.t[tid] = id >= 0 ? exp(static_cast<double>(l)) : 0.0;
       }
       if (tid == 0) {
         s.w = q.w;
@@ -229,6 +230,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
         for (int i = tid; i < part; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
       const int y_listed = __syncthreads_or(id >= 0 && id == q.y);
       if (tid == 0) s.y_listed = y_listed;
+      // ---- without the rest masses count relative to the largest (a list of faint entries has a sum, too)
+      float largest = 0.f;
+      if (a.kind == TB_DISTILL_FORWARD && tid < kMaxList) {
+        largest = -INFINITY;
+        for (int j = lane; j < K; j += 32) largest = fmaxf(largest, s.l[j]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        s.t[tid] = id >= 0 ? exp(static_cast<double>(l) - largest) : 0.0;
+      }
       // ---- an id that occurs twice counts once, with the sum of its masses
       int seen = 0;
       if (MODE == kGrad) {
@@ -258,12 +268,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
           double m = 0.0;
           for (int j = 0; j < K; ++j)
             if (s.id[j] == id) m += exp(static_cast<double>(s.l[j]) - top);
-          s.t[tid] = first ? m * exp(static_cast<double>(top)) : -1.0;
-          l = static_cast<float>(top + log(m));
+          s.t[tid] = first ? m * exp(static_cast<double>(top) - largest) : -1.0;
+          l = static_cast<float>(static_cast<double>(top) - largest + log(m));
         }
         __syncthreads();
         if (id >= 0) s.l[tid] = l;
         __syncthreads();
+      } else if (id >= 0) {
+        s.l[tid] = l - largest;  // (read behind the next wait)
       }
     }
     Numbers n;

@@ -666,3 +666,31 @@ def test_faint_entries_beside_a_repeated_id(low, kind, rest, device):
     ids[1, 1] = ids[1, 0]
     ids[2, 4], logp[2, 4] = ids[2, 5], low - 0.5
     check_list(x, ids, logp, kind, rest)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("offset", [-80.0, -95.0, -120.0, -800.0, -1e4, 60.0, 100.0, 1000.0])
+def test_a_normalised_list_at_any_offset(offset, device):
+    """Without the rest the list is divided by its sum: a common offset of its log-probabilities (a list of unlikely
+    tokens, or of scores) changes nothing but their own rounding, which the 64-bit form sees too.  An id twice, and
+    entries of very different weight."""
+    x = rows(4, 200, torch.float32, device, spread=1.0)
+    ids, logp = lists(x, 6)
+    ids = ids.clone()
+    logp = logp + offset
+    ids[1, 1] = ids[1, 0]
+    logp[2, 3] -= 30.0
+    check_list(x, ids, logp, "forward", False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_faint_entry_that_the_student_rules_out(device):
+    """A mass that 32 bits hold as zero and 64 bits do not, on a logit of -inf: the loss is infinite as for any other."""
+    x = rows(3, 100, torch.float32, device, spread=1.0)
+    ids, logp = lists(x, 5)
+    logp = logp.clone()
+    logp[1, 2], logp[2, 2] = -150.0, -1.0
+    x[1, ids[1, 2].long()] = x[2, ids[2, 2].long()] = -INF
+    for rest in (True, False):
+        loss, d = distill_loss_grad(x, ids, logp, rest=rest)
+        assert loss.isinf().tolist() == [False, True, True] and (loss[1:] > 0).all() and d.isfinite().all()

@@ -346,9 +346,11 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
             torch.where(on & a.isnan(), a, 0.0).sum(1, keepdim=True)
 
     if not rest:
-        t = torch.where(total != 0, t / total, 0.0)
-        kl = plogq(t, t.log(), logp, inside)
-        d = torch.where(total != 0, p - t, 0.0)
+        some = here.any(1, keepdim=True)
+        lt = lt - torch.where(some, torch.logsumexp(l, 1, keepdim=True), 0.0)
+        t = torch.where(lt.isneginf(), 0.0, lt.exp())
+        kl = plogq(t, lt, logp, inside)
+        d = torch.where(some, p - t, 0.0)
     else:
         lr = torch.logsumexp(torch.where(inside, -math.inf, logp), 1, keepdim=True)
         pr, empty = lr.exp(), lr.isneginf()
