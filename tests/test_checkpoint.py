@@ -129,3 +129,38 @@ def test_data_parallel_save_and_resume_per_rank(tmp_path):
     assert all(ok for _, ok, _ in res), res
     files = set(os.listdir(tmp_path / "step_1"))
     assert {"trainer_dp0.pt", "trainer_dp1.pt", "COMPLETE_dp0", "COMPLETE_dp1"} <= files, files
+
+
+def test_a_configuration_saved_before_a_key_was_there(tmp_path):
+    """Keys that the saved configuration lacks count as their defaults, in nested configurations too; any other value,
+    and a key that is gone, is a difference."""
+    from turbol_b200.models.llm import LMConfig
+    from turbol_b200.rl.grpo import GRPOConfig
+
+    def config(**kw):
+        return GRPOConfig(model=LMConfig.tiny(n_layers=1), num_prompts=2, **kw)
+
+    save_checkpoint(str(tmp_path), 3, state={"step_count": 3}, config=config())
+    path = tmp_path / "step_3" / "config.cfg"
+    lines = path.read_text().splitlines()
+    new = ("distill_coef", "distill_topk", "distill_kind", "kv_dtype", "model.embed_scale", "model.rope_scaling",
+           "model.rotary_dim")
+    path.write_text("\n".join(line for line in lines if line.split("=")[0].strip() not in new) + "\n")
+    assert not set(new) & set(read_config(str(path)))
+    assert load_checkpoint(str(tmp_path), config=config())["step_count"] == 3
+    with pytest.raises(ValueError, match="distill_coef"):
+        load_checkpoint(str(tmp_path), config=config(distill_coef=0.1))
+    scaled = config()
+    scaled.model.embed_scale = 2.0
+    with pytest.raises(ValueError, match="model.embed_scale"):
+        load_checkpoint(str(tmp_path), config=scaled)
+    scaled = config()
+    scaled.model.rope_scaling = {"rope_type": "linear", "factor": 2.0}
+    with pytest.raises(ValueError, match="rope_scaling"):
+        load_checkpoint(str(tmp_path), config=scaled)
+    path.write_text(path.read_text() + "gone = 1\n")
+    with pytest.raises(ValueError, match="gone"):
+        load_checkpoint(str(tmp_path), config=config())
+    # (a plain dict has no defaults)
+    with pytest.raises(ValueError, match="kv_dtype"):
+        load_checkpoint(str(tmp_path), config={"kv_dtype": "bf16"})

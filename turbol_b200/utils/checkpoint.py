@@ -46,7 +46,7 @@ import os
 import re
 import shutil
 import threading
-from dataclasses import asdict, is_dataclass
+from dataclasses import MISSING, asdict, fields, is_dataclass
 from typing import Any, Dict, Optional
 
 import torch
@@ -79,6 +79,18 @@ def _flatten_config(cfg, prefix="") -> Dict[str, str]:
             out[key] = ",".join(str(x) for x in v)
         else:
             out[key] = str(v)
+    return out
+
+
+def _default_config(cfg, prefix="") -> Dict[str, str]:
+    """The defaults of a configuration's fields, those of nested ones included, as _flatten_config writes them."""
+    out = {}
+    for f in fields(cfg) if is_dataclass(cfg) else ():
+        v = getattr(cfg, f.name)
+        if is_dataclass(v):
+            out.update(_default_config(v, f"{prefix}{f.name}."))
+        elif f.default is not MISSING or f.default_factory is not MISSING:
+            out.update(_flatten_config({f.name: f.default if f.default is not MISSING else f.default_factory()}, prefix))
     return out
 
 
@@ -295,7 +307,8 @@ def load_checkpoint(directory: str, step: Optional[int] = None, trainer=None, *,
     to ``trainer.checkpoint_ranks()``.  The step must be complete for its
     layout and must hold this rank's marker.  With ``config`` (or
     ``trainer.cfg``) the saved configuration must match key for key unless
-    ``strict_config=False``."""
+    ``strict_config=False``; a key that it lacks (saved before the key was
+    there) counts as the field's default."""
     tp_rank, pp_rank, dp_rank, lay = _resolve_ranks(trainer, tp_rank, pp_rank, dp_rank, layout)
     if step is None:
         step = latest_step(directory)
@@ -331,6 +344,7 @@ def load_checkpoint(directory: str, step: Optional[int] = None, trainer=None, *,
         want = config if config is not None else (getattr(trainer, "cfg", None) if trainer is not None else None)
         if want is not None and strict_config:
             cur = _flatten_config(want)
+            saved_cfg = {**{k: v for k, v in _default_config(want).items() if k in cur}, **saved_cfg}
             diff = {k for k in set(cur) | set(saved_cfg) if cur.get(k) != saved_cfg.get(k)}
             if diff:
                 raise ValueError(f"checkpoint configuration differs in {sorted(diff)}")
