@@ -159,3 +159,32 @@ def test_example(tmp_path, dev):
                             "--num-steps", "2", "--print-every", "1", "--micro-batch", "4", "--distill-coef", "0.2",
                             "--distill-topk", "20", "--distill-kind", "reverse", "--log-dir", str(tmp_path)])
     assert tr.step_count == 2 and math.isfinite(float(tr.distill_kl))
+
+
+@pytest.mark.gpu
+def test_resume_with_the_same_teacher(tmp_path, dev):
+    """A run that distils towards a given model goes on with that model alone; the frozen reference is saved with the
+    run; states without the entry load as they did."""
+    from turbol_b200.utils.checkpoint import load_checkpoint, save_checkpoint
+
+    def trainer(seed=None):
+        teacher = None if seed is None else DecoderLM(tiny(), dev, seed=seed, master=False)
+        return GRPOTrainer(config(distill_coef=0.1, distill_topk=16), dev, teacher=teacher)
+
+    given, own = trainer(5), trainer()
+    given.step()
+    save_checkpoint(str(tmp_path / "given"), 1, given)
+    save_checkpoint(str(tmp_path / "own"), 1, own)
+    again = trainer(5)
+    load_checkpoint(str(tmp_path / "given"), trainer=again)
+    assert torch.equal(again.model.flat, given.model.flat) and again.step_count == 1
+    for where, seed in (("given", None), ("given", 6), ("own", 5)):
+        tr = trainer(seed)
+        before = tr.model.flat.clone()
+        with pytest.raises(ValueError, match="teacher"):
+            load_checkpoint(str(tmp_path / where), trainer=tr)
+        assert torch.equal(tr.model.flat, before)
+    load_checkpoint(str(tmp_path / "own"), trainer=trainer())
+    sd = given.state_dict()
+    del sd["teacher"]
+    trainer(6).load_state_dict(sd)

@@ -31,6 +31,7 @@ module is the algorithm it names.
 """
 from __future__ import annotations
 
+import hashlib
 import time
 from dataclasses import dataclass, field
 from typing import Optional
@@ -272,13 +273,27 @@ class GRPOTrainer:
         return {}
 
     def state_dict(self) -> dict:
-        """Master weights (fp32), the frozen reference weights, optimizer state and
-        the step counter (which also keys the prompt and sampling streams)."""
+        """Master weights (fp32), the frozen reference weights, optimizer state,
+        the step counter (which also keys the prompt and sampling streams), and of a
+        given teacher a digest: its weights stay with the caller."""
         return {"policy": {"flat": self.model.flat, "shadow": self.model.shadow},
                 "optim": self.opt.state_dict(), "ref_shadow": self.ref.shadow,
-                "step_count": self.step_count, "gen_calls": self.gen.calls}
+                "step_count": self.step_count, "gen_calls": self.gen.calls, "teacher": self._teacher_digest()}
+
+    def _teacher_digest(self) -> Optional[str]:
+        """Of a given teacher's weights (sums of their bits over pieces); None where the frozen reference teaches."""
+        if self.teacher is self.ref:
+            return None
+        bits = self.teacher.shadow.view(torch.int16)
+        whole = bits.numel() // 65536 * 65536
+        sums = torch.cat([bits[:whole].view(-1, 65536).sum(1), bits[whole:].sum().view(1)]).cpu()
+        return hashlib.sha256(sums.numpy().tobytes()).hexdigest()
 
     def load_state_dict(self, sd: dict):
+        # (a state from before the key was there says nothing of its teacher)
+        if "teacher" in sd and sd["teacher"] != self._teacher_digest():
+            kind = "the frozen reference" if sd["teacher"] is None else "a given one"
+            raise ValueError(f"the saved run's teacher was {kind} and is not this trainer's")
         with torch.no_grad():
             self.model.flat.copy_(sd["policy"]["flat"])
             self.model.shadow.copy_(sd["policy"]["shadow"])
