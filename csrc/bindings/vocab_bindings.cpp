@@ -264,7 +264,8 @@ std::vector<int64_t> rows_shape(const at::Tensor& ids, int64_t H) {
   return s;
 }
 
-Opt embedding(const at::Tensor& ids, const at::Tensor& weight, double scale, const Opt& out_, const Opt& error) {
+Opt embedding(const at::Tensor& ids, const at::Tensor& weight, double scale, const Opt& out_, const Opt& error,
+              bool first_row) {
   const char* op = "embedding";
   TbEmbeddingArgs a{};
   a.ids64 = ids_of(ids, op);
@@ -275,6 +276,7 @@ Opt embedding(const at::Tensor& ids, const at::Tensor& weight, double scale, con
   const at::Device dev = weight.device();
   chk(ids.device() == dev, op, "all tensors on one device");
   if (is_dual(weight)) no_grad({&weight}, op);
+  if (first_row) no_grad({&weight}, op, "first_row=True");  // (the gradient leaves such ids out)
   const std::vector<int64_t> shape = rows_shape(ids, weight.size(1));
   if (out_) {
     chk(out_->sizes() == at::IntArrayRef(shape) && out_->scalar_type() == weight.scalar_type() && out_->is_contiguous(),
@@ -298,6 +300,7 @@ Opt embedding(const at::Tensor& ids, const at::Tensor& weight, double scale, con
   a.H = static_cast<int>(weight.size(1));
   a.V = static_cast<int>(weight.size(0));
   a.scale = static_cast<float>(scale);
+  a.first_row = first_row;
   cuda_ok(tb_embedding(&a, turbol::StreamFor(weight)), op);
   if (out_) written({&*out_});
   return out;
@@ -383,7 +386,7 @@ struct EmbeddingGradFunction : torch::autograd::Function<EmbeddingGradFunction> 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& weight, const at::Tensor& ids,
                             double scale, const Opt& error) {
-    at::Tensor out = *embedding(ids, weight, scale, std::nullopt, error);
+    at::Tensor out = *embedding(ids, weight, scale, std::nullopt, error, /*first_row=*/false);
     ctx->save_for_backward({ids});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["V"] = weight.size(0);
@@ -428,7 +431,7 @@ void register_vocab_ops(py::module_& m) {
         py::arg("temperature") = 1.0, py::arg("target") = py::none(), py::arg("target_weight") = py::none(),
         py::arg("error") = py::none(), "the same, differentiable in logits (CUDA tensors)");
   m.def("embedding", &embedding, py::arg("ids"), py::arg("weight"), py::arg("scale") = 1.0,
-        py::arg("out") = py::none(), py::arg("error") = py::none(), "scale * weight[ids]");
+        py::arg("out") = py::none(), py::arg("error") = py::none(), py::arg("first_row") = false, "scale * weight[ids]");
   m.def("embedding_grad", &embedding_grad, py::arg("ids"), py::arg("dy"), py::arg("grad"), py::arg("scale") = 1.0,
         py::arg("accumulate") = true, py::arg("error") = py::none(),
         "adds scale * dy to the rows of grad that ids name, in token order");

@@ -38,6 +38,15 @@ __device__ __forceinline__ long long id_of(const void* ids, int ids64, long long
   return ids64 ? static_cast<const long long*>(ids)[t] : static_cast<const int*>(ids)[t];
 }
 
+// A token's row in the lookup: whether it has one, and (in place of the id) where.
+__device__ __forceinline__ bool row_of(const TbEmbeddingArgs& a, long long& id, bool tells) {
+  if (id >= 0 && id < a.V) return true;
+  if ((id >= a.V || a.first_row) && a.err && tells) *a.err = 1;
+  if (!a.first_row) return false;
+  id = 0;
+  return true;
+}
+
 // ---- rows of any alignment: 16 bytes that begin `shift` bytes into the first of two vectors.
 // (What lies beside a row within its tensor is read along and not used.)
 template <typename T>
@@ -83,9 +92,8 @@ __global__ void __launch_bounds__(256) lookup_wide_kernel(TbEmbeddingArgs a, int
   for (long long task = blockIdx.x * 8ll + threadIdx.x / 32; task < tasks; task += gridDim.x * 8ll) {
     const long long t = segs == 1 ? task : task / segs;
     const int first = static_cast<int>(task - t * segs) * 32 * kUnroll + lane;
-    const long long id = id_of(a.ids, a.ids64, t);
-    const bool good = id >= 0 && id < a.V;
-    if (id >= a.V && a.err && lane == 0) *a.err = 1;
+    long long id = id_of(a.ids, a.ids64, t);
+    const bool good = row_of(a, id, lane == 0);
     const T* src = static_cast<const T*>(a.weight) + (good ? id : 0) * a.ld_w;
     T* dst = static_cast<T*>(a.out) + t * a.ld_out;
     tb::Packed<T, E> p[kUnroll];
@@ -113,9 +121,8 @@ __global__ void __launch_bounds__(256) lookup_shift_kernel(TbEmbeddingArgs a) {
   const T* table = static_cast<const T*>(a.weight);
   const T* end = table + (a.V - 1) * a.ld_w + a.H;
   for (long long t = blockIdx.x * 8ll + threadIdx.x / 32; t < a.N; t += gridDim.x * 8ll) {
-    const long long id = id_of(a.ids, a.ids64, t);
-    const bool good = id >= 0 && id < a.V;
-    if (id >= a.V && a.err && lane == 0) *a.err = 1;
+    long long id = id_of(a.ids, a.ids64, t);
+    const bool good = row_of(a, id, lane == 0);
     const T* src = table + (good ? id : 0) * a.ld_w;
     T* dst = static_cast<T*>(a.out) + t * a.ld_out;
     const auto one = [&](int h) { dst[h] = tb::from_f32<T>(good ? tb::to_f32(src[h]) * a.scale : id < 0 ? 0.f : NAN); };
@@ -156,9 +163,8 @@ __global__ void __launch_bounds__(256) lookup_narrow_kernel(TbEmbeddingArgs a) {
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const long long t = total <= UINT_MAX ? static_cast<unsigned>(i) / static_cast<unsigned>(per) : i / per;
     const int h = static_cast<int>(i - t * per) * N;
-    const long long id = id_of(a.ids, a.ids64, t);
-    const bool good = id >= 0 && id < a.V;
-    if (id >= a.V && a.err) *a.err = 1;
+    long long id = id_of(a.ids, a.ids64, t);
+    const bool good = row_of(a, id, true);
     float x[N];
     if (good) tb::load_vec<T, N>(static_cast<const T*>(a.weight) + id * a.ld_w + h, x);
 #pragma unroll

@@ -471,7 +471,7 @@ int tb_distill(const TbDistillArgs* args, cudaStream_t s);
 
 // ---------------- embedding (embedding.cu) ----------------
 // out[t] = scale * weight[ids[t]] (one rounding; negative ids: zeros; ids past V:
-// NaN and *err = 1).
+// NaN and *err = 1; with first_row: both row 0 and *err = 1, as tb_embed_fwd).
 typedef struct {
   const void* ids;  // int32 or int64
   int ids64;
@@ -483,6 +483,7 @@ typedef struct {
   int dtype;
   float scale;
   int* err;
+  int first_row;
 } TbEmbeddingArgs;
 int tb_embedding(const TbEmbeddingArgs* args, cudaStream_t s);
 // grad[v] += scale * sum of the rows dy[t] with ids[t] == v, in token order (zero: =,

@@ -188,3 +188,17 @@ def test_resume_with_the_same_teacher(tmp_path, dev):
     sd = given.state_dict()
     del sd["teacher"]
     trainer(6).load_state_dict(sd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1.0, 16.0])
+def test_ids_outside_the_table_do_not_depend_on_the_scale(scale, dev):
+    """The decoder's embedding reads row 0 for them and gives them no gradient."""
+    m = DecoderLM(tiny(embed_scale=scale), dev, seed=3)
+    ids = torch.tensor([[5, -1, m.cfg.vocab, m.cfg.vocab - 1]], dtype=torch.int32, device=dev)
+    want = m.s["embed"][torch.tensor([5, 0, 0, m.cfg.vocab - 1], device=dev)] * scale
+    assert torch.equal(m.embed(ids), want)
+    m.zero_grad()
+    m.embed_backward(ids, torch.ones(4, m.cfg.hidden, device=dev, dtype=torch.bfloat16))
+    rows = m.g["embed"].abs().sum(1).nonzero().squeeze(1).tolist()
+    assert rows == [5, m.cfg.vocab - 1]

@@ -352,3 +352,25 @@ def test_zeros_beside_the_sums(N, V, H, dtype, dev):
     named = torch.zeros(V, dtype=torch.bool, device=dev)
     named[ids[(ids >= 0) & (ids < V)]] = True
     assert not out[~named].any() and out[named].any(1).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("H,pad", [(8, 0), (33, 2), (512, 0), (515, 1)])
+def test_first_row(H, pad, device):
+    """Ids outside the table read row 0 and are told, negative ones too; not with a gradient."""
+    W = torch.randn(20, H + pad, device=device)[:, :H]
+    ids = torch.tensor([3, -1, 19, 20, -2 ** 31, 2 ** 31 - 1, 0], dtype=torch.int32, device=device)
+    inside = torch.tensor([3, 0, 19, 0, 0, 0, 0], dtype=torch.int32, device=device)
+    err = torch.zeros(1, dtype=torch.int32, device=device)
+    assert torch.equal(embedding(inside, W, 2.0, first_row=True, error=err), embedding(inside, W, 2.0)) and int(err) == 0
+    assert torch.equal(embedding(ids, W, 2.0, first_row=True, error=err), embedding(inside, W, 2.0)) and int(err) == 1
+    err.zero_()
+    embedding(ids[:2].clone(), W, 2.0, first_row=True, error=err)
+    assert int(err) == 1
+    far = torch.tensor([2 ** 40, -2 ** 40], device=device)
+    assert torch.equal(embedding(far, W, first_row=True), W[:1].expand(2, H))
+    leaf = W.clone().requires_grad_()
+    with pytest.raises(ValueError, match="first_row"):
+        embedding(ids, leaf, first_row=True)
+    with torch.no_grad():
+        embedding(ids, leaf, first_row=True)

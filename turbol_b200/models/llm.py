@@ -124,11 +124,12 @@ def apply_rope(cfg: LMConfig, table: torch.Tensor, qkv: torch.Tensor, pos: torch
 
 
 def embed_into(cfg: LMConfig, ids: torch.Tensor, weight: torch.Tensor, out: torch.Tensor):
-    """Writes the (scaled) embedding rows of the int32 ids [N] to out [N, hidden]."""
+    """Writes the (scaled) embedding rows of the int32 ids [N] to out [N, hidden]; ids outside the table read row 0,
+    whatever the scale (and have no gradient)."""
     if cfg.embed_scale == 1.0:
         _ops().embed_fwd(ids, weight, out)
     else:
-        embedding(ids, weight, cfg.embed_scale, out=out)
+        embedding(ids, weight, cfg.embed_scale, out=out, first_row=True)
 
 
 class DecoderLM:

@@ -49,21 +49,23 @@ class _EmbeddingGrad(torch.autograd.Function):
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None,
-              error: Optional[torch.Tensor] = None) -> torch.Tensor:
+              error: Optional[torch.Tensor] = None, first_row: bool = False) -> torch.Tensor:
     """scale * weight[ids] [*ids.shape, H] for ids of any shape (int32 or int64, contiguous) and
     rows ``weight`` [V, H] (bf16, fp16 or fp32; any row stride), rounded once.
 
     A negative id is padding: a row of zeros, without a gradient.  An id past the last
     row gives NaN, no gradient, and sets ``error`` (an int32 device tensor, optional) to 1.
+    ``first_row``: ids outside the table, negative ones too, read row 0 instead and set ``error``,
+    as ``ops.embed_fwd`` does (not with a gradient).
     Differentiable in ``weight`` (a dense gradient of its type), unless ``out`` is given."""
-    if out is None and weight.requires_grad and torch.is_grad_enabled():
+    if out is None and not first_row and weight.requires_grad and torch.is_grad_enabled():
         if weight.is_cuda:
             return _call("embedding_autograd", ids, weight, scale, error)
         _call("embedding", ids, weight, scale, None, error)  # the checks
         return _Embedding.apply(weight, ids, scale, error)
-    y = _call("embedding", ids, weight, scale, out, error)
+    y = _call("embedding", ids, weight, scale, out, error, first_row)
     if y is None:
-        y = ref.embedding(ids, weight, scale, out, error)
+        y = ref.embedding(ids, weight, scale, out, error, first_row)
     return y if out is None else out
 
 

@@ -373,10 +373,15 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
 
 
 # ------------------------------------------------------------------ embedding
-def embedding(ids, weight, scale=1.0, out=None, error=None):
-    """scale * weight[ids], padding (negative ids) zero, ids past the table NaN."""
+def embedding(ids, weight, scale=1.0, out=None, error=None, first_row=False):
+    """scale * weight[ids], padding (negative ids) zero, ids past the table NaN (or both row 0)."""
     i = ids.long()
     bad = i >= weight.shape[0]
+    if first_row:
+        outside = bad | (i < 0)
+        if error is not None and bool(outside.any()):
+            error[0] = 1
+        return embedding(i.masked_fill(outside, 0), weight, scale, out)
     if error is not None and bool(bad.any()):
         error[0] = 1
     y = weight[i.clamp(0, weight.shape[0] - 1)].double() * scale
