@@ -137,7 +137,8 @@ using LossAndGrad = std::optional<std::tuple<at::Tensor, at::Tensor>>;
 
 LossAndGrad distill_loss_grad(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& logprobs,
                               const Opt& weight, const std::string& kind, bool rest, double temperature,
-                              const Opt& target, const Opt& target_weight, const Opt& out_, const Opt& error) {
+                              const Opt& target, const Opt& target_weight, const Opt& out_, const Opt& error,
+                              const Opt& kl) {
   const char* op = "distill_loss_grad";
   TbDistillArgs a = distill_args(logits, ids, logprobs, weight, target, target_weight, distill_kind(kind, rest, op),
                                  temperature, error, op);
@@ -154,6 +155,13 @@ LossAndGrad distill_loss_grad(const at::Tensor& logits, const at::Tensor& ids, c
     for (const Opt* t : {&weight, &target, &target_weight, &error})
       chk(!*t || apart(*out_, **t), op, "out overlaps an input");
   }
+  if (kl) {
+    per_row(kl, a.R, at::kFloat, logits.device(), op, "kl is a contiguous fp32 [R]");
+    no_grad({&*kl}, op, "kl");
+    for (const at::Tensor* t : {&logits, &ids, &logprobs}) chk(apart(*kl, *t), op, "kl overlaps another tensor");
+    for (const Opt* t : {&weight, &target, &target_weight, &out_, &error})
+      chk(!*t || apart(*kl, **t), op, "kl overlaps another tensor");
+  }
   if (!logits.is_cuda()) return std::nullopt;
   c10::DeviceGuard guard(logits.device());
   at::Tensor loss = at::empty({a.R}, logprobs.options());
@@ -162,8 +170,10 @@ LossAndGrad distill_loss_grad(const at::Tensor& logits, const at::Tensor& ids, c
     a.grad = grad.data_ptr();
     a.ld_grad = grad.stride(0);
     a.loss = loss.data_ptr<float>();
+    a.kl = kl ? kl->data_ptr<float>() : nullptr;
     cuda_ok(tb_distill(&a, turbol::StreamFor(logits)), op);
     if (out_) written({&*out_});
+    if (kl) written({&*kl});
   }
   return std::make_tuple(loss, grad);
 }
@@ -421,7 +431,8 @@ void register_vocab_ops(py::module_& m) {
   m.def("distill_loss_grad", &distill_loss_grad, py::arg("logits"), py::arg("ids"), py::arg("logprobs"),
         py::arg("weight") = py::none(), py::arg("kind") = "forward", py::arg("rest") = true,
         py::arg("temperature") = 1.0, py::arg("target") = py::none(), py::arg("target_weight") = py::none(),
-        py::arg("out") = py::none(), py::arg("error") = py::none(), "distillation loss of each row and its gradient");
+        py::arg("out") = py::none(), py::arg("error") = py::none(), py::arg("kl") = py::none(),
+        "distillation loss of each row and its gradient");
   m.def("distill_loss", &distill_loss, py::arg("logits"), py::arg("ids"), py::arg("logprobs"),
         py::arg("weight") = py::none(), py::arg("kind") = "forward", py::arg("rest") = true,
         py::arg("temperature") = 1.0, py::arg("target") = py::none(), py::arg("target_weight") = py::none(),

@@ -163,6 +163,7 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
   s.n = {ex.m, factor, all.m, good ? lns : make_float2(NAN, NAN), kl, whole};
   if (!write) return;
   a.loss[r] = good ? (listed ? w * kl : 0.f) + (c != 0.f ? -c * log_p(s.z_y, all.m, lns) : 0.f) : NAN;
+  if (a.kl) a.kl[r] = good || !listed ? kl : NAN;
   if (a.stats) {
     float4* st = reinterpret_cast<float4*>(a.stats + r * TB_DISTILL_STATS);
     st[0] = make_float4(s.n.origin, s.n.factor, s.n.top, s.n.lns.x);
@@ -196,7 +197,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
       const Weights q(a, a.weight ? a.weight[r] : 1.f, a.target_weight ? a.target_weight[r] : 1.f, a.target ? a.target[r] : -1);
       if (MODE != kGrad && a.err && q.bad && tid == 0) *a.err = 1;
       if (!q.live()) {
-        if (MODE != kGrad && rank == 0 && tid == 0) a.loss[r] = 0.f;
+        if (MODE != kGrad && rank == 0 && tid == 0) {
+          a.loss[r] = 0.f;
+          if (a.kl) a.kl[r] = 0.f;
+        }
         if (MODE != kLoss) {
           for (int v = row.v0 + tid; v < row.v1; v += kThreads) {
             const int e = v * E - row.mis;

@@ -462,6 +462,7 @@ typedef struct {
   float* loss;         // [R]; NULL: a backward pass from `stats`
   float* stats;        // [R, TB_DISTILL_STATS]: written with the loss (may be NULL then), or read
   const float* dloss;  // [R]: the loss's gradient in a backward pass
+  float* kl;           // [R]: the KL without its weight (0 in rows whose weight is 0), may be NULL; with `loss`
   int R, V, K;
   int dtype, kind;
   double temperature;

@@ -694,3 +694,31 @@ def test_a_faint_entry_that_the_student_rules_out(device):
     for rest in (True, False):
         loss, d = distill_loss_grad(x, ids, logp, rest=rest)
         assert loss.isinf().tolist() == [False, True, True] and (loss[1:] > 0).all() and d.isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind,rest", KINDS)
+def test_the_kl_alone(kind, rest, device):
+    """Beside the loss: without the row's weight and target; 0 in rows without weight, whatever they hold."""
+    x = rows(6, 300, torch.float32, device, spread=1.0)
+    ids, logp = lists(x, 7)
+    w = torch.tensor([1.0, 1e-20, 0.0, -3.0, 0.0, 2.0], device=device)
+    y = torch.tensor([3, 5, 7, -1, -1, 9], dtype=torch.int32, device=device)
+    c = torch.tensor([1.0, 40.0, -2.0, 1.0, 1.0, 0.0], device=device)
+    want = by_log_masses(x, ids, logp, kind, rest)
+    x[4] = NAN
+    how = dict(kind=kind, rest=rest, target=y, target_weight=c)
+    kl = torch.full((6,), NAN, device=device)
+    loss, d = distill_loss_grad(x, ids, logp, w, kl=kl, **how)
+    plain = distill_loss_grad(x, ids, logp, w, **how)
+    assert torch.equal(loss, plain[0]) and torch.equal(d, plain[1])
+    on = w != 0
+    compare(kl[on], None, x, [t[on.cpu()] for t in want])
+    assert not kl[~on].any()
+    x[0] = -INF
+    distill_loss_grad(x, ids, logp, w, kl=kl, **how)
+    assert kl.isnan().tolist() == [True] + [False] * 5
+    for bad in (kl[:5], kl.double(), torch.empty(12, device=device)[::2], w, c, kl.clone().requires_grad_(), x.view(-1)[:6]):
+        with pytest.raises(ValueError, match="distill_loss_grad"):
+            distill_loss_grad(x, ids, logp, w, kl=bad, **how)
+    distill_loss_grad(x[:0], ids[:0], logp[:0], kl=kl[:0])

@@ -202,3 +202,23 @@ def test_ids_outside_the_table_do_not_depend_on_the_scale(scale, dev):
     m.embed_backward(ids, torch.ones(4, m.cfg.hidden, device=dev, dtype=torch.bfloat16))
     rows = m.g["embed"].abs().sum(1).nonzero().squeeze(1).tolist()
     assert rows == [5, m.cfg.vocab - 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["forward", "reverse"])
+def test_the_distance_does_not_depend_on_its_weight(kind, dev):
+    """distill_kl beside a policy loss of ordinary size: the same for a coefficient of 1e-7 (the logits are the same;
+    sums of 96 numbers in one order, so the same bits)."""
+    got = []
+    for coef in (1.0, 1e-7):
+        tr = GRPOTrainer(config(distill_coef=coef, distill_topk=16, distill_kind=kind), dev,
+                         teacher=DecoderLM(tiny(), dev, seed=11, master=False))
+        g = torch.Generator(device=dev).manual_seed(2)
+        n = tr.cfg.batch
+        seqs = torch.randint(0, tr.cfg.model.vocab, (n, tr.cfg.seq_len), generator=g, device=dev, dtype=torch.int32)
+        lists = tr._teacher_lists(n)
+        tr._score(tr.teacher, seqs, lists=lists)
+        tr.model.zero_grad()
+        tr._train(seqs, tr.ref_logprobs(seqs), torch.randn(n, generator=g, device=dev), lists)
+        got.append(float(tr.distill_kl))
+    assert got[0] > 1e-3 and got[0] == got[1]

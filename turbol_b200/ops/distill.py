@@ -58,16 +58,18 @@ def distill_loss_grad(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.T
                       weight: Optional[torch.Tensor] = None, kind: str = "forward", rest: bool = True,
                       temperature: float = 1.0, target: Optional[torch.Tensor] = None,
                       target_weight: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                      error: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                      error: Optional[torch.Tensor] = None,
+                      kl: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(loss fp32 [R], its gradient: d loss[r] / d logits[r] in logits' type) of the rows
     ``logits`` [R, V] (bf16, fp16 or fp32; any row stride), for training loops without
     autograd.  ids int32 [R, K], logprobs fp32 [R, K] (K up to 256); weight,
     target_weight fp32 [R] (None: ones), target int32 [R].  ``out`` receives the
-    gradient (logits itself for in-place use)."""
+    gradient (logits itself for in-place use), ``kl`` (fp32 [R]) the rows' KL without weight
+    or target (0 where weight is 0)."""
     y = _call("distill_loss_grad", logits, ids, logprobs, weight, kind, rest, temperature, target, target_weight, out,
-              error)
+              error, kl)
     if y is None:
-        y = ref.distill(logits, ids, logprobs, weight, kind, rest, temperature, target, target_weight, error)
+        y = ref.distill(logits, ids, logprobs, weight, kind, rest, temperature, target, target_weight, error, out_kl=kl)
         y = (y[0], y[1] if out is None else out.copy_(y[1]))
     return (y[0], y[1] if out is None else out)
 

@@ -311,8 +311,9 @@ DISTILL_REST_MIN = 2.0 ** -20
 
 
 def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, temperature=1.0, target=None,
-            target_weight=None, error=None, dtype=None):
-    """(loss fp32 [R], gradient in ``dtype``, default logits') of the distillation loss, computed in 64 bits."""
+            target_weight=None, error=None, dtype=None, out_kl=None):
+    """(loss fp32 [R], gradient in ``dtype``, default logits') of the distillation loss, computed in 64 bits; the KLs
+    alone into ``out_kl``."""
     R, V = logits.shape
     f64 = dict(dtype=torch.float64, device=logits.device)
     w = torch.ones(R, **f64) if weight is None else weight.double()
@@ -366,6 +367,8 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
             kl = (p * f).sum(1, keepdim=True) + pr * fr
             d = torch.where(inside, p * (f - kl), pr * q * (fr - kl))
     on, c = (w != 0)[:, None], c[:, None]
+    if out_kl is not None:
+        out_kl.copy_(torch.where(on, kl, 0.0).squeeze(1))
     loss = torch.where(on, w[:, None] * kl, 0.0) + torch.where(c != 0, -c * logp.gather(1, y), 0.0)
     d = torch.where(on, w[:, None] * d, 0.0) + torch.where(c != 0, c * p, 0.0)
     d.scatter_add_(1, y, -c)

@@ -452,6 +452,7 @@ class GRPOTrainer:
         if lists is not None:  # per token: coefficient / (sequences x response tokens), as the policy loss's mean
             weight = torch.full((mb * Lr,), cfg.distill_coef / (nb * Lr), device=self.device)
             self.distill_kl = torch.zeros((), device=self.device)
+            kl = torch.empty(mb * Lr, device=self.device)
         for s0 in range(0, nb, mb):
             ids = seqs[s0:s0 + mb].contiguous()
             m = ids.shape[0]
@@ -473,10 +474,10 @@ class GRPOTrainer:
             if lists is None:
                 o.logprob(logits, tgt, None, dlp)                      # logits <- d loss / d logits
             else:  # with the distillation's: dlp is the gradient of log p[tgt], so -dlp weighs -log p[tgt]
-                loss, _ = distill_loss_grad(logits, lists[0][s0:s0 + m].view(m * Lr, -1),
-                                            lists[1][s0:s0 + m].view(m * Lr, -1), weight[: m * Lr],
-                                            kind=cfg.distill_kind, target=tgt, target_weight=-dlp, out=logits)
-                self.distill_kl += (loss - dlp * lp).sum() / cfg.distill_coef
+                distill_loss_grad(logits, lists[0][s0:s0 + m].view(m * Lr, -1),
+                                  lists[1][s0:s0 + m].view(m * Lr, -1), weight[: m * Lr],
+                                  kind=cfg.distill_kind, target=tgt, target_weight=-dlp, out=logits, kl=kl[: m * Lr])
+                self.distill_kl += kl[: m * Lr].sum() / (nb * Lr)
             dhr = torch.empty(m * Lr, H, device=self.device, dtype=torch.bfloat16)
             o.gemm(logits, m_.head_weight(), dhr, False, True)          # d h = dLogits W_head
             o.gemm(logits, hr, m_.head_grad(), True, True, accumulate=True, split_k=1)  # dW_head += dLogits^T h
