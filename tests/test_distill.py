@@ -722,3 +722,70 @@ def test_the_kl_alone(kind, rest, device):
         with pytest.raises(ValueError, match="distill_loss_grad"):
             distill_loss_grad(x, ids, logp, w, kl=bad, **how)
     distill_loss_grad(x[:0], ids[:0], logp[:0], kl=kl[:0])
+
+
+def tight(V):
+    """Relative error of a row's sum where every logit is within 4 of the largest: the exponential (2^-22), its argument
+    (up to 6 in size: the factor, the difference, the fused product, 18 x 2^-24 ln 2), the additions of one of the row's
+    1,024 partial sums (V / 1024, and up to 16 more where a warp has the whole of a short row) and the some 16 of joining
+    them, the correction of the argument's rounding, the logarithm (2^-25), and its number's roundings (up to 14 in size)."""
+    return 2.0 ** -24 * (4 + 13 + V / 1024 + 16 + 16 + 2 + 1 + 28)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [1000, 9001, 50001, 151936])
+def test_sums_of_near_logits(V, dtype, device):
+    """Rows of equal logits, and of logits that rise by up to 4, around 0 and around 1,300 (whose product with log2(e) is
+    coarse in fp32): log-probabilities, loss and gradient within the bounds of these sums, not of the worst ones.  A
+    correction of the exponent left out would be off by up to 4e-5."""
+    g = torch.Generator().manual_seed(V)
+    R = 24
+    z = torch.randint(0, 33, (R, V), generator=g).float() / 8
+    z[: R // 2] = 0.0
+    z[R // 2:: 2] = z[R // 2:: 2].sort(1).values
+    # (multiples of 1/8 are exact in fp16 up to 256, of 1/2 up to 1024)
+    c = 700 + 640 * torch.rand(R, generator=g) if dtype == torch.float32 else torch.randint(200, 250, (R,), generator=g).float()
+    c = (c * 8).round() / 8
+    c[::3] = 0.0
+    x = (z + c[:, None]).to(dtype).to(device)
+    assert torch.equal(x.cpu().float(), z + c[:, None])
+    lp = torch.log_softmax(x.double(), 1)
+    logp, ids, _ = topk_logprobs(x, 5)
+    assert ((logp.double() - lp.gather(1, ids.long())).abs() <= tight(V)).all()
+    # the target alone: loss = -log p, gradient = p - [target]
+    y = torch.randint(0, V, (R,), generator=g).int().to(device)
+    zero = torch.zeros(R, device=device)
+    for out in (None, x.clone()):
+        args = (x if out is None else out, ids, logp, zero)
+        loss, d = distill_loss_grad(*args, target=y, out=out)
+        at = torch.arange(R, device=device)
+        assert ((loss.double() + lp[at, y.long()]).abs() <= tight(V)).all()
+        want = lp.exp()
+        want[at, y.long()] -= 1
+        tol = (tight(V) + 18 * 2.0 ** -24 + torch.finfo(dtype).eps / 2) * want.abs() + TINY[dtype]
+        tol[at, y.long()] += tight(V) * lp.exp()[at, y.long()] + 2.0 ** -23
+        assert ((d.double() - want).abs() <= tol).all()
+    # a teacher that agrees: every class's log-ratio is an error alone
+    for kind in ("forward", "reverse"):
+        loss, d = distill_loss_grad(x, ids, logp, kind=kind)
+        assert (loss.abs() <= 4 * tight(V)).all()
+        assert (d.double().abs() <= 4 * tight(V) * (lp.exp() + 2.0 ** -20) + TINY[dtype]).all()
+
+
+@pytest.mark.gpu
+def test_more_rows_than_ctas(dev):
+    """More rows than the grid has CTAs: every row is reached."""
+    R, V, K = 2 ** 20 + 37, 24, 3
+    x = rows(R, V, torch.bfloat16, dev)
+    check_top(x, K)
+    top = topk_logprobs(x, K)
+    w = (torch.arange(R, device=dev) % 7 != 3).float()
+    other = rows(R, V, torch.bfloat16, dev, seed=1)
+    loss, d = distill_loss_grad(other, top.ids, top.logprobs, w)
+    last = slice(R - 2000, R)
+    part = distill_loss_grad(other[last].clone(), top.ids[last].clone(), top.logprobs[last].clone(), w[last].clone())
+    assert torch.equal(loss[last], part[0]) and torch.equal(d[last], part[1])
+    assert loss[w != 0].isfinite().all() and (loss[w != 0] != 0).any() and not d[w == 0].any()
+    out = distill_loss_grad(other, top.ids, top.logprobs, w, out=other)
+    assert torch.equal(out[0], loss) and torch.equal(other, d)

@@ -222,3 +222,20 @@ def test_the_distance_does_not_depend_on_its_weight(kind, dev):
         tr._train(seqs, tr.ref_logprobs(seqs), torch.randn(n, generator=g, device=dev), lists)
         got.append(float(tr.distill_kl))
     assert got[0] > 1e-3 and got[0] == got[1]
+
+
+@pytest.mark.gpu
+def test_the_same_seeds_give_the_same_embedding_gradient(dev):
+    """Two trainers of the same seeds: the same bits in the embedding's gradient after an update's backward passes
+    (the head of its own: what is compared is the lookup's)."""
+    got = []
+    for _ in range(2):
+        tr = GRPOTrainer(config(model=tiny(tie_embeddings=False), distill_coef=0.1, distill_topk=16), dev)
+        g = torch.Generator(device=dev).manual_seed(2)
+        seqs = torch.randint(0, 40, (tr.cfg.batch, tr.cfg.seq_len), generator=g, device=dev, dtype=torch.int32)
+        lists = tr._teacher_lists(tr.cfg.batch)
+        ref_lp = tr.ref_logprobs(seqs, lists)
+        tr.model.zero_grad()
+        tr._train(seqs, ref_lp, torch.randn(tr.cfg.batch, generator=g, device=dev), lists)
+        got.append(tr.model.g["embed"].clone())
+    assert got[0].abs().sum() > 0 and torch.equal(*got)

@@ -374,3 +374,33 @@ def test_first_row(H, pad, device):
         embedding(ids, leaf, first_row=True)
     with torch.no_grad():
         embedding(ids, leaf, first_row=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V,H,how", [(2 ** 20 + 77, 5000, 8, "hot"), (2 ** 20 + 129, 300, 33, "zipf"), (3 * 2 ** 20 + 5, 2 ** 20, 4, "uniform"),
+                                       (2 ** 21 + 1, 11, 16, "runs")])
+def test_longer_pieces(N, V, H, how, dev):
+    """So many tokens that the sums' pieces are longer than 128 of them."""
+    g = torch.Generator(device=dev).manual_seed(N)
+    ids = tokens(N, V, how).int().to(dev)
+    dy = torch.randn(N, H, generator=g, device=dev).bfloat16()
+    check_grad(ids, dy, torch.randn(V, H, generator=g, device=dev), 0.5)
+    got = [embedding_grad(ids, dy, torch.empty(V, H, device=dev), 2.0, accumulate=False) for _ in range(2)]
+    assert torch.equal(*got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [0, 40, 3000])
+def test_rows_far_apart(N, dev):
+    """A gradient whose rows are more than 2^32 bytes apart, overwritten: its own elements alone."""
+    V, H, step = 3, 24, 2 ** 31 + 8
+    buf = torch.full((2 * step + 64,), 3.0, dtype=torch.bfloat16, device=dev)
+    grad = buf.as_strided((V, H), (step, 1))
+    ids = torch.full((N,), 2, dtype=torch.int32, device=dev)
+    dy = torch.ones(N, H, device=dev, dtype=torch.bfloat16)
+    embedding_grad(ids, dy, grad, 0.5, accumulate=False)
+    want = torch.zeros(V, H)
+    want[2] = torch.tensor(N / 2).bfloat16().float()  # (1,500 lies halfway between two bf16 values)
+    assert torch.equal(grad.float().cpu(), want)
+    for a, b in ((H, step), (step + H, 2 * step), (2 * step + H, buf.numel())):
+        assert bool((buf[a:b] == 3.0).all())
