@@ -4,7 +4,7 @@
 // p = softmax(z / T), the row's loss is w KL + c (-log p_y), with
 //
 //   forward:        KL = sum_S t (log t - log p),                 T dKL/dz_j = p_j - t_j
-//                   (t divided by its sum: by the sum of exp(l - max l), whatever the list's own scale)
+//                   (t divided by its sum, whatever the list's own scale)
 //   forward, rest:  ... + t_R (log t_R - log p_R),                T dKL/dz_j = p_j - t_j in S,
 //                                                                 (p_R - t_R) q_j outside
 //                   (p times sum t + t_R where that is not 1)
@@ -43,6 +43,7 @@ using tb::Vec;
 constexpr int kMaxList = 256;  // (a thread for each entry)
 constexpr int kMaxWarps = 16;
 constexpr int kLane = 8;  // vectors of a lane at a time
+constexpr float kPlain = 46.f;  // log-masses up to here (1e20, and 1e-20) are summed as they are
 constexpr double kRestMin = 1.0 / (1 << 20);
 enum { kLoss, kBoth, kGrad };  // what a launch computes (kGrad: from the numbers that kLoss kept)
 
@@ -75,10 +76,10 @@ struct Shared {
   Numbers n;
   // the row's weights and list: what lives over the passes is here, not in registers
   float w, c, z_y;
-  int y, y_listed, twice;
+  int y, y_listed, special;
   __align__(16) int id[kMaxList];  // -1: padding
   float z[kMaxList], l[kMaxList];
-  double t[kMaxList];  // mass of the class (l: its logarithm), without the rest relative to the largest entry;
+  double t[kMaxList];  // mass of the class (l: its logarithm), both perhaps relative to the largest without the rest;
                        // -1 where the entry is not its id's first
   // the softmax sum of the list's elements, the masses' sum, t_R, and their logarithms
   float in_m, in_s;
@@ -131,14 +132,16 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
   if (listed) {
     for (int k = lane; k < a.K; k += 32) {
       const float t = static_cast<float>(s.t[k]);
-      if (s.id[k] < 0 || s.t[k] < 0.0) continue;
+      if (s.id[k] < 0 || t < 0.f) continue;
       const float lp = log_p(s.z[k], all.m, lns);
       const float lt = s.l[k] - s.log_mass;
       if (a.kind == TB_DISTILL_REVERSE) {
         const float p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
         if (p != 0.f) kl += p * (lp - lt);
-      } else if (s.t[k] != 0.0) {  // (a mass below 2^-149 counts where the student has none)
-        kl += lp == -INFINITY ? INFINITY : (a.kind == TB_DISTILL_FORWARD ? t / s.mass : t) * (lt - lp);
+      } else if (t != 0.f) {
+        kl += (a.kind == TB_DISTILL_FORWARD ? t / s.mass : t) * (lt - lp);
+      } else if (lp == -INFINITY && s.t[k] != 0.0) {
+        kl += INFINITY;  // (a mass below 2^-149 that the student rules out)
       }
     }
     kl = tb::warp_sum(kl);
@@ -168,7 +171,7 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
     float4* st = reinterpret_cast<float4*>(a.stats + r * TB_DISTILL_STATS);
     st[0] = make_float4(s.n.origin, s.n.factor, s.n.top, s.n.lns.x);
     st[1] = make_float4(s.n.lns.y, s.n.kl, s.n.whole, s.mass);
-    st[2] = make_float4(s.twice ? 1.f : 0.f, 0.f, 0.f, 0.f);
+    st[2] = make_float4(s.special ? 1.f : 0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -220,9 +223,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
       }
       if (tid < kMaxList) {
         s.id[tid] = id;
-        s.l[tid] = id >= 0 ? l : -INFINITY;
+        s.l[tid] = l;
         if (id >= 0) s.z[tid] = tb::to_f32(row.row[id]);
-        if (a.kind != TB_DISTILL_FORWARD) s.t[tid] = id >= 0 ? exp(static_cast<double>(l)) : 0.0;
+        s.t[tid] = id >= 0 ? exp(static_cast<double>(l)) : 0.0;
       }
       if (tid == 0) {
         s.w = q.w;
@@ -234,16 +237,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
         for (int i = tid; i < part; i += kThreads) dynamic[i] = make_uint4(0, 0, 0, 0);
       const int y_listed = __syncthreads_or(id >= 0 && id == q.y);
       if (tid == 0) s.y_listed = y_listed;
-      // ---- without the rest masses count relative to the largest (a list of faint entries has a sum, too)
-      float largest = 0.f;
-      if (a.kind == TB_DISTILL_FORWARD && tid < kMaxList) {
-        largest = -INFINITY;
-        for (int j = lane; j < K; j += 32) largest = fmaxf(largest, s.l[j]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-        s.t[tid] = id >= 0 ? exp(static_cast<double>(l) - largest) : 0.0;
-      }
-      // ---- an id that occurs twice counts once, with the sum of its masses
+      // ---- an id that occurs twice counts once, with the sum of its masses; without the rest they
+      // count relative to the largest where their sum may leave fp32's range (faint lists, scores)
       int seen = 0;
       if (MODE == kGrad) {
         seen = a.stats[r * TB_DISTILL_STATS + 8] != 0.f;
@@ -258,10 +253,22 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
         const int v = (id + row.mis) / E - row.v0, b = (id + row.mis) % E;
         if (v >= 0 && v < row.v1 - row.v0) atomicOr(reinterpret_cast<uint32_t*>(bytes) + v / 4, 1u << (v % 4 * 8 + b));
       }
-      const int twice = __syncthreads_or(seen);
-      if (tid == 0) s.twice = twice;
-      if (twice) {
-        if (id >= 0) {  // (the logarithm from the largest of its entries: the mass itself may be below 2^-1074)
+      const bool odd = a.kind == TB_DISTILL_FORWARD && id >= 0 && !(fabsf(l) <= kPlain);
+      const int special = __syncthreads_or(seen || odd);
+      if (tid == 0) s.special = special;
+      if (special) {
+        float largest = 0.f;
+        if (a.kind == TB_DISTILL_FORWARD) {
+          largest = -INFINITY;
+          for (int j = lane; j < K; j += 32)
+            if (s.id[j] >= 0) largest = fmaxf(largest, s.l[j]);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        }
+        if (!__syncthreads_or(seen)) {
+          if (id >= 0) s.t[tid] = exp(static_cast<double>(l) - largest);
+          l -= largest;
+        } else if (id >= 0) {  // (the logarithm from the largest of its entries: the mass itself may be below 2^-1074)
           bool first = true;
           float top = l;
           for (int j = 0; j < K; ++j) {
@@ -278,8 +285,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_kernel(TbDi
         __syncthreads();
         if (id >= 0) s.l[tid] = l;
         __syncthreads();
-      } else if (id >= 0) {
-        s.l[tid] = l - largest;  // (read behind the next wait)
       }
     }
     Numbers n;
