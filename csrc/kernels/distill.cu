@@ -23,13 +23,20 @@
 // (t_R is 1 less their sum), and log S is kept as the sum of two fp32 numbers: the loss is a
 // small difference of large ones.
 //
+// Sums over a row and the KL are in fp32 (a loss of ordinary size is off by 1e-7 to 3e-7 of its
+// terms, 64-bit sums would give 3e-8): what they round is far below the logits' own type, and
+// 64-bit additions for every logit would bound the kernel.
+//
 // The floor is one read of the live rows and one write of the gradient.  4,096 rows of 151,936
-// bf16 (all live) take 530 us, 4.7 TB/s: a third of the rows' second reads misses the L2 cache
-// (495 MB read for 360 of 1,184 rows), whose writes pass through it.  Rows kept in shared
-// memory, rings of bulk loads and the next row's first loads ahead gained nothing: then too few
-// loads are in flight, or the sums wait for the stores.  The loss alone, 1,184 rows: 76 us, 4.7
-// TB/s.  Short rows (777 of 32,003 fp16, odd: 37 us for a floor of 14) wait four times per row
-// for all warps: list, repeats, sums, numbers.
+// bf16 (all live) take 517 us out of an empty L2 cache and 530 to 554 (by the machine) one call
+// after another from Python, 4.5 to 4.7 TB/s; in place, as a trainer calls it, 4% more: what is
+// written are the lines that the first pass asked to be kept.  A third of the rows' second reads
+// misses the L2 cache (495 MB read for 360 of 1,184 rows), whose writes pass through it.  Rows
+// kept in shared memory, rings of bulk loads and the next row's first loads ahead gained nothing:
+// then too few loads are in flight, or the sums wait for the stores.  The loss alone, 1,184 rows:
+// 76 us, 4.7 TB/s.  Short rows (777 of 32,003 fp16, odd: 37 us for a floor of 14) wait four times
+// per row for all warps (list, repeats, sums, numbers), and the last wave of rows is thin (622
+// live rows on 592 places).
 #include "kernels.h"
 #include "vocab_rows.cuh"
 
@@ -455,8 +462,9 @@ cudaError_t launch(const TbDistillArgs& a, int groups, cudaStream_t stream) {
 
 // Both passes in one launch: the rows in work, read twice, have to fit the L2 cache beside
 // what is written, so long rows get two CTAs of 512 threads on an SM instead of four of 256
-// (1,024 rows of 1,024 groups: 67 us with 512 and 61 with 256; of 2,004 groups 114 and 122;
-// 4,096 rows of 2,374 groups 496 and 557).
+// (all rows live, an empty L2 cache: 1,024 rows of 1,024 groups take 79 us with 512 threads and
+// 71 with 256, of 1,536 groups 99 and 99, of 2,004 groups 124 and 130; 4,096 rows of 2,374
+// groups 517 and 566).
 template <typename T>
 cudaError_t launch_mode(const TbDistillArgs& a, cudaStream_t s) {
   constexpr int E = Row<T>::E;

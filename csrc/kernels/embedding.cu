@@ -19,11 +19,14 @@
 // the first digit and one for each digit, which also counts the next one.
 //
 // What bounds it, measured with bf16 rows: the lookup moves its bytes (16,384 rows of 4,096:
-// 32 us, 268 MB); the sums do where rows are 16-byte vectors (the same batch: 48 us beside no
+// 32 us; 134 MB written and as much asked for, of which the repeated rows come out of the L2
+// cache: 151 MB from and to DRAM, 4.7 TB/s); the sums do where rows are 16-byte vectors (the same batch: 48 us beside no
 // zeros, 134 MB read and as much written), while rows of odd length take an element per lane
 // (65,537 of 1,025 fp16: 59 us, 134 MB read, 40% of the copy rate) and small batches the chain
 // of launches (6,144 tokens of 1,536: sort 11, sums 16, join 5 us, of 19 MB).  The sort
 // waits on shared memory and on its own launches: 11 us for 6,144 tokens, 24 for 65,537.
+// Narrow rows are all sort and launches: 12,000 tokens of 64 columns take 33 us and 65,536 43
+// (floors of 0.8 and 3.3), where unordered atomic additions of fp32 rows take 14 and 41.
 #include <limits.h>
 #include <math.h>
 
@@ -208,7 +211,8 @@ __device__ __forceinline__ void finish(const TbEmbeddingGradArgs& a, bool vec, l
 }
 
 // Tokens of the one-launch form (512 of 1,536 bf16 take 11.5 us with it and 15.4 sorted, 64 take
-// 3.0 and 9.5; of 4,096 columns 25.8 and 20.4: there every slab compares the ids again).
+// 3.0 and 9.5).  The rule looks at the tokens alone, and so loses where hundreds of tokens have
+// wide rows, whose every slab compares the ids again (512 of 4,096 columns: 25.8 and 20.4).
 constexpr int kFew = 512;
 
 template <typename T, typename G, int N>
@@ -283,8 +287,12 @@ __global__ void __launch_bounds__(256) grad_few_kernel(TbEmbeddingGradArgs a, in
 // ---- the sort
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxBins = 512, kMaxBlocks = 64, kMaxPasses = 4;
 constexpr int kSms = 148;
-// Tokens that are sorted by comparing them all (6,144 tokens of 1,536 bf16: 29.3 us, and 33.8 by
-// the radix sort in two digits, 36.0 in three; 8,192: 38.1 and 36.7, 38.8; 2,048: 22.2 and 19.7, 21.4).
+// Tokens that are sorted by comparing them all.  The rule looks at the tokens alone.  Whole
+// gradients of 1,536 bf16 columns, by comparison and by the radix sort, in us: tables of 30,000
+// rows (two digits) 17.6 and 18.1 for 513 tokens, 24.8 and 20.3 for 2,048, 32.5 and 34.4 for
+// 6,144, 36.1 and 34.1 for 8,192; of 262,145 (three) 15.9 and 18.3, 22.7 and 21.3, 31.3 and
+// 37.7, 38.2 and 44.0.  So it loses up to 4 us from 1,000 to 3,000 tokens and 2 us at 8,192 of
+// tables up to 18 bits, and gains up to 6 us elsewhere.
 constexpr int kCompared = 8192;
 
 struct Plan {
@@ -858,6 +866,11 @@ size_t work_of(const Plan& p, char* w, Work* out) {
   return at;
 }
 
+// `after`: may start before the kernel ahead of it has ended.  The first kernel of a gradient
+// (the sort's first, and the marks) is launched without it and has to stay so: the kernels here
+// let the next one start before they wait themselves, and the CTAs that write zeros never wait.
+// What keeps them behind the caller's earlier work (and the marks, and the workspace's last user)
+// is that the first kernel does not begin before all of it has ended.
 template <typename... P, typename... Args>
 cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, bool after, Args... args) {
   cudaLaunchConfig_t cfg = {};

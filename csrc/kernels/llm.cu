@@ -207,6 +207,8 @@ __global__ void embed_fwd_kernel(const int* __restrict__ ids, const bf16* __rest
   }
 }
 
+// The gradient by atomics (unordered sums): the decoder uses embedding.cu's, whose sums have an
+// order; this one stays for callers of ops.embed_bwd and as a check on the other.
 __global__ void embed_bwd_kernel(const int* __restrict__ ids, const bf16* __restrict__ dout, float* __restrict__ dW,
                                  int T, int D, int V) {
   const long long total = static_cast<long long>(T) * (D / 8);

@@ -219,7 +219,8 @@ __device__ __forceinline__ uint64_t read_once() {
   return p;
 }
 
-// A maximum m and the sum s of 2^((x - m) k1); an infinite m counts as 0 in the exponent
+// A maximum m and the sum s of 2^((x - m) k1), in fp32 (a row's sum is off by 1e-7 or so: each
+// of 1,024 partial sums adds V / 1,024 terms); an infinite m counts as 0 in the exponent
 // (s is then 0, inf or NaN).
 struct SoftSum {
   float m = -INFINITY, s = 0.f;

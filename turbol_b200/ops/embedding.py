@@ -3,7 +3,7 @@
 ``ops.embed_fwd`` / ``ops.embed_bwd`` are the older kernels (bf16 rows, no scale; a
 gradient by atomics, whose last bits differ from run to run).  Here the gradient of a
 row is summed in fp32 in the order of its tokens (long runs of one token in pieces of a
-fixed length), so the same inputs give the same bits.
+fixed length), so the same inputs give the same bits.  The decoder's gradient is this one.
 
 CUDA tensors go to the kernels (csrc/kernels/embedding.cu), CPU tensors to the reference
 math in :mod:`turbol_b200.ops.reference`.
