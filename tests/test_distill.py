@@ -789,3 +789,24 @@ def test_more_rows_than_ctas(dev):
     assert loss[w != 0].isfinite().all() and (loss[w != 0] != 0).any() and not d[w == 0].any()
     out = distill_loss_grad(other, top.ids, top.logprobs, w, out=other)
     assert torch.equal(out[0], loss) and torch.equal(other, d)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1.0, 3.0])
+def test_rows_of_the_lowest_value(T, dtype, device):
+    """Every logit masked with the type's lowest value (or equal at its largest): a flat row, like any constant one."""
+    V = 7
+    ids = torch.tensor([[1, 4]] * 3, dtype=torch.int32, device=device)
+    logp = torch.tensor([[-0.5, -1.5]] * 3, device=device)
+    y = torch.tensor([2, 4, 0], dtype=torch.int32, device=device)
+    low = torch.finfo(dtype).min
+    x = torch.tensor([[low] * V, [0.0] * V, [-low] * V], dtype=dtype, device=device)
+    for kind, rest in KINDS:
+        loss, d = distill_loss_grad(x, ids, logp, kind=kind, rest=rest, temperature=T, target=y)
+        want = definition(x[1:2].expand(3, V), ids, logp, None, kind, rest, T, y, None)
+        compare(loss, d, x, want)
+        leaf = x.clone().requires_grad_()
+        l = distill_loss(leaf, ids, logp, kind=kind, rest=rest, temperature=T, target=y)
+        g, = torch.autograd.grad(l.sum(), leaf)
+        compare(l, g, x, want)

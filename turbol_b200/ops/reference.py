@@ -327,7 +327,10 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
     c = torch.where((y >= 0) & (y < V), c, 0.0)
     live = (w != 0) | (c != 0)
     y = y.clamp(0, V - 1)[:, None]
-    z = torch.where(live[:, None], logits.double() / temperature, 0.0)
+    z = torch.where(live[:, None], logits.double(), 0.0)
+    top = z.amax(1, keepdim=True)
+    # (differences first: next to the type's lowest value the sum's logarithm would be lost)
+    z = (z - torch.where(top.isfinite(), top, 0.0)) / temperature
     lse = torch.logsumexp(z, 1, keepdim=True)
     lse = torch.where(lse.isinf(), math.nan, lse)
     logp = z - lse
