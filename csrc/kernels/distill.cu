@@ -145,8 +145,8 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
       if (a.kind == TB_DISTILL_REVERSE) {
         const float p = tb::ex2(lp * static_cast<float>(tb::kLog2e));
         if (p != 0.f) kl += p * (lp - lt);
-      } else if (t != 0.f) {
-        kl += (a.kind == TB_DISTILL_FORWARD ? t / s.mass : t) * (lt - lp);
+      } else if (const float u = a.kind == TB_DISTILL_FORWARD && t != 0.f ? t / s.mass : t; u != 0.f) {
+        kl += u * (lt - lp);
       } else if (lp == -INFINITY && s.t[k] != 0.0) {
         kl += INFINITY;  // (a mass below 2^-149 that the student rules out)
       }

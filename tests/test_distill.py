@@ -810,3 +810,55 @@ def test_rows_of_the_lowest_value(T, dtype, device):
         l = distill_loss(leaf, ids, logp, kind=kind, rest=rest, temperature=T, target=y)
         g, = torch.autograd.grad(l.sum(), leaf)
         compare(l, g, x, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind,rest", KINDS)
+def test_broken_rows_without_a_list(kind, rest, device):
+    """NaN, +inf or no logit above -inf give NaN in a row with weight, also where its list is all padding."""
+    x = rows(5, 60, torch.float32, device, spread=1.0)
+    x[0, 7], x[1, 7], x[2], x[4] = NAN, INF, -INF, NAN
+    ids, logp = lists(x, 3)
+    w = torch.tensor([1.0, 1.0, 1.0, 1.0, 0.0], device=device)
+    for pad in ("ids", "logp"):
+        a = torch.full_like(ids, -1) if pad == "ids" else ids
+        b = torch.full_like(logp, -INF) if pad == "logp" else logp
+        kl = torch.zeros(5, device=device)
+        loss, d = distill_loss_grad(x, a, b, w, kind=kind, rest=rest, kl=kl)
+        broken = [True, True, True, False, False]
+        assert loss.isnan().tolist() == broken and kl.isnan().tolist() == broken
+        assert d.isnan().all(1).tolist() == broken and d.isnan().any(1).tolist() == broken
+        leaf = x.clone().requires_grad_()
+        g, = torch.autograd.grad(distill_loss(leaf, a, b, w, kind=kind, rest=rest).sum(), leaf)
+        assert g.isnan().all(1).tolist() == broken and g.isnan().any(1).tolist() == broken
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["forward", "reverse"])
+def test_a_rest_of_the_lowest_value(kind, dtype, device):
+    """What is outside the list masked with the type's lowest value: the rest's pull is shared by its logits, and a row's
+    gradient sums to zero (up to its own roundings)."""
+    low = torch.finfo(dtype).min
+    x = torch.tensor([[0.5, low, low, -1.0, low]], dtype=dtype, device=device)
+    ids = torch.tensor([[0, 3]], dtype=torch.int32, device=device)
+    logp = torch.tensor([[-0.7, -1.5]], device=device)
+    loss, d = distill_loss_grad(x, ids, logp, kind=kind)
+    rest = 1 - math.exp(-0.7) - math.exp(-1.5) if kind == "forward" else 0.0
+    assert (d[0, [1, 2, 4]].double() + rest / 3).abs().max() <= torch.finfo(dtype).eps * rest / 3 + 2.0 ** -22
+    assert abs(float(d.double().sum())) <= 5 * torch.finfo(dtype).eps
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_faint_scores_that_the_student_rules_out(device):
+    """Without the rest: a mass that vanishes when it is divided by the sum, on a logit of -inf."""
+    x = rows(1, 50, torch.float32, device, spread=1.0)
+    ids = torch.arange(40, dtype=torch.int32, device=device)[None]
+    x[0, 39] = -INF
+    for faint in (-100.0, -102.0, -103.0, -103.5, -150.0):
+        logp = torch.full((1, 40), 0.0, device=device)
+        logp[0, 39] = faint
+        for shift in (0.0, 30.0, -90.0):
+            kl = torch.empty(1, device=device)
+            loss, _ = distill_loss_grad(x, ids, logp + shift, rest=False, kl=kl)
+            assert loss.isposinf().all() and kl.isposinf().all()

@@ -356,9 +356,13 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
         kl = plogq(t, lt, logp, inside)
         d = torch.where(some, p - t, 0.0)
     else:
-        lr = torch.logsumexp(torch.where(inside, -math.inf, logp), 1, keepdim=True)
-        pr, empty = lr.exp(), lr.isneginf()
-        q = torch.where(empty | inside, 0.0, (logp - lr).exp())
+        outside = torch.where(inside, -math.inf, logp)
+        most = outside.amax(1, keepdim=True)
+        empty = most.isneginf()
+        q = (outside - torch.where(empty, 0.0, most)).exp()  # (differences first here, too)
+        share = q.sum(1, keepdim=True)
+        lr, q = most + share.log(), torch.where(empty, 0.0, q / share)
+        pr = lr.exp()
         if kind == "forward":
             tr = (1 - total).clamp_min(0)
             kl = plogq(t, lt, logp, inside) + torch.where(empty | (tr == 0), 0.0, tr * (tr.clamp_min(1e-300).log() - lr))
@@ -369,6 +373,7 @@ def distill(logits, ids, logprobs, weight=None, kind="forward", rest=True, tempe
             fr = torch.where(empty, 0.0, lr - (1 - total).clamp_min(DISTILL_REST_MIN).log())
             kl = (p * f).sum(1, keepdim=True) + pr * fr
             d = torch.where(inside, p * (f - kl), pr * q * (fr - kl))
+    kl, d = torch.where(lse.isnan(), math.nan, kl), torch.where(lse.isnan(), math.nan, d)  # (whatever the list is)
     on, c = (w != 0)[:, None], c[:, None]
     if out_kl is not None:
         out_kl.copy_(torch.where(on, kl, 0.0).squeeze(1))
