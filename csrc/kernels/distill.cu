@@ -172,7 +172,10 @@ __device__ __forceinline__ void numbers_of(const TbDistillArgs& a, Shared& s, lo
   const float factor = !good ? NAN : none ? 0.f : f * inv_t / sum.s * ex.fix;
   s.n = {ex.m, factor, all.m, good ? lns : make_float2(NAN, NAN), kl, whole};
   if (!write) return;
-  a.loss[r] = good ? (listed ? w * kl : 0.f) + (c != 0.f ? -c * log_p(s.z_y, all.m, lns) : 0.f) : NAN;
+  // (in 64 bits: with masked logits the two may be near fp32's end and cancel)
+  const double from_list = listed ? static_cast<double>(w) * kl : 0.0;
+  const double from_target = c != 0.f ? -static_cast<double>(c) * log_p(s.z_y, all.m, lns) : 0.0;
+  a.loss[r] = good ? static_cast<float>(from_list + from_target) : NAN;
   if (a.kl) a.kl[r] = good || !listed ? kl : NAN;
   if (a.stats) {
     float4* st = reinterpret_cast<float4*>(a.stats + r * TB_DISTILL_STATS);

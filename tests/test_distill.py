@@ -862,3 +862,25 @@ def test_faint_scores_that_the_student_rules_out(device):
             kl = torch.empty(1, device=device)
             loss, _ = distill_loss_grad(x, ids, logp + shift, rest=False, kl=kl)
             assert loss.isposinf().all() and kl.isposinf().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_huge_terms_that_cancel(dtype, device):
+    """A target and listed tokens masked with the type's lowest value: terms near fp32's end whose sum is within it."""
+    low = torch.finfo(dtype).min
+    x = torch.tensor([[0.5, low, 1.0, -1.0, 0.25]] * 3, dtype=dtype, device=device)
+    ids = torch.tensor([[0, 1]] * 3, dtype=torch.int32, device=device)
+    logp = torch.tensor([[-1.2, -0.7]] * 3, device=device)
+    w = torch.tensor([3.5, -3.0, 1.5], device=device)
+    y = torch.tensor([1, 1, 1], dtype=torch.int32, device=device)
+    c = torch.tensor([-1.5, 1.75, -0.5], device=device)
+    for kind, rest in KINDS[:2]:
+        t = torch.tensor([math.exp(-1.2), math.exp(-0.7)], dtype=torch.float64)
+        t = t if rest else t / t.sum()
+        want = -(w.cpu().double() * t[1] + c.cpu().double()) * low  # (what else there is is below 2^-100 of it)
+        mag = (w.cpu().double() * t[1]).abs() + c.cpu().double().abs()
+        loss, d = distill_loss_grad(x, ids, logp, w, kind=kind, rest=rest, target=y, target_weight=c)
+        assert d.isfinite().all()
+        # the mass, its share and the loss: 8 roundings of terms of this size
+        assert ((loss.cpu().double() - want).abs() <= 8 * 2.0 ** -24 * mag * -low).all(), (loss, want)

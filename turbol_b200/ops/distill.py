@@ -20,6 +20,8 @@ and set ``error`` (an int32 device tensor, optional) to 1; a negative target is 
 Rows whose weights are 0 are not read: loss 0, gradient 0, whatever the logits hold.
 In a row with weight, NaN, +inf or no logit above -inf give NaN.  A student without
 any mass outside the list (all its logits there -inf) leaves out the p_R term.
+Log-probabilities are held in fp32: a logit whose distance to the row's largest, over
+T, passes 3.4e38 (a mask of bf16's or fp32's lowest value with T < 1) counts as -inf.
 
 CUDA tensors go to the kernels (csrc/kernels/topk_logprobs.cu,
 csrc/kernels/distill.cu), CPU tensors to the reference math in
