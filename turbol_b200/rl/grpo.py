@@ -293,7 +293,8 @@ class GRPOTrainer:
         # (a state from before the key was there says nothing of its teacher)
         if "teacher" in sd and sd["teacher"] != self._teacher_digest():
             kind = "the frozen reference" if sd["teacher"] is None else "a given one"
-            raise ValueError(f"the saved run's teacher was {kind} and is not this trainer's")
+            raise ValueError(f"the saved run's teacher was {kind} and is not this trainer's "
+                             "(load_checkpoint(strict_config=False) goes on with this one)")
         with torch.no_grad():
             self.model.flat.copy_(sd["policy"]["flat"])
             self.model.shadow.copy_(sd["policy"]["shadow"])

@@ -307,8 +307,9 @@ def load_checkpoint(directory: str, step: Optional[int] = None, trainer=None, *,
     to ``trainer.checkpoint_ranks()``.  The step must be complete for its
     layout and must hold this rank's marker.  With ``config`` (or
     ``trainer.cfg``) the saved configuration must match key for key unless
-    ``strict_config=False``; a key that it lacks (saved before the key was
-    there) counts as the field's default."""
+    ``strict_config=False`` (which also lets a GRPO run go on with another
+    teacher); a key that it lacks (saved before the key was there) counts as
+    the field's default."""
     tp_rank, pp_rank, dp_rank, lay = _resolve_ranks(trainer, tp_rank, pp_rank, dp_rank, layout)
     if step is None:
         step = latest_step(directory)
@@ -350,7 +351,8 @@ def load_checkpoint(directory: str, step: Optional[int] = None, trainer=None, *,
                 raise ValueError(f"checkpoint configuration differs in {sorted(diff)}")
     state["step"] = int(step)
     if trainer is not None:
-        trainer.load_state_dict({k: v for k, v in state.items() if k not in ("replay", "config", "step")})
+        skip = ("replay", "config", "step") if strict_config else ("replay", "config", "step", "teacher")
+        trainer.load_state_dict({k: v for k, v in state.items() if k not in skip})
     return state
 
 
