@@ -20,13 +20,13 @@
 //
 // What bounds it, measured with bf16 rows: the lookup moves its bytes (16,384 rows of 4,096:
 // 32 us; 134 MB written and as much asked for, of which the repeated rows come out of the L2
-// cache: 151 MB from and to DRAM, 4.7 TB/s); the sums do where rows are 16-byte vectors (the same batch: 48 us beside no
-// zeros, 134 MB read and as much written), while rows of odd length take an element per lane
-// (65,537 of 1,025 fp16: 59 us, 134 MB read, 40% of the copy rate) and small batches the chain
-// of launches (6,144 tokens of 1,536: sort 11, sums 16, join 5 us, of 19 MB).  The sort
-// waits on shared memory and on its own launches: 11 us for 6,144 tokens, 24 for 65,537.
-// Narrow rows are all sort and launches: 12,000 tokens of 64 columns take 33 us and 65,536 43
-// (floors of 0.8 and 3.3), where unordered atomic additions of fp32 rows take 14 and 41.
+// cache: 151 MB from and to DRAM, 4.7 TB/s); the sums do where rows are 16-byte vectors (the
+// same batch: 48 us beside no zeros, 134 MB read and as much written), while rows of odd length
+// take an element per lane (65,537 of 1,025 fp16: 59 us, 134 MB read, 40% of the copy rate) and
+// small batches the chain of launches (6,144 tokens of 1,536: sort 11, sums 16, join 5 us, of
+// 19 MB).  The sort waits on shared memory and on its own launches: 11 us for 6,144 tokens, 24
+// for 65,537.  Narrow rows are all sort and launches: 12,000 tokens of 64 columns take 33 us and
+// 65,536 43 (floors of 0.8 and 3.3), where unordered additions of fp32 rows take 14 and 41.
 #include <limits.h>
 #include <math.h>
 
